@@ -9,7 +9,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, 'libasrn_b200.so')
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 ASRN_OK, ASRN_ERR_ARG, ASRN_ERR_UNSUPPORTED, ASRN_ERR_WORKSPACE, ASRN_ERR_CUDA, ASRN_ERR_TIMEOUT, ASRN_ERR_DATA = range(7)
 
@@ -118,6 +118,27 @@ _SIGS = {
                                   + [ctypes.c_float, ctypes.c_float, ctypes.c_int32] + [_P] * 11),
     'asrn_scan_forward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, _P, _P, _P]),
     'asrn_scan_backward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, _P, _P, _P, _P, _P]),
+    'asrn_head_saved_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+    'asrn_head_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+    'asrn_head_forward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P, _P, ctypes.c_float,
+                                         _P, _P, ctypes.c_size_t, _P, ctypes.c_size_t, _P, _P]),
+    'asrn_head_backward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P, ctypes.c_size_t,
+                                          ctypes.c_float, _P, _P, _P, _P, ctypes.c_size_t, _P, _P]),
+    'asrn_preference_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    'asrn_preference_loss': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, _P, _P, ctypes.c_int32,
+                                            ctypes.c_double, ctypes.c_double, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    'asrn_policy_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    'asrn_policy_loss': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int32, _P,
+                                        ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_int32, _P, _P, _P,
+                                        _P, ctypes.c_size_t, _P]),
+    'asrn_pack8': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, _P, _P, _P, _P]),
+    'asrn_unpack8': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, _P, _P, _P, _P]),
+    'asrn_mlp8_saved_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+    'asrn_mlp8_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64] + [ctypes.c_int32] * 4),
+    'asrn_mlp8_forward': (ctypes.c_int, [ctypes.c_int64] + [ctypes.c_int32] * 3 + [_P] * 7 +
+                          [ctypes.c_size_t, _P, ctypes.c_size_t, _P, _P]),
+    'asrn_mlp8_backward': (ctypes.c_int, [ctypes.c_int64] + [ctypes.c_int32] * 3 + [_P] * 4 + [ctypes.c_size_t] +
+                           [_P] * 6 + [ctypes.c_size_t, _P, _P]),
     'asrn_argmax_rows': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int32, _P, _P]),
     'asrn_sampler_seed_state': (ctypes.c_int, [ctypes.c_uint64, _P]),
     'asrn_sampler_jump_poly': (ctypes.c_int, [ctypes.c_uint64, _P]),

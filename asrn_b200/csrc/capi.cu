@@ -161,7 +161,7 @@ const char* asrn_status_string(int status) {
   }
 }
 
-int asrn_abi_version(void) { return 4; }
+int asrn_abi_version(void) { return 5; }
 
 size_t asrn_layer_prepared_bytes(const asrn_layer_config* cfg) {
   if (check_config(cfg) != ASRN_OK) return 0;

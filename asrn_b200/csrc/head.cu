@@ -1,0 +1,458 @@
+// Log probabilities of given tokens through the tied head, forward and backward, without the (rows, V) logits in memory:
+//   s_iv = h_i . w_v / tau,  lse_i = log sum_v exp s_iv,  logp_i = s_{i,y_i} - lse_i
+//   dS_iv = (g_i / tau) (delta_{v,y_i} - exp(s_iv - lse_i)),  dh = dS W,  dW = dS^T h
+// 2 N V d operations forward and 6 N V d backward (the scores are formed again), against 2 N d + 2 V d elements read:
+// bound by the tensor cores at any training size.
+//
+// Positions without a target (token < 0: prompts, padding) are left out before the products: their rows are never
+// gathered, so a batch whose half is prompt costs half. How many rows are left stays on the device.
+//   k_head_count   (many rows) targets per block of 1024 tokens
+//   k_head_gather  the rows with a target, in order, with their tokens and the maps both ways
+//   k_gemm<Lse>    scores by tiles of 256 tokens; each thread keeps the running maximum and sum of exponentials of its
+//                  row over its 128 columns and writes that pair; the target's score goes into none of the sums, it is
+//                  written by itself: with x = s_y - m and S the sum of the others' exp(s - m), logp = -log1p(S exp(-x))
+//                  and 1 - p_y = -expm1(logp) keep their leading digits where p_y is all but 1
+//   k_head_join    the pairs of a row joined: logp, and lse and 1 - p_y for the backward pass
+//   k_gemm<Slope>  backward, by chunks of rows: the scores again, dS in bf16
+//   k_gemm         dh = dS W (parts of V where rows are few) and dW = dS^T h, sums in fp32
+// dS is rounded to bf16 once, as the operand of both products.
+#include "common.cuh"
+#include "gemm_tc.cuh"
+
+namespace asrn {
+
+namespace {
+
+constexpr int kGatherRows = 128, kGatherThreads = 256;
+constexpr int kCountRows = 1024;
+constexpr int64_t kDirectRows = 32768;   // up to here each block counts the targets before it by itself: a launch less
+constexpr float kLog2e = 1.4426950408889634f;
+
+int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
+
+ASRN_DEV float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct HeadSaved {                       // what the forward pass keeps
+  size_t count, tok, row, pos, lse2, rest, hc, total;
+};
+
+HeadSaved head_saved(int64_t N, int64_t d) {
+  HeadSaved w{};
+  const size_t P = (size_t)pad256(N);
+  size_t o = 256;                        // count
+  auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
+  w.tok = take(P * 4);
+  w.row = take(P * 4);
+  w.pos = take(P * 4);
+  w.lse2 = take(P * 4);
+  w.rest = take(P * 4);
+  w.hc = take(P * d * 2);
+  w.total = o;
+  return w;
+}
+
+struct HeadForwardWs {
+  size_t counts, top, part, total;
+};
+
+HeadForwardWs head_forward_ws(int64_t N, int64_t V) {
+  HeadForwardWs w{};
+  const size_t P = (size_t)pad256(N), halves = (size_t)((V + gemm::kBN - 1) / gemm::kBN) * 2;
+  w.counts = 0;
+  w.top = align_up((size_t)((N + kCountRows - 1) / kCountRows) * 4);
+  w.part = align_up(w.top + P * 4);
+  w.total = align_up(w.part + halves * P * 8);
+  return w;
+}
+
+// The backward pass's plan: chunks of rows whose dS stays within a gigabyte.
+struct HeadBackwardWs {
+  int64_t rows, pitch;
+  int chunks, split_h, split_w;
+  size_t ds, dh, dw, total;
+};
+
+HeadBackwardWs head_backward_ws(int64_t N, int64_t V, int64_t d) {
+  HeadBackwardWs w{};
+  w.pitch = (V + 63) / 64 * 64;
+  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 30) / (2 * w.pitch) / 256 * 256);
+  w.chunks = (int)((pad256(N) + most - 1) / most);
+  w.rows = std::max<int64_t>(256, pad256((N + w.chunks - 1) / std::max(1, w.chunks)));
+  w.chunks = (int)((pad256(N) + w.rows - 1) / w.rows);
+  w.split_h = gemm::splits_for(w.rows, d, V, 1);
+  w.split_w = gemm::splits_for(V, d, w.rows, 1);
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
+  w.ds = take((size_t)w.rows * w.pitch * 2);
+  w.dh = take((size_t)w.split_h * w.rows * d * 4);
+  w.dw = take(w.chunks > 1 || w.split_w > 1 ? (size_t)w.split_w * V * d * 4 : 0);
+  w.total = o;
+  return w;
+}
+
+__global__ void __launch_bounds__(kCountRows) k_head_count(int64_t N, const int64_t* __restrict__ tokens,
+                                                           int* __restrict__ counts) {
+  const int64_t i = (int64_t)blockIdx.x * kCountRows + threadIdx.x;
+  const int n = __syncthreads_count(i < N && tokens[i] >= 0);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// Block b takes positions [128 b, 128 b + 128): the targets before them (from the tokens, or from the counts of the
+// blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 256.
+__global__ void __launch_bounds__(kGatherThreads)
+k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ tokens,
+              const int* __restrict__ counts, int* count, int* __restrict__ tok, int* __restrict__ row,
+              int* __restrict__ pos, __nv_bfloat16* __restrict__ hc) {
+  __shared__ int warps[kGatherThreads / 32];
+  __shared__ int at[kGatherRows];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int64_t i0 = (int64_t)blockIdx.x * kGatherRows;
+  int before = 0;
+  const int64_t from = counts ? i0 / kCountRows * kCountRows : 0;
+  if (counts)
+    for (int64_t c = tid; c < i0 / kCountRows; c += kGatherThreads) before += counts[c];
+#pragma unroll 4
+  for (int64_t i = from + tid; i < i0; i += kGatherThreads) before += tokens[i] >= 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) warps[wid] = before;
+  __syncthreads();
+  before = 0;
+  for (int w = 0; w < kGatherThreads / 32; ++w) before += warps[w];
+  __syncthreads();
+  const int64_t i = i0 + tid;
+  const bool mine = tid < kGatherRows && i < N;
+  const int64_t y = mine ? tokens[i] : -1;
+  const unsigned set = __ballot_sync(0xffffffffu, y >= 0);
+  if (lane == 0) warps[wid] = __popc(set);
+  __syncthreads();
+  int r = before + __popc(set & ((1u << lane) - 1u));
+  for (int w = 0; w < wid; ++w) r += warps[w];
+  if (tid < kGatherRows) at[tid] = y >= 0 ? r : -1;
+  if (mine) pos[i] = y >= 0 ? r : -1;
+  if (y >= 0) {
+    tok[r] = y < V ? (int)y : -1;          // outside the vocabulary: NaN from here on
+    row[r] = (int)i;
+  }
+  __syncthreads();
+  const int nv = d / 8;
+  for (int k = wid; k < kGatherRows; k += kGatherThreads / 32) {
+    if (at[k] < 0) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(h + (i0 + k) * d);
+    uint4* dst = reinterpret_cast<uint4*>(hc + (int64_t)at[k] * d);
+    for (int c = lane; c < nv; c += 32) dst[c] = src[c];
+  }
+  if (i0 + kGatherRows >= N) {
+    int total = before;
+    for (int w = 0; w < kGatherRows / 32; ++w) total += warps[w];
+    if (tid == 0) *count = total;
+    const int64_t end = ((int64_t)total + 255) / 256 * 256;
+    uint4* dst = reinterpret_cast<uint4*>(hc);
+    for (int64_t c = (int64_t)total * nv + tid; c < end * nv; c += kGatherThreads) dst[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Running maximum (of the unscaled scores) and sum of exponentials over the thread's columns.
+struct Lse {
+  struct Params {
+    const int* tok;
+    float k;                               // log2(e) / tau
+    float* top;                            // the targets' unscaled scores
+    float2* part;                          // [2 n-tiles][pad]
+    int64_t pad;
+  };
+  const Params& p;
+  int row, V, y, at;
+  bool on;
+  float m = -INFINITY, s = 0.f;
+  ASRN_DEV Lse(const Params& pp, int r, int rows, int, const gemm::Shape& sh, const gemm::Tile& u, int half)
+      : p(pp), row(r), V(sh.N), y(-1), at(u.n * 2 + half), on(r < rows) {
+    if (on) y = p.tok[r];
+  }
+  ASRN_DEV void chunk(float* v, int c) {
+    if (c >= V) return;
+    const int n = V - c, j = y - c;        // n: valid columns, 32 or more but in the last tile
+    if (j >= 0 && j < 32) {
+      float own = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        own = i == j ? v[i] : own;
+        v[i] = i == j ? -INFINITY : v[i];
+      }
+      p.top[row] = own;
+    }
+    float t = m;
+    if (n < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = i < n ? v[i] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t = fmaxf(t, v[i]);
+    const float off = t == -INFINITY ? 0.f : t * p.k;
+    float add = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) add += exp2_fast(fmaf(v[i], p.k, -off));
+    s = s * exp2_fast(fmaf(m, p.k, -off)) + add;
+    m = t;
+  }
+  ASRN_DEV void finish() {
+    if (on) p.part[at * p.pad + row] = make_float2(m, s);
+  }
+};
+
+// Block = 32 positions x 8 warps over the halves of the vocabulary's tiles.
+__global__ void __launch_bounds__(256)
+k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const int* __restrict__ pos,
+            const int* __restrict__ tok, const float* __restrict__ top, const float2* __restrict__ part,
+            float* __restrict__ lse2, float* __restrict__ rest, float* __restrict__ logp) {
+  __shared__ float2 sh[8][32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const int r = i < N ? pos[i] : -1;
+  float m = -INFINITY, s = 0.f;
+  auto join = [&](float2 q) {
+    if (q.y == 0.f) return;                // nothing there
+    const float t = fmaxf(m, q.x);
+    s = (m == t ? s : s * exp2f((m - t) * k)) + (q.x == t ? q.y : q.y * exp2f((q.x - t) * k));
+    m = t;
+  };
+  if (r >= 0)
+#pragma unroll 4
+    for (int j = wid; j < halves; j += 8) join(part[j * pad + r]);
+  sh[wid][lane] = make_float2(m, s);
+  __syncthreads();
+  if (wid || i >= N) return;
+  for (int w = 1; w < 8; ++w) join(sh[w][lane]);
+  if (r < 0) {
+    logp[i] = 0.f;
+    return;
+  }
+  if (tok[r] < 0) {
+    logp[i] = NAN;
+    return;
+  }
+  const float own = top[r], x = (own - m) * inv_tau;
+  const float lp = s == 0.f ? own * 0.f : x > 0.f ? -log1pf(s * expf(-x)) : x - logf(s + expf(x));
+  logp[i] = lp;
+  lse2[r] = own * k - lp * kLog2e;
+  rest[r] = -expm1f(lp);
+}
+
+// dS of one chunk in bf16; the rows that pad the last tile get zeros.
+struct Slope {
+  struct Params {
+    const int *tok, *row;                  // of the chunk's rows
+    const float *lse2, *rest, *g;
+    float k, inv_tau;
+    __nv_bfloat16* out;
+    int64_t pitch;
+    int room;                              // rows of `out`
+  };
+  const Params& p;
+  int V, y;
+  float off, g, own;
+  bool on;
+  __nv_bfloat16* at;
+  ASRN_DEV Slope(const Params& pp, int r, int rows, int, const gemm::Shape& sh, const gemm::Tile&, int)
+      : p(pp), V(sh.N), y(-1), off(0.f), g(0.f), own(0.f), on(r < rows), at(r < pp.room ? pp.out + r * pp.pitch : nullptr) {
+    if (on) {
+      y = p.tok[r];
+      off = p.lse2[r];
+      g = y < 0 ? NAN : p.g[p.row[r]] * p.inv_tau;
+      own = g * p.rest[r];
+    }
+  }
+  ASRN_DEV void chunk(float* v, int c) {
+    if (!at || c >= V) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float e = exp2_fast(fmaf(v[i], p.k, -off));
+      v[i] = !on ? 0.f : c + i == y ? own : -g * e;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(at + c + i) = gemm::pack8(v + i);
+  }
+  ASRN_DEV void finish() {}
+};
+
+// dh of the positions whose rows lie in this chunk: the parts of V added up in order. Positions without a target get
+// zeros with the first chunk.
+__global__ void __launch_bounds__(256)
+k_head_dh(int64_t N, int d, int first, int rows, int splits, const int* __restrict__ pos,
+          const float* __restrict__ part, __nv_bfloat16* __restrict__ dh) {
+  const int nv = d / 8;
+  const int64_t total = N * nv;
+  for (int64_t x = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; x < total; x += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t i = x / nv;
+    const int c = (int)(x % nv) * 8, r = pos[i];
+    float v[8] = {};
+    if (r < 0) {
+      if (first) continue;
+    } else {
+      if (r < first || r >= first + rows) continue;
+      for (int k = 0; k < splits; ++k) {
+        const float4* q = reinterpret_cast<const float4*>(part + ((int64_t)k * rows + (r - first)) * d + c);
+        const float4 a = q[0], b = q[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+    }
+    *reinterpret_cast<uint4*>(dh + i * d + c) = gemm::pack8(v);
+  }
+}
+
+int check_head(int64_t N, int64_t V, int32_t d) {
+  if (N < 0 || V < 1 || d < 1) return ASRN_ERR_ARG;
+  if (d % 8 || d > 16384 || V > (1 << 24) || N > (1 << 24)) return ASRN_ERR_UNSUPPORTED;
+  return ASRN_OK;
+}
+
+}  // namespace
+
+// Parts of K added up in order and rounded: out[n] = bf16(sum_k part[k][n]).
+__global__ void __launch_bounds__(256) k_sum_parts(int64_t n, int parts, const float* __restrict__ part,
+                                                   __nv_bfloat16* __restrict__ out) {
+  for (int64_t x = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; x < n;
+       x += (int64_t)gridDim.x * blockDim.x * 8) {
+    float v[8] = {};
+    for (int k = 0; k < parts; ++k) {
+      const float4* q = reinterpret_cast<const float4*>(part + k * n + x);
+      const float4 a = q[0], b = q[1];
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    *reinterpret_cast<uint4*>(out + x) = gemm::pack8(v);
+  }
+}
+
+int sum_parts(int64_t n, int parts, const float* part, __nv_bfloat16* out, cudaStream_t s) {
+  const int64_t blocks = (n / 8 + 255) / 256;
+  k_sum_parts<<<(unsigned)std::min<int64_t>(blocks, 148 * 8), 256, 0, s>>>(n, parts, part, out);
+  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
+}  // namespace asrn
+
+extern "C" {
+
+size_t asrn_head_saved_bytes(int64_t N, int32_t d) {
+  if (asrn::check_head(N, 1, d)) return 0;
+  return asrn::head_saved(N, d).total;
+}
+
+size_t asrn_head_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t backward) {
+  if (asrn::check_head(N, V, d)) return 0;
+  return backward ? asrn::head_backward_ws(N, V, d).total : asrn::head_forward_ws(N, V).total;
+}
+
+int asrn_head_forward(int64_t N, int64_t V, int32_t d, const void* h, const void* weight, const int64_t* tokens,
+                      float tau, float* logp, void* saved, size_t saved_bytes, void* workspace,
+                      size_t workspace_bytes, int* status, void* stream) {
+  using namespace asrn;
+  int st = check_head(N, V, d);
+  if (st) return st;
+  if (!(tau > 0.f) || tau > 1e30f) return ASRN_ERR_ARG;
+  if (N == 0) return ASRN_OK;
+  if (!h || !weight || !tokens || !logp || (uintptr_t)h % 16 || (uintptr_t)weight % 16) return ASRN_ERR_ARG;
+  const HeadSaved sv = head_saved(N, d);
+  const HeadForwardWs ws = head_forward_ws(N, V);
+  if (!saved || saved_bytes < sv.total || (uintptr_t)saved % 256 || !workspace || workspace_bytes < ws.total ||
+      (uintptr_t)workspace % 256)
+    return ASRN_ERR_WORKSPACE;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* S = reinterpret_cast<char*>(saved);
+  char* W = reinterpret_cast<char*>(workspace);
+  int* count = reinterpret_cast<int*>(S + sv.count);
+  int* tok = reinterpret_cast<int*>(S + sv.tok);
+  int* pos = reinterpret_cast<int*>(S + sv.pos);
+  __nv_bfloat16* hc = reinterpret_cast<__nv_bfloat16*>(S + sv.hc);
+  int* counts = nullptr;
+  if (N > kDirectRows) {
+    counts = reinterpret_cast<int*>(W + ws.counts);
+    k_head_count<<<(unsigned)((N + kCountRows - 1) / kCountRows), kCountRows, 0, s>>>(N, tokens, counts);
+  }
+  k_head_gather<<<(unsigned)((N + kGatherRows - 1) / kGatherRows), kGatherThreads, 0, s>>>(
+      N, V, d, reinterpret_cast<const __nv_bfloat16*>(h), tokens, counts, count, tok,
+      reinterpret_cast<int*>(S + sv.row), pos, hc);
+  if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
+  gemm::Shape sh{};
+  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.splits = 1; sh.group = 16; sh.status = status;
+  const float inv_tau = 1.f / tau;
+  Lse::Params p{tok, kLog2e * inv_tau, reinterpret_cast<float*>(W + ws.top), reinterpret_cast<float2*>(W + ws.part),
+                pad256(N)};
+  if ((st = gemm::launch_cg<1, false, false, Lse>(hc, d, weight, d, sh, p, s))) return st;
+  k_head_join<<<(unsigned)((N + 31) / 32), 256, 0, s>>>(N, (int)((V + gemm::kBN - 1) / gemm::kBN) * 2, p.pad, p.k,
+                                                        inv_tau, pos, tok, p.top, p.part,
+                                                        reinterpret_cast<float*>(S + sv.lse2),
+                                                        reinterpret_cast<float*>(S + sv.rest), logp);
+  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
+int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
+                       float tau, const float* g, void* dh, void* dw, void* workspace, size_t workspace_bytes,
+                       int* status, void* stream) {
+  using namespace asrn;
+  int st = check_head(N, V, d);
+  if (st) return st;
+  if (!(tau > 0.f) || tau > 1e30f) return ASRN_ERR_ARG;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (N == 0) {
+    if (dw && cudaMemsetAsync(dw, 0, (size_t)V * d * 2, s) != cudaSuccess) return ASRN_ERR_CUDA;
+    return ASRN_OK;
+  }
+  if (!weight || !g || (uintptr_t)weight % 16 || (uintptr_t)dh % 16 || (uintptr_t)dw % 16) return ASRN_ERR_ARG;
+  const HeadSaved sv = head_saved(N, d);
+  const HeadBackwardWs ws = head_backward_ws(N, V, d);
+  if (!saved || saved_bytes < sv.total || (uintptr_t)saved % 256 || !workspace || workspace_bytes < ws.total ||
+      (uintptr_t)workspace % 256)
+    return ASRN_ERR_WORKSPACE;
+  const char* S = reinterpret_cast<const char*>(saved);
+  char* W = reinterpret_cast<char*>(workspace);
+  const int* count = reinterpret_cast<const int*>(S + sv.count);
+  __nv_bfloat16* ds = reinterpret_cast<__nv_bfloat16*>(W + ws.ds);
+  float* dhp = reinterpret_cast<float*>(W + ws.dh);
+  float* dwp = reinterpret_cast<float*>(W + ws.dw);
+  const bool direct = ws.chunks == 1 && ws.split_w == 1;
+  for (int c = 0; c < ws.chunks; ++c) {
+    const int64_t first = c * ws.rows;
+    const int rows = (int)ws.rows;
+    const __nv_bfloat16* hc = reinterpret_cast<const __nv_bfloat16*>(S + sv.hc) + first * d;
+    const int64_t left = std::min<int64_t>(rows, pad256(N) - first);   // rows of hc from here on
+    gemm::Shape sh{};
+    sh.M = (int)left; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.m_off = (int)first; sh.splits = 1; sh.group = 16;
+    sh.status = status;
+    Slope::Params p{reinterpret_cast<const int*>(S + sv.tok) + first, reinterpret_cast<const int*>(S + sv.row) + first,
+                    reinterpret_cast<const float*>(S + sv.lse2) + first,
+                    reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau, ds, ws.pitch,
+                    rows};
+    if ((st = gemm::launch_cg<1, false, false, Slope>(hc, d, weight, d, sh, p, s))) return st;
+    if (dh) {
+      gemm::Shape a{};
+      a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.splits = ws.split_h; a.group = 16;
+      a.status = status;
+      if ((st = gemm::launch_cg<1, false, true, gemm::StoreF32>(ds, ws.pitch, weight, d, a, {dhp, 0}, s))) return st;
+      const int64_t work = (N * (d / 8) + 255) / 256;
+      k_head_dh<<<(unsigned)std::min<int64_t>(work, 148 * 8), 256, 0, s>>>(
+          N, d, (int)first, rows, ws.split_h, reinterpret_cast<const int*>(S + sv.pos), dhp,
+          reinterpret_cast<__nv_bfloat16*>(dh));
+      if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
+    }
+    if (dw) {
+      gemm::Shape a{};
+      a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.splits = ws.split_w;
+      a.group = 16; a.status = status;
+      st = direct ? gemm::launch_cg<1, true, true, gemm::StoreBf16>(ds, ws.pitch, hc, d, a,
+                                                                   {reinterpret_cast<__nv_bfloat16*>(dw), nullptr}, s)
+                  : gemm::launch_cg<1, true, true, gemm::StoreF32>(ds, ws.pitch, hc, d, a, {dwp, c > 0}, s);
+      if (st) return st;
+    }
+  }
+  if (dw && !direct) return sum_parts(V * d, ws.split_w, dwp, reinterpret_cast<__nv_bfloat16*>(dw), s);
+  return ASRN_OK;
+}
+
+}  // extern "C"

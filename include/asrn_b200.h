@@ -230,6 +230,67 @@ int asrn_scan_forward(int64_t rows, int64_t L, const float* a, const float* b, f
 int asrn_scan_backward(int64_t rows, int64_t L, const float* a, const float* S, const float* g, float* ga, float* gb,
                        void* stream);
 
+/* ---- fine-tuning: log probabilities through the head, losses, MLP with 8-bit activations -----------------------------
+ * No counterpart in the reference. Operands are bfloat16 unless said otherwise, rows contiguous, pointers to matrices
+ * 16-byte aligned, widths multiples of 8 (else ASRN_ERR_UNSUPPORTED); `saved` and workspaces 256-byte aligned. status:
+ * device int in which the tensor-core kernels' bounded waits record ASRN_ERR_TIMEOUT (may be NULL). All sums run in a
+ * fixed order: results repeat bit for bit.
+ *
+ * asrn_head_forward: logp (N) float32 = log softmax(h W^T / tau)[token] for h (N, d), weight (V, d), tokens (N) int64.
+ * A negative token leaves its position out: logp 0, no gradient, no work. A token >= V gives NaN. `saved` keeps what
+ * the backward pass needs (asrn_head_saved_bytes). N, V <= 2^24.
+ * asrn_head_backward: from g (N) float32 = dL/dlogp, dh (N, d) and dw (V, d); either may be NULL. */
+size_t asrn_head_saved_bytes(int64_t N, int32_t d);
+size_t asrn_head_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t backward);
+int asrn_head_forward(int64_t N, int64_t V, int32_t d, const void* h, const void* weight, const int64_t* tokens,
+                      float tau, float* logp, void* saved, size_t saved_bytes, void* workspace,
+                      size_t workspace_bytes, int* status, void* stream);
+int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
+                       float tau, const float* g, void* dh, void* dw, void* workspace, size_t workspace_bytes,
+                       int* status, void* stream);
+
+/* Preference loss of P answer pairs: logp, ref_logp (2, P, L) float32, mask (2, P, L) bytes; [0] the chosen answers,
+ * [1] the rejected ones. R = sum over the mask of (logp - ref_logp), D = R_chosen - R_rejected.
+ *   kind 0  -(1 - smoothing) log sigma(beta D) - smoothing log sigma(-beta D), 0 <= smoothing < 0.5
+ *   kind 1  (D of the means over the tokens - 1 / (2 beta))^2, smoothing 0
+ * loss: the mean over the pairs whose two answers both have a token (0 without one; other pairs get no gradient). grad
+ * (2, P, L) = dloss/dlogp (may be NULL), rewards (2, P) = beta R. What stands outside the mask is never used.
+ * asrn_policy_loss: clipped policy loss of B sequences: with r = exp(logp - old_logp), q = ref_logp - logp (both
+ * differences held to [-20, 20], without gradient beyond),
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(q) - q - 1)
+ * averaged over all tokens of the mask, or (per_sequence) over each sequence's tokens and then over the sequences that
+ * have one. advantages (B, L) (adv_per_token) or (B); ref_logp may be NULL when kl is 0. grad (B, L) = dloss/dlogp (may
+ * be NULL); stats (2) = mean of exp(q) - q - 1 and share of tokens whose ratio was clipped, over the mask's tokens.
+ * Workspace 16-byte aligned. */
+size_t asrn_preference_workspace_bytes(int64_t P, int64_t L);
+int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* ref_logp, const uint8_t* mask,
+                         int32_t kind, double beta, double smoothing, float* loss, float* grad, float* rewards,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t asrn_policy_workspace_bytes(int64_t B, int64_t L);
+int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_logp, const float* ref_logp,
+                     const float* advantages, int32_t adv_per_token, const uint8_t* mask, double clip_low,
+                     double clip_high, double kl, int32_t per_sequence, float* loss, float* grad, float* stats,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* 8-bit activations: rows of f values in blocks of 32 (the last one shorter), int8 codes (rows, f) and one exponent byte
+ * per block, exps (rows, ceil(f / 32)): value = code 2^e, e the least with max|x| <= 127 2^e and at least -120, code =
+ * x 2^-e rounded to the nearest, ties to even. A block with an infinity or a NaN has e = -128 and reads back as NaN. x:
+ * bfloat16 (every value read back is exact in it).
+ * asrn_mlp8_forward: y (N, dout) = gelu(x W1^T + b1) W2^T + b2 with x (N, d), w1 (ff, d), b1 (ff), w2 (dout, ff), b2
+ * (dout); `saved` (may be NULL: nothing kept) holds x and x W1^T + b1 in 8 bits.
+ * asrn_mlp8_backward: the gradients from dy (N, dout), each of which may be NULL, with the 8-bit values in place of x and
+ * x W1^T + b1. */
+int asrn_pack8(int64_t rows, int32_t f, const void* x, void* codes, void* exps, void* stream);
+int asrn_unpack8(int64_t rows, int32_t f, const void* codes, const void* exps, void* x, void* stream);
+size_t asrn_mlp8_saved_bytes(int64_t N, int32_t d, int32_t ff);
+size_t asrn_mlp8_workspace_bytes(int64_t N, int32_t d, int32_t ff, int32_t dout, int32_t backward);
+int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void* x, const void* w1, const void* b1,
+                      const void* w2, const void* b2, void* y, void* saved, size_t saved_bytes, void* workspace,
+                      size_t workspace_bytes, int* status, void* stream);
+int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void* dy, const void* w1, const void* w2,
+                       const void* saved, size_t saved_bytes, void* dx, void* dw1, void* db1, void* dw2, void* db2,
+                       void* workspace, size_t workspace_bytes, int* status, void* stream);
+
 /* ---- sequence-chunk sharding (one long sequence over several GPUs) --------------------------------------------------
  * Shard r of `world` owns positions [c0, c0 + Lc) of every sequence (L = world * Lc). Its sorted rows hold its own
  * slots and, before each bucket's local run, the up to C earlier-chunk slots some local query has as a candidate (the
