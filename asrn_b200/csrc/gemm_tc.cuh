@@ -390,8 +390,19 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
   return cudaLaunchKernelEx(&cfg, kernel, ma, mb, s, p) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 
+// Blocks in pairs unless one block's 128 rows hold all of M.
+inline int pair_for(int64_t M) { return M > kBM ? 2 : 1; }
+
+template <bool AMn, bool BMn, class Epi>
+int launch(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const Shape& s,
+           const typename Epi::Params& p, cudaStream_t stream) {
+  return pair_for(s.M) == 2 ? launch_cg<2, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, stream)
+                            : launch_cg<1, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, stream);
+}
+
 // Parts of K that give every SM a tile, each of 8 K blocks at least.
-inline int splits_for(int64_t M, int64_t N, int64_t K, int cg) {
+inline int splits_for(int64_t M, int64_t N, int64_t K) {
+  const int cg = pair_for(M);
   const int tiles = std::max(1, tiles_of(M, N, cg)), slots = sm_count() / cg;
   const int64_t most = std::max<int64_t>(1, (K + kBK - 1) / kBK / 8);
   return (int)std::max<int64_t>(1, std::min<int64_t>(slots / tiles, most));

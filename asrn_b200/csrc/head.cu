@@ -83,8 +83,8 @@ HeadBackwardWs head_backward_ws(int64_t N, int64_t V, int64_t d) {
   w.chunks = (int)((pad256(N) + most - 1) / most);
   w.rows = std::max<int64_t>(256, pad256((N + w.chunks - 1) / std::max(1, w.chunks)));
   w.chunks = (int)((pad256(N) + w.rows - 1) / w.rows);
-  w.split_h = gemm::splits_for(w.rows, d, V, 1);
-  w.split_w = gemm::splits_for(V, d, w.rows, 1);
+  w.split_h = gemm::splits_for(w.rows, d, V);
+  w.split_w = gemm::splits_for(V, d, w.rows);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.ds = take((size_t)w.rows * w.pitch * 2);
@@ -384,7 +384,7 @@ int asrn_head_forward(int64_t N, int64_t V, int32_t d, const void* h, const void
   const float inv_tau = 1.f / tau;
   Lse::Params p{tok, kLog2e * inv_tau, reinterpret_cast<float*>(W + ws.top), reinterpret_cast<float2*>(W + ws.part),
                 pad256(N)};
-  if ((st = gemm::launch_cg<1, false, false, Lse>(hc, d, weight, d, sh, p, s))) return st;
+  if ((st = gemm::launch<false, false, Lse>(hc, d, weight, d, sh, p, s))) return st;
   k_head_join<<<(unsigned)((N + 31) / 32), 256, 0, s>>>(N, (int)((V + gemm::kBN - 1) / gemm::kBN) * 2, p.pad, p.k,
                                                         inv_tau, pos, tok, p.top, p.part,
                                                         reinterpret_cast<float*>(S + sv.lse2),
@@ -429,12 +429,12 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
                     reinterpret_cast<const float*>(S + sv.lse2) + first,
                     reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau, ds, ws.pitch,
                     rows};
-    if ((st = gemm::launch_cg<1, false, false, Slope>(hc, d, weight, d, sh, p, s))) return st;
+    if ((st = gemm::launch<false, false, Slope>(hc, d, weight, d, sh, p, s))) return st;
     if (dh) {
       gemm::Shape a{};
       a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.splits = ws.split_h; a.group = 16;
       a.status = status;
-      if ((st = gemm::launch_cg<1, false, true, gemm::StoreF32>(ds, ws.pitch, weight, d, a, {dhp, 0}, s))) return st;
+      if ((st = gemm::launch<false, true, gemm::StoreF32>(ds, ws.pitch, weight, d, a, {dhp, 0}, s))) return st;
       const int64_t work = (N * (d / 8) + 255) / 256;
       k_head_dh<<<(unsigned)std::min<int64_t>(work, 148 * 8), 256, 0, s>>>(
           N, d, (int)first, rows, ws.split_h, reinterpret_cast<const int*>(S + sv.pos), dhp,
@@ -445,9 +445,9 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
       gemm::Shape a{};
       a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.splits = ws.split_w;
       a.group = 16; a.status = status;
-      st = direct ? gemm::launch_cg<1, true, true, gemm::StoreBf16>(ds, ws.pitch, hc, d, a,
+      st = direct ? gemm::launch<true, true, gemm::StoreBf16>(ds, ws.pitch, hc, d, a,
                                                                    {reinterpret_cast<__nv_bfloat16*>(dw), nullptr}, s)
-                  : gemm::launch_cg<1, true, true, gemm::StoreF32>(ds, ws.pitch, hc, d, a, {dwp, c > 0}, s);
+                  : gemm::launch<true, true, gemm::StoreF32>(ds, ws.pitch, hc, d, a, {dwp, c > 0}, s);
       if (st) return st;
     }
   }

@@ -266,8 +266,8 @@ Mlp8Ws mlp8_ws(int64_t N, int64_t d, int64_t ff, int64_t dout, bool backward) {
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.g = take((size_t)N * ff * 2);
   if (backward) {
-    w.split1 = gemm::splits_for(ff, d, N, 1);
-    w.split2 = gemm::splits_for(dout, ff, N, 1);
+    w.split1 = gemm::splits_for(ff, d, N);
+    w.split2 = gemm::splits_for(dout, ff, N);
     w.da = take((size_t)N * ff * 2);
     w.x = take((size_t)N * d * 2);
     w.sum1 = take((size_t)((N + 31) / 32) * ff * 4);
@@ -310,8 +310,8 @@ int weight_grad(int64_t rows, int M, int n, const void* A, const void* B, int sp
   gemm::Shape a{};
   a.M = M; a.N = n; a.K = (int)rows; a.splits = splits; a.group = 16; a.status = status;
   __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-  if (splits == 1) return gemm::launch_cg<1, true, true, gemm::StoreBf16>(A, M, B, n, a, {o, nullptr}, s);
-  const int st = gemm::launch_cg<1, true, true, gemm::StoreF32>(A, M, B, n, a, {part, 0}, s);
+  if (splits == 1) return gemm::launch<true, true, gemm::StoreBf16>(A, M, B, n, a, {o, nullptr}, s);
+  const int st = gemm::launch<true, true, gemm::StoreF32>(A, M, B, n, a, {part, 0}, s);
   return st ? st : sum_parts((int64_t)M * n, splits, part, o, s);
 }
 
@@ -371,9 +371,9 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   a.M = (int)N; a.N = ff; a.K = d; a.splits = 1; a.group = 16; a.status = status;
   Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), g, S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
                S ? reinterpret_cast<int8_t*>(S + sv.ae) : nullptr};
-  if ((st = gemm::launch_cg<1, false, false, Up>(x, d, w1, d, a, p, s))) return st;
+  if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s))) return st;
   a.N = dout; a.K = ff;
-  return gemm::launch_cg<1, false, false, gemm::StoreBf16>(
+  return gemm::launch<false, false, gemm::StoreBf16>(
       g, ff, w2, ff, a, {reinterpret_cast<__nv_bfloat16*>(y), reinterpret_cast<const __nv_bfloat16*>(b2)}, s);
 }
 
@@ -413,11 +413,11 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
     a.N = ff; a.K = dout;
     Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), reinterpret_cast<const int8_t*>(S + sv.ae), da, g,
                    db1 ? sum1 : nullptr};
-    if ((st = gemm::launch_cg<1, false, true, Down>(dy, dout, w2, ff, a, p, s))) return st;
+    if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s))) return st;
   }
   if (dx) {
     a.N = d; a.K = ff;
-    if ((st = gemm::launch_cg<1, false, true, gemm::StoreBf16>(da, ff, w1, d, a,
+    if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, ff, w1, d, a,
                                                                {reinterpret_cast<__nv_bfloat16*>(dx), nullptr}, s)))
       return st;
   }
