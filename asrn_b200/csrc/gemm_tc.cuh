@@ -15,6 +15,7 @@
 // ends.
 #pragma once
 #include <algorithm>
+#include <atomic>
 #include "layout.h"
 #include "umma.cuh"
 
@@ -363,18 +364,31 @@ inline bool operand_map(CUtensorMap* map, const void* base, bool mn, int64_t row
             : make_tmap_bf16(map, base, (uint64_t)depth, (uint64_t)rows, (uint64_t)pitch * 2, kBK, (uint32_t)box_rows);
 }
 
+// The tensor map call needs a current context: a thread gets its device's with its first call here.
+inline bool bind_context() {
+  static thread_local bool bound = false;
+  int dev = 0;
+  if (!bound) bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+  return bound;
+}
+
 template <int CG, bool AMn, bool BMn, class Epi>
 int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const Shape& s,
               const typename Epi::Params& p, cudaStream_t stream) {
   CUtensorMap ma, mb;
-  int dev = 0;                // the tensor map call needs a context: a thread that has none yet gets its device's
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return ASRN_ERR_CUDA;
+  if (!bind_context()) return ASRN_ERR_CUDA;
   if (!operand_map(&ma, A, AMn, s.M, s.K, pitch_a, kBM) || !operand_map(&mb, B, BMn, s.N, s.K, pitch_b, kBN / CG))
     return ASRN_ERR_CUDA;
   auto kernel = k_gemm<CG, AMn, BMn, Epi>;
   constexpr size_t smem = smem_bytes<CG>();
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return ASRN_ERR_CUDA;
+  static std::atomic<uint64_t> ready{0};                  // devices that know the kernel's shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ASRN_ERR_CUDA;
+  if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return ASRN_ERR_CUDA;
+    if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
   const int64_t tiles = (int64_t)tiles_of(s.M, s.N, CG) * s.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, sm_count() / CG) * CG));

@@ -425,7 +425,7 @@ bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L
 extern "C" {
 
 size_t asrn_preference_workspace_bytes(int64_t P, int64_t L) {
-  if (P < 0 || L < 0) return 0;
+  if (P < 0 || L < 0 || asrn::small_loss(2 * P, L)) return 0;
   return asrn::align_up((size_t)(2 * P * asrn::loss_chunks(L)) * sizeof(asrn::RowSum) + 1);
 }
 
@@ -456,7 +456,7 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
 }
 
 size_t asrn_policy_workspace_bytes(int64_t B, int64_t L) {
-  if (B < 0 || L < 0) return 0;
+  if (B < 0 || L < 0 || asrn::small_loss(B, L)) return 0;
   const size_t items = (size_t)(B * asrn::loss_chunks(L));
   return 256 + asrn::align_up(items * sizeof(asrn::TokenSum)) + asrn::align_up(items * sizeof(int));
 }

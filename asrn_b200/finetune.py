@@ -54,6 +54,11 @@ def status(device=None, reset=False):
     return v
 
 
+def _stream(dev):
+    """The current stream's handle on dev, an int (a call that takes about 10 us in all feels a Stream object's 2)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _need_cuda(what, *ts):
     dev = ts[0].device
     for t in ts:
@@ -63,16 +68,18 @@ def _need_cuda(what, *ts):
             raise RuntimeError(f'asrn_b200.{what} runs on CUDA tensors only (there is no CPU implementation)')
         if t.device != dev:
             raise ValueError(f'{what}: tensors on {dev} and {t.device}')
+    return dev
 
 
 def _rows(t):
-    """Contiguous and 16-byte aligned (a view into a larger buffer may be neither)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    """Contiguous and 16-byte aligned (a view into a larger buffer may be neither); read through its address only."""
+    if not t.is_contiguous():
+        t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
 
 
 def _scratch(nbytes, dev):
-    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+    return torch.empty(nbytes or 256, dtype=torch.uint8, device=dev)
 
 
 # ---- head -------------------------------------------------------------------------------------------------------------
@@ -82,28 +89,30 @@ class _HeadLogprobs(torch.autograd.Function):
     def forward(ctx, h, w, tokens, tau):
         d, V, N = h.shape[-1], w.shape[0], tokens.numel()
         dev, lib = h.device, _lib.lib()
-        hr, wr, tok = _rows(h.detach()), _rows(w.detach()), tokens.contiguous()
+        hr, wr, tok = _rows(h), _rows(w), tokens.contiguous()
         out = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
         nb_saved, nb = lib.asrn_head_saved_bytes(N, d), lib.asrn_head_workspace_bytes(N, V, d, 0)
         saved, ws = _scratch(nb_saved, dev), _scratch(nb, dev)
-        _lib.check(lib.asrn_head_forward(N, V, d, _p(hr), _p(wr), _p(tok), tau, _p(out), _p(saved), saved.numel(),
-                                         _p(ws), ws.numel(), _status_word(dev), _lib.stream_ptr(dev)),
-                   'asrn_head_forward')
+        _lib.check(lib.asrn_head_forward(N, V, d, hr.data_ptr(), wr.data_ptr(), tok.data_ptr(), tau, out.data_ptr(),
+                                         saved.data_ptr(), nb_saved, ws.data_ptr(), nb, _status_word(dev),
+                                         _stream(dev)), 'asrn_head_forward')
         ctx.save_for_backward(wr, saved)
-        ctx.meta = (h.shape, N, V, d, tau)
+        ctx.meta = (h.shape, N, V, d, tau, dev, nb_saved)
         return out
 
     @staticmethod
     def backward(ctx, g):
         w, saved = ctx.saved_tensors
-        shape, N, V, d, tau = ctx.meta
-        dev, lib = w.device, _lib.lib()
-        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(V, d, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[1] else None
-        g32 = g.float().contiguous()
-        ws = _scratch(lib.asrn_head_workspace_bytes(N, V, d, 1), dev)
-        _lib.check(lib.asrn_head_backward(N, V, d, _p(w), _p(saved), saved.numel(), tau, _p(g32), _p(dh), _p(dw),
-                                          _p(ws), ws.numel(), _status_word(dev), _lib.stream_ptr(dev)),
+        shape, N, V, d, tau, dev, nb_saved = ctx.meta
+        lib = _lib.lib()
+        need = ctx.needs_input_grad
+        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if need[0] else None
+        dw = torch.empty((V, d), dtype=torch.bfloat16, device=dev) if need[1] else None
+        g32 = _f32(g)
+        nb = lib.asrn_head_workspace_bytes(N, V, d, 1)
+        ws = _scratch(nb, dev)
+        _lib.check(lib.asrn_head_backward(N, V, d, w.data_ptr(), saved.data_ptr(), nb_saved, tau, g32.data_ptr(),
+                                          _p(dh), _p(dw), ws.data_ptr(), nb, _status_word(dev), _stream(dev)),
                    'asrn_head_backward')
         return dh, dw, None, None
 
@@ -160,13 +169,16 @@ class _WithGrad(torch.autograd.Function):
 
 
 def _f32(t):
+    """float32 and contiguous; read through its address only."""
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
     return t.detach().to(torch.float32).contiguous()
 
 
 def _mask(m, shape, what):
     if m.shape != shape or m.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f'{what}: mask has to be bool or uint8 of shape {tuple(shape)}; got {m.dtype} {tuple(m.shape)}')
-    return m.contiguous()
+    return m if m.is_contiguous() else m.contiguous()
 
 
 PreferenceLoss = namedtuple('PreferenceLoss', 'loss grad chosen rejected')
@@ -191,22 +203,21 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
         raise ValueError(f'preference_loss: kind is one of {sorted(_KINDS)}')
     if not beta > 0 or not 0 <= smoothing < 0.5 or (kind == 'ipo' and smoothing):
         raise ValueError("preference_loss: beta > 0, 0 <= smoothing < 0.5, and no smoothing with 'ipo'")
-    _need_cuda('preference_loss', logp, ref_logp, mask)
+    dev, lib = _need_cuda('preference_loss', logp, ref_logp, mask), _lib.lib()
     m = _mask(mask, logp.shape, 'preference_loss')
     _, P, L = logp.shape
-    dev, lib = logp.device, _lib.lib()
     lp, rf = _f32(logp), _f32(ref_logp)
     nb = lib.asrn_preference_workspace_bytes(P, L)
-    out = torch.empty(4 + 2 * P, dtype=torch.float32, device=dev)
-    grad = torch.empty(2, P, L, dtype=torch.float32, device=dev)
-    ws = _scratch(nb, dev)
-    base = out.data_ptr()
-    _lib.check(lib.asrn_preference_loss(P, L, _p(lp), _p(rf), _p(m), _KINDS[kind], beta, smoothing, base, _p(grad),
-                                        base + 16, _p(ws), ws.numel(), _lib.stream_ptr(dev)), 'asrn_preference_loss')
-    loss = out[0]
-    if torch.is_grad_enabled() and logp.requires_grad:
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
+    grad = torch.empty((2, P, L), dtype=torch.float32, device=dev)
+    ws = _scratch(nb, dev) if nb else None
+    _lib.check(lib.asrn_preference_loss(P, L, lp.data_ptr(), rf.data_ptr(), m.data_ptr(), _KINDS[kind], beta, smoothing,
+                                        loss.data_ptr(), grad.data_ptr(), rewards.data_ptr(), _p(ws), nb,
+                                        _stream(dev)), 'asrn_preference_loss')
+    if logp.requires_grad and torch.is_grad_enabled():
         loss = _WithGrad.apply(logp, loss, grad)
-    return PreferenceLoss(loss, grad, out[4:4 + P], out[4 + P:])
+    return PreferenceLoss(loss, grad, *rewards.unbind())
 
 
 def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2), kl=0.0, per='token'):
@@ -229,23 +240,23 @@ def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2)
         raise ValueError('policy_loss: 0 <= clip[0] < 1, clip[1] >= 0 and kl >= 0')
     if kl > 0 and ref_logp is None:
         raise ValueError('policy_loss: a KL term needs ref_logp')
-    _need_cuda('policy_loss', logp, old_logp, advantages, mask, ref_logp)
+    dev, lib = _need_cuda('policy_loss', logp, old_logp, advantages, mask, ref_logp), _lib.lib()
     m = _mask(mask, logp.shape, 'policy_loss')
     B, L = logp.shape
-    dev, lib = logp.device, _lib.lib()
     lp, old, adv = _f32(logp), _f32(old_logp), _f32(advantages)
     ref = None if ref_logp is None else _f32(ref_logp)
     out = torch.empty(3, dtype=torch.float32, device=dev)
-    grad = torch.empty(B, L, dtype=torch.float32, device=dev)
-    ws = _scratch(lib.asrn_policy_workspace_bytes(B, L), dev)
+    grad = torch.empty((B, L), dtype=torch.float32, device=dev)
+    nb = lib.asrn_policy_workspace_bytes(B, L)
+    ws = _scratch(nb, dev) if nb else None
     base = out.data_ptr()
-    _lib.check(lib.asrn_policy_loss(B, L, _p(lp), _p(old), _p(ref), _p(adv), int(adv.dim() == 2), _p(m), low, high, kl,
-                                    _PER[per], base, _p(grad), base + 4, _p(ws), ws.numel(), _lib.stream_ptr(dev)),
-               'asrn_policy_loss')
-    loss = out[0]
-    if torch.is_grad_enabled() and logp.requires_grad:
+    _lib.check(lib.asrn_policy_loss(B, L, lp.data_ptr(), old.data_ptr(), _p(ref), adv.data_ptr(), adv.dim() == 2,
+                                    m.data_ptr(), low, high, kl, _PER[per], base, grad.data_ptr(), base + 4, _p(ws), nb,
+                                    _stream(dev)), 'asrn_policy_loss')
+    loss, k3, clipped = out.unbind()
+    if logp.requires_grad and torch.is_grad_enabled():
         loss = _WithGrad.apply(logp, loss, grad)
-    return PolicyLoss(loss, grad, out[1], out[2])
+    return PolicyLoss(loss, grad, k3, clipped)
 
 
 # ---- activations in 8 bits ----------------------------------------------------------------------------------------------
@@ -285,32 +296,35 @@ class _Mlp8(torch.autograd.Function):
     def forward(ctx, x, w1, b1, w2, b2):
         d, ff, dout = x.shape[-1], w1.shape[0], w2.shape[0]
         N, dev, lib = x.numel() // d, x.device, _lib.lib()
-        xr, w1, b1, w2, b2 = (_rows(t.detach()) for t in (x, w1, b1, w2, b2))
-        y = torch.empty(*x.shape[:-1], dout, dtype=torch.bfloat16, device=dev)
+        xr, w1, b1, w2, b2 = _rows(x), _rows(w1), _rows(b1), _rows(w2), _rows(b2)
+        y = torch.empty((*x.shape[:-1], dout), dtype=torch.bfloat16, device=dev)
         keep = any(ctx.needs_input_grad)
-        saved = _scratch(lib.asrn_mlp8_saved_bytes(N, d, ff), dev) if keep else None
-        ws = _scratch(lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 0), dev)
-        _lib.check(lib.asrn_mlp8_forward(N, d, ff, dout, _p(xr), _p(w1), _p(b1), _p(w2), _p(b2), _p(y), _p(saved),
-                                         saved.numel() if keep else 0, _p(ws), ws.numel(), _status_word(dev),
-                                         _lib.stream_ptr(dev)), 'asrn_mlp8_forward')
+        nb_saved = lib.asrn_mlp8_saved_bytes(N, d, ff) if keep else 0
+        nb = lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 0)
+        saved = _scratch(nb_saved, dev) if keep else None
+        ws = _scratch(nb, dev)
+        _lib.check(lib.asrn_mlp8_forward(N, d, ff, dout, xr.data_ptr(), w1.data_ptr(), b1.data_ptr(), w2.data_ptr(),
+                                         b2.data_ptr(), y.data_ptr(), _p(saved), nb_saved, ws.data_ptr(), nb,
+                                         _status_word(dev), _stream(dev)), 'asrn_mlp8_forward')
         if keep:
             ctx.save_for_backward(w1, w2, saved)
-            ctx.meta = (x.shape, N, d, ff, dout)
+            ctx.meta = (x.shape, N, d, ff, dout, dev, nb_saved)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         w1, w2, saved = ctx.saved_tensors
-        shape, N, d, ff, dout = ctx.meta
-        dev, lib = w1.device, _lib.lib()
-        need = ctx.needs_input_grad
+        shape, N, d, ff, dout, dev, nb_saved = ctx.meta
+        lib = _lib.lib()
         sizes = (shape, (ff, d), (ff,), (dout, ff), (dout,))
-        out = [torch.empty(s, dtype=torch.bfloat16, device=dev) if n else None for s, n in zip(sizes, need)]
-        dyr = _rows(dy.to(torch.bfloat16))
-        ws = _scratch(lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 1), dev)
-        _lib.check(lib.asrn_mlp8_backward(N, d, ff, dout, _p(dyr), _p(w1), _p(w2), _p(saved), saved.numel(),
-                                          *[_p(t) for t in out], _p(ws), ws.numel(), _status_word(dev),
-                                          _lib.stream_ptr(dev)), 'asrn_mlp8_backward')
+        out = [torch.empty(s, dtype=torch.bfloat16, device=dev) if n else None
+               for s, n in zip(sizes, ctx.needs_input_grad)]
+        dyr = _rows(dy)
+        nb = lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 1)
+        ws = _scratch(nb, dev)
+        _lib.check(lib.asrn_mlp8_backward(N, d, ff, dout, dyr.data_ptr(), w1.data_ptr(), w2.data_ptr(),
+                                          saved.data_ptr(), nb_saved, *[_p(t) for t in out], ws.data_ptr(), nb,
+                                          _status_word(dev), _stream(dev)), 'asrn_mlp8_backward')
         return tuple(out)
 
 
