@@ -5,6 +5,8 @@
 // Every sum is formed in a fixed order in fp64 (per thread, then by warp shuffles, then over the blocks' partials in
 // index order): the results do not depend on the blocks' timing. Positions outside the mask are read but selected away,
 // never multiplied, so a NaN or infinity there reaches nothing.
+#include <algorithm>
+#include <initializer_list>
 #include "common.cuh"
 #include "layout.h"
 
@@ -13,8 +15,8 @@ namespace asrn {
 namespace {
 
 constexpr int kLossThreads = 256;
-constexpr int kLossChunk = 2048;         // tokens of one row that a block takes at a time: 8 per thread
-constexpr int kLossPer = kLossChunk / kLossThreads;
+constexpr int kLossChunk = 4 * kLossThreads;   // tokens of one row that a block takes at a time, 4 a thread
+constexpr int kLossBlocks = 5;           // of k_policy_main that an SM holds
 constexpr int kSmallRows = 1024;         // rows a single block keeps in shared memory
 
 struct RowSum {                          // of one chunk of one row
@@ -28,17 +30,62 @@ __device__ __forceinline__ int warp_sum_i(int v) {
   return v;
 }
 
-// Sum over the block, in every thread; `slots` holds one value per warp.
-template <class T> __device__ __forceinline__ T block_sum(T v, T* slots) {
+// Sums over the block, in every thread; `slots` holds N values per warp. By shuffles within a warp, then each warp adds
+// up the warps' sums, in the same order.
+template <int N> __device__ __forceinline__ void block_sum(double (&v)[N], double* slots) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int i = 0; i < N; ++i) v[i] = warp_sum_d(v[i]);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) slots[(threadIdx.x >> 5) * N + i] = v[i];
   __syncthreads();
-  T s = 0;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += slots[i];
-  return s;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum_d(lane < warps ? slots[lane * N + i] : 0.);
 }
+
+// A thread's four values of a chunk of a row: neighbours (Vec: rows and pointers allow 16-byte loads) or a block's width
+// apart. place(j) is the j-th one's place in the chunk.
+template <bool Vec> __device__ __forceinline__ int place(int j) {
+  return Vec ? 4 * (int)threadIdx.x + j : j * kLossThreads + (int)threadIdx.x;
+}
+template <bool Vec> __device__ __forceinline__ void load4(float* v, const float* p, int left) {
+  if (Vec) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (place<Vec>(0) < left) x = __ldg(reinterpret_cast<const float4*>(p + place<Vec>(0)));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = place<Vec>(j) < left ? __ldg(p + place<Vec>(j)) : 0.f;
+  }
+}
+template <bool Vec> __device__ __forceinline__ uint32_t load_mask(const uint8_t* p, int left) {   // bit j
+  uint32_t m = 0;
+  if (Vec) {
+    if (place<Vec>(0) < left) {
+      const uchar4 x = __ldg(reinterpret_cast<const uchar4*>(p + place<Vec>(0)));
+      m = (uint32_t)((x.x != 0) | (x.y != 0) << 1 | (x.z != 0) << 2 | (x.w != 0) << 3);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (place<Vec>(j) < left) m |= (uint32_t)(__ldg(p + place<Vec>(j)) != 0) << j;
+  }
+  return m;
+}
+template <bool Vec> __device__ __forceinline__ void store4(float* p, const float* v, int left) {
+  if (Vec) {
+    if (place<Vec>(0) < left)
+      *reinterpret_cast<float4*>(p + place<Vec>(0)) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (place<Vec>(j) < left) p[place<Vec>(j)] = v[j];
+  }
+}
+
+__device__ __forceinline__ int chunk_left(int64_t L, int64_t t) { return (int)min(L - t, (int64_t)kLossChunk); }
 
 // ---- preference loss -----------------------------------------------------------------------------------------------
 
@@ -86,7 +133,7 @@ __device__ __forceinline__ double log_ratio(const PrefArgs& a, int64_t at) {
 __global__ void __launch_bounds__(1024) k_pref_small(PrefArgs a) {
   __shared__ double tot[kSmallRows];
   __shared__ int64_t cnt[kSmallRows];
-  __shared__ double slots[32];
+  __shared__ double slots[64];
   const int rows = (int)(2 * a.P), P = (int)a.P, lane = threadIdx.x & 31;
   for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
     double s = 0.;
@@ -108,9 +155,10 @@ __global__ void __launch_bounds__(1024) k_pref_small(PrefArgs a) {
   __syncthreads();
   Pair p{0., 0., 0., false};
   if (threadIdx.x < P) p = pair_of(a, tot[threadIdx.x], tot[P + threadIdx.x], cnt[threadIdx.x], cnt[P + threadIdx.x]);
-  const double pairs = fmax(1., block_sum(p.on ? 1. : 0., slots));
-  const double loss = block_sum(p.loss, slots);
-  if (threadIdx.x == 0) a.loss[0] = (float)(loss / pairs);
+  double sums[2] = {p.on ? 1. : 0., p.loss};
+  block_sum(sums, slots);
+  const double pairs = fmax(1., sums[0]);
+  if (threadIdx.x == 0) a.loss[0] = (float)(sums[1] / pairs);
   if (!a.grad) return;
   if (threadIdx.x < P) {
     tot[threadIdx.x] = p.slope0 / pairs;
@@ -126,89 +174,82 @@ __global__ void __launch_bounds__(1024) k_pref_small(PrefArgs a) {
   }
 }
 
-// Row sums by chunks: block (chunk, row).
-__global__ void __launch_bounds__(kLossThreads) k_pref_sums(PrefArgs a, int64_t items, int64_t chunks,
+// Row sums by parts of a row: item = (row, part of `width` tokens, a multiple of the chunk).
+template <bool Vec>
+__global__ void __launch_bounds__(kLossThreads) k_pref_sums(PrefArgs a, int64_t items, int64_t parts, int64_t width,
                                                             RowSum* __restrict__ part) {
-  __shared__ double slots[8];
-  __shared__ int islots[8];
+  __shared__ double slots[16];
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t row = it / chunks, t0 = (it % chunks) * kLossChunk;
-    const int64_t base = row * a.L + t0, left = a.L - t0;
-    float lp[kLossPer], rf[kLossPer];
-    uint8_t m[kLossPer];
-#pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      const bool in = t < left;
-      m[j] = in ? a.mask[base + t] : 0;
-      lp[j] = in ? __ldg(a.logp + base + t) : 0.f;
-      rf[j] = in ? __ldg(a.ref + base + t) : 0.f;
-    }
-    double s = 0.;
+    const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
+    double v[2] = {0., 0.};
     int n = 0;
+#pragma unroll 4
+    for (int64_t t = it % parts * width; t < t1; t += kLossChunk) {
+      float lp[4], rf[4];
+      const uint32_t m = load_mask<Vec>(a.mask + base + t, chunk_left(t1, t));
+      load4<Vec>(lp, a.logp + base + t, chunk_left(t1, t));
+      load4<Vec>(rf, a.ref + base + t, chunk_left(t1, t));
+      n += __popc(m);
 #pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      s += m[j] ? (double)lp[j] - (double)rf[j] : 0.;
-      n += m[j] != 0;
+      for (int j = 0; j < 4; ++j) v[0] += m >> j & 1 ? (double)lp[j] - (double)rf[j] : 0.;
     }
-    s = block_sum(s, slots);
-    n = block_sum(n, islots);
-    if (threadIdx.x == 0) part[it] = RowSum{s, n};
+    v[1] = (double)n;
+    block_sum(v, slots);
+    if (threadIdx.x == 0) part[it] = RowSum{v[0], (int64_t)v[1]};
   }
 }
 
-__device__ __forceinline__ RowSum row_total(const RowSum* part, int64_t row, int64_t chunks) {
+__device__ __forceinline__ RowSum row_total(const RowSum* part, int64_t row, int64_t parts) {
   RowSum t{0., 0};
-  for (int64_t c = 0; c < chunks; ++c) {
-    t.sum += part[row * chunks + c].sum;
-    t.n += part[row * chunks + c].n;
+  for (int64_t c = 0; c < parts; ++c) {
+    t.sum += part[row * parts + c].sum;
+    t.n += part[row * parts + c].n;
   }
   return t;
 }
 
-// The pairs that count, the loss (block 0) and the gradient.
-__global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_t items, int64_t chunks,
+// The pairs that count, the loss (block 0) and the gradient. A block's first threads find the slopes of its items, one
+// each, all at once.
+template <bool Vec>
+__global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_t items, int64_t parts, int64_t width,
                                                               const RowSum* __restrict__ part) {
-  __shared__ double slots[8];
-  __shared__ float slope_s;
-  double on = 0., loss = 0.;
+  __shared__ double slots[16];
+  __shared__ float slope[kLossThreads];
+  double v[2] = {0., 0.};
   for (int64_t p = threadIdx.x; p < a.P; p += kLossThreads) {
-    const RowSum r0 = row_total(part, p, chunks), r1 = row_total(part, a.P + p, chunks);
-    on += r0.n > 0 && r1.n > 0 ? 1. : 0.;
+    const RowSum r0 = row_total(part, p, parts), r1 = row_total(part, a.P + p, parts);
+    v[0] += r0.n > 0 && r1.n > 0 ? 1. : 0.;
     if (blockIdx.x == 0) {
-      loss += pair_of(a, r0.sum, r1.sum, r0.n, r1.n).loss;
+      v[1] += pair_of(a, r0.sum, r1.sum, r0.n, r1.n).loss;
       a.rewards[p] = (float)(a.beta * r0.sum);
       a.rewards[a.P + p] = (float)(a.beta * r1.sum);
     }
   }
-  const double pairs = fmax(1., block_sum(on, slots));
-  if (blockIdx.x == 0) {
-    loss = block_sum(loss, slots);
-    if (threadIdx.x == 0) a.loss[0] = (float)(loss / pairs);
-  }
+  block_sum(v, slots);
+  const double pairs = fmax(1., v[0]);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.loss[0] = (float)(v[1] / pairs);
   if (!a.grad) return;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t row = it / chunks, t0 = (it % chunks) * kLossChunk;
-    const int64_t base = row * a.L + t0, left = a.L - t0;
-    uint8_t m[kLossPer];
-#pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      m[j] = t < left ? a.mask[base + t] : 0;
-    }
+  for (int64_t it0 = blockIdx.x; it0 < items; it0 += (int64_t)gridDim.x * kLossThreads) {
+    const int64_t mine = it0 + (int64_t)threadIdx.x * gridDim.x;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      const int64_t p = row % a.P;
-      const RowSum r0 = row_total(part, p, chunks), r1 = row_total(part, a.P + p, chunks);
+    if (mine < items) {
+      const int64_t row = mine / parts, p = row % a.P;
+      const RowSum r0 = row_total(part, p, parts), r1 = row_total(part, a.P + p, parts);
       const Pair q = pair_of(a, r0.sum, r1.sum, r0.n, r1.n);
-      slope_s = (float)((row < a.P ? q.slope0 : q.slope1) / pairs);
+      slope[threadIdx.x] = (float)((row < a.P ? q.slope0 : q.slope1) / pairs);
     }
     __syncthreads();
-    const float g = slope_s;
-#pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      if (t < left) a.grad[base + t] = m[j] ? g : 0.f;
+    for (int k = 0; k < kLossThreads; ++k) {
+      const int64_t it = it0 + (int64_t)k * gridDim.x;
+      if (it >= items) break;
+      const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
+      const float s = slope[k];
+#pragma unroll 4
+      for (int64_t t = it % parts * width; t < t1; t += kLossChunk) {
+        const uint32_t m = load_mask<Vec>(a.mask + base + t, chunk_left(t1, t));
+        const float d[4] = {m & 1 ? s : 0.f, m & 2 ? s : 0.f, m & 4 ? s : 0.f, m & 8 ? s : 0.f};
+        store4<Vec>(a.grad + base + t, d, chunk_left(t1, t));
+      }
     }
   }
 }
@@ -220,14 +261,14 @@ struct PolicyArgs {
   const float *logp, *old, *ref, *adv;   // (B, L); ref may be null; adv (B, L) or (B)
   const uint8_t* mask;
   int32_t adv_per_token, per_sequence;
-  double log_low, log_high;              // log(1 - clip_low), log(1 + clip_high)
+  float log_low, log_high;               // log(1 - clip_low) rounded up, log(1 + clip_high) rounded down: a float
+                                         // is beyond the rounded bound exactly when it is beyond the bound
   float low, high, kl;                   // 1 - clip_low, 1 + clip_high, KL coefficient
   float *loss, *grad, *stats;            // scalar, (B, L) or null, (2): mean KL estimate, share of clipped tokens
 };
 
-struct TokenSum {
-  double loss, kl;
-  int64_t n, cut;
+struct BlockSum {                        // of one block's tokens
+  double loss, kl, cut;
 };
 
 struct Token {
@@ -235,31 +276,32 @@ struct Token {
   bool cut;
 };
 
-// exp(q) - 1 - q without the cancellation near 0 (Taylor's series below 1/4: its next term is under 4e-7 of the sum).
-__device__ __forceinline__ float expm1_minus(float q) {
-  if (fabsf(q) < 0.25f)
-    return q * q * (0.5f + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720)))));
-  return expm1f(q) - q;
+// x held to [-20, 20], a NaN staying one.
+__device__ __forceinline__ float held20(float x) {
+  float y;
+  asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f41A00000;\n\tmax.NaN.f32 %0, t, 0fC1A00000;\n\t}" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One token of the loss: the ratio's bounds are compared in the log domain, where the log ratio is exact or nearly so,
-// against fp64 bounds: which side a token falls on does not hang on expf's last bit.
+// One token of the loss. The ratio's bounds are compared in the log domain, where the log ratio is exact or nearly so:
+// which side a token falls on does not hang on expf's last bit. exp(q) - 1 - q and exp(q) - 1 come from Taylor's series
+// below 1/4 (its next term is under 4e-7 of the sum), where the differences would cancel.
+template <bool Ref>
 __device__ __forceinline__ Token token_of(const PolicyArgs& a, float lp, float old, float rf, float adv) {
-  Token t{0.f, 0.f, 0.f, false};
-  const float d = lp - old;
-  const bool held = d > 20.f || d < -20.f;
-  const float lr = d > 20.f ? 20.f : d < -20.f ? -20.f : d;
-  t.cut = (adv > 0.f && (double)lr > a.log_high) || (adv < 0.f && (double)lr < a.log_low);
-  const float r = expf(lr);
-  t.loss = t.cut ? -(adv > 0.f ? a.high : a.low) * adv : -r * adv;
-  t.slope = t.cut || held ? 0.f : -r * adv;
-  if (a.ref) {
-    const float dq = rf - lp;
-    const bool qheld = dq > 20.f || dq < -20.f;
-    const float q = dq > 20.f ? 20.f : dq < -20.f ? -20.f : dq;
-    t.kl = expm1_minus(q);
-    t.loss += a.kl * t.kl;
-    if (!qheld) t.slope -= a.kl * expm1f(q);
+  Token t;
+  const float d = lp - old, lr = held20(d);
+  t.cut = adv > 0.f ? lr > a.log_high : adv < 0.f && lr < a.log_low;
+  const float r = t.cut ? (adv > 0.f ? a.high : a.low) : expf(lr);
+  t.loss = -r * adv;
+  t.slope = t.cut || fabsf(d) > 20.f ? 0.f : t.loss;
+  t.kl = 0.f;
+  if (Ref) {
+    const float dq = rf - lp, q = held20(dq);
+    const bool near = fabsf(q) < 0.25f;
+    const float e = expf(q) - 1.f;
+    t.kl = near ? q * q * (0.5f + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720))))) : e - q;
+    t.loss = fmaf(a.kl, t.kl, t.loss);
+    t.slope = fabsf(dq) > 20.f ? t.slope : fmaf(-a.kl, near ? q + t.kl : e, t.slope);
   }
   return t;
 }
@@ -272,11 +314,11 @@ __device__ __forceinline__ void policy_results(const PolicyArgs& a, double loss,
   a.stats[1] = (float)(cut / total);
 }
 
-__global__ void __launch_bounds__(1024) k_policy_small(PolicyArgs a) {
+template <bool Ref> __global__ void __launch_bounds__(1024) k_policy_small(PolicyArgs a) {
   __shared__ int cnt[kSmallRows];
-  __shared__ double slots[32];
+  __shared__ double slots[96];
   const int rows = (int)a.B, L = (int)a.L, lane = threadIdx.x & 31;
-  double n = 0., full = 0.;
+  double n[2] = {0., 0.};
   for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
     int c = 0;
 #pragma unroll 4
@@ -284,137 +326,170 @@ __global__ void __launch_bounds__(1024) k_policy_small(PolicyArgs a) {
     c = warp_sum_i(c);
     if (lane == 0) {
       cnt[r] = c;
-      n += c;
-      full += c > 0 ? 1. : 0.;
+      n[0] += c;
+      n[1] += c > 0 ? 1. : 0.;
     }
   }
-  n = block_sum(n, slots);
-  full = block_sum(full, slots);
-  const double total = fmax(1., n), seqs = fmax(1., full);
-  double loss = 0., kl = 0., cut = 0.;
+  block_sum(n, slots);
+  const double total = fmax(1., n[0]), seqs = fmax(1., n[1]);
+  double v[3] = {0., 0., 0.};
   const int all = rows * L;
+#pragma unroll 2
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const int row = i / L;
+    const bool on = a.mask[i];
+    const float lp = a.logp[i], old = a.old[i], rf = Ref ? a.ref[i] : 0.f, adv = a.adv[a.adv_per_token ? i : row];
     float g = 0.f;
-    if (a.mask[i]) {
-      const Token t = token_of(a, a.logp[i], a.old[i], a.ref ? a.ref[i] : 0.f, a.adv[a.adv_per_token ? i : row]);
+    if (on) {
+      const Token t = token_of<Ref>(a, lp, old, rf, adv);
       const double w = a.per_sequence ? 1. / cnt[row] : 1.;
-      loss += w * (double)t.loss;
-      kl += (double)t.kl;
-      cut += t.cut ? 1. : 0.;
+      v[0] += w * (double)t.loss;
+      v[1] += (double)t.kl;
+      v[2] += t.cut ? 1. : 0.;
       g = (float)((double)t.slope * w / (a.per_sequence ? seqs : total));
     }
     if (a.grad) a.grad[i] = g;
   }
-  loss = block_sum(loss, slots);
-  kl = block_sum(kl, slots);
-  cut = block_sum(cut, slots);
-  if (threadIdx.x == 0) policy_results(a, loss, kl, n, cut, full);
+  block_sum(v, slots);
+  if (threadIdx.x == 0) policy_results(a, v[0], v[1], n[0], v[2], n[1]);
 }
 
-// Tokens of each chunk of each row; block 0 clears the ticket that the next launch's blocks take.
-__global__ void __launch_bounds__(kLossThreads) k_policy_counts(PolicyArgs a, int64_t items, int64_t chunks,
+// Tokens of each part of each row; block 0 clears the ticket that the next launch's blocks take.
+template <bool Vec>
+__global__ void __launch_bounds__(kLossThreads) k_policy_counts(PolicyArgs a, int64_t parts, int64_t width,
                                                                 int* __restrict__ counts, unsigned* ticket) {
-  __shared__ int slots[8];
+  __shared__ double slots[8];
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t row = it / chunks, t0 = (it % chunks) * kLossChunk;
-    const int64_t base = row * a.L + t0, left = a.L - t0;
+  for (int64_t it = blockIdx.x; it < a.B * parts; it += gridDim.x) {
+    const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
     int n = 0;
-#pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      n += t < left ? a.mask[base + t] != 0 : 0;
-    }
-    n = block_sum(n, slots);
-    if (threadIdx.x == 0) counts[it] = n;
+#pragma unroll 4
+    for (int64_t t = it % parts * width; t < t1; t += kLossChunk)
+      n += __popc(load_mask<Vec>(a.mask + base + t, chunk_left(t1, t)));
+    double v[1] = {(double)n};
+    block_sum(v, slots);
+    if (threadIdx.x == 0) counts[it] = (int)v[0];
   }
 }
 
-// The tokens, the gradient and each item's sums; the block that finishes last adds the sums up in index order.
-__global__ void __launch_bounds__(kLossThreads) k_policy_main(PolicyArgs a, int64_t items, int64_t chunks,
-                                                              const int* __restrict__ counts, TokenSum* part,
-                                                              unsigned* ticket) {
-  __shared__ double slots[8];
+__device__ __forceinline__ int row_count(const int* counts, int64_t row, int64_t parts) {
+  int c = 0;
+  for (int64_t k = 0; k < parts; ++k) c += counts[row * parts + k];
+  return c;
+}
+
+// The tokens, the gradient and each block's sums, chunks dealt out in turn (a row's prompt and padding cost little); the
+// block that finishes last adds the sums up in index order.
+template <bool Vec, bool Ref>
+__global__ void __launch_bounds__(kLossThreads, kLossBlocks)
+k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* __restrict__ counts, BlockSum* part,
+              unsigned* ticket) {
+  __shared__ double slots[24];
   __shared__ bool last;
-  double n = 0., full = 0.;
+  double n[2] = {0., 0.};
   for (int64_t b = threadIdx.x; b < a.B; b += kLossThreads) {
-    int64_t c = 0;
-    for (int64_t k = 0; k < chunks; ++k) c += counts[b * chunks + k];
-    n += (double)c;
-    full += c > 0 ? 1. : 0.;
+    const int c = row_count(counts, b, parts);
+    n[0] += (double)c;
+    n[1] += c > 0 ? 1. : 0.;
   }
-  n = block_sum(n, slots);
-  full = block_sum(full, slots);
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t row = it / chunks, t0 = (it % chunks) * kLossChunk;
-    const int64_t base = row * a.L + t0, left = a.L - t0;
-    double w = 1. / fmax(1., n);
-    if (a.per_sequence) {
-      int64_t c = 0;
-      for (int64_t k = 0; k < chunks; ++k) c += counts[row * chunks + k];
-      w = 1. / (fmax(1., (double)c) * fmax(1., full));
+  block_sum(n, slots);
+  const float over = (float)(1. / (a.per_sequence ? fmax(1., n[1]) : fmax(1., n[0])));
+  double v[3] = {0., 0., 0.};
+  int cut = 0;
+  const int64_t step_r = gridDim.x / chunks, step_c = gridDim.x % chunks, stride_c = step_c * kLossChunk;
+  int64_t row = blockIdx.x / chunks, t = blockIdx.x % chunks * kLossChunk;
+  // the mask comes an item ahead: a warp whose tokens are all outside it reads nothing else
+  uint32_t next = row < a.B ? load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t)) : 0;
+  while (row < a.B) {
+    float share = 1.f, row_adv = 0.f;
+    if (a.per_sequence) share = 1.f / (float)max(1, row_count(counts, row, parts));
+    if (!a.adv_per_token) row_adv = a.adv[row];
+    const float w = share * over;
+    const int64_t at = row * a.L + t;
+    const int left = chunk_left(a.L, t);
+    const uint32_t m = next;
+    t += stride_c;
+    row += step_r;
+    if (t >= chunks * kLossChunk) {
+      t -= chunks * kLossChunk;
+      ++row;
     }
-    const float gw = (float)w;
-    const float row_adv = a.adv_per_token ? 0.f : a.adv[row];
-    float lp[kLossPer], old[kLossPer], rf[kLossPer], adv[kLossPer];
-    uint8_t m[kLossPer];
-#pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      const bool in = t < left;
-      m[j] = in ? a.mask[base + t] : 0;
-      lp[j] = in ? __ldg(a.logp + base + t) : 0.f;
-      old[j] = in ? __ldg(a.old + base + t) : 0.f;
-      rf[j] = in && a.ref ? __ldg(a.ref + base + t) : 0.f;
-      adv[j] = in && a.adv_per_token ? __ldg(a.adv + base + t) : row_adv;
+    float lp[4], old[4], rf[4] = {0.f, 0.f, 0.f, 0.f}, adv[4] = {row_adv, row_adv, row_adv, row_adv};
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool any = __any_sync(0xffffffffu, m);
+    if (any) {
+      load4<Vec>(lp, a.logp + at, left);
+      load4<Vec>(old, a.old + at, left);
+      if (Ref) load4<Vec>(rf, a.ref + at, left);
+      if (a.adv_per_token) load4<Vec>(adv, a.adv + at, left);
     }
-    double loss = 0., kl = 0.;
-    int cut = 0, cn = 0;
+    if (row < a.B) next = load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t));
+    if (any) {
+      float loss = 0.f, kl = 0.f;
 #pragma unroll
-    for (int j = 0; j < kLossPer; ++j) {
-      const int64_t t = j * kLossThreads + threadIdx.x;
-      float g = 0.f;
-      if (m[j]) {
-        const Token k = token_of(a, lp[j], old[j], rf[j], adv[j]);
-        loss += (double)k.loss;
-        kl += (double)k.kl;
+      for (int j = 0; j < 4; ++j) {                // a token outside the mask: all zeros, whose loss and slope are zero
+        const bool on = m >> j & 1;
+        const Token k = token_of<Ref>(a, on ? lp[j] : 0.f, on ? old[j] : 0.f, on ? rf[j] : 0.f, on ? adv[j] : 0.f);
+        loss += k.loss;
+        kl += k.kl;
         cut += k.cut;
-        ++cn;
-        g = k.slope * gw;
+        d[j] = k.slope * w;
       }
-      if (a.grad && t < left) a.grad[base + t] = g;
+      v[0] += (double)(share * loss);              // 4 terms in fp32, then fp64
+      v[1] += (double)kl;
     }
-    loss = block_sum(loss, slots);
-    kl = block_sum(kl, slots);
-    const double tc = block_sum((double)cut, slots);
-    const double tn = block_sum((double)cn, slots);
-    if (threadIdx.x == 0) part[it] = TokenSum{a.per_sequence ? loss * w * fmax(1., full) : loss, kl, (int64_t)tn, (int64_t)tc};
+    if (a.grad) store4<Vec>(a.grad + at, d, left);
   }
+  v[2] = (double)cut;
+  block_sum(v, slots);
   if (threadIdx.x == 0) {
+    part[blockIdx.x] = BlockSum{v[0], v[1], v[2]};
     __threadfence();
     last = atomicAdd(ticket, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double loss = 0., kl = 0., cut = 0.;
-  for (int64_t it = threadIdx.x; it < items; it += kLossThreads) {
-    const TokenSum t = part[it];
-    loss += t.loss;
-    kl += t.kl;
-    cut += (double)t.cut;
+  v[0] = v[1] = v[2] = 0.;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += kLossThreads) {
+    const volatile BlockSum* t = part + b;
+    v[0] += t->loss;
+    v[1] += t->kl;
+    v[2] += t->cut;
   }
-  loss = block_sum(loss, slots);
-  kl = block_sum(kl, slots);
-  cut = block_sum(cut, slots);
-  if (threadIdx.x == 0) policy_results(a, loss, kl, n, cut, full);
+  block_sum(v, slots);
+  if (threadIdx.x == 0) policy_results(a, v[0], v[1], n[0], v[2], n[1]);
 }
 
 int64_t loss_chunks(int64_t L) { return (L + kLossChunk - 1) / kLossChunk; }
 
-int loss_grid(int64_t items) {
-  return (int)(items < 148 * 8 ? items : 148 * 8);
+constexpr int kLossGrid = 148 * 8;
+
+// As many blocks as the SMs hold at a time: none waits for another to end.
+int loss_grid(int64_t items, int per_sm = 8) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)148 * per_sm));
+}
+
+// Rows of a multiple of 4 tokens on 16-byte boundaries (the mask's on 4) are read four tokens at a time.
+bool vec_ok(int64_t L, std::initializer_list<const void*> fs, const void* mask) {
+  if (L % 4 || (uintptr_t)mask % 4) return false;
+  for (const void* f : fs)
+    if ((uintptr_t)f % 16) return false;
+  return true;
+}
+
+float rounded(double x, bool up) {
+  const float f = (float)x;
+  return up ? ((double)f < x ? nextafterf(f, INFINITY) : f) : ((double)f > x ? nextafterf(f, -INFINITY) : f);
+}
+
+// Parts of a row that blocks sum apart: as many as fill the GPU, each of a chunk at least. width: tokens of a part.
+int64_t row_parts(int64_t rows, int64_t L) {
+  return std::max<int64_t>(1, std::min<int64_t>(kLossGrid / std::max<int64_t>(1, rows), loss_chunks(L)));
+}
+int64_t part_width(int64_t rows, int64_t L) {
+  const int64_t parts = row_parts(rows, L);
+  return (loss_chunks(L) + parts - 1) / parts * kLossChunk;
 }
 
 bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L <= 16384; }
@@ -426,7 +501,7 @@ extern "C" {
 
 size_t asrn_preference_workspace_bytes(int64_t P, int64_t L) {
   if (P < 0 || L < 0 || asrn::small_loss(2 * P, L)) return 0;
-  return asrn::align_up((size_t)(2 * P * asrn::loss_chunks(L)) * sizeof(asrn::RowSum) + 1);
+  return asrn::align_up((size_t)(2 * P * asrn::row_parts(2 * P, L)) * sizeof(asrn::RowSum) + 1);
 }
 
 int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* ref_logp, const uint8_t* mask,
@@ -447,18 +522,23 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   }
   if (!workspace || workspace_bytes < asrn_preference_workspace_bytes(P, L) || (uintptr_t)workspace % 16)
     return ASRN_ERR_WORKSPACE;
-  const int64_t chunks = loss_chunks(L), items = 2 * P * chunks;
+  const int64_t parts = row_parts(2 * P, L), width = part_width(2 * P, L), items = 2 * P * parts;
   RowSum* part = reinterpret_cast<RowSum*>(workspace);
-  const int grid = items > 0 ? loss_grid(items) : 1;
-  k_pref_sums<<<grid, kLossThreads, 0, s>>>(a, items, chunks, part);
-  k_pref_finish<<<grid, kLossThreads, 0, s>>>(a, items, chunks, part);
+  const int grid = loss_grid(items);
+  if (vec_ok(L, {logp, ref_logp, grad}, mask)) {
+    k_pref_sums<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+    k_pref_finish<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+  } else {
+    k_pref_sums<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+    k_pref_finish<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+  }
   return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 
 size_t asrn_policy_workspace_bytes(int64_t B, int64_t L) {
   if (B < 0 || L < 0 || asrn::small_loss(B, L)) return 0;
-  const size_t items = (size_t)(B * asrn::loss_chunks(L));
-  return 256 + asrn::align_up(items * sizeof(asrn::TokenSum)) + asrn::align_up(items * sizeof(int));
+  return 256 + asrn::align_up(asrn::kLossGrid * sizeof(asrn::BlockSum)) +
+         asrn::align_up((size_t)(B * asrn::row_parts(B, L)) * sizeof(int) + 1);
 }
 
 int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_logp, const float* ref_logp,
@@ -473,22 +553,30 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   if (B * L > 0 && (!logp || !old_logp || !advantages || !mask)) return ASRN_ERR_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const PolicyArgs a{B, L, logp, old_logp, ref_logp, advantages, mask, adv_per_token != 0, per_sequence != 0,
-                     log1p(-clip_low), log1p(clip_high), (float)(1. - clip_low), (float)(1. + clip_high), (float)kl,
+                     rounded(log1p(-clip_low), true), rounded(log1p(clip_high), false), (float)(1. - clip_low), (float)(1. + clip_high), (float)kl,
                      loss, grad, stats};
   if (small_loss(B, L)) {
-    k_policy_small<<<1, 1024, 0, s>>>(a);
+    if (ref_logp) k_policy_small<true><<<1, 1024, 0, s>>>(a);
+    else k_policy_small<false><<<1, 1024, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
   }
   if (!workspace || workspace_bytes < asrn_policy_workspace_bytes(B, L) || (uintptr_t)workspace % 16)
     return ASRN_ERR_WORKSPACE;
-  const int64_t chunks = loss_chunks(L), items = B * chunks;
   char* base = reinterpret_cast<char*>(workspace);
   unsigned* ticket = reinterpret_cast<unsigned*>(base);
-  TokenSum* part = reinterpret_cast<TokenSum*>(base + 256);
-  int* counts = reinterpret_cast<int*>(base + 256 + align_up((size_t)items * sizeof(TokenSum)));
-  const int grid = items > 0 ? loss_grid(items) : 1;
-  k_policy_counts<<<grid, kLossThreads, 0, s>>>(a, items, chunks, counts, ticket);
-  k_policy_main<<<grid, kLossThreads, 0, s>>>(a, items, chunks, counts, part, ticket);
+  BlockSum* part = reinterpret_cast<BlockSum*>(base + 256);
+  int* counts = reinterpret_cast<int*>(base + 256 + align_up(kLossGrid * sizeof(BlockSum)));
+  const int64_t parts = row_parts(B, L), width = part_width(B, L), chunks = loss_chunks(L);
+  const int grid = loss_grid(B * chunks, kLossBlocks), cgrid = loss_grid(B * parts);
+  if (vec_ok(L, {logp, old_logp, ref_logp, adv_per_token ? advantages : nullptr, grad}, mask)) {
+    k_policy_counts<true><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
+    if (ref_logp) k_policy_main<true, true><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
+    else k_policy_main<true, false><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
+  } else {
+    k_policy_counts<false><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
+    if (ref_logp) k_policy_main<false, true><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
+    else k_policy_main<false, false><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
+  }
   return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 
