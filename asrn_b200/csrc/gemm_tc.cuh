@@ -3,13 +3,20 @@
 //
 //   warp 0        streams both operands through a ring of 64-deep K blocks by TMA (128-byte swizzle)
 //   warp 1        issues tcgen05.mma into one of two 256-column TMEM accumulators
-//   warps 2-9     drain the other accumulator: thread = row, two warps per 32-lane quadrant, each half of the columns
+//   warps 2-9     drain the other accumulator: thread = row, two warps per 32-lane quadrant, each half of the columns,
+//                 32 at a time; bf16 results leave by TMA through two 2 KB pieces per warp (direct stores, a row's 16
+//                 bytes per lane, touch 32 half-written sectors each)
 //
 // Either operand may lie in memory with its K dimension innermost (K-major) or with its M / N dimension innermost
 // (MN-major), so the products of a backward pass read the forward pass's tensors as they are. Pairs of blocks
 // (CG = 2) work on one 256 x 256 tile: each block stages its 128 rows of A and its 128 of B's 256 rows, half of what a
 // block working alone has to stage per multiplication, and the pair's first block issues the MMAs for both.
 // Rows (M) and depth (K) may be cut by counts that only the device knows.
+//
+// Products with few tiles or a last round that leaves many SMs idle are walked in equal shares instead (`shares`): the
+// clusters stand side by side in groups, one for each tile of N, and each group takes the same number of K blocks of the
+// M tiles laid end to end, so that the blocks that read the same part of A do so together. A share's pieces of tiles go
+// to fp32 slots that k_join adds up in order.
 //
 // Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, frees its TMEM and
 // ends.
@@ -29,7 +36,11 @@ constexpr int kBytesA = kBM * 128;                       // one block's share of
 template <int CG> constexpr int bytes_b() { return kBN / CG * 128; }
 template <int CG> constexpr int stage_bytes() { return kBytesA + bytes_b<CG>(); }
 template <int CG> constexpr int stages() { return CG == 1 ? 4 : 6; }
-template <int CG> constexpr size_t smem_bytes() { return 1024 + (size_t)stages<CG>() * stage_bytes<CG>() + 256; }
+constexpr int kPiece = 32 * 64;                          // 32 rows x 32 bf16 columns, 64-byte swizzle
+constexpr int kPieces = 2 * kEpiWarps * kPiece;
+template <int CG> constexpr size_t smem_bytes() {
+  return 1024 + (size_t)stages<CG>() * stage_bytes<CG>() + kPieces + 256;
+}
 
 struct Shape {
   int M, N, K;             // bounds known to the host
@@ -37,13 +48,14 @@ struct Shape {
   int m_off;
   const int* k_dev;        // the same for K
   int k_off;
-  int splits;              // parts of K, each with an output of its own
-  int group;               // M tiles walked before the next N tile
+  int shares;              // groups of clusters that walk equal shares, or 0: whole tiles
+  int group;               // whole tiles: M tiles walked before the next N tile
   int* status;
 };
 
 struct Tile {
-  int m, n, sp;
+  int m, n, k0, k1;        // K blocks [k0, k1)
+  int slot;                // of the fp32 pieces
 };
 
 ASRN_DEV int cut(int most, const int* dev, int off) {
@@ -52,17 +64,57 @@ ASRN_DEV int cut(int most, const int* dev, int off) {
   return n < 0 ? 0 : n < most ? n : most;
 }
 
-ASRN_DEV Tile tile_at(int t, int mt, int nt, int group) {
-  Tile r;
-  r.sp = t / (mt * nt);
-  const int u = t - r.sp * mt * nt;
-  const int first = u / (group * nt) * group;
-  const int rows = min(group, mt - first);
-  const int v = u - first * nt;
-  r.m = first + v % rows;
-  r.n = v / rows;
-  return r;
+// Shares of a walk over mt x kblocks blocks where `most` groups stand: 8 blocks each at least, but one per M tile. From
+// the counts that the device knows: rows left out change no sum's order.
+__host__ ASRN_DEV int shares_of(int64_t mt, int64_t kblocks, int most) {
+  const int64_t n = mt * kblocks / 8 > mt ? mt * kblocks / 8 : mt;
+  return n < 1 ? 1 : n < most ? (int)n : most;
 }
+// The first of `shares` shares of mt x kblocks K blocks that holds block u, and a share's first block.
+__host__ ASRN_DEV int64_t share_of(int64_t u, int64_t all, int64_t shares) { return ((u + 1) * shares - 1) / all; }
+__host__ ASRN_DEV int64_t share_begin(int64_t g, int64_t all, int64_t shares) { return all * g / shares; }
+
+// A cluster's tiles, the same sequence for each of its warps.
+struct Walk {
+  int mt, nt, kblocks, group, at, step, share;
+  int64_t u, end;
+  ASRN_DEV Walk(const Shape& s, int M, int K, int cg, int cluster, int clusters)
+      : mt((M + kBM * cg - 1) / (kBM * cg)), nt((s.N + kBN - 1) / kBN), kblocks((K + kBK - 1) / kBK), group(s.group),
+        at(cluster), step(clusters), share(-1), u(0), end(0) {
+    if (s.shares) {
+      share = cluster / nt;
+      at = cluster % nt;
+      const int64_t all = (int64_t)mt * kblocks;
+      const int shares = shares_of(mt, kblocks, s.shares);
+      if (share < shares) {
+        u = share_begin(share, all, shares);
+        end = share_begin(share + 1, all, shares);
+      }
+    }
+  }
+  ASRN_DEV bool next(Tile& t) {
+    if (share >= 0) {
+      if (u >= end) return false;
+      t.m = (int)(u / kblocks);
+      t.n = at;
+      t.k0 = (int)(u - (int64_t)t.m * kblocks);
+      t.k1 = (int)min((int64_t)kblocks, t.k0 + (end - u));
+      t.slot = (share + t.m) * nt + at;
+      u += t.k1 - t.k0;
+      return true;
+    }
+    if (at >= mt * nt) return false;
+    const int first = at / (group * nt) * group;
+    const int rows = min(group, mt - first), v = at - first * nt;
+    t.m = first + v % rows;
+    t.n = v / rows;
+    t.k0 = 0;
+    t.k1 = kblocks;
+    t.slot = 0;
+    at += step;
+    return true;
+  }
+};
 
 ASRN_DEV uint32_t cluster_rank() {
   uint32_t r;
@@ -132,11 +184,73 @@ template <int CG> ASRN_DEV void dealloc(uint32_t taddr) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(2 * kBN) : "memory");
 }
 
-// Epi: struct with a Params type, a constructor (Params, row, rows, column, tile's n index, split, warp half) and
-// chunk(float v[32], column) for four chunks of 32 columns, then finish().
+// Two fp32 values in one register pair: one instruction for both.
+struct F2 {
+  uint64_t v;
+  ASRN_DEV F2() {}
+  ASRN_DEV F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  ASRN_DEV explicit F2(float a) : F2(a, a) {}
+  ASRN_DEV void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+ASRN_DEV F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+ASRN_DEV F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+ASRN_DEV F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+ASRN_DEV float exp2_fast(float x) {                      // 2^x, 2 units in the last place
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+ASRN_DEV uint4 pack8(const float* v) {
+  return make_uint4(umma::pack_bf16x2(v[0], v[1]), umma::pack_bf16x2(v[2], v[3]), umma::pack_bf16x2(v[4], v[5]),
+                    umma::pack_bf16x2(v[6], v[7]));
+}
+
+// A warp's way out for 32 rows x 32 columns of bf16: written to one of two pieces of shared memory, from there by TMA.
+// A piece is written again once the copy before last has read it.
+struct Out {
+  uint8_t* piece;                                        // the warp's two
+  int lane, turn;
+  ASRN_DEV void put(const CUtensorMap* map, const float* v, int column, int first_row) {
+    uint8_t* at = piece + (turn & 1) * kPiece;
+    turn ^= 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = pack8(v + 8 * i);
+    umma::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
+                   "r"(column), "r"(first_row), "r"(umma::smem_u32(at))
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  ASRN_DEV void drain() {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+};
+
+// Epi: struct with a Params type, a constructor (Params, row, rows, shape, tile, half of the columns) and chunk(v[32],
+// column, Out, map_o, map_p), called by whole warps for the tile's chunks of 32 columns, then finish().
 template <int CG, bool AMn, bool BMn, class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
-k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Shape s,
+k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+       const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_p, const Shape s,
        const typename Epi::Params p) {
   using namespace umma;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -145,7 +259,8 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   constexpr int kS = stages<CG>(), kStageB = bytes_b<CG>();
   uint8_t* sA = sm;
   uint8_t* sB = sm + kS * kBytesA;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sB + kS * kStageB);
+  uint8_t* sO = sB + kS * kStageB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sO + kPieces);
   uint64_t* empty = full + kS;
   uint64_t* tfull = empty + kS;
   uint64_t* tempty = tfull + 2;
@@ -174,20 +289,16 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   const uint32_t tmem = *tmem_s;
 
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
-  const int mt = (M + kBM * CG - 1) / (kBM * CG), nt = (s.N + kBN - 1) / kBN;
-  const int kblocks = (K + kBK - 1) / kBK;
-  const int tiles = mt * nt * s.splits;
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  Walk walk(s, M, K, CG, blockIdx.x / CG, gridDim.x / CG);
+  Tile u;
 
   if (wid == 0) {
     if (lane == 0) {                                    // operand producer
       int it = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        const Tile u = tile_at(t, mt, nt, s.group);
+      while (ok && walk.next(u)) {
         const int m0 = (u.m * CG + (int)rank) * kBM, n0 = u.n * kBN + (int)rank * (kBN / CG);
-        const int k0 = (int)((int64_t)kblocks * u.sp / s.splits), k1 = (int)((int64_t)kblocks * (u.sp + 1) / s.splits);
-        for (int kb = k0; kb < k1; ++kb, ++it) {
+        for (int kb = u.k0; kb < u.k1; ++kb, ++it) {
           const int st = it % kS;
           if (it >= kS && !(ok = mbar_wait(empty + st, ((it / kS) - 1) & 1, s.status))) break;
           if (rank == 0) mbar_expect_tx(full + st, (uint32_t)(CG * stage_bytes<CG>()));
@@ -214,13 +325,11 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       constexpr uint32_t idesc = idesc_bf16(kBM * CG, kBN) | (AMn ? 1u << 15 : 0u) | (BMn ? 1u << 16 : 0u);
       int it = 0, jt = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step, ++jt) {
-        const Tile u = tile_at(t, mt, nt, s.group);
-        const int k0 = (int)((int64_t)kblocks * u.sp / s.splits), k1 = (int)((int64_t)kblocks * (u.sp + 1) / s.splits);
+      for (; ok && walk.next(u); ++jt) {
         const int b = jt & 1;
         if (jt >= 2 && !(ok = mbar_wait(tempty + b, ((jt >> 1) - 1) & 1, s.status))) break;
         tc_fence_after();
-        for (int kb = k0; kb < k1; ++kb, ++it) {
+        for (int kb = u.k0; kb < u.k1; ++kb, ++it) {
           const int st = it % kS;
           if (!(ok = mbar_wait(full + st, (it / kS) & 1, s.status))) break;
           tc_fence_after();
@@ -229,7 +338,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           for (int q = 0; q < kBK / 16; ++q)
             mma<CG>(tmem + (uint32_t)(b * kBN), AMn ? desc_mn_sw128(a0 + q * 2048, 8192) : desc_sw128(a0 + q * 32),
                     BMn ? desc_mn_sw128(b0 + q * 2048, 8192) : desc_sw128(b0 + q * 32), idesc,
-                    (kb > k0 || q > 0) ? 1u : 0u);
+                    (kb > u.k0 || q > 0) ? 1u : 0u);
           commit<CG>(empty + st);
         }
         commit<CG>(tfull + b);
@@ -237,16 +346,15 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     }
   } else {                                              // epilogue
     const int q4 = wid & 3, half = (wid - 2) >> 2;
+    Out out{sO + (wid - 2) * 2 * kPiece, lane, 0};
     const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(half * (kBN / 2));
     int jt = 0;
-    for (int t = first; t < tiles; t += step, ++jt) {
-      const Tile u = tile_at(t, mt, nt, s.group);
-      const bool none = (int64_t)kblocks * u.sp / s.splits == (int64_t)kblocks * (u.sp + 1) / s.splits;
+    for (; walk.next(u); ++jt) {
       const int b = jt & 1;
       if (!mbar_wait(tfull + b, (jt >> 1) & 1, s.status)) break;
       tc_fence_after();
       const int c0 = u.n * kBN + half * (kBN / 2);
-      Epi e(p, (u.m * CG + (int)rank) * kBM + q4 * 32 + lane, M, c0, s, u, half);
+      Epi e(p, (u.m * CG + (int)rank) * kBM + q4 * 32 + lane, M, s, u, half);
 #pragma unroll 1
       for (int ch = 0; ch < kBN / 64; ++ch) {
         float v[32];
@@ -261,14 +369,15 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
               asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(peer_u32(tempty + b, 0)) : "memory");
           }
         }
-        if (none) {
+        if (u.k0 == u.k1) {                             // no depth at all
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
-        e.chunk(v, c0 + ch * 32);
+        e.chunk(v, c0 + ch * 32, out, &map_o, &map_p);
       }
       e.finish();
     }
+    out.drain();
   }
   tc_fence_before();
   __syncthreads();
@@ -281,65 +390,118 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
 
 // ---- epilogues that only store -----------------------------------------------------------------------------------------
 
-ASRN_DEV uint4 pack8(const float* v) {
-  return make_uint4(umma::pack_bf16x2(v[0], v[1]), umma::pack_bf16x2(v[2], v[3]), umma::pack_bf16x2(v[4], v[5]),
-                    umma::pack_bf16x2(v[6], v[7]));
+// v += bias[0 .. min(32, n)), n a multiple of 8.
+ASRN_DEV void add_bias(float* v, const __nv_bfloat16* bias, int n) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (i < n) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + i));
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[i + 2 * j] += __uint_as_float(w[j] << 16);
+        v[i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
 }
 
-// fp32 sums of one part of K: out[split][row][column] (N a multiple of 8), stored or added to what is there.
-struct StoreF32 {
+// The fp32 sums of a piece of a tile, whole, to its slot: slot[rows of a tile][256].
+struct StorePiece {
   struct Params {
-    float* out;
-    int add;
+    float* slots;
+    int tile_rows;
   };
   float* at;
-  int N;
-  bool on, add;
-  ASRN_DEV StoreF32(const Params& p, int row, int rows, int, const Shape& s, const Tile& u, int)
-      : at(p.out + ((int64_t)u.sp * s.M + row) * s.N), N(s.N), on(row < rows), add(p.add != 0) {}
-  ASRN_DEV void chunk(const float* v, int c) {
-    if (!on) return;
+  ASRN_DEV StorePiece(const Params& p, int row, int, const Shape&, const Tile& u, int half)
+      : at(p.slots + ((int64_t)u.slot * p.tile_rows + row % p.tile_rows) * kBN - u.n * kBN) {}
+  ASRN_DEV void chunk(const float* v, int c, Out&, const CUtensorMap*, const CUtensorMap*) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4)
-      if (c + i < N) {
-        float4* o = reinterpret_cast<float4*>(at + c + i);
-        float4 x = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        if (add) {
-          const float4 y = *o;
-          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-        }
-        *o = x;
-      }
+      *reinterpret_cast<float4*>(at + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   }
   ASRN_DEV void finish() {}
 };
 
-// bf16(sum + bias): out[row][column] (N a multiple of 8).
+// bf16(sum + bias + before): out[row][column] through map_o (N a multiple of 8). before: fp32 (M, N), the sum of what
+// came earlier; or, when `after` is given, the sum goes there in fp32 instead.
 struct StoreBf16 {
   struct Params {
-    __nv_bfloat16* out;
     const __nv_bfloat16* bias;
+    const float* before;
+    float* after;
   };
   const Params& p;
-  __nv_bfloat16* at;
-  int N;
+  int64_t at;
+  int N, first;
   bool on;
-  ASRN_DEV StoreBf16(const Params& pp, int row, int rows, int, const Shape& s, const Tile&, int)
-      : p(pp), at(pp.out + (int64_t)row * s.N), N(s.N), on(row < rows) {}
-  ASRN_DEV void chunk(float* v, int c) {
-    if (!on) return;
+  ASRN_DEV StoreBf16(const Params& pp, int row, int rows, const Shape& s, const Tile&, int)
+      : p(pp), at((int64_t)row * s.N), N(s.N), first(row & ~31), on(row < rows) {}
+  ASRN_DEV void chunk(float* v, int c, Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+    if (c >= N) return;
+    if (p.bias) add_bias(v, p.bias + c, N - c);
+    if (p.before && on) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (c + i < N) {
-        if (p.bias) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i + j] += __bfloat162float(p.bias[c + i + j]);
+      for (int i = 0; i < 32; i += 4)
+        if (c + i < N) {
+          const float4 y = *reinterpret_cast<const float4*>(p.before + at + c + i);
+          v[i] += y.x; v[i + 1] += y.y; v[i + 2] += y.z; v[i + 3] += y.w;
         }
-        *reinterpret_cast<uint4*>(at + c + i) = pack8(v + i);
-      }
+    }
+    if (p.after) {
+      if (on)
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          if (c + i < N) *reinterpret_cast<float4*>(p.after + at + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+      out.put(map_o, v, c, first);
+    }
   }
   ASRN_DEV void finish() {}
 };
+
+// The pieces of each tile added up in order and rounded: out[row_of ? row_of[r] : r][c]. Block = 32 rows x 256 columns of
+// one tile. Positions i < zero_n with pos[i] < 0 get zero rows (whole grid).
+struct JoinArgs {
+  const float* slots;
+  __nv_bfloat16* out;
+  int tile_rows;
+  const int* row_of;
+  const int* pos;
+  int64_t zero_n;
+};
+static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinArgs a) {
+  const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
+  const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN, kblocks = (K + kBK - 1) / kBK;
+  const int per = a.tile_rows / 32;
+  const int64_t all = (int64_t)mt * kblocks;
+  const int tile = blockIdx.x / per, m = tile / nt, n = tile % nt;
+  const int c = n * kBN + (threadIdx.x & 31) * 8;
+  if (m < mt && c < s.N) {
+    int g0 = 0, g1 = -1;
+    if (kblocks) {
+      const int shares = shares_of(mt, kblocks, s.shares);
+      g0 = (int)share_of((int64_t)m * kblocks, all, shares);
+      g1 = (int)share_of((int64_t)(m + 1) * kblocks - 1, all, shares);
+    }
+    for (int k = threadIdx.x >> 5; k < 32; k += 8) {
+      const int in = blockIdx.x % per * 32 + k, r = m * a.tile_rows + in;
+      if (r >= M) break;
+      float v[8] = {};
+      for (int g = g0; g <= g1; ++g) {
+        const float4* q = reinterpret_cast<const float4*>(
+            a.slots + ((int64_t)((g + m) * nt + n) * a.tile_rows + in) * kBN + (c - n * kBN));
+        const float4 x = q[0], y = q[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+      *reinterpret_cast<uint4*>(a.out + (int64_t)(a.row_of ? a.row_of[r] : r) * s.N + c) = pack8(v);
+    }
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.zero_n; i += (int64_t)gridDim.x * 8)
+    if (a.pos[i] < 0)
+      for (int x = (threadIdx.x & 31) * 8; x < s.N; x += 256)
+        *reinterpret_cast<uint4*>(a.out + i * s.N + x) = make_uint4(0, 0, 0, 0);
+}
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
@@ -353,9 +515,8 @@ inline int sm_count() {
   return n;
 }
 
-inline int tiles_of(int64_t M, int64_t N, int cg) {
-  return (int)(((M + kBM * cg - 1) / (kBM * cg)) * ((N + kBN - 1) / kBN));
-}
+inline int64_t tiles_m(int64_t M, int cg) { return (M + kBM * cg - 1) / (kBM * cg); }
+inline int64_t tiles_n(int64_t N) { return (N + kBN - 1) / kBN; }
 
 // A K-major operand (rows, depth) or an MN-major one (depth, rows), rows of `pitch` elements.
 inline bool operand_map(CUtensorMap* map, const void* base, bool mn, int64_t rows, int64_t depth, int64_t pitch,
@@ -372,12 +533,22 @@ inline bool bind_context() {
   return bound;
 }
 
+// Where an epilogue's bf16 rows go: (rows, columns) of `pitch` elements.
+struct Dest {
+  void* base;
+  int64_t rows, columns, pitch;
+};
+
 template <int CG, bool AMn, bool BMn, class Epi>
 int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const Shape& s,
-              const typename Epi::Params& p, cudaStream_t stream) {
-  CUtensorMap ma, mb;
+              const typename Epi::Params& p, const Dest& o, const Dest& q, cudaStream_t stream) {
+  CUtensorMap ma, mb, mo, mq;
   if (!bind_context()) return ASRN_ERR_CUDA;
   if (!operand_map(&ma, A, AMn, s.M, s.K, pitch_a, kBM) || !operand_map(&mb, B, BMn, s.N, s.K, pitch_b, kBN / CG))
+    return ASRN_ERR_CUDA;
+  mo = mq = ma;                                            // not read where there is no destination
+  if ((o.base && !make_tmap_bf16_sw64(&mo, o.base, (uint64_t)o.columns, (uint64_t)o.rows, (uint64_t)o.pitch * 2, 32, 32)) ||
+      (q.base && !make_tmap_bf16_sw64(&mq, q.base, (uint64_t)q.columns, (uint64_t)q.rows, (uint64_t)q.pitch * 2, 32, 32)))
     return ASRN_ERR_CUDA;
   auto kernel = k_gemm<CG, AMn, BMn, Epi>;
   constexpr size_t smem = smem_bytes<CG>();
@@ -389,7 +560,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
       return ASRN_ERR_CUDA;
     if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
   }
-  const int64_t tiles = (int64_t)tiles_of(s.M, s.N, CG) * s.splits;
+  const int64_t tiles = s.shares ? s.shares * tiles_n(s.N) : tiles_m(s.M, CG) * tiles_n(s.N);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, sm_count() / CG) * CG));
   cfg.blockDim = dim3(kThreads);
@@ -401,7 +572,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 1 ? 0 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, s, p) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, mq, s, p) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 
 // Blocks in pairs unless one block's 128 rows hold all of M.
@@ -409,17 +580,35 @@ inline int pair_for(int64_t M) { return M > kBM ? 2 : 1; }
 
 template <bool AMn, bool BMn, class Epi>
 int launch(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const Shape& s,
-           const typename Epi::Params& p, cudaStream_t stream) {
-  return pair_for(s.M) == 2 ? launch_cg<2, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, stream)
-                            : launch_cg<1, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, stream);
+           const typename Epi::Params& p, cudaStream_t stream, const Dest& o = {}, const Dest& q = {}) {
+  return pair_for(s.M) == 2 ? launch_cg<2, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, o, q, stream)
+                            : launch_cg<1, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, o, q, stream);
 }
 
-// Parts of K that give every SM a tile, each of 8 K blocks at least.
-inline int splits_for(int64_t M, int64_t N, int64_t K) {
+// Groups for a walk in shares: as many as the SMs hold and the work fills. shares_for: 0 (whole tiles)
+// unless shares keep at least 5 % more of the SMs busy (their pieces cost a write and a read in fp32).
+inline int groups_for(int64_t M, int64_t N, int64_t K) {
+  return shares_of(tiles_m(M, pair_for(M)), (K + kBK - 1) / kBK,
+                   (int)std::max<int64_t>(1, sm_count() / pair_for(M) / tiles_n(N)));
+}
+inline int shares_for(int64_t M, int64_t N, int64_t K) {
   const int cg = pair_for(M);
-  const int tiles = std::max(1, tiles_of(M, N, cg)), slots = sm_count() / cg;
-  const int64_t most = std::max<int64_t>(1, (K + kBK - 1) / kBK / 8);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(slots / tiles, most));
+  const int64_t slots = sm_count() / cg, nt = tiles_n(N), tiles = tiles_m(M, cg) * nt, groups = groups_for(M, N, K);
+  const int64_t rounds = (tiles + slots - 1) / slots;
+  return groups * nt <= slots && groups * nt * rounds > 1.05 * tiles ? (int)groups : 0;
+}
+// The slots' sums to out (contiguous rows of N).
+inline int join(const Shape& s, const float* slots, void* out, const int* row_of, const int* pos, int64_t zero_n,
+                cudaStream_t stream) {
+  const int rows = kBM * pair_for(s.M);
+  const int64_t blocks = tiles_m(s.M, pair_for(s.M)) * tiles_n(s.N) * (rows / 32);
+  k_join<<<(unsigned)blocks, 256, 0, stream>>>(s, {slots, reinterpret_cast<__nv_bfloat16*>(out), rows, row_of, pos, zero_n});
+  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+// Bytes of a share walk's slots.
+inline size_t slot_bytes(int64_t M, int64_t N, int shares) {
+  const int cg = pair_for(M);
+  return (size_t)(shares + tiles_m(M, cg)) * tiles_n(N) * kBM * cg * kBN * 4;
 }
 
 }  // namespace gemm

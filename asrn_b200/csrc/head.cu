@@ -30,11 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
 
-ASRN_DEV float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using gemm::exp2_fast;
 
 struct HeadSaved {                       // what the forward pass keeps
   size_t count, tok, row, pos, lse2, rest, hc, total;
@@ -69,27 +65,29 @@ HeadForwardWs head_forward_ws(int64_t N, int64_t V) {
   return w;
 }
 
-// The backward pass's plan: chunks of rows whose dS stays within a gigabyte.
+// The backward pass's plan: chunks of rows whose dS stays within two gigabytes. dh's sums run over V: always in shares.
+// dW's over the rows: shares, or whole tiles when there are enough of them or when the sum runs over several chunks (their
+// sum so far then waits in fp32).
 struct HeadBackwardWs {
   int64_t rows, pitch;
-  int chunks, split_h, split_w;
+  int chunks, shares_h, shares_w;
   size_t ds, dh, dw, total;
 };
 
 HeadBackwardWs head_backward_ws(int64_t N, int64_t V, int64_t d) {
   HeadBackwardWs w{};
   w.pitch = (V + 63) / 64 * 64;
-  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 30) / (2 * w.pitch) / 256 * 256);
+  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 31) / (2 * w.pitch) / 256 * 256);
   w.chunks = (int)((pad256(N) + most - 1) / most);
   w.rows = std::max<int64_t>(256, pad256((N + w.chunks - 1) / std::max(1, w.chunks)));
   w.chunks = (int)((pad256(N) + w.rows - 1) / w.rows);
-  w.split_h = gemm::splits_for(w.rows, d, V);
-  w.split_w = gemm::splits_for(V, d, w.rows);
+  w.shares_h = gemm::groups_for(w.rows, d, V);
+  w.shares_w = w.chunks > 1 ? 0 : gemm::shares_for(V, d, w.rows);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.ds = take((size_t)w.rows * w.pitch * 2);
-  w.dh = take((size_t)w.split_h * w.rows * d * 4);
-  w.dw = take(w.chunks > 1 || w.split_w > 1 ? (size_t)w.split_w * V * d * 4 : 0);
+  w.dh = take(gemm::slot_bytes(w.rows, d, w.shares_h));
+  w.dw = take(w.shares_w ? gemm::slot_bytes(V, d, w.shares_w) : w.chunks > 1 ? (size_t)V * d * 4 : 0);
   w.total = o;
   return w;
 }
@@ -169,11 +167,11 @@ struct Lse {
   int row, V, y, at;
   bool on;
   float m = -INFINITY, s = 0.f;
-  ASRN_DEV Lse(const Params& pp, int r, int rows, int, const gemm::Shape& sh, const gemm::Tile& u, int half)
+  ASRN_DEV Lse(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile& u, int half)
       : p(pp), row(r), V(sh.N), y(-1), at(u.n * 2 + half), on(r < rows) {
     if (on) y = p.tok[r];
   }
-  ASRN_DEV void chunk(float* v, int c) {
+  ASRN_DEV void chunk(float* v, int c, gemm::Out&, const CUtensorMap*, const CUtensorMap*) {
     if (c >= V) return;
     const int n = V - c, j = y - c;        // n: valid columns, 32 or more but in the last tile
     if (j >= 0 && j < 32) {
@@ -193,10 +191,17 @@ struct Lse {
 #pragma unroll
     for (int i = 0; i < 32; ++i) t = fmaxf(t, v[i]);
     const float off = t == -INFINITY ? 0.f : t * p.k;
-    float add = 0.f;
+    const gemm::F2 k2(p.k), off2(-off);
+    gemm::F2 add(0.f);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) add += exp2_fast(fmaf(v[i], p.k, -off));
-    s = s * exp2_fast(fmaf(m, p.k, -off)) + add;
+    for (int i = 0; i < 32; i += 2) {
+      float a, b;
+      gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2).get(a, b);
+      add = gemm::add2(add, gemm::F2(exp2_fast(a), exp2_fast(b)));
+    }
+    float a, b;
+    add.get(a, b);
+    s = s * exp2_fast(fmaf(m, p.k, -off)) + (a + b);
     m = t;
   }
   ASRN_DEV void finish() {
@@ -248,62 +253,37 @@ struct Slope {
     const int *tok, *row;                  // of the chunk's rows
     const float *lse2, *rest, *g;
     float k, inv_tau;
-    __nv_bfloat16* out;
-    int64_t pitch;
-    int room;                              // rows of `out`
   };
   const Params& p;
-  int V, y;
-  float off, g, own;
-  bool on;
-  __nv_bfloat16* at;
-  ASRN_DEV Slope(const Params& pp, int r, int rows, int, const gemm::Shape& sh, const gemm::Tile&, int)
-      : p(pp), V(sh.N), y(-1), off(0.f), g(0.f), own(0.f), on(r < rows), at(r < pp.room ? pp.out + r * pp.pitch : nullptr) {
-    if (on) {
+  int V, y, first;
+  float off, g, own;                       // lse, -dL/dlogp / tau, the target's dS
+  ASRN_DEV Slope(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile&, int)
+      : p(pp), V(sh.N), y(-1), first(r & ~31), off(0.f), g(0.f), own(0.f) {
+    if (r < rows) {
       y = p.tok[r];
       off = p.lse2[r];
-      g = y < 0 ? NAN : p.g[p.row[r]] * p.inv_tau;
-      own = g * p.rest[r];
+      g = y < 0 ? NAN : -p.g[p.row[r]] * p.inv_tau;
+      own = -g * p.rest[r];
     }
   }
-  ASRN_DEV void chunk(float* v, int c) {
-    if (!at || c >= V) return;
+  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+    if (c >= V) return;
+    const gemm::F2 k2(p.k), off2(-off), g2(g);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float e = exp2_fast(fmaf(v[i], p.k, -off));
-      v[i] = !on ? 0.f : c + i == y ? own : -g * e;
+    for (int i = 0; i < 32; i += 2) {
+      float a, b;
+      gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2).get(a, b);
+      gemm::mul2(g2, gemm::F2(exp2_fast(a), exp2_fast(b))).get(v[i], v[i + 1]);
     }
+    const int j = y - c;
+    if (j >= 0 && j < 32) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(at + c + i) = gemm::pack8(v + i);
+      for (int i = 0; i < 32; ++i) v[i] = i == j ? own : v[i];
+    }
+    out.put(map_o, v, c, first);
   }
   ASRN_DEV void finish() {}
 };
-
-// dh of the positions whose rows lie in this chunk: the parts of V added up in order. Positions without a target get
-// zeros with the first chunk.
-__global__ void __launch_bounds__(256)
-k_head_dh(int64_t N, int d, int first, int rows, int splits, const int* __restrict__ pos,
-          const float* __restrict__ part, __nv_bfloat16* __restrict__ dh) {
-  const int nv = d / 8;
-  const int64_t total = N * nv;
-  for (int64_t x = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; x < total; x += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = x / nv;
-    const int c = (int)(x % nv) * 8, r = pos[i];
-    float v[8] = {};
-    if (r < 0) {
-      if (first) continue;
-    } else {
-      if (r < first || r >= first + rows) continue;
-      for (int k = 0; k < splits; ++k) {
-        const float4* q = reinterpret_cast<const float4*>(part + ((int64_t)k * rows + (r - first)) * d + c);
-        const float4 a = q[0], b = q[1];
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-      }
-    }
-    *reinterpret_cast<uint4*>(dh + i * d + c) = gemm::pack8(v);
-  }
-}
 
 int check_head(int64_t N, int64_t V, int32_t d) {
   if (N < 0 || V < 1 || d < 1) return ASRN_ERR_ARG;
@@ -312,28 +292,6 @@ int check_head(int64_t N, int64_t V, int32_t d) {
 }
 
 }  // namespace
-
-// Parts of K added up in order and rounded: out[n] = bf16(sum_k part[k][n]).
-__global__ void __launch_bounds__(256) k_sum_parts(int64_t n, int parts, const float* __restrict__ part,
-                                                   __nv_bfloat16* __restrict__ out) {
-  for (int64_t x = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; x < n;
-       x += (int64_t)gridDim.x * blockDim.x * 8) {
-    float v[8] = {};
-    for (int k = 0; k < parts; ++k) {
-      const float4* q = reinterpret_cast<const float4*>(part + k * n + x);
-      const float4 a = q[0], b = q[1];
-      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-    }
-    *reinterpret_cast<uint4*>(out + x) = gemm::pack8(v);
-  }
-}
-
-int sum_parts(int64_t n, int parts, const float* part, __nv_bfloat16* out, cudaStream_t s) {
-  const int64_t blocks = (n / 8 + 255) / 256;
-  k_sum_parts<<<(unsigned)std::min<int64_t>(blocks, 148 * 8), 256, 0, s>>>(n, parts, part, out);
-  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
-}
 
 }  // namespace asrn
 
@@ -380,7 +338,7 @@ int asrn_head_forward(int64_t N, int64_t V, int32_t d, const void* h, const void
       reinterpret_cast<int*>(S + sv.row), pos, hc);
   if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
   gemm::Shape sh{};
-  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.splits = 1; sh.group = 16; sh.status = status;
+  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.group = 16; sh.status = status;
   const float inv_tau = 1.f / tau;
   Lse::Params p{tok, kLog2e * inv_tau, reinterpret_cast<float*>(W + ws.top), reinterpret_cast<float2*>(W + ws.part),
                 pad256(N)};
@@ -414,44 +372,44 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
   char* W = reinterpret_cast<char*>(workspace);
   const int* count = reinterpret_cast<const int*>(S + sv.count);
   __nv_bfloat16* ds = reinterpret_cast<__nv_bfloat16*>(W + ws.ds);
-  float* dhp = reinterpret_cast<float*>(W + ws.dh);
-  float* dwp = reinterpret_cast<float*>(W + ws.dw);
-  const bool direct = ws.chunks == 1 && ws.split_w == 1;
+  float* dh_slots = reinterpret_cast<float*>(W + ws.dh);
+  float* dw_sum = reinterpret_cast<float*>(W + ws.dw);
   for (int c = 0; c < ws.chunks; ++c) {
     const int64_t first = c * ws.rows;
     const int rows = (int)ws.rows;
     const __nv_bfloat16* hc = reinterpret_cast<const __nv_bfloat16*>(S + sv.hc) + first * d;
     const int64_t left = std::min<int64_t>(rows, pad256(N) - first);   // rows of hc from here on
     gemm::Shape sh{};
-    sh.M = (int)left; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.m_off = (int)first; sh.splits = 1; sh.group = 16;
+    sh.M = (int)left; sh.N = (int)V; sh.K = d; sh.m_dev = count; sh.m_off = (int)first; sh.group = 16;
     sh.status = status;
-    Slope::Params p{reinterpret_cast<const int*>(S + sv.tok) + first, reinterpret_cast<const int*>(S + sv.row) + first,
+    const int* row = reinterpret_cast<const int*>(S + sv.row) + first;
+    Slope::Params p{reinterpret_cast<const int*>(S + sv.tok) + first, row,
                     reinterpret_cast<const float*>(S + sv.lse2) + first,
-                    reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau, ds, ws.pitch,
-                    rows};
-    if ((st = gemm::launch<false, false, Slope>(hc, d, weight, d, sh, p, s))) return st;
+                    reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau};
+    if ((st = gemm::launch<false, false, Slope>(hc, d, weight, d, sh, p, s, {ds, rows, ws.pitch, ws.pitch}))) return st;
     if (dh) {
       gemm::Shape a{};
-      a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.splits = ws.split_h; a.group = 16;
-      a.status = status;
-      if ((st = gemm::launch<false, true, gemm::StoreF32>(ds, ws.pitch, weight, d, a, {dhp, 0}, s))) return st;
-      const int64_t work = (N * (d / 8) + 255) / 256;
-      k_head_dh<<<(unsigned)std::min<int64_t>(work, 148 * 8), 256, 0, s>>>(
-          N, d, (int)first, rows, ws.split_h, reinterpret_cast<const int*>(S + sv.pos), dhp,
-          reinterpret_cast<__nv_bfloat16*>(dh));
-      if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
+      a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.shares = ws.shares_h; a.status = status;
+      const gemm::StorePiece::Params q{dh_slots, gemm::kBM * gemm::pair_for(rows)};
+      if ((st = gemm::launch<false, true, gemm::StorePiece>(ds, ws.pitch, weight, d, a, q, s)) ||
+          (st = gemm::join(a, dh_slots, dh, row, reinterpret_cast<const int*>(S + sv.pos), c ? 0 : N, s)))
+        return st;
     }
     if (dw) {
       gemm::Shape a{};
-      a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.splits = ws.split_w;
-      a.group = 16; a.status = status;
-      st = direct ? gemm::launch<true, true, gemm::StoreBf16>(ds, ws.pitch, hc, d, a,
-                                                                   {reinterpret_cast<__nv_bfloat16*>(dw), nullptr}, s)
-                  : gemm::launch<true, true, gemm::StoreF32>(ds, ws.pitch, hc, d, a, {dwp, c > 0}, s);
-      if (st) return st;
+      a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.shares = ws.shares_w; a.group = 16;
+      a.status = status;
+      if (ws.shares_w) {
+        const gemm::StorePiece::Params q{dw_sum, gemm::kBM * gemm::pair_for(V)};
+        if ((st = gemm::launch<true, true, gemm::StorePiece>(ds, ws.pitch, hc, d, a, q, s)) ||
+            (st = gemm::join(a, dw_sum, dw, nullptr, nullptr, 0, s)))
+          return st;
+      } else {
+        const gemm::StoreBf16::Params q{nullptr, c ? dw_sum : nullptr, c + 1 < ws.chunks ? dw_sum : nullptr};
+        if ((st = gemm::launch<true, true, gemm::StoreBf16>(ds, ws.pitch, hc, d, a, q, s, {dw, V, d, d}))) return st;
+      }
     }
   }
-  if (dw && !direct) return sum_parts(V * d, ws.split_w, dwp, reinterpret_cast<__nv_bfloat16*>(dw), s);
   return ASRN_OK;
 }
 

@@ -275,6 +275,8 @@ bool make_tmap_f32_3d_sw128(void* map /* CUtensorMap */, const void* base, uint6
 // or 128; with a swizzle, box_inner * 2 equals it).
 bool make_tmap_rows_bf16(void* map /* CUtensorMap */, const void* base, uint64_t inner, uint64_t outer,
                          uint64_t row_bytes, uint32_t box_inner, int swizzle_bytes);
+bool make_tmap_bf16_sw64(void* map /* CUtensorMap */, const void* base, uint64_t inner, uint64_t outer,
+                         uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
 bool make_tmap_bf16(void* map /* CUtensorMap */, const void* base, uint64_t inner, uint64_t outer,
                     uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
 // GEMM implementation choice: false while the test hook asrn_test_force_cuda_core holds the CUDA-core kernels.

@@ -11,17 +11,14 @@
 //   k_pack8        x -> Q(x)
 //   k_gemm<Up>     a, Q(a), gelu(a)
 //   k_gemm         y
-//   k_colsum_rows  db2's partial sums
+//   k_prepare      x', and db2's partial sums by 64 rows
 //   k_gemm<Down>   dY W2 -> dA, gelu(a'), db1's partial sums by 32 rows
-//   k_unpack8      x'
-//   k_gemm x 3     dX, dW1, dW2 (parts of N where there are few tiles)
+//   k_gemm x 3     dX, dW1, dW2 (the last two in shares of N: few tiles)
 //   k_colsum       db1, db2
 #include "common.cuh"
 #include "gemm_tc.cuh"
 
 namespace asrn {
-
-int sum_parts(int64_t n, int parts, const float* part, __nv_bfloat16* out, cudaStream_t s);
 
 namespace {
 
@@ -38,31 +35,66 @@ ASRN_DEV float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); 
 ASRN_DEV float scale_of(int e) { return e == kBad ? NAN : pow2(e); }
 ASRN_DEV float inv_scale_of(int e) { return e == kBad ? 0.f : pow2(-e); }
 
+// Codes of four values: v inv + 1.5 2^23 holds the nearest integer, ties to even, in its low bits.
 ASRN_DEV uint32_t codes4(const float* v, float inv) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r |= ((uint32_t)__float2int_rn(v[i] * inv) & 255u) << (8 * i);
-  return r;
+  const gemm::F2 k(inv), magic(12582912.f);
+  float f[4];
+  gemm::fma2(gemm::F2(v[0], v[1]), k, magic).get(f[0], f[1]);
+  gemm::fma2(gemm::F2(v[2], v[3]), k, magic).get(f[2], f[3]);
+  const uint32_t lo = __byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
-ASRN_DEV float value_of(uint32_t w, int i, float scale) { return (float)(int8_t)(w >> (8 * i)) * scale; }
-
-ASRN_DEV float abs_max32(const float* v) {     // a NaN counts as the largest
-  float m = 0.f;
-  bool bad = false;
+// And back: byte + 128 as the low bits of 2^23, less 2^23 + 128, times the scale; each step is exact.
+ASRN_DEV void values4(float* v, uint32_t w, float scale) {
+  const uint32_t u = w ^ 0x80808080u;
+  const gemm::F2 k(scale), off(-8388736.f);
+  float f[4];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    m = fmaxf(m, fabsf(v[i]));
-    bad |= v[i] != v[i];
-  }
-  return bad ? NAN : m;
+  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 + i));
+  gemm::mul2(gemm::add2(gemm::F2(f[0], f[1]), off), k).get(v[0], v[1]);
+  gemm::mul2(gemm::add2(gemm::F2(f[2], f[3]), off), k).get(v[2], v[3]);
 }
 
-// Phi(a) and a phi(a) of the standard normal: gelu = a Phi, gelu' = Phi + a phi.
-struct Normal {
-  float cdf, apdf;
-};
-ASRN_DEV Normal normal_of(float a) {
-  return Normal{0.5f * (1.f + erff(a * 0.70710678118654752f)), a * expf(-0.5f * a * a) * 0.39894228040143268f};
+ASRN_DEV float abs_max32(const float* v) {     // a NaN is the largest
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(m) : "f"(v[i]));
+  return fabsf(m);
+}
+
+// Of two values a: e = exp(-a^2 / 2) and q = Q(|a|), the normal distribution's tail, by Abramowitz and Stegun's 7.1.26,
+// erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), with x = |a| / sqrt 2 (error of q at most 7.5e-8). Then
+// gelu(a) = max(a, 0) - |a| q and gelu'(a) = 1/2 + sign(a) (1/2 - q) + a e / sqrt(2 pi).
+ASRN_DEV void tails(float a0, float a1, gemm::F2& e, gemm::F2& q) {
+  using namespace gemm;
+  const F2 a(a0, a1), m(fabsf(a0), fabsf(a1));
+  float x, y;
+  mul2(mul2(a, a), F2(-0.72134752044448170f)).get(x, y);
+  e = F2(exp2_fast(x), exp2_fast(y));
+  fma2(m, F2(0.3275911f * 0.70710678118654752f), F2(1.f)).get(x, y);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
+  const F2 t(x, y);
+  F2 r = fma2(t, F2(0.5f * 1.061405429f), F2(0.5f * -1.453152027f));
+  r = fma2(r, t, F2(0.5f * 1.421413741f));
+  r = fma2(r, t, F2(0.5f * -0.284496736f));
+  r = fma2(r, t, F2(0.5f * 0.254829592f));
+  q = mul2(mul2(r, t), e);
+}
+
+// The codes of a block to `at` (n values of it, a multiple of 8); its exponent.
+ASRN_DEV int store_codes(const float* v, uint8_t* at, int n) {
+  const int e = block_exp(abs_max32(v));
+  const float inv = inv_scale_of(e);
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (i < n) {
+      uint2 w = make_uint2(codes4(v + i, inv), codes4(v + i + 4, inv));
+      if (e == kBad) w = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(at + i) = w;
+    }
+  return e;
 }
 
 // One thread per block of 32 of a row of bf16.
@@ -84,68 +116,54 @@ __global__ void __launch_bounds__(256) k_pack8(int64_t blocks, int f, int per_ro
         v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
       }
     }
-    const int e = block_exp(abs_max32(v));
-    const float inv = inv_scale_of(e);
-    exps[b] = (int8_t)e;
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (c + i < f)
-        *reinterpret_cast<uint2*>(codes + at + i) = make_uint2(codes4(v + i, inv), codes4(v + i + 4, inv));
+    exps[b] = (int8_t)store_codes(v, codes + at, f - c);
   }
 }
 
 // One thread per 8 values.
+ASRN_DEV void unpack_at(int64_t b, int f, const uint8_t* __restrict__ codes, const int8_t* __restrict__ exps,
+                        __nv_bfloat16* __restrict__ x) {
+  const int per = f / 8, per_row = (f + 31) / 32;
+  const int64_t row = b / per;
+  const int c = (int)(b % per) * 8;
+  const uint2 w = *reinterpret_cast<const uint2*>(codes + row * f + c);
+  const float scale = scale_of(exps[row * per_row + c / 32]);
+  float v[8];
+  values4(v, w.x, scale);
+  values4(v + 4, w.y, scale);
+  *reinterpret_cast<uint4*>(x + row * f + c) = gemm::pack8(v);
+}
 __global__ void __launch_bounds__(256) k_unpack8(int64_t eighths, int f, const uint8_t* __restrict__ codes,
                                                  const int8_t* __restrict__ exps, __nv_bfloat16* __restrict__ x) {
-  const int per = f / 8, per_row = (f + 31) / 32;
-  for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < eighths; b += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = b / per;
-    const int c = (int)(b % per) * 8;
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + row * f + c);
-    const float scale = scale_of(exps[row * per_row + c / 32]);
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = value_of(w.x, i, scale);
-      v[4 + i] = value_of(w.y, i, scale);
-    }
-    *reinterpret_cast<uint4*>(x + row * f + c) = gemm::pack8(v);
-  }
+  for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < eighths; b += (int64_t)gridDim.x * blockDim.x)
+    unpack_at(b, f, codes, exps, x);
 }
 
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
 struct Up {
   struct Params {
     const __nv_bfloat16* bias;
-    __nv_bfloat16* g;
     uint8_t* codes;
     int8_t* exps;
   };
   const Params& p;
   int64_t at, eat;
-  int N;
+  int N, first;
   bool on;
-  ASRN_DEV Up(const Params& pp, int row, int rows, int, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)row * s.N), eat((int64_t)row * ((s.N + 31) / 32)), N(s.N), on(row < rows) {}
-  ASRN_DEV void chunk(float* v, int c) {
-    if (!on || c >= N) return;
+  ASRN_DEV Up(const Params& pp, int row, int rows, const gemm::Shape& s, const gemm::Tile&, int)
+      : p(pp), at((int64_t)row * s.N), eat((int64_t)row * ((s.N + 31) / 32)), N(s.N), first(row & ~31), on(row < rows) {}
+  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+    if (c >= N) return;                        // the columns past N of the last block are zeros
+    gemm::add_bias(v, p.bias + c, N - c);
+    if (p.codes && on) p.exps[eat + c / 32] = (int8_t)store_codes(v, p.codes + at + c, N - c);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      v[i] = c + i < N ? v[i] + __bfloat162float(p.bias[c + i]) : 0.f;
-    if (p.codes) {
-      const int e = block_exp(abs_max32(v));
-      const float inv = inv_scale_of(e);
-      p.exps[eat + c / 32] = (int8_t)e;
-#pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        if (c + i < N)
-          *reinterpret_cast<uint2*>(p.codes + at + c + i) = make_uint2(codes4(v + i, inv), codes4(v + i + 4, inv));
+    for (int i = 0; i < 32; i += 2) {
+      gemm::F2 e, q;
+      tails(v[i], v[i + 1], e, q);
+      gemm::fma2(gemm::F2(-fabsf(v[i]), -fabsf(v[i + 1])), q, gemm::F2(fmaxf(v[i], 0.f), fmaxf(v[i + 1], 0.f)))
+          .get(v[i], v[i + 1]);
     }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= normal_of(v[i]).cdf;
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (c + i < N) *reinterpret_cast<uint4*>(p.g + at + c + i) = gemm::pack8(v + i);
+    out.put(map_o, v, c, first);
   }
   ASRN_DEV void finish() {}
 };
@@ -169,74 +187,95 @@ struct Down {
   struct Params {
     const uint8_t* codes;
     const int8_t* exps;
-    __nv_bfloat16 *da, *g;
-    float* sums;                               // [ceil(rows / 32)][N]
+    float* sums;                               // [ceil(rows / 32)][N], or null
   };
   const Params& p;
   int64_t at, eat;
-  int N, row, rows;
+  int N, first, rows;
   bool on;
-  ASRN_DEV Down(const Params& pp, int r, int m, int, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)r * s.N), eat((int64_t)r * ((s.N + 31) / 32)), N(s.N), row(r), rows(m), on(r < m) {}
-  ASRN_DEV void chunk(float* v, int c) {
+  ASRN_DEV Down(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
+      : p(pp), at((int64_t)r * s.N), eat((int64_t)r * ((s.N + 31) / 32)), N(s.N), first(r & ~31), rows(m), on(r < m) {}
+  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
+    using gemm::F2;
     if (c >= N) return;                        // the same for the whole warp
     const float scale = on ? scale_of(p.exps[eat + c / 32]) : 0.f;
+    float g[32];
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
-      const bool in = on && c + i < N;
       uint2 w = make_uint2(0, 0);
-      if (in) w = *reinterpret_cast<const uint2*>(p.codes + at + c + i);
-      float g[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = value_of(j < 4 ? w.x : w.y, j & 3, scale);
-        const Normal n = normal_of(a);
-        g[j] = a * n.cdf;
-        v[i + j] = in ? v[i + j] * (n.cdf + n.apdf) : 0.f;
-      }
-      if (in) {
-        *reinterpret_cast<uint4*>(p.g + at + c + i) = gemm::pack8(g);
-        *reinterpret_cast<uint4*>(p.da + at + c + i) = gemm::pack8(v + i);
-      }
+      if (on && c + i < N) w = *reinterpret_cast<const uint2*>(p.codes + at + c + i);
+      values4(g + i, w.x, scale);
+      values4(g + i + 4, w.y, scale);
     }
-    const int lane = threadIdx.x & 31;
-    const float s = column_sum(v, lane);
-    const int first = row - lane;              // the warp's rows start on a multiple of 32
-    if (p.sums && first < rows && c + lane < N) p.sums[(int64_t)(first / 32) * N + c + lane] = s;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float a0 = g[i], a1 = g[i + 1];
+      F2 e, q;
+      tails(a0, a1, e, q);
+      float h0, h1;
+      gemm::fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                             // 1/2 - q
+      const F2 cdf = gemm::add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
+      const F2 slope = gemm::fma2(gemm::mul2(F2(a0, a1), F2(0.39894228040143268f)), e, cdf);
+      gemm::mul2(F2(v[i], v[i + 1]), slope).get(v[i], v[i + 1]);
+      gemm::fma2(F2(-fabsf(a0), -fabsf(a1)), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(g[i], g[i + 1]);
+    }
+    out.put(map_o, v, c, first);
+    out.put(map_p, g, c, first);
+    if (p.sums && first < rows) {              // rows past the end are zeros: the operand's rows were
+      const int lane = threadIdx.x & 31;
+      const float s = column_sum(v, lane);
+      if (c + lane < N) p.sums[(int64_t)(first / 32) * N + c + lane] = s;
+    }
   }
   ASRN_DEV void finish() {}
 };
 
-// Sums of bf16 columns over 64 rows: block (64 rows, 256 columns), thread = column.
+// x' from its codes (the first `unpackers` blocks), and sums of dY's columns over 64 rows (the others: block = 64 rows x
+// 256 columns, thread = column).
 constexpr int kColRows = 64;
-__global__ void __launch_bounds__(256) k_colsum_rows(int64_t rows, int n, const __nv_bfloat16* __restrict__ x,
-                                                     float* __restrict__ sums) {
-  const int c = blockIdx.y * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256)
+k_prepare(int unpackers, int64_t eighths, int d, const uint8_t* __restrict__ codes, const int8_t* __restrict__ exps,
+          __nv_bfloat16* __restrict__ x, int64_t rows, int n, const __nv_bfloat16* __restrict__ dy,
+          float* __restrict__ sums) {
+  if ((int)blockIdx.x < unpackers) {
+    for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < eighths; b += (int64_t)unpackers * 256)
+      unpack_at(b, d, codes, exps, x);
+    return;
+  }
+  const int wide = (n + 255) / 256, block = blockIdx.x - unpackers;
+  const int c = block % wide * 256 + threadIdx.x;
   if (c >= n) return;
-  const int64_t r0 = (int64_t)blockIdx.x * kColRows;
+  const int64_t r0 = (int64_t)(block / wide) * kColRows;
   const int64_t r1 = r0 + kColRows < rows ? r0 + kColRows : rows;
   float s = 0.f;
-#pragma unroll 8
-  for (int64_t r = r0; r < r1; ++r) s += __bfloat162float(x[r * n + c]);
-  sums[(int64_t)blockIdx.x * n + c] = s;
+#pragma unroll 16
+  for (int64_t r = r0; r < r1; ++r) s += __bfloat162float(dy[r * n + c]);
+  sums[(int64_t)(block / wide) * n + c] = s;
 }
 
-// out[c] = bf16(sum of parts[..][c]) in order: block = 32 columns x 32 warps.
-__global__ void __launch_bounds__(1024) k_colsum(int64_t parts, int n, const float* __restrict__ sums,
-                                                 __nv_bfloat16* __restrict__ out) {
+// out[c] = bf16(sum of the parts' [..][c]) in order, for two sets: block = 32 columns x 32 warps.
+struct ColSum {
+  int64_t parts;
+  int n;
+  const float* sums;
+  __nv_bfloat16* out;
+};
+__global__ void __launch_bounds__(1024) k_colsum(const ColSum a, const ColSum b, int blocks_a) {
   __shared__ float sh[32][33];
+  const bool second = (int)blockIdx.x >= blocks_a;
+  const ColSum& q = second ? b : a;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int c = ((int)blockIdx.x - (second ? blocks_a : 0)) * 32 + lane;
   float s = 0.f;
-  if (c < n)
+  if (c < q.n)
 #pragma unroll 4
-    for (int64_t k = wid; k < parts; k += 32) s += sums[k * n + c];
+    for (int64_t k = wid; k < q.parts; k += 32) s += q.sums[k * q.n + c];
   sh[wid][lane] = s;
   __syncthreads();
   if (wid) return;
   s = 0.f;
   for (int w = 0; w < 32; ++w) s += sh[w][lane];
-  if (c < n) out[c] = __float2bfloat16_rn(s);
+  if (c < q.n) q.out[c] = __float2bfloat16_rn(s);
 }
 
 struct Mlp8Saved {
@@ -256,8 +295,8 @@ Mlp8Saved mlp8_saved(int64_t N, int64_t d, int64_t ff) {
 }
 
 struct Mlp8Ws {
-  int split1, split2;
-  size_t da, g, x, sum1, sum2, part, total;
+  int shares1, shares2;
+  size_t da, g, x, sum1, sum2, slots, total;
 };
 
 Mlp8Ws mlp8_ws(int64_t N, int64_t d, int64_t ff, int64_t dout, bool backward) {
@@ -266,13 +305,14 @@ Mlp8Ws mlp8_ws(int64_t N, int64_t d, int64_t ff, int64_t dout, bool backward) {
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.g = take((size_t)N * ff * 2);
   if (backward) {
-    w.split1 = gemm::splits_for(ff, d, N);
-    w.split2 = gemm::splits_for(dout, ff, N);
+    w.shares1 = gemm::shares_for(ff, d, N);
+    w.shares2 = gemm::shares_for(dout, ff, N);
     w.da = take((size_t)N * ff * 2);
     w.x = take((size_t)N * d * 2);
     w.sum1 = take((size_t)((N + 31) / 32) * ff * 4);
     w.sum2 = take((size_t)((N + kColRows - 1) / kColRows) * dout * 4);
-    w.part = take((size_t)std::max(w.split1 * d, w.split2 * dout) * ff * 4);
+    w.slots = take(std::max(w.shares1 ? gemm::slot_bytes(ff, d, w.shares1) : 0,
+                            w.shares2 ? gemm::slot_bytes(dout, ff, w.shares2) : 0));
   }
   w.total = o;
   return w;
@@ -304,15 +344,15 @@ int unpack8(int64_t rows, int f, const void* codes, const void* exps, void* x, c
   return launched();
 }
 
-// out (M, n) = A^T B over the rows they share, both as they lie in memory: parts of the rows when there are few tiles.
-int weight_grad(int64_t rows, int M, int n, const void* A, const void* B, int splits, float* part, void* out,
+// out (M, n) = A^T B over the rows they share, both as they lie in memory.
+int weight_grad(int64_t rows, int M, int n, const void* A, const void* B, int shares, float* slots, void* out,
                 int* status, cudaStream_t s) {
   gemm::Shape a{};
-  a.M = M; a.N = n; a.K = (int)rows; a.splits = splits; a.group = 16; a.status = status;
-  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-  if (splits == 1) return gemm::launch<true, true, gemm::StoreBf16>(A, M, B, n, a, {o, nullptr}, s);
-  const int st = gemm::launch<true, true, gemm::StoreF32>(A, M, B, n, a, {part, 0}, s);
-  return st ? st : sum_parts((int64_t)M * n, splits, part, o, s);
+  a.M = M; a.N = n; a.K = (int)rows; a.shares = shares; a.group = 16; a.status = status;
+  if (!shares) return gemm::launch<true, true, gemm::StoreBf16>(A, M, B, n, a, {}, s, {out, M, n, n});
+  const gemm::StorePiece::Params q{slots, gemm::kBM * gemm::pair_for(M)};
+  const int st = gemm::launch<true, true, gemm::StorePiece>(A, M, B, n, a, q, s);
+  return st ? st : gemm::join(a, slots, out, nullptr, nullptr, 0, s);
 }
 
 }  // namespace
@@ -368,13 +408,14 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(workspace) + ws.g);
   if (S && (st = pack8(N, d, x, S + sv.xc, S + sv.xe, s))) return st;
   gemm::Shape a{};
-  a.M = (int)N; a.N = ff; a.K = d; a.splits = 1; a.group = 16; a.status = status;
-  Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), g, S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
-               S ? reinterpret_cast<int8_t*>(S + sv.ae) : nullptr};
-  if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s))) return st;
+  a.M = (int)N; a.N = ff; a.K = d; a.group = 16; a.status = status;
+  const Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
+                     S ? reinterpret_cast<int8_t*>(S + sv.ae) : nullptr};
+  if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s, {g, N, ff, ff}))) return st;
   a.N = dout; a.K = ff;
-  return gemm::launch<false, false, gemm::StoreBf16>(
-      g, ff, w2, ff, a, {reinterpret_cast<__nv_bfloat16*>(y), reinterpret_cast<const __nv_bfloat16*>(b2)}, s);
+  return gemm::launch<false, false, gemm::StoreBf16>(g, ff, w2, ff, a,
+                                                     {reinterpret_cast<const __nv_bfloat16*>(b2), nullptr, nullptr}, s,
+                                                     {y, N, dout, dout});
 }
 
 int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void* dy, const void* w1, const void* w2,
@@ -403,38 +444,40 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
   char* W = reinterpret_cast<char*>(workspace);
   __nv_bfloat16* da = reinterpret_cast<__nv_bfloat16*>(W + ws.da);
   __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(W + ws.g);
-  float* part = reinterpret_cast<float*>(W + ws.part);
+  float* slots = reinterpret_cast<float*>(W + ws.slots);
   float* sum1 = reinterpret_cast<float*>(W + ws.sum1);
   float* sum2 = reinterpret_cast<float*>(W + ws.sum2);
-  const int64_t groups = (N + 31) / 32, blocks = (N + kColRows - 1) / kColRows;
+  const int64_t blocks = (N + kColRows - 1) / kColRows;
   gemm::Shape a{};
-  a.M = (int)N; a.splits = 1; a.group = 16; a.status = status;
+  a.M = (int)N; a.group = 16; a.status = status;
+  if (dw1 || db2) {
+    const int64_t eighths = dw1 ? N * (d / 8) : 0;
+    const unsigned unpackers = dw1 ? grid_for(eighths) : 0;
+    const unsigned summers = db2 ? (unsigned)(blocks * ((dout + 255) / 256)) : 0;
+    k_prepare<<<unpackers + summers, 256, 0, s>>>(
+        (int)unpackers, eighths, d, reinterpret_cast<const uint8_t*>(S + sv.xc),
+        reinterpret_cast<const int8_t*>(S + sv.xe), reinterpret_cast<__nv_bfloat16*>(W + ws.x), N, dout,
+        reinterpret_cast<const __nv_bfloat16*>(dy), sum2);
+    if ((st = launched())) return st;
+  }
   if (dx || dw1 || db1 || dw2) {
     a.N = ff; a.K = dout;
-    Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), reinterpret_cast<const int8_t*>(S + sv.ae), da, g,
-                   db1 ? sum1 : nullptr};
-    if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s))) return st;
+    const Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), reinterpret_cast<const int8_t*>(S + sv.ae),
+                         db1 ? sum1 : nullptr};
+    if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s, {da, N, ff, ff}, {g, N, ff, ff}))) return st;
   }
   if (dx) {
     a.N = d; a.K = ff;
-    if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, ff, w1, d, a,
-                                                               {reinterpret_cast<__nv_bfloat16*>(dx), nullptr}, s)))
-      return st;
+    if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, ff, w1, d, a, {}, s, {dx, N, d, d}))) return st;
   }
-  if (dw1) {
-    if ((st = unpack8(N, d, S + sv.xc, S + sv.xe, W + ws.x, s))) return st;
-    if ((st = weight_grad(N, ff, d, da, W + ws.x, ws.split1, part, dw1, status, s))) return st;
-  }
-  if (dw2 && (st = weight_grad(N, dout, ff, dy, g, ws.split2, part, dw2, status, s))) return st;
-  if (db1) {
-    k_colsum<<<(unsigned)((ff + 31) / 32), 1024, 0, s>>>(groups, ff, sum1, reinterpret_cast<__nv_bfloat16*>(db1));
-    if ((st = launched())) return st;
-  }
-  if (db2) {
-    k_colsum_rows<<<dim3((unsigned)blocks, (unsigned)((dout + 255) / 256)), 256, 0, s>>>(
-        N, dout, reinterpret_cast<const __nv_bfloat16*>(dy), sum2);
-    k_colsum<<<(unsigned)((dout + 31) / 32), 1024, 0, s>>>(blocks, dout, sum2, reinterpret_cast<__nv_bfloat16*>(db2));
-    if ((st = launched())) return st;
+  if (dw1 && (st = weight_grad(N, ff, d, da, W + ws.x, ws.shares1, slots, dw1, status, s))) return st;
+  if (dw2 && (st = weight_grad(N, dout, ff, dy, g, ws.shares2, slots, dw2, status, s))) return st;
+  if (db1 || db2) {
+    const ColSum q1{(N + 31) / 32, db1 ? ff : 0, sum1, reinterpret_cast<__nv_bfloat16*>(db1)};
+    const ColSum q2{blocks, db2 ? dout : 0, sum2, reinterpret_cast<__nv_bfloat16*>(db2)};
+    const int b1 = (q1.n + 31) / 32, b2 = (q2.n + 31) / 32;
+    k_colsum<<<(unsigned)(b1 + b2), 1024, 0, s>>>(q1, q2, b1);
+    return launched();
   }
   return ASRN_OK;
 }

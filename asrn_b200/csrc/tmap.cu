@@ -36,6 +36,21 @@ bool make_tmap_bf16(void* map, const void* base, uint64_t inner, uint64_t outer,
   return r == CUDA_SUCCESS;
 }
 
+// The same with the 64-byte swizzle (box_inner = 32: 64-byte rows).
+bool make_tmap_bf16_sw64(void* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                         uint32_t box_inner, uint32_t box_outer) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+                  dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // Rows of a (outer, inner) bf16 matrix for row gathers: box = one row of box_inner elements (box_inner may exceed
 // inner: the columns past it read zeros), with the shared-memory swizzle of swizzle_bytes (0: none).
 bool make_tmap_rows_bf16(void* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
