@@ -4,8 +4,9 @@
 //   warp 0        streams both operands through a ring of 64-deep K blocks by TMA (128-byte swizzle)
 //   warp 1        issues tcgen05.mma into one of two 256-column TMEM accumulators
 //   warps 2-9     drain the other accumulator: thread = row, two warps per 32-lane quadrant, each half of the columns,
-//                 32 at a time; bf16 results leave by TMA through two 2 KB pieces per warp (direct stores, a row's 16
-//                 bytes per lane, touch 32 half-written sectors each)
+//   (or 2-17)     32 at a time (an epilogue that computes much: four warps, each a quarter); bf16 results leave by TMA
+//                 through 2 KB pieces of shared memory (direct stores, a row's 16 bytes per lane, touch 32 half-written
+//                 sectors each)
 //
 // Either operand may lie in memory with its K dimension innermost (K-major) or with its M / N dimension innermost
 // (MN-major), so the products of a backward pass read the forward pass's tensors as they are. Pairs of blocks
@@ -30,14 +31,13 @@ namespace asrn {
 namespace gemm {
 
 constexpr int kBM = 128, kBN = 256, kBK = 64;
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = (2 + kEpiWarps) * 32;
+template <class Epi> constexpr int threads_of() { return (2 + Epi::kWarps) * 32; }
 constexpr int kBytesA = kBM * 128;                       // one block's share of a stage
 template <int CG> constexpr int bytes_b() { return kBN / CG * 128; }
 template <int CG> constexpr int stage_bytes() { return kBytesA + bytes_b<CG>(); }
 template <int CG> constexpr int stages() { return CG == 1 ? 4 : 6; }
 constexpr int kPiece = 32 * 64;                          // 32 rows x 32 bf16 columns, 64-byte swizzle
-constexpr int kPieces = 2 * kEpiWarps * kPiece;
+constexpr int kPieces = 16 * kPiece;                     // 2 per warp, or 1 where there are 16 warps
 template <int CG> constexpr size_t smem_bytes() {
   return 1024 + (size_t)stages<CG>() * stage_bytes<CG>() + kPieces + 256;
 }
@@ -218,15 +218,15 @@ ASRN_DEV uint4 pack8(const float* v) {
                     umma::pack_bf16x2(v[6], v[7]));
 }
 
-// A warp's way out for 32 rows x 32 columns of bf16: written to one of two pieces of shared memory, from there by TMA.
-// A piece is written again once the copy before last has read it.
-struct Out {
-  uint8_t* piece;                                        // the warp's two
+// A warp's way out for 32 rows x 32 columns of bf16: written to a piece of shared memory, from there by TMA. A piece is
+// written again once the copy that read it last is done.
+template <int Pieces> struct Out {
+  uint8_t* piece;                                        // the warp's own
   int lane, turn;
   ASRN_DEV void put(const CUtensorMap* map, const float* v, int column, int first_row) {
-    uint8_t* at = piece + (turn & 1) * kPiece;
-    turn ^= 1;
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    uint8_t* at = piece + turn * kPiece;
+    turn = (turn + 1) % Pieces;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Pieces - 1) : "memory");
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -245,10 +245,10 @@ struct Out {
   }
 };
 
-// Epi: struct with a Params type, a constructor (Params, row, rows, shape, tile, half of the columns) and chunk(v[32],
+// Epi: struct with a Params type, kWarps (8 or 16), a constructor (Params, row, rows, shape, tile, the warp's part of the columns) and chunk(v[32],
 // column, Out, map_o, map_p), called by whole warps for the tile's chunks of 32 columns, then finish().
 template <int CG, bool AMn, bool BMn, class Epi>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of<Epi>(), 1)
 k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
        const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_p, const Shape s,
        const typename Epi::Params p) {
@@ -275,7 +275,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + i, 1);
-      mbar_init(tempty + i, CG * kEpiWarps);
+      mbar_init(tempty + i, CG * Epi::kWarps);
     }
     fence_mbar_init();
     prefetch_tensormap(&map_a);
@@ -345,21 +345,22 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       }
     }
   } else {                                              // epilogue
-    const int q4 = wid & 3, half = (wid - 2) >> 2;
-    Out out{sO + (wid - 2) * 2 * kPiece, lane, 0};
-    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(half * (kBN / 2));
+    constexpr int kCols = kBN * 4 / Epi::kWarps, kOwn = 16 / Epi::kWarps;
+    const int q4 = wid & 3, part = (wid - 2) >> 2;
+    Out<kOwn> out{sO + (wid - 2) * kOwn * kPiece, lane, 0};
+    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(part * kCols);
     int jt = 0;
     for (; walk.next(u); ++jt) {
       const int b = jt & 1;
       if (!mbar_wait(tfull + b, (jt >> 1) & 1, s.status)) break;
       tc_fence_after();
-      const int c0 = u.n * kBN + half * (kBN / 2);
-      Epi e(p, (u.m * CG + (int)rank) * kBM + q4 * 32 + lane, M, s, u, half);
+      const int c0 = u.n * kBN + part * kCols;
+      Epi e(p, (u.m * CG + (int)rank) * kBM + q4 * 32 + lane, M, s, u, part);
 #pragma unroll 1
-      for (int ch = 0; ch < kBN / 64; ++ch) {
+      for (int ch = 0; ch < kCols / 32; ++ch) {
         float v[32];
         tmem_ld32(trow + (uint32_t)(b * kBN + ch * 32), v);
-        if (ch == kBN / 64 - 1) {                       // the accumulator is read: the next product may have it
+        if (ch == kCols / 32 - 1) {                       // the accumulator is read: the next product may have it
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -405,19 +406,22 @@ ASRN_DEV void add_bias(float* v, const __nv_bfloat16* bias, int n) {
     }
 }
 
-// The fp32 sums of a piece of a tile, whole, to its slot: slot[rows of a tile][256].
+// The fp32 sums of a piece of a tile, whole, to its slot: by blocks of 32 rows x 32 columns, each as the warp holds it
+// (four columns of all 32 rows are 512 neighbouring bytes).
 struct StorePiece {
+  static constexpr int kWarps = 8;
   struct Params {
     float* slots;
     int tile_rows;
   };
   float* at;
-  ASRN_DEV StorePiece(const Params& p, int row, int, const Shape&, const Tile& u, int half)
-      : at(p.slots + ((int64_t)u.slot * p.tile_rows + row % p.tile_rows) * kBN - u.n * kBN) {}
-  ASRN_DEV void chunk(const float* v, int c, Out&, const CUtensorMap*, const CUtensorMap*) {
+  ASRN_DEV StorePiece(const Params& p, int row, int, const Shape&, const Tile& u, int)
+      : at(p.slots + ((int64_t)u.slot * p.tile_rows + (row % p.tile_rows & ~31)) * kBN + (row & 31) * 4 -
+           (int64_t)u.n * kBN * 32) {}
+  template <class O> ASRN_DEV void chunk(const float* v, int c, O&, const CUtensorMap*, const CUtensorMap*) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4)
-      *reinterpret_cast<float4*>(at + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      *reinterpret_cast<float4*>(at + (int64_t)c * 32 + i * 32) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   }
   ASRN_DEV void finish() {}
 };
@@ -425,6 +429,7 @@ struct StorePiece {
 // bf16(sum + bias + before): out[row][column] through map_o (N a multiple of 8). before: fp32 (M, N), the sum of what
 // came earlier; or, when `after` is given, the sum goes there in fp32 instead.
 struct StoreBf16 {
+  static constexpr int kWarps = 8;
   struct Params {
     const __nv_bfloat16* bias;
     const float* before;
@@ -436,7 +441,7 @@ struct StoreBf16 {
   bool on;
   ASRN_DEV StoreBf16(const Params& pp, int row, int rows, const Shape& s, const Tile&, int)
       : p(pp), at((int64_t)row * s.N), N(s.N), first(row & ~31), on(row < rows) {}
-  ASRN_DEV void chunk(float* v, int c, Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
     if (c >= N) return;
     if (p.bias) add_bias(v, p.bias + c, N - c);
     if (p.before && on) {
@@ -459,8 +464,8 @@ struct StoreBf16 {
   ASRN_DEV void finish() {}
 };
 
-// The pieces of each tile added up in order and rounded: out[row_of ? row_of[r] : r][c]. Block = 32 rows x 256 columns of
-// one tile. Positions i < zero_n with pos[i] < 0 get zero rows (whole grid).
+// The pieces of each tile added up in order and rounded: out[row_of ? row_of[r] : r][c], a warp per 32 rows x 32 columns.
+// Positions i < zero_n with pos[i] < 0 get zero rows (whole grid).
 struct JoinArgs {
   const float* slots;
   __nv_bfloat16* out;
@@ -472,10 +477,10 @@ struct JoinArgs {
 static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinArgs a) {
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
   const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN, kblocks = (K + kBK - 1) / kBK;
-  const int per = a.tile_rows / 32;
+  const int per = a.tile_rows / 32, lane = threadIdx.x & 31;              // blocks of 32 rows of a tile
   const int64_t all = (int64_t)mt * kblocks;
-  const int tile = blockIdx.x / per, m = tile / nt, n = tile % nt;
-  const int c = n * kBN + (threadIdx.x & 31) * 8;
+  const int tile = blockIdx.x / per, m = tile / nt, n = tile % nt, part = blockIdx.x % per;
+  const int c = n * kBN + (threadIdx.x >> 5) * 32, r = m * a.tile_rows + part * 32 + lane;
   if (m < mt && c < s.N) {
     int g0 = 0, g1 = -1;
     if (kblocks) {
@@ -483,23 +488,26 @@ static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinAr
       g0 = (int)share_of((int64_t)m * kblocks, all, shares);
       g1 = (int)share_of((int64_t)(m + 1) * kblocks - 1, all, shares);
     }
-    for (int k = threadIdx.x >> 5; k < 32; k += 8) {
-      const int in = blockIdx.x % per * 32 + k, r = m * a.tile_rows + in;
-      if (r >= M) break;
-      float v[8] = {};
-      for (int g = g0; g <= g1; ++g) {
-        const float4* q = reinterpret_cast<const float4*>(
-            a.slots + ((int64_t)((g + m) * nt + n) * a.tile_rows + in) * kBN + (c - n * kBN));
-        const float4 x = q[0], y = q[1];
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    float v[32] = {};
+    for (int g = g0; g <= g1; ++g) {
+      const float4* q = reinterpret_cast<const float4*>(a.slots + ((int64_t)((g + m) * nt + n) * a.tile_rows + part * 32) * kBN +
+                                                        (threadIdx.x >> 5) * 1024) + lane;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 x = q[i * 32];
+        v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
       }
-      *reinterpret_cast<uint4*>(a.out + (int64_t)(a.row_of ? a.row_of[r] : r) * s.N + c) = pack8(v);
+    }
+    if (r < M) {
+      __nv_bfloat16* out = a.out + (int64_t)(a.row_of ? a.row_of[r] : r) * s.N + c;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        if (c + i < s.N) *reinterpret_cast<uint4*>(out + i) = pack8(v + i);
     }
   }
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.zero_n; i += (int64_t)gridDim.x * 8)
     if (a.pos[i] < 0)
-      for (int x = (threadIdx.x & 31) * 8; x < s.N; x += 256)
+      for (int x = lane * 8; x < s.N; x += 256)
         *reinterpret_cast<uint4*>(a.out + i * s.N + x) = make_uint4(0, 0, 0, 0);
 }
 
@@ -563,7 +571,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
   const int64_t tiles = s.shares ? s.shares * tiles_n(s.N) : tiles_m(s.M, CG) * tiles_n(s.N);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, sm_count() / CG) * CG));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads_of<Epi>());
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

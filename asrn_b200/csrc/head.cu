@@ -23,9 +23,9 @@ namespace asrn {
 
 namespace {
 
-constexpr int kGatherRows = 128, kGatherThreads = 256;
+constexpr int kGatherRows = 64, kGatherThreads = 256;
 constexpr int kCountRows = 1024;
-constexpr int64_t kDirectRows = 32768;   // up to here each block counts the targets before it by itself: a launch less
+constexpr int64_t kDirectRows = 4096;    // up to here each block counts the targets before it by itself: a launch less
 constexpr float kLog2e = 1.4426950408889634f;
 
 int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kCountRows) k_head_count(int64_t N, const int6
   if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }
 
-// Block b takes positions [128 b, 128 b + 128): the targets before them (from the tokens, or from the counts of the
+// Block b takes positions [64 b, 64 b + 64): the targets before them (from the tokens, or from the counts of the
 // blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 256.
 __global__ void __launch_bounds__(kGatherThreads)
 k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ tokens,
@@ -113,8 +113,8 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
   const int64_t from = counts ? i0 / kCountRows * kCountRows : 0;
   if (counts)
     for (int64_t c = tid; c < i0 / kCountRows; c += kGatherThreads) before += counts[c];
-#pragma unroll 4
-  for (int64_t i = from + tid; i < i0; i += kGatherThreads) before += tokens[i] >= 0;
+#pragma unroll 8
+  for (int64_t i = from + tid; i < i0; i += kGatherThreads) before += __ldg(tokens + i) >= 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if (lane == 0) warps[wid] = before;
@@ -137,12 +137,12 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
     row[r] = (int)i;
   }
   __syncthreads();
-  const int nv = d / 8;
-  for (int k = wid; k < kGatherRows; k += kGatherThreads / 32) {
-    if (at[k] < 0) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(h + (i0 + k) * d);
-    uint4* dst = reinterpret_cast<uint4*>(hc + (int64_t)at[k] * d);
-    for (int c = lane; c < nv; c += 32) dst[c] = src[c];
+  const unsigned nv = d / 8;
+#pragma unroll 8
+  for (unsigned x = tid; x < kGatherRows * nv; x += kGatherThreads) {
+    const unsigned k = x / nv, c = x - k * nv;
+    if (at[k] >= 0)
+      reinterpret_cast<uint4*>(hc + (int64_t)at[k] * d)[c] = __ldg(reinterpret_cast<const uint4*>(h + (i0 + k) * d) + c);
   }
   if (i0 + kGatherRows >= N) {
     int total = before;
@@ -156,6 +156,7 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
 
 // Running maximum (of the unscaled scores) and sum of exponentials over the thread's columns.
 struct Lse {
+  static constexpr int kWarps = 8;
   struct Params {
     const int* tok;
     float k;                               // log2(e) / tau
@@ -171,7 +172,7 @@ struct Lse {
       : p(pp), row(r), V(sh.N), y(-1), at(u.n * 2 + half), on(r < rows) {
     if (on) y = p.tok[r];
   }
-  ASRN_DEV void chunk(float* v, int c, gemm::Out&, const CUtensorMap*, const CUtensorMap*) {
+  template <class O> ASRN_DEV void chunk(float* v, int c, O&, const CUtensorMap*, const CUtensorMap*) {
     if (c >= V) return;
     const int n = V - c, j = y - c;        // n: valid columns, 32 or more but in the last tile
     if (j >= 0 && j < 32) {
@@ -209,29 +210,51 @@ struct Lse {
   }
 };
 
-// Block = 32 positions x 8 warps over the halves of the vocabulary's tiles.
-__global__ void __launch_bounds__(256)
+// Block = 32 positions x 16 warps over the halves of the vocabulary's tiles, 8 at a time.
+constexpr int kJoinWarps = 16;
+__global__ void __launch_bounds__(kJoinWarps * 32)
 k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const int* __restrict__ pos,
             const int* __restrict__ tok, const float* __restrict__ top, const float2* __restrict__ part,
             float* __restrict__ lse2, float* __restrict__ rest, float* __restrict__ logp) {
-  __shared__ float2 sh[8][32];
+  __shared__ float2 sh[kJoinWarps][32];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + lane;
   const int r = i < N ? pos[i] : -1;
   float m = -INFINITY, s = 0.f;
-  auto join = [&](float2 q) {
-    if (q.y == 0.f) return;                // nothing there
-    const float t = fmaxf(m, q.x);
-    s = (m == t ? s : s * exp2f((m - t) * k)) + (q.x == t ? q.y : q.y * exp2f((q.x - t) * k));
+  auto join = [&](const float2* q, int n) {    // n of at most 8 pairs
+    float t = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t = j < n ? fmaxf(t, q[j].x) : t;
+    if (t == -INFINITY) return;                // nothing yet (a NaN in the sums comes with a NaN target score)
+    s *= exp2_fast((m - t) * k);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) s = fmaf(q[j].y, exp2_fast((q[j].x - t) * k), s);
     m = t;
   };
   if (r >= 0)
-#pragma unroll 4
-    for (int j = wid; j < halves; j += 8) join(part[j * pad + r]);
+    for (int j0 = wid; j0 < halves; j0 += 8 * kJoinWarps) {
+      float2 q[8];
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j * kJoinWarps < halves) {
+          q[j] = __ldg(part + (j0 + j * kJoinWarps) * pad + r);
+          n = j + 1;
+        }
+      join(q, n);
+    }
   sh[wid][lane] = make_float2(m, s);
   __syncthreads();
   if (wid || i >= N) return;
-  for (int w = 1; w < 8; ++w) join(sh[w][lane]);
+  m = -INFINITY;
+  s = 0.f;
+  for (int w = 0; w < kJoinWarps; w += 8) {
+    float2 q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = sh[w + j][lane];
+    join(q, 8);
+  }
   if (r < 0) {
     logp[i] = 0.f;
     return;
@@ -249,6 +272,7 @@ k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const in
 
 // dS of one chunk in bf16; the rows that pad the last tile get zeros.
 struct Slope {
+  static constexpr int kWarps = 16;
   struct Params {
     const int *tok, *row;                  // of the chunk's rows
     const float *lse2, *rest, *g;
@@ -266,7 +290,7 @@ struct Slope {
       own = -g * p.rest[r];
     }
   }
-  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
     if (c >= V) return;
     const gemm::F2 k2(p.k), off2(-off), g2(g);
 #pragma unroll
@@ -343,7 +367,7 @@ int asrn_head_forward(int64_t N, int64_t V, int32_t d, const void* h, const void
   Lse::Params p{tok, kLog2e * inv_tau, reinterpret_cast<float*>(W + ws.top), reinterpret_cast<float2*>(W + ws.part),
                 pad256(N)};
   if ((st = gemm::launch<false, false, Lse>(hc, d, weight, d, sh, p, s))) return st;
-  k_head_join<<<(unsigned)((N + 31) / 32), 256, 0, s>>>(N, (int)((V + gemm::kBN - 1) / gemm::kBN) * 2, p.pad, p.k,
+  k_head_join<<<(unsigned)((N + 31) / 32), kJoinWarps * 32, 0, s>>>(N, (int)((V + gemm::kBN - 1) / gemm::kBN) * 2, p.pad, p.k,
                                                         inv_tau, pos, tok, p.top, p.part,
                                                         reinterpret_cast<float*>(S + sv.lse2),
                                                         reinterpret_cast<float*>(S + sv.rest), logp);

@@ -56,11 +56,16 @@ ASRN_DEV void values4(float* v, uint32_t w, float scale) {
   gemm::mul2(gemm::add2(gemm::F2(f[2], f[3]), off), k).get(v[2], v[3]);
 }
 
-ASRN_DEV float abs_max32(const float* v) {     // a NaN is the largest
-  float m = v[0];
+// The larger magnitude, of either sign; a NaN is the largest.
+ASRN_DEV float abs_max(float a, float b) {
+  asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+  return a;
+}
+ASRN_DEV float abs_max32(const float* v) {
+  float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-  for (int i = 1; i < 32; ++i) asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(m) : "f"(v[i]));
-  return fabsf(m);
+  for (int i = 4; i < 32; ++i) m[i & 3] = abs_max(m[i & 3], v[i]);
+  return fabsf(abs_max(abs_max(m[0], m[1]), abs_max(m[2], m[3])));
 }
 
 // Of two values a: e = exp(-a^2 / 2) and q = Q(|a|), the normal distribution's tail, by Abramowitz and Stegun's 7.1.26,
@@ -83,10 +88,19 @@ ASRN_DEV void tails(float a0, float a1, gemm::F2& e, gemm::F2& q) {
   q = mul2(mul2(r, t), e);
 }
 
-// The codes of a block to `at` (n values of it, a multiple of 8); its exponent.
-ASRN_DEV int store_codes(const float* v, uint8_t* at, int n) {
+// The codes of a block to `at` (n values of it, a multiple of 8; wide: 16-byte stores fit); its exponent.
+ASRN_DEV int store_codes(const float* v, uint8_t* at, int n, bool wide) {
   const int e = block_exp(abs_max32(v));
   const float inv = inv_scale_of(e);
+  if (wide && n >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 16) {
+      uint4 w = make_uint4(codes4(v + i, inv), codes4(v + i + 4, inv), codes4(v + i + 8, inv), codes4(v + i + 12, inv));
+      if (e == kBad) w = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(at + i) = w;
+    }
+    return e;
+  }
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
     if (i < n) {
@@ -97,65 +111,83 @@ ASRN_DEV int store_codes(const float* v, uint8_t* at, int n) {
   return e;
 }
 
-// One thread per block of 32 of a row of bf16.
-__global__ void __launch_bounds__(256) k_pack8(int64_t blocks, int f, int per_row, const __nv_bfloat16* __restrict__ x,
-                                               uint8_t* __restrict__ codes, int8_t* __restrict__ exps) {
-  for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = b / per_row;
-    const int c = (int)(b % per_row) * 32;
-    const int64_t at = row * f + c;
-    float v[32];
+// Where the exponent of block b of a row stands: row * by_row + b * by_block. mlp8 keeps a block's rows side by side (32
+// rows at a time write and read them); pack8 a row's blocks.
+struct Exps {
+  int8_t* at;
+  int64_t by_row, by_block;
+  ASRN_DEV int8_t& operator()(int64_t row, int64_t block) const { return at[row * by_row + block * by_block]; }
+};
+
+// Four threads per block of 32 of a row of bf16, 8 values each.
+__global__ void __launch_bounds__(256) k_pack8(int64_t rows, int f, int wide, const __nv_bfloat16* __restrict__ x,
+                                               uint8_t* __restrict__ codes, const Exps exps) {
+  const int64_t total = rows * wide;                     // wide: threads per row, a multiple of 4
+  for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < total; t0 += (int64_t)gridDim.x * 256) {
+    const int64_t t = t0 + threadIdx.x;
+    const int64_t row = total < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)wide) : t / wide;
+    const int c = (int)(t - row * wide) * 8;
+    const bool in = t < total && c < f;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (in) q = __ldg(reinterpret_cast<const uint4*>(x + row * f + c));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float v[8], m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (c + i < f) q = *reinterpret_cast<const uint4*>(x + at + i);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[i + 2 * j] = __uint_as_float(w[j] << 16);
-        v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
     }
-    exps[b] = (int8_t)store_codes(v, codes + at, f - c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = abs_max(m, v[i]);
+    m = abs_max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fabsf(abs_max(m, __shfl_xor_sync(0xffffffffu, m, 2)));
+    const int e = block_exp(m);
+    const float inv = inv_scale_of(e);
+    if (!in) continue;
+    uint2 k = make_uint2(codes4(v, inv), codes4(v + 4, inv));
+    if (e == kBad) k = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(codes + row * f + c) = k;
+    if (c % 32 == 0) exps(row, c / 32) = (int8_t)e;
   }
 }
 
-// One thread per 8 values.
-ASRN_DEV void unpack_at(int64_t b, int f, const uint8_t* __restrict__ codes, const int8_t* __restrict__ exps,
+// One thread per 8 values: t of them along the rows, `per` to a row.
+ASRN_DEV void unpack_at(int64_t t, int64_t total, int f, const uint8_t* __restrict__ codes, const Exps& exps,
                         __nv_bfloat16* __restrict__ x) {
-  const int per = f / 8, per_row = (f + 31) / 32;
-  const int64_t row = b / per;
-  const int c = (int)(b % per) * 8;
-  const uint2 w = *reinterpret_cast<const uint2*>(codes + row * f + c);
-  const float scale = scale_of(exps[row * per_row + c / 32]);
+  const int per = f / 8;
+  const int64_t row = total < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)per) : t / per;
+  const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes) + t);
+  const float scale = scale_of(exps(row, (t - row * per) / 4));
   float v[8];
   values4(v, w.x, scale);
   values4(v + 4, w.y, scale);
-  *reinterpret_cast<uint4*>(x + row * f + c) = gemm::pack8(v);
+  reinterpret_cast<uint4*>(x)[t] = gemm::pack8(v);
 }
-__global__ void __launch_bounds__(256) k_unpack8(int64_t eighths, int f, const uint8_t* __restrict__ codes,
-                                                 const int8_t* __restrict__ exps, __nv_bfloat16* __restrict__ x) {
-  for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < eighths; b += (int64_t)gridDim.x * blockDim.x)
-    unpack_at(b, f, codes, exps, x);
+__global__ void __launch_bounds__(256) k_unpack8(int64_t total, int f, const uint8_t* __restrict__ codes, const Exps exps,
+                                                 __nv_bfloat16* __restrict__ x) {
+#pragma unroll 2
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256)
+    unpack_at(t, total, f, codes, exps, x);
 }
 
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
 struct Up {
+  static constexpr int kWarps = 16;
   struct Params {
     const __nv_bfloat16* bias;
     uint8_t* codes;
-    int8_t* exps;
+    Exps exps;
   };
   const Params& p;
-  int64_t at, eat;
-  int N, first;
+  int64_t at;
+  int N, row, first;
   bool on;
-  ASRN_DEV Up(const Params& pp, int row, int rows, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)row * s.N), eat((int64_t)row * ((s.N + 31) / 32)), N(s.N), first(row & ~31), on(row < rows) {}
-  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap*) {
+  ASRN_DEV Up(const Params& pp, int r, int rows, const gemm::Shape& s, const gemm::Tile&, int)
+      : p(pp), at((int64_t)r * s.N), N(s.N), row(r), first(r & ~31), on(r < rows) {}
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
     if (c >= N) return;                        // the columns past N of the last block are zeros
     gemm::add_bias(v, p.bias + c, N - c);
-    if (p.codes && on) p.exps[eat + c / 32] = (int8_t)store_codes(v, p.codes + at + c, N - c);
+    if (p.codes && on) p.exps(row, c / 32) = (int8_t)store_codes(v, p.codes + at + c, N - c, N % 16 == 0);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       gemm::F2 e, q;
@@ -184,28 +216,41 @@ ASRN_DEV float column_sum(float* v, int lane) {
 
 // dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows.
 struct Down {
+  static constexpr int kWarps = 16;
   struct Params {
     const uint8_t* codes;
-    const int8_t* exps;
+    Exps exps;
     float* sums;                               // [ceil(rows / 32)][N], or null
   };
   const Params& p;
-  int64_t at, eat;
-  int N, first, rows;
+  int64_t at;
+  int N, row, first, rows;
   bool on;
   ASRN_DEV Down(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)r * s.N), eat((int64_t)r * ((s.N + 31) / 32)), N(s.N), first(r & ~31), rows(m), on(r < m) {}
-  ASRN_DEV void chunk(float* v, int c, gemm::Out& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
+      : p(pp), at((int64_t)r * s.N), N(s.N), row(r), first(r & ~31), rows(m), on(r < m) {}
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
     using gemm::F2;
     if (c >= N) return;                        // the same for the whole warp
-    const float scale = on ? scale_of(p.exps[eat + c / 32]) : 0.f;
+    const float scale = on ? scale_of(p.exps(row, c / 32)) : 0.f;
     float g[32];
+    if (N % 16 == 0 && c + 32 <= N) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint2 w = make_uint2(0, 0);
-      if (on && c + i < N) w = *reinterpret_cast<const uint2*>(p.codes + at + c + i);
-      values4(g + i, w.x, scale);
-      values4(g + i + 4, w.y, scale);
+      for (int i = 0; i < 32; i += 16) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (on) w = __ldg(reinterpret_cast<const uint4*>(p.codes + at + c + i));
+        values4(g + i, w.x, scale);
+        values4(g + i + 4, w.y, scale);
+        values4(g + i + 8, w.z, scale);
+        values4(g + i + 12, w.w, scale);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        uint2 w = make_uint2(0, 0);
+        if (on && c + i < N) w = __ldg(reinterpret_cast<const uint2*>(p.codes + at + c + i));
+        values4(g + i, w.x, scale);
+        values4(g + i + 4, w.y, scale);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
@@ -231,26 +276,44 @@ struct Down {
 };
 
 // x' from its codes (the first `unpackers` blocks), and sums of dY's columns over 64 rows (the others: block = 64 rows x
-// 256 columns, thread = column).
+// 256 columns, a lane 8 columns, a warp every eighth row).
 constexpr int kColRows = 64;
 __global__ void __launch_bounds__(256)
-k_prepare(int unpackers, int64_t eighths, int d, const uint8_t* __restrict__ codes, const int8_t* __restrict__ exps,
+k_prepare(int unpackers, int64_t eighths, int d, const uint8_t* __restrict__ codes, const Exps exps,
           __nv_bfloat16* __restrict__ x, int64_t rows, int n, const __nv_bfloat16* __restrict__ dy,
           float* __restrict__ sums) {
+  __shared__ float sh[8][256];
   if ((int)blockIdx.x < unpackers) {
-    for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < eighths; b += (int64_t)unpackers * 256)
-      unpack_at(b, d, codes, exps, x);
+#pragma unroll 2
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < eighths; t += (int64_t)unpackers * 256)
+      unpack_at(t, eighths, d, codes, exps, x);
     return;
   }
-  const int wide = (n + 255) / 256, block = blockIdx.x - unpackers;
-  const int c = block % wide * 256 + threadIdx.x;
-  if (c >= n) return;
+  const int wide = (n + 255) / 256, block = blockIdx.x - unpackers, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int c0 = block % wide * 256, c = c0 + lane * 8;
   const int64_t r0 = (int64_t)(block / wide) * kColRows;
-  const int64_t r1 = r0 + kColRows < rows ? r0 + kColRows : rows;
-  float s = 0.f;
-#pragma unroll 16
-  for (int64_t r = r0; r < r1; ++r) s += __bfloat162float(dy[r * n + c]);
-  sums[(int64_t)(block / wide) * n + c] = s;
+  float s[8] = {};
+#pragma unroll
+  for (int k = 0; k < kColRows / 8; ++k) {
+    const int64_t r = r0 + k * 8 + wid;
+    if (r < rows && c < n) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(dy + r * n + c));
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[2 * j] += __uint_as_float(w[j] << 16);
+        s[2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[wid][lane + 32 * j] = s[j];
+  __syncthreads();
+  const int own = c0 + lane * 8 + wid;                   // this thread's column: its lane's wid-th
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) t += sh[k][threadIdx.x];
+  if (own < n) sums[(int64_t)(block / wide) * n + own] = t;
 }
 
 // out[c] = bf16(sum of the parts' [..][c]) in order, for two sets: block = 32 columns x 32 warps.
@@ -330,17 +393,13 @@ int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_C
 
 unsigned grid_for(int64_t threads) { return (unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 16); }
 
-int pack8(int64_t rows, int f, const void* x, void* codes, void* exps, cudaStream_t s) {
-  const int64_t blocks = rows * ((f + 31) / 32);
-  k_pack8<<<grid_for(blocks), 256, 0, s>>>(blocks, f, (f + 31) / 32, reinterpret_cast<const __nv_bfloat16*>(x),
-                                           reinterpret_cast<uint8_t*>(codes), reinterpret_cast<int8_t*>(exps));
-  return launched();
-}
+Exps by_rows(const void* p, int f) { return Exps{(int8_t*)p, (f + 31) / 32, 1}; }
+Exps by_blocks(const void* p, int64_t rows) { return Exps{(int8_t*)p, 1, rows}; }
 
-int unpack8(int64_t rows, int f, const void* codes, const void* exps, void* x, cudaStream_t s) {
-  k_unpack8<<<grid_for(rows * (f / 8)), 256, 0, s>>>(rows * (f / 8), f, reinterpret_cast<const uint8_t*>(codes),
-                                                     reinterpret_cast<const int8_t*>(exps),
-                                                     reinterpret_cast<__nv_bfloat16*>(x));
+int pack8(int64_t rows, int f, const void* x, void* codes, const Exps& exps, cudaStream_t s) {
+  const int wide = (f + 31) / 32 * 4;
+  k_pack8<<<grid_for(rows * wide), 256, 0, s>>>(rows, f, wide, reinterpret_cast<const __nv_bfloat16*>(x),
+                                                reinterpret_cast<uint8_t*>(codes), exps);
   return launched();
 }
 
@@ -366,7 +425,7 @@ int asrn_pack8(int64_t rows, int32_t f, const void* x, void* codes, void* exps, 
   if (f % 8) return ASRN_ERR_UNSUPPORTED;
   if (rows == 0) return ASRN_OK;
   if (!x || !codes || !exps || (uintptr_t)x % 16 || (uintptr_t)codes % 8) return ASRN_ERR_ARG;
-  return pack8(rows, f, x, codes, exps, reinterpret_cast<cudaStream_t>(stream));
+  return pack8(rows, f, x, codes, by_rows(exps, f), reinterpret_cast<cudaStream_t>(stream));
 }
 
 int asrn_unpack8(int64_t rows, int32_t f, const void* codes, const void* exps, void* x, void* stream) {
@@ -375,7 +434,9 @@ int asrn_unpack8(int64_t rows, int32_t f, const void* codes, const void* exps, v
   if (f % 8) return ASRN_ERR_UNSUPPORTED;
   if (rows == 0) return ASRN_OK;
   if (!x || !codes || !exps || (uintptr_t)x % 16 || (uintptr_t)codes % 8) return ASRN_ERR_ARG;
-  return unpack8(rows, f, codes, exps, x, reinterpret_cast<cudaStream_t>(stream));
+  k_unpack8<<<grid_for(rows * (f / 8)), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      rows * (f / 8), f, reinterpret_cast<const uint8_t*>(codes), by_rows(exps, f), reinterpret_cast<__nv_bfloat16*>(x));
+  return launched();
 }
 
 size_t asrn_mlp8_saved_bytes(int64_t N, int32_t d, int32_t ff) {
@@ -406,11 +467,11 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* S = reinterpret_cast<char*>(saved);
   __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(workspace) + ws.g);
-  if (S && (st = pack8(N, d, x, S + sv.xc, S + sv.xe, s))) return st;
+  if (S && (st = pack8(N, d, x, S + sv.xc, by_blocks(S + sv.xe, N), s))) return st;
   gemm::Shape a{};
   a.M = (int)N; a.N = ff; a.K = d; a.group = 16; a.status = status;
   const Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
-                     S ? reinterpret_cast<int8_t*>(S + sv.ae) : nullptr};
+                     S ? by_blocks(S + sv.ae, N) : Exps{}};
   if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s, {g, N, ff, ff}))) return st;
   a.N = dout; a.K = ff;
   return gemm::launch<false, false, gemm::StoreBf16>(g, ff, w2, ff, a,
@@ -456,14 +517,13 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
     const unsigned summers = db2 ? (unsigned)(blocks * ((dout + 255) / 256)) : 0;
     k_prepare<<<unpackers + summers, 256, 0, s>>>(
         (int)unpackers, eighths, d, reinterpret_cast<const uint8_t*>(S + sv.xc),
-        reinterpret_cast<const int8_t*>(S + sv.xe), reinterpret_cast<__nv_bfloat16*>(W + ws.x), N, dout,
+        by_blocks(S + sv.xe, N), reinterpret_cast<__nv_bfloat16*>(W + ws.x), N, dout,
         reinterpret_cast<const __nv_bfloat16*>(dy), sum2);
     if ((st = launched())) return st;
   }
   if (dx || dw1 || db1 || dw2) {
     a.N = ff; a.K = dout;
-    const Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), reinterpret_cast<const int8_t*>(S + sv.ae),
-                         db1 ? sum1 : nullptr};
+    const Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), by_blocks(S + sv.ae, N), db1 ? sum1 : nullptr};
     if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s, {da, N, ff, ff}, {g, N, ff, ff}))) return st;
   }
   if (dx) {
