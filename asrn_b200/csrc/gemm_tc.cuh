@@ -35,11 +35,12 @@ template <class Epi> constexpr int threads_of() { return (2 + Epi::kWarps) * 32;
 constexpr int kBytesA = kBM * 128;                       // one block's share of a stage
 template <int CG> constexpr int bytes_b() { return kBN / CG * 128; }
 template <int CG> constexpr int stage_bytes() { return kBytesA + bytes_b<CG>(); }
-template <int CG> constexpr int stages() { return CG == 1 ? 4 : 6; }
+// Pieces of shared memory for results: two per warp of eight; sixteen warps share as many unless the epilogue has two
+// results (kOwn = 2), which costs a stage.
+template <int CG, class Epi> constexpr int stages() { return (CG == 1 ? 4 : 6) - (Epi::kWarps * Epi::kOwn > 16); }
 constexpr int kPiece = 32 * 64;                          // 32 rows x 32 bf16 columns, 64-byte swizzle
-constexpr int kPieces = 16 * kPiece;                     // 2 per warp, or 1 where there are 16 warps
-template <int CG> constexpr size_t smem_bytes() {
-  return 1024 + (size_t)stages<CG>() * stage_bytes<CG>() + kPieces + 256;
+template <int CG, class Epi> constexpr size_t smem_bytes() {
+  return 1024 + (size_t)stages<CG, Epi>() * stage_bytes<CG>() + Epi::kWarps * Epi::kOwn * kPiece + 256;
 }
 
 struct Shape {
@@ -224,13 +225,19 @@ template <int Pieces> struct Out {
   uint8_t* piece;                                        // the warp's own
   int lane, turn;
   ASRN_DEV void put(const CUtensorMap* map, const float* v, int column, int first_row) {
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack8(v + 8 * i);
+    put(map, w, column, first_row);
+  }
+  ASRN_DEV void put(const CUtensorMap* map, const uint4* w, int column, int first_row) {
     uint8_t* at = piece + turn * kPiece;
     turn = (turn + 1) % Pieces;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Pieces - 1) : "memory");
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = pack8(v + 8 * i);
+      *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = w[i];
     umma::fence_proxy_async();
     __syncwarp();
     if (lane == 0) {
@@ -245,7 +252,7 @@ template <int Pieces> struct Out {
   }
 };
 
-// Epi: struct with a Params type, kWarps (8 or 16), a constructor (Params, row, rows, shape, tile, the warp's part of the columns) and chunk(v[32],
+// Epi: struct with a Params type, kWarps (8 or 16), kOwn (pieces per warp), a constructor (Params, row, rows, shape, tile, the warp's part of the columns) and chunk(v[32],
 // column, Out, map_o, map_p), called by whole warps for the tile's chunks of 32 columns, then finish().
 template <int CG, bool AMn, bool BMn, class Epi>
 __global__ void __launch_bounds__(threads_of<Epi>(), 1)
@@ -256,11 +263,11 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sm = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  constexpr int kS = stages<CG>(), kStageB = bytes_b<CG>();
+  constexpr int kS = stages<CG, Epi>(), kStageB = bytes_b<CG>();
   uint8_t* sA = sm;
   uint8_t* sB = sm + kS * kBytesA;
   uint8_t* sO = sB + kS * kStageB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sO + kPieces);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sO + Epi::kWarps * Epi::kOwn * kPiece);
   uint64_t* empty = full + kS;
   uint64_t* tfull = empty + kS;
   uint64_t* tempty = tfull + 2;
@@ -345,7 +352,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       }
     }
   } else {                                              // epilogue
-    constexpr int kCols = kBN * 4 / Epi::kWarps, kOwn = 16 / Epi::kWarps;
+    constexpr int kCols = kBN * 4 / Epi::kWarps, kOwn = Epi::kOwn;
     const int q4 = wid & 3, part = (wid - 2) >> 2;
     Out<kOwn> out{sO + (wid - 2) * kOwn * kPiece, lane, 0};
     const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(part * kCols);
@@ -409,7 +416,7 @@ ASRN_DEV void add_bias(float* v, const __nv_bfloat16* bias, int n) {
 // The fp32 sums of a piece of a tile, whole, to its slot: by blocks of 32 rows x 32 columns, each as the warp holds it
 // (four columns of all 32 rows are 512 neighbouring bytes).
 struct StorePiece {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = 8, kOwn = 2;
   struct Params {
     float* slots;
     int tile_rows;
@@ -429,7 +436,7 @@ struct StorePiece {
 // bf16(sum + bias + before): out[row][column] through map_o (N a multiple of 8). before: fp32 (M, N), the sum of what
 // came earlier; or, when `after` is given, the sum goes there in fp32 instead.
 struct StoreBf16 {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = 8, kOwn = 2;
   struct Params {
     const __nv_bfloat16* bias;
     const float* before;
@@ -559,7 +566,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
       (q.base && !make_tmap_bf16_sw64(&mq, q.base, (uint64_t)q.columns, (uint64_t)q.rows, (uint64_t)q.pitch * 2, 32, 32)))
     return ASRN_ERR_CUDA;
   auto kernel = k_gemm<CG, AMn, BMn, Epi>;
-  constexpr size_t smem = smem_bytes<CG>();
+  constexpr size_t smem = smem_bytes<CG, Epi>();
   static std::atomic<uint64_t> ready{0};                  // devices that know the kernel's shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return ASRN_ERR_CUDA;

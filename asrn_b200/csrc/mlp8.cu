@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256) k_unpack8(int64_t total, int f, const uin
 
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
 struct Up {
-  static constexpr int kWarps = 16;
+  static constexpr int kWarps = 16, kOwn = 1;
   struct Params {
     const __nv_bfloat16* bias;
     uint8_t* codes;
@@ -216,7 +216,7 @@ ASRN_DEV float column_sum(float* v, int lane) {
 
 // dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows.
 struct Down {
-  static constexpr int kWarps = 16;
+  static constexpr int kWarps = 16, kOwn = 2;
   struct Params {
     const uint8_t* codes;
     Exps exps;
@@ -232,40 +232,42 @@ struct Down {
     using gemm::F2;
     if (c >= N) return;                        // the same for the whole warp
     const float scale = on ? scale_of(p.exps(row, c / 32)) : 0.f;
-    float g[32];
-    if (N % 16 == 0 && c + 32 <= N) {
+    uint4 codes[2] = {};
+    if (on) {
+      const uint8_t* at_c = p.codes + at + c;
+      if (N % 16 == 0 && c + 32 <= N) {
+        codes[0] = __ldg(reinterpret_cast<const uint4*>(at_c));
+        codes[1] = __ldg(reinterpret_cast<const uint4*>(at_c) + 1);
+      } else {
+        uint2* w = reinterpret_cast<uint2*>(codes);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (on) w = __ldg(reinterpret_cast<const uint4*>(p.codes + at + c + i));
-        values4(g + i, w.x, scale);
-        values4(g + i + 4, w.y, scale);
-        values4(g + i + 8, w.z, scale);
-        values4(g + i + 12, w.w, scale);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        uint2 w = make_uint2(0, 0);
-        if (on && c + i < N) w = __ldg(reinterpret_cast<const uint2*>(p.codes + at + c + i));
-        values4(g + i, w.x, scale);
-        values4(g + i + 4, w.y, scale);
+        for (int i = 0; i < 4; ++i)
+          if (c + 8 * i < N) w[i] = __ldg(reinterpret_cast<const uint2*>(at_c) + i);
       }
     }
+    uint4 packed[4];
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float a0 = g[i], a1 = g[i + 1];
-      F2 e, q;
-      tails(a0, a1, e, q);
-      float h0, h1;
-      gemm::fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                             // 1/2 - q
-      const F2 cdf = gemm::add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
-      const F2 slope = gemm::fma2(gemm::mul2(F2(a0, a1), F2(0.39894228040143268f)), e, cdf);
-      gemm::mul2(F2(v[i], v[i + 1]), slope).get(v[i], v[i + 1]);
-      gemm::fma2(F2(-fabsf(a0), -fabsf(a1)), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(g[i], g[i + 1]);
+    for (int i = 0; i < 32; i += 8) {
+      const uint4& k = codes[i / 16];
+      float g[8];
+      values4(g, i % 16 ? k.z : k.x, scale);
+      values4(g + 4, i % 16 ? k.w : k.y, scale);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float a0 = g[j], a1 = g[j + 1];
+        F2 e, q;
+        tails(a0, a1, e, q);
+        float h0, h1;
+        gemm::fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                           // 1/2 - q
+        const F2 cdf = gemm::add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
+        const F2 slope = gemm::fma2(gemm::mul2(F2(a0, a1), F2(0.39894228040143268f)), e, cdf);
+        gemm::mul2(F2(v[i + j], v[i + j + 1]), slope).get(v[i + j], v[i + j + 1]);
+        gemm::fma2(F2(-fabsf(a0), -fabsf(a1)), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(g[j], g[j + 1]);
+      }
+      packed[i / 8] = gemm::pack8(g);
     }
+    out.put(map_p, packed, c, first);
     out.put(map_o, v, c, first);
-    out.put(map_p, g, c, first);
     if (p.sums && first < rows) {              // rows past the end are zeros: the operand's rows were
       const int lane = threadIdx.x & 31;
       const float s = column_sum(v, lane);
