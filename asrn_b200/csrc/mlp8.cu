@@ -119,55 +119,83 @@ struct Exps {
   ASRN_DEV int8_t& operator()(int64_t row, int64_t block) const { return at[row * by_row + block * by_block]; }
 };
 
-// Four threads per block of 32 of a row of bf16, 8 values each.
+// t = row * wide + the rest, in 32 bits where `all` of them fit.
+ASRN_DEV int64_t row_of(int64_t t, int64_t all, int wide) {
+  return all < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)wide) : t / wide;
+}
+
+// Four threads per block of 32 of a row of bf16, 8 values each; each thread kEach of them, all loaded first.
+constexpr int kEach = 4;
 __global__ void __launch_bounds__(256) k_pack8(int64_t rows, int f, int wide, const __nv_bfloat16* __restrict__ x,
                                                uint8_t* __restrict__ codes, const Exps exps) {
   const int64_t total = rows * wide;                     // wide: threads per row, a multiple of 4
-  for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < total; t0 += (int64_t)gridDim.x * 256) {
-    const int64_t t = t0 + threadIdx.x;
-    const int64_t row = total < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)wide) : t / wide;
-    const int c = (int)(t - row * wide) * 8;
-    const bool in = t < total && c < f;
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (in) q = __ldg(reinterpret_cast<const uint4*>(x + row * f + c));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    float v[8], m = 0.f;
+  for (int64_t t0 = (int64_t)blockIdx.x * 256 * kEach; t0 < total; t0 += (int64_t)gridDim.x * 256 * kEach) {
+    uint4 q[kEach];
+    int64_t row[kEach];
+    int c[kEach];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    for (int k = 0; k < kEach; ++k) {
+      const int64_t t = t0 + k * 256 + threadIdx.x;
+      row[k] = row_of(t, total, wide);
+      c[k] = (int)(t - row[k] * wide) * 8;
+      if (t >= total) c[k] = f;
+      q[k] = make_uint4(0, 0, 0, 0);
+      if (c[k] < f) q[k] = __ldg(reinterpret_cast<const uint4*>(x + row[k] * f + c[k]));
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = abs_max(m, v[i]);
-    m = abs_max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fabsf(abs_max(m, __shfl_xor_sync(0xffffffffu, m, 2)));
-    const int e = block_exp(m);
-    const float inv = inv_scale_of(e);
-    if (!in) continue;
-    uint2 k = make_uint2(codes4(v, inv), codes4(v + 4, inv));
-    if (e == kBad) k = make_uint2(0, 0);
-    *reinterpret_cast<uint2*>(codes + row * f + c) = k;
-    if (c % 32 == 0) exps(row, c / 32) = (int8_t)e;
+    for (int k = 0; k < kEach; ++k) {
+      const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+      float v[8], m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = abs_max(m, v[i]);
+      m = abs_max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fabsf(abs_max(m, __shfl_xor_sync(0xffffffffu, m, 2)));
+      const int e = block_exp(m);
+      const float inv = inv_scale_of(e);
+      if (c[k] >= f) continue;
+      uint2 o = make_uint2(codes4(v, inv), codes4(v + 4, inv));
+      if (e == kBad) o = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(codes + row[k] * f + c[k]) = o;
+      if (c[k] % 32 == 0) exps(row[k], c[k] / 32) = (int8_t)e;
+    }
   }
 }
 
-// One thread per 8 values: t of them along the rows, `per` to a row.
-ASRN_DEV void unpack_at(int64_t t, int64_t total, int f, const uint8_t* __restrict__ codes, const Exps& exps,
-                        __nv_bfloat16* __restrict__ x) {
+// 8 values per thread and turn, kEach turns loaded first; `blocks` blocks, this one the `block`-th.
+ASRN_DEV void unpack(int64_t block, int64_t blocks, int64_t total, int f, const uint8_t* __restrict__ codes,
+                     const Exps& exps, __nv_bfloat16* __restrict__ x) {
   const int per = f / 8;
-  const int64_t row = total < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)per) : t / per;
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes) + t);
-  const float scale = scale_of(exps(row, (t - row * per) / 4));
-  float v[8];
-  values4(v, w.x, scale);
-  values4(v + 4, w.y, scale);
-  reinterpret_cast<uint4*>(x)[t] = gemm::pack8(v);
+  for (int64_t t0 = block * 256 * kEach; t0 < total; t0 += blocks * 256 * kEach) {
+    uint2 w[kEach];
+    int e[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int64_t t = t0 + k * 256 + threadIdx.x;
+      if (t >= total) break;
+      const int64_t row = row_of(t, total, per);
+      w[k] = __ldg(reinterpret_cast<const uint2*>(codes) + t);
+      e[k] = exps(row, (t - row * per) / 4);
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int64_t t = t0 + k * 256 + threadIdx.x;
+      if (t >= total) break;
+      const float scale = scale_of(e[k]);
+      float v[8];
+      values4(v, w[k].x, scale);
+      values4(v + 4, w[k].y, scale);
+      reinterpret_cast<uint4*>(x)[t] = gemm::pack8(v);
+    }
+  }
 }
 __global__ void __launch_bounds__(256) k_unpack8(int64_t total, int f, const uint8_t* __restrict__ codes, const Exps exps,
                                                  __nv_bfloat16* __restrict__ x) {
-#pragma unroll 2
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256)
-    unpack_at(t, total, f, codes, exps, x);
+  unpack(blockIdx.x, gridDim.x, total, f, codes, exps, x);
 }
 
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
@@ -262,7 +290,7 @@ struct Down {
         const F2 cdf = gemm::add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
         const F2 slope = gemm::fma2(gemm::mul2(F2(a0, a1), F2(0.39894228040143268f)), e, cdf);
         gemm::mul2(F2(v[i + j], v[i + j + 1]), slope).get(v[i + j], v[i + j + 1]);
-        gemm::fma2(F2(-fabsf(a0), -fabsf(a1)), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(g[j], g[j + 1]);
+        gemm::mul2(F2(a0, a1), cdf).get(g[j], g[j + 1]);
       }
       packed[i / 8] = gemm::pack8(g);
     }
@@ -286,9 +314,7 @@ k_prepare(int unpackers, int64_t eighths, int d, const uint8_t* __restrict__ cod
           float* __restrict__ sums) {
   __shared__ float sh[8][256];
   if ((int)blockIdx.x < unpackers) {
-#pragma unroll 2
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < eighths; t += (int64_t)unpackers * 256)
-      unpack_at(t, eighths, d, codes, exps, x);
+    unpack(blockIdx.x, unpackers, eighths, d, codes, exps, x);
     return;
   }
   const int wide = (n + 255) / 256, block = blockIdx.x - unpackers, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -393,7 +419,9 @@ int check_mlp8(int64_t N, int32_t d, int32_t ff, int32_t dout) {
 
 int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
 
-unsigned grid_for(int64_t threads) { return (unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 16); }
+unsigned grid_for(int64_t threads) {
+  return (unsigned)std::min<int64_t>((threads + 256 * kEach - 1) / (256 * kEach), 148 * 16);
+}
 
 Exps by_rows(const void* p, int f) { return Exps{(int8_t*)p, (f + 31) / 32, 1}; }
 Exps by_blocks(const void* p, int64_t rows) { return Exps{(int8_t*)p, 1, rows}; }

@@ -17,6 +17,7 @@ and r.loss.backward() works as well when logp requires a gradient. Everything ru
 stream, and repeats bit for bit; there is no counterpart in the reference.
 """
 from collections import namedtuple
+from functools import lru_cache
 
 import torch
 
@@ -78,6 +79,12 @@ def _rows(t):
     return t if t.data_ptr() % 16 == 0 else t.detach().clone()
 
 
+@lru_cache(1024)
+def _bytes(name, *sizes):
+    """A size query of the library (a pure function of the sizes)."""
+    return getattr(_lib.lib(), name)(*sizes)
+
+
 def _scratch(nbytes, dev):
     return torch.empty(nbytes or 256, dtype=torch.uint8, device=dev)
 
@@ -87,11 +94,11 @@ def _scratch(nbytes, dev):
 class _HeadLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, tokens, tau):
-        d, V, N = h.shape[-1], w.shape[0], tokens.numel()
-        dev, lib = h.device, _lib.lib()
+        V, d = w.shape
+        N, dev, lib = tokens.numel(), h.device, _lib.lib()
         hr, wr, tok = _rows(h), _rows(w), tokens.contiguous()
         out = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-        nb_saved, nb = lib.asrn_head_saved_bytes(N, d), lib.asrn_head_workspace_bytes(N, V, d, 0)
+        nb_saved, nb = _bytes('asrn_head_saved_bytes', N, d), _bytes('asrn_head_workspace_bytes', N, V, d, 0)
         saved, ws = _scratch(nb_saved, dev), _scratch(nb, dev)
         _lib.check(lib.asrn_head_forward(N, V, d, hr.data_ptr(), wr.data_ptr(), tok.data_ptr(), tau, out.data_ptr(),
                                          saved.data_ptr(), nb_saved, ws.data_ptr(), nb, _status_word(dev),
@@ -109,7 +116,7 @@ class _HeadLogprobs(torch.autograd.Function):
         dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if need[0] else None
         dw = torch.empty((V, d), dtype=torch.bfloat16, device=dev) if need[1] else None
         g32 = _f32(g)
-        nb = lib.asrn_head_workspace_bytes(N, V, d, 1)
+        nb = _bytes('asrn_head_workspace_bytes', N, V, d, 1)
         ws = _scratch(nb, dev)
         _lib.check(lib.asrn_head_backward(N, V, d, w.data_ptr(), saved.data_ptr(), nb_saved, tau, g32.data_ptr(),
                                           _p(dh), _p(dw), ws.data_ptr(), nb, _status_word(dev), _stream(dev)),
@@ -123,7 +130,10 @@ def _autocast_bf16():
 
 def _bf16(what, *ts):
     """The operands in bf16: as they are, or cast as autocast casts a linear layer's operands."""
-    if all(t.dtype == torch.bfloat16 for t in ts):
+    for t in ts:
+        if t.dtype is not torch.bfloat16:
+            break
+    else:
         return ts
     if not _autocast_bf16():
         raise NotImplementedError(f'{what} computes in bfloat16: pass bfloat16 tensors or call it under '
@@ -137,17 +147,18 @@ def head_logprobs(h, weight, tokens, temperatura=1.0):
     """log softmax(h weight^T / temperatura) at tokens: h (..., d), weight (V, d) bfloat16 (or float32 under bf16
     autocast), tokens (...) int64 -> float32 (...), differentiable in h and weight. A negative token leaves its
     position out (0, no gradient, none of the work); a token >= V gives NaN. d has to be a multiple of 8."""
-    if h.dim() < 1 or weight.dim() != 2 or h.shape[-1] != weight.shape[1] or tokens.shape != h.shape[:-1]:
+    sh, sw = h.shape, weight.shape
+    if not sh or len(sw) != 2 or sh[-1] != sw[1] or tokens.shape != sh[:-1]:
         raise ValueError(f'head_logprobs: h (..., d), weight (V, d) and tokens (...) do not fit: {tuple(h.shape)}, '
                          f'{tuple(weight.shape)}, {tuple(tokens.shape)}')
-    if tokens.dtype != torch.int64:
+    if tokens.dtype is not torch.int64:
         raise TypeError('head_logprobs: tokens are int64')
     if not 0 < temperatura <= 1e30:
         raise ValueError('head_logprobs: temperatura has to be positive')
     _need_cuda('head_logprobs', h, weight, tokens)
     h, weight = _bf16('head_logprobs', h, weight)
-    if h.shape[-1] % 8:
-        raise NotImplementedError(f'head_logprobs: the width ({h.shape[-1]}) has to be a multiple of 8')
+    if sh[-1] % 8:
+        raise NotImplementedError(f'head_logprobs: the width ({sh[-1]}) has to be a multiple of 8')
     return _HeadLogprobs.apply(h, weight, tokens, float(temperatura))
 
 
@@ -207,7 +218,7 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
     m = _mask(mask, logp.shape, 'preference_loss')
     _, P, L = logp.shape
     lp, rf = _f32(logp), _f32(ref_logp)
-    nb = lib.asrn_preference_workspace_bytes(P, L)
+    nb = _bytes('asrn_preference_workspace_bytes', P, L)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
     grad = torch.empty((2, P, L), dtype=torch.float32, device=dev)
@@ -247,7 +258,7 @@ def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2)
     ref = None if ref_logp is None else _f32(ref_logp)
     out = torch.empty(3, dtype=torch.float32, device=dev)
     grad = torch.empty((B, L), dtype=torch.float32, device=dev)
-    nb = lib.asrn_policy_workspace_bytes(B, L)
+    nb = _bytes('asrn_policy_workspace_bytes', B, L)
     ws = _scratch(nb, dev) if nb else None
     base = out.data_ptr()
     _lib.check(lib.asrn_policy_loss(B, L, lp.data_ptr(), old.data_ptr(), _p(ref), adv.data_ptr(), adv.dim() == 2,
@@ -299,8 +310,8 @@ class _Mlp8(torch.autograd.Function):
         xr, w1, b1, w2, b2 = _rows(x), _rows(w1), _rows(b1), _rows(w2), _rows(b2)
         y = torch.empty((*x.shape[:-1], dout), dtype=torch.bfloat16, device=dev)
         keep = any(ctx.needs_input_grad)
-        nb_saved = lib.asrn_mlp8_saved_bytes(N, d, ff) if keep else 0
-        nb = lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 0)
+        nb_saved = _bytes('asrn_mlp8_saved_bytes', N, d, ff) if keep else 0
+        nb = _bytes('asrn_mlp8_workspace_bytes', N, d, ff, dout, 0)
         saved = _scratch(nb_saved, dev) if keep else None
         ws = _scratch(nb, dev)
         _lib.check(lib.asrn_mlp8_forward(N, d, ff, dout, xr.data_ptr(), w1.data_ptr(), b1.data_ptr(), w2.data_ptr(),
@@ -320,7 +331,7 @@ class _Mlp8(torch.autograd.Function):
         out = [torch.empty(s, dtype=torch.bfloat16, device=dev) if n else None
                for s, n in zip(sizes, ctx.needs_input_grad)]
         dyr = _rows(dy)
-        nb = lib.asrn_mlp8_workspace_bytes(N, d, ff, dout, 1)
+        nb = _bytes('asrn_mlp8_workspace_bytes', N, d, ff, dout, 1)
         ws = _scratch(nb, dev)
         _lib.check(lib.asrn_mlp8_backward(N, d, ff, dout, dyr.data_ptr(), w1.data_ptr(), w2.data_ptr(),
                                           saved.data_ptr(), nb_saved, *[_p(t) for t in out], ws.data_ptr(), nb,
@@ -333,12 +344,12 @@ def mlp8(x, w1, b1, w2, b2):
     under bf16 autocast) -> bfloat16 (..., dout). For the backward pass it keeps x and x w1^T + b1 in 8 bits (pack8's
     form: (d + ff) 33 / 32 bytes a row), and the gradients are those of the values so kept. d, ff and dout have to be
     multiples of 8."""
-    d = x.shape[-1] if x.dim() else 0
-    if w1.dim() != 2 or w2.dim() != 2 or w1.shape[1] != d or b1.shape != w1.shape[:1] or \
-            w2.shape[1] != w1.shape[0] or b2.shape != w2.shape[:1]:
+    sx, s1, s2 = x.shape, w1.shape, w2.shape
+    if not sx or len(s1) != 2 or len(s2) != 2 or s1[1] != sx[-1] or b1.shape != s1[:1] or s2[1] != s1[0] or \
+            b2.shape != s2[:1]:
         raise ValueError('mlp8: x (..., d), w1 (ff, d), b1 (ff), w2 (dout, ff), b2 (dout) do not fit: ' + ', '.join(
             str(tuple(t.shape)) for t in (x, w1, b1, w2, b2)))
     _need_cuda('mlp8', x, w1, b1, w2, b2)
-    if any(n % 8 or n == 0 for n in (*w1.shape, w2.shape[0])):
-        raise NotImplementedError(f'mlp8: the widths ({d}, {w1.shape[0]}, {w2.shape[0]}) have to be multiples of 8')
+    if s1[0] % 8 or s1[1] % 8 or s2[0] % 8 or not s1[0] * s1[1] * s2[0]:
+        raise NotImplementedError(f'mlp8: the widths ({s1[1]}, {s1[0]}, {s2[0]}) have to be multiples of 8')
     return _Mlp8.apply(*_bf16('mlp8', x, w1, b1, w2, b2))
