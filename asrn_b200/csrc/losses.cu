@@ -510,7 +510,6 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   using namespace asrn;
   if (P < 0 || L < 0 || kind < 0 || kind > 1 || !(beta > 0.) || !(smoothing >= 0. && smoothing < 0.5) || !loss)
     return ASRN_ERR_ARG;
-  if (kind == 1 && smoothing != 0.) return ASRN_ERR_ARG;
   if (P > ((int64_t)1 << 30) || L > ((int64_t)1 << 30)) return ASRN_ERR_UNSUPPORTED;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const PrefArgs a{P, L, logp, ref_logp, mask, kind, beta, smoothing, loss, grad, rewards};

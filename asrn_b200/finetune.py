@@ -204,7 +204,7 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
     reference model ([0] the chosen answers, [1] the rejected ones), mask (2, P, L) the answers' tokens. With R the sum
     over the mask of logp - ref_logp and D = R_chosen - R_rejected:
       'sigmoid'  -(1 - smoothing) log sigma(beta D) - smoothing log sigma(-beta D)
-      'ipo'      (D - 1 / (2 beta))^2 with R the mean over the answer's tokens
+      'ipo'      (D - 1 / (2 beta))^2 with R the mean over the answer's tokens (smoothing has no part in it)
     Mean over the pairs whose two answers both have tokens (other pairs get no gradient; 0 without any). Returns
     PreferenceLoss(loss, grad = dloss/dlogp (2, P, L), chosen and rejected = the rewards beta R (P)), float32."""
     if logp.dim() != 3 or logp.shape[0] != 2 or ref_logp.shape != logp.shape:
@@ -212,8 +212,8 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
                          f'{tuple(ref_logp.shape)}')
     if kind not in _KINDS:
         raise ValueError(f'preference_loss: kind is one of {sorted(_KINDS)}')
-    if not beta > 0 or not 0 <= smoothing < 0.5 or (kind == 'ipo' and smoothing):
-        raise ValueError("preference_loss: beta > 0, 0 <= smoothing < 0.5, and no smoothing with 'ipo'")
+    if not beta > 0 or not 0 <= smoothing < 0.5:
+        raise ValueError('preference_loss: beta > 0 and 0 <= smoothing < 0.5')
     dev, lib = _need_cuda('preference_loss', logp, ref_logp, mask), _lib.lib()
     m = _mask(mask, logp.shape, 'preference_loss')
     _, P, L = logp.shape

@@ -252,7 +252,7 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
 /* Preference loss of P answer pairs: logp, ref_logp (2, P, L) float32, mask (2, P, L) bytes; [0] the chosen answers,
  * [1] the rejected ones. R = sum over the mask of (logp - ref_logp), D = R_chosen - R_rejected.
  *   kind 0  -(1 - smoothing) log sigma(beta D) - smoothing log sigma(-beta D), 0 <= smoothing < 0.5
- *   kind 1  (D of the means over the tokens - 1 / (2 beta))^2, smoothing 0
+ *   kind 1  (D of the means over the tokens - 1 / (2 beta))^2 (smoothing has no part in it)
  * loss: the mean over the pairs whose two answers both have a token (0 without one; other pairs get no gradient). grad
  * (2, P, L) = dloss/dlogp (may be NULL), rewards (2, P) = beta R. What stands outside the mask is never used.
  * asrn_policy_loss: clipped policy loss of B sequences: with r = exp(logp - old_logp), q = ref_logp - logp (both
