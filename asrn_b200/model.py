@@ -5,6 +5,9 @@ blocks -> ln_f -> tied head. Mirror of asrn.nucleo.ModeloASRN / BloqueLocal / cr
 The ASRN layers are asrn_b200.ASRNLayer (CUDA kernels of libasrn_b200.so). Under bf16 autocast on CUDA each local
 block runs as the fused asrn_local_block (an LN kernel and three persistent tcgen05 GEMMs with the conv, GELU, bias and
 residual folded in); in fp32 the local blocks, and in every mode the embedding and head, are PyTorch ops.
+logprobs() gives log probabilities of tokens without the (B, L, V) logits (asrn_b200.finetune.head_logprobs), and
+checkpoint='8bits' trains with the local blocks' MLPs keeping their activations in 8 bits (asrn_b200.finetune.mlp8);
+both serve bf16 autocast.
 """
 import math
 
@@ -12,6 +15,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .finetune import head_logprobs, mlp8
 from .layer import ASRNLayer
 
 
@@ -29,6 +33,7 @@ class BloqueLocal(nn.Module):
         if mezcla != 'conv':
             raise NotImplementedError("asrn_b200 builds the default local block (mezcla='conv')")
         self.k, self.mezcla = k, mezcla
+        self.activaciones_8bits = False        # the MLP keeps its activations in 8 bits for the backward pass
         self.ln1 = nn.LayerNorm(d)
         self.conv = nn.Conv1d(d, d, k)
         self.ln2 = nn.LayerNorm(d)
@@ -41,7 +46,16 @@ class BloqueLocal(nn.Module):
         z = self.ln1(h)
         c = F.gelu(self.conv(F.pad(z.transpose(1, 2), (self.k - 1, 0))).transpose(1, 2))
         h = h + self.drop(c)
-        return h + self.drop(self.ff(self.ln2(h)))
+        u = self.ln2(h)
+        if self.activaciones_8bits and self._mlp8_ok(u):
+            return h + self.drop(mlp8(u, self.ff[0].weight, self.ff[0].bias, self.ff[2].weight, self.ff[2].bias))
+        return h + self.drop(self.ff(u))
+
+    def _mlp8_ok(self, u):
+        """mlp8 serves training under bf16 autocast on CUDA and widths that are multiples of 8."""
+        d, ff = self.conv.in_channels, self.ff[0].out_features
+        return (u.is_cuda and torch.is_grad_enabled() and torch.is_autocast_enabled('cuda') and d % 8 == 0 and
+                ff % 8 == 0 and torch.get_autocast_dtype('cuda') == torch.bfloat16)
 
     def _fused_ok(self, h):
         """The fused CUDA block (asrn_local_block) serves bf16 autocast on CUDA, fp32 h, no dropout at work, and the
@@ -104,7 +118,8 @@ def _escalar_profundo(modulo, n_capas):
 
 
 class ModeloASRN(nn.Module):
-    """Same arguments and module names as the reference model (asrn/nucleo.py:1054-1078)."""
+    """Same arguments and module names as the reference model (asrn/nucleo.py:1054-1078). checkpoint='8bits': in
+    training under bf16 autocast the local blocks' MLPs keep their activations in 8 bits."""
 
     def __init__(self, V, d=64, n_capas=2, largo_cada=2, ff=None, k=4, init_profundo=None, checkpoint=False,
                  dropout=0.0, mezcla='conv', memoria_max=1024, protecciones=None, **opciones_capa):
@@ -125,6 +140,8 @@ class ModeloASRN(nn.Module):
                                       for _ in range(n_capas)])
         self.largos = nn.ModuleList([ASRNLayer(d, protecciones, dropout=dropout, **opciones_capa)
                                      for _ in self.pos_largo])
+        for b in self.bloques:
+            b.activaciones_8bits = checkpoint == '8bits'
         if self.init_profundo:
             with torch.no_grad():
                 for b in self.bloques:
@@ -133,6 +150,27 @@ class ModeloASRN(nn.Module):
                     _escalar_profundo(c, n_capas)
 
     def forward(self, x):
+        return self.head(self.estado(x))
+
+    def logprobs(self, x, objetivos=None, temperatura=1.0):
+        """log softmax(logits / temperatura) of the tokens objetivos (B, L) at the positions of x (B, L), float32: by
+        default each position's next token (0 at the last one). A negative target leaves its position out: 0 and no
+        gradient. Under bf16 autocast the (B, L, V) logits are never in memory and positions left out cost nothing
+        (head_logprobs); the fp32 model takes them from its logits."""
+        if objetivos is None:
+            objetivos = F.pad(x[:, 1:], (0, 1), value=-1)
+        if objetivos.shape != x.shape:
+            raise ValueError(f'objetivos must be (B, L) = {tuple(x.shape)}; got {tuple(objetivos.shape)}')
+        h = self.estado(x)
+        if h.is_cuda and torch.is_autocast_enabled('cuda') and h.shape[-1] % 8 == 0 and \
+                torch.get_autocast_dtype('cuda') == torch.bfloat16:
+            return head_logprobs(h, self.head.weight, objetivos, temperatura)
+        lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
+        lp = lp.gather(-1, objetivos.clamp(min=0).unsqueeze(-1)).squeeze(-1)
+        return torch.where(objetivos >= 0, lp, torch.zeros_like(lp))
+
+    def estado(self, x):
+        """The state that the head reads: ln_f of the last block's output (B, L, d)."""
         if self.emb.weight.dtype in (torch.float16, torch.bfloat16):
             raise ValueError(f'the model has {self.emb.weight.dtype} weights: ASRN needs float32 weights; use '
                              'torch.autocast for bf16 (asrn/nucleo.py:1025-1032)')
@@ -146,7 +184,7 @@ class ModeloASRN(nn.Module):
             if i in self.pos_largo:
                 h = self.largos[j](E, h, x, ngram=ng)
                 j += 1
-        return self.head(self.ln_f(h))
+        return self.ln_f(h)
 
     def _ngram_shared(self):
         """True when every ASRN layer has the same n-gram orders and c_vistos (checked again after a change)."""
