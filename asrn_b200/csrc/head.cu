@@ -23,7 +23,7 @@ namespace asrn {
 
 namespace {
 
-constexpr int kGatherRows = 64, kGatherThreads = 256;
+constexpr int kGatherRows = 16, kGatherThreads = 256;
 constexpr int kCountRows = 1024;
 constexpr int64_t kDirectRows = 4096;    // up to here each block counts the targets before it by itself: a launch less
 constexpr float kLog2e = 1.4426950408889634f;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kCountRows) k_head_count(int64_t N, const int6
   if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }
 
-// Block b takes positions [64 b, 64 b + 64): the targets before them (from the tokens, or from the counts of the
+// Block b takes positions [16 b, 16 b + 16): the targets before them (from the tokens, or from the counts of the
 // blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 256.
 __global__ void __launch_bounds__(kGatherThreads)
 k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ tokens,
@@ -125,12 +125,10 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
   const int64_t i = i0 + tid;
   const bool mine = tid < kGatherRows && i < N;
   const int64_t y = mine ? tokens[i] : -1;
-  const unsigned set = __ballot_sync(0xffffffffu, y >= 0);
-  if (lane == 0) warps[wid] = __popc(set);
-  __syncthreads();
-  int r = before + __popc(set & ((1u << lane) - 1u));
-  for (int w = 0; w < wid; ++w) r += warps[w];
+  const unsigned set = __ballot_sync(0xffffffffu, y >= 0);          // the rows are the first warp's
+  const int r = before + __popc(set & ((1u << lane) - 1u));
   if (tid < kGatherRows) at[tid] = y >= 0 ? r : -1;
+  if (tid == 0) warps[0] = __popc(set);
   if (mine) pos[i] = y >= 0 ? r : -1;
   if (y >= 0) {
     tok[r] = y < V ? (int)y : -1;          // outside the vocabulary: NaN from here on
@@ -145,8 +143,7 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
       reinterpret_cast<uint4*>(hc + (int64_t)at[k] * d)[c] = __ldg(reinterpret_cast<const uint4*>(h + (i0 + k) * d) + c);
   }
   if (i0 + kGatherRows >= N) {
-    int total = before;
-    for (int w = 0; w < kGatherRows / 32; ++w) total += warps[w];
+    const int total = before + warps[0];
     if (tid == 0) *count = total;
     const int64_t end = ((int64_t)total + 255) / 256 * 256;
     uint4* dst = reinterpret_cast<uint4*>(hc);

@@ -87,6 +87,11 @@ template <bool Vec> __device__ __forceinline__ void store4(float* p, const float
 
 __device__ __forceinline__ int chunk_left(int64_t L, int64_t t) { return (int)min(L - t, (int64_t)kLossChunk); }
 
+// A kernel launched behind another of the same call starts while that one ends; waits here for its results.
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel's blocks start once all of this one's have come here or ended.
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- preference loss -----------------------------------------------------------------------------------------------
 
 struct PrefArgs {
@@ -179,6 +184,7 @@ template <bool Vec>
 __global__ void __launch_bounds__(kLossThreads) k_pref_sums(PrefArgs a, int64_t items, int64_t parts, int64_t width,
                                                             RowSum* __restrict__ part) {
   __shared__ double slots[16];
+  let_next();
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
     double v[2] = {0., 0.};
@@ -212,9 +218,19 @@ __device__ __forceinline__ RowSum row_total(const RowSum* part, int64_t row, int
 // each, all at once.
 template <bool Vec>
 __global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_t items, int64_t parts, int64_t width,
-                                                              const RowSum* __restrict__ part) {
+                                                              const RowSum* part) {
   __shared__ double slots[16];
   __shared__ float slope[kLossThreads];
+  // the first item's first chunks' masks come while the sums are still being made
+  const int64_t base0 = blockIdx.x / parts * a.L, t0 = blockIdx.x % parts * width;
+  const int64_t end0 = blockIdx.x < items ? min(a.L, t0 + width) : t0;
+  uint32_t early[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t t = t0 + k * kLossChunk;
+    early[k] = t < end0 ? load_mask<Vec>(a.mask + base0 + t, chunk_left(end0, t)) : 0;
+  }
+  wait_previous();
   double v[2] = {0., 0.};
   for (int64_t p = threadIdx.x; p < a.P; p += kLossThreads) {
     const RowSum r0 = row_total(part, p, parts), r1 = row_total(part, a.P + p, parts);
@@ -244,8 +260,19 @@ __global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_
       if (it >= items) break;
       const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
       const float s = slope[k];
+      int64_t t = it % parts * width;
+      if (it == blockIdx.x) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (t < t1) {
+            const float d[4] = {early[q] & 1 ? s : 0.f, early[q] & 2 ? s : 0.f, early[q] & 4 ? s : 0.f,
+                                early[q] & 8 ? s : 0.f};
+            store4<Vec>(a.grad + base + t, d, chunk_left(t1, t));
+            t += kLossChunk;
+          }
+      }
 #pragma unroll 4
-      for (int64_t t = it % parts * width; t < t1; t += kLossChunk) {
+      for (; t < t1; t += kLossChunk) {
         const uint32_t m = load_mask<Vec>(a.mask + base + t, chunk_left(t1, t));
         const float d[4] = {m & 1 ? s : 0.f, m & 2 ? s : 0.f, m & 4 ? s : 0.f, m & 8 ? s : 0.f};
         store4<Vec>(a.grad + base + t, d, chunk_left(t1, t));
@@ -359,6 +386,7 @@ template <bool Vec>
 __global__ void __launch_bounds__(kLossThreads) k_policy_counts(PolicyArgs a, int64_t parts, int64_t width,
                                                                 int* __restrict__ counts, unsigned* ticket) {
   __shared__ double slots[8];
+  let_next();
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
   for (int64_t it = blockIdx.x; it < a.B * parts; it += gridDim.x) {
     const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
@@ -382,10 +410,14 @@ __device__ __forceinline__ int row_count(const int* counts, int64_t row, int64_t
 // block that finishes last adds the sums up in index order.
 template <bool Vec, bool Ref>
 __global__ void __launch_bounds__(kLossThreads, kLossBlocks)
-k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* __restrict__ counts, BlockSum* part,
-              unsigned* ticket) {
+k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* counts, BlockSum* part, unsigned* ticket) {
   __shared__ double slots[24];
   __shared__ bool last;
+  const int64_t step_r = gridDim.x / chunks, step_c = gridDim.x % chunks, stride_c = step_c * kLossChunk;
+  int64_t row = blockIdx.x / chunks, t = blockIdx.x % chunks * kLossChunk;
+  // the mask comes an item ahead: a warp whose tokens are all outside it reads nothing else
+  uint32_t next = row < a.B ? load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t)) : 0;
+  wait_previous();
   double n[2] = {0., 0.};
   for (int64_t b = threadIdx.x; b < a.B; b += kLossThreads) {
     const int c = row_count(counts, b, parts);
@@ -396,10 +428,6 @@ k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* __restrict
   const float over = (float)(1. / (a.per_sequence ? fmax(1., n[1]) : fmax(1., n[0])));
   double v[3] = {0., 0., 0.};
   int cut = 0;
-  const int64_t step_r = gridDim.x / chunks, step_c = gridDim.x % chunks, stride_c = step_c * kLossChunk;
-  int64_t row = blockIdx.x / chunks, t = blockIdx.x % chunks * kLossChunk;
-  // the mask comes an item ahead: a warp whose tokens are all outside it reads nothing else
-  uint32_t next = row < a.B ? load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t)) : 0;
   while (row < a.B) {
     float share = 1.f, row_adv = 0.f;
     if (a.per_sequence) share = 1.f / (float)max(1, row_count(counts, row, parts));
@@ -470,6 +498,20 @@ int loss_grid(int64_t items, int per_sm = 8) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)148 * per_sm));
 }
 
+// Behind the kernel before it on the stream, which it waits for itself (wait_previous).
+template <class... P, class... A> int launch_behind(void (*kernel)(P...), int grid, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kLossThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, (P)args...) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
 // Rows of a multiple of 4 tokens on 16-byte boundaries (the mask's on 4) are read four tokens at a time.
 bool vec_ok(int64_t L, std::initializer_list<const void*> fs, const void* mask) {
   if (L % 4 || (uintptr_t)mask % 4) return false;
@@ -524,14 +566,11 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   const int64_t parts = row_parts(2 * P, L), width = part_width(2 * P, L), items = 2 * P * parts;
   RowSum* part = reinterpret_cast<RowSum*>(workspace);
   const int grid = loss_grid(items);
-  if (vec_ok(L, {logp, ref_logp, grad}, mask)) {
-    k_pref_sums<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
-    k_pref_finish<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
-  } else {
-    k_pref_sums<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
-    k_pref_finish<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
-  }
-  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+  const bool vec = vec_ok(L, {logp, ref_logp, grad}, mask);
+  if (vec) k_pref_sums<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+  else k_pref_sums<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+  if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
+  return launch_behind(vec ? k_pref_finish<true> : k_pref_finish<false>, grid, s, a, items, parts, width, part);
 }
 
 size_t asrn_policy_workspace_bytes(int64_t B, int64_t L) {
@@ -567,16 +606,13 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   int* counts = reinterpret_cast<int*>(base + 256 + align_up(kLossGrid * sizeof(BlockSum)));
   const int64_t parts = row_parts(B, L), width = part_width(B, L), chunks = loss_chunks(L);
   const int grid = loss_grid(B * chunks, kLossBlocks), cgrid = loss_grid(B * parts);
-  if (vec_ok(L, {logp, old_logp, ref_logp, adv_per_token ? advantages : nullptr, grad}, mask)) {
-    k_policy_counts<true><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
-    if (ref_logp) k_policy_main<true, true><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
-    else k_policy_main<true, false><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
-  } else {
-    k_policy_counts<false><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
-    if (ref_logp) k_policy_main<false, true><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
-    else k_policy_main<false, false><<<grid, kLossThreads, 0, s>>>(a, chunks, parts, counts, part, ticket);
-  }
-  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+  const bool vec = vec_ok(L, {logp, old_logp, ref_logp, adv_per_token ? advantages : nullptr, grad}, mask);
+  if (vec) k_policy_counts<true><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
+  else k_policy_counts<false><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
+  if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
+  const auto main_kernel = vec ? (ref_logp ? k_policy_main<true, true> : k_policy_main<true, false>)
+                               : (ref_logp ? k_policy_main<false, true> : k_policy_main<false, false>);
+  return launch_behind(main_kernel, grid, s, a, chunks, parts, counts, part, ticket);
 }
 
 }  // extern "C"
