@@ -60,16 +60,16 @@ def _stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _need_cuda(what, *ts):
-    dev = ts[0].device
+def _need_cuda(what, first, *ts):
+    """The tensors' device; they all have to be on the same GPU."""
+    at = first.get_device()
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f'asrn_b200.{what} runs on CUDA tensors only (there is no CPU implementation)')
-        if t.device != dev:
-            raise ValueError(f'{what}: tensors on {dev} and {t.device}')
-    return dev
+        if t is not None and t.get_device() != at:
+            raise (ValueError if at >= 0 and t.is_cuda else RuntimeError)(
+                f'asrn_b200.{what} runs on CUDA tensors of one device; got {first.device} and {t.device}')
+    if at < 0:
+        raise RuntimeError(f'asrn_b200.{what} runs on CUDA tensors only (there is no CPU implementation)')
+    return first.device
 
 
 def _rows(t):
@@ -113,8 +113,8 @@ class _HeadLogprobs(torch.autograd.Function):
         shape, N, V, d, tau, dev, nb_saved = ctx.meta
         lib = _lib.lib()
         need = ctx.needs_input_grad
-        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if need[0] else None
-        dw = torch.empty((V, d), dtype=torch.bfloat16, device=dev) if need[1] else None
+        dh = w.new_empty(shape) if need[0] else None
+        dw = torch.empty_like(w) if need[1] else None
         g32 = _f32(g)
         nb = _bytes('asrn_head_workspace_bytes', N, V, d, 1)
         ws = _scratch(nb, dev)
@@ -181,13 +181,13 @@ class _WithGrad(torch.autograd.Function):
 
 def _f32(t):
     """float32 and contiguous; read through its address only."""
-    if t.dtype == torch.float32 and t.is_contiguous():
+    if t.dtype is torch.float32 and t.is_contiguous():
         return t
     return t.detach().to(torch.float32).contiguous()
 
 
 def _mask(m, shape, what):
-    if m.shape != shape or m.dtype not in (torch.bool, torch.uint8):
+    if m.shape != shape or (m.dtype is not torch.bool and m.dtype is not torch.uint8):
         raise ValueError(f'{what}: mask has to be bool or uint8 of shape {tuple(shape)}; got {m.dtype} {tuple(m.shape)}')
     return m if m.is_contiguous() else m.contiguous()
 
@@ -207,21 +207,20 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
       'ipo'      (D - 1 / (2 beta))^2 with R the mean over the answer's tokens (smoothing has no part in it)
     Mean over the pairs whose two answers both have tokens (other pairs get no gradient; 0 without any). Returns
     PreferenceLoss(loss, grad = dloss/dlogp (2, P, L), chosen and rejected = the rewards beta R (P)), float32."""
-    if logp.dim() != 3 or logp.shape[0] != 2 or ref_logp.shape != logp.shape:
-        raise ValueError(f'preference_loss: logp and ref_logp are (2, P, L); got {tuple(logp.shape)} and '
+    sh = logp.shape
+    if len(sh) != 3 or sh[0] != 2 or ref_logp.shape != sh:
+        raise ValueError(f'preference_loss: logp and ref_logp are (2, P, L); got {tuple(sh)} and '
                          f'{tuple(ref_logp.shape)}')
     if kind not in _KINDS:
         raise ValueError(f'preference_loss: kind is one of {sorted(_KINDS)}')
     if not beta > 0 or not 0 <= smoothing < 0.5:
         raise ValueError('preference_loss: beta > 0 and 0 <= smoothing < 0.5')
     dev, lib = _need_cuda('preference_loss', logp, ref_logp, mask), _lib.lib()
-    m = _mask(mask, logp.shape, 'preference_loss')
-    _, P, L = logp.shape
+    m = _mask(mask, sh, 'preference_loss')
+    _, P, L = sh
     lp, rf = _f32(logp), _f32(ref_logp)
     nb = _bytes('asrn_preference_workspace_bytes', P, L)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    rewards = torch.empty((2, P), dtype=torch.float32, device=dev)
-    grad = torch.empty((2, P, L), dtype=torch.float32, device=dev)
+    loss, rewards, grad = lp.new_empty(()), lp.new_empty((2, P)), torch.empty_like(lp)
     ws = _scratch(nb, dev) if nb else None
     _lib.check(lib.asrn_preference_loss(P, L, lp.data_ptr(), rf.data_ptr(), m.data_ptr(), _KINDS[kind], beta, smoothing,
                                         loss.data_ptr(), grad.data_ptr(), rewards.data_ptr(), _p(ws), nb,
@@ -239,11 +238,13 @@ def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2)
     per 'token': the mean over the mask's tokens; 'sequence': over each sequence's tokens, then over the sequences that
     have one. Returns PolicyLoss(loss, grad = dloss/dlogp (B, L), kl = the mean of exp(q) - q - 1, clipped = the share
     of tokens whose ratio was clipped), float32."""
-    if logp.dim() != 2 or old_logp.shape != logp.shape or (ref_logp is not None and ref_logp.shape != logp.shape):
+    sh, sa = logp.shape, advantages.shape
+    if len(sh) != 2 or old_logp.shape != sh or (ref_logp is not None and ref_logp.shape != sh):
         raise ValueError('policy_loss: logp, old_logp and ref_logp are (B, L); got ' + ', '.join(
             str(tuple(t.shape)) for t in (logp, old_logp, ref_logp) if t is not None))
-    if advantages.shape not in (logp.shape, logp.shape[:1]):
-        raise ValueError(f'policy_loss: advantages are (B, L) or (B); got {tuple(advantages.shape)}')
+    B, L = sh
+    if sa != sh and (len(sa) != 1 or sa[0] != B):
+        raise ValueError(f'policy_loss: advantages are (B, L) or (B); got {tuple(sa)}')
     if per not in _PER:
         raise ValueError(f'policy_loss: per is one of {sorted(_PER)}')
     low, high = clip
@@ -252,16 +253,14 @@ def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2)
     if kl > 0 and ref_logp is None:
         raise ValueError('policy_loss: a KL term needs ref_logp')
     dev, lib = _need_cuda('policy_loss', logp, old_logp, advantages, mask, ref_logp), _lib.lib()
-    m = _mask(mask, logp.shape, 'policy_loss')
-    B, L = logp.shape
+    m = _mask(mask, sh, 'policy_loss')
     lp, old, adv = _f32(logp), _f32(old_logp), _f32(advantages)
     ref = None if ref_logp is None else _f32(ref_logp)
-    out = torch.empty(3, dtype=torch.float32, device=dev)
-    grad = torch.empty((B, L), dtype=torch.float32, device=dev)
+    out, grad = lp.new_empty(3), torch.empty_like(lp)
     nb = _bytes('asrn_policy_workspace_bytes', B, L)
     ws = _scratch(nb, dev) if nb else None
     base = out.data_ptr()
-    _lib.check(lib.asrn_policy_loss(B, L, lp.data_ptr(), old.data_ptr(), _p(ref), adv.data_ptr(), adv.dim() == 2,
+    _lib.check(lib.asrn_policy_loss(B, L, lp.data_ptr(), old.data_ptr(), _p(ref), adv.data_ptr(), len(sa) == 2,
                                     m.data_ptr(), low, high, kl, _PER[per], base, grad.data_ptr(), base + 4, _p(ws), nb,
                                     _stream(dev)), 'asrn_policy_loss')
     loss, k3, clipped = out.unbind()
@@ -308,7 +307,7 @@ class _Mlp8(torch.autograd.Function):
         d, ff, dout = x.shape[-1], w1.shape[0], w2.shape[0]
         N, dev, lib = x.numel() // d, x.device, _lib.lib()
         xr, w1, b1, w2, b2 = _rows(x), _rows(w1), _rows(b1), _rows(w2), _rows(b2)
-        y = torch.empty((*x.shape[:-1], dout), dtype=torch.bfloat16, device=dev)
+        y = xr.new_empty((*x.shape[:-1], dout))
         keep = any(ctx.needs_input_grad)
         nb_saved = _bytes('asrn_mlp8_saved_bytes', N, d, ff) if keep else 0
         nb = _bytes('asrn_mlp8_workspace_bytes', N, d, ff, dout, 0)
@@ -328,8 +327,7 @@ class _Mlp8(torch.autograd.Function):
         shape, N, d, ff, dout, dev, nb_saved = ctx.meta
         lib = _lib.lib()
         sizes = (shape, (ff, d), (ff,), (dout, ff), (dout,))
-        out = [torch.empty(s, dtype=torch.bfloat16, device=dev) if n else None
-               for s, n in zip(sizes, ctx.needs_input_grad)]
+        out = [w1.new_empty(s) if n else None for s, n in zip(sizes, ctx.needs_input_grad)]
         dyr = _rows(dy)
         nb = _bytes('asrn_mlp8_workspace_bytes', N, d, ff, dout, 1)
         ws = _scratch(nb, dev)
