@@ -7,6 +7,7 @@
 // never multiplied, so a NaN or infinity there reaches nothing.
 #include <algorithm>
 #include <initializer_list>
+#include <cooperative_groups.h>
 #include "common.cuh"
 #include "layout.h"
 
@@ -16,7 +17,8 @@ namespace {
 
 constexpr int kLossThreads = 256;
 constexpr int kLossChunk = 4 * kLossThreads;   // tokens of one row that a block takes at a time, 4 a thread
-constexpr int kLossBlocks = 5;           // of k_policy_main that an SM holds
+constexpr int kLossBlocks = 5;           // that an SM holds at a time, by the kernels' launch bounds
+constexpr int kLossGrid = 148 * 8;
 constexpr int kSmallRows = 1024;         // rows a single block keeps in shared memory
 
 struct RowSum {                          // of one chunk of one row
@@ -91,6 +93,11 @@ __device__ __forceinline__ int chunk_left(int64_t L, int64_t t) { return (int)mi
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next kernel's blocks start once all of this one's have come here or ended.
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Rows in parts that blocks take: items = rows x parts, each of `width` tokens, a multiple of the chunk.
+struct Split {
+  int64_t items, parts, width;
+};
 
 // ---- preference loss -----------------------------------------------------------------------------------------------
 
@@ -179,32 +186,6 @@ __global__ void __launch_bounds__(1024) k_pref_small(PrefArgs a) {
   }
 }
 
-// Row sums by parts of a row: item = (row, part of `width` tokens, a multiple of the chunk).
-template <bool Vec>
-__global__ void __launch_bounds__(kLossThreads) k_pref_sums(PrefArgs a, int64_t items, int64_t parts, int64_t width,
-                                                            RowSum* __restrict__ part) {
-  __shared__ double slots[16];
-  let_next();
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
-    double v[2] = {0., 0.};
-    int n = 0;
-#pragma unroll 4
-    for (int64_t t = it % parts * width; t < t1; t += kLossChunk) {
-      float lp[4], rf[4];
-      const uint32_t m = load_mask<Vec>(a.mask + base + t, chunk_left(t1, t));
-      load4<Vec>(lp, a.logp + base + t, chunk_left(t1, t));
-      load4<Vec>(rf, a.ref + base + t, chunk_left(t1, t));
-      n += __popc(m);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[0] += m >> j & 1 ? (double)lp[j] - (double)rf[j] : 0.;
-    }
-    v[1] = (double)n;
-    block_sum(v, slots);
-    if (threadIdx.x == 0) part[it] = RowSum{v[0], (int64_t)v[1]};
-  }
-}
-
 __device__ __forceinline__ RowSum row_total(const RowSum* part, int64_t row, int64_t parts) {
   RowSum t{0., 0};
   for (int64_t c = 0; c < parts; ++c) {
@@ -214,26 +195,44 @@ __device__ __forceinline__ RowSum row_total(const RowSum* part, int64_t row, int
   return t;
 }
 
-// The pairs that count, the loss (block 0) and the gradient. A block's first threads find the slopes of its items, one
-// each, all at once.
+// First the rows' sums by parts: item = (row, part of `width` tokens, a multiple of the chunk). Returns the masks of the
+// first 16 chunks of the block's first item.
+template <bool Vec> __device__ __forceinline__ uint64_t pref_sums(const PrefArgs& a, const Split& w, RowSum* part) {
+  __shared__ double slots[16];
+  uint64_t bits = 0;
+  for (int64_t it = blockIdx.x; it < w.items; it += gridDim.x) {
+    const int64_t begin = it % w.parts * w.width, base = it / w.parts * a.L + begin;
+    const int64_t len = min(a.L - begin, w.width);         // none in the last parts of a short row
+    double v[2] = {0., 0.};
+    int n = 0;
+#pragma unroll 4
+    for (int64_t t = 0; t < len; t += kLossChunk) {
+      float lp[4], rf[4];
+      const int left = chunk_left(len, t);
+      const uint32_t m = load_mask<Vec>(a.mask + base + t, left);
+      load4<Vec>(lp, a.logp + base + t, left);
+      load4<Vec>(rf, a.ref + base + t, left);
+      if (it == blockIdx.x && t < 16 * kLossChunk) bits |= (uint64_t)m << (t / kLossChunk * 4);
+      n += __popc(m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[0] += m >> j & 1 ? (double)lp[j] - (double)rf[j] : 0.;
+    }
+    v[1] = (double)n;
+    block_sum(v, slots);
+    if (threadIdx.x == 0) part[it] = RowSum{v[0], (int64_t)v[1]};
+  }
+  return bits;
+}
+
+// Then, with every part there, the pairs that count, the loss (block 0) and the gradient. A block's first threads find the
+// slopes of its items, one each, all at once.
 template <bool Vec>
-__global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_t items, int64_t parts, int64_t width,
-                                                              const RowSum* part) {
+__device__ __forceinline__ void pref_finish(const PrefArgs& a, const Split& w, const RowSum* part, uint64_t bits) {
   __shared__ double slots[16];
   __shared__ float slope[kLossThreads];
-  // the first item's first chunks' masks come while the sums are still being made
-  const int64_t base0 = blockIdx.x / parts * a.L, t0 = blockIdx.x % parts * width;
-  const int64_t end0 = blockIdx.x < items ? min(a.L, t0 + width) : t0;
-  uint32_t early[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int64_t t = t0 + k * kLossChunk;
-    early[k] = t < end0 ? load_mask<Vec>(a.mask + base0 + t, chunk_left(end0, t)) : 0;
-  }
-  wait_previous();
   double v[2] = {0., 0.};
   for (int64_t p = threadIdx.x; p < a.P; p += kLossThreads) {
-    const RowSum r0 = row_total(part, p, parts), r1 = row_total(part, a.P + p, parts);
+    const RowSum r0 = row_total(part, p, w.parts), r1 = row_total(part, a.P + p, w.parts);
     v[0] += r0.n > 0 && r1.n > 0 ? 1. : 0.;
     if (blockIdx.x == 0) {
       v[1] += pair_of(a, r0.sum, r1.sum, r0.n, r1.n).loss;
@@ -245,40 +244,55 @@ __global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, int64_
   const double pairs = fmax(1., v[0]);
   if (blockIdx.x == 0 && threadIdx.x == 0) a.loss[0] = (float)(v[1] / pairs);
   if (!a.grad) return;
-  for (int64_t it0 = blockIdx.x; it0 < items; it0 += (int64_t)gridDim.x * kLossThreads) {
+  for (int64_t it0 = blockIdx.x; it0 < w.items; it0 += (int64_t)gridDim.x * kLossThreads) {
     const int64_t mine = it0 + (int64_t)threadIdx.x * gridDim.x;
     __syncthreads();
-    if (mine < items) {
-      const int64_t row = mine / parts, p = row % a.P;
-      const RowSum r0 = row_total(part, p, parts), r1 = row_total(part, a.P + p, parts);
+    if (mine < w.items) {
+      const int64_t row = mine / w.parts, p = row % a.P;
+      const RowSum r0 = row_total(part, p, w.parts), r1 = row_total(part, a.P + p, w.parts);
       const Pair q = pair_of(a, r0.sum, r1.sum, r0.n, r1.n);
       slope[threadIdx.x] = (float)((row < a.P ? q.slope0 : q.slope1) / pairs);
     }
     __syncthreads();
     for (int k = 0; k < kLossThreads; ++k) {
       const int64_t it = it0 + (int64_t)k * gridDim.x;
-      if (it >= items) break;
-      const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
+      if (it >= w.items) break;
+      const int64_t begin = it % w.parts * w.width, base = it / w.parts * a.L + begin;
+      const int64_t len = min(a.L - begin, w.width);
       const float s = slope[k];
-      int64_t t = it % parts * width;
-      if (it == blockIdx.x) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (t < t1) {
-            const float d[4] = {early[q] & 1 ? s : 0.f, early[q] & 2 ? s : 0.f, early[q] & 4 ? s : 0.f,
-                                early[q] & 8 ? s : 0.f};
-            store4<Vec>(a.grad + base + t, d, chunk_left(t1, t));
-            t += kLossChunk;
-          }
-      }
 #pragma unroll 4
-      for (; t < t1; t += kLossChunk) {
-        const uint32_t m = load_mask<Vec>(a.mask + base + t, chunk_left(t1, t));
+      for (int64_t t = 0; t < len; t += kLossChunk) {
+        const int left = chunk_left(len, t);
+        const uint32_t m = it == blockIdx.x && t < 16 * kLossChunk ? (uint32_t)(bits >> (t / kLossChunk * 4)) & 15u
+                                                                   : load_mask<Vec>(a.mask + base + t, left);
         const float d[4] = {m & 1 ? s : 0.f, m & 2 ? s : 0.f, m & 4 ? s : 0.f, m & 8 ? s : 0.f};
-        store4<Vec>(a.grad + base + t, d, chunk_left(t1, t));
+        store4<Vec>(a.grad + base + t, d, left);
       }
     }
   }
+}
+
+// Both in one cooperative launch, or in two that overlap.
+template <bool Vec> __global__ void __launch_bounds__(kLossThreads, kLossBlocks) k_pref(PrefArgs a, Split w, RowSum* part) {
+  const uint64_t bits = pref_sums<Vec>(a, w, part);
+  cooperative_groups::this_grid().sync();
+  pref_finish<Vec>(a, w, part, bits);
+}
+template <bool Vec> __global__ void __launch_bounds__(kLossThreads) k_pref_sums(PrefArgs a, Split w, RowSum* part) {
+  let_next();
+  pref_sums<Vec>(a, w, part);
+}
+template <bool Vec> __global__ void __launch_bounds__(kLossThreads) k_pref_finish(PrefArgs a, Split w, const RowSum* part) {
+  uint64_t bits = 0;                             // the masks of the first item come while the sums are still being made
+  if (blockIdx.x < w.items) {
+    const int64_t begin = blockIdx.x % w.parts * w.width, base = blockIdx.x / w.parts * a.L + begin;
+    const int64_t len = min(a.L - begin, w.width);
+#pragma unroll 4
+    for (int64_t t = 0; t < min(len, (int64_t)16 * kLossChunk); t += kLossChunk)
+      bits |= (uint64_t)load_mask<Vec>(a.mask + base + t, chunk_left(len, t)) << (t / kLossChunk * 4);
+  }
+  wait_previous();
+  pref_finish<Vec>(a, w, part, bits);
 }
 
 // ---- clipped policy loss -------------------------------------------------------------------------------------------
@@ -381,43 +395,41 @@ template <bool Ref> __global__ void __launch_bounds__(1024) k_policy_small(Polic
   if (threadIdx.x == 0) policy_results(a, v[0], v[1], n[0], v[2], n[1]);
 }
 
-// Tokens of each part of each row; block 0 clears the ticket that the next launch's blocks take.
-template <bool Vec>
-__global__ void __launch_bounds__(kLossThreads) k_policy_counts(PolicyArgs a, int64_t parts, int64_t width,
-                                                                int* __restrict__ counts, unsigned* ticket) {
-  __shared__ double slots[8];
-  let_next();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
-  for (int64_t it = blockIdx.x; it < a.B * parts; it += gridDim.x) {
-    const int64_t base = it / parts * a.L, t1 = min(a.L, (it % parts + 1) * width);
-    int n = 0;
-#pragma unroll 4
-    for (int64_t t = it % parts * width; t < t1; t += kLossChunk)
-      n += __popc(load_mask<Vec>(a.mask + base + t, chunk_left(t1, t)));
-    double v[1] = {(double)n};
-    block_sum(v, slots);
-    if (threadIdx.x == 0) counts[it] = (int)v[0];
-  }
-}
-
 __device__ __forceinline__ int row_count(const int* counts, int64_t row, int64_t parts) {
   int c = 0;
   for (int64_t k = 0; k < parts; ++k) c += counts[row * parts + k];
   return c;
 }
 
-// The tokens, the gradient and each block's sums, chunks dealt out in turn (a row's prompt and padding cost little); the
-// block that finishes last adds the sums up in index order.
-template <bool Vec, bool Ref>
-__global__ void __launch_bounds__(kLossThreads, kLossBlocks)
-k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* counts, BlockSum* part, unsigned* ticket) {
+// First the tokens of each part of each row (and block 0 clears the ticket).
+template <bool Vec>
+__device__ __forceinline__ void policy_counts(const PolicyArgs& a, const Split& w, int* counts, unsigned* ticket) {
+  __shared__ double slots[8];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
+  for (int64_t it = blockIdx.x; it < w.items; it += gridDim.x) {
+    const int64_t begin = it % w.parts * w.width, base = it / w.parts * a.L + begin;
+    const int64_t len = min(a.L - begin, w.width);
+    int c = 0;
+#pragma unroll 4
+    for (int64_t t = 0; t < len; t += kLossChunk) c += __popc(load_mask<Vec>(a.mask + base + t, chunk_left(len, t)));
+    double v[1] = {(double)c};
+    block_sum(v, slots);
+    if (threadIdx.x == 0) counts[it] = (int)v[0];
+  }
+}
+
+// Then, once `ready` has every count there, the tokens' losses, the gradient and each block's sums, chunks dealt out in
+// turn (a row's prompt and padding cost little); the block that finishes last adds the sums up in index order.
+template <bool Vec, bool Ref, class Ready>
+__device__ __forceinline__ void policy_main(const PolicyArgs& a, int64_t chunks, int64_t parts, const int* counts,
+                                            BlockSum* part, unsigned* ticket, Ready ready) {
   __shared__ double slots[24];
   __shared__ bool last;
   const int64_t step_r = gridDim.x / chunks, step_c = gridDim.x % chunks, stride_c = step_c * kLossChunk;
   int64_t row = blockIdx.x / chunks, t = blockIdx.x % chunks * kLossChunk;
   // the mask comes an item ahead: a warp whose tokens are all outside it reads nothing else
   uint32_t next = row < a.B ? load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t)) : 0;
-  wait_previous();
+  ready();
   double n[2] = {0., 0.};
   for (int64_t b = threadIdx.x; b < a.B; b += kLossThreads) {
     const int c = row_count(counts, b, parts);
@@ -489,24 +501,50 @@ k_policy_main(PolicyArgs a, int64_t chunks, int64_t parts, const int* counts, Bl
   if (threadIdx.x == 0) policy_results(a, v[0], v[1], n[0], v[2], n[1]);
 }
 
-int64_t loss_chunks(int64_t L) { return (L + kLossChunk - 1) / kLossChunk; }
-
-constexpr int kLossGrid = 148 * 8;
-
-// As many blocks as the SMs hold at a time: none waits for another to end.
-int loss_grid(int64_t items, int per_sm = 8) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)148 * per_sm));
+// Both in one cooperative launch, or in two that overlap.
+template <bool Vec, bool Ref>
+__global__ void __launch_bounds__(kLossThreads, kLossBlocks)
+k_policy(PolicyArgs a, int64_t chunks, Split w, int* counts, BlockSum* part, unsigned* ticket) {
+  policy_counts<Vec>(a, w, counts, ticket);
+  policy_main<Vec, Ref>(a, chunks, w.parts, counts, part, ticket, [] { cooperative_groups::this_grid().sync(); });
+}
+template <bool Vec>
+__global__ void __launch_bounds__(kLossThreads) k_policy_counts(PolicyArgs a, Split w, int* counts, unsigned* ticket) {
+  let_next();
+  policy_counts<Vec>(a, w, counts, ticket);
+}
+template <bool Vec, bool Ref>
+__global__ void __launch_bounds__(kLossThreads, kLossBlocks)
+k_policy_main(PolicyArgs a, int64_t chunks, Split w, const int* counts, BlockSum* part, unsigned* ticket) {
+  policy_main<Vec, Ref>(a, chunks, w.parts, counts, part, ticket, [] { wait_previous(); });
 }
 
-// Behind the kernel before it on the stream, which it waits for itself (wait_previous).
-template <class... P, class... A> int launch_behind(void (*kernel)(P...), int grid, cudaStream_t s, const A&... args) {
+int64_t loss_chunks(int64_t L) { return (L + kLossChunk - 1) / kLossChunk; }
+
+// One cooperative launch up to here, two overlapping ones above: the second launch costs the host about 3 us, the
+// cooperative one the GPU about 4 (it starts on an idle GPU and its barrier is one). See the table at the top.
+constexpr int64_t kTogether = 1 << 19;
+
+int loss_grid(int64_t items, int per_sm) {
+  static int sms = 0;
+  int dev = 0;
+  if (sms == 0 && (cudaGetDevice(&dev) != cudaSuccess ||
+                   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0))
+    sms = 148;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(items, std::min(kLossGrid, sms * per_sm)));
+}
+
+// Cooperatively, or behind the kernel before it on the stream, which it waits for itself (wait_previous).
+template <class... P, class... A>
+int launch_with(cudaLaunchAttributeID how, void (*kernel)(P...), int grid, cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kLossThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = how;
+  if (how == cudaLaunchAttributeCooperative) attr[0].val.cooperative = 1;
+  else attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, (P)args...) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
@@ -525,13 +563,11 @@ float rounded(double x, bool up) {
   return up ? ((double)f < x ? nextafterf(f, INFINITY) : f) : ((double)f > x ? nextafterf(f, -INFINITY) : f);
 }
 
-// Parts of a row that blocks sum apart: as many as fill the GPU, each of a chunk at least. width: tokens of a part.
-int64_t row_parts(int64_t rows, int64_t L) {
-  return std::max<int64_t>(1, std::min<int64_t>(kLossGrid / std::max<int64_t>(1, rows), loss_chunks(L)));
-}
-int64_t part_width(int64_t rows, int64_t L) {
-  const int64_t parts = row_parts(rows, L);
-  return (loss_chunks(L) + parts - 1) / parts * kLossChunk;
+// Rows in parts: as many as a full grid has blocks for, each of a chunk at least (every block adds all parts up again).
+Split split_rows(int64_t rows, int64_t L) {
+  const int64_t chunks = loss_chunks(L);
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kLossGrid / std::max<int64_t>(1, rows), chunks));
+  return Split{rows * parts, parts, (chunks + parts - 1) / parts * kLossChunk};
 }
 
 bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L <= 16384; }
@@ -543,7 +579,7 @@ extern "C" {
 
 size_t asrn_preference_workspace_bytes(int64_t P, int64_t L) {
   if (P < 0 || L < 0 || asrn::small_loss(2 * P, L)) return 0;
-  return asrn::align_up((size_t)(2 * P * asrn::row_parts(2 * P, L)) * sizeof(asrn::RowSum) + 1);
+  return asrn::align_up((size_t)asrn::split_rows(2 * P, L).items * sizeof(asrn::RowSum) + 1);
 }
 
 int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* ref_logp, const uint8_t* mask,
@@ -563,20 +599,24 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   }
   if (!workspace || workspace_bytes < asrn_preference_workspace_bytes(P, L) || (uintptr_t)workspace % 16)
     return ASRN_ERR_WORKSPACE;
-  const int64_t parts = row_parts(2 * P, L), width = part_width(2 * P, L), items = 2 * P * parts;
+  const Split w = split_rows(2 * P, L);
   RowSum* part = reinterpret_cast<RowSum*>(workspace);
-  const int grid = loss_grid(items);
   const bool vec = vec_ok(L, {logp, ref_logp, grad}, mask);
-  if (vec) k_pref_sums<true><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
-  else k_pref_sums<false><<<grid, kLossThreads, 0, s>>>(a, items, parts, width, part);
+  if (2 * P * L <= kTogether)
+    return launch_with(cudaLaunchAttributeCooperative, vec ? k_pref<true> : k_pref<false>, loss_grid(w.items, kLossBlocks), s,
+                       a, w, part);
+  const int grid = loss_grid(w.items, 8);
+  if (vec) k_pref_sums<true><<<grid, kLossThreads, 0, s>>>(a, w, part);
+  else k_pref_sums<false><<<grid, kLossThreads, 0, s>>>(a, w, part);
   if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
-  return launch_behind(vec ? k_pref_finish<true> : k_pref_finish<false>, grid, s, a, items, parts, width, part);
+  return launch_with(cudaLaunchAttributeProgrammaticStreamSerialization, vec ? k_pref_finish<true> : k_pref_finish<false>,
+                     grid, s, a, w, part);
 }
 
 size_t asrn_policy_workspace_bytes(int64_t B, int64_t L) {
   if (B < 0 || L < 0 || asrn::small_loss(B, L)) return 0;
   return 256 + asrn::align_up(asrn::kLossGrid * sizeof(asrn::BlockSum)) +
-         asrn::align_up((size_t)(B * asrn::row_parts(B, L)) * sizeof(int) + 1);
+         asrn::align_up((size_t)asrn::split_rows(B, L).items * sizeof(int) + 1);
 }
 
 int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_logp, const float* ref_logp,
@@ -604,15 +644,22 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   unsigned* ticket = reinterpret_cast<unsigned*>(base);
   BlockSum* part = reinterpret_cast<BlockSum*>(base + 256);
   int* counts = reinterpret_cast<int*>(base + 256 + align_up(kLossGrid * sizeof(BlockSum)));
-  const int64_t parts = row_parts(B, L), width = part_width(B, L), chunks = loss_chunks(L);
-  const int grid = loss_grid(B * chunks, kLossBlocks), cgrid = loss_grid(B * parts);
+  const Split w = split_rows(B, L);
+  const int64_t chunks = loss_chunks(L);
   const bool vec = vec_ok(L, {logp, old_logp, ref_logp, adv_per_token ? advantages : nullptr, grad}, mask);
-  if (vec) k_policy_counts<true><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
-  else k_policy_counts<false><<<cgrid, kLossThreads, 0, s>>>(a, parts, width, counts, ticket);
+  const int grid = loss_grid(B * chunks, kLossBlocks);
+  if (B * L <= kTogether) {
+    const auto kernel = vec ? (ref_logp ? k_policy<true, true> : k_policy<true, false>)
+                            : (ref_logp ? k_policy<false, true> : k_policy<false, false>);
+    return launch_with(cudaLaunchAttributeCooperative, kernel, grid, s, a, chunks, w, counts, part, ticket);
+  }
+  const int cgrid = loss_grid(w.items, 8);
+  if (vec) k_policy_counts<true><<<cgrid, kLossThreads, 0, s>>>(a, w, counts, ticket);
+  else k_policy_counts<false><<<cgrid, kLossThreads, 0, s>>>(a, w, counts, ticket);
   if (cudaGetLastError() != cudaSuccess) return ASRN_ERR_CUDA;
-  const auto main_kernel = vec ? (ref_logp ? k_policy_main<true, true> : k_policy_main<true, false>)
-                               : (ref_logp ? k_policy_main<false, true> : k_policy_main<false, false>);
-  return launch_behind(main_kernel, grid, s, a, chunks, parts, counts, part, ticket);
+  const auto kernel = vec ? (ref_logp ? k_policy_main<true, true> : k_policy_main<true, false>)
+                          : (ref_logp ? k_policy_main<false, true> : k_policy_main<false, false>);
+  return launch_with(cudaLaunchAttributeProgrammaticStreamSerialization, kernel, grid, s, a, chunks, w, counts, part, ticket);
 }
 
 }  // extern "C"
