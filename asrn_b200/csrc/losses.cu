@@ -521,9 +521,11 @@ k_policy_main(PolicyArgs a, int64_t chunks, Split w, const int* counts, BlockSum
 
 int64_t loss_chunks(int64_t L) { return (L + kLossChunk - 1) / kLossChunk; }
 
-// One cooperative launch up to here, two overlapping ones above: the second launch costs the host about 3 us, the
-// cooperative one the GPU about 4 (it starts on an idle GPU and its barrier is one). See the table at the top.
-constexpr int64_t kTogether = 1 << 19;
+// Tokens up to which one cooperative launch does it all, and above which two overlapping launches do. The second launch
+// costs the host about 2.5 us; the cooperative one costs the GPU about 4: it starts on an idle GPU, holds fewer blocks, and
+// waits at its barrier. Us a call, two launches / one: preference 20.9 / 18.3 at 2^16 and at 2^21 tokens, 22.7 / 26.5 at
+// 512 pairs x 4096 (27.5 / 24.6 at 1024 x 2048); policy 19.5 / 17.3 at 2^16, 19.5 / 18.4 at 2^20, 20.5 / 22.6 at 2^21.
+constexpr int64_t kPrefTogether = 1 << 21, kPolicyTogether = 1 << 20;
 
 int loss_grid(int64_t items, int per_sm) {
   static int sms = 0;
@@ -570,6 +572,7 @@ Split split_rows(int64_t rows, int64_t L) {
   return Split{rows * parts, parts, (chunks + parts - 1) / parts * kLossChunk};
 }
 
+// One block by itself: no workspace to allocate, 15.8 us a call against 17.7 for the cooperative launch.
 bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L <= 16384; }
 
 }  // namespace
@@ -602,7 +605,7 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   const Split w = split_rows(2 * P, L);
   RowSum* part = reinterpret_cast<RowSum*>(workspace);
   const bool vec = vec_ok(L, {logp, ref_logp, grad}, mask);
-  if (2 * P * L <= kTogether)
+  if (2 * P * L <= kPrefTogether)
     return launch_with(cudaLaunchAttributeCooperative, vec ? k_pref<true> : k_pref<false>, loss_grid(w.items, kLossBlocks), s,
                        a, w, part);
   const int grid = loss_grid(w.items, 8);
@@ -648,7 +651,7 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   const int64_t chunks = loss_chunks(L);
   const bool vec = vec_ok(L, {logp, old_logp, ref_logp, adv_per_token ? advantages : nullptr, grad}, mask);
   const int grid = loss_grid(B * chunks, kLossBlocks);
-  if (B * L <= kTogether) {
+  if (B * L <= kPolicyTogether) {
     const auto kernel = vec ? (ref_logp ? k_policy<true, true> : k_policy<true, false>)
                             : (ref_logp ? k_policy<false, true> : k_policy<false, false>);
     return launch_with(cudaLaunchAttributeCooperative, kernel, grid, s, a, chunks, w, counts, part, ticket);
