@@ -37,10 +37,12 @@ template <int CG> constexpr int bytes_b() { return kBN / CG * 128; }
 template <int CG> constexpr int stage_bytes() { return kBytesA + bytes_b<CG>(); }
 // Pieces of shared memory for results: two per warp of eight; sixteen warps share as many unless the epilogue has two
 // results (kOwn = 2), which costs a stage.
-template <int CG, class Epi> constexpr int stages() { return (CG == 1 ? 4 : 6) - (Epi::kWarps * Epi::kOwn > 16); }
+template <int CG, class Epi> constexpr int stages() {
+  return (CG == 1 ? 4 : 6) - (Epi::kWarps * Epi::kOwn > 16) - (Epi::kTable > 0);
+}
 constexpr int kPiece = 32 * 64;                          // 32 rows x 32 bf16 columns, 64-byte swizzle
 template <int CG, class Epi> constexpr size_t smem_bytes() {
-  return 1024 + (size_t)stages<CG, Epi>() * stage_bytes<CG>() + Epi::kWarps * Epi::kOwn * kPiece + 256;
+  return 1024 + (size_t)stages<CG, Epi>() * stage_bytes<CG>() + Epi::kWarps * Epi::kOwn * kPiece + Epi::kTable + 256;
 }
 
 struct Shape {
@@ -222,6 +224,7 @@ ASRN_DEV uint4 pack8(const float* v) {
 // A warp's way out for 32 rows x 32 columns of bf16: written to a piece of shared memory, from there by TMA. A piece is
 // written again once the copy that read it last is done.
 template <int Pieces> struct Out {
+  const uint32_t* table;                                 // the epilogue's
   uint8_t* piece;                                        // the warp's own
   int lane, turn;
   ASRN_DEV void put(const CUtensorMap* map, const float* v, int column, int first_row) {
@@ -252,7 +255,8 @@ template <int Pieces> struct Out {
   }
 };
 
-// Epi: struct with a Params type, kWarps (8 or 16), kOwn (pieces per warp), a constructor (Params, row, rows, shape, tile, the warp's part of the columns) and chunk(v[32],
+// Epi: struct with a Params type, kWarps (8 or 16), kOwn (pieces per warp), kTable (bytes of a table that its fill() makes
+// once per block; costs a stage), a constructor (Params, row, rows, shape, tile, the warp's part of the columns) and chunk(v[32],
 // column, Out, map_o, map_p), called by whole warps for the tile's chunks of 32 columns, then finish().
 template <int CG, bool AMn, bool BMn, class Epi>
 __global__ void __launch_bounds__(threads_of<Epi>(), 1)
@@ -267,7 +271,8 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   uint8_t* sA = sm;
   uint8_t* sB = sm + kS * kBytesA;
   uint8_t* sO = sB + kS * kStageB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sO + Epi::kWarps * Epi::kOwn * kPiece);
+  uint32_t* table = reinterpret_cast<uint32_t*>(sO + Epi::kWarps * Epi::kOwn * kPiece);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sO + Epi::kWarps * Epi::kOwn * kPiece + Epi::kTable);
   uint64_t* empty = full + kS;
   uint64_t* tfull = empty + kS;
   uint64_t* tempty = tfull + 2;
@@ -289,6 +294,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     prefetch_tensormap(&map_b);
   }
   if (wid == 1) alloc<CG>(tmem_s);
+  if constexpr (Epi::kTable > 0) Epi::fill(table, tid, threads_of<Epi>());
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync();
@@ -354,7 +360,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   } else {                                              // epilogue
     constexpr int kCols = kBN * 4 / Epi::kWarps, kOwn = Epi::kOwn;
     const int q4 = wid & 3, part = (wid - 2) >> 2;
-    Out<kOwn> out{sO + (wid - 2) * kOwn * kPiece, lane, 0};
+    Out<kOwn> out{table, sO + (wid - 2) * kOwn * kPiece, lane, 0};
     const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(part * kCols);
     int jt = 0;
     for (; walk.next(u); ++jt) {
@@ -416,7 +422,7 @@ ASRN_DEV void add_bias(float* v, const __nv_bfloat16* bias, int n) {
 // The fp32 sums of a piece of a tile, whole, to its slot: by blocks of 32 rows x 32 columns, each as the warp holds it
 // (four columns of all 32 rows are 512 neighbouring bytes).
 struct StorePiece {
-  static constexpr int kWarps = 8, kOwn = 2;
+  static constexpr int kWarps = 8, kOwn = 2, kTable = 0;
   struct Params {
     float* slots;
     int tile_rows;
@@ -436,7 +442,7 @@ struct StorePiece {
 // bf16(sum + bias + before): out[row][column] through map_o (N a multiple of 8). before: fp32 (M, N), the sum of what
 // came earlier; or, when `after` is given, the sum goes there in fp32 instead.
 struct StoreBf16 {
-  static constexpr int kWarps = 8, kOwn = 2;
+  static constexpr int kWarps = 8, kOwn = 2, kTable = 0;
   struct Params {
     const __nv_bfloat16* bias;
     const float* before;

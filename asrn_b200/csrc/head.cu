@@ -153,7 +153,7 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
 
 // Running maximum (of the unscaled scores) and sum of exponentials over the thread's columns.
 struct Lse {
-  static constexpr int kWarps = 8, kOwn = 1;
+  static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
   struct Params {
     const int* tok;
     float k;                               // log2(e) / tau
@@ -269,7 +269,7 @@ k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const in
 
 // dS of one chunk in bf16; the rows that pad the last tile get zeros.
 struct Slope {
-  static constexpr int kWarps = 16, kOwn = 1;
+  static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
   struct Params {
     const int *tok, *row;                  // of the chunk's rows
     const float *lse2, *rest, *g;

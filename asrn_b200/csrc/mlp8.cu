@@ -15,6 +15,7 @@
 //   k_gemm<Down>   dY W2 -> dA, gelu(a'), db1's partial sums by 32 rows
 //   k_gemm x 3     dX, dW1, dW2 (the last two in shares of N: few tiles)
 //   k_colsum       db1, db2
+#include <cuda_fp16.h>
 #include "common.cuh"
 #include "gemm_tc.cuh"
 
@@ -88,26 +89,28 @@ ASRN_DEV void tails(float a0, float a1, gemm::F2& e, gemm::F2& q) {
   q = mul2(mul2(r, t), e);
 }
 
-// The codes of a block to `at` (n values of it, a multiple of 8; wide: 16-byte stores fit); its exponent.
-ASRN_DEV int store_codes(const float* v, uint8_t* at, int n, bool wide) {
+// mlp8 keeps a's codes by 32 rows x 32 columns, as a warp of the products' epilogues holds them: first 16 columns of the 32
+// rows, then the other 16, so that its 16 bytes a lane are 512 neighbouring ones (rows as they lie would make 32 half-used
+// accesses of each). The last rows may be fewer than 32. A lane's two places:
+struct CodesAt {
+  int64_t first;
+  int other;                                             // from the first 16 columns to the others
+  ASRN_DEV CodesAt(int row, int rows, int c, int f) {
+    const int in = min(32, rows - (row & ~31));
+    first = (int64_t)(row & ~31) * ((f + 31) / 32 * 32) + c * in + (row & 31) * 16;
+    other = in * 16;
+  }
+};
+// The codes of a lane's 32 columns; their exponent.
+ASRN_DEV int store_codes(const float* v, uint8_t* codes, const CodesAt& at) {
   const int e = block_exp(abs_max32(v));
   const float inv = inv_scale_of(e);
-  if (wide && n >= 32) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 16) {
-      uint4 w = make_uint4(codes4(v + i, inv), codes4(v + i + 4, inv), codes4(v + i + 8, inv), codes4(v + i + 12, inv));
-      if (e == kBad) w = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(at + i) = w;
-    }
-    return e;
+  for (int i = 0; i < 32; i += 16) {
+    uint4 w = make_uint4(codes4(v + i, inv), codes4(v + i + 4, inv), codes4(v + i + 8, inv), codes4(v + i + 12, inv));
+    if (e == kBad) w = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(codes + at.first + (i ? at.other : 0)) = w;
   }
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (i < n) {
-      uint2 w = make_uint2(codes4(v + i, inv), codes4(v + i + 4, inv));
-      if (e == kBad) w = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>(at + i) = w;
-    }
   return e;
 }
 
@@ -200,22 +203,21 @@ __global__ void __launch_bounds__(256) k_unpack8(int64_t total, int f, const uin
 
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
 struct Up {
-  static constexpr int kWarps = 16, kOwn = 1;
+  static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
   struct Params {
     const __nv_bfloat16* bias;
     uint8_t* codes;
     Exps exps;
   };
   const Params& p;
-  int64_t at;
-  int N, row, first;
+  int N, row, first, rows;
   bool on;
-  ASRN_DEV Up(const Params& pp, int r, int rows, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)r * s.N), N(s.N), row(r), first(r & ~31), on(r < rows) {}
+  ASRN_DEV Up(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
+      : p(pp), N(s.N), row(r), first(r & ~31), rows(m), on(r < m) {}
   template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
     if (c >= N) return;                        // the columns past N of the last block are zeros
     gemm::add_bias(v, p.bias + c, N - c);
-    if (p.codes && on) p.exps(row, c / 32) = (int8_t)store_codes(v, p.codes + at + c, N - c, N % 16 == 0);
+    if (p.codes && on) p.exps(row, c / 32) = (int8_t)store_codes(v, p.codes, CodesAt(row, rows, c, N));
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       gemm::F2 e, q;
@@ -242,57 +244,91 @@ ASRN_DEV float column_sum(float* v, int lane) {
   return v[0];
 }
 
+// gelu(a) and gelu'(a) for the pair's cdf and density.
+ASRN_DEV void gelu_both(float a0, float a1, gemm::F2& g, gemm::F2& slope) {
+  using namespace gemm;
+  F2 e, q;
+  tails(a0, a1, e, q);
+  float h0, h1;
+  fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                                       // 1/2 - q
+  const F2 a(a0, a1), cdf = add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
+  g = mul2(a, cdf);
+  slope = fma2(mul2(a, F2(0.39894228040143268f)), e, cdf);
+}
+
 // dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows.
+// a' = code 2^e takes 256 values for each e, so gelu and gelu' of the 16 exponents that matter lie in a table of shared
+// memory (gelu in bf16, as it leaves; gelu' in fp16, whose 2^-12 adds 1 % to the bf16 rounding of dA): one 32-bit load
+// for an element instead of about 20 instructions. Blocks with another exponent (all of a below 0.004, or some above 254)
+// are computed.
 struct Down {
-  static constexpr int kWarps = 16, kOwn = 2;
+  static constexpr int kWarps = 16, kOwn = 2, kLow = -14, kExps = 16, kTable = kExps * 1024;
   struct Params {
     const uint8_t* codes;
     Exps exps;
     float* sums;                               // [ceil(rows / 32)][N], or null
   };
   const Params& p;
-  int64_t at;
   int N, row, first, rows;
   bool on;
   ASRN_DEV Down(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
-      : p(pp), at((int64_t)r * s.N), N(s.N), row(r), first(r & ~31), rows(m), on(r < m) {}
+      : p(pp), N(s.N), row(r), first(r & ~31), rows(m), on(r < m) {}
+  static ASRN_DEV void fill(uint32_t* table, int tid, int threads) {
+    for (int t = tid; t < kExps * 128; t += threads) {     // two codes each: code = place - 128
+      const float scale = pow2(t / 128 + kLow), a0 = (float)(2 * (t % 128) - 128) * scale, a1 = a0 + scale;
+      gemm::F2 g, slope;
+      gelu_both(a0, a1, g, slope);
+      float g0, g1, s0, s1;
+      g.get(g0, g1);
+      slope.get(s0, s1);
+      const uint32_t w = umma::pack_bf16x2(g0, g1);
+      table[2 * t] = w << 16 | __half_as_ushort(__float2half_rn(s0));
+      table[2 * t + 1] = (w & 0xffff0000u) | __half_as_ushort(__float2half_rn(s1));
+    }
+  }
   template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
-    using gemm::F2;
     if (c >= N) return;                        // the same for the whole warp
-    const float scale = on ? scale_of(p.exps(row, c / 32)) : 0.f;
+    const int exp = on ? p.exps(row, c / 32) : kLow;
     uint4 codes[2] = {};
     if (on) {
-      const uint8_t* at_c = p.codes + at + c;
-      if (N % 16 == 0 && c + 32 <= N) {
-        codes[0] = __ldg(reinterpret_cast<const uint4*>(at_c));
-        codes[1] = __ldg(reinterpret_cast<const uint4*>(at_c) + 1);
-      } else {
-        uint2* w = reinterpret_cast<uint2*>(codes);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + 8 * i < N) w[i] = __ldg(reinterpret_cast<const uint2*>(at_c) + i);
-      }
+      const CodesAt at(row, rows, c, N);
+      codes[0] = __ldg(reinterpret_cast<const uint4*>(p.codes + at.first));
+      codes[1] = __ldg(reinterpret_cast<const uint4*>(p.codes + at.first + at.other));
     }
     uint4 packed[4];
+    if (__all_sync(0xffffffffu, exp >= kLow && exp < kLow + kExps)) {
+      const uint32_t* row_of_e = out.table + (exp - kLow) * 256 + 128;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      const uint4& k = codes[i / 16];
-      float g[8];
-      values4(g, i % 16 ? k.z : k.x, scale);
-      values4(g + 4, i % 16 ? k.w : k.y, scale);
+      for (int i = 0; i < 32; i += 8) {
+        const uint4& k = codes[i / 16];
+        uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float a0 = g[j], a1 = g[j + 1];
-        F2 e, q;
-        tails(a0, a1, e, q);
-        float h0, h1;
-        gemm::fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                           // 1/2 - q
-        const F2 cdf = gemm::add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
-        const F2 slope = gemm::fma2(gemm::mul2(F2(a0, a1), F2(0.39894228040143268f)), e, cdf);
-        gemm::mul2(F2(v[i + j], v[i + j + 1]), slope).get(v[i + j], v[i + j + 1]);
-        gemm::mul2(F2(a0, a1), cdf).get(g[j], g[j + 1]);
+        for (int j = 0; j < 8; j += 2) {
+          const uint32_t four = (j < 4) == (i % 16 == 0) ? (j < 4 ? k.x : k.w) : (j < 4 ? k.z : k.y);
+          const uint32_t t0 = row_of_e[(int8_t)(four >> (8 * (j & 3)))], t1 = row_of_e[(int8_t)(four >> (8 * (j & 3) + 8))];
+          v[i + j] *= __half2float(__ushort_as_half((unsigned short)t0));
+          v[i + j + 1] *= __half2float(__ushort_as_half((unsigned short)t1));
+          w[j / 2] = __byte_perm(t0, t1, 0x7632);
+        }
+        packed[i / 8] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      packed[i / 8] = gemm::pack8(g);
+    } else {
+      const float scale = scale_of(exp);
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        const uint4& k = codes[i / 16];
+        float g[8];
+        values4(g, i % 16 ? k.z : k.x, scale);
+        values4(g + 4, i % 16 ? k.w : k.y, scale);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          gemm::F2 f, slope;
+          gelu_both(g[j], g[j + 1], f, slope);
+          f.get(g[j], g[j + 1]);
+          gemm::mul2(gemm::F2(v[i + j], v[i + j + 1]), slope).get(v[i + j], v[i + j + 1]);
+        }
+        packed[i / 8] = gemm::pack8(g);
+      }
     }
     out.put(map_p, packed, c, first);
     out.put(map_o, v, c, first);
@@ -379,7 +415,7 @@ Mlp8Saved mlp8_saved(int64_t N, int64_t d, int64_t ff) {
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.xc = take((size_t)N * d);
   w.xe = take((size_t)N * ((d + 31) / 32));
-  w.ac = take((size_t)N * ff);
+  w.ac = take((size_t)N * ((ff + 31) / 32) * 32);
   w.ae = take((size_t)N * ((ff + 31) / 32));
   w.total = o;
   return w;
