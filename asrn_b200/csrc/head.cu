@@ -269,7 +269,7 @@ k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const in
 
 // dS of one chunk in bf16; the rows that pad the last tile get zeros.
 struct Slope {
-  static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
+  static constexpr int kWarps = 8, kOwn = 2, kTable = 0;
   struct Params {
     const int *tok, *row;                  // of the chunk's rows
     const float *lse2, *rest, *g;
