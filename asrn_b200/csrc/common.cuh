@@ -86,6 +86,14 @@ ASRN_DEV void red_add_bf16(__nv_bfloat16* addr, float a) {
   asm volatile("red.global.add.noftz.bf16 [%0], %1;" ::"l"(addr), "h"(v) : "memory");
 }
 
+// ---- overlapping launches ---------------------------------------------------------------------------------------------
+// A kernel launched with programmatic stream serialisation may start while the one before it on the stream ends; it waits
+// here until that one's results are there.
+ASRN_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel's blocks start once all of this one's have come here or ended. After wait_previous: then everything
+// before this kernel is complete when the next one starts, and only this kernel's results have to be waited for.
+ASRN_DEV void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- torch-compatible scalar math ----------------------------------------------------------------------------------
 // torch.nn.functional.softplus with beta = 1, threshold = 20.
 ASRN_DEV float softplus_t(float x) { return x > 20.f ? x : log1pf(expf(x)); }

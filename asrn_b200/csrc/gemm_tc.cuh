@@ -300,6 +300,8 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
   if (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_s;
+  wait_previous();                                      // the setup above overlaps the end of the kernel before
+  let_next();
 
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
   Walk walk(s, M, K, CG, blockIdx.x / CG, gridDim.x / CG);
@@ -488,6 +490,8 @@ struct JoinArgs {
   int64_t zero_n;
 };
 static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinArgs a) {
+  wait_previous();
+  let_next();
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
   const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN, kblocks = (K + kBK - 1) / kBK;
   const int per = a.tile_rows / 32, lane = threadIdx.x & 31;              // blocks of 32 rows of a tile
@@ -587,12 +591,14 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
   cfg.blockDim = dim3(threads_of<Epi>());
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 1 ? 0 : 1;
+  cfg.numAttrs = CG;
   return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, mq, s, p) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 
@@ -623,8 +629,17 @@ inline int join(const Shape& s, const float* slots, void* out, const int* row_of
                 cudaStream_t stream) {
   const int rows = kBM * pair_for(s.M);
   const int64_t blocks = tiles_m(s.M, pair_for(s.M)) * tiles_n(s.N) * (rows / 32);
-  k_join<<<(unsigned)blocks, 256, 0, stream>>>(s, {slots, reinterpret_cast<__nv_bfloat16*>(out), rows, row_of, pos, zero_n});
-  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const JoinArgs a{slots, reinterpret_cast<__nv_bfloat16*>(out), rows, row_of, pos, zero_n};
+  return cudaLaunchKernelEx(&cfg, k_join, s, a) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
 }
 // Bytes of a share walk's slots.
 inline size_t slot_bytes(int64_t M, int64_t N, int shares) {

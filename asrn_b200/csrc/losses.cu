@@ -89,11 +89,6 @@ template <bool Vec> __device__ __forceinline__ void store4(float* p, const float
 
 __device__ __forceinline__ int chunk_left(int64_t L, int64_t t) { return (int)min(L - t, (int64_t)kLossChunk); }
 
-// A kernel launched behind another of the same call starts while that one ends; waits here for its results.
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next kernel's blocks start once all of this one's have come here or ended.
-__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Rows in parts that blocks take: items = rows x parts, each of `width` tokens, a multiple of the chunk.
 struct Split {
   int64_t items, parts, width;
