@@ -319,22 +319,31 @@ __device__ __forceinline__ float held20(float x) {
   return y;
 }
 
+// e^x for |x| <= 20: 2^(x log2 e), the product's rounding (and log2 e's own) made up for.
+__device__ __forceinline__ float exp_held(float x) {
+  const float t = x * 1.4426950408889634f;
+  const float lost = fmaf(x, 1.4426950408889634f, -t) + x * 1.9259629911e-8f;
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fmaf(e * 0.6931471805599453f, lost, e);
+}
+
 // One token of the loss. The ratio's bounds are compared in the log domain, where the log ratio is exact or nearly so:
-// which side a token falls on does not hang on expf's last bit. exp(q) - 1 - q and exp(q) - 1 come from Taylor's series
+// which side a token falls on does not hang on an exponential's last bit. exp(q) - 1 - q and exp(q) - 1 come from Taylor's series
 // below 1/4 (its next term is under 4e-7 of the sum), where the differences would cancel.
 template <bool Ref>
 __device__ __forceinline__ Token token_of(const PolicyArgs& a, float lp, float old, float rf, float adv) {
   Token t;
   const float d = lp - old, lr = held20(d);
   t.cut = adv > 0.f ? lr > a.log_high : adv < 0.f && lr < a.log_low;
-  const float r = t.cut ? (adv > 0.f ? a.high : a.low) : expf(lr);
+  const float r = t.cut ? (adv > 0.f ? a.high : a.low) : exp_held(lr);
   t.loss = -r * adv;
   t.slope = t.cut || fabsf(d) > 20.f ? 0.f : t.loss;
   t.kl = 0.f;
   if (Ref) {
     const float dq = rf - lp, q = held20(dq);
     const bool near = fabsf(q) < 0.25f;
-    const float e = expf(q) - 1.f;
+    const float e = exp_held(q) - 1.f;
     t.kl = near ? q * q * (0.5f + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720))))) : e - q;
     t.loss = fmaf(a.kl, t.kl, t.loss);
     t.slope = fabsf(dq) > 20.f ? t.slope : fmaf(-a.kl, near ? q + t.kl : e, t.slope);
@@ -424,7 +433,14 @@ __device__ __forceinline__ void policy_main(const PolicyArgs& a, int64_t chunks,
   int64_t row = blockIdx.x / chunks, t = blockIdx.x % chunks * kLossChunk;
   // the mask comes an item ahead: a warp whose tokens are all outside it reads nothing else
   uint32_t next = row < a.B ? load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t)) : 0;
+  // and so do its row's count and advantage
+  const auto row_share = [&](int64_t r) {
+    return a.per_sequence && r < a.B ? 1.f / (float)max(1, row_count(counts, r, parts)) : 1.f;
+  };
+  const auto row_advantage = [&](int64_t r) { return a.adv_per_token || r >= a.B ? 0.f : __ldg(a.adv + r); };
+  float next_adv = row_advantage(row);
   ready();
+  float next_share = row_share(row);
   double n[2] = {0., 0.};
   for (int64_t b = threadIdx.x; b < a.B; b += kLossThreads) {
     const int c = row_count(counts, b, parts);
@@ -436,9 +452,7 @@ __device__ __forceinline__ void policy_main(const PolicyArgs& a, int64_t chunks,
   double v[3] = {0., 0., 0.};
   int cut = 0;
   while (row < a.B) {
-    float share = 1.f, row_adv = 0.f;
-    if (a.per_sequence) share = 1.f / (float)max(1, row_count(counts, row, parts));
-    if (!a.adv_per_token) row_adv = a.adv[row];
+    const float share = next_share, row_adv = next_adv;
     const float w = share * over;
     const int64_t at = row * a.L + t;
     const int left = chunk_left(a.L, t);
@@ -459,6 +473,8 @@ __device__ __forceinline__ void policy_main(const PolicyArgs& a, int64_t chunks,
       if (a.adv_per_token) load4<Vec>(adv, a.adv + at, left);
     }
     if (row < a.B) next = load_mask<Vec>(a.mask + row * a.L + t, chunk_left(a.L, t));
+    next_share = row_share(row);
+    next_adv = row_advantage(row);
     if (any) {
       float loss = 0.f, kl = 0.f;
 #pragma unroll
