@@ -19,6 +19,10 @@
 // M tiles laid end to end, so that the blocks that read the same part of A do so together. A share's pieces of tiles go
 // to fp32 slots that k_join adds up in order.
 //
+// An operand that was rounded to bf16 can be given as two, the rounded values and what the rounding took, stacked in one
+// tensor: the product then runs over K twice (`passes`), the second time on the remainders. Operators do so for few rows,
+// where one rounding error can be most of a result's; a sum over many rows averages them.
+//
 // Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, frees its TMEM and
 // ends.
 #pragma once
@@ -54,6 +58,8 @@ struct Shape {
   int shares;              // groups of clusters that walk equal shares, or 0: whole tiles
   int group;               // whole tiles: M tiles walked before the next N tile
   int* status;
+  int passes_less_one;     // 1: K is walked again with the operands' outer coordinates moved by these
+  int a_step, b_step;
 };
 
 struct Tile {
@@ -84,6 +90,7 @@ struct Walk {
   ASRN_DEV Walk(const Shape& s, int M, int K, int cg, int cluster, int clusters)
       : mt((M + kBM * cg - 1) / (kBM * cg)), nt((s.N + kBN - 1) / kBN), kblocks((K + kBK - 1) / kBK), group(s.group),
         at(cluster), step(clusters), share(-1), u(0), end(0) {
+    kblocks *= 1 + s.passes_less_one;
     if (s.shares) {
       share = cluster / nt;
       at = cluster % nt;
@@ -210,6 +217,11 @@ ASRN_DEV F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+// v less what rounding it to bf16 leaves.
+ASRN_DEV void remainder(float* v) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] -= round_bf16(v[i]);
+}
 ASRN_DEV float exp2_fast(float x) {                      // 2^x, 2 units in the last place
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -309,11 +321,14 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
 
   if (wid == 0) {
     if (lane == 0) {                                    // operand producer
+      const int kblocks = (K + kBK - 1) / kBK;          // of one pass
       int it = 0;
       bool ok = true;
       while (ok && walk.next(u)) {
         const int m0 = (u.m * CG + (int)rank) * kBM, n0 = u.n * kBN + (int)rank * (kBN / CG);
-        for (int kb = u.k0; kb < u.k1; ++kb, ++it) {
+        for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+          const int again = kt >= kblocks, kb = kt - again * kblocks;
+          const int a_at = again * s.a_step, b_at = again * s.b_step;
           const int st = it % kS;
           if (it >= kS && !(ok = mbar_wait(empty + st, ((it / kS) - 1) & 1, s.status))) break;
           if (rank == 0) mbar_expect_tx(full + st, (uint32_t)(CG * stage_bytes<CG>()));
@@ -321,16 +336,16 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           if (AMn) {
 #pragma unroll
             for (int i = 0; i < kBM / 64; ++i)
-              load_box<CG>(sA + st * kBytesA + i * 8192, &map_a, m0 + i * 64, kb * kBK, bar);
+              load_box<CG>(sA + st * kBytesA + i * 8192, &map_a, m0 + i * 64, kb * kBK + a_at, bar);
           } else {
-            load_box<CG>(sA + st * kBytesA, &map_a, kb * kBK, m0, bar);
+            load_box<CG>(sA + st * kBytesA, &map_a, kb * kBK, m0 + a_at, bar);
           }
           if (BMn) {
 #pragma unroll
             for (int i = 0; i < kBN / CG / 64; ++i)
-              load_box<CG>(sB + st * kStageB + i * 8192, &map_b, n0 + i * 64, kb * kBK, bar);
+              load_box<CG>(sB + st * kStageB + i * 8192, &map_b, n0 + i * 64, kb * kBK + b_at, bar);
           } else {
-            load_box<CG>(sB + st * kStageB, &map_b, kb * kBK, n0, bar);
+            load_box<CG>(sB + st * kStageB, &map_b, kb * kBK, n0 + b_at, bar);
           }
         }
       }
@@ -493,7 +508,8 @@ static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinAr
   wait_previous();
   let_next();
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
-  const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN, kblocks = (K + kBK - 1) / kBK;
+  const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN;
+  const int kblocks = (K + kBK - 1) / kBK * (1 + s.passes_less_one);
   const int per = a.tile_rows / 32, lane = threadIdx.x & 31;              // blocks of 32 rows of a tile
   const int64_t all = (int64_t)mt * kblocks;
   const int tile = blockIdx.x / per, m = tile / nt, n = tile % nt, part = blockIdx.x % per;
@@ -569,7 +585,9 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
               const typename Epi::Params& p, const Dest& o, const Dest& q, cudaStream_t stream) {
   CUtensorMap ma, mb, mo, mq;
   if (!bind_context()) return ASRN_ERR_CUDA;
-  if (!operand_map(&ma, A, AMn, s.M, s.K, pitch_a, kBM) || !operand_map(&mb, B, BMn, s.N, s.K, pitch_b, kBN / CG))
+  const int again = s.passes_less_one;                     // the stacked operand is longer in its outer dimension
+  if (!operand_map(&ma, A, AMn, AMn ? s.M : s.M + again * s.a_step, AMn ? s.K + again * s.a_step : s.K, pitch_a, kBM) ||
+      !operand_map(&mb, B, BMn, BMn ? s.N : s.N + again * s.b_step, BMn ? s.K + again * s.b_step : s.K, pitch_b, kBN / CG))
     return ASRN_ERR_CUDA;
   mo = mq = ma;                                            // not read where there is no destination
   if ((o.base && !make_tmap_bf16_sw64(&mo, o.base, (uint64_t)o.columns, (uint64_t)o.rows, (uint64_t)o.pitch * 2, 32, 32)) ||

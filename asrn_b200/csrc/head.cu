@@ -15,7 +15,8 @@
 //   k_head_join    the pairs of a row joined: logp, and lse and 1 - p_y for the backward pass
 //   k_gemm<Slope>  backward, by chunks of rows: the scores again, dS in bf16
 //   k_gemm         dh = dS W (parts of V where rows are few) and dW = dS^T h, sums in fp32
-// dS is rounded to bf16 once, as the operand of both products.
+// dS is rounded to bf16 once, as the operand of both products; for few rows (kTwiceRows), where the target's own rounding
+// error would be nearly all of dh's and dW's, the products take its remainder too.
 #include "common.cuh"
 #include "gemm_tc.cuh"
 
@@ -26,6 +27,7 @@ namespace {
 constexpr int kGatherRows = 16, kGatherThreads = 256;
 constexpr int kCountRows = 1024;
 constexpr int64_t kDirectRows = 4096;    // up to here each block counts the targets before it by itself: a launch less
+constexpr int64_t kTwiceRows = 512, kTwiceWork = (int64_t)1 << 34;   // and rows x V x d: 34 us more at the most
 constexpr float kLog2e = 1.4426950408889634f;
 
 int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -70,7 +72,7 @@ HeadForwardWs head_forward_ws(int64_t N, int64_t V) {
 // sum so far then waits in fp32).
 struct HeadBackwardWs {
   int64_t rows, pitch;
-  int chunks, shares_h, shares_w;
+  int twice, chunks, shares_h, shares_w;
   size_t ds, dh, dw, total;
 };
 
@@ -81,11 +83,12 @@ HeadBackwardWs head_backward_ws(int64_t N, int64_t V, int64_t d) {
   w.chunks = (int)((pad256(N) + most - 1) / most);
   w.rows = std::max<int64_t>(256, pad256((N + w.chunks - 1) / std::max(1, w.chunks)));
   w.chunks = (int)((pad256(N) + w.rows - 1) / w.rows);
-  w.shares_h = gemm::groups_for(w.rows, d, V);
-  w.shares_w = w.chunks > 1 ? 0 : gemm::shares_for(V, d, w.rows);
+  w.twice = N <= kTwiceRows && N * V * d <= kTwiceWork && w.chunks == 1;
+  w.shares_h = gemm::groups_for(w.rows, d, V * (1 + w.twice));
+  w.shares_w = w.chunks > 1 ? 0 : gemm::shares_for(V, d, w.rows * (1 + w.twice));
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
-  w.ds = take((size_t)w.rows * w.pitch * 2);
+  w.ds = take((size_t)(1 + w.twice) * w.rows * w.pitch * 2);
   w.dh = take(gemm::slot_bytes(w.rows, d, w.shares_h));
   w.dw = take(w.shares_w ? gemm::slot_bytes(V, d, w.shares_w) : w.chunks > 1 ? (size_t)V * d * 4 : 0);
   w.total = o;
@@ -274,6 +277,7 @@ struct Slope {
     const int *tok, *row;                  // of the chunk's rows
     const float *lse2, *rest, *g;
     float k, inv_tau;
+    int below;                             // rows from dS to its remainder, 0: none
   };
   const Params& p;
   int V, y, first;
@@ -302,6 +306,10 @@ struct Slope {
       for (int i = 0; i < 32; ++i) v[i] = i == j ? own : v[i];
     }
     out.put(map_o, v, c, first);
+    if (p.below) {
+      gemm::remainder(v);
+      out.put(map_o, v, c, first + p.below);
+    }
   }
   ASRN_DEV void finish() {}
 };
@@ -406,11 +414,13 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
     const int* row = reinterpret_cast<const int*>(S + sv.row) + first;
     Slope::Params p{reinterpret_cast<const int*>(S + sv.tok) + first, row,
                     reinterpret_cast<const float*>(S + sv.lse2) + first,
-                    reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau};
-    if ((st = gemm::launch<false, false, Slope>(hc, d, weight, d, sh, p, s, {ds, rows, ws.pitch, ws.pitch}))) return st;
+                    reinterpret_cast<const float*>(S + sv.rest) + first, g, kLog2e / tau, 1.f / tau,
+                    ws.twice ? rows : 0};
+    if ((st = gemm::launch<false, false, Slope>(hc, d, weight, d, sh, p, s, {ds, (1 + ws.twice) * rows, ws.pitch, ws.pitch}))) return st;
     if (dh) {
       gemm::Shape a{};
       a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.shares = ws.shares_h; a.status = status;
+      a.passes_less_one = ws.twice; a.a_step = rows;
       const gemm::StorePiece::Params q{dh_slots, gemm::kBM * gemm::pair_for(rows)};
       if ((st = gemm::launch<false, true, gemm::StorePiece>(ds, ws.pitch, weight, d, a, q, s)) ||
           (st = gemm::join(a, dh_slots, dh, row, reinterpret_cast<const int*>(S + sv.pos), c ? 0 : N, s)))
@@ -419,7 +429,7 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
     if (dw) {
       gemm::Shape a{};
       a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.shares = ws.shares_w; a.group = 16;
-      a.status = status;
+      a.status = status; a.passes_less_one = ws.twice; a.a_step = rows;
       if (ws.shares_w) {
         const gemm::StorePiece::Params q{dw_sum, gemm::kBM * gemm::pair_for(V)};
         if ((st = gemm::launch<true, true, gemm::StorePiece>(ds, ws.pitch, hc, d, a, q, s)) ||

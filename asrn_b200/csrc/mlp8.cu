@@ -7,7 +7,8 @@
 // (d + ff) 33/32 bytes a row instead of bf16 x, a and gelu(a) and their fp32 neighbours.
 //
 // Bound by the tensor cores: 12 N d ff operations in six products; the elementwise work is their epilogue. gelu(a) and
-// dA are rounded to bf16 once each, as operands; dY W2 stays in fp32 until it is multiplied by gelu'.
+// dA are rounded to bf16 once each, as operands (up to kTwiceRows rows the products take what the rounding took, too); dY
+// W2 stays in fp32 until it is multiplied by gelu'.
 //   k_pack8        x -> Q(x)
 //   k_gemm<Up>     a, Q(a), gelu(a)
 //   k_gemm         y
@@ -23,6 +24,7 @@ namespace asrn {
 
 namespace {
 
+constexpr int64_t kTwiceRows = 512;
 constexpr int kBad = -128;                     // exponent byte of a block that holds an infinity or a NaN
 
 // The exponent of a block whose largest magnitude is m.
@@ -208,6 +210,7 @@ struct Up {
     const __nv_bfloat16* bias;
     uint8_t* codes;
     Exps exps;
+    int below;                                 // rows from gelu(a) to its remainder, 0: none
   };
   const Params& p;
   int N, row, first, rows;
@@ -215,7 +218,7 @@ struct Up {
   ASRN_DEV Up(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
       : p(pp), N(s.N), row(r), first(r & ~31), rows(m), on(r < m) {}
   template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
-    if (c >= N) return;                        // the columns past N of the last block are zeros
+    if (c >= N || first >= rows) return;       // the same for the whole warp; columns past N of the last block are zeros
     gemm::add_bias(v, p.bias + c, N - c);
     if (p.codes && on) p.exps(row, c / 32) = (int8_t)store_codes(v, p.codes, CodesAt(row, rows, c, N));
 #pragma unroll
@@ -226,6 +229,10 @@ struct Up {
           .get(v[i], v[i + 1]);
     }
     out.put(map_o, v, c, first);
+    if (p.below) {
+      gemm::remainder(v);
+      out.put(map_o, v, c, first + p.below);
+    }
   }
   ASRN_DEV void finish() {}
 };
@@ -267,6 +274,7 @@ struct Down {
     const uint8_t* codes;
     Exps exps;
     float* sums;                               // [ceil(rows / 32)][N], or null
+    int below;                                 // rows from dA and gelu(a') to their remainders, 0: none
   };
   const Params& p;
   int N, row, first, rows;
@@ -287,7 +295,7 @@ struct Down {
     }
   }
   template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
-    if (c >= N) return;                        // the same for the whole warp
+    if (c >= N || first >= rows) return;       // the same for the whole warp
     const int exp = on ? p.exps(row, c / 32) : kLow;
     uint4 codes[2] = {};
     if (on) {
@@ -295,8 +303,8 @@ struct Down {
       codes[0] = __ldg(reinterpret_cast<const uint4*>(p.codes + at.first));
       codes[1] = __ldg(reinterpret_cast<const uint4*>(p.codes + at.first + at.other));
     }
-    uint4 packed[4];
-    if (__all_sync(0xffffffffu, exp >= kLow && exp < kLow + kExps)) {
+    uint4 packed[4], rest[4];
+    if (!p.below && __all_sync(0xffffffffu, exp >= kLow && exp < kLow + kExps)) {
       const uint32_t* row_of_e = out.table + (exp - kLow) * 256 + 128;
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
@@ -328,11 +336,24 @@ struct Down {
           gemm::mul2(gemm::F2(v[i + j], v[i + j + 1]), slope).get(v[i + j], v[i + j + 1]);
         }
         packed[i / 8] = gemm::pack8(g);
+        if (p.below) {
+          float r[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[j] = g[j] - round_bf16(g[j]);
+          rest[i / 8] = gemm::pack8(r);
+        }
       }
+      if (p.below) out.put(map_p, rest, c, first + p.below);
     }
     out.put(map_p, packed, c, first);
     out.put(map_o, v, c, first);
-    if (p.sums && first < rows) {              // rows past the end are zeros: the operand's rows were
+    if (p.below) {
+      float r[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = v[i] - round_bf16(v[i]);
+      out.put(map_o, r, c, first + p.below);
+    }
+    if (p.sums) {                              // rows past the end are zeros: the operand's rows were
       const int lane = threadIdx.x & 31;
       const float s = column_sum(v, lane);
       if (c + lane < N) p.sums[(int64_t)(first / 32) * N + c + lane] = s;
@@ -422,7 +443,8 @@ Mlp8Saved mlp8_saved(int64_t N, int64_t d, int64_t ff) {
 }
 
 struct Mlp8Ws {
-  int shares1, shares2;
+  int64_t rows;                                // of gelu(a) and dA, their remainders among them
+  int below, shares1, shares2;                 // below: rows to the remainders (a multiple of 32), 0: none
   size_t da, g, x, sum1, sum2, slots, total;
 };
 
@@ -430,11 +452,13 @@ Mlp8Ws mlp8_ws(int64_t N, int64_t d, int64_t ff, int64_t dout, bool backward) {
   Mlp8Ws w{};
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
-  w.g = take((size_t)N * ff * 2);
+  w.below = N <= kTwiceRows ? (int)((N + 31) / 32 * 32) : 0;
+  w.rows = w.below ? 2 * w.below : N;
+  w.g = take((size_t)w.rows * ff * 2);
   if (backward) {
-    w.shares1 = gemm::shares_for(ff, d, N);
-    w.shares2 = gemm::shares_for(dout, ff, N);
-    w.da = take((size_t)N * ff * 2);
+    w.shares1 = gemm::shares_for(ff, d, w.rows);
+    w.shares2 = gemm::shares_for(dout, ff, w.rows);
+    w.da = take((size_t)w.rows * ff * 2);
     w.x = take((size_t)N * d * 2);
     w.sum1 = take((size_t)((N + 31) / 32) * ff * 4);
     w.sum2 = take((size_t)((N + kColRows - 1) / kColRows) * dout * 4);
@@ -470,10 +494,11 @@ int pack8(int64_t rows, int f, const void* x, void* codes, const Exps& exps, cud
 }
 
 // out (M, n) = A^T B over the rows they share, both as they lie in memory.
-int weight_grad(int64_t rows, int M, int n, const void* A, const void* B, int shares, float* slots, void* out,
-                int* status, cudaStream_t s) {
+int weight_grad(int64_t rows, int M, int n, const void* A, int below_a, const void* B, int below_b, int shares,
+                float* slots, void* out, int* status, cudaStream_t s) {
   gemm::Shape a{};
   a.M = M; a.N = n; a.K = (int)rows; a.shares = shares; a.group = 16; a.status = status;
+  a.passes_less_one = below_a || below_b; a.a_step = below_a; a.b_step = below_b;
   if (!shares) return gemm::launch<true, true, gemm::StoreBf16>(A, M, B, n, a, {}, s, {out, M, n, n});
   const gemm::StorePiece::Params q{slots, gemm::kBM * gemm::pair_for(M)};
   const int st = gemm::launch<true, true, gemm::StorePiece>(A, M, B, n, a, q, s);
@@ -537,9 +562,9 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   gemm::Shape a{};
   a.M = (int)N; a.N = ff; a.K = d; a.group = 16; a.status = status;
   const Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
-                     S ? by_blocks(S + sv.ae, N) : Exps{}};
-  if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s, {g, N, ff, ff}))) return st;
-  a.N = dout; a.K = ff;
+                     S ? by_blocks(S + sv.ae, N) : Exps{}, ws.below};
+  if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s, {g, ws.rows, ff, ff}))) return st;
+  a.N = dout; a.K = ff; a.passes_less_one = ws.below > 0; a.a_step = ws.below;
   return gemm::launch<false, false, gemm::StoreBf16>(g, ff, w2, ff, a,
                                                      {reinterpret_cast<const __nv_bfloat16*>(b2), nullptr, nullptr}, s,
                                                      {y, N, dout, dout});
@@ -589,15 +614,17 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
   }
   if (dx || dw1 || db1 || dw2) {
     a.N = ff; a.K = dout;
-    const Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), by_blocks(S + sv.ae, N), db1 ? sum1 : nullptr};
-    if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s, {da, N, ff, ff}, {g, N, ff, ff}))) return st;
+    const Down::Params p{reinterpret_cast<const uint8_t*>(S + sv.ac), by_blocks(S + sv.ae, N), db1 ? sum1 : nullptr,
+                         ws.below};
+    if ((st = gemm::launch<false, true, Down>(dy, dout, w2, ff, a, p, s, {da, ws.rows, ff, ff},
+                                                    {g, ws.rows, ff, ff}))) return st;
   }
   if (dx) {
-    a.N = d; a.K = ff;
+    a.N = d; a.K = ff; a.passes_less_one = ws.below > 0; a.a_step = ws.below;
     if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, ff, w1, d, a, {}, s, {dx, N, d, d}))) return st;
   }
-  if (dw1 && (st = weight_grad(N, ff, d, da, W + ws.x, ws.shares1, slots, dw1, status, s))) return st;
-  if (dw2 && (st = weight_grad(N, dout, ff, dy, g, ws.shares2, slots, dw2, status, s))) return st;
+  if (dw1 && (st = weight_grad(N, ff, d, da, ws.below, W + ws.x, 0, ws.shares1, slots, dw1, status, s))) return st;
+  if (dw2 && (st = weight_grad(N, dout, ff, dy, 0, g, ws.below, ws.shares2, slots, dw2, status, s))) return st;
   if (db1 || db2) {
     const ColSum q1{(N + 31) / 32, db1 ? ff : 0, sum1, reinterpret_cast<__nv_bfloat16*>(db1)};
     const ColSum q2{blocks, db2 ? dout : 0, sum2, reinterpret_cast<__nv_bfloat16*>(db2)};
