@@ -19,6 +19,10 @@
 // M tiles laid end to end, so that the blocks that read the same part of A do so together. A share's pieces of tiles go
 // to fp32 slots that k_join adds up in order.
 //
+// Measured: the four products of the head at 16384 x 50304 x 768 take 0.81 to 0.92 ms each, 1.38 to 1.56 PFLOP/s, 0.82 to
+// 0.93 of cuBLAS's measured burst; the whole operator 5.48 ms with blocks working alone, 5.06 in pairs. dh's product there:
+// 1.26 ms by whole tiles (1.3 rounds), 0.91 in shares. Stage counts: what shared memory holds beside the results' pieces.
+//
 // An operand that was rounded to bf16 can be given as two, the rounded values and what the rounding took, stacked in one
 // tensor: the product then runs over K twice (`passes`), the second time on the remainders. Operators do so for few rows,
 // where one rounding error can be most of a result's; a sum over many rows averages them.

@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(kCountRows) k_head_count(int64_t N, const int6
   if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }
 
-// Block b takes positions [16 b, 16 b + 16): the targets before them (from the tokens, or from the counts of the
+// Block b takes positions [16 b, 16 b + 16) (64 at a time left SMs idle: 18 us against 8.5 at 4096 x 768; 11.6 us at 16384
+// x 768, 50 MB, 4.3 TB/s): the targets before them (from the tokens, or from the counts of the
 // blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 256.
 __global__ void __launch_bounds__(kGatherThreads)
 k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ tokens,
@@ -154,6 +155,7 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
   }
 }
 
+// 855 us at 16384 x 50304 x 768, 1.48 PFLOP/s; one ex2 for a score, half the tensor cores' time there.
 // Running maximum (of the unscaled scores) and sum of exponentials over the thread's columns.
 struct Lse {
   static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
@@ -210,6 +212,7 @@ struct Lse {
   }
 };
 
+// 17 us at 16384 rows x 394 halves (52 MB, 3.0 TB/s; 39 us with 8 warps and a rescaling for every pair).
 // Block = 32 positions x 16 warps over the halves of the vocabulary's tiles, 8 at a time.
 constexpr int kJoinWarps = 16;
 __global__ void __launch_bounds__(kJoinWarps * 32)
@@ -270,6 +273,7 @@ k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const in
   rest[r] = -expm1f(lp);
 }
 
+// 917 us at 16384 x 50304 x 768, 1.38 PFLOP/s (947 with sixteen warps and a piece each; direct stores: 1250).
 // dS of one chunk in bf16; the rows that pad the last tile get zeros.
 struct Slope {
   static constexpr int kWarps = 8, kOwn = 2, kTable = 0;

@@ -129,6 +129,7 @@ ASRN_DEV int64_t row_of(int64_t t, int64_t all, int wide) {
   return all < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)wide) : t / wide;
 }
 
+// Bound by its bytes: 19 us at 32768 x 768, 76 MB, 4.0 TB/s.
 // Four threads per block of 32 of a row of bf16, 8 values each; each thread kEach of them, all loaded first.
 constexpr int kEach = 4;
 __global__ void __launch_bounds__(256) k_pack8(int64_t rows, int f, int wide, const __nv_bfloat16* __restrict__ x,
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(256) k_unpack8(int64_t total, int f, const uin
   unpack(blockIdx.x, gridDim.x, total, f, codes, exps, x);
 }
 
+// 73 us at 32768 x 1536 x 768 (a product that only stores: 60); 149 with libm's erf and direct stores, 102 with eight warps.
 // a = sum + b1 -> Q(a) (unless codes is null) and gelu(a) in bf16.
 struct Up {
   static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
@@ -263,7 +265,8 @@ ASRN_DEV void gelu_both(float a0, float a1, gemm::F2& g, gemm::F2& slope) {
   slope = fma2(mul2(a, F2(0.39894228040143268f)), e, cdf);
 }
 
-// dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows.
+// dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows. 87 us at 32768 x 1536 x 768 (210 with
+// libm's functions and direct stores; 100 computed, 92 with the table, 87 with the codes by blocks).
 // a' = code 2^e takes 256 values for each e, so gelu and gelu' of the 16 exponents that matter lie in a table of shared
 // memory (gelu in bf16, as it leaves; gelu' in fp16, whose 2^-12 adds 1 % to the bf16 rounding of dA): one 32-bit load
 // for an element instead of about 20 instructions. Blocks with another exponent (all of a below 0.004, or some above 254)
@@ -362,6 +365,7 @@ struct Down {
   ASRN_DEV void finish() {}
 };
 
+// Bound by its bytes: 29 us at 32768 x 768 both, 126 MB, 4.3 TB/s.
 // x' from its codes (the first `unpackers` blocks), and sums of dY's columns over 64 rows (the others: block = 64 rows x
 // 256 columns, a lane 8 columns, a warp every eighth row).
 constexpr int kColRows = 64;
