@@ -321,6 +321,7 @@ struct Slope {
 int check_head(int64_t N, int64_t V, int32_t d) {
   if (N < 0 || V < 1 || d < 1) return ASRN_ERR_ARG;
   if (d % 8 || d > 16384 || V > (1 << 24) || N > (1 << 24)) return ASRN_ERR_UNSUPPORTED;
+  if (((N + 127) / 128) * ((V + 255) / 256) >= (1 << 30)) return ASRN_ERR_UNSUPPORTED;      // tiles are counted in 32 bits
   return ASRN_OK;
 }
 

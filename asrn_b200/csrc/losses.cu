@@ -5,8 +5,8 @@
 // Every sum is formed in a fixed order in fp64 (per thread, then by warp shuffles, then over the blocks' partials in
 // index order): the results do not depend on the blocks' timing. On the device: preference 512 pairs x 4096 19 us (54.5 MB),
 // policy 512 x 8192 26 us (88 MB, a third of the tokens counted): dependent rounds of loads, and about 100 instructions
-// for a counted token; small calls 5.5 to 8 us, half of what the host needs to issue them. Positions outside the mask are read but selected away,
-// never multiplied, so a NaN or infinity there reaches nothing.
+// for a counted token; small calls 5.5 to 8 us, half of what the host needs to issue them. Positions outside the mask are
+// read but selected away, never multiplied, so a NaN or infinity there reaches nothing.
 #include <algorithm>
 #include <initializer_list>
 #include <cooperative_groups.h>

@@ -552,7 +552,7 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   if (st) return st;
   if (N == 0) return ASRN_OK;
   if (!x || !w1 || !b1 || !w2 || !b2 || !y || (uintptr_t)x % 16 || (uintptr_t)w1 % 16 || (uintptr_t)w2 % 16 ||
-      (uintptr_t)y % 16)
+      (uintptr_t)y % 16 || (uintptr_t)b1 % 16 || (uintptr_t)b2 % 16)
     return ASRN_ERR_ARG;
   const Mlp8Saved sv = mlp8_saved(N, d, ff);
   const Mlp8Ws ws = mlp8_ws(N, d, ff, dout, false);

@@ -294,6 +294,7 @@ def pack8(x):
 
 def unpack8(p):
     """The bfloat16 tensor that pack8's result stands for."""
+    _need_cuda('unpack8', p.codes, p.exps)
     rows, f = p.codes.shape
     x = torch.empty(p.shape, dtype=torch.bfloat16, device=p.codes.device)
     _lib.check(_lib.lib().asrn_unpack8(rows, f, _p(p.codes), _p(p.exps), _p(x), _lib.stream_ptr(x.device)),
@@ -303,12 +304,12 @@ def unpack8(p):
 
 class _Mlp8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w1, b1, w2, b2):
+    def forward(ctx, x, w1, b1, w2, b2, grad):
         d, ff, dout = x.shape[-1], w1.shape[0], w2.shape[0]
         N, dev, lib = x.numel() // d, x.device, _lib.lib()
         xr, w1, b1, w2, b2 = _rows(x), _rows(w1), _rows(b1), _rows(w2), _rows(b2)
         y = xr.new_empty((*x.shape[:-1], dout))
-        keep = any(ctx.needs_input_grad)
+        keep = grad and any(ctx.needs_input_grad)
         nb_saved = _bytes('asrn_mlp8_saved_bytes', N, d, ff) if keep else 0
         nb = _bytes('asrn_mlp8_workspace_bytes', N, d, ff, dout, 0)
         saved = _scratch(nb_saved, dev) if keep else None
@@ -334,7 +335,7 @@ class _Mlp8(torch.autograd.Function):
         _lib.check(lib.asrn_mlp8_backward(N, d, ff, dout, dyr.data_ptr(), w1.data_ptr(), w2.data_ptr(),
                                           saved.data_ptr(), nb_saved, *[_p(t) for t in out], ws.data_ptr(), nb,
                                           _status_word(dev), _stream(dev)), 'asrn_mlp8_backward')
-        return tuple(out)
+        return (*out, None)
 
 
 def mlp8(x, w1, b1, w2, b2):
@@ -350,4 +351,4 @@ def mlp8(x, w1, b1, w2, b2):
     _need_cuda('mlp8', x, w1, b1, w2, b2)
     if s1[0] % 8 or s1[1] % 8 or s2[0] % 8 or not s1[0] * s1[1] * s2[0]:
         raise NotImplementedError(f'mlp8: the widths ({s1[1]}, {s1[0]}, {s2[0]}) have to be multiples of 8')
-    return _Mlp8.apply(*_bf16('mlp8', x, w1, b1, w2, b2))
+    return _Mlp8.apply(*_bf16('mlp8', x, w1, b1, w2, b2), torch.is_grad_enabled())

@@ -231,14 +231,14 @@ int asrn_scan_backward(int64_t rows, int64_t L, const float* a, const float* S, 
                        void* stream);
 
 /* ---- fine-tuning: log probabilities through the head, losses, MLP with 8-bit activations -----------------------------
- * No counterpart in the reference. Operands are bfloat16 unless said otherwise, rows contiguous, pointers to matrices
+ * No counterpart in the reference. Operands are bfloat16 unless said otherwise, rows contiguous, pointers to them
  * 16-byte aligned, widths multiples of 8 (else ASRN_ERR_UNSUPPORTED); `saved` and workspaces 256-byte aligned. status:
  * device int in which the tensor-core kernels' bounded waits record ASRN_ERR_TIMEOUT (may be NULL). All sums run in a
  * fixed order: results repeat bit for bit.
  *
  * asrn_head_forward: logp (N) float32 = log softmax(h W^T / tau)[token] for h (N, d), weight (V, d), tokens (N) int64.
  * A negative token leaves its position out: logp 0, no gradient, no work. A token >= V gives NaN. `saved` keeps what
- * the backward pass needs (asrn_head_saved_bytes). N, V <= 2^24.
+ * the backward pass needs (asrn_head_saved_bytes). N, V <= 2^24, N V < 2^45.
  * asrn_head_backward: from g (N) float32 = dL/dlogp, dh (N, d) and dw (V, d); either may be NULL. */
 size_t asrn_head_saved_bytes(int64_t N, int32_t d);
 size_t asrn_head_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t backward);

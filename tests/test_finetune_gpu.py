@@ -552,6 +552,13 @@ def test_mlp8_shapes_and_what_it_keeps(cuda):
     with torch.autocast('cuda', dtype=torch.bfloat16):
         assert torch.equal(asrn.mlp8(x.float(), w1.float(), b1.float(), w2.float(), b2.float()), y)
     w = w1.clone().requires_grad_()
+    torch.cuda.synchronize()
+    with torch.no_grad():                                # nothing is kept where no gradient is wanted
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        out = asrn.mlp8(x, w, b1, w2, b2)
+        peak = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(out, y) and peak <= y.nbytes + 2 * 96 * 128 * 2 + 2 * 512
     only, = torch.autograd.grad(asrn.mlp8(x, w, b1, w2, b2).sum(), w)
     full = run_mlp(x, w1, b1, w2, b2, torch.ones_like(y))
     assert torch.equal(only, full['dw1'])

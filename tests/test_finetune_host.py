@@ -37,6 +37,7 @@ def test_refusals(lib):
     assert head(N=-1) == ARG and head(V=0) == ARG and head(tau=0.0) == ARG and head(tau=float('nan')) == ARG
     assert head(h=None) == ARG and head(h=odd) == ARG and head(w=odd) == ARG
     assert head(d=12) == UNSUPPORTED and head(V=1 << 25) == UNSUPPORTED and head(N=1 << 25) == UNSUPPORTED
+    assert head(N=1 << 24, V=1 << 24) == UNSUPPORTED
     assert head(saved=None) == WORKSPACE and head(nb=16) == WORKSPACE and head(nw=16) == WORKSPACE
     assert head(saved=odd) == WORKSPACE and head(N=0) == 0
     back = lambda d=16, g=ok, tau=1.0, nb=1 << 40, nw=1 << 40: lib.asrn_head_backward(  # noqa: E731
@@ -52,10 +53,10 @@ def test_refusals(lib):
         B, L, ok, ok, ref, adv, 0, ok, lo, hi, kl, 0, ok, None, ok, ok, nw, None)
     assert pol(B=-1) == ARG and pol(lo=1.0) == ARG and pol(hi=-0.1) == ARG and pol(kl=0.1) == ARG and pol(kl=-1.0) == ARG
     assert pol(adv=None) == ARG and pol(nw=8) == WORKSPACE
-    mlp = lambda N=4, d=16, ff=32, do=16, x=ok, nw=1 << 40, sv=None, ns=0: lib.asrn_mlp8_forward(  # noqa: E731
-        N, d, ff, do, x, ok, ok, ok, ok, ok, sv, ns, ok, nw, None, None)
+    mlp = lambda N=4, d=16, ff=32, do=16, x=ok, nw=1 << 40, sv=None, ns=0, b=ok: lib.asrn_mlp8_forward(  # noqa: E731
+        N, d, ff, do, x, ok, b, ok, ok, ok, sv, ns, ok, nw, None, None)
     assert mlp(N=-1) == ARG and mlp(ff=0) == ARG and mlp(d=12) == UNSUPPORTED and mlp(do=4) == UNSUPPORTED
-    assert mlp(x=odd) == ARG and mlp(x=None) == ARG and mlp(nw=0) == WORKSPACE and mlp(sv=ok, ns=8) == WORKSPACE
+    assert mlp(b=odd) == ARG and mlp(x=odd) == ARG and mlp(x=None) == ARG and mlp(nw=0) == WORKSPACE and mlp(sv=ok, ns=8) == WORKSPACE
     assert mlp(N=0) == 0
     assert lib.asrn_mlp8_backward(4, 16, 32, 16, ok, ok, ok, None, 0, *[ok] * 6, 1 << 40, None, None) == WORKSPACE
     assert lib.asrn_mlp8_backward(4, 16, 32, 16, odd, ok, ok, ok, 1 << 40, *[ok] * 6, 1 << 40, None, None) == ARG
