@@ -634,17 +634,17 @@ int launch(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const
                             : launch_cg<1, AMn, BMn, Epi>(A, pitch_a, B, pitch_b, s, p, o, q, stream);
 }
 
-// Groups for a walk in shares: as many as the SMs hold and the work fills. shares_for: 0 (whole tiles)
-// unless shares keep at least 5 % more of the SMs busy (their pieces cost a write and a read in fp32).
+// Groups for a walk in shares: as many as the SMs hold and the work fills. shares_for: 0 (whole tiles) unless shares save 40
+// K blocks in a row, about 11 us: what the pieces and their joining cost on the device (6 to 8 us) and the host (3 us).
 inline int groups_for(int64_t M, int64_t N, int64_t K) {
   return shares_of(tiles_m(M, pair_for(M)), (K + kBK - 1) / kBK,
                    (int)std::max<int64_t>(1, sm_count() / pair_for(M) / tiles_n(N)));
 }
 inline int shares_for(int64_t M, int64_t N, int64_t K) {
   const int cg = pair_for(M);
-  const int64_t slots = sm_count() / cg, nt = tiles_n(N), tiles = tiles_m(M, cg) * nt, groups = groups_for(M, N, K);
-  const int64_t rounds = (tiles + slots - 1) / slots;
-  return groups * nt <= slots && groups * nt * rounds > 1.05 * tiles ? (int)groups : 0;
+  const int64_t slots = sm_count() / cg, nt = tiles_n(N), mt = tiles_m(M, cg), groups = groups_for(M, N, K);
+  const int64_t rounds = (mt * nt + slots - 1) / slots, kb = (K + kBK - 1) / kBK;
+  return groups * nt <= slots && rounds * kb - mt * kb / groups > 40 ? (int)groups : 0;
 }
 // The slots' sums to out (contiguous rows of N).
 inline int join(const Shape& s, const float* slots, void* out, const int* row_of, const int* pos, int64_t zero_n,
