@@ -24,7 +24,7 @@
 // 1.26 ms by whole tiles (1.3 rounds), 0.91 in shares. Stage counts: what shared memory holds beside the results' pieces.
 //
 // An operand that was rounded to bf16 can be given as two, the rounded values and what the rounding took, stacked in one
-// tensor: the product then runs over K twice (`passes`), the second time on the remainders. Operators do so for few rows,
+// tensor: the product then runs over K twice (`second_pass`), the second time on the remainders. Operators do so for few rows,
 // where one rounding error can be most of a result's; a sum over many rows averages them.
 //
 // Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, frees its TMEM and
@@ -62,7 +62,7 @@ struct Shape {
   int shares;              // groups of clusters that walk equal shares, or 0: whole tiles
   int group;               // whole tiles: M tiles walked before the next N tile
   int* status;
-  int passes_less_one;     // 1: K is walked again with the operands' outer coordinates moved by these
+  int second_pass;         // 1: K is walked again with the operands' outer coordinates moved by these
   int a_step, b_step;
 };
 
@@ -94,7 +94,7 @@ struct Walk {
   ASRN_DEV Walk(const Shape& s, int M, int K, int cg, int cluster, int clusters)
       : mt((M + kBM * cg - 1) / (kBM * cg)), nt((s.N + kBN - 1) / kBN), kblocks((K + kBK - 1) / kBK), group(s.group),
         at(cluster), step(clusters), share(-1), u(0), end(0) {
-    kblocks *= 1 + s.passes_less_one;
+    kblocks *= 1 + s.second_pass;
     if (s.shares) {
       share = cluster / nt;
       at = cluster % nt;
@@ -513,7 +513,7 @@ static __global__ void __launch_bounds__(256) k_join(const Shape s, const JoinAr
   let_next();
   const int M = cut(s.M, s.m_dev, s.m_off), K = cut(s.K, s.k_dev, s.k_off);
   const int mt = (M + a.tile_rows - 1) / a.tile_rows, nt = (s.N + kBN - 1) / kBN;
-  const int kblocks = (K + kBK - 1) / kBK * (1 + s.passes_less_one);
+  const int kblocks = (K + kBK - 1) / kBK * (1 + s.second_pass);
   const int per = a.tile_rows / 32, lane = threadIdx.x & 31;              // blocks of 32 rows of a tile
   const int64_t all = (int64_t)mt * kblocks;
   const int tile = blockIdx.x / per, m = tile / nt, n = tile % nt, part = blockIdx.x % per;
@@ -589,7 +589,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
               const typename Epi::Params& p, const Dest& o, const Dest& q, cudaStream_t stream) {
   CUtensorMap ma, mb, mo, mq;
   if (!bind_context()) return ASRN_ERR_CUDA;
-  const int again = s.passes_less_one;                     // the stacked operand is longer in its outer dimension
+  const int again = s.second_pass;                     // the stacked operand is longer in its outer dimension
   if (!operand_map(&ma, A, AMn, AMn ? s.M : s.M + again * s.a_step, AMn ? s.K + again * s.a_step : s.K, pitch_a, kBM) ||
       !operand_map(&mb, B, BMn, BMn ? s.N : s.N + again * s.b_step, BMn ? s.K + again * s.b_step : s.K, pitch_b, kBN / CG))
     return ASRN_ERR_CUDA;

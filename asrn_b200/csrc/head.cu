@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(kCountRows) k_head_count(int64_t N, const int6
 
 // Block b takes positions [16 b, 16 b + 16) (64 at a time left SMs idle: 18 us against 8.5 at 4096 x 768; 11.6 us at 16384
 // x 768, 50 MB, 4.3 TB/s): the targets before them (from the tokens, or from the counts of the
-// blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 256.
+// blocks of 1024), then its own, in order. The last block zeroes the rows up to the next multiple of 64: dW's sums run over
+// whole K blocks (what the rows after those hold reaches nothing that is kept).
 __global__ void __launch_bounds__(kGatherThreads)
 k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ tokens,
               const int* __restrict__ counts, int* count, int* __restrict__ tok, int* __restrict__ row,
@@ -149,13 +150,13 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
   if (i0 + kGatherRows >= N) {
     const int total = before + warps[0];
     if (tid == 0) *count = total;
-    const int64_t end = ((int64_t)total + 255) / 256 * 256;
+    const int64_t end = ((int64_t)total + 63) / 64 * 64;
     uint4* dst = reinterpret_cast<uint4*>(hc);
     for (int64_t c = (int64_t)total * nv + tid; c < end * nv; c += kGatherThreads) dst[c] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// 855 us at 16384 x 50304 x 768, 1.48 PFLOP/s; one ex2 for a score, half the tensor cores' time there.
+// 855 us at 16384 x 50304 x 768, 1.48 PFLOP/s; one ex2 for a score takes a third of the tensor cores' time there.
 // Running maximum (of the unscaled scores) and sum of exponentials over the thread's columns.
 struct Lse {
   static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
@@ -285,10 +286,11 @@ struct Slope {
   };
   const Params& p;
   int V, y, first;
+  bool on;
   float off, g, own;                       // lse, -dL/dlogp / tau, the target's dS
   ASRN_DEV Slope(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile&, int)
-      : p(pp), V(sh.N), y(-1), first(r & ~31), off(0.f), g(0.f), own(0.f) {
-    if (r < rows) {
+      : p(pp), V(sh.N), y(-1), first(r & ~31), on(r < rows), off(0.f), g(0.f), own(0.f) {
+    if (on) {
       y = p.tok[r];
       off = p.lse2[r];
       g = y < 0 ? NAN : -p.g[p.row[r]] * p.inv_tau;
@@ -308,6 +310,10 @@ struct Slope {
     if (j >= 0 && j < 32) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = i == j ? own : v[i];
+    }
+    if (!on) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
     }
     out.put(map_o, v, c, first);
     if (p.below) {
@@ -425,7 +431,7 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
     if (dh) {
       gemm::Shape a{};
       a.M = rows; a.N = d; a.K = (int)V; a.m_dev = count; a.m_off = (int)first; a.shares = ws.shares_h; a.status = status;
-      a.passes_less_one = ws.twice; a.a_step = rows;
+      a.second_pass = ws.twice; a.a_step = rows;
       const gemm::StorePiece::Params q{dh_slots, gemm::kBM * gemm::pair_for(rows)};
       if ((st = gemm::launch<false, true, gemm::StorePiece>(ds, ws.pitch, weight, d, a, q, s)) ||
           (st = gemm::join(a, dh_slots, dh, row, reinterpret_cast<const int*>(S + sv.pos), c ? 0 : N, s)))
@@ -434,7 +440,7 @@ int asrn_head_backward(int64_t N, int64_t V, int32_t d, const void* weight, cons
     if (dw) {
       gemm::Shape a{};
       a.M = (int)V; a.N = d; a.K = (int)left; a.k_dev = count; a.k_off = (int)first; a.shares = ws.shares_w; a.group = 16;
-      a.status = status; a.passes_less_one = ws.twice; a.a_step = rows;
+      a.status = status; a.second_pass = ws.twice; a.a_step = rows;
       if (ws.shares_w) {
         const gemm::StorePiece::Params q{dw_sum, gemm::kBM * gemm::pair_for(V)};
         if ((st = gemm::launch<true, true, gemm::StorePiece>(ds, ws.pitch, hc, d, a, q, s)) ||

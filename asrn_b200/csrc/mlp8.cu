@@ -502,7 +502,7 @@ int weight_grad(int64_t rows, int M, int n, const void* A, int below_a, const vo
                 float* slots, void* out, int* status, cudaStream_t s) {
   gemm::Shape a{};
   a.M = M; a.N = n; a.K = (int)rows; a.shares = shares; a.group = 16; a.status = status;
-  a.passes_less_one = below_a || below_b; a.a_step = below_a; a.b_step = below_b;
+  a.second_pass = below_a || below_b; a.a_step = below_a; a.b_step = below_b;
   if (!shares) return gemm::launch<true, true, gemm::StoreBf16>(A, M, B, n, a, {}, s, {out, M, n, n});
   const gemm::StorePiece::Params q{slots, gemm::kBM * gemm::pair_for(M)};
   const int st = gemm::launch<true, true, gemm::StorePiece>(A, M, B, n, a, q, s);
@@ -568,7 +568,7 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   const Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
                      S ? by_blocks(S + sv.ae, N) : Exps{}, ws.below};
   if ((st = gemm::launch<false, false, Up>(x, d, w1, d, a, p, s, {g, ws.rows, ff, ff}))) return st;
-  a.N = dout; a.K = ff; a.passes_less_one = ws.below > 0; a.a_step = ws.below;
+  a.N = dout; a.K = ff; a.second_pass = ws.below > 0; a.a_step = ws.below;
   return gemm::launch<false, false, gemm::StoreBf16>(g, ff, w2, ff, a,
                                                      {reinterpret_cast<const __nv_bfloat16*>(b2), nullptr, nullptr}, s,
                                                      {y, N, dout, dout});
@@ -624,7 +624,7 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
                                                     {g, ws.rows, ff, ff}))) return st;
   }
   if (dx) {
-    a.N = d; a.K = ff; a.passes_less_one = ws.below > 0; a.a_step = ws.below;
+    a.N = d; a.K = ff; a.second_pass = ws.below > 0; a.a_step = ws.below;
     if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, ff, w1, d, a, {}, s, {dx, N, d, d}))) return st;
   }
   if (dw1 && (st = weight_grad(N, ff, d, da, ws.below, W + ws.x, 0, ws.shares1, slots, dw1, status, s))) return st;
