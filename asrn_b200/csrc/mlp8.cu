@@ -562,7 +562,7 @@ int asrn_mlp8_forward(int64_t N, int32_t d, int32_t ff, int32_t dout, const void
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* S = reinterpret_cast<char*>(saved);
   __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(workspace) + ws.g);
-  if (S && (st = pack8(N, d, x, S + sv.xc, by_blocks(S + sv.xe, N), s))) return st;
+  if (S && (st = pack8(N, d, x, S + sv.xc, by_rows(S + sv.xe, d), s))) return st;
   gemm::Shape a{};
   a.M = (int)N; a.N = ff; a.K = d; a.group = 16; a.status = status;
   const Up::Params p{reinterpret_cast<const __nv_bfloat16*>(b1), S ? reinterpret_cast<uint8_t*>(S + sv.ac) : nullptr,
@@ -612,7 +612,7 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
     const unsigned summers = db2 ? (unsigned)(blocks * ((dout + 255) / 256)) : 0;
     k_prepare<<<unpackers + summers, 256, 0, s>>>(
         (int)unpackers, eighths, d, reinterpret_cast<const uint8_t*>(S + sv.xc),
-        by_blocks(S + sv.xe, N), reinterpret_cast<__nv_bfloat16*>(W + ws.x), N, dout,
+        by_rows(S + sv.xe, d), reinterpret_cast<__nv_bfloat16*>(W + ws.x), N, dout,
         reinterpret_cast<const __nv_bfloat16*>(dy), sum2);
     if ((st = launched())) return st;
   }
