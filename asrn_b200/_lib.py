@@ -173,6 +173,24 @@ def lib():
     return _lib
 
 
+_finetune = None
+
+
+def finetune():
+    """The PyTorch module of the fine-tuning operators, linked with the library (built with it; raises if missing)."""
+    global _finetune
+    if _finetune is None:
+        lib()
+        import torch  # noqa: F401  (its libraries first: the module is linked with them)
+        try:
+            from . import _finetune as module
+        except ImportError as e:
+            raise RuntimeError(f'asrn_b200._finetune cannot be loaded ({e}): build it with '
+                               '`python -m asrn_b200.build`') from e
+        _finetune = module
+    return _finetune
+
+
 def gemm_override():
     """'cuda_core' while the test hook asrn_test_force_cuda_core holds the bf16 work on the CUDA-core kernels, else
     None (the default: tensor cores)."""

@@ -1,4 +1,4 @@
-"""Build libasrn_b200.so in-tree from asrn_b200/csrc/*.cu for sm_100a (B200).
+"""Build libasrn_b200.so in-tree from asrn_b200/csrc/*.cu for sm_100a (B200), and _finetune.so, its PyTorch module.
 
     python -m asrn_b200.build            # incremental: recompiles sources newer than their object
     python -m asrn_b200.build --force
@@ -17,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, '_build')
 LIB = os.path.join(HERE, 'libasrn_b200.so')
+MODULE = os.path.join(HERE, '_finetune.so')
 ROOT = os.path.dirname(HERE)
 
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
@@ -64,7 +65,29 @@ def build(force=False, verbose=False, extra=()):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f'link failed: {" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
+    _build_module(force)
     return LIB
+
+
+def _build_module(force):
+    """_finetune.so from csrc/binding.cpp: linked with PyTorch's libraries and, through $ORIGIN, with LIB."""
+    src = os.path.join(SRC, 'binding.cpp')
+    newest = max(os.path.getmtime(src), _deps_mtime())
+    if not force and os.path.exists(MODULE) and os.path.getmtime(MODULE) >= newest:
+        return
+    import sysconfig
+    import torch
+    at = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    include = [os.path.join(at, 'include'), os.path.join(at, 'include', 'torch', 'csrc', 'api', 'include'),
+               os.path.join(cuda, 'include'), sysconfig.get_paths()['include']]
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-DTORCH_EXTENSION_NAME=_finetune',
+           '-I' + os.path.join(ROOT, 'include'), *[a for i in include for a in ('-isystem', i)], src, '-o', MODULE,
+           '-L' + HERE, '-lasrn_b200', '-L' + os.path.join(at, 'lib'), '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10',
+           '-lc10_cuda', '-L' + os.path.join(cuda, 'lib64'), '-lcudart', '-Wl,-rpath,$ORIGIN']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f'g++ failed: {" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
 
 
 if __name__ == '__main__':

@@ -674,3 +674,27 @@ def test_refusals(cuda):
         ft.pack8(rand((2, 12), 130))
     with pytest.raises(TypeError):
         ft.pack8(h.float())
+
+
+@pytest.mark.parametrize('mode', [torch.no_grad, torch.inference_mode])
+def test_forward_without_gradients_is_the_same(cuda, mode):
+    import asrn_b200 as asrn
+    g = torch.Generator(cuda).manual_seed(3)
+    rand = lambda *s: torch.randn(*s, device=cuda, generator=g).bfloat16()  # noqa: E731
+    h, w, y = rand(33, 64), rand(97, 64).requires_grad_(), torch.arange(33, device=cuda)
+    u, b, v = rand(48, 64), rand(48), rand(64, 48)
+    lp, out = asrn.head_logprobs(h, w, y), asrn.mlp8(h, u.requires_grad_(), b, v, h[0])
+    with mode():
+        lp2, out2 = asrn.head_logprobs(h, w, y), asrn.mlp8(h, u, b, v, h[0])
+    assert not lp2.requires_grad and not out2.requires_grad and lp.requires_grad and out.requires_grad
+    assert torch.equal(lp, lp2) and torch.equal(out, out2)
+
+
+def test_a_weight_changed_in_place_is_noticed(cuda):
+    import asrn_b200 as asrn
+    w = torch.ones(8, 8, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    lp = asrn.head_logprobs(w[:3].detach(), w, torch.zeros(3, dtype=torch.int64, device=cuda))
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match='modified'):
+        lp.sum().backward()

@@ -78,3 +78,24 @@ def test_no_cpu_path():
     m = asrn.create_model(V=32, d=16, n_capas=2, checkpoint='8bits')
     assert all(b.activaciones_8bits for b in m.bloques)
     assert not any(b.activaciones_8bits for b in asrn.create_model(V=32, d=16, n_capas=2, checkpoint=True).bloques)
+
+
+def test_errors_are_the_packages_own():
+    import asrn_b200 as asrn
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    z, i = torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int64)
+    for error, call in [
+            (ValueError, lambda: asrn.head_logprobs(b(3, 8), b(5, 16), i)),
+            (TypeError, lambda: asrn.head_logprobs(b(3, 8), b(5, 8), i.int())),
+            (ValueError, lambda: asrn.head_logprobs(b(3, 8), b(5, 8), i, temperatura=0.0)),
+            (ValueError, lambda: asrn.head_logprobs(b(3, 8), b(5, 8), i, temperatura=float('nan'))),
+            (ValueError, lambda: asrn.preference_loss(z, z, z.bool(), kind='hinge')),
+            (ValueError, lambda: asrn.preference_loss(z, z, z.bool(), beta=0.0)),
+            (ValueError, lambda: asrn.preference_loss(z, z[:, :2], z.bool())),
+            (ValueError, lambda: asrn.policy_loss(z[0], z[0], z[0, :2], z[0].bool())),
+            (ValueError, lambda: asrn.policy_loss(z[0], z[0], z[0], z[0].bool(), kl=0.1)),
+            (ValueError, lambda: asrn.policy_loss(z[0], z[0], z[0], z[0].bool(), clip=(1.0, 0.2))),
+            (ValueError, lambda: asrn.mlp8(b(3, 8), b(8, 16), b(8), b(8, 8), b(8))),
+            (TypeError, lambda: asrn.finetune.pack8(torch.zeros(3, 8)))]:
+        with pytest.raises(error):
+            call()
