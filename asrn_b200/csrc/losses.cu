@@ -536,9 +536,9 @@ int64_t loss_chunks(int64_t L) { return (L + kLossChunk - 1) / kLossChunk; }
 
 // Tokens up to which one cooperative launch does it all, and above which two overlapping launches do. The second launch
 // costs the host about 2.5 us; the cooperative one costs the GPU about 4: it starts on an idle GPU, holds fewer blocks, and
-// waits at its barrier. Us a call, two launches / one: preference 20.9 / 18.3 at 2^16 and at 2^21 tokens, 22.7 / 26.5 at
-// 512 pairs x 4096 (27.5 / 24.6 at 1024 x 2048); policy 19.5 / 17.3 at 2^16, 19.5 / 18.4 at 2^20, 20.5 / 22.6 at 2^21.
-constexpr int64_t kPrefTogether = 1 << 21, kPolicyTogether = 1 << 20;
+// waits at its barrier. Us a call, two launches / one: preference 16.1 / 13.3 at 2^18 tokens, 16.4 / 14.4 at 512 x 2048, 16.4 /
+// 16.4 at 2^21, 22.5 / 25.7 at 2^22; policy 11.0 / 10.3 at 2^18, 12.3 / 13.5 at 2^19, 14.4 / 18.4 at 2^20.
+constexpr int64_t kPrefTogether = 1 << 21, kPolicyTogether = 1 << 18;
 
 int loss_grid(int64_t items, int per_sm) {
   static int sms = 0;
@@ -585,8 +585,11 @@ Split split_rows(int64_t rows, int64_t L) {
   return Split{rows * parts, parts, (chunks + parts - 1) / parts * kLossChunk};
 }
 
-// One block by itself: no workspace to allocate, 15.8 us a call against 17.7 for the cooperative launch.
-bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L <= 16384; }
+// Tokens up to which one block does it by itself, without a workspace. Us a call, one block / the cooperative launch:
+// preference 11.9 / 13.3 at 2^14 tokens, 15.0 / 13.7 at 2^15; policy, with more to compute for a token, 8.8 / 10.2 at 2^12,
+// 12.1 / 10.2 at 2^13.
+constexpr int64_t kPrefSmall = 1 << 14, kPolicySmall = 1 << 12;
+bool small_loss(int64_t rows, int64_t L, int64_t most) { return rows <= kSmallRows && rows * L <= most; }
 
 }  // namespace
 }  // namespace asrn
@@ -594,7 +597,7 @@ bool small_loss(int64_t rows, int64_t L) { return rows <= kSmallRows && rows * L
 extern "C" {
 
 size_t asrn_preference_workspace_bytes(int64_t P, int64_t L) {
-  if (P < 0 || L < 0 || asrn::small_loss(2 * P, L)) return 0;
+  if (P < 0 || L < 0 || asrn::small_loss(2 * P, L, asrn::kPrefSmall)) return 0;
   return asrn::align_up((size_t)asrn::split_rows(2 * P, L).items * sizeof(asrn::RowSum) + 1);
 }
 
@@ -609,7 +612,7 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
   const PrefArgs a{P, L, logp, ref_logp, mask, kind, beta, smoothing, loss, grad, rewards};
   if (P * L > 0 && (!logp || !ref_logp || !mask)) return ASRN_ERR_ARG;
   if (P > 0 && !rewards) return ASRN_ERR_ARG;
-  if (small_loss(2 * P, L)) {
+  if (small_loss(2 * P, L, kPrefSmall)) {
     k_pref_small<<<1, 1024, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
   }
@@ -630,7 +633,7 @@ int asrn_preference_loss(int64_t P, int64_t L, const float* logp, const float* r
 }
 
 size_t asrn_policy_workspace_bytes(int64_t B, int64_t L) {
-  if (B < 0 || L < 0 || asrn::small_loss(B, L)) return 0;
+  if (B < 0 || L < 0 || asrn::small_loss(B, L, asrn::kPolicySmall)) return 0;
   return 256 + asrn::align_up(asrn::kLossGrid * sizeof(asrn::BlockSum)) +
          asrn::align_up((size_t)asrn::split_rows(B, L).items * sizeof(int) + 1);
 }
@@ -649,7 +652,7 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   const PolicyArgs a{B, L, logp, old_logp, ref_logp, advantages, mask, adv_per_token != 0, per_sequence != 0,
                      rounded(log1p(-clip_low), true), rounded(log1p(clip_high), false), (float)(1. - clip_low), (float)(1. + clip_high), (float)kl,
                      loss, grad, stats};
-  if (small_loss(B, L)) {
+  if (small_loss(B, L, kPolicySmall)) {
     if (ref_logp) k_policy_small<true><<<1, 1024, 0, s>>>(a);
     else k_policy_small<false><<<1, 1024, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
