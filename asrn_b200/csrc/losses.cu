@@ -645,9 +645,8 @@ int asrn_policy_loss(int64_t B, int64_t L, const float* logp, const float* old_l
   using namespace asrn;
   if (B < 0 || L < 0 || !(clip_low >= 0. && clip_low < 1.) || !(clip_high >= 0.) || !(kl >= 0.) || !loss || !stats)
     return ASRN_ERR_ARG;
-  if (kl > 0. && !ref_logp) return ASRN_ERR_ARG;
   if (B > ((int64_t)1 << 30) || L > ((int64_t)1 << 30)) return ASRN_ERR_UNSUPPORTED;
-  if (B * L > 0 && (!logp || !old_logp || !advantages || !mask)) return ASRN_ERR_ARG;
+  if (B * L > 0 && (!logp || !old_logp || !advantages || !mask || (kl > 0. && !ref_logp))) return ASRN_ERR_ARG;
   if (L == 0) B = 0;                     // sequences without positions: nothing to count, read or write but the results
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const PolicyArgs a{B, L, logp, old_logp, ref_logp, advantages, mask, adv_per_token != 0, per_sequence != 0,

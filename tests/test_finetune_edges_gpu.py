@@ -22,3 +22,11 @@ def test_losses_of_many_sequences_without_positions(cuda, rows):
     e = torch.zeros(2, rows, 0, device='cuda')
     r = asrn.preference_loss(e, e, e.bool())
     assert float(r.loss) == 0 and r.grad.shape == e.shape and (r.chosen == 0).all() and (r.rejected == 0).all()
+
+
+def test_policy_without_sequences_and_with_a_reference(cuda):
+    """An empty batch has no log probabilities of the reference model in memory either: not an error."""
+    import asrn_b200 as asrn
+    e = torch.zeros(0, 5, device='cuda')
+    r = asrn.policy_loss(e, e, e[:, 0], e.bool(), ref_logp=e, kl=0.1)
+    assert float(r.loss) == 0 and float(r.kl) == 0 and r.grad.shape == (0, 5)
