@@ -27,8 +27,8 @@
 // tensor: the product then runs over K twice (`second_pass`), the second time on the remainders. Operators do so for few rows,
 // where one rounding error can be most of a result's; a sum over many rows averages them.
 //
-// Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, frees its TMEM and
-// ends.
+// Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, waits (bounded, too)
+// for the copies and the multiplications that it has under way, frees its TMEM and ends.
 #pragma once
 #include <algorithm>
 #include <atomic>
@@ -353,6 +353,11 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           }
         }
       }
+      // No block may end with copies under way into its shared memory. The first block's barriers count the pair's; the other
+      // one waits for it at the end.
+      if (rank == 0)
+        for (int i = max(0, it - kS); i < it; ++i)
+          if (!mbar_wait_limit(full + i % kS, (i / kS) & 1, nullptr, kWaitLimitNs)) break;
     }
   } else if (wid == 1) {
     if (lane == 0 && rank == 0) {                       // MMA issuer, for both blocks of a pair
@@ -377,6 +382,8 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         }
         commit<CG>(tfull + b);
       }
+      // Nor with multiplications under way: the last of these barriers follows all of them.
+      if (jt > 0) mbar_wait_limit(tfull + ((jt - 1) & 1), ((jt - 1) >> 1) & 1, nullptr, kWaitLimitNs);
     }
   } else {                                              // epilogue
     constexpr int kCols = kBN * 4 / Epi::kWarps, kOwn = Epi::kOwn;
