@@ -6,13 +6,12 @@
 // Errors are raised as the Python package raises them: ValueError, TypeError, NotImplementedError, and RuntimeError for
 // tensors that are not on a GPU and for CUDA errors.
 #include <ATen/autocast_mode.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
-#include <array>
-#include <mutex>
+#include <cstring>
 #include <sstream>
 
 #include "asrn_b200.h"
@@ -79,30 +78,46 @@ Tensor mask_of(const char* what, const Tensor& m, at::IntArrayRef sizes) {
   return m.contiguous();
 }
 
-// The devices' status words of the kernels' bounded waits (none while a graph that would own it is captured).
-// Never freed: at the program's end CUDA may be gone before this module.
-auto& words = *new std::array<Tensor, 64>;
-std::mutex words_lock;
+// The devices' status words of the kernels' bounded waits, in page-locked host memory that the devices write: a call sees
+// what an earlier one recorded without waiting for the GPU. Never freed: at the program's end CUDA may be gone before this
+// module. (Allocated in the relaxed capture mode: that is no part of a graph that may be under capture.)
+constexpr int kDevices = 64;
 
-int* status_word(c10::Device dev) {
-  std::lock_guard<std::mutex> hold(words_lock);
-  Tensor& w = words.at(dev.index());
-  if (!w.defined()) {
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
-    w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(dev));
-  }
-  return w.data_ptr<int>();
+volatile int* words() {
+  static int* const at = [] {
+    void* p = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    C10_CUDA_CHECK(e);
+    memset(p, 0, kDevices * sizeof(int));
+    return static_cast<int*>(p);
+  }();
+  return at;
+}
+
+// The device's word for the call `what`, which is refused while the word holds an error.
+int* status_word(const char* what, c10::Device dev) {
+  TORCH_CHECK(dev.index() < kDevices, "asrn_b200.", what, ": device index ", (int)dev.index());
+  volatile int* w = words() + dev.index();
+  const int v = *w;
+  TORCH_CHECK(v == ASRN_OK, "asrn_b200.", what, ": a bounded wait of an earlier call on ", dev, " gave up (",
+              asrn_status_string(v), "): results since then are void. asrn_b200.finetune.status(reset=True) allows new calls");
+  return const_cast<int*>(w);
+}
+
+int64_t status_address(int64_t device) {
+  if (device < 0 || device >= kDevices) throw py::value_error(text("status: device index ", device));
+  return (int64_t)(words() + device);
 }
 
 int64_t status(int64_t device, bool reset) {
-  Tensor w;
-  {
-    std::lock_guard<std::mutex> hold(words_lock);
-    w = words.at(device);
-  }
-  if (!w.defined()) return 0;
-  const int64_t v = w.item<int>();
-  if (reset) w.zero_();
+  volatile int* w = reinterpret_cast<volatile int*>(status_address(device));
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  C10_CUDA_CHECK(cudaDeviceSynchronize());
+  const int64_t v = *w;
+  if (reset) *w = ASRN_OK;
   return v;
 }
 
@@ -133,7 +148,7 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
     Tensor saved = scratch(nb_saved, dev);
     const Tensor ws = scratch(nb, dev);
     check(asrn_head_forward(N, V, d, hr.data_ptr(), w.data_ptr(), tok.data_ptr<int64_t>(), (float)tau, out.data_ptr<float>(),
-                            saved.data_ptr(), nb_saved, ws.data_ptr(), nb, status_word(dev), stream_of(dev)),
+                            saved.data_ptr(), nb_saved, ws.data_ptr(), nb, status_word("head_logprobs", dev), stream_of(dev)),
           "asrn_head_forward");
     ctx->save_for_backward({w, saved});
     ctx->saved_data["sizes"] = h.sizes().vec();
@@ -155,7 +170,8 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
     const Tensor ws = scratch(nb, dev);
     check(asrn_head_backward(N, V, d, w.data_ptr(), saved.data_ptr(), saved.numel(), (float)ctx->saved_data["tau"].toDouble(),
                              g.data_ptr<float>(), dh.defined() ? dh.data_ptr() : nullptr,
-                             dw.defined() ? dw.data_ptr() : nullptr, ws.data_ptr(), nb, status_word(dev), stream_of(dev)),
+                             dw.defined() ? dw.data_ptr() : nullptr, ws.data_ptr(), nb, status_word("head_logprobs", dev),
+                             stream_of(dev)),
           "asrn_head_backward");
     return {dh, dw, Tensor(), Tensor()};
   }
@@ -272,8 +288,8 @@ struct Mlp8 : torch::autograd::Function<Mlp8> {
     Tensor saved = keep ? scratch(nb_saved, dev) : Tensor();
     const Tensor ws = scratch(nb, dev);
     check(asrn_mlp8_forward(N, d, ff, dout, xr.data_ptr(), u1.data_ptr(), c1.data_ptr(), u2.data_ptr(), c2.data_ptr(),
-                            y.data_ptr(), keep ? saved.data_ptr() : nullptr, nb_saved, ws.data_ptr(), nb, status_word(dev),
-                            stream_of(dev)),
+                            y.data_ptr(), keep ? saved.data_ptr() : nullptr, nb_saved, ws.data_ptr(), nb,
+                            status_word("mlp8", dev), stream_of(dev)),
           "asrn_mlp8_forward");
     if (keep) {
       ctx->save_for_backward({u1, u2, saved});
@@ -300,7 +316,8 @@ struct Mlp8 : torch::autograd::Function<Mlp8> {
     const size_t nb = asrn_mlp8_workspace_bytes(N, d, ff, dout, 1);
     const Tensor ws = scratch(nb, dev);
     check(asrn_mlp8_backward(N, d, ff, dout, dy.data_ptr(), w1.data_ptr(), w2.data_ptr(), saved.data_ptr(), saved.numel(),
-                             at[0], at[1], at[2], at[3], at[4], ws.data_ptr(), nb, status_word(dev), stream_of(dev)),
+                             at[0], at[1], at[2], at[3], at[4], ws.data_ptr(), nb, status_word("mlp8", dev),
+                             stream_of(dev)),
           "asrn_mlp8_backward");
     return out;
   }
@@ -332,4 +349,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack8", torch::wrap_pybind_function(&unpack8));
   m.def("mlp8", torch::wrap_pybind_function(&mlp8));
   m.def("status", torch::wrap_pybind_function(&status));
+  m.def("status_address", torch::wrap_pybind_function(&status_address));
 }

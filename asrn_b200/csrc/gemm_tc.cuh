@@ -27,8 +27,8 @@
 // tensor: the product then runs over K twice (`second_pass`), the second time on the remainders. Operators do so for few rows,
 // where one rounding error can be most of a result's; a sum over many rows averages them.
 //
-// Every wait is bounded (umma::mbar_wait); after a timeout the kernel records it in the status word, waits (bounded, too)
-// for the copies and the multiplications that it has under way, frees its TMEM and ends.
+// Every wait is bounded; after a timeout the kernel records it in the status word, waits (bounded, too) for the copies and
+// the multiplications that it has under way, frees its TMEM and ends. What the word holds from earlier calls stops no later one.
 #pragma once
 #include <algorithm>
 #include <atomic>
@@ -143,6 +143,17 @@ ASRN_DEV uint32_t peer_u32(const void* p, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(umma::smem_u32(p)), "r"(rank));
   return r;
+}
+
+// umma::mbar_wait, but for the status word, which is only written: each role of a block ends with the first of its waits
+// that runs out, so a block ends after a few limits whatever the word held before. It may lie in the host's memory.
+ASRN_DEV bool wait(uint64_t* bar, uint32_t parity, int* status) {
+  if (umma::mbar_wait_limit(bar, parity, nullptr, umma::kWaitLimitNs)) return true;
+  if (status) {
+    *reinterpret_cast<volatile int*>(status) = ASRN_ERR_TIMEOUT;
+    __threadfence_system();
+  }
+  return false;
 }
 
 template <int CG> ASRN_DEV void load_box(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -334,7 +345,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           const int again = kt >= kblocks, kb = kt - again * kblocks;
           const int a_at = again * s.a_step, b_at = again * s.b_step;
           const int st = it % kS;
-          if (it >= kS && !(ok = mbar_wait(empty + st, ((it / kS) - 1) & 1, s.status))) break;
+          if (it >= kS && !(ok = wait(empty + st, ((it / kS) - 1) & 1, s.status))) break;
           if (rank == 0) mbar_expect_tx(full + st, (uint32_t)(CG * stage_bytes<CG>()));
           const uint32_t bar = CG == 1 ? smem_u32(full + st) : peer_u32(full + st, 0);
           if (AMn) {
@@ -366,11 +377,11 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       bool ok = true;
       for (; ok && walk.next(u); ++jt) {
         const int b = jt & 1;
-        if (jt >= 2 && !(ok = mbar_wait(tempty + b, ((jt >> 1) - 1) & 1, s.status))) break;
+        if (jt >= 2 && !(ok = wait(tempty + b, ((jt >> 1) - 1) & 1, s.status))) break;
         tc_fence_after();
         for (int kb = u.k0; kb < u.k1; ++kb, ++it) {
           const int st = it % kS;
-          if (!(ok = mbar_wait(full + st, (it / kS) & 1, s.status))) break;
+          if (!(ok = wait(full + st, (it / kS) & 1, s.status))) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(sA + st * kBytesA), b0 = smem_u32(sB + st * kStageB);
 #pragma unroll
@@ -393,7 +404,7 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     int jt = 0;
     for (; walk.next(u); ++jt) {
       const int b = jt & 1;
-      if (!mbar_wait(tfull + b, (jt >> 1) & 1, s.status)) break;
+      if (!wait(tfull + b, (jt >> 1) & 1, s.status)) break;
       tc_fence_after();
       const int c0 = u.n * kBN + part * kCols;
       Epi e(p, (u.m * CG + (int)rank) * kBM + q4 * 32 + lane, M, s, u, part);

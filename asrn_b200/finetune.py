@@ -24,9 +24,12 @@ from . import _lib
 
 
 def status(device=None, reset=False):
-    """0, or the first error these kernels recorded on the device (ASRN_ERR_TIMEOUT: a bounded wait gave up and that
-    call's results are void). Synchronises."""
+    """0, or the error that these kernels recorded on the device (ASRN_ERR_TIMEOUT: a bounded wait gave up, and the
+    results since then are void). Synchronises. While an error stands head_logprobs, mlp8 and their backward passes raise
+    RuntimeError as soon as the host sees it; reset=True clears it and allows new calls."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
+    if dev.type != 'cuda':
+        raise ValueError(f'status: {dev} is not a CUDA device')
     index = torch.cuda.current_device() if dev.index is None else dev.index
     return _lib.finetune().status(index, reset)
 

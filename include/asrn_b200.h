@@ -233,8 +233,9 @@ int asrn_scan_backward(int64_t rows, int64_t L, const float* a, const float* S, 
 /* ---- fine-tuning: log probabilities through the head, losses, MLP with 8-bit activations -----------------------------
  * No counterpart in the reference. Operands are bfloat16 unless said otherwise, rows contiguous, pointers to them
  * 16-byte aligned, widths multiples of 8 (else ASRN_ERR_UNSUPPORTED); `saved` and workspaces 256-byte aligned. status:
- * device int in which the tensor-core kernels' bounded waits record ASRN_ERR_TIMEOUT (may be NULL). All sums run in a
- * fixed order: results repeat bit for bit.
+ * int that the device can write (device memory, or the host's page-locked) in which the tensor-core kernels' bounded waits
+ * record ASRN_ERR_TIMEOUT: what that call left is void. It is never read: what it holds stops no later call (may be NULL).
+ * All sums run in a fixed order: results repeat bit for bit.
  *
  * asrn_head_forward: logp (N) float32 = log softmax(h W^T / tau)[token] for h (N, d), weight (V, d), tokens (N) int64.
  * A negative token leaves its position out: logp 0, no gradient, no work. A token >= V gives NaN. `saved` keeps what

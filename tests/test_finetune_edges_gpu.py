@@ -1,7 +1,11 @@
 """The fine-tuning operators (asrn_b200.finetune) at their edges: sizes, values and calls that the tests by operator
 (test_finetune_gpu.py, whose references and bounds these use) do not reach."""
+import ctypes
+
 import pytest
 import torch
+
+from test_finetune_gpu import rand
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +34,58 @@ def test_policy_without_sequences_and_with_a_reference(cuda):
     e = torch.zeros(0, 5, device='cuda')
     r = asrn.policy_loss(e, e, e[:, 0], e.bool(), ref_logp=e, kl=0.1)
     assert float(r.loss) == 0 and float(r.kl) == 0 and r.grad.shape == (0, 5)
+
+
+# ---- bounded waits ------------------------------------------------------------------------------------------------------
+
+TIMEOUT = 5
+
+
+def test_a_recorded_timeout_is_raised_until_it_is_cleared(cuda):
+    """The word is written here as a kernel whose wait gives up writes it: no call goes on as if nothing had happened,
+    forward or backward, and all do once it is cleared."""
+    import asrn_b200 as asrn
+    from asrn_b200 import _lib
+    from asrn_b200 import finetune as ft
+    h, w, y = rand((40, 64), 300), rand((99, 64), 301, 0.1).requires_grad_(), torch.arange(40, device='cuda')
+    u, b, v, c = rand((48, 64), 302, 0.1), rand((48,), 303), rand((64, 48), 304), rand((64,), 305)
+    calls = [lambda: asrn.head_logprobs(h, w, y), lambda: asrn.mlp8(w, u, b, v, c)]
+    outs = [f() for f in calls]
+    want = [torch.autograd.grad(o.float().sum(), w, retain_graph=True)[0] for o in outs]
+    assert ft.status() == 0
+    word = ctypes.c_int.from_address(_lib.finetune().status_address(0))
+    word.value = TIMEOUT
+    try:
+        for f in calls + [lambda o=o: torch.autograd.grad(o.float().sum(), w, retain_graph=True) for o in outs]:
+            with pytest.raises(RuntimeError, match='bounded wait'):
+                f()
+        assert ft.status() == TIMEOUT and ft.status() == TIMEOUT
+        assert ft.status(reset=True) == TIMEOUT and ft.status() == 0
+    finally:
+        word.value = 0
+    assert all(torch.equal(f(), o) for f, o in zip(calls, outs))
+    assert all(torch.equal(torch.autograd.grad(o.float().sum(), w)[0], a) for o, a in zip(outs, want))
+    with pytest.raises(ValueError):
+        ft.status('cpu')
+
+
+def test_an_earlier_calls_timeout_stops_no_later_call(cuda):
+    """The C entries with a status word that already holds a timeout: the products wait for their operands all the same."""
+    from asrn_b200 import _lib
+    L, P, s = _lib.lib(), _lib.ptr, _lib.stream_ptr(cuda)
+    N, V, d, ff = 600, 5003, 256, 512
+    h, w = rand((N, d), 310), rand((V, d), 311, 0.1)
+    y = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(312)).cuda()
+    u, b, v, c = rand((ff, d), 313, 0.1), rand((ff,), 314), rand((d, ff), 315, 0.1), rand((d,), 316)
+    buf = lambda n: torch.empty(n, dtype=torch.uint8, device='cuda')  # noqa: E731
+    nb = [L.asrn_head_saved_bytes(N, d), L.asrn_head_workspace_bytes(N, V, d, 0), L.asrn_mlp8_workspace_bytes(N, d, ff, d, 0)]
+    mem = [buf(n) for n in nb]
+    out = []
+    for before in (0, TIMEOUT):
+        word = torch.full((1,), before, dtype=torch.int32, device='cuda')
+        lp, z = torch.full((N,), 7.0, device='cuda'), torch.full((N, d), 7.0, dtype=torch.bfloat16, device='cuda')
+        assert L.asrn_head_forward(N, V, d, P(h), P(w), P(y), 1.0, P(lp), P(mem[0]), nb[0], P(mem[1]), nb[1], P(word), s) == 0
+        assert L.asrn_mlp8_forward(N, d, ff, d, P(h), P(u), P(b), P(v), P(c), P(z), None, 0, P(mem[2]), nb[2], P(word), s) == 0
+        assert int(word) == before
+        out.append((lp, z))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
