@@ -155,7 +155,7 @@ class ModeloASRN(nn.Module):
     def logprobs(self, x, objetivos=None, temperatura=1.0):
         """log softmax(logits / temperatura) of the tokens objetivos (B, L) at the positions of x (B, L), float32: by
         default each position's next token (0 at the last one). A negative target leaves its position out: 0 and no
-        gradient. Under bf16 autocast the (B, L, V) logits are never in memory and positions left out cost nothing
+        gradient; one outside the vocabulary gives NaN. Under bf16 autocast the (B, L, V) logits are never in memory and positions left out cost nothing
         (head_logprobs); the fp32 model takes them from its logits."""
         if objetivos is None:
             objetivos = F.pad(x[:, 1:], (0, 1), value=-1)
@@ -166,7 +166,9 @@ class ModeloASRN(nn.Module):
                 torch.get_autocast_dtype('cuda') == torch.bfloat16:
             return head_logprobs(h, self.head.weight, objetivos, temperatura)
         lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
-        lp = lp.gather(-1, objetivos.clamp(min=0).unsqueeze(-1)).squeeze(-1)
+        V = lp.shape[-1]                                 # an index outside would stop the GPU's context
+        lp = lp.gather(-1, objetivos.clamp(0, V - 1).unsqueeze(-1)).squeeze(-1)
+        lp = lp * torch.where(objetivos < V, 1.0, math.nan)
         return torch.where(objetivos >= 0, lp, torch.zeros_like(lp))
 
     def estado(self, x):

@@ -1,0 +1,27 @@
+"""The fine-tuning operators at the model's edges, as far as they need no GPU."""
+import pytest
+import torch
+
+
+def model(V=11, d=16):
+    """A model whose state is given: what the fp32 log probabilities make of it."""
+    import asrn_b200 as asrn
+    m = asrn.create_model(V=V, d=d, n_capas=2, semilla=0)
+    h = torch.randn(2, 5, d, generator=torch.Generator().manual_seed(1)).requires_grad_()
+    m.estado = lambda x: h
+    return m, h, torch.zeros(2, 5, dtype=torch.int64)
+
+
+def test_fp32_logprobs_of_a_token_outside_the_vocabulary():
+    """NaN, with a NaN gradient, as in bf16: torch's gather would fail on the host and stop the context on a GPU."""
+    m, h, x = model()
+    y = torch.tensor([[3, 10, 11, -1, 0], [1 << 40, -100, 2, 5, 9]])
+    lp = m.logprobs(x, y)
+    assert lp.isnan().tolist() == [[False, False, True, False, False], [True, False, False, False, False]]
+    assert (lp[y < 0] == 0).all()
+    want = torch.log_softmax(m.head(h), -1)
+    for at in ((0, 0), (0, 1), (1, 4)):
+        assert lp[at] == want[at][y[at]]
+    lp.sum().backward()
+    assert h.grad.isnan().any(-1).tolist() == lp.isnan().tolist()
+    assert (h.grad[0, 3] == 0).all()
