@@ -161,6 +161,8 @@ class ModeloASRN(nn.Module):
             objetivos = F.pad(x[:, 1:], (0, 1), value=-1)
         if objetivos.shape != x.shape:
             raise ValueError(f'objetivos must be (B, L) = {tuple(x.shape)}; got {tuple(objetivos.shape)}')
+        if not 0 < temperatura <= 1e30:
+            raise ValueError('logprobs: temperatura has to be positive')
         h = self.estado(x)
         if h.is_cuda and torch.is_autocast_enabled('cuda') and h.shape[-1] % 8 == 0 and \
                 torch.get_autocast_dtype('cuda') == torch.bfloat16:

@@ -25,3 +25,11 @@ def test_fp32_logprobs_of_a_token_outside_the_vocabulary():
     lp.sum().backward()
     assert h.grad.isnan().any(-1).tolist() == lp.isnan().tolist()
     assert (h.grad[0, 3] == 0).all()
+
+
+@pytest.mark.parametrize('tau', [0.0, -1.0, float('nan'), float('inf')])
+def test_fp32_logprobs_refuse_what_bf16_refuses(tau):
+    m, _, x = model()
+    with pytest.raises(ValueError, match='temperatura'):
+        m.logprobs(x, temperatura=tau)
+    assert m.logprobs(x, temperatura=0.5).shape == x.shape
