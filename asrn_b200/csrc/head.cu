@@ -229,7 +229,12 @@ k_head_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const in
     float t = m;
 #pragma unroll
     for (int j = 0; j < 8; ++j) t = j < n ? fmaxf(t, q[j].x) : t;
-    if (t == -INFINITY) return;                // nothing yet (a NaN in the sums comes with a NaN target score)
+    if (t == -INFINITY) {                      // no score yet but NaNs, which the maxima pass over: the sums hold them
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) s += q[j].y;
+      return;
+    }
     s *= exp2_fast((m - t) * k);
 #pragma unroll
     for (int j = 0; j < 8; ++j)

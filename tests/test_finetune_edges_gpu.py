@@ -10,6 +10,25 @@ from test_finetune_gpu import rand
 pytestmark = pytest.mark.gpu
 
 
+# ---- head ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('V,bad', [(2, 1), (129, 128), (257, 256), (300, 256), (257, 0), (1000, 700)])
+def test_head_a_nan_in_the_weight_reaches_every_target(cuda, V, bad):
+    """Each row's sum runs over all of the vocabulary, the row of `weight` that holds a NaN too."""
+    import asrn_b200 as asrn
+    N, d = 40, 64
+    h, w = rand((N, d), 200), rand((V, d), 201, 0.1)
+    y = torch.arange(N, device='cuda') % V
+    clean = asrn.head_logprobs(h, w, y)
+    assert clean.isfinite().all()
+    w[bad, 5] = float('nan')
+    if V > 256:
+        w[256:] = w[bad]                                     # a part of the vocabulary that holds nothing else
+    assert asrn.head_logprobs(h, w, y).isnan().all()
+    y[3] = -1
+    assert asrn.head_logprobs(h, w, y).isnan().tolist() == [i != 3 for i in range(N)]
+
+
 # ---- losses -------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize('rows', [1024, 1025, 2000])
