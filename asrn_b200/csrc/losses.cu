@@ -126,7 +126,8 @@ __device__ __forceinline__ Pair pair_of(const PrefArgs& a, double r0, double r1,
     const double soft = log1p(exp(-fabs(x)));                    // -log sigma(|x|)
     const double e = exp(-fabs(x));
     const double up = x >= 0. ? e / (1. + e) : 1. / (1. + e);     // sigma(-x)
-    p.loss = (1. - a.smoothing) * (soft - fmin(x, 0.)) + a.smoothing * (soft + fmax(x, 0.));
+    p.loss = (1. - a.smoothing) * (soft - fmin(x, 0.));
+    if (a.smoothing > 0.) p.loss += a.smoothing * (soft + fmax(x, 0.));      // infinite where x is
     if (x != x) p.loss = x;
     p.slope0 = a.beta * (a.smoothing - up);
     p.slope1 = -p.slope0;

@@ -1,11 +1,12 @@
 """The fine-tuning operators (asrn_b200.finetune) at their edges: sizes, values and calls that the tests by operator
 (test_finetune_gpu.py, whose references and bounds these use) do not reach."""
 import ctypes
+import math
 
 import pytest
 import torch
 
-from test_finetune_gpu import rand
+from test_finetune_gpu import E, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -53,6 +54,22 @@ def test_policy_without_sequences_and_with_a_reference(cuda):
     e = torch.zeros(0, 5, device='cuda')
     r = asrn.policy_loss(e, e, e[:, 0], e.bool(), ref_logp=e, kl=0.1)
     assert float(r.loss) == 0 and float(r.kl) == 0 and r.grad.shape == (0, 5)
+
+
+@pytest.mark.parametrize('eps', [0.0, 0.25])
+def test_preference_infinite_margins(cuda, eps):
+    """A token that the reference model holds impossible: the margin is infinite, and the loss what its formula gives
+    there, 0 where the pair is on the right side and nothing is smoothed."""
+    import asrn_b200 as asrn
+    inf = float('inf')
+    lp = torch.zeros(2, 2, 3, device='cuda')
+    m = torch.ones_like(lp, dtype=torch.bool)
+    for side, want, slope in ((0, inf if eps else 0.0, eps), (1, inf, eps - 1.0)):
+        ref = lp.clone()
+        ref[side, 1, 1] = -inf                               # R is +inf in that answer; the other pair's margin is 0
+        r = asrn.preference_loss(lp, ref, m, beta=0.5, smoothing=eps)
+        assert float(r.loss) == pytest.approx(want if want else math.log(2) / 2, rel=4 * E)
+        assert r.grad[0, 1].tolist() == [0.25 * slope] * 3 and r.grad[1, 1].tolist() == [-0.25 * slope] * 3
 
 
 # ---- bounded waits ------------------------------------------------------------------------------------------------------
