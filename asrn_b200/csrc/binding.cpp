@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <cstring>
@@ -136,6 +138,21 @@ void to_bf16(const char* what, std::initializer_list<Tensor*> ts) {
   for (Tensor* t : ts) *t = t->to(at::kBFloat16);
 }
 
+// The backward passes here are no differentiable functions themselves. Where one is recorded (create_graph), what it makes
+// depends on the node's inputs and on `more` through a node that raises: a second derivative is refused, not left out.
+std::shared_ptr<torch::autograd::Node> refusal(const char* what, const variable_list& more) {
+  torch::autograd::edge_list edges = torch::autograd::get_current_node()->next_edges();
+  for (const Tensor& t : more) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  return std::make_shared<torch::autograd::Error>(text("asrn_b200.", what, ": the second derivative is not implemented"),
+                                                  std::move(edges));
+}
+void once(const char* what, variable_list& made, const variable_list& grads) {
+  if (!at::GradMode::is_enabled()) return;
+  const auto node = refusal(what, grads);
+  for (Tensor& t : made)
+    if (t.defined()) torch::autograd::set_history(t, node);
+}
+
 // ---- head ---------------------------------------------------------------------------------------------------------------
 
 struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
@@ -173,7 +190,9 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
                              dw.defined() ? dw.data_ptr() : nullptr, ws.data_ptr(), nb, status_word("head_logprobs", dev),
                              stream_of(dev)),
           "asrn_head_backward");
-    return {dh, dw, Tensor(), Tensor()};
+    variable_list out{dh, dw, Tensor(), Tensor()};
+    once("head_logprobs", out, grads);
+    return out;
   }
 };
 
@@ -244,6 +263,27 @@ Four policy_loss(const Tensor& logp, const Tensor& old, const Tensor& adv, const
                          grad.data_ptr<float>(), o + 1, nb ? ws.data_ptr() : nullptr, nb, stream_of(dev)),
         "asrn_policy_loss");
   return {out.select(0, 0), grad, out.select(0, 1), out.select(0, 2)};
+}
+
+// The loss as a function of logp whose gradient is known: the backward pass scales it.
+struct KnownGradient : torch::autograd::Function<KnownGradient> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logp, const Tensor& loss, const Tensor& grad) {
+    ctx->save_for_backward({grad});
+    ctx->saved_data["type"] = (int64_t)logp.scalar_type();
+    return loss.clone();
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    Tensor grad = ctx->get_saved_variables()[0];
+    if (at::GradMode::is_enabled()) {                      // it depends on logp; the product with grads[0] is recorded
+      grad = grad.detach();
+      torch::autograd::set_history(grad, refusal("the losses", {}));
+    }
+    return {(grad * grads[0]).to((at::ScalarType)ctx->saved_data["type"].toInt()), Tensor(), Tensor()};
+  }
+};
+
+Tensor known_gradient(const Tensor& logp, const Tensor& loss, const Tensor& grad) {
+  return KnownGradient::apply(logp, loss, grad);
 }
 
 // ---- activations in 8 bits ------------------------------------------------------------------------------------------------
@@ -319,6 +359,7 @@ struct Mlp8 : torch::autograd::Function<Mlp8> {
                              at[0], at[1], at[2], at[3], at[4], ws.data_ptr(), nb, status_word("mlp8", dev),
                              stream_of(dev)),
           "asrn_mlp8_backward");
+    once("mlp8", out, grads);
     return out;
   }
 };
@@ -345,6 +386,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("head_logprobs", torch::wrap_pybind_function(&head_logprobs));
   m.def("preference_loss", torch::wrap_pybind_function(&preference_loss));
   m.def("policy_loss", torch::wrap_pybind_function(&policy_loss));
+  m.def("known_gradient", torch::wrap_pybind_function(&known_gradient));
   m.def("pack8", torch::wrap_pybind_function(&pack8));
   m.def("unpack8", torch::wrap_pybind_function(&unpack8));
   m.def("mlp8", torch::wrap_pybind_function(&mlp8));

@@ -14,7 +14,7 @@ The losses return their gradient with the loss (one pass over the tokens makes b
     logp.backward(r.grad)
 
 and r.loss.backward() works as well when logp requires a gradient. Everything runs on CUDA tensors, on the current
-stream, and repeats bit for bit; there is no counterpart in the reference.
+stream, and repeats bit for bit; second derivatives are refused. There is no counterpart in the reference.
 """
 from collections import namedtuple
 
@@ -41,21 +41,6 @@ def head_logprobs(h, weight, tokens, temperatura=1.0):
     return _lib.finetune().head_logprobs(h, weight, tokens, temperatura)
 
 
-class _WithGrad(torch.autograd.Function):
-    """A loss whose gradient is known: backward scales it."""
-
-    @staticmethod
-    def forward(ctx, logp, loss, grad):
-        ctx.save_for_backward(grad)
-        ctx.dtype = logp.dtype
-        return loss.clone()
-
-    @staticmethod
-    def backward(ctx, g):
-        grad, = ctx.saved_tensors
-        return (grad * g).to(ctx.dtype), None, None
-
-
 PreferenceLoss = namedtuple('PreferenceLoss', 'loss grad chosen rejected')
 PolicyLoss = namedtuple('PolicyLoss', 'loss grad kl clipped')
 
@@ -75,7 +60,7 @@ def preference_loss(logp, ref_logp, mask, beta=0.1, smoothing=0.0, kind='sigmoid
         raise ValueError(f'preference_loss: kind is one of {sorted(_KINDS)}')
     loss, grad, chosen, rejected = _lib.finetune().preference_loss(logp, ref_logp, mask, _KINDS[kind], beta, smoothing)
     if logp.requires_grad and torch.is_grad_enabled():
-        loss = _WithGrad.apply(logp, loss, grad)
+        loss = _lib.finetune().known_gradient(logp, loss, grad)
     return PreferenceLoss(loss, grad, chosen, rejected)
 
 
@@ -93,7 +78,7 @@ def policy_loss(logp, old_logp, advantages, mask, ref_logp=None, clip=(0.2, 0.2)
     loss, grad, k3, clipped = _lib.finetune().policy_loss(logp, old_logp, advantages, mask, ref_logp, low, high, kl,
                                                           _PER[per])
     if logp.requires_grad and torch.is_grad_enabled():
-        loss = _WithGrad.apply(logp, loss, grad)
+        loss = _lib.finetune().known_gradient(logp, loss, grad)
     return PolicyLoss(loss, grad, k3, clipped)
 
 

@@ -72,6 +72,45 @@ def test_preference_infinite_margins(cuda, eps):
         assert r.grad[0, 1].tolist() == [0.25 * slope] * 3 and r.grad[1, 1].tolist() == [-0.25 * slope] * 3
 
 
+# ---- derivatives --------------------------------------------------------------------------------------------------------
+
+def penalty_calls():
+    import asrn_b200 as asrn
+    h, w, y = rand((5, 16), 230), rand((9, 16), 231, 0.3), torch.arange(5, device='cuda')
+    u, v, b = rand((8, 16), 232, 0.3), rand((16, 8), 233, 0.3), rand((8,), 234)
+    z, m = torch.zeros(2, 3, 4, device='cuda'), torch.ones(2, 3, 4, dtype=torch.bool, device='cuda')
+    return {'head': (h, lambda x: asrn.head_logprobs(x, w, y).sum()),
+            'mlp8': (h, lambda x: asrn.mlp8(x, u, b, v, h[0]).float().square().sum()),
+            'preference': (z.clone(), lambda x: asrn.preference_loss(x, z, m).loss),
+            'policy': (z[0].clone(), lambda x: asrn.policy_loss(x, z[0], z[0, :, 0] + 1, m[0]).loss)}
+
+
+@pytest.mark.parametrize('which', ['head', 'mlp8', 'preference', 'policy'])
+def test_second_derivatives_are_refused(cuda, which):
+    x, f = penalty_calls()[which]
+    x.requires_grad_()
+    first, = torch.autograd.grad(f(x), x)
+    d, = torch.autograd.grad(f(x), x, create_graph=True)
+    assert torch.equal(d, first)                             # the first derivative is there as ever
+    penalty = d.float().square().sum() + x.float().square().sum()      # another term keeps the graph alive
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(penalty, x)
+    d, = torch.autograd.grad(f(x), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        (d.float().square().sum() + x.float().square().sum()).backward()
+
+
+def test_loss_scaled_by_a_parameter_that_learns(cuda):
+    """The gradient is linear in what the loss is multiplied by, and that derivative is there."""
+    import asrn_b200 as asrn
+    z, m = torch.zeros(2, 3, 4, device='cuda'), torch.ones(2, 3, 4, dtype=torch.bool, device='cuda')
+    x, s = z.clone().requires_grad_(), torch.tensor(3.0, device='cuda', requires_grad=True)
+    r = asrn.preference_loss(x, z, m)
+    d, = torch.autograd.grad(r.loss * s, x, create_graph=True)
+    ds, = torch.autograd.grad(d.sum() + d[0].sum(), s)
+    assert torch.allclose(ds, r.grad.sum() + r.grad[0].sum())
+
+
 # ---- bounded waits ------------------------------------------------------------------------------------------------------
 
 TIMEOUT = 5
