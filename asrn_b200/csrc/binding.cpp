@@ -215,12 +215,17 @@ Tensor head_logprobs(Tensor h, Tensor weight, const Tensor& tokens, double tau) 
 
 using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 
+void no_tangent(const char* what, const Tensor& logp) {
+  if (logp._fw_grad(0).defined()) not_implemented(text(what, ": forward-mode derivatives are not implemented"));
+}
+
 Four preference_loss(const Tensor& logp, const Tensor& ref, const Tensor& mask, int64_t kind, double beta, double smoothing) {
   if (logp.dim() != 3 || logp.size(0) != 2 || ref.sizes() != logp.sizes())
     throw py::value_error(text("preference_loss: logp and ref_logp are (2, P, L); got ", logp.sizes(), " and ", ref.sizes()));
   if (!(beta > 0) || !(smoothing >= 0 && smoothing < 0.5))
     throw py::value_error("preference_loss: beta > 0 and 0 <= smoothing < 0.5");
   const c10::Device dev = device_of("preference_loss", {&logp, &ref, &mask});
+  no_tangent("preference_loss", logp);
   at::AutoDispatchBelowADInplaceOrView below;            // nothing here is differentiated
   c10::cuda::CUDAGuard guard(dev);
   const Tensor m = mask_of("preference_loss", mask, logp.sizes()), lp = f32(logp), rf = f32(ref);
@@ -250,6 +255,7 @@ Four policy_loss(const Tensor& logp, const Tensor& old, const Tensor& adv, const
     throw py::value_error("policy_loss: 0 <= clip[0] < 1, clip[1] >= 0 and kl >= 0");
   if (kl > 0 && !ref.defined()) throw py::value_error("policy_loss: a KL term needs ref_logp");
   const c10::Device dev = device_of("policy_loss", {&logp, &old, &adv, &mask, &ref});
+  no_tangent("policy_loss", logp);
   at::AutoDispatchBelowADInplaceOrView below;            // nothing here is differentiated
   c10::cuda::CUDAGuard guard(dev);
   const Tensor m = mask_of("policy_loss", mask, logp.sizes()), lp = f32(logp), ol = f32(old), ad = f32(adv);

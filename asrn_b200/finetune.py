@@ -14,7 +14,8 @@ The losses return their gradient with the loss (one pass over the tokens makes b
     logp.backward(r.grad)
 
 and r.loss.backward() works as well when logp requires a gradient. Everything runs on CUDA tensors, on the current
-stream, and repeats bit for bit; second derivatives are refused. There is no counterpart in the reference.
+stream, and repeats bit for bit; second derivatives and forward-mode ones are refused. There is no
+counterpart in the reference.
 """
 from collections import namedtuple
 

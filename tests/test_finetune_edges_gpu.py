@@ -111,6 +111,14 @@ def test_loss_scaled_by_a_parameter_that_learns(cuda):
     assert torch.allclose(ds, r.grad.sum() + r.grad[0].sum())
 
 
+@pytest.mark.parametrize('which', ['head', 'mlp8', 'preference', 'policy'])
+def test_forward_mode_is_refused(cuda, which):
+    import torch.autograd.forward_ad as fwd
+    x, f = penalty_calls()[which]
+    with fwd.dual_level(), pytest.raises(NotImplementedError if which in ('preference', 'policy') else RuntimeError):
+        f(fwd.make_dual(x, torch.ones_like(x)))
+
+
 # ---- bounded waits ------------------------------------------------------------------------------------------------------
 
 TIMEOUT = 5
