@@ -24,6 +24,12 @@ def firmas_de_piezas(piezas):
     return piezas.to(torch.float32)
 
 
+def _sin_ganchos(m):
+    """True when calling m is its class's forward and nothing else: no hooks, no forward put on the module itself."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or
+                'forward' in vars(m))
+
+
 class BloqueLocal(nn.Module):
     """Causal local context: dense convolution over the k-1 previous tokens and the current one, then an MLP
     (asrn/nucleo.py:969-1014, the default mezcla='conv')."""
@@ -52,10 +58,17 @@ class BloqueLocal(nn.Module):
         return h + self.drop(self.ff(u))
 
     def _mlp8_ok(self, u):
-        """mlp8 serves training under bf16 autocast on CUDA and widths that are multiples of 8."""
+        """mlp8 serves training under bf16 autocast on CUDA and widths that are multiples of 8, for the MLP as it was built:
+        modules put in its place, and modules with hooks or a forward of their own, are called."""
+        if not (u.is_cuda and torch.is_grad_enabled() and torch.is_autocast_enabled('cuda') and
+                torch.get_autocast_dtype('cuda') == torch.bfloat16):
+            return False
+        modules = [self.ff, *self.ff]
+        if [type(m) for m in modules] != [nn.Sequential, nn.Linear, nn.GELU, nn.Linear]:
+            return False
         d, ff = self.conv.in_channels, self.ff[0].out_features
-        return (u.is_cuda and torch.is_grad_enabled() and torch.is_autocast_enabled('cuda') and d % 8 == 0 and
-                ff % 8 == 0 and torch.get_autocast_dtype('cuda') == torch.bfloat16)
+        return (d % 8 == 0 and ff % 8 == 0 and self.ff[0].bias is not None and self.ff[2].bias is not None and
+                self.ff[1].approximate == 'none' and all(map(_sin_ganchos, modules)))
 
     def _fused_ok(self, h):
         """The fused CUDA block (asrn_local_block) serves bf16 autocast on CUDA, fp32 h, no dropout at work, and the

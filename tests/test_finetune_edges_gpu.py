@@ -172,3 +172,50 @@ def test_an_earlier_calls_timeout_stops_no_later_call(cuda):
         assert int(word) == before
         out.append((lp, z))
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+# ---- the model's blocks --------------------------------------------------------------------------------------------------
+
+def block8(d=64):
+    import asrn_b200 as asrn
+    m = asrn.create_model(V=64, d=d, n_capas=2, semilla=0, checkpoint='8bits').cuda().train()
+    return m.bloques[0], torch.randn(2, 33, d, generator=torch.Generator().manual_seed(1)).cuda()
+
+
+@pytest.mark.parametrize('how', ['hook', 'pre-hook', 'backward hook', 'other linear', 'activation', 'no bias', 'forward'])
+def test_8bit_blocks_call_the_mlps_own_modules_where_they_do_more(cuda, how):
+    blq, h = block8()
+    seen = []
+    lin, act = blq.ff[0], blq.ff[1]
+    if how == 'hook':
+        lin.register_forward_hook(lambda m, i, o: seen.append(1) or o * 2)
+    elif how == 'pre-hook':
+        blq.ff.register_forward_pre_hook(lambda m, i: seen.append(1))
+    elif how == 'backward hook':
+        act.register_full_backward_hook(lambda m, i, o: seen.append(1))
+    elif how == 'other linear':
+        class Twice(torch.nn.Linear):
+            def forward(self, x):
+                seen.append(1)
+                return 2 * super().forward(x)
+        new = Twice(lin.in_features, lin.out_features).cuda()
+        new.load_state_dict(lin.state_dict())
+        blq.ff[0] = new
+    elif how == 'activation':
+        class Relu(torch.nn.ReLU):
+            def forward(self, x):
+                seen.append(1)
+                return super().forward(x)
+        blq.ff[1] = Relu()
+    elif how == 'no bias':
+        blq.ff[0].bias = None
+        seen.append(1)
+    else:
+        own = lin.forward
+        lin.forward = lambda x: seen.append(1) or own(x)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        out = blq(h)
+        out.sum().backward()
+        assert seen
+        blq.activaciones_8bits = False
+        assert torch.equal(blq(h), out)
