@@ -168,8 +168,9 @@ class ModeloASRN(nn.Module):
     def logprobs(self, x, objetivos=None, temperatura=1.0):
         """log softmax(logits / temperatura) of the tokens objetivos (B, L) at the positions of x (B, L), float32: by
         default each position's next token (0 at the last one). A negative target leaves its position out: 0 and no
-        gradient; one outside the vocabulary gives NaN. Under bf16 autocast the (B, L, V) logits are never in memory and positions left out cost nothing
-        (head_logprobs); the fp32 model takes them from its logits."""
+        gradient; one outside the vocabulary gives NaN. Under bf16 autocast the (B, L, V) logits are not kept and
+        positions left out cost nothing (head_logprobs); the fp32 model, and one whose head was replaced or has hooks,
+        takes them from its logits."""
         if objetivos is None:
             objetivos = F.pad(x[:, 1:], (0, 1), value=-1)
         if objetivos.shape != x.shape:
@@ -178,7 +179,8 @@ class ModeloASRN(nn.Module):
             raise ValueError('logprobs: temperatura has to be positive')
         h = self.estado(x)
         if h.is_cuda and torch.is_autocast_enabled('cuda') and h.shape[-1] % 8 == 0 and \
-                torch.get_autocast_dtype('cuda') == torch.bfloat16:
+                torch.get_autocast_dtype('cuda') == torch.bfloat16 and type(self.head) is nn.Linear and \
+                self.head.bias is None and _sin_ganchos(self.head):
             return head_logprobs(h, self.head.weight, objetivos, temperatura)
         lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
         V = lp.shape[-1]                                 # an index outside would stop the GPU's context

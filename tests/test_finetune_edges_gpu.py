@@ -219,3 +219,24 @@ def test_8bit_blocks_call_the_mlps_own_modules_where_they_do_more(cuda, how):
         assert seen
         blq.activaciones_8bits = False
         assert torch.equal(blq(h), out)
+
+
+@pytest.mark.parametrize('how', ['hook', 'bias', 'other class'])
+def test_logprobs_call_the_head_where_it_does_more(cuda, how):
+    """A head that is more than its weight (a hook, a bias, a class of its own) is called, in bf16 too."""
+    import asrn_b200 as asrn
+    m = asrn.create_model(V=64, d=64, n_capas=2, semilla=0).cuda()
+    x = torch.randint(0, 64, (2, 33), generator=torch.Generator().manual_seed(2)).cuda()
+    if how == 'hook':
+        m.head.register_forward_hook(lambda _, i, o: o * 3)
+    else:
+        class Shifted(torch.nn.Linear):
+            def forward(self, h):
+                return 3 * super().forward(h)
+        new = (Shifted if how == 'other class' else torch.nn.Linear)(64, 64, bias=how == 'bias').cuda()
+        m.head = new
+    with torch.no_grad(), torch.autocast('cuda', dtype=torch.bfloat16):
+        h = m.estado(x)
+        m.estado = lambda x: h
+        want = torch.log_softmax(m(x).float(), -1)[:, :-1].gather(-1, x[:, 1:, None])[..., 0]
+        assert torch.equal(m.logprobs(x)[:, :-1], want)
