@@ -141,6 +141,8 @@ class ModeloASRN(nn.Module):
         assert V <= 2 ** 24, 'token signatures are exact up to 2**24 tokens'
         self.config = dict(V=V, d=d, n_capas=n_capas, largo_cada=largo_cada, ff=ff or 2 * d, k=k, dropout=dropout,
                            mezcla=mezcla, memoria_max=memoria_max, opciones_capa=dict(opciones_capa))
+        if isinstance(checkpoint, str) and checkpoint != '8bits':
+            raise ValueError(f"checkpoint is False, True or '8bits'; got {checkpoint!r}")
         self.n_capas, self.checkpoint = n_capas, checkpoint
         self.init_profundo = n_capas >= 8 if init_profundo is None else bool(init_profundo)
         self.pos_largo = [i for i in range(n_capas - 1) if i % largo_cada == 0]

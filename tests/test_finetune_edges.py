@@ -33,3 +33,13 @@ def test_fp32_logprobs_refuse_what_bf16_refuses(tau):
     with pytest.raises(ValueError, match='temperatura'):
         m.logprobs(x, temperatura=tau)
     assert m.logprobs(x, temperatura=0.5).shape == x.shape
+
+
+def test_checkpoint_takes_no_other_text():
+    """A mistyped '8bits' turned nothing on and said nothing."""
+    import asrn_b200 as asrn
+    for text in ('8bit', '8 bits', 'fp8', ''):
+        with pytest.raises(ValueError, match='checkpoint'):
+            asrn.create_model(V=11, d=16, n_capas=2, checkpoint=text)
+    for value in (False, True, None, 0, 1):
+        assert asrn.create_model(V=11, d=16, n_capas=2, checkpoint=value).checkpoint is value
