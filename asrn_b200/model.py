@@ -275,11 +275,13 @@ def _migrate_streak(pesos):
     return pesos
 
 
-def cargar(archivo, dispositivo=None, confiar=False, protecciones=None):
+def cargar(archivo, dispositivo=None, confiar=False, protecciones=None, checkpoint=False):
     """Load a model written by guardar() here or by the reference's guardar() / entrenar() (its v83 to v89 files;
     asrn/nucleo.py:2110-2133, asrn/__init__.py:73-75). Read with torch.load(weights_only=True) unless confiar=True.
     Weights missing from files older than v87 keep their initial (neutral) values, as the reference does; any other
-    missing or unexpected weight is an error. Returns the model on `dispositivo` (default: cuda) in eval mode."""
+    missing or unexpected weight is an error. The file does not say how the model is trained: `checkpoint` does, as in
+    crear_modelo ('8bits' to tune a trained model with 8-bit activations). Returns the model on `dispositivo` (default:
+    cuda) in eval mode."""
     import os
     if not os.path.isfile(archivo):
         raise FileNotFoundError(f'no such file: {archivo}')
@@ -294,8 +296,8 @@ def cargar(archivo, dispositivo=None, confiar=False, protecciones=None):
         raise ValueError(f'{archivo}: not a model written by guardar() / entrenar() of ASRN')
     c = dict(r['config'])
     m = ModeloASRN(c['V'], c['d'], c['n_capas'], c['largo_cada'], c['ff'], c['k'], init_profundo=False,
-                   dropout=c.get('dropout', 0.0), mezcla=c.get('mezcla', 'conv'), memoria_max=c.get('memoria_max', 1024),
-                   protecciones=protecciones, **c['opciones_capa'])
+                   checkpoint=checkpoint, dropout=c.get('dropout', 0.0), mezcla=c.get('mezcla', 'conv'),
+                   memoria_max=c.get('memoria_max', 1024), protecciones=protecciones, **c['opciones_capa'])
     faltan, sobran = m.load_state_dict(_migrate_streak(r['pesos']), strict=False)
     raros = [n for n in faltan if n.rsplit('.', 1)[-1] not in _NEW_IN_V87]
     if sobran or raros:

@@ -43,3 +43,16 @@ def test_checkpoint_takes_no_other_text():
             asrn.create_model(V=11, d=16, n_capas=2, checkpoint=text)
     for value in (False, True, None, 0, 1):
         assert asrn.create_model(V=11, d=16, n_capas=2, checkpoint=value).checkpoint is value
+
+
+def test_a_loaded_model_can_keep_activations_in_8_bits(tmp_path):
+    import asrn_b200 as asrn
+    m = asrn.create_model(V=11, d=16, n_capas=2, semilla=0, checkpoint='8bits')
+    asrn.save(m, str(tmp_path / 'm.pt'))
+    load = lambda **kw: asrn.load(str(tmp_path / 'm.pt'), dispositivo='cpu', **kw)  # noqa: E731
+    assert not any(b.activaciones_8bits for b in load().bloques)         # the file does not say
+    back = load(checkpoint='8bits')
+    assert back.checkpoint == '8bits' and all(b.activaciones_8bits for b in back.bloques)
+    assert all(torch.equal(a, b) for a, b in zip(m.state_dict().values(), back.state_dict().values()))
+    with pytest.raises(ValueError):
+        load(checkpoint='8')
