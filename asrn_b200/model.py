@@ -34,12 +34,15 @@ class BloqueLocal(nn.Module):
     """Causal local context: dense convolution over the k-1 previous tokens and the current one, then an MLP
     (asrn/nucleo.py:969-1014, the default mezcla='conv')."""
 
+    # True: the MLP keeps its activations in 8 bits for the backward pass. Of the class: blocks that were pickled before
+    # it was there have none of their own.
+    activaciones_8bits = False
+
     def __init__(self, d, k=4, ff=128, dropout=0.0, mezcla='conv', memoria_max=1024):
         super().__init__()
         if mezcla != 'conv':
             raise NotImplementedError("asrn_b200 builds the default local block (mezcla='conv')")
         self.k, self.mezcla = k, mezcla
-        self.activaciones_8bits = False        # the MLP keeps its activations in 8 bits for the backward pass
         self.ln1 = nn.LayerNorm(d)
         self.conv = nn.Conv1d(d, d, k)
         self.ln2 = nn.LayerNorm(d)

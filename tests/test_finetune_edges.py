@@ -56,3 +56,12 @@ def test_a_loaded_model_can_keep_activations_in_8_bits(tmp_path):
     assert all(torch.equal(a, b) for a, b in zip(m.state_dict().values(), back.state_dict().values()))
     with pytest.raises(ValueError):
         load(checkpoint='8')
+
+
+def test_a_block_pickled_without_the_8bit_setting_still_runs():
+    import asrn_b200 as asrn
+    blq = asrn.create_model(V=11, d=16, n_capas=2, semilla=0).bloques[0]
+    h = torch.randn(2, 5, 16, generator=torch.Generator().manual_seed(3))
+    want = blq(h)
+    vars(blq).pop('activaciones_8bits', None)
+    assert torch.equal(blq(h), want)
