@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_finetune_gpu import E, rand
+from test_finetune_gpu import E, U, lengths_mask, mlp_reference, policy_reference, pref_reference, rand, run_mlp
 
 pytestmark = pytest.mark.gpu
 
@@ -28,6 +28,61 @@ def test_head_a_nan_in_the_weight_reaches_every_target(cuda, V, bad):
     assert asrn.head_logprobs(h, w, y).isnan().all()
     y[3] = -1
     assert asrn.head_logprobs(h, w, y).isnan().tolist() == [i != 3 for i in range(N)]
+
+
+def head_by_rows(h, w, y, g):
+    """head_reference's logp, dh, dw and bounds' sums, some rows at a time."""
+    w = w.double()
+    lp, dh, sh = [], [], []
+    dw, sw, size = torch.zeros_like(w), torch.zeros_like(w), 0.0
+    for i in range(0, h.shape[0], 128):
+        hi, yi, gi = h[i:i + 128].double(), y[i:i + 128], g[i:i + 128].double()
+        z = hi @ w.t()
+        on = (yi >= 0).double()
+        logz = torch.log_softmax(z, 1)
+        at = yi.clamp(min=0)[:, None]
+        own = logz.gather(1, at)[:, 0]
+        ds = -logz.exp() * (on * gi)[:, None]
+        others = ds.sum(1) - ds.gather(1, at)[:, 0]
+        ds.scatter_(1, at, -others[:, None])
+        lp.append(own * on)
+        dh.append(ds @ w)
+        sh.append(ds.abs() @ w.abs())
+        dw += ds.t() @ hi
+        sw += ds.abs().t() @ hi.abs()
+        size = max(size, float((hi.abs() @ w.abs().t()).amax()))
+    return torch.cat(lp), torch.cat(dh), dw, torch.cat(sh), sw, size
+
+
+@pytest.mark.parametrize('N,V,d,left', [(1500, 1 << 20, 8, 'third'), (1025, 1 << 20, 16, 'none'), (6000, 200003, 64, 'third'),
+                                        (6000, 200003, 64, 'first'), (6000, 200003, 64, 'edge'),
+                                        (6000, 200003, 64, 'all')])
+def test_head_rows_in_several_chunks(cuda, N, V, d, left):
+    """dS of all rows is over two gigabytes: it is made by chunks of rows, dW adding up over them; targets in every
+    chunk, in the first one only, up to the second one's very start, and none at all."""
+    import asrn_b200 as asrn
+    from asrn_b200 import _lib
+    pad, pitch = (N + 255) // 256 * 256, (V + 63) // 64 * 64
+    assert _lib.lib().asrn_head_workspace_bytes(N, V, d, 1) < 0.9 * 2 * pad * pitch
+    y = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(210)).cuda()
+    if left == 'third':
+        y[::3] = -1
+    elif left == 'first':
+        y[500:] = -1
+    elif left == 'edge':
+        y[3072:] = -1                                        # the first chunk's rows: half of them, in blocks of 256
+    elif left == 'all':
+        y[:] = -1
+    h, w = rand((N, d), 211).requires_grad_(), rand((V, d), 212, 0.1).requires_grad_()
+    g = rand((N,), 213, dtype=torch.float32)
+    logp = asrn.head_logprobs(h, w, y)
+    dh, dw = torch.autograd.grad(logp, (h, w), g)
+    ref, rh, rw, sh, sw, size = head_by_rows(h.detach(), w.detach(), y, g)
+    tol = 4 * E * (d / 16 + 2) * size + 16 * E * (1 + ref.abs())
+    assert ((logp.double() - ref).abs() <= tol).all()
+    assert (logp[y < 0] == 0).all() and (dh[y < 0] == 0).all()
+    assert ((dh.double() - rh).abs() <= U * (rh.abs() + sh) + 1e-30).all()
+    assert ((dw.double() - rw).abs() <= U * (rw.abs() + sw) + 1e-30).all()
 
 
 # ---- losses -------------------------------------------------------------------------------------------------------------
@@ -70,6 +125,91 @@ def test_preference_infinite_margins(cuda, eps):
         r = asrn.preference_loss(lp, ref, m, beta=0.5, smoothing=eps)
         assert float(r.loss) == pytest.approx(want if want else math.log(2) / 2, rel=4 * E)
         assert r.grad[0, 1].tolist() == [0.25 * slope] * 3 and r.grad[1, 1].tolist() == [-0.25 * slope] * 3
+
+
+@pytest.mark.parametrize('P,L', [(700, 2049), (300, 4096), (300, 20001), (300, 20000)])
+@pytest.mark.parametrize('kind,eps', [('sigmoid', 0.2), ('ipo', 0.0)])
+def test_preference_two_launches(cuda, P, L, kind, eps):
+    """More than 2^21 tokens; from 16 chunks of 1024 in a row's part on the masks are read again."""
+    import asrn_b200 as asrn
+    assert 2 * P * L > 1 << 21
+    ref = -rand((2, P, L), 240, dtype=torch.float32).abs()
+    logp = ref + rand((2, P, L), 241, 0.02, torch.float32)
+    mask = torch.stack([lengths_mask(P, L, 242, range(7, P, 9)), lengths_mask(P, L, 243, range(3, P, 11))])
+    logp = torch.where(mask, logp, float('nan'))
+    ref = torch.where(mask, ref, float('inf'))
+    r = asrn.preference_loss(logp, ref, mask, beta=0.3, smoothing=eps, kind=kind)
+    loss, grad, rew = pref_reference(logp, ref, mask, 0.3, eps, kind)
+    assert abs(float(r.loss) - float(loss)) <= 4 * E * max(1.0, abs(float(loss)))
+    assert (r.grad.double() - grad).abs().max() <= 4 * E * max(float(grad.abs().max()), 1e-30)
+    assert (r.grad[~mask] == 0).all()
+    got = torch.stack([r.chosen, r.rejected]).double()
+    assert (got - rew).abs().max() <= 4 * E * max(float(rew.abs().max()), 1e-30)
+
+
+@pytest.mark.parametrize('B,L', [(300, 1111), (129, 4096), (20, 40001)])
+@pytest.mark.parametrize('per', ['token', 'sequence'])
+@pytest.mark.parametrize('per_token,with_ref', [(False, True), (False, False), (True, True)])
+def test_policy_two_launches(cuda, B, L, per, per_token, with_ref):
+    """More than 2^18 tokens."""
+    import asrn_b200 as asrn
+    assert B * L > 1 << 18
+    old = -rand((B, L), 250, dtype=torch.float32).abs() * 3
+    logp = old + rand((B, L), 251, 0.3, torch.float32)
+    ref = old + rand((B, L), 252, 0.3, torch.float32) if with_ref else None
+    adv = rand((B, L) if per_token else (B,), 253, dtype=torch.float32)
+    mask = lengths_mask(B, L, 254, range(5, B, 6))
+    bad = torch.full_like(logp, float('nan'))
+    logp, old = torch.where(mask, logp, bad), torch.where(mask, old, bad)
+    ref = None if ref is None else torch.where(mask, ref, bad)
+    adv = torch.where(mask, adv, bad) if per_token else adv
+    kl = 0.1 if with_ref else 0.0
+    r = asrn.policy_loss(logp, old, adv, mask, ref_logp=ref, clip=(0.2, 0.3), kl=kl, per=per)
+    a = torch.where(mask, adv, torch.zeros_like(adv)) if per_token else adv
+    loss, grad, k3, cut = policy_reference(logp, old, a, mask, ref, (0.2, 0.3), kl, per)
+    size = 8 * float(a.abs().max()) + 1
+    assert abs(float(r.loss) - float(loss)) <= 8 * E * size
+    assert (r.grad.double() - grad).abs().max() <= 16 * E * max(float(grad.abs().max()), 1e-30)
+    assert (r.grad[~mask] == 0).all()
+    assert abs(float(r.kl) - float(k3)) <= 8 * E * max(1.0, float(k3)) and abs(float(r.clipped) - float(cut)) <= 2 * E
+
+
+def test_policy_ratio_against_exp(cuda):
+    """With an advantage of 1, no upper bound and 2^12 tokens the gradient is -exp(logp - old_logp) / 2^12: the
+    exponential by itself. ex2.approx is off by 2^-22 of its result at most, the product's rounding is made up for to the
+    first order (the second is below 2^-40), and the last addition rounds once: 2^-24."""
+    import asrn_b200 as asrn
+    d = torch.cat([torch.linspace(-20, 20, 3000), torch.linspace(-0.01, 0.01, 1090),
+                   torch.tensor([20.0, -20.0, 0.0, -0.0, 1e-30, 2.0 ** -24])]).view(1, -1).cuda()
+    assert d.numel() == 4096
+    m = torch.ones_like(d, dtype=torch.bool)
+    r = asrn.policy_loss(d, torch.zeros_like(d), torch.ones(1, device='cuda'), m, clip=(0.2, 1e30))
+    got, want = -r.grad.double() * 4096, d.double().exp()
+    assert float(r.clipped) == 0 and ((got - want).abs() <= (2.0 ** -22 + 2.0 ** -24) * 1.01 * want).all()
+
+
+# ---- 8 bits -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('N', [600, 2051])
+def test_mlp8_exponents_outside_the_table(cuda, N):
+    """More than 512 rows, and columns whose x w1^T + b1 is above 254 or below 0.004 all over: gelu and its derivative
+    of those blocks are computed, not looked up. Exact sums, as in test_mlp8_on_exact_sums, and its bound."""
+    from asrn_b200 import finetune as ft
+    d, ff, dout = 64, 160, 64
+    g = torch.Generator().manual_seed(220)
+    ints = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g).float()  # noqa: E731
+    x, w1, b1 = ints(-4, 4, N, d) / 4, ints(-2, 2, ff, d) / 8, ints(-8, 8, ff) / 8
+    scale = torch.tensor([1.0, 2.0 ** 10, 2.0 ** -12, 1.0, 2.0 ** 20]).repeat_interleave(32)
+    w1, b1 = w1 * scale[:, None], b1 * scale
+    w2, b2, dy = ints(-4, 4, dout, ff) / 16, ints(-4, 4, dout) / 4, ints(-8, 8, N, dout) / 64
+    ts = [t.bfloat16().cuda() for t in (x, w1, b1, w2, b2, dy)]
+    e = ft.pack8((ts[0].float() @ ts[1].float().t() + ts[2].float()).bfloat16()).exps
+    assert (e[:, 0] >= -14).all() and (e[:, 1] > 1).any() and (e[:, 2] < -14).all() and (e[:, 4] > 1).all()
+    got = run_mlp(*ts)
+    want, size = mlp_reference(*ts)
+    for k in want:
+        err = (got[k].double() - want[k]).abs()
+        assert (err <= U * (want[k].abs() + size[k]) + 1e-30).all(), (k, float((err / (size[k] + 1e-30)).max()))
 
 
 # ---- derivatives --------------------------------------------------------------------------------------------------------
