@@ -25,7 +25,9 @@
 //
 // An operand that was rounded to bf16 can be given as two, the rounded values and what the rounding took, stacked in one
 // tensor: the product then runs over K twice (`second_pass`), the second time on the remainders. Operators do so for few rows,
-// where one rounding error can be most of a result's; a sum over many rows averages them.
+// where it is cheap: a weight's gradient, a sum over these rows, would hold one rounding error for nearly all of its own,
+// where many rows average them. Results by row (the sums run over a width or the vocabulary) gain a factor of 1.4 in the
+// 2-norm at any number of rows; they come along.
 //
 // Every wait is bounded; after a timeout the kernel records it in the status word, waits (bounded, too) for the copies and
 // the multiplications that it has under way, frees its TMEM and ends. What the word holds from earlier calls stops no later one.

@@ -1,12 +1,14 @@
 // Losses of fine-tuning on per-token log probabilities, each with its gradient in the same call: the preference loss of
 // answer pairs and the clipped policy loss with a KL term. Both read each token once (13 and 17 to 21 bytes with the
-// gradient written) and compute next to nothing, so they are bound by HBM when large and by the launches when small.
+// gradient written; the policy loss reads only the mask where a warp's tokens are all outside it) and compute next to
+// nothing, so HBM bounds what they could do when large, and the launches when small.
 //
 // Every sum is formed in a fixed order in fp64 (per thread, then by warp shuffles, then over the blocks' partials in
-// index order): the results do not depend on the blocks' timing. On the device: preference 512 pairs x 4096 19 us (54.5 MB),
+// index order; in policy_main four neighbouring tokens are added in fp32 first): the results do not depend on the blocks'
+// timing. On the device: preference 512 pairs x 4096 19 us (54.5 MB),
 // policy 512 x 8192 26 us (88 MB, a third of the tokens counted): dependent rounds of loads, and about 100 instructions
-// for a counted token; small calls 5.5 to 8 us, half of what the host needs to issue them. Positions outside the mask are
-// read but selected away, never multiplied, so a NaN or infinity there reaches nothing.
+// for a counted token; small calls 5.5 to 8 us, half of what the host needs to issue them. What is read outside the mask is
+// selected away, never multiplied, so a NaN or infinity there reaches nothing.
 #include <algorithm>
 #include <initializer_list>
 #include <cooperative_groups.h>
@@ -322,7 +324,9 @@ __device__ __forceinline__ float held20(float x) {
   return y;
 }
 
-// e^x for |x| <= 20: 2^(x log2 e), the product's rounding (and log2 e's own) made up for.
+// e^x for |x| <= 20 as 2^t, t = x log2 e rounded. What the rounding took (the product's by fma, and the part of log2 e that
+// its float leaves out) is x log2 e - t = `lost`, below 2^-19; 2^lost = 1 + lost ln 2 to the first order, whose error is below
+// 2^-40: within ex2.approx's 2^-22 and one rounding of e^x.
 __device__ __forceinline__ float exp_held(float x) {
   const float t = x * 1.4426950408889634f;
   const float lost = fmaf(x, 1.4426950408889634f, -t) + x * 1.9259629911e-8f;
