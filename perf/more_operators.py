@@ -138,7 +138,7 @@ def _own(c, s):
         r = asrn.layer_norm(s['x'], s['w'], s['b'], residual=s['res'], eps=EPS, dtype=TYPES[c['y']])
         out = dict(y=r) if s['res'] is None else dict(y=r[0], s=r[1])
         into = _given(dx=s['x'], dres=s['res'], dw=s['w'], db=s['b'])
-        up = (s['dy'],) if s['res'] is None else (s['dy'], s['ds']) if c['grad'] else None
+        up = None if not c['grad'] else (s['dy'],) if s['res'] is None else (s['dy'], s['ds'])
     elif c['op'] == 'linear':
         act = None if c['act'] == 'none' else c['act']
         out = dict(y=asrn.linear(s['x'], s['w'], s['b'], activation=act, residual=s['res']))
