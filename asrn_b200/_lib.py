@@ -139,6 +139,23 @@ _SIGS = {
                           [ctypes.c_size_t, _P, ctypes.c_size_t, _P, _P]),
     'asrn_mlp8_backward': (ctypes.c_int, [ctypes.c_int64] + [ctypes.c_int32] * 3 + [_P] * 4 + [ctypes.c_size_t] +
                            [_P] * 6 + [ctypes.c_size_t, _P, _P]),
+    'asrn_layer_norm': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int32, _P, ctypes.c_int32, _P, _P,
+                                       ctypes.c_int32, ctypes.c_float, _P, _P, ctypes.c_int32, _P, _P]),
+    'asrn_layer_norm_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+    'asrn_layer_norm_backward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int32, _P, _P, ctypes.c_int32,
+                                                _P, _P, ctypes.c_int32] + [_P] * 5 + [ctypes.c_size_t, _P]),
+    'asrn_linear_forward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, ctypes.c_int32, _P,
+                                           ctypes.c_int32, _P, _P, _P, _P]),
+    'asrn_linear_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64] + [ctypes.c_int32] * 4),
+    'asrn_linear_backward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _P, ctypes.c_int32, _P, _P,
+                                            ctypes.c_int32] + [_P] * 5 + [ctypes.c_size_t, _P, _P]),
+    'asrn_head_stats_saved_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+    'asrn_head_stats_workspace_bytes': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int32] * 3),
+    'asrn_head_stats_forward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P, _P, ctypes.c_float,
+                                               ctypes.c_int32] + [_P] * 5 + [ctypes.c_size_t, _P, ctypes.c_size_t, _P,
+                                                                             _P]),
+    'asrn_head_stats_backward': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P, ctypes.c_size_t,
+                                                ctypes.c_float] + [_P] * 5 + [ctypes.c_size_t, _P, _P]),
     'asrn_argmax_rows': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int32, _P, _P]),
     'asrn_sampler_seed_state': (ctypes.c_int, [ctypes.c_uint64, _P]),
     'asrn_sampler_jump_poly': (ctypes.c_int, [ctypes.c_uint64, _P]),

@@ -386,6 +386,335 @@ Tensor mlp8(Tensor x, Tensor w1, Tensor b1, Tensor w2, Tensor b2) {
   return Mlp8::apply(x, w1, b1, w2, b2, keep && at::GradMode::is_enabled());
 }
 
+// Whether a call on these tensors is recorded (also where only a forward-mode derivative is: the recorded call refuses it).
+bool recorded(std::initializer_list<const Tensor*> ts) {
+  bool grad = false, tangent = false;
+  for (const Tensor* t : ts)
+    if (t->defined()) {
+      grad |= t->requires_grad();
+      tangent |= t->_fw_grad(0).defined();
+    }
+  return (grad && at::GradMode::is_enabled()) || tangent;
+}
+int type_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 1 : 0; }
+bool float_or_bf16(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+using MaybeTensor = std::optional<Tensor>;
+Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
+MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+void* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ---- head: entropy and likeliest tokens -----------------------------------------------------------------------------------
+
+struct StatsOut {
+  Tensor logp, entropy, top_logp, top_tokens, saved, weight;
+};
+
+StatsOut stats_forward(const Tensor& h, const Tensor& weight, const Tensor& tokens, double tau, int64_t top) {
+  const c10::Device dev = h.device();
+  const int64_t V = weight.size(0), d = weight.size(1), N = h.numel() / d;
+  const Tensor hr = rows(h), tok = tokens.defined() ? tokens.contiguous() : tokens;
+  const std::vector<int64_t> sizes(h.sizes().begin(), h.sizes().end() - 1);
+  StatsOut o;
+  o.weight = rows(weight);
+  if (tok.defined()) o.logp = empty(sizes, at::kFloat, dev);
+  o.entropy = empty(sizes, at::kFloat, dev);
+  if (top) {
+    std::vector<int64_t> wide = sizes;
+    wide.push_back(top);
+    o.top_logp = empty(wide, at::kFloat, dev);
+    o.top_tokens = empty(wide, at::kLong, dev);
+  }
+  const size_t nb_saved = asrn_head_stats_saved_bytes(N, d), nb = asrn_head_stats_workspace_bytes(N, V, d, top, 0);
+  o.saved = scratch(nb_saved, dev);
+  const Tensor ws = scratch(nb, dev);
+  check(asrn_head_stats_forward(N, V, d, hr.data_ptr(), o.weight.data_ptr(), (const int64_t*)data_or_null(tok), (float)tau, top,
+                                (float*)data_or_null(o.logp), o.entropy.data_ptr<float>(), (float*)data_or_null(o.top_logp),
+                                (int64_t*)data_or_null(o.top_tokens), o.saved.data_ptr(), nb_saved, ws.data_ptr(), nb,
+                                status_word("head_stats", dev), stream_of(dev)),
+        "asrn_head_stats_forward");
+  return o;
+}
+
+// Outputs: entropy, then logp where tokens were given, then the two of the likeliest tokens where they are wanted.
+struct HeadStats : torch::autograd::Function<HeadStats> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& weight, const MaybeTensor& tokens,
+                               double tau, int64_t top) {
+    const StatsOut o = stats_forward(h, weight, or_none(tokens), tau, top);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({o.weight, o.saved});
+    ctx->saved_data["sizes"] = h.sizes().vec();
+    ctx->saved_data["tau"] = tau;
+    variable_list out{o.entropy};
+    if (o.logp.defined()) out.push_back(o.logp);
+    if (top) {
+      ctx->mark_non_differentiable({o.top_logp, o.top_tokens});
+      out.push_back(o.top_logp);
+      out.push_back(o.top_tokens);
+    }
+    ctx->saved_data["logp"] = o.logp.defined();
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const Tensor &w = kept[0], &saved = kept[1];
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const c10::Device dev = w.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const int64_t V = w.size(0), d = w.size(1);
+    int64_t N = 1;
+    for (size_t i = 0; i + 1 < sizes.size(); ++i) N *= sizes[i];
+    Tensor gh = grads[0], g;
+    if (ctx->saved_data["logp"].toBool()) g = grads[1];
+    if (gh.defined()) gh = f32(gh);
+    if (g.defined()) g = f32(g);
+    Tensor dh, dw;
+    if (ctx->needs_input_grad(0)) dh = empty(sizes, at::kBFloat16, dev);
+    if (ctx->needs_input_grad(1)) dw = empty({V, d}, at::kBFloat16, dev);
+    const size_t nb = asrn_head_stats_workspace_bytes(N, V, d, 0, 1);
+    const Tensor ws = scratch(nb, dev);
+    check(asrn_head_stats_backward(N, V, d, w.data_ptr(), saved.data_ptr(), saved.numel(),
+                                   (float)ctx->saved_data["tau"].toDouble(), (const float*)data_or_null(g),
+                                   (const float*)data_or_null(gh), data_or_null(dh), data_or_null(dw), ws.data_ptr(), nb,
+                                   status_word("head_stats", dev), stream_of(dev)),
+          "asrn_head_stats_backward");
+    variable_list out{dh, dw, Tensor(), Tensor(), Tensor()};
+    once("head_stats", out, grads);
+    return out;
+  }
+};
+
+std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> head_stats(Tensor h, Tensor weight, const MaybeTensor& tokens_or_none,
+                                                                     double tau, int64_t top) {
+  const Tensor tokens = or_none(tokens_or_none);
+  if (h.dim() < 1 || weight.dim() != 2 || h.size(-1) != weight.size(1) ||
+      (tokens.defined() && tokens.sizes() != h.sizes().slice(0, h.dim() - 1)))
+    throw py::value_error(text("head_stats: h (..., d), weight (V, d) and tokens (...) do not fit: ", h.sizes(), ", ",
+                               weight.sizes(), tokens.defined() ? text(", ", tokens.sizes()) : ""));
+  if (tokens.defined() && tokens.scalar_type() != at::kLong) throw py::type_error("head_stats: tokens are int64");
+  if (!(tau > 0 && tau <= 1e30)) throw py::value_error("head_stats: temperatura has to be positive");
+  if (top < 0 || top > 32 || top > weight.size(0))
+    throw py::value_error(text("head_stats: top is 0 to 32 and at most the vocabulary; got ", top));
+  const c10::Device dev = device_of("head_stats", {&h, &weight, &tokens});
+  c10::cuda::CUDAGuard guard(dev);
+  to_bf16("head_stats", {&h, &weight});
+  if (h.size(-1) % 8 || weight.numel() == 0)
+    not_implemented(text("head_stats: the width (", h.size(-1), ") has to be a multiple of 8, and the vocabulary not empty"));
+  MaybeTensor logp, top_logp, top_tokens;
+  if (!recorded({&h, &weight})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const StatsOut o = stats_forward(h, weight, tokens, tau, top);
+    if (o.logp.defined()) logp = o.logp;
+    if (top) {
+      top_logp = o.top_logp;
+      top_tokens = o.top_tokens;
+    }
+    return {logp, o.entropy, top_logp, top_tokens};
+  }
+  const variable_list out = HeadStats::apply(h, weight, tokens_or_none, tau, top);
+  if (tokens.defined()) logp = out[1];
+  if (top) {
+    top_logp = out[out.size() - 2];
+    top_tokens = out[out.size() - 1];
+  }
+  return {logp, out[0], top_logp, top_tokens};
+}
+
+// ---- layer norm -----------------------------------------------------------------------------------------------------------
+
+struct NormOut {
+  Tensor y, sum, read, weight, stats;          // read: x or the sum, what the backward pass reads; stats: where kept
+};
+
+NormOut norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, double eps,
+                     at::ScalarType type, bool keep) {
+  const c10::Device dev = x.device();
+  const int64_t d = weight.size(0), N = x.numel() / d;
+  const Tensor xr = rows(x), b = bias.defined() ? rows(bias) : bias, r = residual.defined() ? rows(residual) : residual;
+  NormOut o;
+  o.weight = rows(weight);
+  o.y = empty(x.sizes(), type, dev);
+  if (r.defined()) o.sum = empty(x.sizes(), r.scalar_type(), dev);
+  if (keep) o.stats = empty({N, 2}, at::kFloat, dev);
+  check(asrn_layer_norm(N, d, xr.data_ptr(), type_code(xr), data_or_null(r), r.defined() ? type_code(r) : 0,
+                        o.weight.data_ptr(), data_or_null(b), type_code(o.weight), (float)eps, data_or_null(o.sum),
+                        o.y.data_ptr(), type_code(o.y), (float*)data_or_null(o.stats), stream_of(dev)),
+        "asrn_layer_norm");
+  o.read = r.defined() ? o.sum : xr;
+  return o;
+}
+
+// Outputs: y, and the sum where there is a residual.
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias_or_none,
+                               const MaybeTensor& residual_or_none, double eps, int64_t type) {
+    const Tensor bias = or_none(bias_or_none), residual = or_none(residual_or_none);
+    const NormOut o = norm_forward(x, weight, bias, residual, eps, (at::ScalarType)type, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({o.read, o.weight, o.stats});
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->saved_data["types"] = (int64_t)x.scalar_type();
+    ctx->saved_data["y"] = type;
+    ctx->saved_data["bias"] = bias.defined();
+    if (!residual.defined()) return {o.y};
+    return {o.y, o.sum};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const Tensor &read = kept[0], &w = kept[1], &stats = kept[2];
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const at::ScalarType x_type = (at::ScalarType)ctx->saved_data["types"].toInt();
+    const c10::Device dev = read.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const int64_t d = w.size(0), N = stats.size(0);
+    const bool both = grads.size() > 1, biased = ctx->saved_data["bias"].toBool();   // inputs left out are not counted
+    const Tensor dy = grads[0].defined() ? rows(grads[0])
+                                         : at::zeros(sizes, at::TensorOptions()
+                                                                .dtype((at::ScalarType)ctx->saved_data["y"].toInt())
+                                                                .device(dev));
+    const Tensor ds = both && grads[1].defined() ? rows(grads[1]) : Tensor();
+    const bool need_x = ctx->needs_input_grad(0), need_r = both && ctx->needs_input_grad(2 + biased),
+               need_w = ctx->needs_input_grad(1), need_b = biased && ctx->needs_input_grad(2), same = read.scalar_type() == x_type;
+    Tensor out, other, dw, db;                 // the gradient in the type of what was normalised, and in x's
+    if (need_r || (need_x && same)) out = empty(sizes, read.scalar_type(), dev);
+    if (need_x && !same) other = empty(sizes, x_type, dev);
+    if (need_w) dw = empty({d}, w.scalar_type(), dev);
+    if (need_b) db = empty({d}, w.scalar_type(), dev);
+    const size_t nb = need_w || need_b ? asrn_layer_norm_workspace_bytes(N, d) : 0;
+    const Tensor ws = nb ? scratch(nb, dev) : Tensor();
+    check(asrn_layer_norm_backward(N, d, read.data_ptr(), type_code(read), stats.data_ptr<float>(), dy.data_ptr(), type_code(dy),
+                                   data_or_null(ds), w.data_ptr(), type_code(w), data_or_null(out), data_or_null(other),
+                                   data_or_null(dw), data_or_null(db), data_or_null(ws), nb, stream_of(dev)),
+          "asrn_layer_norm_backward");
+    variable_list made{need_x ? (same ? out : other) : Tensor(), dw, db, need_r ? out : Tensor(), Tensor(), Tensor()};
+    once("layer_norm", made, grads);
+    return made;
+  }
+};
+
+std::tuple<Tensor, MaybeTensor> layer_norm(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_or_none,
+                                           const MaybeTensor& residual_or_none, double eps, const py::object& dtype) {
+  const Tensor bias = or_none(bias_or_none), residual = or_none(residual_or_none);
+  if (x.dim() < 1 || weight.dim() != 1 || x.size(-1) != weight.size(0) || (bias.defined() && bias.sizes() != weight.sizes()) ||
+      (residual.defined() && residual.sizes() != x.sizes()))
+    throw py::value_error(text("layer_norm: x (..., d), weight (d), bias (d) and residual (..., d) do not fit: ", x.sizes(),
+                               ", ", weight.sizes(), bias.defined() ? text(", ", bias.sizes()) : "",
+                               residual.defined() ? text(", ", residual.sizes()) : ""));
+  if (!(eps >= 0 && eps < 1e30)) throw py::value_error("layer_norm: eps has to be 0 or more");
+  for (const Tensor* t : {&x, &weight, &bias, &residual})
+    if (t->defined() && !float_or_bf16(*t)) throw py::type_error("layer_norm takes float32 or bfloat16 tensors");
+  if (bias.defined() && bias.scalar_type() != weight.scalar_type())
+    throw py::type_error("layer_norm: weight and bias are of one type");
+  at::ScalarType type = x.scalar_type();
+  if (!dtype.is_none()) {
+    if (!THPDtype_Check(dtype.ptr())) throw py::type_error("layer_norm: dtype is torch.float32 or torch.bfloat16");
+    type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+    if (type != at::kFloat && type != at::kBFloat16) throw py::type_error("layer_norm: dtype is torch.float32 or torch.bfloat16");
+  }
+  const c10::Device dev = device_of("layer_norm", {&x, &weight, &bias, &residual});
+  c10::cuda::CUDAGuard guard(dev);
+  if (x.size(-1) == 0 || x.size(-1) > 16384)
+    not_implemented(text("layer_norm: rows of 1 to 16384 values; got ", x.size(-1)));
+  if (!recorded({&x, &weight, &bias, &residual})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const NormOut o = norm_forward(x, weight, bias, residual, eps, type, false);
+    return {o.y, maybe(o.sum)};
+  }
+  const variable_list out = LayerNorm::apply(x, weight, bias_or_none, residual_or_none, eps, (int64_t)type);
+  return {out[0], residual.defined() ? MaybeTensor(out[1]) : MaybeTensor()};
+}
+
+// ---- product with bias, activation and residual ----------------------------------------------------------------------------
+
+struct LinearOut {
+  Tensor y, x, weight, slope;
+};
+
+LinearOut linear_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, int64_t act,
+                         bool keep) {
+  const c10::Device dev = x.device();
+  const int64_t n = weight.size(0), d = weight.size(1), N = x.numel() / d;
+  LinearOut o;
+  o.x = rows(x);
+  o.weight = rows(weight);
+  const Tensor b = bias.defined() ? rows(bias) : bias, r = residual.defined() ? rows(residual) : residual;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = n;
+  o.y = empty(sizes, r.defined() ? r.scalar_type() : at::kBFloat16, dev);
+  if (keep && act) o.slope = empty({N, n}, at::kHalf, dev);
+  check(asrn_linear_forward(N, d, n, o.x.data_ptr(), o.weight.data_ptr(), data_or_null(b), act, data_or_null(r),
+                            r.defined() ? type_code(r) : 0, o.y.data_ptr(), data_or_null(o.slope), status_word("linear", dev),
+                            stream_of(dev)),
+        "asrn_linear_forward");
+  return o;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias,
+                        const MaybeTensor& residual, int64_t act) {
+    const LinearOut o = linear_forward(x, weight, or_none(bias), or_none(residual), act, true);
+    ctx->save_for_backward({o.x, o.weight, o.slope});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return o.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const Tensor &x = kept[0], &w = kept[1], &slope = kept[2];
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const c10::Device dev = x.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const int64_t n = w.size(0), d = w.size(1), N = x.numel() / d;
+    const bool biased = ctx->saved_data["bias"].toBool();  // inputs left out are not counted
+    Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) dx = empty(x.sizes(), at::kBFloat16, dev);
+    if (ctx->needs_input_grad(1)) dw = empty({n, d}, at::kBFloat16, dev);
+    if (biased && ctx->needs_input_grad(2)) db = empty({n}, at::kBFloat16, dev);
+    if (dx.defined() || dw.defined() || db.defined()) {
+      const Tensor dy = rows(grads[0]);
+      const size_t nb = asrn_linear_workspace_bytes(N, d, n, act, type_code(dy));
+      const Tensor ws = scratch(nb, dev);
+      check(asrn_linear_backward(N, d, n, dy.data_ptr(), type_code(dy), x.data_ptr(), w.data_ptr(), act, data_or_null(slope),
+                                 data_or_null(dx), data_or_null(dw), data_or_null(db), ws.data_ptr(), nb,
+                                 status_word("linear", dev), stream_of(dev)),
+            "asrn_linear_backward");
+    }
+    variable_list out{dx, dw, db, Tensor(), Tensor()};
+    once("linear", out, grads);
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2 + biased)) out[3] = grads[0];       // the residual's gradient is the result's
+    return out;
+  }
+};
+
+Tensor linear(Tensor x, Tensor weight, const MaybeTensor& bias_or_none, int64_t act, const MaybeTensor& residual_or_none) {
+  Tensor bias = or_none(bias_or_none);
+  const Tensor residual = or_none(residual_or_none);
+  bool fits = x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) &&
+              (!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0)));
+  if (fits && residual.defined())
+    fits = residual.dim() == x.dim() && residual.size(-1) == weight.size(0) &&
+           residual.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+  if (!fits)
+    throw py::value_error(text("linear: x (..., d), weight (n, d), bias (n) and residual (..., n) do not fit: ", x.sizes(), ", ",
+                               weight.sizes(), bias.defined() ? text(", ", bias.sizes()) : "",
+                               residual.defined() ? text(", ", residual.sizes()) : ""));
+  if (residual.defined() && !float_or_bf16(residual))
+    throw py::type_error("linear: the residual is float32 or bfloat16");
+  const c10::Device dev = device_of("linear", {&x, &weight, &bias, &residual});
+  c10::cuda::CUDAGuard guard(dev);
+  if (weight.size(0) % 8 || weight.size(1) % 8 || !weight.numel())
+    not_implemented(text("linear: the widths (", weight.size(1), ", ", weight.size(0), ") have to be multiples of 8"));
+  if (bias.defined())
+    to_bf16("linear", {&x, &weight, &bias});
+  else
+    to_bf16("linear", {&x, &weight});
+  if (!recorded({&x, &weight, &bias, &residual})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_forward(x, weight, bias, residual, act, false).y;
+  }
+  return Linear::apply(x, weight, maybe(bias), residual_or_none, act);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -396,6 +725,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack8", torch::wrap_pybind_function(&pack8));
   m.def("unpack8", torch::wrap_pybind_function(&unpack8));
   m.def("mlp8", torch::wrap_pybind_function(&mlp8));
+  m.def("head_stats", torch::wrap_pybind_function(&head_stats));
+  m.def("layer_norm", torch::wrap_pybind_function(&layer_norm));
+  m.def("linear", torch::wrap_pybind_function(&linear));
   m.def("status", torch::wrap_pybind_function(&status));
   m.def("status_address", torch::wrap_pybind_function(&status_address));
 }

@@ -279,6 +279,12 @@ template <int Pieces> struct Out {
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
   }
+  // The warp's pieces, side by side, once no copy reads them any more.
+  ASRN_DEV uint8_t* room() {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    return piece;
+  }
   ASRN_DEV void drain() {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -598,11 +604,16 @@ inline bool bind_context() {
   return bound;
 }
 
-// Where an epilogue's bf16 rows go: (rows, columns) of `pitch` elements.
+// Where an epilogue's rows go: (rows, columns) of `pitch` elements of 16 bits, 32 columns a piece, or of fp32, 16 columns.
 struct Dest {
   void* base;
   int64_t rows, columns, pitch;
+  bool f32;
 };
+inline bool dest_map(CUtensorMap* map, const Dest& o) {
+  return o.f32 ? make_tmap_f32_sw64(map, o.base, (uint64_t)o.columns, (uint64_t)o.rows, (uint64_t)o.pitch * 4, 16, 32)
+               : make_tmap_bf16_sw64(map, o.base, (uint64_t)o.columns, (uint64_t)o.rows, (uint64_t)o.pitch * 2, 32, 32);
+}
 
 template <int CG, bool AMn, bool BMn, class Epi>
 int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, const Shape& s,
@@ -614,9 +625,7 @@ int launch_cg(const void* A, int64_t pitch_a, const void* B, int64_t pitch_b, co
       !operand_map(&mb, B, BMn, BMn ? s.N : s.N + again * s.b_step, BMn ? s.K + again * s.b_step : s.K, pitch_b, kBN / CG))
     return ASRN_ERR_CUDA;
   mo = mq = ma;                                            // not read where there is no destination
-  if ((o.base && !make_tmap_bf16_sw64(&mo, o.base, (uint64_t)o.columns, (uint64_t)o.rows, (uint64_t)o.pitch * 2, 32, 32)) ||
-      (q.base && !make_tmap_bf16_sw64(&mq, q.base, (uint64_t)q.columns, (uint64_t)q.rows, (uint64_t)q.pitch * 2, 32, 32)))
-    return ASRN_ERR_CUDA;
+  if ((o.base && !dest_map(&mo, o)) || (q.base && !dest_map(&mq, q))) return ASRN_ERR_CUDA;
   auto kernel = k_gemm<CG, AMn, BMn, Epi>;
   constexpr size_t smem = smem_bytes<CG, Epi>();
   static std::atomic<uint64_t> ready{0};                  // devices that know the kernel's shared memory

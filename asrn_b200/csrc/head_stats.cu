@@ -1,0 +1,592 @@
+// Log probabilities through the tied head with the distribution's entropy and its likeliest tokens, forward and backward:
+//   s_iv = h_i . w_v / tau,  lse = log sum_v exp s_v,  logp = s_y - lse,  H = lse - sum_v p_v s_v,  the `top` largest s_v - lse
+//   dS_v = (1 / tau) [g (delta_{v,y} - p_v) - gH p_v (log p_v + H)],  dh = dS W,  dW = dS^T h
+// The products are those of the log probabilities alone (head.cu): 2 N V d operations forward and 6 N V d backward, bound by the
+// tensor cores at any training size, and by the weight's bytes where rows are few.
+//
+//   k_gemm<Scan>   scores by tiles; each thread keeps of its row's 128 columns the maximum m, S = sum exp(s - m), T = sum
+//                  exp(s - m) (s - m), and where the likeliest tokens are wanted the two largest scores, the largest with its
+//                  column in the low 7 bits; the target is in none of the sums
+//   k_stats_join   a row's sums joined: logp, H
+//   k_stats_top    a warp per row: the groups of 128 columns by their largest scores, for as long as one may hold one of the
+//                  likeliest tokens; what it may be is scored again from h and W with a sum in 64 bits. So the order of
+//                  the tokens is that of their exact scores, whatever the products' fp32 sums rounded; equal scores are
+//                  in the order of their numbers.
+//   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
+#include "head.cuh"
+
+namespace asrn {
+
+namespace {
+
+using gemm::exp2_fast;
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kNothing = -3.3e38f;       // of columns that do not count: its exponential is 0, and its bits can be marked
+constexpr float kLeast = -200.f;           // log2 of what is as good as 0: keeps 0 x infinity out of the sums of p log p
+constexpr int kMaxTop = 32;
+
+struct StatsSaved {                        // HeadSaved with logp in the place of `rest`, and
+  HeadSaved head;
+  size_t ent, total;
+};
+
+StatsSaved stats_saved(int64_t N, int64_t d) {
+  StatsSaved w{};
+  w.head = head_saved(N, d);
+  w.ent = w.head.total;
+  w.total = align_up(w.ent + (size_t)pad256(N) * 4);
+  return w;
+}
+
+int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
+
+struct StatsWs {
+  size_t counts, top, part, ent, base, pairs, total;
+};
+
+StatsWs stats_ws(int64_t N, int64_t V, int top) {
+  StatsWs w{};
+  const size_t P = (size_t)pad256(N), halves = (size_t)halves_of(V);
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
+  w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
+  w.top = take(P * 4);
+  w.part = take(halves * P * 8);
+  w.ent = take(halves * P * 4);
+  w.base = take(top ? P * 8 : 0);
+  w.pairs = take(top ? halves * P * 8 : 0);
+  w.total = o;
+  return w;
+}
+
+template <bool Top> struct Scan {
+  static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
+  struct Params {
+    const int* tok;
+    float k;                               // log2(e) / tau
+    float* top;                            // the targets' unscaled scores
+    float2* part;                          // m, S: [2 n-tiles][pad]
+    float* ent;                            // T log2(e): the same
+    float2* pairs;                         // the two largest: [pad][2 n-tiles]
+    int64_t pad;
+  };
+  const Params& p;
+  int row, V, y, at, halves;
+  bool on;
+  float m = -INFINITY, s = 0.f, t = 0.f, first = kNothing, second = kNothing;
+  ASRN_DEV Scan(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile& u, int half)
+      : p(pp), row(r), V(sh.N), y(-1), at(u.n * 2 + half), halves((sh.N + gemm::kBN - 1) / gemm::kBN * 2), on(r < rows) {
+    if (on) y = p.tok[r];
+  }
+  template <class O> ASRN_DEV void chunk(float* v, int c, O&, const CUtensorMap*, const CUtensorMap*) {
+    if (c >= V) return;
+    const int n = V - c, j = y - c;        // n: valid columns, 32 or more but in the last tile
+    if (j >= 0 && j < 32) {
+      float own = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        own = i == j ? v[i] : own;
+        v[i] = i == j ? kNothing : v[i];
+      }
+      p.top[row] = own;
+    }
+    if (n < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = i < n ? v[i] : kNothing;
+    }
+    float now = m;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) now = fmaxf(now, v[i]);
+    const float off = now <= kNothing ? 0.f : now * p.k;
+    const gemm::F2 k2(p.k), off2(-off);
+    gemm::F2 add(0.f), sum(0.f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float a, b;
+      gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2).get(a, b);
+      const gemm::F2 e(exp2_fast(a), exp2_fast(b));
+      add = gemm::add2(add, e);
+      sum = gemm::fma2(e, gemm::F2(fmaxf(a, kLeast), fmaxf(b, kLeast)), sum);
+    }
+    float a, b;
+    const float step = fmaxf(fmaf(m, p.k, -off), kLeast), f = exp2_fast(fmaf(m, p.k, -off));
+    sum.get(a, b);
+    t = fmaf(f, fmaf(step, s, t), a + b);
+    add.get(a, b);
+    s = fmaf(s, f, a + b);
+    m = now;
+    if constexpr (Top) {                   // two chains, then one; i and the chunk's place in the half in the low bits
+      float m1[2] = {kNothing, kNothing}, m2[2] = {kNothing, kNothing};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float u = __uint_as_float((__float_as_uint(v[i]) & ~127u) | (uint32_t)i);
+        m2[i & 1] = fmaxf(m2[i & 1], fminf(m1[i & 1], u));
+        m1[i & 1] = fmaxf(m1[i & 1], u);
+      }
+      const float lo = fminf(m1[0], m1[1]);
+      const float hi = __uint_as_float(__float_as_uint(fmaxf(m1[0], m1[1])) | (uint32_t)(c & 96));
+      second = fmaxf(fmaxf(second, fminf(first, hi)), fmaxf(lo, fmaxf(m2[0], m2[1])));
+      first = fmaxf(first, hi);
+    }
+  }
+  ASRN_DEV void finish() {
+    if (!on) return;
+    p.part[at * p.pad + row] = make_float2(m <= kNothing ? -INFINITY : m, s);
+    p.ent[at * p.pad + row] = t;
+    if (Top) p.pairs[(int64_t)row * halves + at] = make_float2(first, second);
+  }
+};
+
+// Block = 32 positions x 16 warps over the halves of the vocabulary's tiles, 8 at a time. A position's void when its target is
+// outside the vocabulary or its scores have no log-sum-exp (an infinity or a NaN among them): NaN in all its results.
+constexpr int kJoinWarps = 16;
+__global__ void __launch_bounds__(kJoinWarps * 32)
+k_stats_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const int* __restrict__ pos,
+             const int* __restrict__ tok, const float* __restrict__ top, const float2* __restrict__ part,
+             const float* __restrict__ ent, float* __restrict__ lse2, float* __restrict__ kept_logp,
+             float* __restrict__ kept_ent, double* __restrict__ base, float* __restrict__ logp, float* __restrict__ entropy) {
+  __shared__ float sh[3][kJoinWarps][32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const int r = i < N ? pos[i] : -1;
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  auto join = [&](const float* qm, const float* qs, const float* qt, int n) {   // n of at most 8
+    float now = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now = j < n ? fmaxf(now, qm[j]) : now;
+    if (now == -INFINITY) {                      // no score yet but NaNs, which the maxima pass over: the sums hold them
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) s += qs[j];
+      return;
+    }
+    float step = fmaxf((m - now) * k, kLeast), f = exp2_fast((m - now) * k);
+    t = f * fmaf(step, s, t);
+    s *= f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) {
+        step = fmaxf((qm[j] - now) * k, kLeast);
+        f = exp2_fast((qm[j] - now) * k);
+        t = fmaf(f, fmaf(step, qs[j], qt[j]), t);
+        s = fmaf(qs[j], f, s);
+      }
+    m = now;
+  };
+  if (r >= 0)
+    for (int j0 = wid; j0 < halves; j0 += 8 * kJoinWarps) {
+      float qm[8], qs[8], qt[8];
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j * kJoinWarps < halves) {
+          const int64_t at = (j0 + j * kJoinWarps) * pad + r;
+          const float2 q = __ldg(part + at);
+          qm[j] = q.x;
+          qs[j] = q.y;
+          qt[j] = __ldg(ent + at);
+          n = j + 1;
+        }
+      join(qm, qs, qt, n);
+    }
+  sh[0][wid][lane] = m;
+  sh[1][wid][lane] = s;
+  sh[2][wid][lane] = t;
+  __syncthreads();
+  if (wid || i >= N) return;
+  m = -INFINITY;
+  s = t = 0.f;
+  for (int w = 0; w < kJoinWarps; w += 8) {
+    float qm[8], qs[8], qt[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      qm[j] = sh[0][w + j][lane];
+      qs[j] = sh[1][w + j][lane];
+      qt[j] = sh[2][w + j][lane];
+    }
+    join(qm, qs, qt, 8);
+  }
+  if (r < 0) {
+    if (logp) logp[i] = 0.f;
+    entropy[i] = 0.f;
+    return;
+  }
+  t *= kLn2;                                     // the sums so far: without the target
+  const int y = tok[r];
+  float lp = 0.f, H, l2, off;                    // lse = from / tau + off
+  float from = m;
+  if (y < 0) {
+    off = logf(s);
+    H = off - t / s;
+    l2 = m * k + log2f(s);
+  } else {
+    const float own = top[r], x = (own - m) * inv_tau;
+    if (s == 0.f) {
+      lp = H = own * 0.f;
+      off = 0.f;
+      from = own;
+      l2 = own * k;
+    } else if (x > 0.f) {
+      const float f = expf(-x), a = s * f;
+      lp = -log1pf(a);
+      H = -lp - f * (t - fminf(x, -kLeast) * s) / (1.f + a);
+      off = -lp;
+      from = own;
+      l2 = own * k - lp * kLog2e;
+    } else {
+      const float e = expf(x), all = s + e;
+      off = logf(all);
+      lp = x - off;
+      H = off - (t + e * fmaxf(x, kLeast)) / all;
+      l2 = m * k + log2f(all);
+    }
+  }
+  if (y == -1 || !(fabsf(l2) < INFINITY)) lp = H = l2 = NAN;
+  H = H < 0.f ? 0.f : H;                         // what the rounding of two equal terms leaves
+  if (logp) logp[i] = lp;
+  entropy[i] = H;
+  lse2[r] = l2;
+  kept_logp[r] = lp;
+  kept_ent[r] = H;
+  if (base) base[r] = (double)from * inv_tau + off;
+}
+
+// A score as a number that orders as it does; 0: none.
+ASRN_DEV uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v) & ~127u;
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// h . w for n of up to four rows of W, products of bf16 exact in fp32, summed in 64 bits; size: the largest sum of their magnitudes.
+ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, int n, double* out, float& size) {
+  const int lane = threadIdx.x & 31;
+  double acc[4] = {};
+  float mag[4] = {};
+  for (int c = lane; c < vecs; c += 32) {
+    const uint4 a = __ldg(h + c);
+    uint4 b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = __ldg(W + (int64_t)token[j < n ? j : 0] * vecs + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t y[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = __uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16);
+        const float hi = __uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u);
+        acc[j] += (double)lo;
+        acc[j] += (double)hi;
+        mag[j] += fabsf(lo) + fabsf(hi);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    out[j] = warp_sum_d(acc[j]);
+    if (j < n) size = fmaxf(size, warp_sum(mag[j]));
+  }
+}
+
+// The best so far, lane l the l-th, larger scores first, then smaller numbers.
+struct Best {
+  double score = -INFINITY;
+  int token = 0x7fffffff;
+  ASRN_DEV void put(double s, int t) {           // minus infinity is not put in
+    if (s == -INFINITY) return;
+    const int lane = threadIdx.x & 31;
+    const unsigned behind = __ballot_sync(0xffffffffu, s > score || (s == score && t < token));
+    const double up = __shfl_up_sync(0xffffffffu, score, 1);
+    const int ut = __shfl_up_sync(0xffffffffu, token, 1);
+    if (!behind) return;
+    const int at = __ffs(behind) - 1;
+    if (lane > at) {
+      score = up;
+      token = ut;
+    } else if (lane == at) {
+      score = s;
+      token = t;
+    }
+  }
+};
+
+constexpr int kTopWarps = 4;
+__global__ void __launch_bounds__(kTopWarps * 32)
+k_stats_top(int64_t N, int V, int d, int top, int halves, float inv_tau, const uint4* __restrict__ hc,
+            const uint4* __restrict__ W, const int* __restrict__ pos, const int* __restrict__ tok,
+            const float* __restrict__ lse2, const double* __restrict__ base, const float2* __restrict__ pairs,
+            float* __restrict__ top_logp, int64_t* __restrict__ top_tokens) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = (int64_t)blockIdx.x * kTopWarps + (threadIdx.x >> 5);
+  if (i >= N) return;
+  const int r = pos[i];
+  const bool bad = r >= 0 && !(fabsf(lse2[r]) < INFINITY);
+  if (r < 0 || bad) {
+    if (lane < top) {
+      top_logp[i * top + lane] = bad ? NAN : 0.f;
+      top_tokens[i * top + lane] = -1;
+    }
+    return;
+  }
+  const int vecs = d / 8, y = tok[r];
+  const uint4* h = hc + (int64_t)r * vecs;
+  const float2* mine = pairs + (int64_t)r * halves;
+  Best best;
+  float size = 0.f;                              // the largest sum of |h w| seen
+  double s[4];
+  if (y >= 0) {
+    const int t[4] = {y};
+    dots(h, W, vecs, t, 1, s, size);
+    best.put(s[0], y);
+  }
+  // The groups in the order of their largest scores, equal ones by their numbers: each lane holds the next of its own, those
+  // after `last`.
+  uint32_t key = 0xffffffffu, last = 0xffffffffu;
+  int group = -1, last_group = -1;
+  auto find = [&]() {
+    key = 0;
+    group = 0x7fffffff;
+#pragma unroll 4
+    for (int g = lane; g < halves; g += 32) {
+      const float v = __ldg(&mine[g].x);
+      const uint32_t o = v <= -3e38f ? 0u : order_of(v);
+      if ((o < last || (o == last && g > last_group)) && o > key) {
+        key = o;
+        group = g;
+      }
+    }
+  };
+  auto next = [&](float2& pair) {                // the next group, -1: none left
+    const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+    if (most == 0) return -1;
+    const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
+    last = most;
+    last_group = g;
+    if (group == g && key == most) find();
+    __syncwarp();
+    pair = __ldg(mine + g);
+    return g;
+  };
+  auto column = [&](int g, float v) { return g * 128 + (int)(__float_as_uint(v) & 127u); };
+  // All columns of a group but one and the target's.
+  auto expand = [&](int g, int except) {
+    const int end = min(V, g * 128 + 128);
+    for (int c = g * 128; c < end; c += 4) {
+      const int n = min(4, end - c);
+      const int t[4] = {c, c + 1, c + 2, c + 3};
+      dots(h, W, vecs, t, n, s, size);
+      for (int j = 0; j < n; ++j)
+        if (t[j] != except && t[j] != y) best.put(s[j], t[j]);
+    }
+  };
+  // How far a largest score may lie above what is noted: its low bits, and the products' rounding (twice what the sums in fp32,
+  // 16 products at a time, may be off by, with twice the magnitudes seen).
+  auto above = [&](float v) { return (double)v + fabsf(v) * 0x1p-15f + (float)(d / 16 + 2) * 0x1p-21f * size; };
+  auto worst = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
+
+  find();
+  // The first `top` groups' largest, four at a time; their pairs by lane.
+  float2 pair, held = make_float2(kNothing, kNothing);
+  int held_group = -1, held_column = -1, have = 0;
+  bool more = true;
+  while (have < top && more) {
+    int t[4] = {}, n = 0;
+    while (n < 4 && have < top) {
+      const int g = next(pair);
+      if (g < 0) {
+        more = false;
+        break;
+      }
+      t[n] = column(g, pair.x);
+      if (lane == have) {
+        held = pair;
+        held_group = g;
+        held_column = t[n];
+      }
+      ++n;
+      ++have;
+    }
+    if (n) dots(h, W, vecs, t, n, s, size);
+    for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
+  }
+  // Their second ones, where they may count.
+  for (int q = 0; q < have; ++q) {
+    const float v = __shfl_sync(0xffffffffu, held.y, q);
+    const int g = __shfl_sync(0xffffffffu, held_group, q), c = __shfl_sync(0xffffffffu, held_column, q);
+    if (v > -3e38f && above(v) >= worst()) expand(g, c);
+  }
+  // And the groups after them.
+  while (more) {
+    const int g = next(pair);
+    if (g < 0 || above(pair.x) < worst()) break;
+    const int t[4] = {column(g, pair.x)};
+    dots(h, W, vecs, t, 1, s, size);
+    best.put(s[0], t[0]);
+    if (pair.y > -3e38f && above(pair.y) >= worst()) expand(g, t[0]);
+  }
+  // Scores of minus infinity are in no group: the smallest numbers that are left.
+  const int found = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < V));
+  for (int c = 0, l = found; l < top && c < V; ++c) {
+    if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
+    if (lane == l) best.token = c;
+    ++l;
+  }
+  if (lane < top) {
+    top_logp[i * top + lane] = (float)(best.score * inv_tau - base[r]);
+    top_tokens[i * top + lane] = best.token;
+  }
+}
+
+// dS of one chunk in bf16; the rows that pad the last tile get zeros. With x = log2 p: dS = p (a + b x).
+struct Slope {
+  static constexpr int kWarps = 8, kOwn = 2, kTable = 0;
+  struct Params {
+    const int *tok, *row;                  // of the chunk's rows
+    const float *lse2, *logp, *ent;
+    const float *g, *gh;                   // by position; either may be null
+    float k, inv_tau;
+    int below;                             // rows from dS to its remainder, 0: none
+  };
+  const Params& p;
+  int V, y, first;
+  bool on;
+  float off, a, b, own;                    // own: the target's dS
+  ASRN_DEV Slope(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile&, int)
+      : p(pp), V(sh.N), y(-1), first(r & ~31), on(r < rows), off(0.f), a(0.f), b(0.f), own(0.f) {
+    if (!on) return;
+    y = p.tok[r];
+    off = p.lse2[r];
+    const int at = p.row[r];
+    const float g = p.g && y >= 0 ? p.g[at] * p.inv_tau : 0.f, gh = p.gh ? p.gh[at] * p.inv_tau : 0.f;
+    const float H = p.ent[r], lp = p.logp[r];
+    a = -g - gh * H;
+    b = -gh * kLn2;
+    const float slow = lp < kLeast * kLn2 ? 0.f : expf(lp) * (lp + H);    // p (log p + H)
+    own = -g * expm1f(lp) - gh * slow;
+    if (y == -1) a = NAN;
+  }
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap*) {
+    if (c >= V) return;
+    const gemm::F2 k2(p.k), off2(-off), a2(a), b2(b);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float x0, x1;
+      gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2).get(x0, x1);
+      const gemm::F2 e(exp2_fast(x0), exp2_fast(x1));
+      gemm::mul2(e, gemm::fma2(b2, gemm::F2(fmaxf(x0, kLeast), fmaxf(x1, kLeast)), a2)).get(v[i], v[i + 1]);
+    }
+    const int j = y - c;
+    if (j >= 0 && j < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = i == j ? own : v[i];
+    }
+    if (!on) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    }
+    out.put(map_o, v, c, first);
+    if (p.below) {
+      gemm::remainder(v);
+      out.put(map_o, v, c, first + p.below);
+    }
+  }
+  ASRN_DEV void finish() {}
+};
+
+}  // namespace
+
+}  // namespace asrn
+
+extern "C" {
+
+size_t asrn_head_stats_saved_bytes(int64_t N, int32_t d) {
+  if (asrn::check_head(N, 1, d)) return 0;
+  return asrn::stats_saved(N, d).total;
+}
+
+size_t asrn_head_stats_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t top, int32_t backward) {
+  if (asrn::check_head(N, V, d)) return 0;
+  return backward ? asrn::head_backward_ws(N, V, d).total : asrn::stats_ws(N, V, top).total;
+}
+
+int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, const void* weight, const int64_t* tokens,
+                            float tau, int32_t top, float* logp, float* entropy, float* top_logp, int64_t* top_tokens,
+                            void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes, int* status,
+                            void* stream) {
+  using namespace asrn;
+  int st = check_head(N, V, d);
+  if (st) return st;
+  if (!(tau > 0.f) || tau > 1e30f || top < 0 || top > V) return ASRN_ERR_ARG;
+  if (top > kMaxTop) return ASRN_ERR_UNSUPPORTED;
+  if (N == 0) return ASRN_OK;
+  if (!h || !weight || !entropy || (tokens && !logp) || (top && (!top_logp || !top_tokens)) || (uintptr_t)h % 16 ||
+      (uintptr_t)weight % 16)
+    return ASRN_ERR_ARG;
+  const StatsSaved sv = stats_saved(N, d);
+  const StatsWs ws = stats_ws(N, V, top);
+  if (!saved || saved_bytes < sv.total || (uintptr_t)saved % 256 || !workspace || workspace_bytes < ws.total ||
+      (uintptr_t)workspace % 256)
+    return ASRN_ERR_WORKSPACE;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* S = reinterpret_cast<char*>(saved);
+  char* W = reinterpret_cast<char*>(workspace);
+  if ((st = head_gather(N, V, d, h, tokens, reinterpret_cast<int*>(W + ws.counts), S, sv.head, s))) return st;
+  const int *tok = reinterpret_cast<int*>(S + sv.head.tok), *pos = reinterpret_cast<int*>(S + sv.head.pos);
+  const void* hc = S + sv.head.hc;
+  float* lse2 = reinterpret_cast<float*>(S + sv.head.lse2);
+  double* base = top ? reinterpret_cast<double*>(W + ws.base) : nullptr;
+  const int halves = halves_of(V);
+  gemm::Shape sh{};
+  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = reinterpret_cast<int*>(S + sv.head.count); sh.group = 16;
+  sh.status = status;
+  const float inv_tau = 1.f / tau, k = kLog2e * inv_tau;
+  float* own = reinterpret_cast<float*>(W + ws.top);
+  float2* part = reinterpret_cast<float2*>(W + ws.part);
+  float* ent = reinterpret_cast<float*>(W + ws.ent);
+  float2* pairs = reinterpret_cast<float2*>(W + ws.pairs);
+  if (top)
+    st = gemm::launch<false, false, Scan<true>>(hc, d, weight, d, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
+  else
+    st = gemm::launch<false, false, Scan<false>>(hc, d, weight, d, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
+  if (st) return st;
+  k_stats_join<<<(unsigned)((N + 31) / 32), kJoinWarps * 32, 0, s>>>(
+      N, halves, pad256(N), k, inv_tau, pos, tok, own, part, ent, lse2, reinterpret_cast<float*>(S + sv.head.rest),
+      reinterpret_cast<float*>(S + sv.ent), base, logp, entropy);
+  if (top)
+    k_stats_top<<<(unsigned)((N + kTopWarps - 1) / kTopWarps), kTopWarps * 32, 0, s>>>(
+        N, (int)V, d, top, halves, inv_tau, reinterpret_cast<const uint4*>(hc), reinterpret_cast<const uint4*>(weight), pos,
+        tok, lse2, base, pairs, top_logp, top_tokens);
+  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
+int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
+                             float tau, const float* g, const float* g_entropy, void* dh, void* dw, void* workspace,
+                             size_t workspace_bytes, int* status, void* stream) {
+  using namespace asrn;
+  int st = check_head(N, V, d);
+  if (st) return st;
+  if (!(tau > 0.f) || tau > 1e30f) return ASRN_ERR_ARG;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (N == 0) {
+    if (dw && cudaMemsetAsync(dw, 0, (size_t)V * d * 2, s) != cudaSuccess) return ASRN_ERR_CUDA;
+    return ASRN_OK;
+  }
+  if (!weight || (uintptr_t)weight % 16 || (uintptr_t)dh % 16 || (uintptr_t)dw % 16) return ASRN_ERR_ARG;
+  const StatsSaved sv = stats_saved(N, d);
+  const HeadBackwardWs ws = head_backward_ws(N, V, d);
+  if (!saved || saved_bytes < sv.total || (uintptr_t)saved % 256 || !workspace || workspace_bytes < ws.total ||
+      (uintptr_t)workspace % 256)
+    return ASRN_ERR_WORKSPACE;
+  const char* S = reinterpret_cast<const char*>(saved);
+  auto floats = [&](size_t at, int64_t first) { return reinterpret_cast<const float*>(S + at) + first; };
+  auto ints = [&](size_t at, int64_t first) { return reinterpret_cast<const int*>(S + at) + first; };
+  return head_backward<Slope>(N, V, d, weight, S, sv.head, ws, reinterpret_cast<char*>(workspace), dh, dw, status, s,
+                              [&](int64_t first, int below) {
+                                return Slope::Params{ints(sv.head.tok, first), ints(sv.head.row, first),
+                                                     floats(sv.head.lse2, first), floats(sv.head.rest, first),
+                                                     floats(sv.ent, first), g, g_entropy, kLog2e / tau, 1.f / tau, below};
+                              });
+}
+
+}  // extern "C"

@@ -265,6 +265,9 @@ bool make_tmap_f32(void* map /* CUtensorMap */, const void* base, uint64_t inner
 // The same with the 128-byte shared-memory swizzle (box_inner = 32 fp32).
 bool make_tmap_f32_sw128(void* map /* CUtensorMap */, const void* base, uint64_t inner, uint64_t outer,
                          uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
+// The same with the 64-byte one (box_inner = 16 fp32).
+bool make_tmap_f32_sw64(void* map /* CUtensorMap */, const void* base, uint64_t inner, uint64_t outer,
+                        uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
 // 3-D maps over row-major (d2, d1, d0) tensors (innermost d0), boxes box0 x box1 x 1, 128-byte swizzle; a box reaching
 // outside [0, d1) of its sequence reads zeros there.
 bool make_tmap_bf16_3d(void* map /* CUtensorMap */, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,

@@ -1,0 +1,464 @@
+// The matrix product with bias, activation and residual in its epilogue, forward and backward:
+//   a = x W^T + b,  y = act(a) + r;  kept: act'(a) in fp16
+//   dA = dY act'(a),  dX = dA W,  dW = dA^T x,  db = sum of dA,  dr = dY
+// x, W, b bf16; r bf16 or fp32, y of r's type (bf16 without); act: none, gelu (erf), silu, relu.
+//
+// act'(a) is kept rather than a: it lies in [-0.13, 1.13], where fp16 is off by 2^-11 of it at the most, an eighth of what dA's
+// rounding to bf16 takes (a in bf16 would move act'(a) by as much as that), and the backward pass has nothing left to compute. dA is rounded once, as
+// operand of both products; up to kTwiceRows rows they take what the rounding took, too.
+//
+//   k_linear_few   up to kFewRows rows: memory bound (the weight is read once, 2 operations a byte and row), so the rows of W are
+//                  spread over all SMs, sixteen a block, K over its warps; mma.sync, whose 16 x 8 tiles fit such rows
+//   k_gemm<Fused>  more rows: tcgen05 products, the rest in the epilogue
+//   k_linear_slope backward: dA in bf16 and its columns' sums by 64 rows
+//   k_gemm x 2     dX, dW (dW in shares of the rows where its tiles are few)
+//   k_colsum       db
+#include <cuda_fp16.h>
+#include "common.cuh"
+#include "gemm_tc.cuh"
+#include "products.cuh"
+
+namespace asrn {
+
+namespace {
+
+constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
+constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
+constexpr int64_t kTwiceRows = 512;
+constexpr int64_t kFewRows = 64;
+
+ASRN_DEV uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Of two values: act(a) in place, the slopes as fp16. Infinite a give the limits (products with what vanishes take |a| held
+// to 200), NaN stays.
+template <int Act> ASRN_DEV uint32_t activate(float& a0, float& a1) {
+  using namespace gemm;
+  if constexpr (Act == kGelu) {
+    F2 e, q;
+    tails(a0, a1, e, q);
+    const float m0 = fminf(fabsf(a0), 200.f), m1 = fminf(fabsf(a1), 200.f);
+    float h0, h1, s0, s1;
+    fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                                     // 1/2 - q
+    const F2 cdf = add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
+    fma2(mul2(F2(copysignf(m0, a0), copysignf(m1, a1)), F2(0.39894228040143268f)), e, cdf).get(s0, s1);
+    fma2(F2(-m0, -m1), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(a0, a1);
+    return half2_of(s0, s1);
+  } else if constexpr (Act == kSilu) {
+    float* a[2] = {&a0, &a1};
+    float s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float low = fmaxf(*a[i], -200.f);
+      float p = 1.f + exp2_fast(*a[i] * -1.4426950408889634f);
+      asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(p));
+      s[i] = p * fmaf(fminf(low, 200.f), 1.f - p, 1.f);
+      *a[i] = low * p;
+    }
+    return half2_of(s[0], s[1]);
+  } else {
+    const uint32_t s = half2_of(a0 > 0.f ? 1.f : 0.f, a1 > 0.f ? 1.f : 0.f);
+    a0 = a0 < 0.f ? 0.f : a0;
+    a1 = a1 < 0.f ? 0.f : a1;
+    return s;
+  }
+}
+// The same for 2 n values.
+template <int N> ASRN_DEV void activate(int act, float* v, uint32_t* s) {
+  if (act == kGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = activate<kGelu>(v[2 * i], v[2 * i + 1]);
+  } else if (act == kSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = activate<kSilu>(v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = activate<kRelu>(v[2 * i], v[2 * i + 1]);
+  }
+}
+
+// What follows the product.
+struct Rest {
+  const __nv_bfloat16* bias;                 // or null
+  const void* res;
+  int act, res_type;
+  int keep;                                  // the slopes are wanted
+};
+
+struct Fused {
+  static constexpr int kWarps = 16, kOwn = 2, kTable = 0;
+  using Params = Rest;
+  const Params& p;
+  int N, first, rows;
+  ASRN_DEV Fused(const Params& pp, int r, int m, const gemm::Shape& s, const gemm::Tile&, int)
+      : p(pp), N(s.N), first(r & ~31), rows(m) {}
+
+  // v += the residual's 32 x 32 values, brought through the warp's pieces: whole rows of them are read side by side, where each
+  // lane's own row would touch 32 half-used sectors at a time.
+  template <class O> ASRN_DEV void add_residual(float* v, int c, O& out) {
+    const int lane = threadIdx.x & 31;
+    if (p.res_type == kF32) {
+      const float* res = reinterpret_cast<const float*>(p.res);
+      float4 q[8];
+      const int col = c + (lane & 7) * 4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = first + i * 4 + (lane >> 3);
+        q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && col < N) q[i] = __ldg(reinterpret_cast<const float4*>(res + (int64_t)r * N + col));
+      }
+      uint8_t* room = out.room();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        *reinterpret_cast<float4*>(room + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = q[i];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(room + lane * 128 + ((i ^ (lane & 7)) << 4));
+        v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
+      }
+    } else {
+      const __nv_bfloat16* res = reinterpret_cast<const __nv_bfloat16*>(p.res);
+      uint4 q[4];
+      const int col = c + (lane & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = first + i * 8 + (lane >> 2);
+        q[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows && col < N) q[i] = __ldg(reinterpret_cast<const uint4*>(res + (int64_t)r * N + col));
+      }
+      uint8_t* room = out.room();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        *reinterpret_cast<uint4*>(room + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)) = q[i];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(room + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4));
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[8 * i + 2 * j] += __uint_as_float(w[j] << 16);
+          v[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
+        }
+      }
+    }
+    __syncwarp();                            // the pieces are written again by what follows
+  }
+
+  template <class O> ASRN_DEV void chunk(float* v, int c, O& out, const CUtensorMap* map_o, const CUtensorMap* map_p) {
+    if (c >= N || first >= rows) return;     // the same for the whole warp
+    if (p.bias) gemm::add_bias(v, p.bias + c, N - c);
+    if (p.act) {
+      uint32_t s[16];
+      activate<16>(p.act, v, s);
+      if (p.keep) {
+        uint4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+        out.put(map_p, w, c, first);
+      }
+    }
+    if (p.res_type != kNone) add_residual(v, c, out);
+    if (p.res_type == kF32) {
+#pragma unroll
+      for (int half = 0; half < 32; half += 16) {
+        if (c + half >= N) break;
+        uint4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = make_uint4(__float_as_uint(v[half + 4 * i]), __float_as_uint(v[half + 4 * i + 1]),
+                            __float_as_uint(v[half + 4 * i + 2]), __float_as_uint(v[half + 4 * i + 3]));
+        out.put(map_o, w, c + half, first);
+      }
+    } else {
+      out.put(map_o, v, c, first);
+    }
+  }
+  ASRN_DEV void finish() {}
+};
+
+// D (16 x 8) += A (16 x 16) B (16 x 8).
+ASRN_DEV void mma16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 columns of y for up to 8 NT rows of x: A = 16 rows of W, B = the rows of x. The order of K inside a tile is free as long as
+// A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
+// memory, and four lanes read 64 neighbouring bytes. Warp w takes every eighth 32 of K; their sums meet in shared memory.
+constexpr int kFewWarps = 8;
+template <int NT>
+__global__ void __launch_bounds__(kFewWarps * 32)
+k_linear_few(int rows, int n, int d, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w, const Rest p,
+             void* __restrict__ y, __half* __restrict__ slope) {
+  constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
+  __shared__ float sh[kFewWarps][8 * NT][17];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int o0 = blockIdx.x * 16;
+  const bool on[2] = {o0 + g < n, o0 + g + 8 < n};
+  const __nv_bfloat16* wp = w + (int64_t)(o0 + g) * d + 8 * t;
+  const __nv_bfloat16* xp = x + (int64_t)g * d + 8 * t;
+  float acc[NT][4] = {};
+  for (int k0 = wid * 32; k0 < d; k0 += kU * kFewWarps * 32) {
+    uint4 a[kU][2], b[kU][NT];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int k = k0 + u * kFewWarps * 32;
+      const bool in = k + 8 * t < d;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[u][i] = make_uint4(0, 0, 0, 0);
+        if (in && on[i]) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (int64_t)i * 8 * d + k));
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        b[u][i] = make_uint4(0, 0, 0, 0);
+        if (in && i * 8 + g < rows) b[u][i] = __ldg(reinterpret_cast<const uint4*>(xp + (int64_t)i * 8 * d + k));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        mma16x8(acc[i], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][i].x, b[u][i].y);
+        mma16x8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sh[wid][i * 8 + 2 * t + (j & 1)][g + (j >> 1) * 8] = acc[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 8 * NT * 8; e += kFewWarps * 32) {       // two columns each
+    const int r = e / 8, c = e % 8 * 2;
+    if (r >= rows || o0 + c >= n) continue;
+    float v[2] = {};
+#pragma unroll
+    for (int k = 0; k < kFewWarps; ++k) {
+      v[0] += sh[k][r][c];
+      v[1] += sh[k][r][c + 1];
+    }
+    const int64_t at = (int64_t)r * n + o0 + c;
+    if (p.bias) {
+      v[0] += __bfloat162float(p.bias[o0 + c]);
+      v[1] += __bfloat162float(p.bias[o0 + c + 1]);
+    }
+    if (p.act) {
+      uint32_t s;
+      activate<1>(p.act, v, &s);
+      if (p.keep) *reinterpret_cast<uint32_t*>(slope + at) = s;
+    }
+    if (p.res_type == kF32) {
+      const float2 r2 = __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.res) + at));
+      *reinterpret_cast<float2*>(reinterpret_cast<float*>(y) + at) = make_float2(v[0] + r2.x, v[1] + r2.y);
+    } else {
+      if (p.res_type == kBf16) {
+        const uint32_t r2 = __ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(p.res) + at));
+        v[0] += __uint_as_float(r2 << 16);
+        v[1] += __uint_as_float(r2 & 0xffff0000u);
+      }
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(y) + at) = pack2_bf16(v[0], v[1]);
+    }
+  }
+}
+
+// dA = dY slope in bf16 (da null: not wanted; slope null: 1), its remainder `below` rows further on unless that is 0 (then rows
+// from `rows` to `below` are zeros in both), and its columns' sums over 64 rows. Block = 64 rows x 256 columns, a lane 8 columns,
+// a warp every eighth row.
+constexpr int kSlopeRows = 64;
+template <bool F32>
+__global__ void __launch_bounds__(256)
+k_linear_slope(int64_t rows, int n, int below, const void* __restrict__ dy, const __half* __restrict__ slope,
+               __nv_bfloat16* __restrict__ da, float* __restrict__ sums) {
+  __shared__ float sh[8][256];
+  const int wide = (n + 255) / 256, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int c0 = blockIdx.x % wide * 256, c = c0 + lane * 8;
+  const int64_t r0 = (int64_t)(blockIdx.x / wide) * kSlopeRows;
+  float s[8] = {};
+  constexpr int kEach = kSlopeRows / 8, kHalf = kEach / 2;
+#pragma unroll
+  for (int h = 0; h < kEach; h += kHalf) {
+    uint4 q[kHalf][2], f[kHalf];
+#pragma unroll
+    for (int k = 0; k < kHalf; ++k) {
+      const int64_t r = r0 + (h + k) * 8 + wid, at = r * n + c;
+      q[k][0] = q[k][1] = make_uint4(0, 0, 0, 0);
+      if (r < rows && c < n) {
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(dy) + at * (F32 ? 4 : 2));
+        q[k][0] = __ldg(src);
+        if (F32) q[k][1] = __ldg(src + 1);
+        if (slope) f[k] = __ldg(reinterpret_cast<const uint4*>(slope + at));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kHalf; ++k) {
+      const int64_t r = r0 + (h + k) * 8 + wid;
+      if (c >= n || r >= (rows > below ? rows : below)) continue;
+      float v[8];
+      const uint32_t w[8] = {q[k][0].x, q[k][0].y, q[k][0].z, q[k][0].w, q[k][1].x, q[k][1].y, q[k][1].z, q[k][1].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = __uint_as_float(F32 ? w[j] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+      if (slope && r < rows) {
+        const uint32_t z[4] = {f[k].x, f[k].y, f[k].z, f[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&z[j]));
+          v[2 * j] *= x.x;
+          v[2 * j + 1] *= x.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+      if (da) {
+        *reinterpret_cast<uint4*>(da + r * n + c) = gemm::pack8(v);
+        if (below) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] -= round_bf16(v[j]);
+          *reinterpret_cast<uint4*>(da + (r + below) * n + c) = gemm::pack8(v);
+        }
+      }
+    }
+  }
+  if (!sums || r0 >= rows) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[wid][lane + 32 * j] = s[j];
+  __syncthreads();
+  const int own = c0 + lane * 8 + wid;                   // this thread's column: its lane's wid-th
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v += sh[k][threadIdx.x];
+  if (own < n) sums[(int64_t)(blockIdx.x / wide) * n + own] = v;
+}
+
+struct LinearWs {
+  int below, shares;                           // below: rows to dA's remainder (a multiple of 32), 0: none
+  int64_t rows;                                // of dA, its remainder among them
+  size_t da, sums, slots, total;
+};
+
+// own: dA is dY itself.
+LinearWs linear_ws(int64_t N, int64_t d, int64_t n, bool own) {
+  LinearWs w{};
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
+  w.below = N <= kTwiceRows && !own ? (int)((N + 31) / 32 * 32) : 0;
+  w.rows = w.below ? 2 * w.below : N;
+  w.shares = gemm::shares_for(n, d, w.rows);
+  w.da = take(own ? 0 : (size_t)w.rows * n * 2);
+  w.sums = take((size_t)((N + kSlopeRows - 1) / kSlopeRows) * n * 4);
+  w.slots = take(w.shares ? gemm::slot_bytes(n, d, w.shares) : 0);
+  w.total = o;
+  return w;
+}
+
+int check_linear(int64_t N, int32_t d, int32_t n) {
+  if (N < 0 || d < 1 || n < 1) return ASRN_ERR_ARG;
+  if (d % 8 || n % 8 || d > 65536 || n > (1 << 20) || N > (1 << 26)) return ASRN_ERR_UNSUPPORTED;
+  if ((int64_t)((N + 127) / 128) * ((std::max(d, n) + 255) / 256) >= ((int64_t)1 << 30)) return ASRN_ERR_UNSUPPORTED;
+  return ASRN_OK;
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
+
+template <int NT>
+int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, void* y, void* slope, cudaStream_t s) {
+  k_linear_few<NT><<<(unsigned)((n + 15) / 16), kFewWarps * 32, 0, s>>>(
+      (int)N, n, d, reinterpret_cast<const __nv_bfloat16*>(x), reinterpret_cast<const __nv_bfloat16*>(w), p, y,
+      reinterpret_cast<__half*>(slope));
+  return launched();
+}
+
+}  // namespace
+}  // namespace asrn
+
+extern "C" {
+
+int asrn_linear_forward(int64_t N, int32_t d, int32_t n, const void* x, const void* weight, const void* bias, int32_t act,
+                        const void* residual, int32_t res_type, void* y, void* slope, int* status, void* stream) {
+  using namespace asrn;
+  int st = check_linear(N, d, n);
+  if (st) return st;
+  if (act < 0 || act > kRelu || (residual && res_type != kF32 && res_type != kBf16)) return ASRN_ERR_ARG;
+  if (N == 0) return ASRN_OK;
+  if (!x || !weight || !y || ((uintptr_t)x | (uintptr_t)weight | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y |
+                              (uintptr_t)slope) % 16)
+    return ASRN_ERR_ARG;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const Rest p{reinterpret_cast<const __nv_bfloat16*>(bias), residual, act, residual ? res_type : kNone, act && slope};
+  if (N <= kFewRows)
+    return N <= 8    ? few<1>(N, d, n, x, weight, p, y, slope, s)
+           : N <= 16 ? few<2>(N, d, n, x, weight, p, y, slope, s)
+           : N <= 32 ? few<4>(N, d, n, x, weight, p, y, slope, s)
+                     : few<8>(N, d, n, x, weight, p, y, slope, s);
+  gemm::Shape a{};
+  a.M = (int)N; a.N = n; a.K = d; a.group = 16; a.status = status;
+  return gemm::launch<false, false, Fused>(x, d, weight, d, a, p, s, {y, N, n, n, p.res_type == kF32},
+                                           {p.keep ? slope : nullptr, N, n, n});
+}
+
+size_t asrn_linear_workspace_bytes(int64_t N, int32_t d, int32_t n, int32_t act, int32_t y_type) {
+  if (asrn::check_linear(N, d, n) || N == 0) return 0;
+  return asrn::linear_ws(N, d, n, !act && y_type == asrn::kBf16).total;
+}
+
+int asrn_linear_backward(int64_t N, int32_t d, int32_t n, const void* dy, int32_t y_type, const void* x, const void* weight,
+                         int32_t act, const void* slope, void* dx, void* dw, void* db, void* workspace,
+                         size_t workspace_bytes, int* status, void* stream) {
+  using namespace asrn;
+  int st = check_linear(N, d, n);
+  if (st) return st;
+  if (act < 0 || act > kRelu || (y_type != kF32 && y_type != kBf16)) return ASRN_ERR_ARG;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (N == 0) {
+    if ((dw && cudaMemsetAsync(dw, 0, (size_t)n * d * 2, s) != cudaSuccess) ||
+        (db && cudaMemsetAsync(db, 0, (size_t)n * 2, s) != cudaSuccess))
+      return ASRN_ERR_CUDA;
+    return ASRN_OK;
+  }
+  if (!dy || !x || !weight || (act && !slope) || ((uintptr_t)dy | (uintptr_t)x | (uintptr_t)weight | (uintptr_t)slope |
+                                                  (uintptr_t)dx | (uintptr_t)dw) % 16 || (uintptr_t)db % 2)
+    return ASRN_ERR_ARG;
+  const bool own = !act && y_type == kBf16;
+  const LinearWs ws = linear_ws(N, d, n, own);
+  if (!workspace || workspace_bytes < ws.total || (uintptr_t)workspace % 256) return ASRN_ERR_WORKSPACE;
+  char* W = reinterpret_cast<char*>(workspace);
+  float* sums = reinterpret_cast<float*>(W + ws.sums);
+  __nv_bfloat16* made = reinterpret_cast<__nv_bfloat16*>(W + ws.da);
+  if (db || (!own && (dx || dw))) {
+    const int64_t all = std::max<int64_t>(N, ws.below), blocks = (all + kSlopeRows - 1) / kSlopeRows * ((n + 255) / 256);
+    __nv_bfloat16* to = own || !(dx || dw) ? nullptr : made;
+    const __half* f = act ? reinterpret_cast<const __half*>(slope) : nullptr;
+    if (y_type == kF32)
+      k_linear_slope<true><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, dy, f, to, db ? sums : nullptr);
+    else
+      k_linear_slope<false><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, dy, f, to, db ? sums : nullptr);
+    if ((st = launched())) return st;
+  }
+  const void* da = own ? dy : made;
+  if (dx) {
+    gemm::Shape a{};
+    a.M = (int)N; a.N = d; a.K = n; a.group = 16; a.status = status;
+    a.second_pass = ws.below > 0; a.a_step = ws.below;
+    if ((st = gemm::launch<false, true, gemm::StoreBf16>(da, n, weight, d, a, {}, s, {dx, N, d, d}))) return st;
+  }
+  if (dw && (st = weight_grad(N, n, d, da, ws.below, x, 0, ws.shares, reinterpret_cast<float*>(W + ws.slots), dw, status, s)))
+    return st;
+  if (db) {
+    const ColSum q{(N + kSlopeRows - 1) / kSlopeRows, n, sums, reinterpret_cast<__nv_bfloat16*>(db)};
+    k_colsum<<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(q, ColSum{}, (n + 31) / 32);
+    return launched();
+  }
+  return ASRN_OK;
+}
+
+}  // extern "C"

@@ -101,6 +101,21 @@ bool make_tmap_f32_sw128(void* map, const void* base, uint64_t inner, uint64_t o
   return r == CUDA_SUCCESS;
 }
 
+// The same with the 64-byte swizzle (box_inner = 16).
+bool make_tmap_f32_sw64(void* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                        uint32_t box_inner, uint32_t box_outer) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base),
+                  dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // Row-major bf16 tensor (d2, d1, d0) as a 3-D map (innermost d0), boxes of box0 x box1 x 1 with the 128-byte swizzle:
 // per-sequence rows, so a box that starts before row 0 or runs past row d1 - 1 of its sequence reads zeros there.
 bool make_tmap_bf16_3d(void* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box0,

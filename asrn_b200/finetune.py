@@ -113,3 +113,41 @@ def mlp8(x, w1, b1, w2, b2):
     form: (d + ff) 33 / 32 bytes a row), and the gradients are those of the values so kept. d, ff and dout have to be
     multiples of 8."""
     return _lib.finetune().mlp8(x, w1, b1, w2, b2)
+
+
+def layer_norm(x, weight, bias=None, residual=None, eps=1e-5, dtype=None):
+    """Layer norm over the last dimension, x (..., d), weight and bias (d), d up to 16384, each float32 or bfloat16 ->
+    y of type `dtype` (default: x's). With residual (..., d) the sum s = x + residual, rounded to the residual's type, is
+    normalised and handed on: returns (y, s), one pass over memory for both. Sums and statistics in fp32. Differentiable
+    in x, weight, bias and residual; the weight's gradient is summed in fp32, in a fixed order."""
+    y, s = _lib.finetune().layer_norm(x, weight, bias, residual, eps, dtype)
+    return y if residual is None else (y, s)
+
+
+_ACTIVATIONS = {None: 0, 'gelu': 1, 'silu': 2, 'relu': 3}
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """activation(x weight^T + bias) + residual in one product: x (..., d), weight (n, d), bias (n) bfloat16 (or float32
+    under bf16 autocast), activation None, 'gelu' (erf), 'silu' or 'relu', residual (..., n) float32 or bfloat16 -> (..., n)
+    of the residual's type, bfloat16 without one. d and n have to be multiples of 8. For the backward pass it keeps x and
+    the activation's slope in fp16. Up to 64 rows take a kernel that spreads the weight over the whole GPU."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"linear: activation is None, 'gelu', 'silu' or 'relu'; got {activation!r}")
+    return _lib.finetune().linear(x, weight, bias, _ACTIVATIONS[activation], residual)
+
+
+HeadStats = namedtuple('HeadStats', 'logp entropy top_logp top_tokens')
+
+
+def head_stats(h, weight, tokens=None, temperatura=1.0, top=0):
+    """The distribution p = softmax(h weight^T / temperatura) by its statistics, without its (tokens, V) logits: h (..., d),
+    weight (V, d) bfloat16 (or float32 under bf16 autocast), tokens (...) int64 or None. Returns HeadStats:
+      logp        log p[token] (None without tokens), float32, head_logprobs' values
+      entropy     - sum p log p, float32
+      top_logp, top_tokens   (..., top) the `top` (up to 32) likeliest tokens and their log probabilities, the likeliest first,
+                  equal ones by their number; ranked by scores summed in 64 bits (None without top)
+    Differentiable in h and weight through logp and entropy. A negative token leaves its position out (0, tokens -1, no
+    gradient, none of the work); a token >= V, and scores whose exponentials have no finite sum, give NaN and tokens -1. d has
+    to be a multiple of 8; the backward pass holds what head_logprobs' does."""
+    return HeadStats(*_lib.finetune().head_stats(h, weight, tokens, temperatura, top))

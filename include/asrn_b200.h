@@ -292,6 +292,54 @@ int asrn_mlp8_backward(int64_t N, int32_t d, int32_t ff, int32_t dout, const voi
                        const void* saved, size_t saved_bytes, void* dx, void* dw1, void* db1, void* dw2, void* db2,
                        void* workspace, size_t workspace_bytes, int* status, void* stream);
 
+/* ---- layer norm, products with an epilogue, statistics of the head's distribution -----------------------------------
+ * Types: 0 float32, 1 bfloat16. Rows contiguous. No counterpart in the reference beyond the modules these stand for. Results
+ * repeat bit for bit.
+ *
+ * asrn_layer_norm: y (rows, d) = (s - mean s) / sqrt(var s + eps) weight + bias by rows, with s = x, or x + residual
+ * rounded to the residual's type and written to `sum`. bias and residual may be NULL; bias is of the weight's type. stats
+ * (rows, 2) float32, may be NULL: each row's mean and 1 / sqrt(var + eps), for the backward pass. d <= 16384; any alignment that
+ * the types allow (widths that are multiples of 8 and 16-byte aligned pointers are read 16 bytes at a time). eps >= 0.
+ * asrn_layer_norm_backward: s_in = what was normalised (x, or sum), of s_type; dy = dL/dy; ds = dL/dsum or NULL. out (s_type) and
+ * `other` (the other type) = dL/dx = dL/dresidual, dw and db (d) of the weight's type; each may be NULL. The workspace (256-byte
+ * aligned) is needed for dw and db. */
+int asrn_layer_norm(int64_t rows, int32_t d, const void* x, int32_t x_type, const void* residual, int32_t res_type,
+                    const void* weight, const void* bias, int32_t w_type, float eps, void* sum, void* y, int32_t y_type,
+                    float* stats, void* stream);
+size_t asrn_layer_norm_workspace_bytes(int64_t rows, int32_t d);
+int asrn_layer_norm_backward(int64_t rows, int32_t d, const void* s_in, int32_t s_type, const float* stats, const void* dy,
+                             int32_t y_type, const void* ds, const void* weight, int32_t w_type, void* out, void* other,
+                             void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* asrn_linear_forward: y (N, n) = act(x W^T + bias) + residual: x (N, d), weight (n, d), bias (n) bfloat16, residual and y of
+ * res_type (y bfloat16 without a residual); bias, residual may be NULL. act: 0 none, 1 gelu (erf), 2 silu, 3 relu. slope (N, n)
+ * 16 bits each (fp16), may be NULL: act'(x W^T + bias), for the backward pass. d and n multiples of 8, all pointers 16-byte
+ * aligned. status as above.
+ * asrn_linear_backward: from dy (N, n) of y_type, dx (N, d), dw (n, d), db (n) bfloat16, each of which may be NULL (the
+ * residual's gradient is dy); slope may be NULL when act is 0. */
+int asrn_linear_forward(int64_t N, int32_t d, int32_t n, const void* x, const void* weight, const void* bias, int32_t act,
+                        const void* residual, int32_t res_type, void* y, void* slope, int* status, void* stream);
+size_t asrn_linear_workspace_bytes(int64_t N, int32_t d, int32_t n, int32_t act, int32_t y_type);
+int asrn_linear_backward(int64_t N, int32_t d, int32_t n, const void* dy, int32_t y_type, const void* x, const void* weight,
+                         int32_t act, const void* slope, void* dx, void* dw, void* db, void* workspace,
+                         size_t workspace_bytes, int* status, void* stream);
+
+/* asrn_head_stats_forward: asrn_head_forward's logp with entropy (N) = - sum p log p, p = softmax(h W^T / tau), and the `top`
+ * (0 to 32, at most V) likeliest tokens, top_tokens (N, top) int64 with their log probabilities top_logp (N, top), by
+ * their scores summed in 64 bits, equal ones by their numbers. tokens may be NULL: every position counts, and logp is not
+ * written. A negative token leaves its position out: 0 everywhere and tokens -1; a token >= V, and scores without a finite log of
+ * their sum of exponentials, give NaN and tokens -1.
+ * asrn_head_stats_backward: from g = dL/dlogp and g_entropy = dL/dentropy (N), either may be NULL. */
+size_t asrn_head_stats_saved_bytes(int64_t N, int32_t d);
+size_t asrn_head_stats_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t top, int32_t backward);
+int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, const void* weight, const int64_t* tokens,
+                            float tau, int32_t top, float* logp, float* entropy, float* top_logp, int64_t* top_tokens,
+                            void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes, int* status,
+                            void* stream);
+int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
+                             float tau, const float* g, const float* g_entropy, void* dh, void* dw, void* workspace,
+                             size_t workspace_bytes, int* status, void* stream);
+
 /* ---- sequence-chunk sharding (one long sequence over several GPUs) --------------------------------------------------
  * Shard r of `world` owns positions [c0, c0 + Lc) of every sequence (L = world * Lc). Its sorted rows hold its own
  * slots and, before each bucket's local run, the up to C earlier-chunk slots some local query has as a candidate (the
