@@ -7,13 +7,15 @@
 //   k_gemm<Scan>   scores by tiles; each thread keeps of its row's 128 columns the maximum m, S = sum exp(s - m), T = sum
 //                  exp(s - m) (s - m), and where the likeliest tokens are wanted the two largest scores, the largest with its
 //                  column in the low 7 bits; the target is in none of the sums
+//   k_stats_few    the same for few rows
 //   k_stats_join   a row's sums joined: logp, H
 //   k_stats_top    a warp per row: the groups of 128 columns by their largest scores, for as long as one may hold one of the
-//                  likeliest tokens; what it may be is scored again from h and W with a sum in 64 bits. So the order of
-//                  the tokens is that of their exact scores, whatever the products' fp32 sums rounded; equal scores are
+//                  likeliest tokens. Where the products' rounding leaves their order open, what may count is scored again
+//                  from h and W with a sum in 64 bits: the order of the tokens is that of their exact scores, equal ones
 //                  in the order of their numbers.
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
 #include "head.cuh"
+#include "products.cuh"
 
 namespace asrn {
 
@@ -39,7 +41,7 @@ StatsSaved stats_saved(int64_t N, int64_t d) {
   return w;
 }
 
-int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
+__host__ ASRN_DEV int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
 
 struct StatsWs {
   size_t counts, top, part, ent, base, pairs, total;
@@ -138,6 +140,100 @@ template <bool Top> struct Scan {
   }
 };
 
+// The same for up to kFewRows rows, bound by the weight's bytes: block = 128 columns (one group), a warp 16 of them and all of K;
+// mma.sync from registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a
+// lane takes 8 neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do.
+// Then a warp per row of h over the 128 scores.
+constexpr int64_t kFewRows = 64;
+template <int NT, bool Top>
+__global__ void __launch_bounds__(256)
+k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w, const int* __restrict__ count,
+            const typename Scan<Top>::Params p) {
+  constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
+  __shared__ __align__(16) float sh[8 * NT][132];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int v0 = blockIdx.x * 128 + wid * 16;
+  const bool on[2] = {v0 + g < V, v0 + g + 8 < V};
+  const __nv_bfloat16* wp = w + (int64_t)(v0 + g) * d + 8 * t;
+  const __nv_bfloat16* hp = h + (int64_t)g * d + 8 * t;
+  wait_previous();
+  let_next();
+  const int rows = *count;
+  float acc[NT][4] = {};
+  for (int k0 = 0; k0 < d; k0 += kU * 32) {
+    uint4 a[kU][2], b[kU][NT];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int k = k0 + u * 32;
+      const bool in = k + 8 * t < d;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[u][i] = make_uint4(0, 0, 0, 0);
+        if (in && on[i]) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (int64_t)i * 8 * d + k));
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        b[u][i] = make_uint4(0, 0, 0, 0);
+        if (in && i * 8 + g < rows) b[u][i] = __ldg(reinterpret_cast<const uint4*>(hp + (int64_t)i * 8 * d + k));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        mma16x8(acc[i], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][i].x, b[u][i].y);
+        mma16x8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sh[i * 8 + 2 * t + (j & 1)][wid * 16 + g + (j >> 1) * 8] = acc[i][j];
+  __syncthreads();
+  const int halves = halves_of(V), at = blockIdx.x;
+  for (int r = wid; r < rows && r < 8 * NT; r += 8) {
+    const int y = p.tok[r], c0 = at * 128 + lane * 4;
+    const float4 q = *reinterpret_cast<const float4*>(&sh[r][lane * 4]);
+    float v[4] = {q.x, q.y, q.z, q.w};
+    float m = -INFINITY, first = kNothing, second = kNothing;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c0 + j == y) p.top[r] = v[j];
+      if (c0 + j == y || c0 + j >= V) v[j] = kNothing;
+      m = fmaxf(m, v[j]);
+      if (Top) {
+        const float u = __uint_as_float((__float_as_uint(v[j]) & ~127u) | (uint32_t)(lane * 4 + j));
+        second = fmaxf(second, fminf(first, u));
+        first = fmaxf(first, u);
+      }
+    }
+    m = warp_max(m);
+    const float off = m <= kNothing ? 0.f : m * p.k;
+    float s = 0.f, e = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = fmaf(v[j], p.k, -off), f = exp2_fast(x);
+      s += f;
+      e = fmaf(f, fmaxf(x, kLeast), e);
+    }
+    s = warp_sum(s);
+    e = warp_sum(e);
+    if (Top) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+        second = fmaxf(fmaxf(second, s2), fminf(first, f2));
+        first = fmaxf(first, f2);
+      }
+    }
+    if (lane == 0) {
+      p.part[at * p.pad + r] = make_float2(m <= kNothing ? -INFINITY : m, s);
+      p.ent[at * p.pad + r] = e;
+      if (Top) p.pairs[(int64_t)r * halves + at] = make_float2(first, second);
+    }
+  }
+}
+
 // Block = 32 positions x 16 warps over the halves of the vocabulary's tiles, 8 at a time. A position's void when its target is
 // outside the vocabulary or its scores have no log-sum-exp (an infinity or a NaN among them): NaN in all its results.
 constexpr int kJoinWarps = 16;
@@ -149,6 +245,8 @@ k_stats_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const i
   __shared__ float sh[3][kJoinWarps][32];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  wait_previous();
+  let_next();
   const int r = i < N ? pos[i] : -1;
   float m = -INFINITY, s = 0.f, t = 0.f;
   auto join = [&](const float* qm, const float* qs, const float* qt, int n) {   // n of at most 8
@@ -252,17 +350,16 @@ k_stats_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const i
   if (base) base[r] = (double)from * inv_tau + off;
 }
 
-// A score as a number that orders as it does; 0: none.
+// A noted score as a number that orders as it does; 0: none.
 ASRN_DEV uint32_t order_of(float v) {
   const uint32_t u = __float_as_uint(v) & ~127u;
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// h . w for n of up to four rows of W, products of bf16 exact in fp32, summed in 64 bits; size: the largest sum of their magnitudes.
-ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, int n, double* out, float& size) {
+// h . w for n of up to four rows of W, products of bf16 exact in fp32, summed in 64 bits.
+ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, int n, double* out) {
   const int lane = threadIdx.x & 31;
   double acc[4] = {};
-  float mag[4] = {};
   for (int c = lane; c < vecs; c += 32) {
     const uint4 a = __ldg(h + c);
     uint4 b[4];
@@ -274,19 +371,59 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, i
       const uint32_t y[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float lo = __uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16);
-        const float hi = __uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u);
-        acc[j] += (double)lo;
-        acc[j] += (double)hi;
-        mag[j] += fabsf(lo) + fabsf(hi);
+        acc[j] += (double)(__uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16));
+        acc[j] += (double)(__uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u));
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    out[j] = warp_sum_d(acc[j]);
-    if (j < n) size = fmaxf(size, warp_sum(mag[j]));
+  for (int j = 0; j < 4; ++j) out[j] = warp_sum_d(acc[j]);
+}
+// The same in fp32 for eight rows from `first` on (those past `last` repeat it): the lanes 4 j to 4 j + 3 get row j's, with j's bits
+// in the order 4, 2, 1 of the lane's bits 4, 3, 2.
+ASRN_DEV float dots8(const uint4* h, const uint4* W, int vecs, int first, int last) {
+  const int lane = threadIdx.x & 31;
+  float acc[8] = {};
+  for (int c = lane; c < vecs; c += 32) {
+    const uint4 a = __ldg(h + c);
+    uint4 b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __ldg(W + (int64_t)min(first + j, last) * vecs + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t y[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[j] = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), acc[j]);
+        acc[j] = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), acc[j]);
+      }
+    }
   }
+#pragma unroll
+  for (int n = 4, o = 16; n > 0; n >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float keep = up ? acc[j + n] : acc[j], send = up ? acc[j] : acc[j + n];
+      acc[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 2);
+  return acc[0] + __shfl_xor_sync(0xffffffffu, acc[0], 1);
+}
+// sum |h w| of one row of W.
+ASRN_DEV float magnitude(const uint4* h, const uint4* W, int vecs, int token) {
+  float s = 0.f;
+  for (int c = threadIdx.x & 31; c < vecs; c += 32) {
+    const uint4 a = __ldg(h + c), b = __ldg(W + (int64_t)token * vecs + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      s += fabsf(__uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16)) +
+           fabsf(__uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u));
+  }
+  return warp_sum(s);
 }
 
 // The best so far, lane l the l-th, larger scores first, then smaller numbers.
@@ -311,14 +448,20 @@ struct Best {
   }
 };
 
+// A row's likeliest tokens from the groups' two largest scores. In most rows these tell: the scores that count stand further apart
+// than what the products' rounding may have moved them by, and no group's second may be among them. Where they do not, what may
+// count is scored again, first by sums in fp32, what they leave by sums in 64 bits.
 constexpr int kTopWarps = 4;
 __global__ void __launch_bounds__(kTopWarps * 32)
-k_stats_top(int64_t N, int V, int d, int top, int halves, float inv_tau, const uint4* __restrict__ hc,
+k_stats_top(int64_t N, int V, int d, int top, int halves, int64_t pad, float inv_tau, const uint4* __restrict__ hc,
             const uint4* __restrict__ W, const int* __restrict__ pos, const int* __restrict__ tok,
             const float* __restrict__ lse2, const double* __restrict__ base, const float2* __restrict__ pairs,
-            float* __restrict__ top_logp, int64_t* __restrict__ top_tokens) {
+            const float2* __restrict__ part, const float* __restrict__ own, float* __restrict__ top_logp,
+            int64_t* __restrict__ top_tokens) {
   const int lane = threadIdx.x & 31;
   const int64_t i = (int64_t)blockIdx.x * kTopWarps + (threadIdx.x >> 5);
+  wait_previous();
+  let_next();
   if (i >= N) return;
   const int r = pos[i];
   const bool bad = r >= 0 && !(fabsf(lse2[r]) < INFINITY);
@@ -332,22 +475,14 @@ k_stats_top(int64_t N, int V, int d, int top, int halves, float inv_tau, const u
   const int vecs = d / 8, y = tok[r];
   const uint4* h = hc + (int64_t)r * vecs;
   const float2* mine = pairs + (int64_t)r * halves;
-  Best best;
-  float size = 0.f;                              // the largest sum of |h w| seen
-  double s[4];
-  if (y >= 0) {
-    const int t[4] = {y};
-    dots(h, W, vecs, t, 1, s, size);
-    best.put(s[0], y);
-  }
   // The groups in the order of their largest scores, equal ones by their numbers: each lane holds the next of its own, those
   // after `last`.
-  uint32_t key = 0xffffffffu, last = 0xffffffffu;
+  uint32_t key = 0, last = 0xffffffffu;
   int group = -1, last_group = -1;
   auto find = [&]() {
     key = 0;
     group = 0x7fffffff;
-#pragma unroll 4
+#pragma unroll 8
     for (int g = lane; g < halves; g += 32) {
       const float v = __ldg(&mine[g].x);
       const uint32_t o = v <= -3e38f ? 0u : order_of(v);
@@ -363,71 +498,116 @@ k_stats_top(int64_t N, int V, int d, int top, int halves, float inv_tau, const u
     const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
     last = most;
     last_group = g;
+    pair = __ldg(mine + g);
     if (group == g && key == most) find();
     __syncwarp();
-    pair = __ldg(mine + g);
     return g;
   };
   auto column = [&](int g, float v) { return g * 128 + (int)(__float_as_uint(v) & 127u); };
+
+  // The first `top` groups by lane, and the one after them.
+  find();
+  float2 pair = make_float2(kNothing, kNothing), held = pair;
+  int held_group = 0, have = 0, after = -1;
+  while (true) {
+    after = next(pair);
+    if (after < 0 || have == top) break;
+    if (lane == have) {
+      held = pair;
+      held_group = after;
+    }
+    ++have;
+  }
+  const int held_column = column(held_group, held.x);
+  Best best;
+  const float sure = lane < have ? __ldg(&part[(int64_t)held_group * pad + r].x) : 0.f;
+  for (int q = 0; q < have; ++q)
+    best.put(__shfl_sync(0xffffffffu, sure, q), __shfl_sync(0xffffffffu, held_column, q));
+  if (y >= 0) best.put(own[r], y);
+  // Twice what the sums in fp32, 16 products at a time, may be off by, for two scores, with twice the magnitudes of the best one.
+  const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
+  const float size = likeliest < V ? magnitude(h, W, vecs, likeliest) : 0.f, slack = (float)(d / 16 + 2) * 0x1p-21f * size;
+  // The most that a score may be whose note is v: the note's low bits, and the rounding.
+  auto above = [&](float v) { return (double)v + fabsf(v) * 0x1p-15f + slack; };
+  auto worst = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
+  {
+    const double low = worst(), next_score = __shfl_down_sync(0xffffffffu, best.score, 1);
+    const double below = lane < 31 ? next_score : -INFINITY;
+    const bool close = lane < top && (best.score - below <= slack || best.token >= V);
+    const bool hidden = lane < have && held.y > -3e38f && above(held.y) >= low;
+    const bool more = after >= 0 && above(pair.x) >= low;
+    if (!more && !__any_sync(0xffffffffu, close || hidden) && !(top == 32 && y >= 0)) {
+      if (lane < top) {
+        top_logp[i * top + lane] = (float)(best.score * inv_tau - base[r]);
+        top_tokens[i * top + lane] = best.token;
+      }
+      return;
+    }
+  }
+
+  if (size == 0.f) {                             // a row of zeros: all scores are 0
+    uint32_t any = 0;
+    for (int c = lane; c < vecs; c += 32) {
+      const uint4 a = __ldg(h + c);
+      any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
+    }
+    if (!__any_sync(0xffffffffu, any)) {
+      if (lane < top) {
+        top_logp[i * top + lane] = (float)-base[r];
+        top_tokens[i * top + lane] = lane;
+      }
+      return;
+    }
+  }
+
+  best = Best{};
+  double s[4];
+  for (int q = 0; q < have; q += 4) {
+    int t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = __shfl_sync(0xffffffffu, held_column, min(q + j, have - 1));
+    dots(h, W, vecs, t, 4, s);
+    for (int j = 0; j < 4 && q + j < have; ++j) best.put(s[j], t[j]);
+  }
+  if (y >= 0) {
+    const int t[4] = {y};
+    dots(h, W, vecs, t, 1, s);
+    best.put(s[0], y);
+  }
   // All columns of a group but one and the target's.
   auto expand = [&](int g, int except) {
     const int end = min(V, g * 128 + 128);
-    for (int c = g * 128; c < end; c += 4) {
-      const int n = min(4, end - c);
-      const int t[4] = {c, c + 1, c + 2, c + 3};
-      dots(h, W, vecs, t, n, s, size);
-      for (int j = 0; j < n; ++j)
-        if (t[j] != except && t[j] != y) best.put(s[j], t[j]);
+    for (int c = g * 128; c < end; c += 8) {
+      const float about = dots8(h, W, vecs, c, end - 1);
+      const int mine_c = c + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
+      const double low = worst();
+      unsigned count = __ballot_sync(0xffffffffu, !(lane & 3) && mine_c < end && mine_c != except && mine_c != y &&
+                                                      (double)about + slack >= low);
+      while (count) {
+        int t[4] = {}, n = 0;
+        while (count && n < 4) {
+          t[n++] = __shfl_sync(0xffffffffu, mine_c, __ffs(count) - 1);
+          count &= count - 1;
+        }
+        dots(h, W, vecs, t, n, s);
+        for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
+      }
     }
   };
-  // How far a largest score may lie above what is noted: its low bits, and the products' rounding (twice what the sums in fp32,
-  // 16 products at a time, may be off by, with twice the magnitudes seen).
-  auto above = [&](float v) { return (double)v + fabsf(v) * 0x1p-15f + (float)(d / 16 + 2) * 0x1p-21f * size; };
-  auto worst = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
-
-  find();
-  // The first `top` groups' largest, four at a time; their pairs by lane.
-  float2 pair, held = make_float2(kNothing, kNothing);
-  int held_group = -1, held_column = -1, have = 0;
-  bool more = true;
-  while (have < top && more) {
-    int t[4] = {}, n = 0;
-    while (n < 4 && have < top) {
-      const int g = next(pair);
-      if (g < 0) {
-        more = false;
-        break;
-      }
-      t[n] = column(g, pair.x);
-      if (lane == have) {
-        held = pair;
-        held_group = g;
-        held_column = t[n];
-      }
-      ++n;
-      ++have;
-    }
-    if (n) dots(h, W, vecs, t, n, s, size);
-    for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
-  }
-  // Their second ones, where they may count.
   for (int q = 0; q < have; ++q) {
     const float v = __shfl_sync(0xffffffffu, held.y, q);
     const int g = __shfl_sync(0xffffffffu, held_group, q), c = __shfl_sync(0xffffffffu, held_column, q);
     if (v > -3e38f && above(v) >= worst()) expand(g, c);
   }
-  // And the groups after them.
-  while (more) {
-    const int g = next(pair);
-    if (g < 0 || above(pair.x) < worst()) break;
-    const int t[4] = {column(g, pair.x)};
-    dots(h, W, vecs, t, 1, s, size);
+  for (; after >= 0 && above(pair.x) >= worst(); after = next(pair)) {
+    const int t[4] = {column(after, pair.x)};
+    dots(h, W, vecs, t, 1, s);
     best.put(s[0], t[0]);
-    if (pair.y > -3e38f && above(pair.y) >= worst()) expand(g, t[0]);
+    if (pair.y > -3e38f && above(pair.y) >= worst()) expand(after, t[0]);
   }
   // Scores of minus infinity are in no group: the smallest numbers that are left.
-  const int found = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < V));
-  for (int c = 0, l = found; l < top && c < V; ++c) {
+  int l = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < V));
+  for (int c = 0; l < top && c < V; ++c) {
     if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
     if (lane == l) best.token = c;
     ++l;
@@ -494,6 +674,37 @@ struct Slope {
   ASRN_DEV void finish() {}
 };
 
+// A launch whose blocks may start while the kernel before it ends (it has a wait_previous).
+template <class... P, class... A>
+int launch_next(void (*kernel)(P...), int64_t blocks, int threads, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
+template <int NT, bool Top>
+int few(int64_t V, int d, const void* hc, const void* weight, const int* count, const typename Scan<Top>::Params& p,
+        cudaStream_t s) {
+  return launch_next(k_stats_few<NT, Top>, halves_of(V), 256, s, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
+                     reinterpret_cast<const __nv_bfloat16*>(weight), count, p);
+}
+template <bool Top>
+int scan(int64_t N, int64_t V, int d, const void* hc, const void* weight, const gemm::Shape& sh,
+         const typename Scan<Top>::Params& p, cudaStream_t s) {
+  if (N > kFewRows) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
+  return N <= 8    ? few<1, Top>(V, d, hc, weight, sh.m_dev, p, s)
+         : N <= 16 ? few<2, Top>(V, d, hc, weight, sh.m_dev, p, s)
+         : N <= 32 ? few<4, Top>(V, d, hc, weight, sh.m_dev, p, s)
+                   : few<8, Top>(V, d, hc, weight, sh.m_dev, p, s);
+}
+
 }  // namespace
 
 }  // namespace asrn
@@ -546,18 +757,17 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   float* ent = reinterpret_cast<float*>(W + ws.ent);
   float2* pairs = reinterpret_cast<float2*>(W + ws.pairs);
   if (top)
-    st = gemm::launch<false, false, Scan<true>>(hc, d, weight, d, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
+    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
   else
-    st = gemm::launch<false, false, Scan<false>>(hc, d, weight, d, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
-  if (st) return st;
-  k_stats_join<<<(unsigned)((N + 31) / 32), kJoinWarps * 32, 0, s>>>(
-      N, halves, pad256(N), k, inv_tau, pos, tok, own, part, ent, lse2, reinterpret_cast<float*>(S + sv.head.rest),
-      reinterpret_cast<float*>(S + sv.ent), base, logp, entropy);
-  if (top)
-    k_stats_top<<<(unsigned)((N + kTopWarps - 1) / kTopWarps), kTopWarps * 32, 0, s>>>(
-        N, (int)V, d, top, halves, inv_tau, reinterpret_cast<const uint4*>(hc), reinterpret_cast<const uint4*>(weight), pos,
-        tok, lse2, base, pairs, top_logp, top_tokens);
-  return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
+  if (st || (st = launch_next(k_stats_join, (N + 31) / 32, kJoinWarps * 32, s, N, halves, pad256(N), k, inv_tau, pos, tok, own,
+                              part, ent, lse2, reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent),
+                              base, logp, entropy)))
+    return st;
+  if (!top) return ASRN_OK;
+  return launch_next(k_stats_top, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, N, (int)V, d, top, halves, pad256(N),
+                     inv_tau, reinterpret_cast<const uint4*>(hc), reinterpret_cast<const uint4*>(weight), pos, tok, lse2, base,
+                     pairs, part, own, top_logp, top_tokens);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,

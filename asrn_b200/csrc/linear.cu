@@ -184,35 +184,28 @@ struct Fused {
   ASRN_DEV void finish() {}
 };
 
-// D (16 x 8) += A (16 x 16) B (16 x 8).
-ASRN_DEV void mma16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // 16 columns of y for up to 8 NT rows of x: A = 16 rows of W, B = the rows of x. The order of K inside a tile is free as long as
 // A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
-// memory, and four lanes read 64 neighbouring bytes. Warp w takes every eighth 32 of K; their sums meet in shared memory.
+// memory, and four lanes read 64 neighbouring bytes. A block's warps take every eighth 32 of K; the blocks of a cluster share K
+// where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's.
 constexpr int kFewWarps = 8;
 template <int NT>
 __global__ void __launch_bounds__(kFewWarps * 32)
-k_linear_few(int rows, int n, int d, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w, const Rest p,
-             void* __restrict__ y, __half* __restrict__ slope) {
+k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
+             const Rest p, void* __restrict__ y, __half* __restrict__ slope) {
   constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
   __shared__ float sh[kFewWarps][8 * NT][17];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int o0 = blockIdx.x * 16;
+  const int rank = split > 1 ? (int)gemm::cluster_rank() : 0, o0 = blockIdx.x / split * 16, step = split * kFewWarps * 32;
   const bool on[2] = {o0 + g < n, o0 + g + 8 < n};
   const __nv_bfloat16* wp = w + (int64_t)(o0 + g) * d + 8 * t;
   const __nv_bfloat16* xp = x + (int64_t)g * d + 8 * t;
   float acc[NT][4] = {};
-  for (int k0 = wid * 32; k0 < d; k0 += kU * kFewWarps * 32) {
+  for (int k0 = (rank * kFewWarps + wid) * 32; k0 < d; k0 += kU * step) {
     uint4 a[kU][2], b[kU][NT];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int k = k0 + u * kFewWarps * 32;
+      const int k = k0 + u * step;
       const bool in = k + 8 * t < d;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -238,14 +231,36 @@ k_linear_few(int rows, int n, int d, const __nv_bfloat16* __restrict__ x, const 
 #pragma unroll
     for (int j = 0; j < 4; ++j) sh[wid][i * 8 + 2 * t + (j & 1)][g + (j >> 1) * 8] = acc[i][j];
   __syncthreads();
-  for (int e = threadIdx.x; e < 8 * NT * 8; e += kFewWarps * 32) {       // two columns each
+  if (split > 1) {                                       // the warps' sums to the first one's place, for the other blocks
+    for (int e = threadIdx.x; e < 8 * NT * 16; e += kFewWarps * 32) {
+      float v = sh[0][e / 16][e % 16];
+#pragma unroll
+      for (int k = 1; k < kFewWarps; ++k) v += sh[k][e / 16][e % 16];
+      sh[0][e / 16][e % 16] = v;
+    }
+    gemm::cluster_sync();
+  }
+  // Two columns each; a cluster's blocks take the pairs in turn.
+  for (int e = threadIdx.x * split + rank; e < 8 * NT * 8; e += kFewWarps * 32 * split) {
     const int r = e / 8, c = e % 8 * 2;
     if (r >= rows || o0 + c >= n) continue;
     float v[2] = {};
+    if (split > 1) {
+      for (int k = 0; k < split; ++k) {
+        const uint32_t at = gemm::peer_u32(&sh[0][r][c], k);
 #pragma unroll
-    for (int k = 0; k < kFewWarps; ++k) {
-      v[0] += sh[k][r][c];
-      v[1] += sh[k][r][c + 1];
+        for (int j = 0; j < 2; ++j) {
+          float q;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(at + 4 * j));
+          v[j] += q;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) {
+        v[0] += sh[k][r][c];
+        v[1] += sh[k][r][c + 1];
+      }
     }
     const int64_t at = (int64_t)r * n + o0 + c;
     if (p.bias) {
@@ -269,6 +284,7 @@ k_linear_few(int rows, int n, int d, const __nv_bfloat16* __restrict__ x, const 
       *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(y) + at) = pack2_bf16(v[0], v[1]);
     }
   }
+  if (split > 1) gemm::cluster_sync();                   // no block ends while another reads its sums
 }
 
 // dA = dY slope in bf16 (da null: not wanted; slope null: 1), its remainder `below` rows further on unless that is 0 (then rows
@@ -372,10 +388,23 @@ int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_C
 
 template <int NT>
 int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, void* y, void* slope, cudaStream_t s) {
-  k_linear_few<NT><<<(unsigned)((n + 15) / 16), kFewWarps * 32, 0, s>>>(
-      (int)N, n, d, reinterpret_cast<const __nv_bfloat16*>(x), reinterpret_cast<const __nv_bfloat16*>(w), p, y,
-      reinterpret_cast<__half*>(slope));
-  return launched();
+  const int blocks = (n + 15) / 16;
+  int split = 1;                                         // blocks of a cluster: until the SMs are full or K is
+  while (split < 8 && blocks * split < gemm::sm_count() && d > split * kFewWarps * 32) split *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(blocks * split));
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1;
+  return cudaLaunchKernelEx(&cfg, k_linear_few<NT>, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
+                            reinterpret_cast<const __nv_bfloat16*>(w), p, y, reinterpret_cast<__half*>(slope)) == cudaSuccess
+             ? ASRN_OK
+             : ASRN_ERR_CUDA;
 }
 
 }  // namespace

@@ -177,7 +177,7 @@ struct Backward {
   float* parts;
 };
 template <int V, int ST, int YT, int C, int T>
-__global__ void __launch_bounds__(threads_of(T), 1) k_norm_back(const Backward f) {
+__global__ void __launch_bounds__(threads_of(T), T == 256 ? 2 : 1) k_norm_back(const Backward f) {
   constexpr int kRows = threads_of(T) / T;               // of a block at a time
   __shared__ float room[2][2][32];
   __shared__ float sums[T == 32 ? 2 * 32 * C * V : 1];
@@ -286,6 +286,119 @@ __global__ void __launch_bounds__(threads_of(T), 1) k_norm_back(const Backward f
   }
 }
 
+// The same for rows that a warp holds, eight values a load (d <= 1024): each warp's next row comes to shared memory by
+// asynchronous copies while it works on the one before, which costs no registers beside the columns' sums.
+constexpr int kWarps = 4;
+ASRN_DEV void copy_row(uint8_t* to, const void* from, int64_t at, int bytes, int lane) {
+  const char* p = reinterpret_cast<const char*>(from) + at;
+  for (int b = lane * 16; b < bytes; b += 512)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + b)), "l"(p + b)
+                 : "memory");
+}
+ASRN_DEV Raw<8> staged(const uint8_t* p, int c, int t) {
+  Raw<8> r;
+  const uint4* q = reinterpret_cast<const uint4*>(p + c * (t == kBf16 ? 2 : 4));
+  r.a = q[0];
+  if (t == kF32) r.b = q[1];
+  return r;
+}
+constexpr int row_bytes(int d, int t) { return d * (t == kBf16 ? 2 : 4); }
+size_t staged_bytes(int d, int st, int yt, bool ds) {
+  return (size_t)kWarps * 2 * (row_bytes(d, st) * (1 + ds) + row_bytes(d, yt));
+}
+template <int ST, int YT, int C>
+__global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_norm_back_rows(const Backward f) {
+  extern __shared__ __align__(16) uint8_t room[];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int sb = row_bytes(f.d, ST), yb = row_bytes(f.d, YT), stage = sb * (f.ds ? 2 : 1) + yb;
+  uint8_t* mine = room + wid * 2 * stage;
+  auto fetch = [&](int64_t row, int turn) {
+    if (row < f.rows) {
+      uint8_t* to = mine + turn * stage;
+      copy_row(to, f.s, row * sb, sb, lane);
+      copy_row(to + sb, f.dy, row * yb, yb, lane);
+      if (f.ds) copy_row(to + sb + yb, f.ds, row * sb, sb, lane);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float dw[C * 8] = {}, db[C * 8] = {};
+  const float inv = 1.f / (float)f.d;
+  const int64_t step = (int64_t)gridDim.x * kWarps, row0 = (int64_t)blockIdx.x * kWarps + wid;
+  int turn = 0;
+  fetch(row0, 0);
+  float2 next = row0 < f.rows ? __ldg(f.stats + row0) : make_float2(0.f, 0.f);
+  for (int64_t row = row0; row < f.rows; row += step, turn ^= 1) {
+    __syncwarp();                                        // the room's last row has been read by every lane
+    fetch(row + step, turn ^ 1);
+    const float2 mk = next;
+    if (row + step < f.rows) next = __ldg(f.stats + row + step);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint8_t* at = mine + turn * stage;
+    float h[C * 8], g[C * 8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int c = (lane + i * 32) * 8;
+      float *u = h + i * 8, *e = g + i * 8;
+      if (c >= f.d) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = e[j] = 0.f;
+        continue;
+      }
+      float w[8];
+      floats(load((Raw<8>*)0, f.w, c, f.wt), f.wt, w);
+      floats(staged(at, c, ST), ST, u);
+      floats(staged(at + sb, c, YT), YT, e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[j] = (u[j] - mk.x) * mk.y;
+        dw[i * 8 + j] = fmaf(e[j], u[j], dw[i * 8 + j]);
+        db[i * 8 + j] += e[j];
+        e[j] *= w[j];
+        s1 += e[j];
+        s2 = fmaf(e[j], u[j], s2);
+      }
+    }
+    if (!f.out && !f.other) continue;
+    s1 = warp_sum(s1) * inv;
+    s2 = warp_sum(s2) * inv;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int c = (lane + i * 32) * 8;
+      if (c >= f.d) continue;
+      float *u = h + i * 8, *e = g + i * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = mk.y * (e[j] - s1 - u[j] * s2);
+      if (f.ds) {
+        floats(staged(at + sb + yb, c, ST), ST, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] += u[j];
+      }
+      if (f.out) store<8>(f.out, row * f.d + c, ST, e);
+      if (f.other) store<8>(f.other, row * f.d + c, 1 - ST, e);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!f.parts) return;
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(room);          // [2][C 8][32]
+  for (int w = 0; w < kWarps; ++w) {                     // the block's warps, one after another
+    if (wid == w)
+#pragma unroll
+      for (int i = 0; i < C * 8; ++i) {
+        sums[i * 32 + lane] = w ? sums[i * 32 + lane] + dw[i] : dw[i];
+        sums[(C * 8 + i) * 32 + lane] = w ? sums[(C * 8 + i) * 32 + lane] + db[i] : db[i];
+      }
+    __syncthreads();
+  }
+  float* part = f.parts + (int64_t)blockIdx.x * 2 * f.d;
+  for (int c = threadIdx.x; c < f.d; c += blockDim.x) {
+    const int q = c / 8, own = (q / 32 * 8 + c % 8) * 32 + q % 32;       // where column c's thread put it
+    part[c] = sums[own];
+    part[f.d + c] = sums[C * 256 + own];
+  }
+}
+
 // out[c] = the sum of the parts' [..][c] in order, c < n of 2 d: block = 32 columns x 32 warps.
 __global__ void __launch_bounds__(1024) k_norm_sums(int parts, int d, const float* __restrict__ sums, void* dw, void* db,
                                                     int wt) {
@@ -317,11 +430,10 @@ int sms() {
   return v;
 }
 
-// Blocks of the backward pass: as many as stay on the SMs at once, and four rows for each warp or block at least (each block
-// costs 2 d sums more).
+// Blocks of the backward pass: as many as stay on the SMs at once, each with 2 d sums of its own.
 int64_t blocks_back(int64_t rows, int d) {
-  const int64_t per = d <= 1024 ? 4 : 1;
-  return std::max<int64_t>(1, std::min<int64_t>((int64_t)sms() * (d <= 1024 ? 4 : 2), (rows + 4 * per - 1) / (4 * per)));
+  const int per = d <= 1024 ? kWarps : 1, stay = d <= 256 ? 5 : d <= 768 ? 3 : d <= 4096 ? 2 : 1;
+  return std::max<int64_t>(1, std::min<int64_t>((int64_t)sms() * stay, (rows + per - 1) / per));
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
@@ -339,13 +451,19 @@ template <int XT, int RT> int widths(const Forward& f, cudaStream_t s) {
   if (f.d <= 1024) return run<8, XT, RT, 4, 32>(f, s);
   if (f.d <= 2048) return run<8, XT, RT, 1, 256>(f, s);
   if (f.d <= 4096) return run<8, XT, RT, 2, 256>(f, s);
-  if (f.d <= 8192) return run<8, XT, RT, 4, 256>(f, s);
+  if (f.d <= 8192) return run<8, XT, RT, 2, 512>(f, s);
   return run<8, XT, RT, 4, 512>(f, s);
 }
-int singles(const Forward& f, cudaStream_t s) {
+template <class Args> int singles(const Args& f, cudaStream_t s) {
+  if (f.d <= 128) return run<1, -1, -1, 4, 32>(f, s);
   if (f.d <= 256) return run<1, -1, -1, 8, 32>(f, s);
+  if (f.d <= 384) return run<1, -1, -1, 12, 32>(f, s);
+  if (f.d <= 512) return run<1, -1, -1, 16, 32>(f, s);
+  if (f.d <= 768) return run<1, -1, -1, 24, 32>(f, s);
   if (f.d <= 1024) return run<1, -1, -1, 32, 32>(f, s);
-  if (f.d <= 8192) return run<1, -1, -1, 32, 256>(f, s);
+  if (f.d <= 2048) return run<1, -1, -1, 8, 256>(f, s);
+  if (f.d <= 4096) return run<1, -1, -1, 16, 256>(f, s);
+  if (f.d <= 8192) return run<1, -1, -1, 16, 512>(f, s);
   return run<1, -1, -1, 32, 512>(f, s);
 }
 
@@ -353,21 +471,32 @@ template <int V, int ST, int YT, int C, int T> int run(const Backward& f, cudaSt
   k_norm_back<V, ST, YT, C, T><<<(unsigned)blocks_back(f.rows, f.d), threads_of(T), 0, s>>>(f);
   return launched();
 }
+template <int ST, int YT, int C> int run_rows(const Backward& f, cudaStream_t s) {
+  auto kernel = k_norm_back_rows<ST, YT, C>;
+  constexpr size_t most = (size_t)kWarps * 2 * (row_bytes(C * 256, ST) * 2 + row_bytes(C * 256, YT));
+  static std::atomic<uint64_t> ready{0};                 // devices that know the kernel's shared memory
+  int dev = 0;
+  if (most > 48 << 10) {
+    if (cudaGetDevice(&dev) != cudaSuccess) return ASRN_ERR_CUDA;
+    if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+        return ASRN_ERR_CUDA;
+      if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+  }
+  const size_t bytes = std::max<size_t>(staged_bytes(f.d, ST, YT, f.ds != nullptr), f.parts ? C * 8 * 32 * 2 * 4 : 0);
+  kernel<<<(unsigned)blocks_back(f.rows, f.d), kWarps * 32, bytes, s>>>(f);
+  return launched();
+}
 template <int ST, int YT> int widths(const Backward& f, cudaStream_t s) {
-  if (f.d <= 256) return run<8, ST, YT, 1, 32>(f, s);
-  if (f.d <= 512) return run<8, ST, YT, 2, 32>(f, s);
-  if (f.d <= 768) return run<8, ST, YT, 3, 32>(f, s);
-  if (f.d <= 1024) return run<8, ST, YT, 4, 32>(f, s);
+  if (f.d <= 256) return run_rows<ST, YT, 1>(f, s);
+  if (f.d <= 512) return run_rows<ST, YT, 2>(f, s);
+  if (f.d <= 768) return run_rows<ST, YT, 3>(f, s);
+  if (f.d <= 1024) return run_rows<ST, YT, 4>(f, s);
   if (f.d <= 2048) return run<8, ST, YT, 1, 256>(f, s);
   if (f.d <= 4096) return run<8, ST, YT, 2, 256>(f, s);
-  if (f.d <= 8192) return run<8, ST, YT, 4, 256>(f, s);
+  if (f.d <= 8192) return run<8, ST, YT, 2, 512>(f, s);
   return run<8, ST, YT, 4, 512>(f, s);
-}
-int singles(const Backward& f, cudaStream_t s) {
-  if (f.d <= 256) return run<1, -1, -1, 8, 32>(f, s);
-  if (f.d <= 1024) return run<1, -1, -1, 32, 32>(f, s);
-  if (f.d <= 8192) return run<1, -1, -1, 32, 256>(f, s);
-  return run<1, -1, -1, 32, 512>(f, s);
 }
 
 int check_norm(int64_t rows, int32_t d) {

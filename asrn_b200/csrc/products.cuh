@@ -1,5 +1,5 @@
-// What the operators around the products of an MLP share: gelu and its slope in an epilogue, column sums, and the product
-// that makes a weight's gradient.
+// What the operators around the products share: gelu and its slope in an epilogue, column sums, the product that makes a
+// weight's gradient, and the multiplication of products with few rows.
 #pragma once
 #include "gemm_tc.cuh"
 
@@ -88,6 +88,14 @@ inline int weight_grad(int64_t rows, int M, int n, const void* A, int below_a, c
   const gemm::StorePiece::Params q{slots, gemm::kBM * gemm::pair_for(M)};
   const int st = gemm::launch<true, true, gemm::StorePiece>(A, M, B, n, a, q, s);
   return st ? st : gemm::join(a, slots, out, nullptr, nullptr, 0, s);
+}
+
+// D (16 x 8) += A (16 x 16) B (16 x 8).
+ASRN_DEV void mma16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 }  // namespace asrn
