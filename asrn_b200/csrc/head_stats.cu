@@ -62,6 +62,12 @@ StatsWs stats_ws(int64_t N, int64_t V, int top) {
   return w;
 }
 
+ASRN_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <bool Top> struct Scan {
   static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
   struct Params {
@@ -99,36 +105,49 @@ template <bool Top> struct Scan {
     }
     float now = m;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) now = fmaxf(now, v[i]);
+    for (int i = 0; i < 32; i += 2) now = max3(now, v[i], v[i + 1]);
     const float off = now <= kNothing ? 0.f : now * p.k;
     const gemm::F2 k2(p.k), off2(-off);
     gemm::F2 add(0.f), sum(0.f);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       float a, b;
-      gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2).get(a, b);
+      const gemm::F2 x = gemm::fma2(gemm::F2(v[i], v[i + 1]), k2, off2);
+      x.get(a, b);
       const gemm::F2 e(exp2_fast(a), exp2_fast(b));
       add = gemm::add2(add, e);
-      sum = gemm::fma2(e, gemm::F2(fmaxf(a, kLeast), fmaxf(b, kLeast)), sum);
+      sum = gemm::fma2(e, x, sum);
     }
-    float a, b;
-    const float step = fmaxf(fmaf(m, p.k, -off), kLeast), f = exp2_fast(fmaf(m, p.k, -off));
+    float a, b, c0, c1;
     sum.get(a, b);
-    t = fmaf(f, fmaf(step, s, t), a + b);
-    add.get(a, b);
-    s = fmaf(s, f, a + b);
-    m = now;
-    if constexpr (Top) {                   // two chains, then one; i and the chunk's place in the half in the low bits
-      float m1[2] = {kNothing, kNothing}, m2[2] = {kNothing, kNothing};
+    add.get(c0, c1);
+    float part = a + b;
+    if (!(fabsf(part) < INFINITY)) {       // 0 x infinity, of a column that does not count: again without it
+      part = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float u = __uint_as_float((__float_as_uint(v[i]) & ~127u) | (uint32_t)i);
-        m2[i & 1] = fmaxf(m2[i & 1], fminf(m1[i & 1], u));
-        m1[i & 1] = fmaxf(m1[i & 1], u);
+        const float x = fmaf(v[i], p.k, -off);
+        part = fmaf(exp2_fast(x), fmaxf(x, kLeast), part);
+      }
+    }
+    const float step = fmaxf(fmaf(m, p.k, -off), kLeast), f = exp2_fast(fmaf(m, p.k, -off));
+    t = fmaf(f, fmaf(step, s, t), part);
+    s = fmaf(s, f, c0 + c1);
+    m = now;
+    if constexpr (Top) {                   // two chains of pairs, then one; the chunk's place in the half in the low bits, too
+      float m1[2] = {kNothing, kNothing}, m2[2] = {kNothing, kNothing};
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const float u0 = __uint_as_float((__float_as_uint(v[i]) & ~127u) | (uint32_t)i);
+        const float u1 = __uint_as_float((__float_as_uint(v[i + 1]) & ~127u) | (uint32_t)(i + 1));
+        const float hi = fmaxf(u0, u1), lo = fminf(u0, u1);
+        float &q1 = m1[i >> 1 & 1], &q2 = m2[i >> 1 & 1];
+        q2 = max3(q2, lo, fminf(q1, hi));
+        q1 = fmaxf(q1, hi);
       }
       const float lo = fminf(m1[0], m1[1]);
       const float hi = __uint_as_float(__float_as_uint(fmaxf(m1[0], m1[1])) | (uint32_t)(c & 96));
-      second = fmaxf(fmaxf(second, fminf(first, hi)), fmaxf(lo, fmaxf(m2[0], m2[1])));
+      second = fmaxf(max3(second, lo, fminf(first, hi)), fmaxf(m2[0], m2[1]));
       first = fmaxf(first, hi);
     }
   }
@@ -144,7 +163,7 @@ template <bool Top> struct Scan {
 // mma.sync from registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a
 // lane takes 8 neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do.
 // Then a warp per row of h over the 128 scores.
-constexpr int64_t kFewRows = 64;
+constexpr int64_t kFewRows = 64, kFewScores = (int64_t)1 << 20;
 template <int NT, bool Top>
 __global__ void __launch_bounds__(256)
 k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w, const int* __restrict__ count,
@@ -350,16 +369,82 @@ k_stats_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const i
   if (base) base[r] = (double)from * inv_tau + off;
 }
 
-// A noted score as a number that orders as it does; 0: none.
+// A noted score as a number that orders as it does, its low 7 bits 0; 0: none.
 ASRN_DEV uint32_t order_of(float v) {
-  const uint32_t u = __float_as_uint(v) & ~127u;
-  return u >> 31 ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(v);
+  return v <= -3e38f ? 0u : (u >> 31 ? ~u : u | 0x80000000u) & ~127u;
 }
+
+// A row's groups in the order of their largest scores, equal ones by their numbers. Each lane holds the next of its own; up to
+// 32 Each groups all of them, in registers.
+template <int Each> struct Groups {
+  const float2* pairs;
+  uint32_t key[Each], best;                      // a group's order, its place among the lane's in the low bits, the first's larger
+  ASRN_DEV Groups(const float2* p, int groups) : pairs(p), best(0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < Each; ++j) {
+      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].x)) : 0u;
+      key[j] = o ? o | (uint32_t)(Each - 1 - j) : 0u;
+      best = max(best, key[j]);
+    }
+  }
+  ASRN_DEV int next(float2& pair) {              // the next group, -1: none left
+    const int lane = threadIdx.x & 31;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, best & ~127u);
+    if (most == 0) return -1;
+    const int j = Each - 1 - (int)(best & 127u);
+    const int mine = (best & ~127u) == most ? lane + 32 * j : 0x7fffffff;
+    const int g = (int)__reduce_min_sync(0xffffffffu, (unsigned)mine);
+    pair = __ldg(pairs + g);
+    if (mine == g) {
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < Each; ++i) {
+        if (i == j) key[i] = 0;
+        best = max(best, key[i]);
+      }
+    }
+    __syncwarp();
+    return g;
+  }
+};
+// Any number of groups: read again after each.
+template <> struct Groups<0> {
+  const float2* pairs;
+  int groups, group, last_group;
+  uint32_t key, last;
+  ASRN_DEV Groups(const float2* p, int n) : pairs(p), groups(n), last_group(-1), last(0xffffffffu) { find(); }
+  ASRN_DEV void find() {
+    key = 0;
+    group = 0x7fffffff;
+#pragma unroll 8
+    for (int g = threadIdx.x & 31; g < groups; g += 32) {
+      const uint32_t o = order_of(__ldg(&pairs[g].x));
+      if ((o < last || (o == last && g > last_group)) && o > key) {
+        key = o;
+        group = g;
+      }
+    }
+  }
+  ASRN_DEV int next(float2& pair) {
+    const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+    if (most == 0) return -1;
+    const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
+    last = most;
+    last_group = g;
+    pair = __ldg(pairs + g);
+    if (group == g && key == most) find();
+    __syncwarp();
+    return g;
+  }
+};
 
 // h . w for n of up to four rows of W, products of bf16 exact in fp32, summed in 64 bits.
 ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, int n, double* out) {
   const int lane = threadIdx.x & 31;
   double acc[4] = {};
+#pragma unroll 2
   for (int c = lane; c < vecs; c += 32) {
     const uint4 a = __ldg(h + c);
     uint4 b[4];
@@ -415,6 +500,7 @@ ASRN_DEV float dots8(const uint4* h, const uint4* W, int vecs, int first, int la
 // sum |h w| of one row of W.
 ASRN_DEV float magnitude(const uint4* h, const uint4* W, int vecs, int token) {
   float s = 0.f;
+#pragma unroll 4
   for (int c = threadIdx.x & 31; c < vecs; c += 32) {
     const uint4 a = __ldg(h + c), b = __ldg(W + (int64_t)token * vecs + c);
     const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
@@ -448,173 +534,182 @@ struct Best {
   }
 };
 
-// A row's likeliest tokens from the groups' two largest scores. In most rows these tell: the scores that count stand further apart
-// than what the products' rounding may have moved them by, and no group's second may be among them. Where they do not, what may
-// count is scored again, first by sums in fp32, what they leave by sums in 64 bits.
-constexpr int kTopWarps = 4;
-__global__ void __launch_bounds__(kTopWarps * 32)
-k_stats_top(int64_t N, int V, int d, int top, int halves, int64_t pad, float inv_tau, const uint4* __restrict__ hc,
-            const uint4* __restrict__ W, const int* __restrict__ pos, const int* __restrict__ tok,
-            const float* __restrict__ lse2, const double* __restrict__ base, const float2* __restrict__ pairs,
-            const float2* __restrict__ part, const float* __restrict__ own, float* __restrict__ top_logp,
-            int64_t* __restrict__ top_tokens) {
-  const int lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * kTopWarps + (threadIdx.x >> 5);
+// A row's likeliest tokens from the groups' two largest scores, a warp per row. In most rows these tell: the scores that count stand
+// further apart than what the products' rounding may have moved them by, and no group's second may be among them. Where they do
+// not (one row in six at 50304 x 768 and 8 tokens), the block's warps together score what may count again, first by sums in fp32,
+// what these leave by sums in 64 bits.
+constexpr int kTopWarps = 8, kItems = 1024;
+struct TopArgs {
+  int64_t N, pad;
+  int V, d, top, halves;
+  float inv_tau;
+  const uint4 *hc, *W;
+  const int *pos, *tok;
+  const float* lse2;
+  const double* base;
+  const float2 *pairs, *part;
+  const float* own;
+  float* top_logp;
+  int64_t* top_tokens;
+};
+// A slow row, as its warp leaves it to the block.
+struct Open {
+  int row;                                       // -1: none
+  float slack;
+  double low;
+};
+// The most that a score may be whose note is v: the note's low bits, and the rounding.
+ASRN_DEV double above(float v, float slack) { return (double)v + fabsf(v) * 0x1p-15f + slack; }
+
+template <int Each>
+__global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
+  __shared__ Open open[kTopWarps];
+  __shared__ double scores[kTopWarps][kMaxTop];
+  __shared__ int tokens[kTopWarps][kMaxTop];
+  __shared__ int items[kItems], count;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, top = f.top, vecs = f.d / 8;
+  const int64_t i = (int64_t)blockIdx.x * kTopWarps + wid;
   wait_previous();
   let_next();
-  if (i >= N) return;
-  const int r = pos[i];
-  const bool bad = r >= 0 && !(fabsf(lse2[r]) < INFINITY);
-  if (r < 0 || bad) {
+  auto write = [&](int64_t at, float logp, int token) {
     if (lane < top) {
-      top_logp[i * top + lane] = bad ? NAN : 0.f;
-      top_tokens[i * top + lane] = -1;
-    }
-    return;
-  }
-  const int vecs = d / 8, y = tok[r];
-  const uint4* h = hc + (int64_t)r * vecs;
-  const float2* mine = pairs + (int64_t)r * halves;
-  // The groups in the order of their largest scores, equal ones by their numbers: each lane holds the next of its own, those
-  // after `last`.
-  uint32_t key = 0, last = 0xffffffffu;
-  int group = -1, last_group = -1;
-  auto find = [&]() {
-    key = 0;
-    group = 0x7fffffff;
-#pragma unroll 8
-    for (int g = lane; g < halves; g += 32) {
-      const float v = __ldg(&mine[g].x);
-      const uint32_t o = v <= -3e38f ? 0u : order_of(v);
-      if ((o < last || (o == last && g > last_group)) && o > key) {
-        key = o;
-        group = g;
-      }
+      f.top_logp[at * top + lane] = logp;
+      f.top_tokens[at * top + lane] = token;
     }
   };
-  auto next = [&](float2& pair) {                // the next group, -1: none left
-    const uint32_t most = __reduce_max_sync(0xffffffffu, key);
-    if (most == 0) return -1;
-    const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
-    last = most;
-    last_group = g;
-    pair = __ldg(mine + g);
-    if (group == g && key == most) find();
-    __syncwarp();
-    return g;
-  };
-  auto column = [&](int g, float v) { return g * 128 + (int)(__float_as_uint(v) & 127u); };
-
-  // The first `top` groups by lane, and the one after them.
-  find();
-  float2 pair = make_float2(kNothing, kNothing), held = pair;
-  int held_group = 0, have = 0, after = -1;
-  while (true) {
-    after = next(pair);
-    if (after < 0 || have == top) break;
-    if (lane == have) {
-      held = pair;
-      held_group = after;
-    }
-    ++have;
-  }
-  const int held_column = column(held_group, held.x);
-  Best best;
-  const float sure = lane < have ? __ldg(&part[(int64_t)held_group * pad + r].x) : 0.f;
-  for (int q = 0; q < have; ++q)
-    best.put(__shfl_sync(0xffffffffu, sure, q), __shfl_sync(0xffffffffu, held_column, q));
-  if (y >= 0) best.put(own[r], y);
-  // Twice what the sums in fp32, 16 products at a time, may be off by, for two scores, with twice the magnitudes of the best one.
-  const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
-  const float size = likeliest < V ? magnitude(h, W, vecs, likeliest) : 0.f, slack = (float)(d / 16 + 2) * 0x1p-21f * size;
-  // The most that a score may be whose note is v: the note's low bits, and the rounding.
-  auto above = [&](float v) { return (double)v + fabsf(v) * 0x1p-15f + slack; };
-  auto worst = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
-  {
-    const double low = worst(), next_score = __shfl_down_sync(0xffffffffu, best.score, 1);
-    const double below = lane < 31 ? next_score : -INFINITY;
-    const bool close = lane < top && (best.score - below <= slack || best.token >= V);
-    const bool hidden = lane < have && held.y > -3e38f && above(held.y) >= low;
-    const bool more = after >= 0 && above(pair.x) >= low;
-    if (!more && !__any_sync(0xffffffffu, close || hidden) && !(top == 32 && y >= 0)) {
-      if (lane < top) {
-        top_logp[i * top + lane] = (float)(best.score * inv_tau - base[r]);
-        top_tokens[i * top + lane] = best.token;
+  Open left{-1, 0.f, 0.0};
+  const int r = i < f.N ? f.pos[i] : -1;
+  if (r < 0) {
+    if (i < f.N) write(i, 0.f, -1);
+  } else if (!(fabsf(f.lse2[r]) < INFINITY)) {
+    write(i, NAN, -1);
+  } else {
+    const int y = f.tok[r];
+    const float own = y >= 0 ? f.own[r] : 0.f;
+    const double base = f.base[r];
+    const uint4* h = f.hc + (int64_t)r * vecs;
+    Groups<Each> groups(f.pairs + (int64_t)r * f.halves, f.halves);
+    // The first `top` groups by lane, and the one after them.
+    float2 pair = make_float2(kNothing, kNothing), held = pair;
+    int held_group = 0, have = 0, after = -1;
+    while (true) {
+      after = groups.next(pair);
+      if (after < 0 || have == top) break;
+      if (lane == have) {
+        held = pair;
+        held_group = after;
       }
-      return;
+      ++have;
     }
-  }
-
-  if (size == 0.f) {                             // a row of zeros: all scores are 0
-    uint32_t any = 0;
-    for (int c = lane; c < vecs; c += 32) {
-      const uint4 a = __ldg(h + c);
-      any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
-    }
-    if (!__any_sync(0xffffffffu, any)) {
-      if (lane < top) {
-        top_logp[i * top + lane] = (float)-base[r];
-        top_tokens[i * top + lane] = lane;
-      }
-      return;
-    }
-  }
-
-  best = Best{};
-  double s[4];
-  for (int q = 0; q < have; q += 4) {
-    int t[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = __shfl_sync(0xffffffffu, held_column, min(q + j, have - 1));
-    dots(h, W, vecs, t, 4, s);
-    for (int j = 0; j < 4 && q + j < have; ++j) best.put(s[j], t[j]);
-  }
-  if (y >= 0) {
-    const int t[4] = {y};
-    dots(h, W, vecs, t, 1, s);
-    best.put(s[0], y);
-  }
-  // All columns of a group but one and the target's.
-  auto expand = [&](int g, int except) {
-    const int end = min(V, g * 128 + 128);
-    for (int c = g * 128; c < end; c += 8) {
-      const float about = dots8(h, W, vecs, c, end - 1);
-      const int mine_c = c + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
-      const double low = worst();
-      unsigned count = __ballot_sync(0xffffffffu, !(lane & 3) && mine_c < end && mine_c != except && mine_c != y &&
-                                                      (double)about + slack >= low);
-      while (count) {
-        int t[4] = {}, n = 0;
-        while (count && n < 4) {
-          t[n++] = __shfl_sync(0xffffffffu, mine_c, __ffs(count) - 1);
-          count &= count - 1;
+    Best best;
+    const float sure = lane < have ? __ldg(&f.part[(int64_t)held_group * f.pad + r].x) : 0.f;
+    const int column = held_group * 128 + (int)(__float_as_uint(held.x) & 127u);
+    for (int q = 0; q < have; ++q) best.put(__shfl_sync(0xffffffffu, sure, q), __shfl_sync(0xffffffffu, column, q));
+    if (y >= 0) best.put(own, y);
+    // Twice what the sums in fp32, 16 products at a time, may be off by, for two scores, with twice the magnitudes of the best one.
+    const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
+    const float size = likeliest < f.V ? magnitude(h, f.W, vecs, likeliest) : 0.f;
+    const float slack = (float)(f.d / 16 + 2) * 0x1p-21f * size;
+    const double low = __shfl_sync(0xffffffffu, best.score, top - 1), then = __shfl_down_sync(0xffffffffu, best.score, 1);
+    const bool close = lane < top && (best.score - (lane < 31 ? then : -INFINITY) <= slack || best.token >= f.V);
+    const bool hidden = lane < have && held.y > -3e38f && above(held.y, slack) >= low;
+    const bool more = (after >= 0 && above(pair.x, slack) >= low) || (top == 32 && y >= 0);
+    if (!more && !__any_sync(0xffffffffu, close || hidden)) {
+      write(i, (float)(best.score * f.inv_tau - base), best.token);
+    } else {
+      uint32_t any = size != 0.f;
+      if (!any)
+        for (int c = lane; c < vecs; c += 32) {
+          const uint4 a = __ldg(h + c);
+          any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
         }
-        dots(h, W, vecs, t, n, s);
-        for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
-      }
+      if (__any_sync(0xffffffffu, any))
+        left = Open{r, slack, low};
+      else                                       // a row of zeros: all scores are 0
+        write(i, (float)-base, lane);
     }
-  };
-  for (int q = 0; q < have; ++q) {
-    const float v = __shfl_sync(0xffffffffu, held.y, q);
-    const int g = __shfl_sync(0xffffffffu, held_group, q), c = __shfl_sync(0xffffffffu, held_column, q);
-    if (v > -3e38f && above(v) >= worst()) expand(g, c);
   }
-  for (; after >= 0 && above(pair.x) >= worst(); after = next(pair)) {
-    const int t[4] = {column(after, pair.x)};
-    dots(h, W, vecs, t, 1, s);
-    best.put(s[0], t[0]);
-    if (pair.y > -3e38f && above(pair.y) >= worst()) expand(after, t[0]);
-  }
-  // Scores of minus infinity are in no group: the smallest numbers that are left.
-  int l = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < V));
-  for (int c = 0; l < top && c < V; ++c) {
-    if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
-    if (lane == l) best.token = c;
-    ++l;
-  }
-  if (lane < top) {
-    top_logp[i * top + lane] = (float)(best.score * inv_tau - base[r]);
-    top_tokens[i * top + lane] = best.token;
+  if (lane == 0) open[wid] = left;
+  __syncthreads();
+
+  for (int q = 0; q < kTopWarps; ++q) {
+    const Open o = open[q];
+    if (o.row < 0) continue;
+    const int y = f.tok[o.row];
+    const uint4* h = f.hc + (int64_t)o.row * vecs;
+    const float2* mine = f.pairs + (int64_t)o.row * f.halves;
+    Best best;
+    double s[4];
+    int t[4] = {}, n = 0;
+    auto exact = [&]() {
+      if (n == 0) return;
+      dots(h, f.W, vecs, t, n, s);
+      for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
+      n = 0;
+    };
+    if (y >= 0 && wid == 0) t[n++] = y;
+    // What may count, as items for the warps: a group's largest alone (its column, the sign bit set), or the group by
+    // sixteenths of 8 columns. In one go, or where that is too much by so many groups that their sixteenths fit.
+    int window = f.halves;
+    for (int g0 = 0; g0 < f.halves;) {
+      if (threadIdx.x == 0) count = 0;
+      __syncthreads();
+      for (int g = g0 + threadIdx.x; g < min(g0 + window, f.halves); g += kTopWarps * 32) {
+        const float2 pair = __ldg(mine + g);
+        if (!(pair.x > -3e38f && above(pair.x, o.slack) >= o.low)) continue;
+        const bool whole = pair.y > -3e38f && above(pair.y, o.slack) >= o.low;
+        const int at = atomicAdd(&count, whole ? 16 : 1);
+        if (!whole) {
+          if (at < kItems) items[at] = (int)(0x80000000u | (uint32_t)(g * 128 + (int)(__float_as_uint(pair.x) & 127u)));
+        } else {
+          for (int j = 0; j < 16; ++j)
+            if (at + j < kItems) items[at + j] = g * 16 + j;
+        }
+      }
+      __syncthreads();
+      const int all = count;
+      if (all > kItems) {                        // only with the first window
+        window = kItems / 16;
+        __syncthreads();
+        continue;
+      }
+      for (int k = wid; k < all; k += kTopWarps) {
+        const int item = items[k];
+        if (item < 0) {
+          t[n++] = item & 0x7fffffff;
+          if (n == 4) exact();
+          continue;
+        }
+        const int c = item * 8, end = min(f.V, c + 8);
+        if (c >= f.V) continue;
+        const float about = dots8(h, f.W, vecs, c, end - 1);
+        const int own = c + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
+        unsigned set = __ballot_sync(0xffffffffu, !(lane & 3) && own < end && own != y && (double)about + o.slack >= o.low);
+        for (; set; set &= set - 1) {
+          t[n++] = __shfl_sync(0xffffffffu, own, __ffs(set) - 1);
+          if (n == 4) exact();
+        }
+      }
+      __syncthreads();
+      g0 += window;
+    }
+    exact();
+    scores[wid][lane] = best.score;
+    tokens[wid][lane] = best.token;
+    __syncthreads();
+    if (wid == 0) {
+      for (int w = 1; w < kTopWarps; ++w)
+        for (int j = 0; j < top && scores[w][j] != -INFINITY; ++j) best.put(scores[w][j], tokens[w][j]);
+      // Scores of minus infinity are in no group: the smallest numbers that are left.
+      int l = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < f.V));
+      for (int c = 0; l < top && c < f.V; ++c) {
+        if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
+        if (lane == l) best.token = c;
+        ++l;
+      }
+      write((int64_t)blockIdx.x * kTopWarps + q, (float)(best.score * f.inv_tau - f.base[o.row]), best.token);
+    }
+    __syncthreads();
   }
 }
 
@@ -698,7 +793,7 @@ int few(int64_t V, int d, const void* hc, const void* weight, const int* count, 
 template <bool Top>
 int scan(int64_t N, int64_t V, int d, const void* hc, const void* weight, const gemm::Shape& sh,
          const typename Scan<Top>::Params& p, cudaStream_t s) {
-  if (N > kFewRows) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
+  if (N > kFewRows || N * V > kFewScores) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
   return N <= 8    ? few<1, Top>(V, d, hc, weight, sh.m_dev, p, s)
          : N <= 16 ? few<2, Top>(V, d, hc, weight, sh.m_dev, p, s)
          : N <= 32 ? few<4, Top>(V, d, hc, weight, sh.m_dev, p, s)
@@ -765,9 +860,9 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
                               base, logp, entropy)))
     return st;
   if (!top) return ASRN_OK;
-  return launch_next(k_stats_top, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, N, (int)V, d, top, halves, pad256(N),
-                     inv_tau, reinterpret_cast<const uint4*>(hc), reinterpret_cast<const uint4*>(weight), pos, tok, lse2, base,
-                     pairs, part, own, top_logp, top_tokens);
+  const TopArgs f{N, pad256(N), (int)V, d, top, halves, inv_tau, reinterpret_cast<const uint4*>(hc),
+                  reinterpret_cast<const uint4*>(weight), pos, tok, lse2, base, pairs, part, own, top_logp, top_tokens};
+  return launch_next(halves <= 512 ? k_stats_top<16> : k_stats_top<0>, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, f);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,

@@ -25,7 +25,7 @@ namespace {
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
 constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
 constexpr int64_t kTwiceRows = 512;
-constexpr int64_t kFewRows = 64;
+constexpr int64_t kFewRows = 64, kFewValues = (int64_t)1 << 20;
 
 ASRN_DEV uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -424,7 +424,7 @@ int asrn_linear_forward(int64_t N, int32_t d, int32_t n, const void* x, const vo
     return ASRN_ERR_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Rest p{reinterpret_cast<const __nv_bfloat16*>(bias), residual, act, residual ? res_type : kNone, act && slope};
-  if (N <= kFewRows)
+  if (N <= kFewRows && N * n <= kFewValues)
     return N <= 8    ? few<1>(N, d, n, x, weight, p, y, slope, s)
            : N <= 16 ? few<2>(N, d, n, x, weight, p, y, slope, s)
            : N <= 32 ? few<4>(N, d, n, x, weight, p, y, slope, s)
