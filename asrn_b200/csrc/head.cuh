@@ -84,6 +84,7 @@ k_head_gather(int64_t N, int64_t V, int d, const __nv_bfloat16* __restrict__ h, 
   __shared__ int at[kGatherRows];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int64_t i0 = (int64_t)blockIdx.x * kGatherRows;
+  let_next();                                            // launched after all that was before it: nothing else is waited for
   int before = tokens || tid ? 0 : (int)i0;
   const int64_t from = !tokens ? i0 : counts ? i0 / kCountRows * kCountRows : 0;
   if (counts)

@@ -8,9 +8,8 @@
 //                  exp(s - m) (s - m), and where the likeliest tokens are wanted the two largest scores, the largest with its
 //                  column in the low 7 bits; the target is in none of the sums
 //   k_stats_few    the same for few rows
-//   k_stats_join   a row's sums joined: logp, H
-//   k_stats_top    a warp per row: the groups of 128 columns by their largest scores, for as long as one may hold one of the
-//                  likeliest tokens. Where the products' rounding leaves their order open, what may count is scored again
+//   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups of 128 columns by their largest scores, for as
+//                  long as one may hold one of the likeliest tokens. Where the products' rounding leaves their order open, what may count is scored again
 //                  from h and W with a sum in 64 bits: the order of the tokens is that of their exact scores, equal ones
 //                  in the order of their numbers.
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
@@ -44,7 +43,7 @@ StatsSaved stats_saved(int64_t N, int64_t d) {
 __host__ ASRN_DEV int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
 
 struct StatsWs {
-  size_t counts, top, part, ent, base, pairs, total;
+  size_t counts, top, part, second, total;
 };
 
 StatsWs stats_ws(int64_t N, int64_t V, int top) {
@@ -54,10 +53,8 @@ StatsWs stats_ws(int64_t N, int64_t V, int top) {
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
   w.top = take(P * 4);
-  w.part = take(halves * P * 8);
-  w.ent = take(halves * P * 4);
-  w.base = take(top ? P * 8 : 0);
-  w.pairs = take(top ? halves * P * 8 : 0);
+  w.part = take(halves * P * 16);
+  w.second = take(top ? halves * P * 4 : 0);
   w.total = o;
   return w;
 }
@@ -74,10 +71,8 @@ template <bool Top> struct Scan {
     const int* tok;
     float k;                               // log2(e) / tau
     float* top;                            // the targets' unscaled scores
-    float2* part;                          // m, S: [2 n-tiles][pad]
-    float* ent;                            // T log2(e): the same
-    float2* pairs;                         // the two largest: [pad][2 n-tiles]
-    int64_t pad;
+    float4* part;                          // m, S, T log2(e) and the largest: [rows][2 n-tiles]
+    float* second;                         // the second largest: the same
   };
   const Params& p;
   int row, V, y, at, halves;
@@ -153,9 +148,8 @@ template <bool Top> struct Scan {
   }
   ASRN_DEV void finish() {
     if (!on) return;
-    p.part[at * p.pad + row] = make_float2(m <= kNothing ? -INFINITY : m, s);
-    p.ent[at * p.pad + row] = t;
-    if (Top) p.pairs[(int64_t)row * halves + at] = make_float2(first, second);
+    p.part[(int64_t)row * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, t, first);
+    if (Top) p.second[(int64_t)row * halves + at] = second;
   }
 };
 
@@ -246,128 +240,67 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
       }
     }
     if (lane == 0) {
-      p.part[at * p.pad + r] = make_float2(m <= kNothing ? -INFINITY : m, s);
-      p.ent[at * p.pad + r] = e;
-      if (Top) p.pairs[(int64_t)r * halves + at] = make_float2(first, second);
+      p.part[(int64_t)r * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, e, first);
+      if (Top) p.second[(int64_t)r * halves + at] = second;
     }
   }
 }
 
-// Block = 32 positions x 16 warps over the halves of the vocabulary's tiles, 8 at a time. A position's void when its target is
-// outside the vocabulary or its scores have no log-sum-exp (an infinity or a NaN among them): NaN in all its results.
-constexpr int kJoinWarps = 16;
-__global__ void __launch_bounds__(kJoinWarps * 32)
-k_stats_join(int64_t N, int halves, int64_t pad, float k, float inv_tau, const int* __restrict__ pos,
-             const int* __restrict__ tok, const float* __restrict__ top, const float2* __restrict__ part,
-             const float* __restrict__ ent, float* __restrict__ lse2, float* __restrict__ kept_logp,
-             float* __restrict__ kept_ent, double* __restrict__ base, float* __restrict__ logp, float* __restrict__ entropy) {
-  __shared__ float sh[3][kJoinWarps][32];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
-  wait_previous();
-  let_next();
-  const int r = i < N ? pos[i] : -1;
+// Sums relative to a maximum: S = sum exp(s - m), T = log2(e) sum exp(s - m) (s - m).
+struct Sums {
   float m = -INFINITY, s = 0.f, t = 0.f;
-  auto join = [&](const float* qm, const float* qs, const float* qt, int n) {   // n of at most 8
-    float now = m;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) now = j < n ? fmaxf(now, qm[j]) : now;
-    if (now == -INFINITY) {                      // no score yet but NaNs, which the maxima pass over: the sums hold them
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n) s += qs[j];
+  ASRN_DEV void add(float m2, float s2, float t2, float k) {
+    const float now = fmaxf(m, m2);
+    if (now == -INFINITY) {                        // no score yet but NaNs, which the maxima pass over: the sums hold them
+      s += s2;
       return;
     }
-    float step = fmaxf((m - now) * k, kLeast), f = exp2_fast((m - now) * k);
-    t = f * fmaf(step, s, t);
-    s *= f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) {
-        step = fmaxf((qm[j] - now) * k, kLeast);
-        f = exp2_fast((qm[j] - now) * k);
-        t = fmaf(f, fmaf(step, qs[j], qt[j]), t);
-        s = fmaf(qs[j], f, s);
-      }
+    const float x1 = (m - now) * k, x2 = (m2 - now) * k, f1 = exp2_fast(x1), f2 = exp2_fast(x2);
+    t = fmaf(f2, fmaf(fmaxf(x2, kLeast), s2, t2), f1 * fmaf(fmaxf(x1, kLeast), s, t));
+    s = fmaf(s2, f2, s * f1);
     m = now;
-  };
-  if (r >= 0)
-    for (int j0 = wid; j0 < halves; j0 += 8 * kJoinWarps) {
-      float qm[8], qs[8], qt[8];
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j * kJoinWarps < halves) {
-          const int64_t at = (j0 + j * kJoinWarps) * pad + r;
-          const float2 q = __ldg(part + at);
-          qm[j] = q.x;
-          qs[j] = q.y;
-          qt[j] = __ldg(ent + at);
-          n = j + 1;
-        }
-      join(qm, qs, qt, n);
-    }
-  sh[0][wid][lane] = m;
-  sh[1][wid][lane] = s;
-  sh[2][wid][lane] = t;
-  __syncthreads();
-  if (wid || i >= N) return;
-  m = -INFINITY;
-  s = t = 0.f;
-  for (int w = 0; w < kJoinWarps; w += 8) {
-    float qm[8], qs[8], qt[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      qm[j] = sh[0][w + j][lane];
-      qs[j] = sh[1][w + j][lane];
-      qt[j] = sh[2][w + j][lane];
-    }
-    join(qm, qs, qt, 8);
   }
-  if (r < 0) {
-    if (logp) logp[i] = 0.f;
-    entropy[i] = 0.f;
-    return;
-  }
-  t *= kLn2;                                     // the sums so far: without the target
-  const int y = tok[r];
-  float lp = 0.f, H, l2, off;                    // lse = from / tau + off
-  float from = m;
-  if (y < 0) {
-    off = logf(s);
-    H = off - t / s;
-    l2 = m * k + log2f(s);
-  } else {
-    const float own = top[r], x = (own - m) * inv_tau;
-    if (s == 0.f) {
+};
+
+// What a row's sums (without the target's score) give. A row is void when its target is outside the vocabulary or its scores have no
+// finite log of their sum of exponentials (an infinity or a NaN among them): NaN in all its results.
+struct Row {
+  float lp, H, l2;                                 // logp, entropy, log2 of the sum of exponentials
+  double base;                                     // log of it
+  ASRN_DEV Row(int y, float own, const Sums& q, float k, float inv_tau) : lp(0.f) {
+    const float t = q.t * kLn2;
+    float from = q.m, off;                         // base = from / tau + off
+    if (y < 0) {
+      off = logf(q.s);
+      H = off - t / q.s;
+      l2 = q.m * k + log2f(q.s);
+    } else if (q.s == 0.f) {
       lp = H = own * 0.f;
       off = 0.f;
       from = own;
       l2 = own * k;
-    } else if (x > 0.f) {
-      const float f = expf(-x), a = s * f;
-      lp = -log1pf(a);
-      H = -lp - f * (t - fminf(x, -kLeast) * s) / (1.f + a);
-      off = -lp;
-      from = own;
-      l2 = own * k - lp * kLog2e;
     } else {
-      const float e = expf(x), all = s + e;
-      off = logf(all);
-      lp = x - off;
-      H = off - (t + e * fmaxf(x, kLeast)) / all;
-      l2 = m * k + log2f(all);
+      const float x = (own - q.m) * inv_tau;
+      if (x > 0.f) {
+        const float f = expf(-x), a = q.s * f;
+        lp = -log1pf(a);
+        H = -lp - f * (t - fminf(x, -kLeast) * q.s) / (1.f + a);
+        off = -lp;
+        from = own;
+        l2 = own * k - lp * kLog2e;
+      } else {
+        const float e = expf(x), all = q.s + e;
+        off = logf(all);
+        lp = x - off;
+        H = off - (t + e * fmaxf(x, kLeast)) / all;
+        l2 = q.m * k + log2f(all);
+      }
     }
+    if (y == -1 || !(fabsf(l2) < INFINITY)) lp = H = l2 = NAN;
+    H = H < 0.f ? 0.f : H;                         // what the rounding of two equal terms leaves
+    base = (double)from * inv_tau + off;
   }
-  if (y == -1 || !(fabsf(l2) < INFINITY)) lp = H = l2 = NAN;
-  H = H < 0.f ? 0.f : H;                         // what the rounding of two equal terms leaves
-  if (logp) logp[i] = lp;
-  entropy[i] = H;
-  lse2[r] = l2;
-  kept_logp[r] = lp;
-  kept_ent[r] = H;
-  if (base) base[r] = (double)from * inv_tau + off;
-}
+};
 
 // A noted score as a number that orders as it does, its low 7 bits 0; 0: none.
 ASRN_DEV uint32_t order_of(float v) {
@@ -378,13 +311,14 @@ ASRN_DEV uint32_t order_of(float v) {
 // A row's groups in the order of their largest scores, equal ones by their numbers. Each lane holds the next of its own; up to
 // 32 Each groups all of them, in registers.
 template <int Each> struct Groups {
-  const float2* pairs;
+  const float4* part;
+  const float* second;
   uint32_t key[Each], best;                      // a group's order, its place among the lane's in the low bits, the first's larger
-  ASRN_DEV Groups(const float2* p, int groups) : pairs(p), best(0) {
+  ASRN_DEV Groups(const float4* p, const float* q, int groups) : part(p), second(q), best(0) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int j = 0; j < Each; ++j) {
-      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].x)) : 0u;
+      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].w)) : 0u;
       key[j] = o ? o | (uint32_t)(Each - 1 - j) : 0u;
       best = max(best, key[j]);
     }
@@ -396,7 +330,7 @@ template <int Each> struct Groups {
     const int j = Each - 1 - (int)(best & 127u);
     const int mine = (best & ~127u) == most ? lane + 32 * j : 0x7fffffff;
     const int g = (int)__reduce_min_sync(0xffffffffu, (unsigned)mine);
-    pair = __ldg(pairs + g);
+    pair = make_float2(__ldg(&part[g].w), __ldg(second + g));
     if (mine == g) {
       best = 0;
 #pragma unroll
@@ -411,16 +345,20 @@ template <int Each> struct Groups {
 };
 // Any number of groups: read again after each.
 template <> struct Groups<0> {
-  const float2* pairs;
+  const float4* part;
+  const float* second;
   int groups, group, last_group;
   uint32_t key, last;
-  ASRN_DEV Groups(const float2* p, int n) : pairs(p), groups(n), last_group(-1), last(0xffffffffu) { find(); }
+  ASRN_DEV Groups(const float4* p, const float* q, int n)
+      : part(p), second(q), groups(n), last_group(-1), last(0xffffffffu) {
+    find();
+  }
   ASRN_DEV void find() {
     key = 0;
     group = 0x7fffffff;
 #pragma unroll 8
     for (int g = threadIdx.x & 31; g < groups; g += 32) {
-      const uint32_t o = order_of(__ldg(&pairs[g].x));
+      const uint32_t o = order_of(__ldg(&part[g].w));
       if ((o < last || (o == last && g > last_group)) && o > key) {
         key = o;
         group = g;
@@ -433,7 +371,7 @@ template <> struct Groups<0> {
     const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
     last = most;
     last_group = g;
-    pair = __ldg(pairs + g);
+    pair = make_float2(__ldg(&part[g].w), __ldg(second + g));
     if (group == g && key == most) find();
     __syncwarp();
     return g;
@@ -539,30 +477,29 @@ struct Best {
 // not (one row in six at 50304 x 768 and 8 tokens), the block's warps together score what may count again, first by sums in fp32,
 // what these leave by sums in 64 bits.
 constexpr int kTopWarps = 8, kItems = 1024;
-struct TopArgs {
-  int64_t N, pad;
+struct RowArgs {
+  int64_t N;
   int V, d, top, halves;
-  float inv_tau;
+  float k, inv_tau;
   const uint4 *hc, *W;
   const int *pos, *tok;
-  const float* lse2;
-  const double* base;
-  const float2 *pairs, *part;
-  const float* own;
-  float* top_logp;
+  const float4* part;
+  const float *second, *own;
+  float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass
+  float *logp, *entropy, *top_logp;              // by positions; logp may be null
   int64_t* top_tokens;
 };
 // A slow row, as its warp leaves it to the block.
 struct Open {
   int row;                                       // -1: none
   float slack;
-  double low;
+  double low, base;
 };
 // The most that a score may be whose note is v: the note's low bits, and the rounding.
 ASRN_DEV double above(float v, float slack) { return (double)v + fabsf(v) * 0x1p-15f + slack; }
 
 template <int Each>
-__global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
+__global__ void __launch_bounds__(kTopWarps * 32) k_stats_rows(const RowArgs f) {
   __shared__ Open open[kTopWarps];
   __shared__ double scores[kTopWarps][kMaxTop];
   __shared__ int tokens[kTopWarps][kMaxTop];
@@ -577,18 +514,55 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
       f.top_tokens[at * top + lane] = token;
     }
   };
-  Open left{-1, 0.f, 0.0};
+  Open left{-1, 0.f, 0.0, 0.0};
   const int r = i < f.N ? f.pos[i] : -1;
+  const int y = r >= 0 ? f.tok[r] : -1;
+  const float own = y >= 0 ? f.own[r] : 0.f;
+  float lp = 0.f, H = 0.f, l2 = 0.f;
+  double base = 0.0;
+  if (r >= 0) {                                  // the row's sums: by lanes, then the lanes'
+    Sums q;
+    for (int g0 = 0; g0 < f.halves; g0 += 128) {
+      float4 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int g = g0 + j * 32 + lane;
+        p[j] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        if (g < f.halves) p[j] = __ldg(f.part + (int64_t)r * f.halves + g);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q.add(p[j].x, p[j].y, p[j].z, f.k);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      q.add(__shfl_down_sync(0xffffffffu, q.m, o), __shfl_down_sync(0xffffffffu, q.s, o), __shfl_down_sync(0xffffffffu, q.t, o),
+            f.k);
+    q.m = __shfl_sync(0xffffffffu, q.m, 0);
+    q.s = __shfl_sync(0xffffffffu, q.s, 0);
+    q.t = __shfl_sync(0xffffffffu, q.t, 0);
+    const Row row(y, own, q, f.k, f.inv_tau);
+    lp = row.lp;
+    H = row.H;
+    l2 = row.l2;
+    base = row.base;
+    if (lane == 0) {
+      f.lse2[r] = l2;
+      f.kept_logp[r] = lp;
+      f.kept_ent[r] = H;
+    }
+  }
+  if (lane == 0 && i < f.N) {
+    if (f.logp) f.logp[i] = lp;
+    f.entropy[i] = H;
+  }
+  if (top == 0) return;
   if (r < 0) {
     if (i < f.N) write(i, 0.f, -1);
-  } else if (!(fabsf(f.lse2[r]) < INFINITY)) {
+  } else if (!(fabsf(l2) < INFINITY)) {
     write(i, NAN, -1);
   } else {
-    const int y = f.tok[r];
-    const float own = y >= 0 ? f.own[r] : 0.f;
-    const double base = f.base[r];
     const uint4* h = f.hc + (int64_t)r * vecs;
-    Groups<Each> groups(f.pairs + (int64_t)r * f.halves, f.halves);
+    Groups<Each> groups(f.part + (int64_t)r * f.halves, f.second + (int64_t)r * f.halves, f.halves);
     // The first `top` groups by lane, and the one after them.
     float2 pair = make_float2(kNothing, kNothing), held = pair;
     int held_group = 0, have = 0, after = -1;
@@ -602,7 +576,7 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
       ++have;
     }
     Best best;
-    const float sure = lane < have ? __ldg(&f.part[(int64_t)held_group * f.pad + r].x) : 0.f;
+    const float sure = lane < have ? __ldg(&f.part[(int64_t)r * f.halves + held_group].x) : 0.f;
     const int column = held_group * 128 + (int)(__float_as_uint(held.x) & 127u);
     for (int q = 0; q < have; ++q) best.put(__shfl_sync(0xffffffffu, sure, q), __shfl_sync(0xffffffffu, column, q));
     if (y >= 0) best.put(own, y);
@@ -624,7 +598,7 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
           any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
         }
       if (__any_sync(0xffffffffu, any))
-        left = Open{r, slack, low};
+        left = Open{r, slack, low, base};
       else                                       // a row of zeros: all scores are 0
         write(i, (float)-base, lane);
     }
@@ -637,7 +611,7 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
     if (o.row < 0) continue;
     const int y = f.tok[o.row];
     const uint4* h = f.hc + (int64_t)o.row * vecs;
-    const float2* mine = f.pairs + (int64_t)o.row * f.halves;
+    const int64_t at_row = (int64_t)o.row * f.halves;
     Best best;
     double s[4];
     int t[4] = {}, n = 0;
@@ -655,7 +629,7 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
       if (threadIdx.x == 0) count = 0;
       __syncthreads();
       for (int g = g0 + threadIdx.x; g < min(g0 + window, f.halves); g += kTopWarps * 32) {
-        const float2 pair = __ldg(mine + g);
+        const float2 pair = make_float2(__ldg(&f.part[at_row + g].w), __ldg(f.second + at_row + g));
         if (!(pair.x > -3e38f && above(pair.x, o.slack) >= o.low)) continue;
         const bool whole = pair.y > -3e38f && above(pair.y, o.slack) >= o.low;
         const int at = atomicAdd(&count, whole ? 16 : 1);
@@ -707,7 +681,7 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_top(const TopArgs f) {
         if (lane == l) best.token = c;
         ++l;
       }
-      write((int64_t)blockIdx.x * kTopWarps + q, (float)(best.score * f.inv_tau - f.base[o.row]), best.token);
+      write((int64_t)blockIdx.x * kTopWarps + q, (float)(best.score * f.inv_tau - o.base), best.token);
     }
     __syncthreads();
   }
@@ -841,28 +815,24 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   const int *tok = reinterpret_cast<int*>(S + sv.head.tok), *pos = reinterpret_cast<int*>(S + sv.head.pos);
   const void* hc = S + sv.head.hc;
   float* lse2 = reinterpret_cast<float*>(S + sv.head.lse2);
-  double* base = top ? reinterpret_cast<double*>(W + ws.base) : nullptr;
   const int halves = halves_of(V);
   gemm::Shape sh{};
   sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = reinterpret_cast<int*>(S + sv.head.count); sh.group = 16;
   sh.status = status;
   const float inv_tau = 1.f / tau, k = kLog2e * inv_tau;
   float* own = reinterpret_cast<float*>(W + ws.top);
-  float2* part = reinterpret_cast<float2*>(W + ws.part);
-  float* ent = reinterpret_cast<float*>(W + ws.ent);
-  float2* pairs = reinterpret_cast<float2*>(W + ws.pairs);
+  float4* part = reinterpret_cast<float4*>(W + ws.part);
+  float* second = reinterpret_cast<float*>(W + ws.second);
   if (top)
-    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
+    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, second}, s);
   else
-    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, ent, pairs, pad256(N)}, s);
-  if (st || (st = launch_next(k_stats_join, (N + 31) / 32, kJoinWarps * 32, s, N, halves, pad256(N), k, inv_tau, pos, tok, own,
-                              part, ent, lse2, reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent),
-                              base, logp, entropy)))
-    return st;
-  if (!top) return ASRN_OK;
-  const TopArgs f{N, pad256(N), (int)V, d, top, halves, inv_tau, reinterpret_cast<const uint4*>(hc),
-                  reinterpret_cast<const uint4*>(weight), pos, tok, lse2, base, pairs, part, own, top_logp, top_tokens};
-  return launch_next(halves <= 512 ? k_stats_top<16> : k_stats_top<0>, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, f);
+    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, second}, s);
+  if (st) return st;
+  const RowArgs f{N, (int)V, d, top, halves, k, inv_tau, reinterpret_cast<const uint4*>(hc),
+                  reinterpret_cast<const uint4*>(weight), pos, tok, part, second, own, lse2,
+                  reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent), logp, entropy, top_logp,
+                  top_tokens};
+  return launch_next(halves <= 512 ? k_stats_rows<16> : k_stats_rows<0>, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, f);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
