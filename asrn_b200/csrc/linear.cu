@@ -32,18 +32,20 @@ ASRN_DEV uint32_t half2_of(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Of two values: act(a) in place, the slopes as fp16. Infinite a give the limits (products with what vanishes take |a| held
-// to 200), NaN stays.
-template <int Act> ASRN_DEV uint32_t activate(float& a0, float& a1) {
+// Of two values: act(a) in place, the slopes as fp16. Large: infinite a give the limits (products with what vanishes take |a| held
+// to kLarge), NaN stays; else |a| <= kLarge or NaN.
+constexpr float kLarge = 200.f;
+template <int Act, bool Large> ASRN_DEV uint32_t activate(float& a0, float& a1) {
   using namespace gemm;
   if constexpr (Act == kGelu) {
     F2 e, q;
     tails(a0, a1, e, q);
-    const float m0 = fminf(fabsf(a0), 200.f), m1 = fminf(fabsf(a1), 200.f);
+    const float m0 = Large ? fminf(fabsf(a0), kLarge) : fabsf(a0), m1 = Large ? fminf(fabsf(a1), kLarge) : fabsf(a1);
+    const F2 held = Large ? F2(copysignf(m0, a0), copysignf(m1, a1)) : F2(a0, a1);
     float h0, h1, s0, s1;
     fma2(q, F2(-1.f), F2(0.5f)).get(h0, h1);                                     // 1/2 - q
     const F2 cdf = add2(F2(copysignf(h0, a0), copysignf(h1, a1)), F2(0.5f));
-    fma2(mul2(F2(copysignf(m0, a0), copysignf(m1, a1)), F2(0.39894228040143268f)), e, cdf).get(s0, s1);
+    fma2(mul2(held, F2(0.39894228040143268f)), e, cdf).get(s0, s1);
     fma2(F2(-m0, -m1), q, F2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))).get(a0, a1);
     return half2_of(s0, s1);
   } else if constexpr (Act == kSilu) {
@@ -51,10 +53,10 @@ template <int Act> ASRN_DEV uint32_t activate(float& a0, float& a1) {
     float s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float low = fmaxf(*a[i], -200.f);
+      const float low = Large ? fmaxf(*a[i], -kLarge) : *a[i];
       float p = 1.f + exp2_fast(*a[i] * -1.4426950408889634f);
       asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(p));
-      s[i] = p * fmaf(fminf(low, 200.f), 1.f - p, 1.f);
+      s[i] = p * fmaf(Large ? fminf(low, kLarge) : low, 1.f - p, 1.f);
       *a[i] = low * p;
     }
     return half2_of(s[0], s[1]);
@@ -65,18 +67,21 @@ template <int Act> ASRN_DEV uint32_t activate(float& a0, float& a1) {
     return s;
   }
 }
-// The same for 2 n values.
+template <int Act, bool Large, int N> ASRN_DEV void activate_all(float* v, uint32_t* s) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = activate<Act, Large>(v[2 * i], v[2 * i + 1]);
+}
+// The same for 2 N values.
 template <int N> ASRN_DEV void activate(int act, float* v, uint32_t* s) {
-  if (act == kGelu) {
+  float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = activate<kGelu>(v[2 * i], v[2 * i + 1]);
-  } else if (act == kSilu) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = activate<kSilu>(v[2 * i], v[2 * i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = activate<kRelu>(v[2 * i], v[2 * i + 1]);
-  }
+  for (int i = 0; i < 2 * N; ++i) most = fmaxf(most, fabsf(v[i]));
+  if (act == kRelu)
+    activate_all<kRelu, true, N>(v, s);
+  else if (most > kLarge)
+    act == kGelu ? activate_all<kGelu, true, N>(v, s) : activate_all<kSilu, true, N>(v, s);
+  else
+    act == kGelu ? activate_all<kGelu, false, N>(v, s) : activate_all<kSilu, false, N>(v, s);
 }
 
 // What follows the product.

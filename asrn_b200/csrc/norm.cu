@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(threads_of(T), T == 256 ? 2 : 1) k_norm_back(c
 
 // The same for rows that a warp holds, eight values a load (d <= 1024): each warp's next row comes to shared memory by
 // asynchronous copies while it works on the one before, which costs no registers beside the columns' sums.
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kStages = 2;
 ASRN_DEV void copy_row(uint8_t* to, const void* from, int64_t at, int bytes, int lane) {
   const char* p = reinterpret_cast<const char*>(from) + at;
   for (int b = lane * 16; b < bytes; b += 512)
@@ -304,14 +304,14 @@ ASRN_DEV Raw<8> staged(const uint8_t* p, int c, int t) {
 }
 constexpr int row_bytes(int d, int t) { return d * (t == kBf16 ? 2 : 4); }
 size_t staged_bytes(int d, int st, int yt, bool ds) {
-  return (size_t)kWarps * 2 * (row_bytes(d, st) * (1 + ds) + row_bytes(d, yt));
+  return (size_t)kWarps * kStages * (row_bytes(d, st) * (1 + ds) + row_bytes(d, yt));
 }
 template <int ST, int YT, int C>
 __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_norm_back_rows(const Backward f) {
   extern __shared__ __align__(16) uint8_t room[];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int sb = row_bytes(f.d, ST), yb = row_bytes(f.d, YT), stage = sb * (f.ds ? 2 : 1) + yb;
-  uint8_t* mine = room + wid * 2 * stage;
+  uint8_t* mine = room + wid * kStages * stage;
   auto fetch = [&](int64_t row, int turn) {
     if (row < f.rows) {
       uint8_t* to = mine + turn * stage;
@@ -325,14 +325,15 @@ __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_nor
   const float inv = 1.f / (float)f.d;
   const int64_t step = (int64_t)gridDim.x * kWarps, row0 = (int64_t)blockIdx.x * kWarps + wid;
   int turn = 0;
-  fetch(row0, 0);
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) fetch(row0 + j * step, j);
   float2 next = row0 < f.rows ? __ldg(f.stats + row0) : make_float2(0.f, 0.f);
-  for (int64_t row = row0; row < f.rows; row += step, turn ^= 1) {
+  for (int64_t row = row0; row < f.rows; row += step, turn = turn + 1 == kStages ? 0 : turn + 1) {
     __syncwarp();                                        // the room's last row has been read by every lane
-    fetch(row + step, turn ^ 1);
+    fetch(row + (kStages - 1) * step, turn == 0 ? kStages - 1 : turn - 1);
     const float2 mk = next;
     if (row + step < f.rows) next = __ldg(f.stats + row + step);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
     const uint8_t* at = mine + turn * stage;
     float h[C * 8], g[C * 8], s1 = 0.f, s2 = 0.f;
@@ -473,7 +474,7 @@ template <int V, int ST, int YT, int C, int T> int run(const Backward& f, cudaSt
 }
 template <int ST, int YT, int C> int run_rows(const Backward& f, cudaStream_t s) {
   auto kernel = k_norm_back_rows<ST, YT, C>;
-  constexpr size_t most = (size_t)kWarps * 2 * (row_bytes(C * 256, ST) * 2 + row_bytes(C * 256, YT));
+  constexpr size_t most = (size_t)kWarps * kStages * (row_bytes(C * 256, ST) * 2 + row_bytes(C * 256, YT));
   static std::atomic<uint64_t> ready{0};                 // devices that know the kernel's shared memory
   int dev = 0;
   if (most > 48 << 10) {
