@@ -5,9 +5,10 @@ blocks -> ln_f -> tied head. Mirror of asrn.nucleo.ModeloASRN / BloqueLocal / cr
 The ASRN layers are asrn_b200.ASRNLayer (CUDA kernels of libasrn_b200.so). Under bf16 autocast on CUDA each local
 block runs as the fused asrn_local_block (an LN kernel and three persistent tcgen05 GEMMs with the conv, GELU, bias and
 residual folded in); in fp32 the local blocks, and in every mode the embedding and head, are PyTorch ops.
-logprobs() gives log probabilities of tokens without the (B, L, V) logits (asrn_b200.finetune.head_logprobs), and
-checkpoint='8bits' trains with the local blocks' MLPs keeping their activations in 8 bits (asrn_b200.finetune.mlp8);
-both serve bf16 autocast.
+logprobs() gives log probabilities of tokens without the (B, L, V) logits (asrn_b200.finetune.head_logprobs), stats() these
+with entropies and likeliest tokens (head_stats), checkpoint='8bits' trains with the local blocks' MLPs keeping their
+activations in 8 bits (mlp8), and fundido=True runs the local blocks' norms, sums and MLPs where the fused block does not serve
+(training, other widths) as layer_norm and linear; all of these serve bf16 autocast.
 """
 import math
 
@@ -15,7 +16,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .finetune import head_logprobs, mlp8
+from .finetune import HeadStats, head_logprobs, head_stats, layer_norm, linear, mlp8
 from .layer import ASRNLayer
 
 
@@ -30,6 +31,12 @@ def _sin_ganchos(m):
                 'forward' in vars(m))
 
 
+def _norma_de_serie(m):
+    """True for a norm over the last dimension with weight and bias whose call is nn.LayerNorm's forward and nothing else."""
+    return (type(m) is nn.LayerNorm and len(m.normalized_shape) == 1 and m.normalized_shape[0] <= 16384 and
+            m.weight is not None and m.bias is not None and m.weight.dtype == m.bias.dtype == torch.float32 and _sin_ganchos(m))
+
+
 class BloqueLocal(nn.Module):
     """Causal local context: dense convolution over the k-1 previous tokens and the current one, then an MLP
     (asrn/nucleo.py:969-1014, the default mezcla='conv')."""
@@ -37,6 +44,8 @@ class BloqueLocal(nn.Module):
     # True: the MLP keeps its activations in 8 bits for the backward pass. Of the class: blocks that were pickled before
     # it was there have none of their own.
     activaciones_8bits = False
+    # True: norms, residual sums and the MLP as layer_norm and linear. Of the class, as above.
+    fundido = False
 
     def __init__(self, d, k=4, ff=128, dropout=0.0, mezcla='conv', memoria_max=1024):
         super().__init__()
@@ -52,6 +61,8 @@ class BloqueLocal(nn.Module):
     def forward(self, h):
         if self._fused_ok(h):
             return self._fused(h)
+        if self.fundido and self._fundido_ok(h):
+            return self._fundido(h)
         z = self.ln1(h)
         c = F.gelu(self.conv(F.pad(z.transpose(1, 2), (self.k - 1, 0))).transpose(1, 2))
         h = h + self.drop(c)
@@ -60,18 +71,43 @@ class BloqueLocal(nn.Module):
             return h + self.drop(mlp8(u, self.ff[0].weight, self.ff[0].bias, self.ff[2].weight, self.ff[2].bias))
         return h + self.drop(self.ff(u))
 
-    def _mlp8_ok(self, u):
-        """mlp8 serves training under bf16 autocast on CUDA and widths that are multiples of 8, for the MLP as it was built:
-        modules put in its place, and modules with hooks or a forward of their own, are called."""
-        if not (u.is_cuda and torch.is_grad_enabled() and torch.is_autocast_enabled('cuda') and
+    def _fundido(self, h):
+        """The block by layer_norm and linear: what the norms and the MLP's products round to bf16 are their results alone,
+        and the sums stay in h's fp32."""
+        z = layer_norm(h, self.ln1.weight, self.ln1.bias, eps=self.ln1.eps, dtype=torch.bfloat16)
+        c = self.drop(F.gelu(self.conv(F.pad(z.transpose(1, 2), (self.k - 1, 0))).transpose(1, 2)))
+        u, h = layer_norm(c, self.ln2.weight, self.ln2.bias, residual=h, eps=self.ln2.eps, dtype=torch.bfloat16)
+        if self.activaciones_8bits and self._mlp8_ok(u):
+            return h + self.drop(mlp8(u, self.ff[0].weight, self.ff[0].bias, self.ff[2].weight, self.ff[2].bias))
+        a = linear(u, self.ff[0].weight, self.ff[0].bias, 'gelu')
+        if self.training and self.drop.p > 0:
+            return h + self.drop(linear(a, self.ff[2].weight, self.ff[2].bias))
+        return linear(a, self.ff[2].weight, self.ff[2].bias, residual=h)
+
+    def _fundido_ok(self, h):
+        """layer_norm and linear serve bf16 autocast on CUDA, an fp32 h and widths that are multiples of 8, for the modules as
+        they were built (as _mlp8_ok)."""
+        if not (h.is_cuda and h.dtype == torch.float32 and torch.is_autocast_enabled('cuda') and
                 torch.get_autocast_dtype('cuda') == torch.bfloat16):
             return False
+        return (self._mlp_as_built() and _norma_de_serie(self.ln1) and _norma_de_serie(self.ln2))
+
+    def _mlp_as_built(self):
+        """The MLP's modules are as they were built, of widths that are multiples of 8."""
         modules = [self.ff, *self.ff]
         if [type(m) for m in modules] != [nn.Sequential, nn.Linear, nn.GELU, nn.Linear]:
             return False
         d, ff = self.conv.in_channels, self.ff[0].out_features
         return (d % 8 == 0 and ff % 8 == 0 and self.ff[0].bias is not None and self.ff[2].bias is not None and
                 self.ff[1].approximate == 'none' and all(map(_sin_ganchos, modules)))
+
+    def _mlp8_ok(self, u):
+        """mlp8 serves training under bf16 autocast on CUDA and widths that are multiples of 8, for the MLP as it was built:
+        modules put in its place, and modules with hooks or a forward of their own, are called."""
+        if not (u.is_cuda and torch.is_grad_enabled() and torch.is_autocast_enabled('cuda') and
+                torch.get_autocast_dtype('cuda') == torch.bfloat16):
+            return False
+        return self._mlp_as_built()
 
     def _fused_ok(self, h):
         """The fused CUDA block (asrn_local_block) serves bf16 autocast on CUDA, fp32 h, no dropout at work, and the
@@ -135,10 +171,14 @@ def _escalar_profundo(modulo, n_capas):
 
 class ModeloASRN(nn.Module):
     """Same arguments and module names as the reference model (asrn/nucleo.py:1054-1078). checkpoint='8bits': in
-    training under bf16 autocast the local blocks' MLPs keep their activations in 8 bits."""
+    training under bf16 autocast the local blocks' MLPs keep their activations in 8 bits. fundido=True: under bf16
+    autocast the local blocks' norms, residual sums and MLPs, and ln_f, run as layer_norm and linear (in training, and at
+    widths that the fused inference block does not take)."""
+
+    fundido = False                                      # of the class, as BloqueLocal's
 
     def __init__(self, V, d=64, n_capas=2, largo_cada=2, ff=None, k=4, init_profundo=None, checkpoint=False,
-                 dropout=0.0, mezcla='conv', memoria_max=1024, protecciones=None, **opciones_capa):
+                 dropout=0.0, mezcla='conv', memoria_max=1024, protecciones=None, fundido=False, **opciones_capa):
         super().__init__()
         assert n_capas >= 2 and largo_cada >= 1
         assert V <= 2 ** 24, 'token signatures are exact up to 2**24 tokens'
@@ -146,7 +186,7 @@ class ModeloASRN(nn.Module):
                            mezcla=mezcla, memoria_max=memoria_max, opciones_capa=dict(opciones_capa))
         if isinstance(checkpoint, str) and checkpoint != '8bits':
             raise ValueError(f"checkpoint is False, True or '8bits'; got {checkpoint!r}")
-        self.n_capas, self.checkpoint = n_capas, checkpoint
+        self.n_capas, self.checkpoint, self.fundido = n_capas, checkpoint, bool(fundido)
         self.init_profundo = n_capas >= 8 if init_profundo is None else bool(init_profundo)
         self.pos_largo = [i for i in range(n_capas - 1) if i % largo_cada == 0]
         self.emb = nn.Embedding(V, d)
@@ -160,6 +200,7 @@ class ModeloASRN(nn.Module):
                                      for _ in self.pos_largo])
         for b in self.bloques:
             b.activaciones_8bits = checkpoint == '8bits'
+            b.fundido = self.fundido
         if self.init_profundo:
             with torch.no_grad():
                 for b in self.bloques:
@@ -183,9 +224,7 @@ class ModeloASRN(nn.Module):
         if not 0 < temperatura <= 1e30:
             raise ValueError('logprobs: temperatura has to be positive')
         h = self.estado(x)
-        if h.is_cuda and torch.is_autocast_enabled('cuda') and h.shape[-1] % 8 == 0 and \
-                torch.get_autocast_dtype('cuda') == torch.bfloat16 and type(self.head) is nn.Linear and \
-                self.head.bias is None and _sin_ganchos(self.head):
+        if self._cabeza_ok(h):
             return head_logprobs(h, self.head.weight, objetivos, temperatura)
         lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
         V = lp.shape[-1]                                 # an index outside would stop the GPU's context
@@ -193,8 +232,50 @@ class ModeloASRN(nn.Module):
         lp = lp * torch.where(objetivos < V, 1.0, math.nan)
         return torch.where(objetivos >= 0, lp, torch.zeros_like(lp))
 
+    def _cabeza_ok(self, h):
+        """The head's kernels serve bf16 autocast on CUDA, for a head that is its weight alone."""
+        return (h.is_cuda and torch.is_autocast_enabled('cuda') and h.shape[-1] % 8 == 0 and
+                torch.get_autocast_dtype('cuda') == torch.bfloat16 and type(self.head) is nn.Linear and
+                self.head.bias is None and _sin_ganchos(self.head))
+
+    def stats(self, x, objetivos=None, temperatura=1.0, top=0):
+        """The distributions softmax(logits / temperatura) at the positions of x (B, L) by their statistics, as
+        head_stats gives them: HeadStats(logp, entropy, top_logp, top_tokens), float32 (B, L) and (B, L, top). objetivos
+        (B, L): tokens whose log probabilities are wanted (logp is None without); a negative one leaves its position out. For
+        a loss with an entropy term, and for the alternatives to a model's tokens. Under bf16 autocast the (B, L, V) logits
+        are not kept; the fp32 model, and one whose head was replaced or has hooks, takes the same from its logits."""
+        if objetivos is not None and objetivos.shape != x.shape:
+            raise ValueError(f'objetivos must be (B, L) = {tuple(x.shape)}; got {tuple(objetivos.shape)}')
+        if not 0 < temperatura <= 1e30:
+            raise ValueError('stats: temperatura has to be positive')
+        V = self.head.weight.shape[0] if isinstance(self.head, nn.Linear) else None
+        if not 0 <= top <= (32 if V is None else min(32, V)):
+            raise ValueError(f'stats: top is 0 to 32 and at most the vocabulary; got {top}')
+        h = self.estado(x)
+        if self._cabeza_ok(h):
+            return head_stats(h, self.head.weight, objetivos, temperatura, top)
+        lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
+        entropy = -(lp.exp() * lp.clamp(min=-1e4)).sum(-1)       # 0 for p = 0
+        logp = top_logp = top_tokens = None
+        out = entropy.isnan()
+        on = torch.ones_like(out) if objetivos is None else objetivos >= 0
+        zero = torch.zeros_like(entropy)
+        if objetivos is not None:
+            out = out | (objetivos >= lp.shape[-1])
+            logp = lp.gather(-1, objetivos.clamp(0, lp.shape[-1] - 1).unsqueeze(-1)).squeeze(-1)
+            logp = torch.where(on, torch.where(out, math.nan, logp), zero)
+        if top:
+            with torch.no_grad():
+                top_logp, top_tokens = lp.sort(dim=-1, descending=True, stable=True)
+                bad = out.unsqueeze(-1)
+                top_logp = torch.where(bad, math.nan, top_logp[..., :top])
+                top_logp = torch.where(on.unsqueeze(-1), top_logp, torch.zeros_like(top_logp))
+                top_tokens = torch.where(on.unsqueeze(-1) & ~bad, top_tokens[..., :top], -1)
+        return HeadStats(logp, torch.where(on, torch.where(out, math.nan, entropy), zero), top_logp, top_tokens)
+
     def estado(self, x):
-        """The state that the head reads: ln_f of the last block's output (B, L, d)."""
+        """The state that the head reads: ln_f of the last block's output (B, L, d), in fp32 (fundido under bf16 autocast: in
+        bf16, as the head takes it)."""
         if self.emb.weight.dtype in (torch.float16, torch.bfloat16):
             raise ValueError(f'the model has {self.emb.weight.dtype} weights: ASRN needs float32 weights; use '
                              'torch.autocast for bf16 (asrn/nucleo.py:1025-1032)')
@@ -208,6 +289,9 @@ class ModeloASRN(nn.Module):
             if i in self.pos_largo:
                 h = self.largos[j](E, h, x, ngram=ng)
                 j += 1
+        if self.fundido and _norma_de_serie(self.ln_f) and h.is_cuda and h.dtype == torch.float32 and \
+                torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16:
+            return layer_norm(h, self.ln_f.weight, self.ln_f.bias, eps=self.ln_f.eps, dtype=torch.bfloat16)
         return self.ln_f(h)
 
     def _ngram_shared(self):
@@ -278,12 +362,12 @@ def _migrate_streak(pesos):
     return pesos
 
 
-def cargar(archivo, dispositivo=None, confiar=False, protecciones=None, checkpoint=False):
+def cargar(archivo, dispositivo=None, confiar=False, protecciones=None, checkpoint=False, fundido=False):
     """Load a model written by guardar() here or by the reference's guardar() / entrenar() (its v83 to v89 files;
     asrn/nucleo.py:2110-2133, asrn/__init__.py:73-75). Read with torch.load(weights_only=True) unless confiar=True.
     Weights missing from files older than v87 keep their initial (neutral) values, as the reference does; any other
-    missing or unexpected weight is an error. The file does not say how the model is trained: `checkpoint` does, as in
-    crear_modelo ('8bits' to tune a trained model with 8-bit activations). Returns the model on `dispositivo` (default:
+    missing or unexpected weight is an error. The file does not say how the model is trained: `checkpoint` and `fundido` do,
+    as in crear_modelo ('8bits' to tune a trained model with 8-bit activations). Returns the model on `dispositivo` (default:
     cuda) in eval mode."""
     import os
     if not os.path.isfile(archivo):
@@ -300,7 +384,7 @@ def cargar(archivo, dispositivo=None, confiar=False, protecciones=None, checkpoi
     c = dict(r['config'])
     m = ModeloASRN(c['V'], c['d'], c['n_capas'], c['largo_cada'], c['ff'], c['k'], init_profundo=False,
                    checkpoint=checkpoint, dropout=c.get('dropout', 0.0), mezcla=c.get('mezcla', 'conv'),
-                   memoria_max=c.get('memoria_max', 1024), protecciones=protecciones, **c['opciones_capa'])
+                   memoria_max=c.get('memoria_max', 1024), protecciones=protecciones, fundido=fundido, **c['opciones_capa'])
     faltan, sobran = m.load_state_dict(_migrate_streak(r['pesos']), strict=False)
     raros = [n for n in faltan if n.rsplit('.', 1)[-1] not in _NEW_IN_V87]
     if sobran or raros:

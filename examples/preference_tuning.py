@@ -2,10 +2,11 @@
 it: log probabilities through the tied head (model.logprobs), the preference and the clipped policy loss, and local
 blocks that keep their activations in 8 bits (checkpoint='8bits').
 
-    python examples/preference_tuning.py [--V 256 --d 64 --pairs 8 --length 128 --steps 20]
+    python examples/preference_tuning.py [--V 256 --d 64 --pairs 8 --length 128 --steps 20 --fused --entropy 0.01]
 
 The prompts are random; a chosen answer repeats its prompt, a rejected one is random. In the second part answers are
-drawn from the model itself and rewarded for each token that the prompt holds.
+drawn from the model itself and rewarded for each token that the prompt holds; with --entropy the answers' entropy is
+rewarded, too (model.stats). --fused trains with layer_norm and linear in the local blocks (fundido=True).
 """
 import argparse
 import os
@@ -45,8 +46,9 @@ def preference_steps(model, optimiser, x, targets, steps):
     return torch.stack(losses).tolist(), float((r.chosen - r.rejected).mean())
 
 
-def policy_steps(model, optimiser, prompt, answers, steps):
-    """One rollout, `steps` updates on it: the reward is the share of the answer's tokens that the prompt holds."""
+def policy_steps(model, optimiser, prompt, answers, steps, entropy=0.0):
+    """One rollout, `steps` updates on it: the reward is the share of the answer's tokens that the prompt holds. entropy: the
+    weight of the mean entropy over the answers' positions in the loss."""
     L0 = prompt.shape[1]
     model.eval()
     with torch.autocast('cuda', dtype=torch.bfloat16):
@@ -62,12 +64,19 @@ def policy_steps(model, optimiser, prompt, answers, steps):
     with torch.no_grad(), torch.autocast('cuda', dtype=torch.bfloat16):
         old = model.logprobs(x, targets)
     losses = []
+    share = -entropy * mask / mask.sum().clamp(min=1)
     for _ in range(steps):
         with torch.autocast('cuda', dtype=torch.bfloat16):
-            logp = model.logprobs(x, targets)
+            if entropy:
+                logp, spread, _, _ = model.stats(x, targets)
+            else:
+                logp = model.logprobs(x, targets)
         r = asrn.policy_loss(logp.detach(), old, advantages, mask, ref_logp=old, kl=0.04)
         optimiser.zero_grad(set_to_none=True)
-        logp.backward(r.grad)
+        if entropy:
+            torch.autograd.backward((logp, spread), (r.grad, share))
+        else:
+            logp.backward(r.grad)
         optimiser.step()
         losses.append(r.loss)
     return torch.stack(losses).tolist(), float(r.kl)
@@ -81,13 +90,16 @@ def main(argv=None):
     a.add_argument('--pairs', type=int, default=8)
     a.add_argument('--length', type=int, default=128)
     a.add_argument('--steps', type=int, default=20)
+    a.add_argument('--entropy', type=float, default=0.0)
+    a.add_argument('--fused', action='store_true')
     a = a.parse_args(argv)
-    model = asrn.create_model(V=a.V, d=a.d, n_capas=a.layers, semilla=0, checkpoint='8bits').cuda().train()
+    model = asrn.create_model(V=a.V, d=a.d, n_capas=a.layers, semilla=0, checkpoint='8bits',
+                              fundido=a.fused).cuda().train()
     optimiser = torch.optim.Adam(model.parameters(), lr=1e-3)
     x, targets = pairs(a.pairs, a.length, a.V, seed=0)
     pref, margin = preference_steps(model, optimiser, x, targets, a.steps)
     print(f'preference loss {pref[0]:.4f} -> {pref[-1]:.4f}, reward margin {margin:.3f}')
-    policy, kl = policy_steps(model, optimiser, x[:a.pairs, :a.length // 2], a.length // 2, a.steps)
+    policy, kl = policy_steps(model, optimiser, x[:a.pairs, :a.length // 2], a.length // 2, a.steps, a.entropy)
     print(f'policy loss {policy[0]:.4f} -> {policy[-1]:.4f}, KL {kl:.4f}')
     return pref, policy
 

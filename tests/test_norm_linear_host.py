@@ -108,3 +108,13 @@ def test_the_packages_errors_and_no_cpu_path():
             (ValueError, lambda: asrn.head_stats(b(3, 8), b(5, 8), temperatura=-1.0))]:
         with pytest.raises(error):
             call()
+
+
+def test_the_models_option():
+    import asrn_b200 as asrn
+    m = asrn.create_model(V=32, d=16, n_capas=2, fundido=True)
+    assert m.fundido and all(b.fundido for b in m.bloques) and 'fundido' not in m.config
+    n = asrn.create_model(V=32, d=16, n_capas=2)
+    assert not n.fundido and not any(b.fundido for b in n.bloques)
+    del m.bloques[0].__dict__['fundido'], m.__dict__['fundido']      # as blocks and models pickled before the option was there
+    assert m.bloques[0].fundido is False and m.fundido is False
