@@ -5,13 +5,13 @@
 // tensor cores at any training size, and by the weight's bytes where rows are few.
 //
 //   k_gemm<Scan>   scores by tiles; each thread keeps of its row's 128 columns the maximum m, S = sum exp(s - m), T = sum
-//                  exp(s - m) (s - m), and where the likeliest tokens are wanted the two largest scores, the largest with its
-//                  column in the low 7 bits; the target is in none of the sums
+//                  exp(s - m) (s - m); the target is in none of the sums. Where the likeliest tokens are wanted, it notes the
+//                  two largest scores of each group of 32 to 128 columns, with their column in the low 7 bits
 //   k_stats_few    the same for few rows
-//   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups of 128 columns by their largest scores, for as
-//                  long as one may hold one of the likeliest tokens. Where the products' rounding leaves their order open, what may count is scored again
-//                  from h and W with a sum in 64 bits: the order of the tokens is that of their exact scores, equal ones
-//                  in the order of their numbers.
+//   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups in the order of their largest notes, for as long as one
+//                  may hold one of the likeliest tokens, whose scores are formed again: by sums in fp32, and where these
+//                  leave the order open by sums in 64 bits. So the order of the tokens is that of their exact scores, equal
+//                  ones by their numbers.
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
 #include "head.cuh"
 #include "products.cuh"
@@ -42,8 +42,14 @@ StatsSaved stats_saved(int64_t N, int64_t d) {
 
 __host__ ASRN_DEV int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
 
+// Columns of a group, as few as leave a row 1024 groups, which a warp holds in registers: of a group that holds two of the likeliest
+// tokens all columns have to be looked at. (With groups of 128 for all, k_stats_rows takes 150 of its 270 us at 16384 x 50304 x 768
+// and 8 tokens for them, 390 of 570 for 20, and at a vocabulary of 1265, of which 20 are wanted, 5.4 ms instead of 0.3.)
+int span_of(int64_t V) { return V <= 32768 ? 32 : V <= 65536 ? 64 : 128; }
+int64_t notes_of(int64_t V) { return (V + span_of(V) - 1) / span_of(V); }
+
 struct StatsWs {
-  size_t counts, top, part, second, total;
+  size_t counts, top, part, notes, total;
 };
 
 StatsWs stats_ws(int64_t N, int64_t V, int top) {
@@ -54,7 +60,7 @@ StatsWs stats_ws(int64_t N, int64_t V, int top) {
   w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
   w.top = take(P * 4);
   w.part = take(halves * P * 16);
-  w.second = take(top ? halves * P * 4 : 0);
+  w.notes = take(top ? (size_t)notes_of(V) * P * 8 : 0);
   w.total = o;
   return w;
 }
@@ -71,8 +77,9 @@ template <bool Top> struct Scan {
     const int* tok;
     float k;                               // log2(e) / tau
     float* top;                            // the targets' unscaled scores
-    float4* part;                          // m, S, T log2(e) and the largest: [rows][2 n-tiles]
-    float* second;                         // the second largest: the same
+    float4* part;                          // m, S, T log2(e): [rows][2 n-tiles]
+    float2* notes;                         // the two largest of each group: [rows][groups]
+    int span, groups;
   };
   const Params& p;
   int row, V, y, at, halves;
@@ -141,19 +148,22 @@ template <bool Top> struct Scan {
         q1 = fmaxf(q1, hi);
       }
       const float lo = fminf(m1[0], m1[1]);
-      const float hi = __uint_as_float(__float_as_uint(fmaxf(m1[0], m1[1])) | (uint32_t)(c & 96));
+      const float hi = __uint_as_float(__float_as_uint(fmaxf(m1[0], m1[1])) | (uint32_t)(c & (p.span - 1)));
       second = fmaxf(max3(second, lo, fminf(first, hi)), fmaxf(m2[0], m2[1]));
       first = fmaxf(first, hi);
+      if (((c + 32) & (p.span - 1)) == 0 || c + 32 >= V) {
+        if (on) p.notes[(int64_t)row * p.groups + c / p.span] = make_float2(first, second);
+        first = second = kNothing;
+      }
     }
   }
   ASRN_DEV void finish() {
     if (!on) return;
-    p.part[(int64_t)row * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, t, first);
-    if (Top) p.second[(int64_t)row * halves + at] = second;
+    p.part[(int64_t)row * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, t, 0.f);
   }
 };
 
-// The same for up to kFewRows rows, bound by the weight's bytes: block = 128 columns (one group), a warp 16 of them and all of K;
+// The same for up to kFewRows rows and kFewScores scores, bound by the weight's bytes: block = 128 columns (one group), a warp 16 of them and all of K;
 // mma.sync from registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a
 // lane takes 8 neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do.
 // Then a warp per row of h over the 128 scores.
@@ -215,7 +225,7 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
       if (c0 + j == y || c0 + j >= V) v[j] = kNothing;
       m = fmaxf(m, v[j]);
       if (Top) {
-        const float u = __uint_as_float((__float_as_uint(v[j]) & ~127u) | (uint32_t)(lane * 4 + j));
+        const float u = __uint_as_float((__float_as_uint(v[j]) & ~127u) | (uint32_t)((lane * 4 + j) & (p.span - 1)));
         second = fmaxf(second, fminf(first, u));
         first = fmaxf(first, u);
       }
@@ -232,34 +242,20 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
     s = warp_sum(s);
     e = warp_sum(e);
     if (Top) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
+      for (int o = 1; o < p.span / 4; o <<= 1) {         // over the lanes of a group
         const float f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
         second = fmaxf(fmaxf(second, s2), fminf(first, f2));
         first = fmaxf(first, f2);
       }
+      if (lane % (p.span / 4) == 0 && c0 < V) p.notes[(int64_t)r * p.groups + c0 / p.span] = make_float2(first, second);
     }
-    if (lane == 0) {
-      p.part[(int64_t)r * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, e, first);
-      if (Top) p.second[(int64_t)r * halves + at] = second;
-    }
+    if (lane == 0) p.part[(int64_t)r * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, e, 0.f);
   }
 }
 
 // Sums relative to a maximum: S = sum exp(s - m), T = log2(e) sum exp(s - m) (s - m).
 struct Sums {
-  float m = -INFINITY, s = 0.f, t = 0.f;
-  ASRN_DEV void add(float m2, float s2, float t2, float k) {
-    const float now = fmaxf(m, m2);
-    if (now == -INFINITY) {                        // no score yet but NaNs, which the maxima pass over: the sums hold them
-      s += s2;
-      return;
-    }
-    const float x1 = (m - now) * k, x2 = (m2 - now) * k, f1 = exp2_fast(x1), f2 = exp2_fast(x2);
-    t = fmaf(f2, fmaf(fmaxf(x2, kLeast), s2, t2), f1 * fmaf(fmaxf(x1, kLeast), s, t));
-    s = fmaf(s2, f2, s * f1);
-    m = now;
-  }
+  float m, s, t;
 };
 
 // What a row's sums (without the target's score) give. A row is void when its target is outside the vocabulary or its scores have no
@@ -311,14 +307,13 @@ ASRN_DEV uint32_t order_of(float v) {
 // A row's groups in the order of their largest scores, equal ones by their numbers. Each lane holds the next of its own; up to
 // 32 Each groups all of them, in registers.
 template <int Each> struct Groups {
-  const float4* part;
-  const float* second;
+  const float2* notes;
   uint32_t key[Each], best;                      // a group's order, its place among the lane's in the low bits, the first's larger
-  ASRN_DEV Groups(const float4* p, const float* q, int groups) : part(p), second(q), best(0) {
+  ASRN_DEV Groups(const float2* p, int groups) : notes(p), best(0) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int j = 0; j < Each; ++j) {
-      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].w)) : 0u;
+      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].x)) : 0u;
       key[j] = o ? o | (uint32_t)(Each - 1 - j) : 0u;
       best = max(best, key[j]);
     }
@@ -330,7 +325,7 @@ template <int Each> struct Groups {
     const int j = Each - 1 - (int)(best & 127u);
     const int mine = (best & ~127u) == most ? lane + 32 * j : 0x7fffffff;
     const int g = (int)__reduce_min_sync(0xffffffffu, (unsigned)mine);
-    pair = make_float2(__ldg(&part[g].w), __ldg(second + g));
+    pair = __ldg(notes + g);
     if (mine == g) {
       best = 0;
 #pragma unroll
@@ -345,12 +340,11 @@ template <int Each> struct Groups {
 };
 // Any number of groups: read again after each.
 template <> struct Groups<0> {
-  const float4* part;
-  const float* second;
+  const float2* notes;
   int groups, group, last_group;
   uint32_t key, last;
-  ASRN_DEV Groups(const float4* p, const float* q, int n)
-      : part(p), second(q), groups(n), last_group(-1), last(0xffffffffu) {
+  ASRN_DEV Groups(const float2* p, int n, uint32_t after = 0xffffffffu, int after_group = -1)
+      : notes(p), groups(n), last_group(after_group), last(after) {
     find();
   }
   ASRN_DEV void find() {
@@ -358,7 +352,7 @@ template <> struct Groups<0> {
     group = 0x7fffffff;
 #pragma unroll 8
     for (int g = threadIdx.x & 31; g < groups; g += 32) {
-      const uint32_t o = order_of(__ldg(&part[g].w));
+      const uint32_t o = order_of(__ldg(&notes[g].x));
       if ((o < last || (o == last && g > last_group)) && o > key) {
         key = o;
         group = g;
@@ -371,15 +365,15 @@ template <> struct Groups<0> {
     const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
     last = most;
     last_group = g;
-    pair = make_float2(__ldg(&part[g].w), __ldg(second + g));
+    pair = __ldg(notes + g);
     if (group == g && key == most) find();
     __syncwarp();
     return g;
   }
 };
 
-// h . w for n of up to four rows of W, products of bf16 exact in fp32, summed in 64 bits.
-ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, int n, double* out) {
+// h . w for four rows of W, products of bf16 exact in fp32, summed in 64 bits.
+ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int (&token)[4], double (&out)[4]) {
   const int lane = threadIdx.x & 31;
   double acc[4] = {};
 #pragma unroll 2
@@ -387,7 +381,7 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, i
     const uint4 a = __ldg(h + c);
     uint4 b[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = __ldg(W + (int64_t)token[j < n ? j : 0] * vecs + c);
+    for (int j = 0; j < 4; ++j) b[j] = __ldg(W + (int64_t)token[j] * vecs + c);
     const uint32_t x[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -402,65 +396,67 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int* token, i
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = warp_sum_d(acc[j]);
 }
-// The same in fp32 for eight rows from `first` on (those past `last` repeat it): the lanes 4 j to 4 j + 3 get row j's, with j's bits
-// in the order 4, 2, 1 of the lane's bits 4, 3, 2.
-ASRN_DEV float dots8(const uint4* h, const uint4* W, int vecs, int first, int last) {
-  const int lane = threadIdx.x & 31;
-  float acc[8] = {};
-  for (int c = lane; c < vecs; c += 32) {
-    const uint4 a = __ldg(h + c);
-    uint4 b[8];
+// The same for sixteen rows of W by mma.sync, in two chains of fp32 sums: lane 4 j gets the rows j (first) and j + 8 (second)
+// that its lanes 4 j to 4 j + 3 name. Loads as in k_stats_few. size: the largest sum |h w| of the first eight.
+struct Pair {
+  float a, b;
+  ASRN_DEV float of(int j) const {               // row j's, for the whole warp
+    const float x = __shfl_sync(0xffffffffu, a, j % 8 * 4), y = __shfl_sync(0xffffffffu, b, j % 8 * 4);
+    return j < 8 ? x : y;
+  }
+};
+// The rows that the lanes name on their way to L2, all at once (the sums below ask for them 128 bytes at a time).
+ASRN_DEV void fetch16(const uint4* W, int vecs, int row_a, int row_b) {
+  const int t = threadIdx.x & 3;
+  const uint4 *wa = W + (int64_t)row_a * vecs, *wb = W + (int64_t)row_b * vecs;
+  for (int k = t * 8; k < vecs; k += 32) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(wa + k));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(wb + k));
+  }
+}
+template <bool Size>
+ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int row_b, float* size) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  const uint4 *wa = W + (int64_t)row_a * vecs, *wb = W + (int64_t)row_b * vecs;
+  float acc[2][4] = {}, mag[4] = {};
+  for (int k = t; k - t < vecs; k += 8) {
+    uint4 a[2], b[2], x[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = __ldg(W + (int64_t)min(first + j, last) * vecs + c);
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+    for (int u = 0; u < 2; ++u) {
+      const int at = min(k + 4 * u, vecs - 1);   // what is past the end meets zeros of h
+      a[u] = __ldg(wa + at);
+      b[u] = __ldg(wb + at);
+      x[u] = __ldg(h + at);                      // the first of eight columns; the others are not looked at
+      if (k + 4 * u >= vecs) x[u] = make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t y[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[j] = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), acc[j]);
-        acc[j] = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), acc[j]);
+    for (int u = 0; u < 2; ++u) {
+      mma16x8(acc[u], a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
+      mma16x8(acc[u], a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
+      if (Size) {
+        constexpr uint32_t m = 0x7fff7fffu;
+        mma16x8(mag, a[u].x & m, 0, a[u].y & m, 0, x[u].x & m, x[u].y & m);
+        mma16x8(mag, a[u].z & m, 0, a[u].w & m, 0, x[u].z & m, x[u].w & m);
       }
     }
   }
-#pragma unroll
-  for (int n = 4, o = 16; n > 0; n >>= 1, o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const float keep = up ? acc[j + n] : acc[j], send = up ? acc[j] : acc[j + n];
-      acc[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-    }
-  }
-  acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 2);
-  return acc[0] + __shfl_xor_sync(0xffffffffu, acc[0], 1);
-}
-// sum |h w| of one row of W.
-ASRN_DEV float magnitude(const uint4* h, const uint4* W, int vecs, int token) {
-  float s = 0.f;
-#pragma unroll 4
-  for (int c = threadIdx.x & 31; c < vecs; c += 32) {
-    const uint4 a = __ldg(h + c), b = __ldg(W + (int64_t)token * vecs + c);
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      s += fabsf(__uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16)) +
-           fabsf(__uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u));
-  }
-  return warp_sum(s);
+  if (Size) *size = warp_max(mag[0]);
+  return Pair{acc[0][0] + acc[1][0], acc[0][2] + acc[1][2]};
 }
 
-// The best so far, lane l the l-th, larger scores first, then smaller numbers.
-struct Best {
-  double score = -INFINITY;
+// The best so far, lane l the l-th, larger scores first, then smaller numbers; and the largest that was not kept.
+template <class T> struct Best {
+  T score = -INFINITY, lost = -INFINITY;
   int token = 0x7fffffff;
-  ASRN_DEV void put(double s, int t) {           // minus infinity is not put in
+  ASRN_DEV void put(T s, int t) {                // minus infinity is not put in
     if (s == -INFINITY) return;
     const int lane = threadIdx.x & 31;
     const unsigned behind = __ballot_sync(0xffffffffu, s > score || (s == score && t < token));
-    const double up = __shfl_up_sync(0xffffffffu, score, 1);
-    const int ut = __shfl_up_sync(0xffffffffu, token, 1);
+    const T out = behind ? __shfl_sync(0xffffffffu, score, 31) : s;
+    lost = lost < out ? out : lost;
     if (!behind) return;
+    const T up = __shfl_up_sync(0xffffffffu, score, 1);
+    const int ut = __shfl_up_sync(0xffffffffu, token, 1);
     const int at = __ffs(behind) - 1;
     if (lane > at) {
       score = up;
@@ -472,74 +468,48 @@ struct Best {
   }
 };
 
-// A row's likeliest tokens from the groups' two largest scores, a warp per row. In most rows these tell: the scores that count stand
-// further apart than what the products' rounding may have moved them by, and no group's second may be among them. Where they do
-// not (one row in six at 50304 x 768 and 8 tokens), the block's warps together score what may count again, first by sums in fp32,
-// what these leave by sums in 64 bits.
-constexpr int kTopWarps = 8, kItems = 1024;
+constexpr int kRowWarps = 4;
 struct RowArgs {
   int64_t N;
-  int V, d, top, halves;
+  int V, d, top, halves, span, groups;
   float k, inv_tau;
   const uint4 *hc, *W;
   const int *pos, *tok;
   const float4* part;
-  const float *second, *own;
+  const float2* notes;
+  const float* own;
   float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass
   float *logp, *entropy, *top_logp;              // by positions; logp may be null
   int64_t* top_tokens;
 };
-// A slow row, as its warp leaves it to the block.
-struct Open {
-  int row;                                       // -1: none
-  float slack;
-  double low, base;
-};
-// The most that a score may be whose note is v: the note's low bits, and the rounding.
-ASRN_DEV double above(float v, float slack) { return (double)v + fabsf(v) * 0x1p-15f + slack; }
 
 template <int Each>
-__global__ void __launch_bounds__(kTopWarps * 32) k_stats_rows(const RowArgs f) {
-  __shared__ Open open[kTopWarps];
-  __shared__ double scores[kTopWarps][kMaxTop];
-  __shared__ int tokens[kTopWarps][kMaxTop];
-  __shared__ int items[kItems], count;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, top = f.top, vecs = f.d / 8;
-  const int64_t i = (int64_t)blockIdx.x * kTopWarps + wid;
+__global__ void __launch_bounds__(kRowWarps * 32, 7) k_stats_rows(const RowArgs f) {
+  const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
+  const int64_t i = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   wait_previous();
   let_next();
-  auto write = [&](int64_t at, float logp, int token) {
-    if (lane < top) {
-      f.top_logp[at * top + lane] = logp;
-      f.top_tokens[at * top + lane] = token;
-    }
-  };
-  Open left{-1, 0.f, 0.0, 0.0};
-  const int r = i < f.N ? f.pos[i] : -1;
-  const int y = r >= 0 ? f.tok[r] : -1;
-  const float own = y >= 0 ? f.own[r] : 0.f;
+  if (i >= f.N) return;
+  const int r = f.pos[i], y = r >= 0 ? f.tok[r] : -1;
   float lp = 0.f, H = 0.f, l2 = 0.f;
   double base = 0.0;
   if (r >= 0) {                                  // the row's sums: by lanes, then the lanes'
-    Sums q;
-    for (int g0 = 0; g0 < f.halves; g0 += 128) {
-      float4 p[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int g = g0 + j * 32 + lane;
-        p[j] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-        if (g < f.halves) p[j] = __ldg(f.part + (int64_t)r * f.halves + g);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q.add(p[j].x, p[j].y, p[j].z, f.k);
+    const float own = y >= 0 ? f.own[r] : 0.f;
+    const float4* part = f.part + (int64_t)r * f.halves;
+    Sums q{-INFINITY, 0.f, 0.f};
+#pragma unroll 4
+    for (int g = lane; g < f.halves; g += 32) q.m = fmaxf(q.m, __ldg(&part[g].x));
+    q.m = warp_max(q.m);
+    const float off = q.m == -INFINITY ? 0.f : q.m;    // no score but NaNs, which the maxima pass over: the sums hold them
+#pragma unroll 4
+    for (int g = lane; g < f.halves; g += 32) {
+      const float4 p = __ldg(part + g);
+      const float x = (p.x - off) * f.k, e = exp2_fast(x);
+      q.t = fmaf(e, fmaf(fmaxf(x, kLeast), p.y, p.z), q.t);
+      q.s = fmaf(e, p.y, q.s);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      q.add(__shfl_down_sync(0xffffffffu, q.m, o), __shfl_down_sync(0xffffffffu, q.s, o), __shfl_down_sync(0xffffffffu, q.t, o),
-            f.k);
-    q.m = __shfl_sync(0xffffffffu, q.m, 0);
-    q.s = __shfl_sync(0xffffffffu, q.s, 0);
-    q.t = __shfl_sync(0xffffffffu, q.t, 0);
+    q.s = warp_sum(q.s);
+    q.t = warp_sum(q.t);
     const Row row(y, own, q, f.k, f.inv_tau);
     lp = row.lp;
     H = row.H;
@@ -551,21 +521,29 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_rows(const RowArgs f) 
       f.kept_ent[r] = H;
     }
   }
-  if (lane == 0 && i < f.N) {
+  if (lane == 0) {
     if (f.logp) f.logp[i] = lp;
     f.entropy[i] = H;
   }
   if (top == 0) return;
-  if (r < 0) {
-    if (i < f.N) write(i, 0.f, -1);
-  } else if (!(fabsf(l2) < INFINITY)) {
-    write(i, NAN, -1);
-  } else {
-    const uint4* h = f.hc + (int64_t)r * vecs;
-    Groups<Each> groups(f.part + (int64_t)r * f.halves, f.second + (int64_t)r * f.halves, f.halves);
-    // The first `top` groups by lane, and the one after them.
-    float2 pair = make_float2(kNothing, kNothing), held = pair;
-    int held_group = 0, have = 0, after = -1;
+  auto write = [&](float logp, int token) {
+    if (lane < top) {
+      f.top_logp[i * top + lane] = logp;
+      f.top_tokens[i * top + lane] = token;
+    }
+  };
+  if (r < 0 || !(fabsf(l2) < INFINITY)) {
+    write(r < 0 ? 0.f : NAN, -1);
+    return;
+  }
+  const uint4* h = f.hc + (int64_t)r * vecs;
+  const float2* notes = f.notes + (int64_t)r * f.groups;
+
+  // The first `top` groups by lane, and the one after them.
+  float2 pair = make_float2(kNothing, kNothing), held = pair;
+  int held_group = 0, have = 0, after = -1;
+  {
+    Groups<Each> groups(notes, f.groups);
     while (true) {
       after = groups.next(pair);
       if (after < 0 || have == top) break;
@@ -575,116 +553,128 @@ __global__ void __launch_bounds__(kTopWarps * 32) k_stats_rows(const RowArgs f) 
       }
       ++have;
     }
-    Best best;
-    const float sure = lane < have ? __ldg(&f.part[(int64_t)r * f.halves + held_group].x) : 0.f;
-    const int column = held_group * 128 + (int)(__float_as_uint(held.x) & 127u);
-    for (int q = 0; q < have; ++q) best.put(__shfl_sync(0xffffffffu, sure, q), __shfl_sync(0xffffffffu, column, q));
-    if (y >= 0) best.put(own, y);
-    // Twice what the sums in fp32, 16 products at a time, may be off by, for two scores, with twice the magnitudes of the best one.
-    const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
-    const float size = likeliest < f.V ? magnitude(h, f.W, vecs, likeliest) : 0.f;
-    const float slack = (float)(f.d / 16 + 2) * 0x1p-21f * size;
-    const double low = __shfl_sync(0xffffffffu, best.score, top - 1), then = __shfl_down_sync(0xffffffffu, best.score, 1);
-    const bool close = lane < top && (best.score - (lane < 31 ? then : -INFINITY) <= slack || best.token >= f.V);
-    const bool hidden = lane < have && held.y > -3e38f && above(held.y, slack) >= low;
-    const bool more = (after >= 0 && above(pair.x, slack) >= low) || (top == 32 && y >= 0);
-    if (!more && !__any_sync(0xffffffffu, close || hidden)) {
-      write(i, (float)(best.score * f.inv_tau - base), best.token);
-    } else {
-      uint32_t any = size != 0.f;
-      if (!any)
-        for (int c = lane; c < vecs; c += 32) {
-          const uint4 a = __ldg(h + c);
-          any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
-        }
-      if (__any_sync(0xffffffffu, any))
-        left = Open{r, slack, low, base};
-      else                                       // a row of zeros: all scores are 0
-        write(i, (float)-base, lane);
-    }
   }
-  if (lane == 0) open[wid] = left;
-  __syncthreads();
+  const int column = held_group * f.span + (int)(__float_as_uint(held.x) & 127u);
 
-  for (int q = 0; q < kTopWarps; ++q) {
-    const Open o = open[q];
-    if (o.row < 0) continue;
-    const int y = f.tok[o.row];
-    const uint4* h = f.hc + (int64_t)o.row * vecs;
-    const int64_t at_row = (int64_t)o.row * f.halves;
-    Best best;
-    double s[4];
-    int t[4] = {}, n = 0;
-    auto exact = [&]() {
-      if (n == 0) return;
-      dots(h, f.W, vecs, t, n, s);
-      for (int j = 0; j < n; ++j) best.put(s[j], t[j]);
-      n = 0;
-    };
-    if (y >= 0 && wid == 0) t[n++] = y;
-    // What may count, as items for the warps: a group's largest alone (its column, the sign bit set), or the group by
-    // sixteenths of 8 columns. In one go, or where that is too much by so many groups that their sixteenths fit.
-    int window = f.halves;
-    for (int g0 = 0; g0 < f.halves;) {
-      if (threadIdx.x == 0) count = 0;
-      __syncthreads();
-      for (int g = g0 + threadIdx.x; g < min(g0 + window, f.halves); g += kTopWarps * 32) {
-        const float2 pair = make_float2(__ldg(&f.part[at_row + g].w), __ldg(f.second + at_row + g));
-        if (!(pair.x > -3e38f && above(pair.x, o.slack) >= o.low)) continue;
-        const bool whole = pair.y > -3e38f && above(pair.y, o.slack) >= o.low;
-        const int at = atomicAdd(&count, whole ? 16 : 1);
-        if (!whole) {
-          if (at < kItems) items[at] = (int)(0x80000000u | (uint32_t)(g * 128 + (int)(__float_as_uint(pair.x) & 127u)));
-        } else {
-          for (int j = 0; j < 16; ++j)
-            if (at + j < kItems) items[at + j] = g * 16 + j;
-        }
-      }
-      __syncthreads();
-      const int all = count;
-      if (all > kItems) {                        // only with the first window
-        window = kItems / 16;
-        __syncthreads();
-        continue;
-      }
-      for (int k = wid; k < all; k += kTopWarps) {
-        const int item = items[k];
-        if (item < 0) {
-          t[n++] = item & 0x7fffffff;
-          if (n == 4) exact();
-          continue;
-        }
-        const int c = item * 8, end = min(f.V, c + 8);
-        if (c >= f.V) continue;
-        const float about = dots8(h, f.W, vecs, c, end - 1);
-        const int own = c + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
-        unsigned set = __ballot_sync(0xffffffffu, !(lane & 3) && own < end && own != y && (double)about + o.slack >= o.low);
-        for (; set; set &= set - 1) {
-          t[n++] = __shfl_sync(0xffffffffu, own, __ffs(set) - 1);
-          if (n == 4) exact();
-        }
-      }
-      __syncthreads();
-      g0 += window;
+  // Their largest, and the target, sixteen at a time.
+  Best<float> best;
+  float size = 0.f;
+  const int count = have + (y >= 0);
+  for (int q = 0; q < count; q += 16) {
+    int rows[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int at = min(q + (lane >> 2) + 8 * j, count - 1), t = __shfl_sync(0xffffffffu, column, max(min(at, have - 1), 0));
+      rows[j] = at < have ? t : y;
     }
-    exact();
-    scores[wid][lane] = best.score;
-    tokens[wid][lane] = best.token;
-    __syncthreads();
-    if (wid == 0) {
-      for (int w = 1; w < kTopWarps; ++w)
-        for (int j = 0; j < top && scores[w][j] != -INFINITY; ++j) best.put(scores[w][j], tokens[w][j]);
-      // Scores of minus infinity are in no group: the smallest numbers that are left.
-      int l = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < f.V));
-      for (int c = 0; l < top && c < f.V; ++c) {
-        if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
-        if (lane == l) best.token = c;
-        ++l;
-      }
-      write((int64_t)blockIdx.x * kTopWarps + q, (float)(best.score * f.inv_tau - o.base), best.token);
+    fetch16(f.W, vecs, rows[0], rows[1]);
+    const Pair about = q ? dots16<false>(h, f.W, vecs, rows[0], rows[1], nullptr)
+                         : dots16<true>(h, f.W, vecs, rows[0], rows[1], &size);
+    for (int j = 0; j < 16 && q + j < count; ++j) {
+      const int t = __shfl_sync(0xffffffffu, j < 8 ? rows[0] : rows[1], j % 8 * 4);
+      best.put(about.of(j), t);
     }
-    __syncthreads();
   }
+  // With twice the magnitudes of the first ones: what a sum here is off by at most, two chains of sums of 16 products, truncated
+  // (`off`), and with that what a note is (one chain), beside its low bits.
+  const float off = (float)(f.d / 32 + 4) * 0x1p-22f * size, slack = (float)(f.d / 16 + 2) * 0x1p-22f * size + off;
+  auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack); };
+  auto low = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
+  // The columns of a group that may count, but for one and the target's.
+  auto expand = [&](int g, int except, auto&& take) {
+    const int begin = g * f.span, end = min(f.V, begin + f.span);
+    for (int c = begin; c < end; c += 16) fetch16(f.W, vecs, min(c + (lane >> 2), end - 1), min(c + (lane >> 2) + 8, end - 1));
+    for (int c = begin; c < end; c += 16) {
+      const int ra = c + (lane >> 2), rb = ra + 8;
+      const Pair about = dots16<false>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1), nullptr);
+      const float least = low() - 2 * off;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int own = j ? rb : ra;
+        const float v = j ? about.b : about.a;
+        unsigned set = __ballot_sync(0xffffffffu, !(lane & 3) && own < end && own != y && own != except && v >= least);
+        for (; set; set &= set - 1) {
+          const int from = __ffs(set) - 1;
+          take(__shfl_sync(0xffffffffu, v, from), __shfl_sync(0xffffffffu, own, from));
+        }
+      }
+    }
+  };
+  auto about_put = [&](float about, int token) { best.put(about, token); };
+  const float lowest = low();
+  unsigned hidden = __ballot_sync(0xffffffffu, lane < have && held.y > -3e38f && above(held.y) >= lowest);
+  for (; hidden; hidden &= hidden - 1) {
+    const int q = __ffs(hidden) - 1;
+    if (above(__shfl_sync(0xffffffffu, held.y, q)) >= low())
+      expand(__shfl_sync(0xffffffffu, held_group, q), __shfl_sync(0xffffffffu, column, q), about_put);
+  }
+  if (after >= 0 && above(pair.x) >= low()) {
+    Groups<0> rest(notes, f.groups, order_of(pair.x), after);
+    for (; after >= 0 && above(pair.x) >= low(); after = rest.next(pair)) {
+      const int c = after * f.span + (int)(__float_as_uint(pair.x) & 127u);
+      best.put(dots16<false>(h, f.W, vecs, c, c, nullptr).of(0), c);
+      if (pair.y > -3e38f && above(pair.y) >= low()) expand(after, c, about_put);
+    }
+  }
+
+  // Scores that stand as near one another as the sums may be off: by sums in 64 bits.
+  const float least = low() - 2 * off, then = __shfl_down_sync(0xffffffffu, best.score, 1);
+  const bool near = lane < top && lane < 31 && best.score - then <= 2 * off;
+  double score = best.score;
+  if (__any_sync(0xffffffffu, near) || best.lost >= least) {
+    double s[4];
+    Best<double> exact;
+    if (best.lost < least) {                     // the few that were kept hold all that may count
+      for (int q = 0; q < 32; q += 4) {
+        int t[4];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float sc = __shfl_sync(0xffffffffu, best.score, q + j);
+          const int tk = __shfl_sync(0xffffffffu, best.token, q + j);
+          t[j] = sc >= least && tk < f.V ? tk : -1;
+          any |= t[j] >= 0;
+        }
+        if (!any) break;                         // in order: none after these
+        const int rows[4] = {max(t[0], 0), max(t[1], 0), max(t[2], 0), max(t[3], 0)};
+        dots(h, f.W, vecs, rows, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t[j] >= 0) exact.put(s[j], t[j]);
+      }
+    } else if (size == 0.f && !__any_sync(0xffffffffu, [&] {
+                 uint32_t any = 0;
+                 for (int c = lane; c < vecs; c += 32) {
+                   const uint4 a = __ldg(h + c);
+                   any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
+                 }
+                 return any;
+               }())) {                           // a row of zeros: all scores are 0
+      exact.score = 0.0;
+      exact.token = lane;
+    } else {                                     // many that are equal or all but that: all of them
+      auto exact_put = [&](float, int token) {
+        const int t[4] = {token, token, token, token};
+        dots(h, f.W, vecs, t, s);
+        exact.put(s[0], token);
+      };
+      if (y >= 0) exact_put(0.f, y);
+      for (int g = 0; g < f.groups; ++g) {
+        const float v = __ldg(&notes[g].x);
+        if (v > -3e38f && above(v) >= low()) expand(g, -1, exact_put);
+      }
+    }
+    best.token = exact.token;
+    score = exact.score;
+  }
+  // Scores of minus infinity are in no group: the smallest numbers that are left.
+  int l = __popc(__ballot_sync(0xffffffffu, lane < top && best.token < f.V));
+  for (int c = 0; l < top && c < f.V; ++c) {
+    if (__any_sync(0xffffffffu, lane < l && best.token == c)) continue;
+    if (lane == l) best.token = c;
+    ++l;
+  }
+  write((float)(score * f.inv_tau - base), best.token);
 }
 
 // dS of one chunk in bf16; the rows that pad the last tile get zeros. With x = log2 p: dS = p (a + b x).
@@ -822,17 +812,18 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   const float inv_tau = 1.f / tau, k = kLog2e * inv_tau;
   float* own = reinterpret_cast<float*>(W + ws.top);
   float4* part = reinterpret_cast<float4*>(W + ws.part);
-  float* second = reinterpret_cast<float*>(W + ws.second);
+  float2* notes = reinterpret_cast<float2*>(W + ws.notes);
+  const int span = span_of(V), groups = (int)notes_of(V);
   if (top)
-    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, second}, s);
+    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   else
-    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, second}, s);
+    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   if (st) return st;
-  const RowArgs f{N, (int)V, d, top, halves, k, inv_tau, reinterpret_cast<const uint4*>(hc),
-                  reinterpret_cast<const uint4*>(weight), pos, tok, part, second, own, lse2,
+  const RowArgs f{N, (int)V, d, top, halves, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
+                  reinterpret_cast<const uint4*>(weight), pos, tok, part, notes, own, lse2,
                   reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent), logp, entropy, top_logp,
                   top_tokens};
-  return launch_next(halves <= 512 ? k_stats_rows<16> : k_stats_rows<0>, (N + kTopWarps - 1) / kTopWarps, kTopWarps * 32, s, f);
+  return launch_next(groups <= 512 ? k_stats_rows<16> : groups <= 1024 ? k_stats_rows<32> : k_stats_rows<0>, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, s, f);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
