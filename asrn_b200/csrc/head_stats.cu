@@ -40,12 +40,13 @@ StatsSaved stats_saved(int64_t N, int64_t d) {
   return w;
 }
 
-__host__ ASRN_DEV int halves_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * 2; }
+// A row's sums are kept by 64 columns, what one thread of the products' epilogue holds of it.
+constexpr int kPart = 64;
+__host__ ASRN_DEV int parts_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * (gemm::kBN / kPart); }
 
-// Columns of a group, as few as leave a row 1024 groups, which a warp holds in registers: of a group that holds two of the likeliest
-// tokens all columns have to be looked at. (With groups of 128 for all, k_stats_rows takes 150 of its 270 us at 16384 x 50304 x 768
-// and 8 tokens for them, 390 of 570 for 20, and at a vocabulary of 1265, of which 20 are wanted, 5.4 ms instead of 0.3.)
-int span_of(int64_t V) { return V <= 32768 ? 32 : V <= 65536 ? 64 : 128; }
+// Columns of a group: of a group that holds two of the likeliest tokens all have to be looked at, so 32 as long as a row's groups
+// stay few enough for a warp to hold in registers.
+int span_of(int64_t V) { return V <= 32768 ? 32 : 64; }
 int64_t notes_of(int64_t V) { return (V + span_of(V) - 1) / span_of(V); }
 
 struct StatsWs {
@@ -54,12 +55,12 @@ struct StatsWs {
 
 StatsWs stats_ws(int64_t N, int64_t V, int top) {
   StatsWs w{};
-  const size_t P = (size_t)pad256(N), halves = (size_t)halves_of(V);
+  const size_t P = (size_t)pad256(N), parts = (size_t)parts_of(V);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes); return at; };
   w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
   w.top = take(P * 4);
-  w.part = take(halves * P * 16);
+  w.part = take(parts * P * 16);
   w.notes = take(top ? (size_t)notes_of(V) * P * 8 : 0);
   w.total = o;
   return w;
@@ -71,22 +72,28 @@ ASRN_DEV float max3(float a, float b, float c) {
   return r;
 }
 
+// What is noted of a group: its largest score, and its second largest with the largest one's column in the low 6 bits.
+ASRN_DEV float2 note_of(float most, float first, float second) {
+  return make_float2(most, __uint_as_float((__float_as_uint(second) & ~63u) | (__float_as_uint(first) & 63u)));
+}
+ASRN_DEV int column_of(float2 note) { return (int)(__float_as_uint(note.y) & 63u); }
+
 template <bool Top> struct Scan {
-  static constexpr int kWarps = 8, kOwn = 1, kTable = 0;
+  static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
   struct Params {
     const int* tok;
     float k;                               // log2(e) / tau
     float* top;                            // the targets' unscaled scores
-    float4* part;                          // m, S, T log2(e): [rows][2 n-tiles]
-    float2* notes;                         // the two largest of each group: [rows][groups]
+    float4* part;                          // m, S, T log2(e): [rows][parts]
+    float2* notes;                         // of each group: [rows][groups]
     int span, groups;
   };
   const Params& p;
-  int row, V, y, at, halves;
+  int row, V, y, at, parts;
   bool on;
-  float m = -INFINITY, s = 0.f, t = 0.f, first = kNothing, second = kNothing;
-  ASRN_DEV Scan(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile& u, int half)
-      : p(pp), row(r), V(sh.N), y(-1), at(u.n * 2 + half), halves((sh.N + gemm::kBN - 1) / gemm::kBN * 2), on(r < rows) {
+  float m = -INFINITY, s = 0.f, t = 0.f, most = kNothing, first = kNothing, second = kNothing;
+  ASRN_DEV Scan(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile& u, int quarter)
+      : p(pp), row(r), V(sh.N), y(-1), at(u.n * (gemm::kBN / kPart) + quarter), parts(parts_of(sh.N)), on(r < rows) {
     if (on) y = p.tok[r];
   }
   template <class O> ASRN_DEV void chunk(float* v, int c, O&, const CUtensorMap*, const CUtensorMap*) {
@@ -105,9 +112,11 @@ template <bool Top> struct Scan {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = i < n ? v[i] : kNothing;
     }
-    float now = m;
+    float here = v[0];
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) now = max3(now, v[i], v[i + 1]);
+    for (int i = 1; i < 31; i += 2) here = max3(here, v[i], v[i + 1]);
+    here = fmaxf(here, v[31]);
+    const float now = fmaxf(m, here);
     const float off = now <= kNothing ? 0.f : now * p.k;
     const gemm::F2 k2(p.k), off2(-off);
     gemm::F2 add(0.f), sum(0.f);
@@ -136,12 +145,12 @@ template <bool Top> struct Scan {
     t = fmaf(f, fmaf(step, s, t), part);
     s = fmaf(s, f, c0 + c1);
     m = now;
-    if constexpr (Top) {                   // two chains of pairs, then one; the chunk's place in the half in the low bits, too
+    if constexpr (Top) {                   // two chains of pairs, then one; the chunk's place in the group in the low bits, too
       float m1[2] = {kNothing, kNothing}, m2[2] = {kNothing, kNothing};
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        const float u0 = __uint_as_float((__float_as_uint(v[i]) & ~127u) | (uint32_t)i);
-        const float u1 = __uint_as_float((__float_as_uint(v[i + 1]) & ~127u) | (uint32_t)(i + 1));
+        const float u0 = __uint_as_float((__float_as_uint(v[i]) & ~63u) | (uint32_t)i);
+        const float u1 = __uint_as_float((__float_as_uint(v[i + 1]) & ~63u) | (uint32_t)(i + 1));
         const float hi = fmaxf(u0, u1), lo = fminf(u0, u1);
         float &q1 = m1[i >> 1 & 1], &q2 = m2[i >> 1 & 1];
         q2 = max3(q2, lo, fminf(q1, hi));
@@ -151,15 +160,16 @@ template <bool Top> struct Scan {
       const float hi = __uint_as_float(__float_as_uint(fmaxf(m1[0], m1[1])) | (uint32_t)(c & (p.span - 1)));
       second = fmaxf(max3(second, lo, fminf(first, hi)), fmaxf(m2[0], m2[1]));
       first = fmaxf(first, hi);
+      most = fmaxf(most, here);
       if (((c + 32) & (p.span - 1)) == 0 || c + 32 >= V) {
-        if (on) p.notes[(int64_t)row * p.groups + c / p.span] = make_float2(first, second);
-        first = second = kNothing;
+        if (on) p.notes[(int64_t)row * p.groups + c / p.span] = note_of(most, first, second);
+        most = first = second = kNothing;
       }
     }
   }
   ASRN_DEV void finish() {
     if (!on) return;
-    p.part[(int64_t)row * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, t, 0.f);
+    p.part[(int64_t)row * parts + at] = make_float4(m <= kNothing ? -INFINITY : m, s, t, 0.f);
   }
 };
 
@@ -213,9 +223,9 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
 #pragma unroll
     for (int j = 0; j < 4; ++j) sh[i * 8 + 2 * t + (j & 1)][wid * 16 + g + (j >> 1) * 8] = acc[i][j];
   __syncthreads();
-  const int halves = halves_of(V), at = blockIdx.x;
+  const int parts = parts_of(V);
   for (int r = wid; r < rows && r < 8 * NT; r += 8) {
-    const int y = p.tok[r], c0 = at * 128 + lane * 4;
+    const int y = p.tok[r], c0 = blockIdx.x * 128 + lane * 4;
     const float4 q = *reinterpret_cast<const float4*>(&sh[r][lane * 4]);
     float v[4] = {q.x, q.y, q.z, q.w};
     float m = -INFINITY, first = kNothing, second = kNothing;
@@ -225,12 +235,24 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
       if (c0 + j == y || c0 + j >= V) v[j] = kNothing;
       m = fmaxf(m, v[j]);
       if (Top) {
-        const float u = __uint_as_float((__float_as_uint(v[j]) & ~127u) | (uint32_t)((lane * 4 + j) & (p.span - 1)));
+        const float u = __uint_as_float((__float_as_uint(v[j]) & ~63u) | (uint32_t)((lane * 4 + j) & (p.span - 1)));
         second = fmaxf(second, fminf(first, u));
         first = fmaxf(first, u);
       }
     }
-    m = warp_max(m);
+    if (Top) {
+      float most = fmaxf(m, kNothing);
+      for (int o = 1; o < p.span / 4; o <<= 1) {         // over the lanes of a group
+        const float f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+        second = fmaxf(fmaxf(second, s2), fminf(first, f2));
+        first = fmaxf(first, f2);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if (lane % (p.span / 4) == 0 && c0 < V) p.notes[(int64_t)r * p.groups + c0 / p.span] = note_of(most, first, second);
+    }
+    // The two parts' sums, each over half of the warp.
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float off = m <= kNothing ? 0.f : m * p.k;
     float s = 0.f, e = 0.f;
 #pragma unroll
@@ -239,17 +261,13 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
       s += f;
       e = fmaf(f, fmaxf(x, kLeast), e);
     }
-    s = warp_sum(s);
-    e = warp_sum(e);
-    if (Top) {
-      for (int o = 1; o < p.span / 4; o <<= 1) {         // over the lanes of a group
-        const float f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
-        second = fmaxf(fmaxf(second, s2), fminf(first, f2));
-        first = fmaxf(first, f2);
-      }
-      if (lane % (p.span / 4) == 0 && c0 < V) p.notes[(int64_t)r * p.groups + c0 / p.span] = make_float2(first, second);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      e += __shfl_xor_sync(0xffffffffu, e, o);
     }
-    if (lane == 0) p.part[(int64_t)r * halves + at] = make_float4(m <= kNothing ? -INFINITY : m, s, e, 0.f);
+    if (lane % 16 == 0)
+      p.part[(int64_t)r * parts + blockIdx.x * 2 + lane / 16] = make_float4(m <= kNothing ? -INFINITY : m, s, e, 0.f);
   }
 }
 
@@ -311,9 +329,12 @@ template <int Each> struct Groups {
   uint32_t key[Each], best;                      // a group's order, its place among the lane's in the low bits, the first's larger
   ASRN_DEV Groups(const float2* p, int groups) : notes(p), best(0) {
     const int lane = threadIdx.x & 31;
+    float v[Each];
+#pragma unroll
+    for (int j = 0; j < Each; ++j) v[j] = __ldg(&p[min(lane + 32 * j, groups - 1)].x);   // no condition: all under way at once
 #pragma unroll
     for (int j = 0; j < Each; ++j) {
-      const uint32_t o = lane + 32 * j < groups ? order_of(__ldg(&p[lane + 32 * j].x)) : 0u;
+      const uint32_t o = lane + 32 * j < groups ? order_of(v[j]) : 0u;
       key[j] = o ? o | (uint32_t)(Each - 1 - j) : 0u;
       best = max(best, key[j]);
     }
@@ -396,6 +417,20 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int (&token)[
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = warp_sum_d(acc[j]);
 }
+// sum |h w| of one row of W.
+ASRN_DEV float magnitude(const uint4* h, const uint4* W, int vecs, int token) {
+  float s = 0.f;
+#pragma unroll 4
+  for (int c = threadIdx.x & 31; c < vecs; c += 32) {
+    const uint4 a = __ldg(h + c), b = __ldg(W + (int64_t)token * vecs + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      s += fabsf(__uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16)) +
+           fabsf(__uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u));
+  }
+  return warp_sum(s);
+}
 // The same for sixteen rows of W by mma.sync, in two chains of fp32 sums: lane 4 j gets the rows j (first) and j + 8 (second)
 // that its lanes 4 j to 4 j + 3 name. Loads as in k_stats_few. size: the largest sum |h w| of the first eight.
 struct Pair {
@@ -405,24 +440,15 @@ struct Pair {
     return j < 8 ? x : y;
   }
 };
-// The rows that the lanes name on their way to L2, all at once (the sums below ask for them 128 bytes at a time).
-ASRN_DEV void fetch16(const uint4* W, int vecs, int row_a, int row_b) {
-  const int t = threadIdx.x & 3;
-  const uint4 *wa = W + (int64_t)row_a * vecs, *wb = W + (int64_t)row_b * vecs;
-  for (int k = t * 8; k < vecs; k += 32) {
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(wa + k));
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(wb + k));
-  }
-}
-template <bool Size>
+template <int U, bool Size>
 ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int row_b, float* size) {
   const int lane = threadIdx.x & 31, t = lane & 3;
   const uint4 *wa = W + (int64_t)row_a * vecs, *wb = W + (int64_t)row_b * vecs;
   float acc[2][4] = {}, mag[4] = {};
-  for (int k = t; k - t < vecs; k += 8) {
-    uint4 a[2], b[2], x[2];
+  for (int k = t; k - t < vecs; k += 4 * U) {
+    uint4 a[U], b[U], x[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int at = min(k + 4 * u, vecs - 1);   // what is past the end meets zeros of h
       a[u] = __ldg(wa + at);
       b[u] = __ldg(wb + at);
@@ -430,9 +456,9 @@ ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int ro
       if (k + 4 * u >= vecs) x[u] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      mma16x8(acc[u], a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
-      mma16x8(acc[u], a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
+    for (int u = 0; u < U; ++u) {
+      mma16x8(acc[u & 1], a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
+      mma16x8(acc[u & 1], a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
       if (Size) {
         constexpr uint32_t m = 0x7fff7fffu;
         mma16x8(mag, a[u].x & m, 0, a[u].y & m, 0, x[u].x & m, x[u].y & m);
@@ -471,7 +497,7 @@ template <class T> struct Best {
 constexpr int kRowWarps = 4;
 struct RowArgs {
   int64_t N;
-  int V, d, top, halves, span, groups;
+  int V, d, top, parts, span, groups;
   float k, inv_tau;
   const uint4 *hc, *W;
   const int *pos, *tok;
@@ -483,30 +509,43 @@ struct RowArgs {
   int64_t* top_tokens;
 };
 
-template <int Each>
-__global__ void __launch_bounds__(kRowWarps * 32, 7) k_stats_rows(const RowArgs f) {
+// U: steps of K whose loads are under way together: 2, so that many rows share an SM, or 8 where rows are few and a slow one's
+// latency is what counts.
+template <int Each, int U>
+__global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(const RowArgs f) {
   const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
   const int64_t i = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   wait_previous();
   let_next();
   if (i >= f.N) return;
   const int r = f.pos[i], y = r >= 0 ? f.tok[r] : -1;
-  float lp = 0.f, H = 0.f, l2 = 0.f;
+  float lp = 0.f, H = 0.f, l2 = 0.f, own = 0.f;
   double base = 0.0;
   if (r >= 0) {                                  // the row's sums: by lanes, then the lanes'
-    const float own = y >= 0 ? f.own[r] : 0.f;
-    const float4* part = f.part + (int64_t)r * f.halves;
+    own = y >= 0 ? f.own[r] : 0.f;
+    const float4* part = f.part + (int64_t)r * f.parts;
     Sums q{-INFINITY, 0.f, 0.f};
-#pragma unroll 4
-    for (int g = lane; g < f.halves; g += 32) q.m = fmaxf(q.m, __ldg(&part[g].x));
+    constexpr int kAt = 8;                       // loads under way at once
+    for (int g0 = lane; g0 - lane < f.parts; g0 += 32 * kAt) {
+      float v[kAt];
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) v[j] = __ldg(&part[min(g0 + 32 * j, f.parts - 1)].x);
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) q.m = fmaxf(q.m, v[j]);
+    }
     q.m = warp_max(q.m);
-    const float off = q.m == -INFINITY ? 0.f : q.m;    // no score but NaNs, which the maxima pass over: the sums hold them
-#pragma unroll 4
-    for (int g = lane; g < f.halves; g += 32) {
-      const float4 p = __ldg(part + g);
-      const float x = (p.x - off) * f.k, e = exp2_fast(x);
-      q.t = fmaf(e, fmaf(fmaxf(x, kLeast), p.y, p.z), q.t);
-      q.s = fmaf(e, p.y, q.s);
+    const float from = q.m == -INFINITY ? 0.f : q.m;   // no score but NaNs, which the maxima pass over: the sums hold them
+    for (int g0 = lane; g0 - lane < f.parts; g0 += 32 * kAt) {
+      float4 p[kAt];
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) p[j] = __ldg(part + min(g0 + 32 * j, f.parts - 1));
+#pragma unroll
+      for (int j = 0; j < kAt; ++j)
+        if (g0 + 32 * j < f.parts) {
+          const float x = (p[j].x - from) * f.k, e = exp2_fast(x);
+          q.t = fmaf(e, fmaf(fmaxf(x, kLeast), p[j].y, p[j].z), q.t);
+          q.s = fmaf(e, p[j].y, q.s);
+        }
     }
     q.s = warp_sum(q.s);
     q.t = warp_sum(q.t);
@@ -554,11 +593,31 @@ __global__ void __launch_bounds__(kRowWarps * 32, 7) k_stats_rows(const RowArgs 
       ++have;
     }
   }
-  const int column = held_group * f.span + (int)(__float_as_uint(held.x) & 127u);
+  const int column = held_group * f.span + column_of(held);
 
-  // Their largest, and the target, sixteen at a time.
+  // Their largest, and the target: in most rows these are the answer, as the products summed them. For the row's scores may be off by
+  // `slack` (sums of 16 products, truncated; with twice the magnitudes of the likeliest one), notes by their low bits more.
   Best<float> best;
-  float size = 0.f;
+  for (int q = 0; q < have; ++q) best.put(__shfl_sync(0xffffffffu, held.x, q), __shfl_sync(0xffffffffu, column, q));
+  if (y >= 0) best.put(own, y);
+  auto low = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
+  const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
+  float size = likeliest < f.V ? magnitude(h, f.W, vecs, likeliest) : 0.f, off = 0.f;
+  float slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
+  auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack + off); };
+  {
+    const float lowest = low() - slack, then = __shfl_down_sync(0xffffffffu, best.score, 1);
+    const bool open = size == 0.f || (lane < top && (best.token >= f.V || (lane < 31 && best.score - then <= 2 * slack))) ||
+                      (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
+                      (after >= 0 && above(pair.x) >= lowest) || best.lost >= lowest - slack;
+    if (!__any_sync(0xffffffffu, open)) {
+      write((float)((double)best.score * f.inv_tau - base), best.token);
+      return;
+    }
+  }
+
+  // Else the scores again, sixteen at a time.
+  best = Best<float>{};
   const int count = have + (y >= 0);
   for (int q = 0; q < count; q += 16) {
     int rows[2];
@@ -567,26 +626,27 @@ __global__ void __launch_bounds__(kRowWarps * 32, 7) k_stats_rows(const RowArgs 
       const int at = min(q + (lane >> 2) + 8 * j, count - 1), t = __shfl_sync(0xffffffffu, column, max(min(at, have - 1), 0));
       rows[j] = at < have ? t : y;
     }
-    fetch16(f.W, vecs, rows[0], rows[1]);
-    const Pair about = q ? dots16<false>(h, f.W, vecs, rows[0], rows[1], nullptr)
-                         : dots16<true>(h, f.W, vecs, rows[0], rows[1], &size);
+    const Pair about = q ? dots16<U, false>(h, f.W, vecs, rows[0], rows[1], nullptr)
+                         : dots16<U, true>(h, f.W, vecs, rows[0], rows[1], &size);
     for (int j = 0; j < 16 && q + j < count; ++j) {
       const int t = __shfl_sync(0xffffffffu, j < 8 ? rows[0] : rows[1], j % 8 * 4);
       best.put(about.of(j), t);
     }
   }
-  // With twice the magnitudes of the first ones: what a sum here is off by at most, two chains of sums of 16 products, truncated
-  // (`off`), and with that what a note is (one chain), beside its low bits.
-  const float off = (float)(f.d / 32 + 4) * 0x1p-22f * size, slack = (float)(f.d / 16 + 2) * 0x1p-22f * size + off;
-  auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack); };
-  auto low = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
+  // What a sum here is off by at most: two chains. The magnitudes: of the first eight, or should those be rows of zeros of eight from
+  // all over the vocabulary.
+  if (size == 0.f) {
+    const int sample = (int)((int64_t)(lane >> 2) * f.V / 8);
+    dots16<U, true>(h, f.W, vecs, sample, sample, &size);
+  }
+  off = (float)(f.d / 32 + 4) * 0x1p-22f * size;
+  slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
   // The columns of a group that may count, but for one and the target's.
   auto expand = [&](int g, int except, auto&& take) {
     const int begin = g * f.span, end = min(f.V, begin + f.span);
-    for (int c = begin; c < end; c += 16) fetch16(f.W, vecs, min(c + (lane >> 2), end - 1), min(c + (lane >> 2) + 8, end - 1));
     for (int c = begin; c < end; c += 16) {
       const int ra = c + (lane >> 2), rb = ra + 8;
-      const Pair about = dots16<false>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1), nullptr);
+      const Pair about = dots16<U, false>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1), nullptr);
       const float least = low() - 2 * off;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -611,8 +671,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 7) k_stats_rows(const RowArgs 
   if (after >= 0 && above(pair.x) >= low()) {
     Groups<0> rest(notes, f.groups, order_of(pair.x), after);
     for (; after >= 0 && above(pair.x) >= low(); after = rest.next(pair)) {
-      const int c = after * f.span + (int)(__float_as_uint(pair.x) & 127u);
-      best.put(dots16<false>(h, f.W, vecs, c, c, nullptr).of(0), c);
+      const int c = after * f.span + column_of(pair);
+      best.put(dots16<U, false>(h, f.W, vecs, c, c, nullptr).of(0), c);
       if (pair.y > -3e38f && above(pair.y) >= low()) expand(after, c, about_put);
     }
   }
@@ -751,7 +811,7 @@ int launch_next(void (*kernel)(P...), int64_t blocks, int threads, cudaStream_t 
 template <int NT, bool Top>
 int few(int64_t V, int d, const void* hc, const void* weight, const int* count, const typename Scan<Top>::Params& p,
         cudaStream_t s) {
-  return launch_next(k_stats_few<NT, Top>, halves_of(V), 256, s, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
+  return launch_next(k_stats_few<NT, Top>, parts_of(V) / 2, 256, s, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
                      reinterpret_cast<const __nv_bfloat16*>(weight), count, p);
 }
 template <bool Top>
@@ -805,7 +865,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   const int *tok = reinterpret_cast<int*>(S + sv.head.tok), *pos = reinterpret_cast<int*>(S + sv.head.pos);
   const void* hc = S + sv.head.hc;
   float* lse2 = reinterpret_cast<float*>(S + sv.head.lse2);
-  const int halves = halves_of(V);
+  const int parts = parts_of(V);
   gemm::Shape sh{};
   sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = reinterpret_cast<int*>(S + sv.head.count); sh.group = 16;
   sh.status = status;
@@ -819,11 +879,17 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   else
     st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   if (st) return st;
-  const RowArgs f{N, (int)V, d, top, halves, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
+  const RowArgs f{N, (int)V, d, top, parts, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
                   reinterpret_cast<const uint4*>(weight), pos, tok, part, notes, own, lse2,
                   reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent), logp, entropy, top_logp,
                   top_tokens};
-  return launch_next(groups <= 512 ? k_stats_rows<16> : groups <= 1024 ? k_stats_rows<32> : k_stats_rows<0>, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, s, f);
+  auto rows = N <= (int64_t)gemm::sm_count() * kRowWarps ? groups <= 512    ? k_stats_rows<16, 8>
+                                                           : groups <= 1024 ? k_stats_rows<32, 8>
+                                                                            : k_stats_rows<0, 8>
+              : groups <= 512                            ? k_stats_rows<16, 2>
+              : groups <= 1024                           ? k_stats_rows<32, 2>
+                                                         : k_stats_rows<0, 2>;
+  return launch_next(rows, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, s, f);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,
