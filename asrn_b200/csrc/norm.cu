@@ -6,20 +6,26 @@
 // s (or x) and each row's m and k in fp32.
 //
 // Bound by memory: each row is read once into registers and written once. A warp holds a row of up to 1024 values, a block
-// of 256 or 512 threads a longer one, eight values (16 or 32 bytes) a load; widths that are no multiple of 8, and rows that are not
-// 16-byte aligned, go value by value. The backward pass's blocks stay for many rows with their columns' sums of dy h and dy
-// in registers; a block's sums go to fp32 parts that k_norm_sums adds up in order.
+// of 256 or 512 threads a longer one, eight values (16 or 32 bytes) a load. Rows of a width that is no multiple of 8 start anywhere
+// between two such loads: they are read from the last boundary before them on, their first value the `shift`-th of its eight; the
+// rows' ends are written value by value (k_norm_shifted, and Shifted below). Tensors that are not 16-byte aligned go value by value.
+// The backward pass's blocks stay for many rows with their columns' sums of dy h and dy in registers; a block's sums go to fp32
+// parts that k_norm_sums adds up in order.
 #include "common.cuh"
 #include "layout.h"
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace asrn {
 
 namespace {
 
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
+using F32 = std::integral_constant<int, kF32>;
+using Bf16 = std::integral_constant<int, kBf16>;
+using None = std::integral_constant<int, kNone>;
 constexpr int kMaxD = 16384;
 
 // V values of type t at an element offset, as they lie in memory; then as floats.
@@ -108,12 +114,10 @@ __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
   const int64_t at = row * f.d;
   Raw<V> rx[C], rr[C];
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int c = (tid + i * T) * V;
-    if (c < f.d) {
-      rx[i] = load((Raw<V>*)0, f.x, at + c, xt);
-      if (rt != kNone) rr[i] = load((Raw<V>*)0, f.res, at + c, rt);
-    }
+  for (int i = 0; i < C; ++i) {                          // without a condition: all under way at once
+    const int64_t c = at + min((tid + i * T) * V, f.d - V);
+    rx[i] = load((Raw<V>*)0, f.x, c, xt);
+    if (rt != kNone) rr[i] = load((Raw<V>*)0, f.res, c, rt);
   }
   float v[C * V], s = 0.f;
 #pragma unroll
@@ -165,6 +169,131 @@ __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
   }
 }
 
+// ---- rows that start anywhere -------------------------------------------------------------------------------------------------
+// Vector v of a row whose first value is the shift-th of its eight holds the columns 8 v - shift + j. The weights stand in shared memory
+// by planes of every eighth column (so that neighbouring vectors read neighbouring words), fp32.
+struct Planes {
+  float* at;
+  int pitch;
+  ASRN_DEV Planes(float* p, int d) : at(p), pitch(d / 8 + 3) {}
+  static __host__ ASRN_DEV int floats(int d) { return 8 * (d / 8 + 3); }
+  ASRN_DEV void fill(const void* w, int t, int d) const {
+    for (int c = threadIdx.x; c < d; c += blockDim.x) {
+      float v;
+      asrn::floats(load((Raw<1>*)0, w, c, t), t, &v);
+      at[(c & 7) * pitch + (c >> 3) + 1] = v;
+    }
+  }
+  ASRN_DEV float operator()(int v, int j, int shift) const {
+    const int q = j - shift;
+    return at[(q < 0 ? (q + 8) * pitch : q * pitch + 1) + v];
+  }
+};
+// Eight values at a flat index that is a multiple of 8, those past the tensor's end as zeros.
+ASRN_DEV Raw<8> load_to(const void* p, int64_t at, int64_t total, int t) {
+  if (at + 8 <= total) return load((Raw<8>*)0, p, at, t);
+  Raw<8> r;
+  uint32_t w[8] = {};
+  for (int j = 0; j < 8 && at + j < total; ++j) {
+    const uint32_t u = load((Raw<1>*)0, p, at + j, t).a;
+    if (t == kBf16)
+      w[j / 2] |= u << (16 * (j & 1));
+    else
+      w[j] = u;
+  }
+  r.a = make_uint4(w[0], w[1], w[2], w[3]);
+  r.b = make_uint4(w[4], w[5], w[6], w[7]);
+  return r;
+}
+// Those of a vector's values that are the row's: j from `low` on, below `high`.
+struct Span {
+  int low, high;
+  ASRN_DEV Span(int v, int shift, int d) : low(v == 0 ? shift : 0), high(min(8, d + shift - 8 * v)) {}
+  ASRN_DEV bool whole() const { return low == 0 && high == 8; }
+  ASRN_DEV bool none() const { return low >= high; }
+};
+ASRN_DEV void store_span(void* p, int64_t at, int t, const float* v, const Span& in) {
+  if (in.whole()) {
+    store<8>(p, at, t, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j >= in.low && j < in.high) store<1>(p, at + j, t, v + j);
+  }
+}
+
+template <int XT, int RT, int C, int T>
+__global__ void __launch_bounds__(threads_of(T), T == 32 ? (C < 3 ? 6 : 4) : 1) k_norm_shifted(const Forward f) {
+  extern __shared__ float planes[];
+  __shared__ float room[2][2][32];
+  constexpr int kRows = threads_of(T) / T;
+  const Planes w(planes, f.d), b(planes + Planes::floats(f.d), f.d);
+  w.fill(f.w, f.wt, f.d);
+  if (f.b) b.fill(f.b, f.wt, f.d);
+  __syncthreads();
+  const int tid = T == 32 ? threadIdx.x & 31 : threadIdx.x, wid = T == 32 ? threadIdx.x >> 5 : 0;
+  const int64_t total = f.rows * f.d;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + wid; row < f.rows; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+    const int shift = (int)(row * f.d & 7);
+    const int64_t at = row * f.d - shift;
+    const int last = (f.d + shift - 1) / 8;              // of the row's vectors
+    Raw<8> rx[C], rr[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int64_t to = at + 8 * min(tid + i * T, last);
+      rx[i] = load_to(f.x, to, total, XT);
+      if (RT != kNone) rr[i] = load_to(f.res, to, total, RT);
+    }
+    float u[C * 8], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = tid + i * T;
+      const Span in(v, shift, f.d);
+      float* e = u + i * 8;
+      floats(rx[i], XT, e);
+      if (RT != kNone) {
+        float r[8];
+        floats(rr[i], RT, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] += r[j];
+          if (RT == kBf16) e[j] = round_bf16(e[j]);
+        }
+        if (!in.none()) store_span(f.sum, at + 8 * v, RT, e, in);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += j >= in.low && j < in.high ? e[j] : 0.f;
+    }
+    const float m = row_sum<T>(s, room[turn][0]) / (float)f.d;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const Span in(tid + i * T, shift, f.d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float q = j >= in.low && j < in.high ? u[i * 8 + j] - m : 0.f;
+        s = fmaf(q, q, s);
+      }
+    }
+    const float k = 1.f / sqrtf(row_sum<T>(s, room[turn][1]) / (float)f.d + f.eps);
+    if (f.stats && tid == 0) f.stats[row] = make_float2(m, k);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = tid + i * T;
+      const Span in(v, shift, f.d);
+      if (in.none()) continue;
+      float* e = u + i * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = (e[j] - m) * k * w(v, j, shift);
+        if (f.b) e[j] += b(v, j, shift);
+      }
+      store_span(f.y, at + 8 * v, f.yt, e, in);
+    }
+  }
+}
+
 // s, ds and out of type ST, dy of type YT; `other`: the same gradient in the other type. parts: [blocks][2][d] sums of dy h
 // and dy, or null.
 struct Backward {
@@ -190,13 +319,11 @@ __global__ void __launch_bounds__(threads_of(T), T == 256 ? 2 : 1) k_norm_back(c
     const int64_t at = row * f.d;
     Raw<V> rs[C], ry[C], rd[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int c = (tid + i * T) * V;
-      if (c < f.d) {
-        rs[i] = load((Raw<V>*)0, f.s, at + c, st);
-        ry[i] = load((Raw<V>*)0, f.dy, at + c, yt);
-        if (f.ds) rd[i] = load((Raw<V>*)0, f.ds, at + c, st);
-      }
+    for (int i = 0; i < C; ++i) {                        // without a condition: all under way at once
+      const int64_t c = at + min((tid + i * T) * V, f.d - V);
+      rs[i] = load((Raw<V>*)0, f.s, c, st);
+      ry[i] = load((Raw<V>*)0, f.dy, c, yt);
+      if (f.ds) rd[i] = load((Raw<V>*)0, f.ds, c, st);
     }
     const float2 mk = __ldg(f.stats + row);
     float h[C * V], g[C * V], s1 = 0.f, s2 = 0.f;
@@ -286,14 +413,109 @@ __global__ void __launch_bounds__(threads_of(T), T == 256 ? 2 : 1) k_norm_back(c
   }
 }
 
-// The same for rows that a warp holds, eight values a load (d <= 1024): each warp's next row comes to shared memory by
-// asynchronous copies while it works on the one before, which costs no registers beside the columns' sums.
+// The same for rows that start anywhere, by blocks. A block's rows are eight apart, so that they all start alike.
+template <int ST, int YT, int C, int T>
+__global__ void __launch_bounds__(T, T == 256 ? 2 : 1) k_norm_back_shifted(const Backward f) {
+  extern __shared__ float planes[];
+  __shared__ float room[2][2][32];
+  const Planes w(planes, f.d);
+  w.fill(f.w, f.wt, f.d);
+  __syncthreads();
+  const int tid = threadIdx.x, shift = (int)((int64_t)blockIdx.x * f.d & 7), last = (f.d + shift - 1) / 8;
+  const int64_t total = f.rows * f.d;
+  float dw[C * 8] = {}, db[C * 8] = {};
+  const float inv = 1.f / (float)f.d;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < f.rows; row += gridDim.x, turn ^= 1) {
+    const int64_t at = row * f.d - shift;
+    Raw<8> rs[C], ry[C], rd[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int64_t to = at + 8 * min(tid + i * T, last);
+      rs[i] = load_to(f.s, to, total, ST);
+      ry[i] = load_to(f.dy, to, total, YT);
+      if (f.ds) rd[i] = load_to(f.ds, to, total, ST);
+    }
+    const float2 mk = __ldg(f.stats + row);
+    float h[C * 8], g[C * 8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = tid + i * T;
+      const Span in(v, shift, f.d);
+      float *u = h + i * 8, *e = g + i * 8;
+      floats(rs[i], ST, u);
+      floats(ry[i], YT, e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool on = j >= in.low && j < in.high;
+        u[j] = on ? (u[j] - mk.x) * mk.y : 0.f;
+        e[j] = on ? e[j] : 0.f;
+        dw[i * 8 + j] = fmaf(e[j], u[j], dw[i * 8 + j]);
+        db[i * 8 + j] += e[j];
+        e[j] = on ? e[j] * w(v, j, shift) : 0.f;
+        s1 += e[j];
+        s2 = fmaf(e[j], u[j], s2);
+      }
+    }
+    if (!f.out && !f.other) continue;
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if ((tid & 31) == 0) {                               // the rooms of two rows in turn: one barrier a row
+      room[turn][0][tid >> 5] = s1;
+      room[turn][1][tid >> 5] = s2;
+    }
+    __syncthreads();
+    s1 = s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < T / 32; ++i) {
+      s1 += room[turn][0][i];
+      s2 += room[turn][1][i];
+    }
+    s1 *= inv;
+    s2 *= inv;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = tid + i * T;
+      const Span in(v, shift, f.d);
+      if (in.none()) continue;
+      float *u = h + i * 8, *e = g + i * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = mk.y * (e[j] - s1 - u[j] * s2);
+      if (f.ds) {
+        floats(rd[i], ST, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] += u[j];
+      }
+      if (f.out) store_span(f.out, at + 8 * v, ST, e, in);
+      if (f.other) store_span(f.other, at + 8 * v, 1 - ST, e, in);
+    }
+  }
+  if (!f.parts) return;
+  float* part = f.parts + (int64_t)blockIdx.x * 2 * f.d;
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = (tid + i * T) * 8 - shift + j;
+      if (c >= 0 && c < f.d) {
+        part[c] = dw[i * 8 + j];
+        part[f.d + c] = db[i * 8 + j];
+      }
+    }
+}
+
+// The same for rows that a warp holds, eight values a load (d <= 1024; Shifted: 7 less): each warp's next row comes to shared memory
+// by asynchronous copies while it works on the one before, which costs no registers beside the columns' sums. 72 us at 32768 x 768,
+// fp32 s and ds, bf16 dy and dx, 403 MB, 5.6 TB/s; with three or four rows under way, and fewer warps, 77 and more.
 constexpr int kWarps = 4, kStages = 2;
-ASRN_DEV void copy_row(uint8_t* to, const void* from, int64_t at, int bytes, int lane) {
+ASRN_DEV void copy_row(uint8_t* to, const void* from, int64_t at, int bytes, int64_t left, int lane) {
   const char* p = reinterpret_cast<const char*>(from) + at;
-  for (int b = lane * 16; b < bytes; b += 512)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + b)), "l"(p + b)
+  for (int b = lane * 16; b < bytes; b += 512) {
+    const int n = (int)max((int64_t)0, min((int64_t)16, left - b));        // the tensor's last bytes: the rest are zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + b)),
+                 "l"(n ? p + b : p), "r"(n)
                  : "memory");
+  }
 }
 ASRN_DEV Raw<8> staged(const uint8_t* p, int c, int t) {
   Raw<8> r;
@@ -302,31 +524,41 @@ ASRN_DEV Raw<8> staged(const uint8_t* p, int c, int t) {
   if (t == kF32) r.b = q[1];
   return r;
 }
-constexpr int row_bytes(int d, int t) { return d * (t == kBf16 ? 2 : 4); }
+// Bytes of a row as it is staged: whole vectors, one more where rows start anywhere.
+constexpr int row_bytes(int d, int t) { return ((d + 7) / 8 + (d % 8 != 0)) * (t == kBf16 ? 16 : 32); }
 size_t staged_bytes(int d, int st, int yt, bool ds) {
   return (size_t)kWarps * kStages * (row_bytes(d, st) * (1 + ds) + row_bytes(d, yt));
 }
-template <int ST, int YT, int C>
+template <int ST, int YT, int C, bool Shifted>
 __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_norm_back_rows(const Backward f) {
   extern __shared__ __align__(16) uint8_t room[];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int sb = row_bytes(f.d, ST), yb = row_bytes(f.d, YT), stage = sb * (f.ds ? 2 : 1) + yb;
+  constexpr int se = ST == kBf16 ? 2 : 4, ye = YT == kBf16 ? 2 : 4;
   uint8_t* mine = room + wid * kStages * stage;
+  const int64_t step = (int64_t)gridDim.x * kWarps, row0 = (int64_t)blockIdx.x * kWarps + wid, total = f.rows * f.d;
+  const int shift = Shifted ? (int)(row0 * f.d & 7) : 0;   // a warp's rows start alike: step is a multiple of 8
+  const Planes w(reinterpret_cast<float*>(room + (size_t)kWarps * kStages * stage), f.d);
   auto fetch = [&](int64_t row, int turn) {
     if (row < f.rows) {
       uint8_t* to = mine + turn * stage;
-      copy_row(to, f.s, row * sb, sb, lane);
-      copy_row(to + sb, f.dy, row * yb, yb, lane);
-      if (f.ds) copy_row(to + sb + yb, f.ds, row * sb, sb, lane);
+      const int64_t at = row * f.d - shift, left = total - at;
+      const int n = Shifted ? (f.d + shift + 7) / 8 * 8 : f.d;
+      copy_row(to, f.s, at * se, n * se, left * se, lane);
+      copy_row(to + sb, f.dy, at * ye, n * ye, left * ye, lane);
+      if (f.ds) copy_row(to + sb + yb, f.ds, at * se, n * se, left * se, lane);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   float dw[C * 8] = {}, db[C * 8] = {};
   const float inv = 1.f / (float)f.d;
-  const int64_t step = (int64_t)gridDim.x * kWarps, row0 = (int64_t)blockIdx.x * kWarps + wid;
   int turn = 0;
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) fetch(row0 + j * step, j);
+  if (Shifted) {
+    w.fill(f.w, f.wt, f.d);
+    __syncthreads();
+  }
   float2 next = row0 < f.rows ? __ldg(f.stats + row0) : make_float2(0.f, 0.f);
   for (int64_t row = row0; row < f.rows; row += step, turn = turn + 1 == kStages ? 0 : turn + 1) {
     __syncwarp();                                        // the room's last row has been read by every lane
@@ -339,23 +571,36 @@ __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_nor
     float h[C * 8], g[C * 8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int c = (lane + i * 32) * 8;
+      const int v = lane + i * 32;
+      const Span in(v, shift, f.d);
       float *u = h + i * 8, *e = g + i * 8;
-      if (c >= f.d) {
+      if (in.none()) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] = e[j] = 0.f;
         continue;
       }
-      float w[8];
-      floats(load((Raw<8>*)0, f.w, c, f.wt), f.wt, w);
-      floats(staged(at, c, ST), ST, u);
-      floats(staged(at + sb, c, YT), YT, e);
+      float q[8];
+      if (Shifted) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = w(v, j, shift);
+      } else {
+        floats(load((Raw<8>*)0, f.w, v * 8, f.wt), f.wt, q);
+      }
+      floats(staged(at, v * 8, ST), ST, u);
+      floats(staged(at + sb, v * 8, YT), YT, e);
+      if (Shifted && !in.whole())
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < in.low || j >= in.high) {
+            u[j] = mk.x;
+            e[j] = q[j] = 0.f;
+          }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         u[j] = (u[j] - mk.x) * mk.y;
         dw[i * 8 + j] = fmaf(e[j], u[j], dw[i * 8 + j]);
         db[i * 8 + j] += e[j];
-        e[j] *= w[j];
+        e[j] *= q[j];
         s1 += e[j];
         s2 = fmaf(e[j], u[j], s2);
       }
@@ -365,38 +610,54 @@ __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_nor
     s2 = warp_sum(s2) * inv;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int c = (lane + i * 32) * 8;
-      if (c >= f.d) continue;
+      const int v = lane + i * 32;
+      const Span in(v, shift, f.d);
+      if (in.none()) continue;
       float *u = h + i * 8, *e = g + i * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) e[j] = mk.y * (e[j] - s1 - u[j] * s2);
       if (f.ds) {
-        floats(staged(at + sb + yb, c, ST), ST, u);
+        floats(staged(at + sb + yb, v * 8, ST), ST, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] += u[j];
       }
-      if (f.out) store<8>(f.out, row * f.d + c, ST, e);
-      if (f.other) store<8>(f.other, row * f.d + c, 1 - ST, e);
+      const int64_t to = row * f.d - shift + v * 8;
+      if (f.out) Shifted ? store_span(f.out, to, ST, e, in) : store<8>(f.out, to, ST, e);
+      if (f.other) Shifted ? store_span(f.other, to, 1 - ST, e, in) : store<8>(f.other, to, 1 - ST, e);
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (!f.parts) return;
   __syncthreads();
-  float* sums = reinterpret_cast<float*>(room);          // [2][C 8][32]
-  for (int w = 0; w < kWarps; ++w) {                     // the block's warps, one after another
-    if (wid == w)
+  // The columns' sums [2][8][32 C + 1], a vector's columns in planes; the block's warps add theirs one after another. Where rows start
+  // anywhere, a warp's columns are not another's: by their own places [2][d] then.
+  float* sums = reinterpret_cast<float*>(room);
+  if (Shifted) {
+    for (int c = threadIdx.x; c < 2 * f.d; c += blockDim.x) sums[c] = 0.f;
+    __syncthreads();
+  }
+  for (int k = 0; k < kWarps; ++k) {
+    if (wid == k)
 #pragma unroll
       for (int i = 0; i < C * 8; ++i) {
-        sums[i * 32 + lane] = w ? sums[i * 32 + lane] + dw[i] : dw[i];
-        sums[(C * 8 + i) * 32 + lane] = w ? sums[(C * 8 + i) * 32 + lane] + db[i] : db[i];
+        if (Shifted) {
+          const int c = (lane + i / 8 * 32) * 8 - shift + i % 8;
+          if (c >= 0 && c < f.d) {
+            sums[c] += dw[i];
+            sums[f.d + c] += db[i];
+          }
+        } else {
+          sums[i * 32 + lane] = k ? sums[i * 32 + lane] + dw[i] : dw[i];
+          sums[(C * 8 + i) * 32 + lane] = k ? sums[(C * 8 + i) * 32 + lane] + db[i] : db[i];
+        }
       }
     __syncthreads();
   }
   float* part = f.parts + (int64_t)blockIdx.x * 2 * f.d;
   for (int c = threadIdx.x; c < f.d; c += blockDim.x) {
-    const int q = c / 8, own = (q / 32 * 8 + c % 8) * 32 + q % 32;       // where column c's thread put it
+    const int q = c / 8, own = Shifted ? c : (q / 32 * 8 + c % 8) * 32 + q % 32;       // where column c's thread put it
     part[c] = sums[own];
-    part[f.d + c] = sums[C * 256 + own];
+    part[f.d + c] = sums[own + (Shifted ? f.d : C * 256)];
   }
 }
 
@@ -431,10 +692,12 @@ int sms() {
   return v;
 }
 
-// Blocks of the backward pass: as many as stay on the SMs at once, each with 2 d sums of its own.
+// Blocks of the backward pass: as many as stay on the SMs at once, each with 2 d sums of its own; a multiple of 8 where rows start
+// anywhere, so that a warp's or block's own rows start alike.
 int64_t blocks_back(int64_t rows, int d) {
   const int per = d <= 1024 ? kWarps : 1, stay = d <= 256 ? 5 : d <= 768 ? 3 : d <= 4096 ? 2 : 1;
-  return std::max<int64_t>(1, std::min<int64_t>((int64_t)sms() * stay, (rows + per - 1) / per));
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((int64_t)sms() * stay, (rows + per - 1) / per));
+  return d % 8 ? (n + 7) / 8 * 8 : n;
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
@@ -455,29 +718,20 @@ template <int XT, int RT> int widths(const Forward& f, cudaStream_t s) {
   if (f.d <= 8192) return run<8, XT, RT, 2, 512>(f, s);
   return run<8, XT, RT, 4, 512>(f, s);
 }
+// Value by value, for tensors that are not 16-byte aligned, and the six odd widths below kMaxD.
 template <class Args> int singles(const Args& f, cudaStream_t s) {
-  if (f.d <= 128) return run<1, -1, -1, 4, 32>(f, s);
   if (f.d <= 256) return run<1, -1, -1, 8, 32>(f, s);
-  if (f.d <= 384) return run<1, -1, -1, 12, 32>(f, s);
-  if (f.d <= 512) return run<1, -1, -1, 16, 32>(f, s);
-  if (f.d <= 768) return run<1, -1, -1, 24, 32>(f, s);
   if (f.d <= 1024) return run<1, -1, -1, 32, 32>(f, s);
-  if (f.d <= 2048) return run<1, -1, -1, 8, 256>(f, s);
-  if (f.d <= 4096) return run<1, -1, -1, 16, 256>(f, s);
-  if (f.d <= 8192) return run<1, -1, -1, 16, 512>(f, s);
+  if (f.d <= 8192) return run<1, -1, -1, 32, 256>(f, s);
   return run<1, -1, -1, 32, 512>(f, s);
 }
 
-template <int V, int ST, int YT, int C, int T> int run(const Backward& f, cudaStream_t s) {
-  k_norm_back<V, ST, YT, C, T><<<(unsigned)blocks_back(f.rows, f.d), threads_of(T), 0, s>>>(f);
-  return launched();
-}
-template <int ST, int YT, int C> int run_rows(const Backward& f, cudaStream_t s) {
-  auto kernel = k_norm_back_rows<ST, YT, C>;
-  constexpr size_t most = (size_t)kWarps * kStages * (row_bytes(C * 256, ST) * 2 + row_bytes(C * 256, YT));
-  static std::atomic<uint64_t> ready{0};                 // devices that know the kernel's shared memory
-  int dev = 0;
-  if (most > 48 << 10) {
+// A kernel whose dynamic shared memory may pass 48 KB: `most` is what any call asks for.
+template <class Kernel, class Args>
+int launch(Kernel kernel, std::atomic<uint64_t>& ready, size_t most, int64_t blocks, int threads, size_t bytes, const Args& f,
+           cudaStream_t s) {
+  if (most > 48 << 10) {                                 // `ready`: devices that know it
+    int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ASRN_ERR_CUDA;
     if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
@@ -485,19 +739,67 @@ template <int ST, int YT, int C> int run_rows(const Backward& f, cudaStream_t s)
       if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
   }
-  const size_t bytes = std::max<size_t>(staged_bytes(f.d, ST, YT, f.ds != nullptr), f.parts ? C * 8 * 32 * 2 * 4 : 0);
-  kernel<<<(unsigned)blocks_back(f.rows, f.d), kWarps * 32, bytes, s>>>(f);
+  kernel<<<(unsigned)blocks, threads, bytes, s>>>(f);
   return launched();
 }
+
+template <int XT, int RT, int C, int T> int run_shifted(const Forward& f, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  constexpr int per = threads_of(T) / T;
+  const int64_t most = (int64_t)sms() * (T == 32 ? (C < 3 ? 6 : 4) : T == 256 ? 4 : 2);
+  return launch(k_norm_shifted<XT, RT, C, T>, ready, (size_t)2 * Planes::floats(T * C * 8) * 4,
+                std::min(most, (f.rows + per - 1) / per), threads_of(T), (size_t)2 * Planes::floats(f.d) * 4, f, s);
+}
+template <int XT, int RT> int shifted(const Forward& f, cudaStream_t s) {
+  const int n = f.d + 7;                                 // values from the last boundary before the row to its end, at most
+  if (n <= 256) return run_shifted<XT, RT, 1, 32>(f, s);
+  if (n <= 512) return run_shifted<XT, RT, 2, 32>(f, s);
+  if (n <= 768) return run_shifted<XT, RT, 3, 32>(f, s);
+  if (n <= 1024) return run_shifted<XT, RT, 4, 32>(f, s);
+  if (n <= 2048) return run_shifted<XT, RT, 1, 256>(f, s);
+  if (n <= 4096) return run_shifted<XT, RT, 2, 256>(f, s);
+  if (n <= 8192) return run_shifted<XT, RT, 2, 512>(f, s);
+  return n <= kMaxD ? run_shifted<XT, RT, 4, 512>(f, s) : singles(f, s);
+}
+
+template <int V, int ST, int YT, int C, int T> int run(const Backward& f, cudaStream_t s) {
+  k_norm_back<V, ST, YT, C, T><<<(unsigned)blocks_back(f.rows, f.d), threads_of(T), 0, s>>>(f);
+  return launched();
+}
+template <int ST, int YT, int C, bool Shifted> int run_rows(const Backward& f, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  constexpr int d = C * 256 - Shifted;                   // the largest
+  constexpr size_t sums = std::max<size_t>(C * 8 * 32 * 2 * 4, 2 * d * 4);
+  constexpr size_t most = kWarps * kStages * (row_bytes(d, ST) * 2 + row_bytes(d, YT)) + 8 * (d / 8 + 3) * 4 + sums;
+  const size_t bytes = staged_bytes(f.d, ST, YT, f.ds != nullptr) + (Shifted ? Planes::floats(f.d) * 4 : 0);
+  return launch(k_norm_back_rows<ST, YT, C, Shifted>, ready, most, blocks_back(f.rows, f.d), kWarps * 32,
+                std::max<size_t>(bytes, f.parts ? sums : 0), f, s);
+}
+template <int ST, int YT, int C, int T> int run_shifted(const Backward& f, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  return launch(k_norm_back_shifted<ST, YT, C, T>, ready, (size_t)Planes::floats(T * C * 8) * 4, blocks_back(f.rows, f.d), T,
+                (size_t)Planes::floats(f.d) * 4, f, s);
+}
 template <int ST, int YT> int widths(const Backward& f, cudaStream_t s) {
-  if (f.d <= 256) return run_rows<ST, YT, 1>(f, s);
-  if (f.d <= 512) return run_rows<ST, YT, 2>(f, s);
-  if (f.d <= 768) return run_rows<ST, YT, 3>(f, s);
-  if (f.d <= 1024) return run_rows<ST, YT, 4>(f, s);
+  if (f.d <= 256) return run_rows<ST, YT, 1, false>(f, s);
+  if (f.d <= 512) return run_rows<ST, YT, 2, false>(f, s);
+  if (f.d <= 768) return run_rows<ST, YT, 3, false>(f, s);
+  if (f.d <= 1024) return run_rows<ST, YT, 4, false>(f, s);
   if (f.d <= 2048) return run<8, ST, YT, 1, 256>(f, s);
   if (f.d <= 4096) return run<8, ST, YT, 2, 256>(f, s);
   if (f.d <= 8192) return run<8, ST, YT, 2, 512>(f, s);
   return run<8, ST, YT, 4, 512>(f, s);
+}
+template <int ST, int YT> int shifted(const Backward& f, cudaStream_t s) {
+  const int n = f.d + 7;
+  if (n <= 256) return run_rows<ST, YT, 1, true>(f, s);
+  if (n <= 512) return run_rows<ST, YT, 2, true>(f, s);
+  if (n <= 768) return run_rows<ST, YT, 3, true>(f, s);
+  if (n <= 1024) return run_rows<ST, YT, 4, true>(f, s);
+  if (n <= 2048) return run_shifted<ST, YT, 1, 256>(f, s);
+  if (n <= 4096) return run_shifted<ST, YT, 2, 256>(f, s);
+  if (n <= 8192) return run_shifted<ST, YT, 2, 512>(f, s);
+  return n <= kMaxD ? run_shifted<ST, YT, 4, 512>(f, s) : singles(f, s);
 }
 
 int check_norm(int64_t rows, int32_t d) {
@@ -506,11 +808,10 @@ int check_norm(int64_t rows, int32_t d) {
   return ASRN_OK;
 }
 bool type_ok(int t) { return t == kF32 || t == kBf16; }
-// Every tensor's address allows 16-byte loads of rows of d.
-bool vectors(int d, std::initializer_list<const void*> ps) {
+bool aligned(std::initializer_list<const void*> ps) {
   uintptr_t all = 0;
   for (const void* p : ps) all |= (uintptr_t)p;
-  return d % 8 == 0 && all % 16 == 0;
+  return all % 16 == 0;
 }
 // And is a multiple of its type's size.
 bool placed(const void* p, int t) { return (uintptr_t)p % (t == kBf16 ? 2 : 4) == 0; }
@@ -535,10 +836,13 @@ int asrn_layer_norm(int64_t rows, int32_t d, const void* x, int32_t x_type, cons
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Forward f{rows, d, x, residual, weight, bias, x_type, residual ? res_type : kNone, w_type, y_type, eps, sum, y,
                   reinterpret_cast<float2*>(stats)};
-  if (!vectors(d, {x, residual, weight, bias, residual ? sum : nullptr, y})) return singles(f, s);
-  if (x_type == kF32)
-    return f.rt == kNone ? widths<kF32, kNone>(f, s) : f.rt == kF32 ? widths<kF32, kF32>(f, s) : widths<kF32, kBf16>(f, s);
-  return f.rt == kNone ? widths<kBf16, kNone>(f, s) : f.rt == kF32 ? widths<kBf16, kF32>(f, s) : widths<kBf16, kBf16>(f, s);
+  if (!aligned({x, residual, weight, bias, residual ? sum : nullptr, y})) return singles(f, s);
+  auto with = [&](auto xt, auto rt) {
+    constexpr int a = decltype(xt)::value, b = decltype(rt)::value;
+    return d % 8 ? shifted<a, b>(f, s) : widths<a, b>(f, s);
+  };
+  if (x_type == kF32) return f.rt == kNone ? with(F32{}, None{}) : f.rt == kF32 ? with(F32{}, F32{}) : with(F32{}, Bf16{});
+  return f.rt == kNone ? with(Bf16{}, None{}) : f.rt == kF32 ? with(Bf16{}, F32{}) : with(Bf16{}, Bf16{});
 }
 
 size_t asrn_layer_norm_workspace_bytes(int64_t rows, int32_t d) {
@@ -570,12 +874,16 @@ int asrn_layer_norm_backward(int64_t rows, int32_t d, const void* s_in, int32_t 
   const Backward f{rows, d, s_in, dy, ds, weight, s_type, y_type, w_type, reinterpret_cast<const float2*>(stats), out, other,
                    sums ? reinterpret_cast<float*>(workspace) : nullptr};
   if (!sums && !out && !other) return ASRN_OK;
-  if (!vectors(d, {s_in, dy, ds, weight, out, other}))
+  auto with = [&](auto a, auto b) {
+    constexpr int x = decltype(a)::value, y = decltype(b)::value;
+    return d % 8 ? shifted<x, y>(f, s) : widths<x, y>(f, s);
+  };
+  if (!aligned({s_in, dy, ds, weight, out, other}))
     st = singles(f, s);
   else if (s_type == kF32)
-    st = y_type == kF32 ? widths<kF32, kF32>(f, s) : widths<kF32, kBf16>(f, s);
+    st = y_type == kF32 ? with(F32{}, F32{}) : with(F32{}, Bf16{});
   else
-    st = y_type == kF32 ? widths<kBf16, kF32>(f, s) : widths<kBf16, kBf16>(f, s);
+    st = y_type == kF32 ? with(Bf16{}, F32{}) : with(Bf16{}, Bf16{});
   if (st || !sums) return st;
   k_norm_sums<<<(unsigned)((2 * d + 31) / 32), 1024, 0, s>>>((int)blocks_back(rows, d), d, f.parts, dw, db, w_type);
   return launched();
