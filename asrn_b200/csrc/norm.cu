@@ -80,10 +80,11 @@ template <int V> ASRN_DEV void store(void* p, int64_t at, int t, const float* v)
   }
 }
 
-// The sum over a row's T threads: a warp's, or a whole block's (each sum with its own room, so one barrier serves).
+// The sum over a row's T threads: a warp's or half of one, or a whole block's (each sum with its own room, so one barrier serves).
 template <int T> ASRN_DEV float row_sum(float v, float* room) {
-  v = warp_sum(v);
-  if constexpr (T == 32) return v;
+#pragma unroll
+  for (int o = (T < 32 ? T : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (T <= 32) return v;
   if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
   __syncthreads();
   float s = 0.f;
@@ -92,7 +93,7 @@ template <int T> ASRN_DEV float row_sum(float v, float* room) {
   return s;
 }
 
-constexpr int threads_of(int T) { return T == 32 ? 128 : T; }
+constexpr int threads_of(int T) { return T <= 32 ? 128 : T; }
 
 // V values a load, C loads a thread, T threads a row; types XT, RT known at compile time unless they are -1.
 struct Forward {
@@ -108,10 +109,11 @@ template <int V, int XT, int RT, int C, int T>
 __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
   __shared__ float room[2][32];
   const int xt = XT < 0 ? f.xt : XT, rt = RT < 0 ? f.rt : RT;
-  const int tid = T == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = T == 32 ? (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= f.rows) return;
-  const int64_t at = row * f.d;
+  const int tid = T <= 32 ? threadIdx.x % T : threadIdx.x;
+  const int64_t own = T <= 32 ? (int64_t)blockIdx.x * (blockDim.x / T) + threadIdx.x / T : blockIdx.x;
+  const bool on = own < f.rows;                          // a warp's second row may be none: it goes along
+  const int64_t row = T < 32 ? min(own, f.rows - 1) : own, at = row * f.d;
+  if (T == 32 && !on) return;
   Raw<V> rx[C], rr[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {                          // without a condition: all under way at once
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
         u[j] += r[j];
         if (rt == kBf16) u[j] = round_bf16(u[j]);
       }
-      store<V>(f.sum, at + c, rt, u);
+      if (T >= 32 || on) store<V>(f.sum, at + c, rt, u);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) s += u[j];
@@ -151,11 +153,11 @@ __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
 #pragma unroll
       for (int j = 0; j < V; ++j) s = fmaf(v[i * V + j] - m, v[i * V + j] - m, s);
   const float k = 1.f / sqrtf(row_sum<T>(s, room[1]) / (float)f.d + f.eps);
-  if (f.stats && tid == 0) f.stats[row] = make_float2(m, k);
+  if (f.stats && tid == 0 && on) f.stats[row] = make_float2(m, k);
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const int c = (tid + i * T) * V;
-    if (c >= f.d) continue;
+    if (c >= f.d || !on) continue;
     float w[V], b[V], *u = v + i * V;
     floats(load((Raw<V>*)0, f.w, c, f.wt), f.wt, w);
 #pragma unroll
@@ -222,8 +224,12 @@ ASRN_DEV void store_span(void* p, int64_t at, int t, const float* v, const Span&
   }
 }
 
+// Its blocks that stay on an SM at once.
+constexpr int stay_shifted(int C, int T) {
+  return T <= 32 ? (C == 1 ? 10 : C == 2 ? 7 : C == 3 ? 5 : 4) : T == 256 ? (C == 1 ? 5 : 4) : C == 2 ? 2 : 1;
+}
 template <int XT, int RT, int C, int T>
-__global__ void __launch_bounds__(threads_of(T), T == 32 ? (C < 3 ? 6 : 4) : 1) k_norm_shifted(const Forward f) {
+__global__ void __launch_bounds__(threads_of(T), stay_shifted(C, T)) k_norm_shifted(const Forward f) {
   extern __shared__ float planes[];
   __shared__ float room[2][2][32];
   constexpr int kRows = threads_of(T) / T;
@@ -231,19 +237,29 @@ __global__ void __launch_bounds__(threads_of(T), T == 32 ? (C < 3 ? 6 : 4) : 1) 
   w.fill(f.w, f.wt, f.d);
   if (f.b) b.fill(f.b, f.wt, f.d);
   __syncthreads();
-  const int tid = T == 32 ? threadIdx.x & 31 : threadIdx.x, wid = T == 32 ? threadIdx.x >> 5 : 0;
-  const int64_t total = f.rows * f.d;
+  const int tid = T <= 32 ? threadIdx.x % T : threadIdx.x, sub = T <= 32 ? threadIdx.x / T : 0;
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + wid; row < f.rows; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < f.rows; first += (int64_t)gridDim.x * kRows, turn ^= 1) {
+    const int64_t row = min(first + sub, f.rows - 1);
+    const bool on = first + sub < f.rows;                // else the last row goes along, for its warp's other half
     const int shift = (int)(row * f.d & 7);
     const int64_t at = row * f.d - shift;
     const int last = (f.d + shift - 1) / 8;              // of the row's vectors
     Raw<8> rx[C], rr[C];
+    if (row + 1 < f.rows) {                              // without a condition of each: all under way at once
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int64_t to = at + 8 * min(tid + i * T, last);
-      rx[i] = load_to(f.x, to, total, XT);
-      if (RT != kNone) rr[i] = load_to(f.res, to, total, RT);
+      for (int i = 0; i < C; ++i) {
+        const int64_t to = at + 8 * min(tid + i * T, last);
+        rx[i] = load((Raw<8>*)0, f.x, to, XT);
+        if (RT != kNone) rr[i] = load((Raw<8>*)0, f.res, to, RT);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int64_t to = at + 8 * min(tid + i * T, last);
+        rx[i] = load_to(f.x, to, f.rows * f.d, XT);
+        if (RT != kNone) rr[i] = load_to(f.res, to, f.rows * f.d, RT);
+      }
     }
     float u[C * 8], s = 0.f;
 #pragma unroll
@@ -260,7 +276,7 @@ __global__ void __launch_bounds__(threads_of(T), T == 32 ? (C < 3 ? 6 : 4) : 1) 
           e[j] += r[j];
           if (RT == kBf16) e[j] = round_bf16(e[j]);
         }
-        if (!in.none()) store_span(f.sum, at + 8 * v, RT, e, in);
+        if (!in.none() && on) store_span(f.sum, at + 8 * v, RT, e, in);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += j >= in.low && j < in.high ? e[j] : 0.f;
@@ -277,12 +293,12 @@ __global__ void __launch_bounds__(threads_of(T), T == 32 ? (C < 3 ? 6 : 4) : 1) 
       }
     }
     const float k = 1.f / sqrtf(row_sum<T>(s, room[turn][1]) / (float)f.d + f.eps);
-    if (f.stats && tid == 0) f.stats[row] = make_float2(m, k);
+    if (f.stats && tid == 0 && on) f.stats[row] = make_float2(m, k);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int v = tid + i * T;
       const Span in(v, shift, f.d);
-      if (in.none()) continue;
+      if (in.none() || !on) continue;
       float* e = u + i * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -429,12 +445,22 @@ __global__ void __launch_bounds__(T, T == 256 ? 2 : 1) k_norm_back_shifted(const
   for (int64_t row = blockIdx.x; row < f.rows; row += gridDim.x, turn ^= 1) {
     const int64_t at = row * f.d - shift;
     Raw<8> rs[C], ry[C], rd[C];
+    if (row + 1 < f.rows) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int64_t to = at + 8 * min(tid + i * T, last);
-      rs[i] = load_to(f.s, to, total, ST);
-      ry[i] = load_to(f.dy, to, total, YT);
-      if (f.ds) rd[i] = load_to(f.ds, to, total, ST);
+      for (int i = 0; i < C; ++i) {
+        const int64_t to = at + 8 * min(tid + i * T, last);
+        rs[i] = load((Raw<8>*)0, f.s, to, ST);
+        ry[i] = load((Raw<8>*)0, f.dy, to, YT);
+        if (f.ds) rd[i] = load((Raw<8>*)0, f.ds, to, ST);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int64_t to = at + 8 * min(tid + i * T, last);
+        rs[i] = load_to(f.s, to, total, ST);
+        ry[i] = load_to(f.dy, to, total, YT);
+        if (f.ds) rd[i] = load_to(f.ds, to, total, ST);
+      }
     }
     const float2 mk = __ldg(f.stats + row);
     float h[C * 8], g[C * 8], s1 = 0.f, s2 = 0.f;
@@ -704,11 +730,12 @@ int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_C
 
 template <int V, int XT, int RT, int C, int T> int run(const Forward& f, cudaStream_t s) {
   // few rows: a warp for a block, so that they spread over the SMs
-  const int threads = T > 32 ? T : f.rows <= 4 * sms() ? 32 : threads_of(T), per = T == 32 ? threads / 32 : 1;
+  const int threads = T > 32 ? T : f.rows <= 4 * sms() ? 32 : threads_of(T), per = T <= 32 ? threads / T : 1;
   k_norm<V, XT, RT, C, T><<<(unsigned)((f.rows + per - 1) / per), threads, 0, s>>>(f);
   return launched();
 }
 template <int XT, int RT> int widths(const Forward& f, cudaStream_t s) {
+  if (f.d <= 128) return run<8, XT, RT, 1, 16>(f, s);
   if (f.d <= 256) return run<8, XT, RT, 1, 32>(f, s);
   if (f.d <= 512) return run<8, XT, RT, 2, 32>(f, s);
   if (f.d <= 768) return run<8, XT, RT, 3, 32>(f, s);
@@ -746,12 +773,13 @@ int launch(Kernel kernel, std::atomic<uint64_t>& ready, size_t most, int64_t blo
 template <int XT, int RT, int C, int T> int run_shifted(const Forward& f, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
   constexpr int per = threads_of(T) / T;
-  const int64_t most = (int64_t)sms() * (T == 32 ? (C < 3 ? 6 : 4) : T == 256 ? 4 : 2);
+  const int64_t most = (int64_t)sms() * stay_shifted(C, T);
   return launch(k_norm_shifted<XT, RT, C, T>, ready, (size_t)2 * Planes::floats(T * C * 8) * 4,
                 std::min(most, (f.rows + per - 1) / per), threads_of(T), (size_t)2 * Planes::floats(f.d) * 4, f, s);
 }
 template <int XT, int RT> int shifted(const Forward& f, cudaStream_t s) {
   const int n = f.d + 7;                                 // values from the last boundary before the row to its end, at most
+  if (n <= 128) return run_shifted<XT, RT, 1, 16>(f, s);
   if (n <= 256) return run_shifted<XT, RT, 1, 32>(f, s);
   if (n <= 512) return run_shifted<XT, RT, 2, 32>(f, s);
   if (n <= 768) return run_shifted<XT, RT, 3, 32>(f, s);
