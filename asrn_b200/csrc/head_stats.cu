@@ -45,9 +45,12 @@ constexpr int kPart = 64;
 __host__ ASRN_DEV int parts_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * (gemm::kBN / kPart); }
 
 // Columns of a group: of a group that holds two of the likeliest tokens all have to be looked at, so 32 as long as a row's groups
-// stay few enough for a warp to hold in registers.
-int span_of(int64_t V) { return V <= 32768 ? 32 : 64; }
-int64_t notes_of(int64_t V) { return (V + span_of(V) - 1) / span_of(V); }
+// stay few enough for a warp to hold in registers. Where a row would have four such pairs or more, groups of 1: all scores are kept
+// (10816 x 1265 x 608: 20 tokens 296 us so, 402 by groups of 32; 8 tokens 183 and 158).
+int span_of(int64_t V, int top) { return V <= 2048 && 8 * top * top >= V ? 1 : V <= 32768 ? 32 : 64; }
+int64_t notes_of(int64_t V, int top) { return (V + span_of(V, top) - 1) / span_of(V, top); }
+// Bytes of a row's notes: two numbers a group, or one a column (whole chunks of 32).
+int64_t note_bytes(int64_t V, int top) { return span_of(V, top) == 1 ? (V + 31) / 32 * 128 : notes_of(V, top) * 8; }
 
 struct StatsWs {
   size_t counts, top, part, notes, total;
@@ -61,7 +64,7 @@ StatsWs stats_ws(int64_t N, int64_t V, int top) {
   w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
   w.top = take(P * 4);
   w.part = take(parts * P * 16);
-  w.notes = take(top ? (size_t)notes_of(V) * P * 8 : 0);
+  w.notes = take(top ? (size_t)note_bytes(V, top) * P : 0);
   w.total = o;
   return w;
 }
@@ -76,7 +79,6 @@ ASRN_DEV float max3(float a, float b, float c) {
 ASRN_DEV float2 note_of(float most, float first, float second) {
   return make_float2(most, __uint_as_float((__float_as_uint(second) & ~63u) | (__float_as_uint(first) & 63u)));
 }
-ASRN_DEV int column_of(float2 note) { return (int)(__float_as_uint(note.y) & 63u); }
 
 template <bool Top> struct Scan {
   static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
@@ -85,7 +87,7 @@ template <bool Top> struct Scan {
     float k;                               // log2(e) / tau
     float* top;                            // the targets' unscaled scores
     float4* part;                          // m, S, T log2(e): [rows][parts]
-    float2* notes;                         // of each group: [rows][groups]
+    float2* notes;                         // of each group: [rows][groups]; span 1: the scores, floats [rows][whole chunks]
     int span, groups;
   };
   const Params& p;
@@ -145,7 +147,16 @@ template <bool Top> struct Scan {
     t = fmaf(f, fmaf(step, s, t), part);
     s = fmaf(s, f, c0 + c1);
     m = now;
-    if constexpr (Top) {                   // two chains of pairs, then one; the chunk's place in the group in the low bits, too
+    if constexpr (Top) {
+      if (p.span == 1) {
+        if (on) {
+          float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.notes) + (int64_t)row * ((V + 31) / 32 * 32) + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) to[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        return;
+      }
+      // Two chains of pairs, then one; the chunk's place in the group in the low bits, too.
       float m1[2] = {kNothing, kNothing}, m2[2] = {kNothing, kNothing};
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
@@ -240,7 +251,11 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
         first = fmaxf(first, u);
       }
     }
-    if (Top) {
+    if (Top && p.span == 1) {
+      const int wide = (V + 31) / 32 * 32;
+      if (c0 < wide)
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.notes) + (int64_t)r * wide + c0) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (Top) {
       float most = fmaxf(m, kNothing);
       for (int o = 1; o < p.span / 4; o <<= 1) {         // over the lanes of a group
         const float f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
@@ -322,16 +337,24 @@ ASRN_DEV uint32_t order_of(float v) {
   return v <= -3e38f ? 0u : (u >> 31 ? ~u : u | 0x80000000u) & ~127u;
 }
 
+// A row's notes; Whole: its scores, groups of one column.
+template <bool Whole> struct Notes {
+  const float* at;
+  ASRN_DEV float largest(int g) const { return __ldg(at + (Whole ? g : 2 * g)); }
+  ASRN_DEV float2 operator()(int g) const {
+    return Whole ? make_float2(__ldg(at + g), kNothing) : __ldg(reinterpret_cast<const float2*>(at) + g);
+  }
+};
 // A row's groups in the order of their largest scores, equal ones by their numbers. Each lane holds the next of its own; up to
 // 32 Each groups all of them, in registers.
-template <int Each> struct Groups {
-  const float2* notes;
+template <int Each, class Notes> struct Groups {
+  Notes notes;
   uint32_t key[Each], best;                      // a group's order, its place among the lane's in the low bits, the first's larger
-  ASRN_DEV Groups(const float2* p, int groups) : notes(p), best(0) {
+  ASRN_DEV Groups(const Notes& p, int groups) : notes(p), best(0) {
     const int lane = threadIdx.x & 31;
     float v[Each];
 #pragma unroll
-    for (int j = 0; j < Each; ++j) v[j] = __ldg(&p[min(lane + 32 * j, groups - 1)].x);   // no condition: all under way at once
+    for (int j = 0; j < Each; ++j) v[j] = notes.largest(min(lane + 32 * j, groups - 1));  // no condition: all under way at once
 #pragma unroll
     for (int j = 0; j < Each; ++j) {
       const uint32_t o = lane + 32 * j < groups ? order_of(v[j]) : 0u;
@@ -346,7 +369,7 @@ template <int Each> struct Groups {
     const int j = Each - 1 - (int)(best & 127u);
     const int mine = (best & ~127u) == most ? lane + 32 * j : 0x7fffffff;
     const int g = (int)__reduce_min_sync(0xffffffffu, (unsigned)mine);
-    pair = __ldg(notes + g);
+    pair = notes(g);
     if (mine == g) {
       best = 0;
 #pragma unroll
@@ -360,11 +383,11 @@ template <int Each> struct Groups {
   }
 };
 // Any number of groups: read again after each.
-template <> struct Groups<0> {
-  const float2* notes;
+template <class Notes> struct Groups<0, Notes> {
+  Notes notes;
   int groups, group, last_group;
   uint32_t key, last;
-  ASRN_DEV Groups(const float2* p, int n, uint32_t after = 0xffffffffu, int after_group = -1)
+  ASRN_DEV Groups(const Notes& p, int n, uint32_t after = 0xffffffffu, int after_group = -1)
       : notes(p), groups(n), last_group(after_group), last(after) {
     find();
   }
@@ -373,7 +396,7 @@ template <> struct Groups<0> {
     group = 0x7fffffff;
 #pragma unroll 8
     for (int g = threadIdx.x & 31; g < groups; g += 32) {
-      const uint32_t o = order_of(__ldg(&notes[g].x));
+      const uint32_t o = order_of(notes.largest(g));
       if ((o < last || (o == last && g > last_group)) && o > key) {
         key = o;
         group = g;
@@ -386,7 +409,7 @@ template <> struct Groups<0> {
     const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
     last = most;
     last_group = g;
-    pair = __ldg(notes + g);
+    pair = notes(g);
     if (group == g && key == most) find();
     __syncwarp();
     return g;
@@ -502,8 +525,7 @@ struct RowArgs {
   const uint4 *hc, *W;
   const int *pos, *tok;
   const float4* part;
-  const float2* notes;
-  const float* own;
+  const float *notes, *own;
   float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass
   float *logp, *entropy, *top_logp;              // by positions; logp may be null
   int64_t* top_tokens;
@@ -511,8 +533,8 @@ struct RowArgs {
 
 // U: steps of K whose loads are under way together: 2, so that many rows share an SM, or 8 where rows are few and a slow one's
 // latency is what counts.
-template <int Each, int U>
-__global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(const RowArgs f) {
+template <int Each, int U, bool Whole>
+__global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7) k_stats_rows(const RowArgs f) {
   const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
   const int64_t i = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   wait_previous();
@@ -576,13 +598,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(co
     return;
   }
   const uint4* h = f.hc + (int64_t)r * vecs;
-  const float2* notes = f.notes + (int64_t)r * f.groups;
+  const Notes<Whole> notes{f.notes + (int64_t)r * (Whole ? (f.V + 31) / 32 * 32 : 2 * f.groups)};
+  auto column_of = [&](int g, float2 note) { return Whole ? g : g * f.span + (int)(__float_as_uint(note.y) & 63u); };
 
   // The first `top` groups by lane, and the one after them.
   float2 pair = make_float2(kNothing, kNothing), held = pair;
   int held_group = 0, have = 0, after = -1;
   {
-    Groups<Each> groups(notes, f.groups);
+    Groups<Each, Notes<Whole>> groups(notes, f.groups);
     while (true) {
       after = groups.next(pair);
       if (after < 0 || have == top) break;
@@ -593,7 +616,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(co
       ++have;
     }
   }
-  const int column = held_group * f.span + column_of(held);
+  const int column = column_of(held_group, held);
 
   // Their largest, and the target: in most rows these are the answer, as the products summed them. For the row's scores may be off by
   // `slack` (sums of 16 products, truncated; with twice the magnitudes of the likeliest one), notes by their low bits more.
@@ -669,9 +692,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(co
       expand(__shfl_sync(0xffffffffu, held_group, q), __shfl_sync(0xffffffffu, column, q), about_put);
   }
   if (after >= 0 && above(pair.x) >= low()) {
-    Groups<0> rest(notes, f.groups, order_of(pair.x), after);
+    Groups<0, Notes<Whole>> rest(notes, f.groups, order_of(pair.x), after);
     for (; after >= 0 && above(pair.x) >= low(); after = rest.next(pair)) {
-      const int c = after * f.span + column_of(pair);
+      const int c = column_of(after, pair);
       best.put(dots16<U, false>(h, f.W, vecs, c, c, nullptr).of(0), c);
       if (pair.y > -3e38f && above(pair.y) >= low()) expand(after, c, about_put);
     }
@@ -720,7 +743,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : 7) k_stats_rows(co
       };
       if (y >= 0) exact_put(0.f, y);
       for (int g = 0; g < f.groups; ++g) {
-        const float v = __ldg(&notes[g].x);
+        const float v = notes.largest(g);
         if (v > -3e38f && above(v) >= low()) expand(g, -1, exact_put);
       }
     }
@@ -873,22 +896,22 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   float* own = reinterpret_cast<float*>(W + ws.top);
   float4* part = reinterpret_cast<float4*>(W + ws.part);
   float2* notes = reinterpret_cast<float2*>(W + ws.notes);
-  const int span = span_of(V), groups = (int)notes_of(V);
+  const int span = span_of(V, top), groups = (int)notes_of(V, top);
   if (top)
     st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   else
     st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   if (st) return st;
   const RowArgs f{N, (int)V, d, top, parts, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
-                  reinterpret_cast<const uint4*>(weight), pos, tok, part, notes, own, lse2,
+                  reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own, lse2,
                   reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent), logp, entropy, top_logp,
                   top_tokens};
-  auto rows = N <= (int64_t)gemm::sm_count() * kRowWarps ? groups <= 512    ? k_stats_rows<16, 8>
-                                                           : groups <= 1024 ? k_stats_rows<32, 8>
-                                                                            : k_stats_rows<0, 8>
-              : groups <= 512                            ? k_stats_rows<16, 2>
-              : groups <= 1024                           ? k_stats_rows<32, 2>
-                                                         : k_stats_rows<0, 2>;
+  const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps;
+  auto rows = span == 1       ? V <= 512 ? (few ? k_stats_rows<16, 8, true> : k_stats_rows<16, 2, true>)
+                                         : (few ? k_stats_rows<64, 8, true> : k_stats_rows<64, 2, true>)
+              : groups <= 512  ? (few ? k_stats_rows<16, 8, false> : k_stats_rows<16, 2, false>)
+              : groups <= 1024 ? (few ? k_stats_rows<32, 8, false> : k_stats_rows<32, 2, false>)
+                               : (few ? k_stats_rows<0, 8, false> : k_stats_rows<0, 2, false>);
   return launch_next(rows, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, s, f);
 }
 
