@@ -4,14 +4,15 @@
 // The products are those of the log probabilities alone (head.cu): 2 N V d operations forward and 6 N V d backward, bound by the
 // tensor cores at any training size, and by the weight's bytes where rows are few.
 //
-//   k_gemm<Scan>   scores by tiles; each thread keeps of its row's 128 columns the maximum m, S = sum exp(s - m), T = sum
-//                  exp(s - m) (s - m); the target is in none of the sums. Where the likeliest tokens are wanted, it notes the
-//                  two largest scores of each group of 32 to 128 columns, with their column in the low 7 bits
+//   k_gemm<Scan>   scores by tiles; each thread keeps of its row's 64 columns the maximum m, S = sum exp(s - m), T = sum
+//                  exp(s - m) (s - m); the target is in none of the sums. Where the likeliest tokens are wanted, it notes of each
+//                  group of 32 or 64 columns the largest score, and the second largest with the largest one's column in its low
+//                  6 bits (small vocabularies: all scores)
 //   k_stats_few    the same for few rows
-//   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups in the order of their largest notes, for as long as one
-//                  may hold one of the likeliest tokens, whose scores are formed again: by sums in fp32, and where these
-//                  leave the order open by sums in 64 bits. So the order of the tokens is that of their exact scores, equal
-//                  ones by their numbers.
+//   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups with the largest scores, which in most rows are the
+//                  likeliest tokens'. Where the products' rounding leaves their order open, or a second score of a group may
+//                  count, scores are formed again from h and W: by sums in fp32, and where these leave the order open by sums
+//                  in 64 bits. So the order of the tokens is that of their exact scores, equal ones by their numbers.
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
 #include "head.cuh"
 #include "products.cuh"
@@ -184,7 +185,7 @@ template <bool Top> struct Scan {
   }
 };
 
-// The same for up to kFewRows rows and kFewScores scores, bound by the weight's bytes: block = 128 columns (one group), a warp 16 of them and all of K;
+// The same for up to kFewRows rows and kFewScores scores, bound by the weight's bytes: block = 128 columns, a warp 16 of them and all of K;
 // mma.sync from registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a
 // lane takes 8 neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do.
 // Then a warp per row of h over the 128 scores.
@@ -744,7 +745,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
       if (y >= 0) exact_put(0.f, y);
       for (int g = 0; g < f.groups; ++g) {
         const float v = notes.largest(g);
-        if (v > -3e38f && above(v) >= low()) expand(g, -1, exact_put);
+        if (!(v > -3e38f && above(v) >= low())) continue;
+        // nothing of it comes before the last one that counts so far, not as its equal either
+        const double last = __shfl_sync(0xffffffffu, exact.score, top - 1);
+        const int number = __shfl_sync(0xffffffffu, exact.token, top - 1);
+        if ((double)above(v) < last || ((double)above(v) == last && number < g * f.span)) continue;
+        expand(g, -1, exact_put);
       }
     }
     best.token = exact.token;

@@ -181,6 +181,36 @@ def test_scores_that_fp32_sums_cannot_tell_apart(cuda):
     check(h.cuda(), w.cuda(), targets(20, V, 27), top=32, grads=False)
 
 
+@pytest.mark.parametrize('V', [220, 1500, 5003, 33001, 70001])
+@pytest.mark.parametrize('N', [3, 100, 700])
+@pytest.mark.parametrize('top', [1, 6, 20, 32])
+def test_rankings_of_every_kind(cuda, V, N, top):
+    """Every way the notes are kept and the rows are ranked: plain scores, twins, near twins, several of a group, rows of zeros."""
+    d = 72
+    w = rand((V, d), 60, 0.2)
+    w[V // 2:V // 2 + 40] *= 4                            # neighbours that are likely
+    w[-30:] = w[V // 2:V // 2 + 30].clone()               # and their twins
+    w[-60:-30] = w[V // 2:V // 2 + 30].clone()
+    w[-60:-30, 3] += 2.0 ** -8 * w[-60:-30, 3]            # near twins: one coordinate's last bit or two
+    h = rand((N, d), 61)
+    h[::5] = 0
+    h[1::5, 3] = 2.0 ** -9                                # where that coordinate hardly counts
+    check(h, w, targets(N, V, 62, 7), top=top, grads=False)
+    check(h, w, None, tau=0.7, top=top, grads=False)
+
+
+def test_weights_of_zeros(cuda):
+    """All tokens are as likely: the first ones, whatever the hidden state."""
+    import asrn_b200 as asrn
+    for N, V in ((700, 5003), (6, 50304), (600, 1000)):
+        h, w = rand((N, 64), 63), torch.zeros(V, 64, dtype=torch.bfloat16, device='cuda')
+        r = check(h, w, targets(N, V, 64), top=20, grads=False)
+        assert torch.equal(r.top_tokens, torch.arange(20, device='cuda').expand(N, 20))
+        w[V // 3:] = rand((V - V // 3, 64), 65, 0.1)      # and where a part of them is
+        check(h, w, None, top=20, grads=False)
+        check(-h.abs(), w.abs(), targets(N, V, 66), top=20, grads=False)
+
+
 def test_likeliest_tokens_in_one_group(cuda):
     """Common tokens have neighbouring numbers: all of the likeliest stand in one group of 128, or in two."""
     V, d = 4000, 64
