@@ -409,7 +409,7 @@ struct StatsOut {
   Tensor logp, entropy, top_logp, top_tokens, saved, weight;
 };
 
-StatsOut stats_forward(const Tensor& h, const Tensor& weight, const Tensor& tokens, double tau, int64_t top) {
+StatsOut stats_forward(const Tensor& h, const Tensor& weight, const Tensor& tokens, double tau, int64_t top, bool keep) {
   const c10::Device dev = h.device();
   const int64_t V = weight.size(0), d = weight.size(1), N = h.numel() / d;
   const Tensor hr = rows(h), tok = tokens.defined() ? tokens.contiguous() : tokens;
@@ -424,12 +424,13 @@ StatsOut stats_forward(const Tensor& h, const Tensor& weight, const Tensor& toke
     o.top_logp = empty(wide, at::kFloat, dev);
     o.top_tokens = empty(wide, at::kLong, dev);
   }
-  const size_t nb_saved = asrn_head_stats_saved_bytes(N, d), nb = asrn_head_stats_workspace_bytes(N, V, d, top, 0);
-  o.saved = scratch(nb_saved, dev);
+  const bool saved = keep || tok.defined();                  // what is gathered needs the room
+  const size_t nb_saved = saved ? asrn_head_stats_saved_bytes(N, d) : 0, nb = asrn_head_stats_workspace_bytes(N, V, d, top, 0);
+  if (saved) o.saved = scratch(nb_saved, dev);
   const Tensor ws = scratch(nb, dev);
   check(asrn_head_stats_forward(N, V, d, hr.data_ptr(), o.weight.data_ptr(), (const int64_t*)data_or_null(tok), (float)tau, top,
                                 (float*)data_or_null(o.logp), o.entropy.data_ptr<float>(), (float*)data_or_null(o.top_logp),
-                                (int64_t*)data_or_null(o.top_tokens), o.saved.data_ptr(), nb_saved, ws.data_ptr(), nb,
+                                (int64_t*)data_or_null(o.top_tokens), data_or_null(o.saved), nb_saved, ws.data_ptr(), nb,
                                 status_word("head_stats", dev), stream_of(dev)),
         "asrn_head_stats_forward");
   return o;
@@ -439,7 +440,7 @@ StatsOut stats_forward(const Tensor& h, const Tensor& weight, const Tensor& toke
 struct HeadStats : torch::autograd::Function<HeadStats> {
   static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& weight, const MaybeTensor& tokens,
                                double tau, int64_t top) {
-    const StatsOut o = stats_forward(h, weight, or_none(tokens), tau, top);
+    const StatsOut o = stats_forward(h, weight, or_none(tokens), tau, top, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({o.weight, o.saved});
     ctx->saved_data["sizes"] = h.sizes().vec();
@@ -502,7 +503,7 @@ std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> head_stats(Tensor h, T
   MaybeTensor logp, top_logp, top_tokens;
   if (!recorded({&h, &weight})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const StatsOut o = stats_forward(h, weight, tokens, tau, top);
+    const StatsOut o = stats_forward(h, weight, tokens, tau, top, false);
     if (o.logp.defined()) logp = o.logp;
     if (top) {
       top_logp = o.top_logp;

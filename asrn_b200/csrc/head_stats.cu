@@ -84,7 +84,7 @@ ASRN_DEV float2 note_of(float most, float first, float second) {
 template <bool Top> struct Scan {
   static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
   struct Params {
-    const int* tok;
+    const int* tok;                        // null: no targets
     float k;                               // log2(e) / tau
     float* top;                            // the targets' unscaled scores
     float4* part;                          // m, S, T log2(e): [rows][parts]
@@ -97,7 +97,7 @@ template <bool Top> struct Scan {
   float m = -INFINITY, s = 0.f, t = 0.f, most = kNothing, first = kNothing, second = kNothing;
   ASRN_DEV Scan(const Params& pp, int r, int rows, const gemm::Shape& sh, const gemm::Tile& u, int quarter)
       : p(pp), row(r), V(sh.N), y(-1), at(u.n * (gemm::kBN / kPart) + quarter), parts(parts_of(sh.N)), on(r < rows) {
-    if (on) y = p.tok[r];
+    if (on && p.tok) y = p.tok[r];
   }
   template <class O> ASRN_DEV void chunk(float* v, int c, O&, const CUtensorMap*, const CUtensorMap*) {
     if (c >= V) return;
@@ -192,8 +192,8 @@ template <bool Top> struct Scan {
 constexpr int64_t kFewRows = 64, kFewScores = (int64_t)1 << 20;
 template <int NT, bool Top>
 __global__ void __launch_bounds__(256)
-k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w, const int* __restrict__ count,
-            const typename Scan<Top>::Params p) {
+k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w,
+            const int* __restrict__ count, const typename Scan<Top>::Params p) {
   constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
   __shared__ __align__(16) float sh[8 * NT][132];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -203,7 +203,7 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
   const __nv_bfloat16* hp = h + (int64_t)g * d + 8 * t;
   wait_previous();
   let_next();
-  const int rows = *count;
+  const int rows = count ? *count : N;
   float acc[NT][4] = {};
   for (int k0 = 0; k0 < d; k0 += kU * 32) {
     uint4 a[kU][2], b[kU][NT];
@@ -237,7 +237,7 @@ k_stats_few(int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat
   __syncthreads();
   const int parts = parts_of(V);
   for (int r = wid; r < rows && r < 8 * NT; r += 8) {
-    const int y = p.tok[r], c0 = blockIdx.x * 128 + lane * 4;
+    const int y = p.tok ? p.tok[r] : kNoTarget, c0 = blockIdx.x * 128 + lane * 4;
     const float4 q = *reinterpret_cast<const float4*>(&sh[r][lane * 4]);
     float v[4] = {q.x, q.y, q.z, q.w};
     float m = -INFINITY, first = kNothing, second = kNothing;
@@ -524,10 +524,10 @@ struct RowArgs {
   int V, d, top, parts, span, groups;
   float k, inv_tau;
   const uint4 *hc, *W;
-  const int *pos, *tok;
+  const int *pos, *tok;                          // null: every position is a row, without a target
   const float4* part;
   const float *notes, *own;
-  float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass
+  float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass; or null
   float *logp, *entropy, *top_logp;              // by positions; logp may be null
   int64_t* top_tokens;
 };
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   wait_previous();
   let_next();
   if (i >= f.N) return;
-  const int r = f.pos[i], y = r >= 0 ? f.tok[r] : -1;
+  const int r = f.pos ? f.pos[i] : (int)i, y = r < 0 ? -1 : f.tok ? f.tok[r] : kNoTarget;
   float lp = 0.f, H = 0.f, l2 = 0.f, own = 0.f;
   double base = 0.0;
   if (r >= 0) {                                  // the row's sums: by lanes, then the lanes'
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     H = row.H;
     l2 = row.l2;
     base = row.base;
-    if (lane == 0) {
+    if (lane == 0 && f.lse2) {
       f.lse2[r] = l2;
       f.kept_logp[r] = lp;
       f.kept_ent[r] = H;
@@ -838,19 +838,19 @@ int launch_next(void (*kernel)(P...), int64_t blocks, int threads, cudaStream_t 
 }
 
 template <int NT, bool Top>
-int few(int64_t V, int d, const void* hc, const void* weight, const int* count, const typename Scan<Top>::Params& p,
+int few(int64_t N, int64_t V, int d, const void* hc, const void* weight, const int* count, const typename Scan<Top>::Params& p,
         cudaStream_t s) {
-  return launch_next(k_stats_few<NT, Top>, parts_of(V) / 2, 256, s, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
+  return launch_next(k_stats_few<NT, Top>, parts_of(V) / 2, 256, s, (int)N, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
                      reinterpret_cast<const __nv_bfloat16*>(weight), count, p);
 }
 template <bool Top>
 int scan(int64_t N, int64_t V, int d, const void* hc, const void* weight, const gemm::Shape& sh,
          const typename Scan<Top>::Params& p, cudaStream_t s) {
   if (N > kFewRows || N * V > kFewScores) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
-  return N <= 8    ? few<1, Top>(V, d, hc, weight, sh.m_dev, p, s)
-         : N <= 16 ? few<2, Top>(V, d, hc, weight, sh.m_dev, p, s)
-         : N <= 32 ? few<4, Top>(V, d, hc, weight, sh.m_dev, p, s)
-                   : few<8, Top>(V, d, hc, weight, sh.m_dev, p, s);
+  return N <= 8    ? few<1, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
+         : N <= 16 ? few<2, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
+         : N <= 32 ? few<4, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
+                   : few<8, Top>(N, V, d, hc, weight, sh.m_dev, p, s);
 }
 
 }  // namespace
@@ -884,19 +884,21 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
     return ASRN_ERR_ARG;
   const StatsSaved sv = stats_saved(N, d);
   const StatsWs ws = stats_ws(N, V, top);
-  if (!saved || saved_bytes < sv.total || (uintptr_t)saved % 256 || !workspace || workspace_bytes < ws.total ||
+  if (!saved && tokens) return ASRN_ERR_WORKSPACE;
+  if ((saved && (saved_bytes < sv.total || (uintptr_t)saved % 256)) || !workspace || workspace_bytes < ws.total ||
       (uintptr_t)workspace % 256)
     return ASRN_ERR_WORKSPACE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* S = reinterpret_cast<char*>(saved);
   char* W = reinterpret_cast<char*>(workspace);
-  if ((st = head_gather(N, V, d, h, tokens, reinterpret_cast<int*>(W + ws.counts), S, sv.head, s))) return st;
-  const int *tok = reinterpret_cast<int*>(S + sv.head.tok), *pos = reinterpret_cast<int*>(S + sv.head.pos);
-  const void* hc = S + sv.head.hc;
-  float* lse2 = reinterpret_cast<float*>(S + sv.head.lse2);
+  // Nothing kept and every position counted: h's rows as they lie.
+  if (S && (st = head_gather(N, V, d, h, tokens, reinterpret_cast<int*>(W + ws.counts), S, sv.head, s))) return st;
+  auto kept = [&](size_t at) { return S ? S + at : nullptr; };
+  const int *tok = reinterpret_cast<int*>(kept(sv.head.tok)), *pos = reinterpret_cast<int*>(kept(sv.head.pos));
+  const void* hc = S ? kept(sv.head.hc) : h;
   const int parts = parts_of(V);
   gemm::Shape sh{};
-  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = reinterpret_cast<int*>(S + sv.head.count); sh.group = 16;
+  sh.M = (int)N; sh.N = (int)V; sh.K = d; sh.m_dev = reinterpret_cast<int*>(kept(sv.head.count)); sh.group = 16;
   sh.status = status;
   const float inv_tau = 1.f / tau, k = kLog2e * inv_tau;
   float* own = reinterpret_cast<float*>(W + ws.top);
@@ -909,9 +911,9 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
     st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   if (st) return st;
   const RowArgs f{N, (int)V, d, top, parts, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
-                  reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own, lse2,
-                  reinterpret_cast<float*>(S + sv.head.rest), reinterpret_cast<float*>(S + sv.ent), logp, entropy, top_logp,
-                  top_tokens};
+                  reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own,
+                  reinterpret_cast<float*>(kept(sv.head.lse2)), reinterpret_cast<float*>(kept(sv.head.rest)),
+                  reinterpret_cast<float*>(kept(sv.ent)), logp, entropy, top_logp, top_tokens};
   const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps;
   auto rows = span == 1       ? V <= 512 ? (few ? k_stats_rows<16, 8, true> : k_stats_rows<16, 2, true>)
                                          : (few ? k_stats_rows<64, 8, true> : k_stats_rows<64, 2, true>)

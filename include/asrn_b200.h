@@ -328,7 +328,7 @@ int asrn_linear_backward(int64_t N, int32_t d, int32_t n, const void* dy, int32_
  * (0 to 32, at most V) likeliest tokens, top_tokens (N, top) int64 with their log probabilities top_logp (N, top), by
  * their scores summed in 64 bits, equal ones by their numbers. tokens may be NULL: every position counts, and logp is not
  * written. A negative token leaves its position out: 0 everywhere and tokens -1; a token >= V, and scores without a finite log of
- * their sum of exponentials, give NaN and tokens -1.
+ * their sum of exponentials, give NaN and tokens -1. `saved` may be NULL without tokens, where no backward pass follows.
  * asrn_head_stats_backward: from g = dL/dlogp and g_entropy = dL/dentropy (N), either may be NULL. */
 size_t asrn_head_stats_saved_bytes(int64_t N, int32_t d);
 size_t asrn_head_stats_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t top, int32_t backward);

@@ -265,6 +265,20 @@ def test_logp_agrees_with_head_logprobs(cuda):
         assert (p.float() - q.float()).abs().max() <= 2 * U * p.float().abs().max()
 
 
+@pytest.mark.parametrize('N,V', [(1, 50304), (9, 5003), (64, 700), (130, 5003), (900, 40000)])
+def test_without_targets_and_gradients(cuda, N, V):
+    """Nothing is gathered then: the values are those of the call that keeps them."""
+    import asrn_b200 as asrn
+    h, w = rand((N, 136), 70), rand((V, 136), 71, 0.1)
+    a = check(h, w, None, top=7, grads=False)
+    b = check(h, w, None, top=7)
+    assert torch.equal(a.entropy, b.entropy) and torch.equal(a.top_tokens, b.top_tokens) and torch.equal(a.top_logp, b.top_logp)
+    h[N // 2] = float('nan')
+    c = asrn.head_stats(h, w, top=7)
+    ok = torch.arange(N, device='cuda') != N // 2
+    assert torch.equal(c.entropy[ok], a.entropy[ok]) and c.entropy[N // 2].isnan() and (c.top_tokens[N // 2] == -1).all()
+
+
 def test_shapes_views_streams_autocast_and_empty(cuda):
     import asrn_b200 as asrn
     big, w, y = rand((6, 50, 100), 40), rand((321, 64), 41, 0.1), targets(300, 321, 42).view(6, 50)

@@ -156,6 +156,44 @@ def test_norm_views_streams_and_empty(cuda):
     assert torch.equal(gx, gr)
 
 
+@pytest.mark.parametrize('d', [768, 333])
+@pytest.mark.parametrize('x,res', [(BF16, F32), (F32, F32), (F32, None)])
+def test_norm_one_gradient_at_a_time_and_shared_inputs(cuda, d, x, res):
+    import asrn_b200 as asrn
+    t = dict(x=rand((90, d), 100, dtype=x), w=rand((d,), 101, dtype=F32), b=rand((d,), 102, dtype=F32),
+             res=None if res is None else rand((90, d), 103, dtype=res))
+    t = {k: v for k, v in t.items() if v is not None}
+    dy = rand((90, d), 104, dtype=x)
+    call = lambda q: asrn.layer_norm(q['x'], q['w'], q['b'], residual=q.get('res'))  # noqa: E731
+    first = lambda r: r if res is None else r[0]  # noqa: E731
+    every = {k: v.clone().requires_grad_() for k, v in t.items()}
+    want = dict(zip(every, torch.autograd.grad(first(call(every)), tuple(every.values()), dy)))
+    for need in t:
+        one = {k: v.clone().requires_grad_(k == need) for k, v in t.items()}
+        got, = torch.autograd.grad(first(call(one)), (one[need],), dy)
+        assert torch.equal(got, want[need]), need
+    if x == res:                                          # the same tensor as both summands
+        both = t['x'].clone().requires_grad_()
+        y, s = asrn.layer_norm(both, t['w'], t['b'], residual=both)
+        got, = torch.autograd.grad(y, (both,), dy)
+        two = t['x'].clone().requires_grad_()
+        want, = torch.autograd.grad(asrn.layer_norm(2 * two, t['w'], t['b']), (two,), dy)
+        assert torch.equal(s, 2 * both) and torch.equal(got, want)
+
+
+def test_norm_rows_at_the_end_of_their_memory(cuda):
+    """Odd widths are read by whole vectors: what lies before and behind the rows reaches nothing and is left alone."""
+    import asrn_b200 as asrn
+    for N, d in ((1, 3), (2, 7), (5, 77), (9, 130), (7, 333), (3, 1021), (3, 2051), (3, 5001)):
+        room = torch.full((N * d + 64,), float('nan'), device='cuda')
+        x = room[32:32 + N * d].view(N, d)                # 128 bytes in: aligned, NaN on both sides
+        x.copy_(rand((N, d), 105, dtype=F32))
+        w, b = rand((d,), 106, dtype=F32), rand((d,), 107, dtype=F32)
+        check_norm(x, w, b)
+        assert torch.equal(asrn.layer_norm(x, w, b), asrn.layer_norm(x.clone(), w, b))
+        assert room[:32].isnan().all() and room[32 + N * d:].isnan().all()
+
+
 def test_norm_repeats_bit_for_bit_and_in_a_graph(cuda):
     import asrn_b200 as asrn
     x, w, b = rand((3001, 520), 23, dtype=F32), rand((520,), 24, dtype=F32), rand((520,), 25, dtype=F32)

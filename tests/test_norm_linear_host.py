@@ -75,7 +75,7 @@ def test_stats_refusals(lib, at):
     assert f(tau=0.0) == ARG and f(tau=float('nan')) == ARG and f(top=-1) == ARG and f(top=10) == ARG
     assert f(V=99, top=33) == UNSUPPORTED and f(h=None) == ARG and f(w=odd) == ARG and f(en=None) == ARG
     assert f(lp=None) == ARG and f(tl=None) == ARG and f(tt=None) == ARG
-    assert f(sv=None) == WORKSPACE and f(ns=8) == WORKSPACE and f(nw=8) == WORKSPACE and f(ws=odd) == WORKSPACE
+    assert f(sv=None) == WORKSPACE and f(tok=None, sv=None, nw=8) == WORKSPACE and f(ns=8) == WORKSPACE and f(nw=8) == WORKSPACE and f(ws=odd) == WORKSPACE
     assert f(N=0) == 0
     g = lambda N=4, w=ok, tau=1.0, sv=ok, ns=1 << 40, dh=ok, ws=ok, nw=1 << 40: lib.asrn_head_stats_backward(  # noqa: E731
         N, 9, 16, w, sv, ns, tau, None, None, dh, ok, ws, nw, None, None)
