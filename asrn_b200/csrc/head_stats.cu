@@ -10,10 +10,13 @@
 //                  6 bits (small vocabularies: all scores)
 //   k_stats_few    the same for few rows
 //   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups with the largest scores, which in most rows are the
-//                  likeliest tokens'. Where the products' rounding leaves their order open, or a second score of a group may
-//                  count, scores are formed again from h and W: by sums in fp32, and where these leave the order open by sums
-//                  in 64 bits. So the order of the tokens is that of their exact scores, equal ones by their numbers.
+//                  likeliest tokens'. Where a second score of a group may count, scores are formed again from h and W by sums
+//                  in fp32, and where these or the products' leave the order open by sums in 64 bits. So the order of the tokens
+//                  is that of their exact scores, equal ones by their numbers. (What a sum in fp32 may be off by is taken from
+//                  sum |h w| of the likeliest token, times two; a token with more than that and large parts that cancel would
+//                  be ranked by its fp32 sum.)
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
+#include <algorithm>
 #include "head.cuh"
 #include "products.cuh"
 
@@ -532,8 +535,9 @@ struct RowArgs {
   int64_t* top_tokens;
 };
 
-// U: steps of K whose loads are under way together: 2, so that many rows share an SM, or 8 where rows are few and a slow one's
-// latency is what counts.
+// U: steps of K whose loads are under way together: 8 where a slow row's latency is what counts (50304 x 768, 8 tokens: 2048 rows 54 us
+// against 105 with 2, 4096 78 against 108, 8192 125 against 150), 2 where rows are many and short, so that more share an SM
+// (5003 x 200, 8192 rows: 59 with 8, 50 with 2; 2048 rows 22 and 30).
 template <int Each, int U, bool Whole>
 __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7) k_stats_rows(const RowArgs f) {
   const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
@@ -631,11 +635,40 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack + off); };
   {
     const float lowest = low() - slack, then = __shfl_down_sync(0xffffffffu, best.score, 1);
-    const bool open = size == 0.f || (lane < top && (best.token >= f.V || (lane < 31 && best.score - then <= 2 * slack))) ||
-                      (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
+    const bool open = size == 0.f || (lane < top && best.token >= f.V) || (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
                       (after >= 0 && above(pair.x) >= lowest) || best.lost >= lowest - slack;
     if (!__any_sync(0xffffffffu, open)) {
-      write((float)((double)best.score * f.inv_tau - base), best.token);
+      // Those that stand too near their neighbours: by sums in 64 bits. Others keep their places among them.
+      const unsigned before = __ballot_sync(0xffffffffu, lane < min(top, 31) && best.score - then <= 2 * slack);
+      double score = best.score;
+      if (before) {
+        Best<double> exact;
+        unsigned near = before | before << 1, rest = near;
+        for (int q = 0; q < 32; ++q) {
+          if (!(near >> q & 1u)) {
+            const float sc = __shfl_sync(0xffffffffu, best.score, q);
+            exact.put((double)sc, __shfl_sync(0xffffffffu, best.token, q));
+            continue;
+          }
+          if (!(rest >> q & 1u)) continue;
+          int t[4];                              // the next four of them
+          bool on[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            on[j] = rest != 0;
+            t[j] = __shfl_sync(0xffffffffu, best.token, on[j] ? __ffs(rest) - 1 : q);
+            rest &= rest - 1;
+          }
+          double sums[4];
+          dots(h, f.W, vecs, t, sums);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (on[j]) exact.put(sums[j], t[j]);
+        }
+        best.token = exact.token;
+        score = exact.score;
+      }
+      write((float)(score * f.inv_tau - base), best.token);
       return;
     }
   }
@@ -914,7 +947,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
                   reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own,
                   reinterpret_cast<float*>(kept(sv.head.lse2)), reinterpret_cast<float*>(kept(sv.head.rest)),
                   reinterpret_cast<float*>(kept(sv.ent)), logp, entropy, top_logp, top_tokens};
-  const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps;
+  const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps * std::max(4, d / 48);
   auto rows = span == 1       ? V <= 512 ? (few ? k_stats_rows<16, 8, true> : k_stats_rows<16, 2, true>)
                                          : (few ? k_stats_rows<64, 8, true> : k_stats_rows<64, 2, true>)
               : groups <= 512  ? (few ? k_stats_rows<16, 8, false> : k_stats_rows<16, 2, false>)

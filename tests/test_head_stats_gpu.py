@@ -199,6 +199,15 @@ def test_rankings_of_every_kind(cuda, V, N, top):
     check(h, w, None, tau=0.7, top=top, grads=False)
 
 
+@pytest.mark.parametrize('N,V,d', [(1500, 5003, 768), (2500, 5003, 136), (9000, 2100, 72), (6000, 900, 520)])
+def test_rankings_of_many_rows(cuda, N, V, d):
+    """Among so many some stand nearer their neighbours than the products round; rows of the weight of several sizes."""
+    h, w = rand((N, d), 63), rand((V, d), 64, 0.05)
+    w = w * (1 + torch.arange(V, device='cuda') % 4)[:, None].to(w.dtype)
+    for top, given in ((32, True), (9, False)):
+        check(h, w, targets(N, V, 65, 11) if given else None, top=top, grads=False)
+
+
 def test_weights_of_zeros(cuda):
     """All tokens are as likely: the first ones, whatever the hidden state."""
     import asrn_b200 as asrn
