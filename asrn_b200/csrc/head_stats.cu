@@ -84,6 +84,9 @@ ASRN_DEV float2 note_of(float most, float first, float second) {
   return make_float2(most, __uint_as_float((__float_as_uint(second) & ~63u) | (__float_as_uint(first) & 63u)));
 }
 
+// Bound by the tensor cores and, where the two largest of each group are tracked, by the epilogue's instructions beside them (16 warps;
+// with 8 the epilogue waits for itself): 16384 x 50304 x 768 (1.27 TFLOP) 870 us without, 1000 us with, 1.27 PFLOP/s; a look at
+// 2048 rows: tensor pipe 62 % active, L2 hits 84 %.
 template <bool Top> struct Scan {
   static constexpr int kWarps = 16, kOwn = 1, kTable = 0;
   struct Params {
@@ -188,11 +191,13 @@ template <bool Top> struct Scan {
   }
 };
 
-// The same for up to kFewRows rows and kFewScores scores, bound by the weight's bytes: block = 128 columns, a warp 16 of them and all of K;
-// mma.sync from registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a
-// lane takes 8 neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do.
-// Then a warp per row of h over the 128 scores.
-constexpr int64_t kFewRows = 64, kFewScores = (int64_t)1 << 20;
+// The same for few rows, bound by the weight's bytes: block = 128 columns, a warp 16 of them and all of K; mma.sync from
+// registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a lane takes 8
+// neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do. Then a warp per row
+// of h over the 128 scores. 8 x 50304 x 768: 11 to 12 us, 6.4 TB/s and more (part of the 77 MB may be left in L2).
+// The whole call as a graph replay, so | by tiles, us: 50304 x 768, 1 row 17 | 22, 8 rows 19 | 23, 20 rows 26 | 24;
+// 16384 x 768, 8 rows 10 | 12, 16 rows 17 | 13; 5003 x 200, 32 rows 7.8 | 8.9, 64 rows 11.4 | 9.3.
+bool few_rows(int64_t N, int64_t V) { return N <= 8 || (N <= 32 && N * V < (1 << 18)); }
 template <int NT, bool Top>
 __global__ void __launch_bounds__(256)
 k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w,
@@ -799,7 +804,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   write((float)(score * f.inv_tau - base), best.token);
 }
 
-// dS of one chunk in bf16; the rows that pad the last tile get zeros. With x = log2 p: dS = p (a + b x).
+// dS of one chunk in bf16; the rows that pad the last tile get zeros. With x = log2 p: dS = p (a + b x). 2048 x 50304 x 768: 126 us, tensor
+// pipe 74 % active, 1.25 PFLOP/s.
 struct Slope {
   static constexpr int kWarps = 8, kOwn = 2, kTable = 0;
   struct Params {
@@ -879,11 +885,10 @@ int few(int64_t N, int64_t V, int d, const void* hc, const void* weight, const i
 template <bool Top>
 int scan(int64_t N, int64_t V, int d, const void* hc, const void* weight, const gemm::Shape& sh,
          const typename Scan<Top>::Params& p, cudaStream_t s) {
-  if (N > kFewRows || N * V > kFewScores) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
+  if (!few_rows(N, V)) return gemm::launch<false, false, Scan<Top>>(hc, d, weight, d, sh, p, s);
   return N <= 8    ? few<1, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
          : N <= 16 ? few<2, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
-         : N <= 32 ? few<4, Top>(N, V, d, hc, weight, sh.m_dev, p, s)
-                   : few<8, Top>(N, V, d, hc, weight, sh.m_dev, p, s);
+                   : few<4, Top>(N, V, d, hc, weight, sh.m_dev, p, s);
 }
 
 }  // namespace

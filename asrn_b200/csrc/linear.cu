@@ -10,7 +10,8 @@
 //   k_linear_few   up to kFewRows rows: memory bound (the weight is read once, 2 operations a byte and row), so the rows of W are
 //                  spread over all SMs, sixteen a block, K over its warps; mma.sync, whose 16 x 8 tiles fit such rows
 //   k_gemm<Fused>  more rows: tcgen05 products, the rest in the epilogue
-//   k_linear_slope backward: dA in bf16 and its columns' sums by 64 rows
+//   k_linear_slope backward: dA in bf16 and its columns' sums by 64 rows; memory bound: 32768 x 1536 from bf16 dY 47 us (302 MB,
+//                  6.3 TB/s), 32768 x 768 from fp32 dY without a slope 24.5
 //   k_gemm x 2     dX, dW (dW in shares of the rows where its tiles are few)
 //   k_colsum       db
 #include <cuda_fp16.h>
@@ -25,6 +26,9 @@ namespace {
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
 constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
 constexpr int64_t kTwiceRows = 512;
+// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 7.0, 65 rows | 11.0; 1536 -> 768 7.9 | 14.5. Where y has more
+// values the tiles fill the SMs: 768 -> 8192, 64 rows 13.3 | 11.1; 768 -> 16384, 32 rows 12.2 | 11.4; 768 -> 50304, 16 rows 17,
+// 32 rows 33 | 21.
 constexpr int64_t kFewRows = 64, kFewValues = (int64_t)1 << 20;
 
 ASRN_DEV uint32_t half2_of(float a, float b) {
@@ -92,6 +96,9 @@ struct Rest {
   int keep;                                  // the slopes are wanted
 };
 
+// 16 warps: with 8 the epilogue, not the products, sets the pace. 32768 x 768 x 1536 (77 GFLOP; 46 us at the measured burst, a library
+// product alone 61.5 us): without anything 65 us, gelu 77, with the slopes kept 85, bf16 residual 80, fp32 106; 32768 x 1536 x 768: 63,
+// 70, 76, fp32 residual 82.
 struct Fused {
   static constexpr int kWarps = 16, kOwn = 2, kTable = 0;
   using Params = Rest;
@@ -192,7 +199,8 @@ struct Fused {
 // 16 columns of y for up to 8 NT rows of x: A = 16 rows of W, B = the rows of x. The order of K inside a tile is free as long as
 // A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
 // memory, and four lanes read 64 neighbouring bytes. A block's warps take every eighth 32 of K; the blocks of a cluster share K
-// where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's.
+// where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's. Graph replays at 768 ->
+// 1536: 1, 8, 16, 32, 64 rows 3.5, 3.6, 4.5, 5.7, 7.0 us, launch and one round trip to memory (2.4 MB take 0.4).
 constexpr int kFewWarps = 8;
 template <int NT>
 __global__ void __launch_bounds__(kFewWarps * 32)

@@ -225,7 +225,7 @@ struct Up {
 // dG = sum -> dA = dG gelu'(a') and gelu(a') in bf16, and dA's column sums by 32 rows. 87 us at 32768 x 1536 x 768 (210 with
 // libm's functions and direct stores; 100 computed, 92 with the table, 87 with the codes by blocks).
 // a' = code 2^e takes 256 values for each e, so gelu and gelu' of the 16 exponents that matter lie in a table of shared
-// memory (gelu in bf16, as it leaves; gelu' in fp16, so that both fit 32 bits: its 2^-12 adds 1 % to the bf16 rounding of
+// memory (gelu in bf16, as it leaves; gelu' in fp16, so that both fit 32 bits: its 2^-11 adds 1 % to the bf16 rounding of
 // dA, and where it is subnormal, for a < -4.6, it is off by up to 2^-25, less than gelu_both's own 3.6e-7): one 32-bit load
 // for an element instead of about 20 instructions. Blocks with another exponent (all of a below 0.004, or some above 254)
 // are computed.

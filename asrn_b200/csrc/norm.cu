@@ -10,7 +10,7 @@
 // between two such loads: they are read from the last boundary before them on, their first value the `shift`-th of its eight; the
 // rows' ends are written value by value (k_norm_shifted, and Shifted below). Tensors that are not 16-byte aligned go value by value.
 // The backward pass's blocks stay for many rows with their columns' sums of dy h and dy in registers; a block's sums go to fp32
-// parts that k_norm_sums adds up in order.
+// parts that k_norm_sums adds up in order (4 us at 32768 x 768).
 #include "common.cuh"
 #include "layout.h"
 
@@ -96,6 +96,8 @@ template <int T> ASRN_DEV float row_sum(float v, float* room) {
 constexpr int threads_of(int T) { return T <= 32 ? 128 : T; }
 
 // V values a load, C loads a thread, T threads a row; types XT, RT known at compile time unless they are -1.
+// 32768 x 768, bf16 x, fp32 r and s, bf16 y: 302 MB in 51 us, 5.9 TB/s; 64 rows 2 us, latency (a row's load and two reductions).
+// 65536 x 100 with 16 threads a row 25 us, with 32 threads 43.
 struct Forward {
   int64_t rows;
   int d;
@@ -223,6 +225,11 @@ ASRN_DEV void store_span(void* p, int64_t at, int t, const float* v, const Span&
       if (j >= in.low && j < in.high) store<1>(p, at + j, t, v + j);
   }
 }
+
+// Rows that start anywhere. Each vector is loaded whole, from the last 16-byte boundary before the row on, and its values outside the
+// row count for nothing; the weights lie in shared memory, where any shift reads them without bank conflicts (Planes); blocks stay for
+// many rows so that they are filled once. 33870 x 431 bf16 43 us, with gradients 128 (value by value
+// 190); 2067 x 7159 46 us.
 
 // Its blocks that stay on an SM at once.
 constexpr int stay_shifted(int C, int T) {
