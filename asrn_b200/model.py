@@ -80,9 +80,9 @@ class BloqueLocal(nn.Module):
         if self.activaciones_8bits and self._mlp8_ok(u):
             return h + self.drop(mlp8(u, self.ff[0].weight, self.ff[0].bias, self.ff[2].weight, self.ff[2].bias))
         a = linear(u, self.ff[0].weight, self.ff[0].bias, 'gelu')
-        if self.training and self.drop.p > 0:
-            return h + self.drop(linear(a, self.ff[2].weight, self.ff[2].bias))
-        return linear(a, self.ff[2].weight, self.ff[2].bias, residual=h)
+        if type(self.drop) is nn.Dropout and _sin_ganchos(self.drop) and not (self.drop.training and self.drop.p > 0):
+            return linear(a, self.ff[2].weight, self.ff[2].bias, residual=h)
+        return h + self.drop(linear(a, self.ff[2].weight, self.ff[2].bias))
 
     def _fundido_ok(self, h):
         """layer_norm and linear serve bf16 autocast on CUDA, an fp32 h and widths that are multiples of 8, for the modules as

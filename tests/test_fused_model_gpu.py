@@ -114,6 +114,38 @@ def test_what_is_not_as_built_is_called(cuda):
         assert not torch.equal(blq(h), one)
 
 
+def test_dropout_goes_by_its_own_mode_and_is_called_where_it_has_hooks(cuda):
+    f, _ = make(cuda, fundido=True)
+    blq = f.bloques[0]
+    h = torch.randn(2, 30, 64, generator=torch.Generator().manual_seed(8)).to(cuda)
+    seen = []
+    with torch.no_grad(), torch.autocast('cuda', dtype=torch.bfloat16):
+        f.eval()
+        plain = blq._fundido(h)
+        hook = blq.drop.register_forward_hook(lambda *a: seen.append(1))
+        blq._fundido(h)
+        assert len(seen) == 2                              # after the conv and after the MLP
+        hook.remove()
+        blq.drop.p = 0.5
+        assert torch.equal(blq._fundido(h), plain)         # not in training
+        blq.drop.train()
+        assert not torch.equal(blq._fundido(h), plain)     # the module alone is
+        blq.drop = torch.nn.Identity()
+        assert (blq._fundido(h) - plain).abs().max() <= 2 * U * plain.abs().max()
+
+
+def test_recomputed_blocks_give_the_same_gradients(cuda):
+    """checkpoint=True runs a block's forward pass again in the backward pass: the kernels repeat bit for bit. What is not
+    bitwise the same is what PyTorch's own operations (the embedding's sum) add up in any order."""
+    f, x = make(cuda, fundido=True)
+    g, _ = make(cuda, fundido=True, checkpoint=True)
+    f.train(), g.train()
+    loss = lambda m, x: -m.logprobs(x).mean()  # noqa: E731
+    a, b = grads(f, x, loss), grads(g, x, loss)
+    assert torch.equal(a['ln_f.weight'], b['ln_f.weight']) and torch.equal(a['bloques.3.ff.2.weight'], b['bloques.3.ff.2.weight'])
+    assert torch.equal(a['bloques.3.ln2.weight'], b['bloques.3.ln2.weight'])
+
+
 def test_saved_models_load_either_way(cuda, tmp_path):
     import asrn_b200 as asrn
     f, x = make(cuda, fundido=True)

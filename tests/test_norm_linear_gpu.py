@@ -425,6 +425,70 @@ def test_linear_gradient_against_differences(cuda):
             assert (diff - along).abs() <= tol, (act, i, float(diff), float(along))
 
 
+def test_what_is_kept_for_the_backward_pass_may_not_be_overwritten(cuda):
+    import asrn_b200 as asrn
+    x, r = rand((40, 64), 110).requires_grad_(), rand((40, 64), 111, dtype=F32).requires_grad_()
+    w, ww = rand((64,), 112, dtype=F32).requires_grad_(), rand((64, 64), 113, 0.1)
+    y, s = asrn.layer_norm(x, w, residual=r)
+    s.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.float().sum().backward()
+    c = x.detach() * 1
+    y = asrn.linear(c, ww.requires_grad_(), activation='gelu')
+    y.mul_(2)                                            # the result is not kept
+    torch.autograd.grad(y.float().sum(), (ww,), retain_graph=True)
+    c.zero_()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.float().sum().backward()
+    y, s = asrn.layer_norm(x, w, residual=r)
+    first = torch.autograd.grad((y, s), (x, r, w), (torch.ones_like(y), torch.ones_like(s)), retain_graph=True)
+    again = torch.autograd.grad((y, s), (x, r, w), (torch.ones_like(y), torch.ones_like(s)))
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+def test_inference_mode_and_saved_tensor_hooks(cuda):
+    import asrn_b200 as asrn
+    x, r, w = rand((70, 64), 114), rand((70, 64), 115, dtype=F32), rand((64, 64), 116, 0.1)
+    want = (*asrn.layer_norm(x, r[0], residual=r), asrn.linear(x, w, activation='silu', residual=r), *asrn.head_stats(x, w, top=3)[1:])
+    with torch.inference_mode():
+        got = (*asrn.layer_norm(x, r[0], residual=r), asrn.linear(x, w, activation='silu', residual=r), *asrn.head_stats(x, w, top=3)[1:])
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    leaves = [t.clone().requires_grad_() for t in (x, r, w)]
+
+    def loss():
+        y, s = asrn.layer_norm(leaves[0], leaves[1][0], residual=leaves[1])
+        return asrn.head_stats(asrn.linear(y, leaves[2], activation='silu', residual=s).bfloat16(), leaves[2]).entropy.sum()
+    want = [g.clone() for g in torch.autograd.grad(loss(), leaves)]
+    with torch.autograd.graph.save_on_cpu():
+        held = loss()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(held, leaves), want))
+
+
+@pytest.mark.parametrize('N', [1, 40, 700])
+def test_two_streams_at_once(cuda, N):
+    import asrn_b200 as asrn
+    t = [(rand((N, 768), 120 + i), rand((N, 768), 122 + i, dtype=F32), rand((1536, 768), 124 + i, 0.03), rand((5003, 768), 126 + i, 0.03))
+         for i in range(2)]
+
+    def chain(x, r, w, head):
+        y, s = asrn.layer_norm(x, r[0], residual=r)
+        a = asrn.linear(y, w, activation='gelu')
+        b = asrn.linear(a, w.t().contiguous(), residual=s)
+        return (b, *asrn.head_stats(b.bfloat16(), head, top=4)[1:])
+    with torch.no_grad():
+        want = [chain(*q) for q in t]
+        streams = [torch.cuda.Stream() for _ in t]
+        torch.cuda.synchronize()
+        got = [None, None]
+        for _ in range(20):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i] = chain(*t[i])
+        torch.cuda.synchronize()
+    for g, q in zip(got, want):
+        assert all(torch.equal(p, o) for p, o in zip(g, q))
+
+
 def test_second_and_forward_mode_derivatives_are_refused(cuda):
     import asrn_b200 as asrn
     x, w = rand((20, 64), 70).requires_grad_(), rand((64, 64), 71, 0.1).requires_grad_()
