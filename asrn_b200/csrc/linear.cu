@@ -202,6 +202,15 @@ struct Fused {
 // where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's. Graph replays at 768 ->
 // 1536: 1, 8, 16, 32, 64 rows 3.5, 3.6, 4.5, 5.7, 7.0 us, launch and one round trip to memory (2.4 MB take 0.4).
 constexpr int kFewWarps = 8;
+ASRN_DEV float2 residual_of(const Rest& p, int64_t at) {
+  if (p.res_type == kF32) return __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.res) + at));
+  if (p.res_type == kNone) return make_float2(0.f, 0.f);
+  const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(p.res) + at));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+ASRN_DEV float2 bias_of(const Rest& p, int c) {
+  return p.bias ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.bias + c)) : make_float2(0.f, 0.f);
+}
 template <int NT>
 __global__ void __launch_bounds__(kFewWarps * 32)
 k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
@@ -213,6 +222,16 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
   const bool on[2] = {o0 + g < n, o0 + g + 8 < n};
   const __nv_bfloat16* wp = w + (int64_t)(o0 + g) * d + 8 * t;
   const __nv_bfloat16* xp = x + (int64_t)g * d + 8 * t;
+  wait_previous();
+  let_next();
+  // Up to 8 rows a thread writes two values at most: their bias and residual are on their way while the products run. (1536 -> 768:
+  // 3.4 us with, 3.7 without; with more rows the registers that hold them cost more, 64 rows 9.1 and 7.7.)
+  const int mine = threadIdx.x * split + rank;
+  float2 early = make_float2(0.f, 0.f), shift = early;
+  if (NT == 1 && mine / 8 < rows && o0 + mine % 8 * 2 < n) {
+    early = residual_of(p, (int64_t)(mine / 8) * n + o0 + mine % 8 * 2);
+    shift = bias_of(p, o0 + mine % 8 * 2);
+  }
   float acc[NT][4] = {};
   for (int k0 = (rank * kFewWarps + wid) * 32; k0 < d; k0 += kU * step) {
     uint4 a[kU][2], b[kU][NT];
@@ -254,7 +273,7 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
     gemm::cluster_sync();
   }
   // Two columns each; a cluster's blocks take the pairs in turn.
-  for (int e = threadIdx.x * split + rank; e < 8 * NT * 8; e += kFewWarps * 32 * split) {
+  for (int e = mine; e < 8 * NT * 8; e += kFewWarps * 32 * split) {
     const int r = e / 8, c = e % 8 * 2;
     if (r >= rows || o0 + c >= n) continue;
     float v[2] = {};
@@ -276,26 +295,23 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
       }
     }
     const int64_t at = (int64_t)r * n + o0 + c;
-    if (p.bias) {
-      v[0] += __bfloat162float(p.bias[o0 + c]);
-      v[1] += __bfloat162float(p.bias[o0 + c + 1]);
-    }
+    if (NT > 1) shift = bias_of(p, o0 + c);
+    v[0] += shift.x;
+    v[1] += shift.y;
     if (p.act) {
       uint32_t s;
       activate<1>(p.act, v, &s);
       if (p.keep) *reinterpret_cast<uint32_t*>(slope + at) = s;
     }
-    if (p.res_type == kF32) {
-      const float2 r2 = __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.res) + at));
-      *reinterpret_cast<float2*>(reinterpret_cast<float*>(y) + at) = make_float2(v[0] + r2.x, v[1] + r2.y);
-    } else {
-      if (p.res_type == kBf16) {
-        const uint32_t r2 = __ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(p.res) + at));
-        v[0] += __uint_as_float(r2 << 16);
-        v[1] += __uint_as_float(r2 & 0xffff0000u);
-      }
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(y) + at) = pack2_bf16(v[0], v[1]);
+    if (p.res_type != kNone) {
+      if (NT > 1) early = residual_of(p, at);
+      v[0] += early.x;
+      v[1] += early.y;
     }
+    if (p.res_type == kF32)
+      *reinterpret_cast<float2*>(reinterpret_cast<float*>(y) + at) = make_float2(v[0], v[1]);
+    else
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(y) + at) = pack2_bf16(v[0], v[1]);
   }
   if (split > 1) gemm::cluster_sync();                   // no block ends while another reads its sums
 }
@@ -408,12 +424,14 @@ int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, vo
   cfg.gridDim = dim3((unsigned)(blocks * split));
   cfg.blockDim = dim3(kFewWarps * 32);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1;
+  cfg.numAttrs = split > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k_linear_few<NT>, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
                             reinterpret_cast<const __nv_bfloat16*>(w), p, y, reinterpret_cast<__half*>(slope)) == cudaSuccess
              ? ASRN_OK
