@@ -94,6 +94,22 @@ ASRN_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"
 // before this kernel is complete when the next one starts, and only this kernel's results have to be waited for.
 ASRN_DEV void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Such a launch.
+template <class... P, class... A>
+int launch_next(void (*kernel)(P...), int64_t blocks, int threads, size_t shared, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
+}
+
 // ---- torch-compatible scalar math ----------------------------------------------------------------------------------
 // torch.nn.functional.softplus with beta = 1, threshold = 20.
 ASRN_DEV float softplus_t(float x) { return x > 20.f ? x : log1pf(expf(x)); }

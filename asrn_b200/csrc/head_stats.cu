@@ -861,25 +861,10 @@ struct Slope {
   ASRN_DEV void finish() {}
 };
 
-// A launch whose blocks may start while the kernel before it ends (it has a wait_previous).
-template <class... P, class... A>
-int launch_next(void (*kernel)(P...), int64_t blocks, int threads, cudaStream_t s, const A&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA;
-}
-
 template <int NT, bool Top>
 int few(int64_t N, int64_t V, int d, const void* hc, const void* weight, const int* count, const typename Scan<Top>::Params& p,
         cudaStream_t s) {
-  return launch_next(k_stats_few<NT, Top>, parts_of(V) / 2, 256, s, (int)N, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
+  return launch_next(k_stats_few<NT, Top>, parts_of(V) / 2, 256, 0, s, (int)N, (int)V, d, reinterpret_cast<const __nv_bfloat16*>(hc),
                      reinterpret_cast<const __nv_bfloat16*>(weight), count, p);
 }
 template <bool Top>
@@ -958,7 +943,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
               : groups <= 512  ? (few ? k_stats_rows<16, 8, false> : k_stats_rows<16, 2, false>)
               : groups <= 1024 ? (few ? k_stats_rows<32, 8, false> : k_stats_rows<32, 2, false>)
                                : (few ? k_stats_rows<0, 8, false> : k_stats_rows<0, 2, false>);
-  return launch_next(rows, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, s, f);
+  return launch_next(rows, (N + kRowWarps - 1) / kRowWarps, kRowWarps * 32, 0, s, f);
 }
 
 int asrn_head_stats_backward(int64_t N, int64_t V, int32_t d, const void* weight, const void* saved, size_t saved_bytes,

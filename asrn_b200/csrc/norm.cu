@@ -110,6 +110,8 @@ struct Forward {
 template <int V, int XT, int RT, int C, int T>
 __global__ void __launch_bounds__(threads_of(T), 1) k_norm(const Forward f) {
   __shared__ float room[2][32];
+  wait_previous();
+  let_next();
   const int xt = XT < 0 ? f.xt : XT, rt = RT < 0 ? f.rt : RT;
   const int tid = T <= 32 ? threadIdx.x % T : threadIdx.x;
   const int64_t own = T <= 32 ? (int64_t)blockIdx.x * (blockDim.x / T) + threadIdx.x / T : blockIdx.x;
@@ -241,6 +243,8 @@ __global__ void __launch_bounds__(threads_of(T), stay_shifted(C, T)) k_norm_shif
   __shared__ float room[2][2][32];
   constexpr int kRows = threads_of(T) / T;
   const Planes w(planes, f.d), b(planes + Planes::floats(f.d), f.d);
+  wait_previous();
+  let_next();
   w.fill(f.w, f.wt, f.d);
   if (f.b) b.fill(f.b, f.wt, f.d);
   __syncthreads();
@@ -333,6 +337,8 @@ __global__ void __launch_bounds__(threads_of(T), T == 256 ? 2 : 1) k_norm_back(c
   constexpr int kRows = threads_of(T) / T;               // of a block at a time
   __shared__ float room[2][2][32];
   __shared__ float sums[T == 32 ? 2 * 32 * C * V : 1];
+  wait_previous();
+  let_next();
   const int st = ST < 0 ? f.st : ST, yt = YT < 0 ? f.yt : YT;
   const int tid = T == 32 ? threadIdx.x & 31 : threadIdx.x, wid = T == 32 ? threadIdx.x >> 5 : 0;
   float dw[C * V] = {}, db[C * V] = {};
@@ -442,6 +448,8 @@ __global__ void __launch_bounds__(T, T == 256 ? 2 : 1) k_norm_back_shifted(const
   extern __shared__ float planes[];
   __shared__ float room[2][2][32];
   const Planes w(planes, f.d);
+  wait_previous();
+  let_next();
   w.fill(f.w, f.wt, f.d);
   __syncthreads();
   const int tid = threadIdx.x, shift = (int)((int64_t)blockIdx.x * f.d & 7), last = (f.d + shift - 1) / 8;
@@ -586,6 +594,8 @@ __global__ void __launch_bounds__(kWarps * 32, C == 1 ? 5 : C < 4 ? 3 : 2) k_nor
   float dw[C * 8] = {}, db[C * 8] = {};
   const float inv = 1.f / (float)f.d;
   int turn = 0;
+  wait_previous();
+  let_next();
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) fetch(row0 + j * step, j);
   if (Shifted) {
@@ -699,6 +709,8 @@ __global__ void __launch_bounds__(1024) k_norm_sums(int parts, int d, const floa
                                                     int wt) {
   __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  wait_previous();
+  let_next();
   float s = 0.f;
   if (c < 2 * d)
 #pragma unroll 8
@@ -733,13 +745,10 @@ int64_t blocks_back(int64_t rows, int d) {
   return d % 8 ? (n + 7) / 8 * 8 : n;
 }
 
-int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
-
 template <int V, int XT, int RT, int C, int T> int run(const Forward& f, cudaStream_t s) {
   // few rows: a warp for a block, so that they spread over the SMs
   const int threads = T > 32 ? T : f.rows <= 4 * sms() ? 32 : threads_of(T), per = T <= 32 ? threads / T : 1;
-  k_norm<V, XT, RT, C, T><<<(unsigned)((f.rows + per - 1) / per), threads, 0, s>>>(f);
-  return launched();
+  return launch_next(k_norm<V, XT, RT, C, T>, (f.rows + per - 1) / per, threads, 0, s, f);
 }
 template <int XT, int RT> int widths(const Forward& f, cudaStream_t s) {
   if (f.d <= 128) return run<8, XT, RT, 1, 16>(f, s);
@@ -773,8 +782,7 @@ int launch(Kernel kernel, std::atomic<uint64_t>& ready, size_t most, int64_t blo
       if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
   }
-  kernel<<<(unsigned)blocks, threads, bytes, s>>>(f);
-  return launched();
+  return launch_next(kernel, blocks, threads, bytes, s, f);
 }
 
 template <int XT, int RT, int C, int T> int run_shifted(const Forward& f, cudaStream_t s) {
@@ -798,8 +806,7 @@ template <int XT, int RT> int shifted(const Forward& f, cudaStream_t s) {
 }
 
 template <int V, int ST, int YT, int C, int T> int run(const Backward& f, cudaStream_t s) {
-  k_norm_back<V, ST, YT, C, T><<<(unsigned)blocks_back(f.rows, f.d), threads_of(T), 0, s>>>(f);
-  return launched();
+  return launch_next(k_norm_back<V, ST, YT, C, T>, blocks_back(f.rows, f.d), threads_of(T), 0, s, f);
 }
 template <int ST, int YT, int C, bool Shifted> int run_rows(const Backward& f, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
@@ -920,8 +927,7 @@ int asrn_layer_norm_backward(int64_t rows, int32_t d, const void* s_in, int32_t 
   else
     st = y_type == kF32 ? with(Bf16{}, F32{}) : with(Bf16{}, Bf16{});
   if (st || !sums) return st;
-  k_norm_sums<<<(unsigned)((2 * d + 31) / 32), 1024, 0, s>>>((int)blocks_back(rows, d), d, f.parts, dw, db, w_type);
-  return launched();
+  return launch_next(k_norm_sums, (2 * d + 31) / 32, 1024, 0, s, (int)blocks_back(rows, d), d, f.parts, dw, db, w_type);
 }
 
 }  // extern "C"
