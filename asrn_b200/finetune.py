@@ -1,11 +1,15 @@
-"""Fine-tuning on the device: log probabilities through the tied head, losses on them, and an MLP whose activations are
-kept in 8 bits (the C ABI's asrn_head_*, asrn_preference_loss, asrn_policy_loss, asrn_mlp8_*, asrn_pack8).
+"""Fine-tuning on the device: log probabilities through the tied head, losses on them, an MLP whose activations are
+kept in 8 bits, and the norm, the product and the head's statistics that training and answering share (the C ABI's
+asrn_head_*, asrn_preference_loss, asrn_policy_loss, asrn_mlp8_*, asrn_pack8, asrn_layer_norm*, asrn_linear_*).
 
     head_logprobs    log softmax(h W^T / temperatura)[token] and its gradients; the (tokens, V) logits are not kept
     preference_loss  logistic or squared (IPO) loss of pairs of a chosen and a rejected answer
     policy_loss      clipped policy loss with an advantage per answer or token and a KL term against a reference model
     mlp8             gelu(x W1^T + b1) W2^T + b2 that keeps x and x W1^T + b1 in 8 bits for its backward pass
     pack8, unpack8   the 8-bit form by itself
+    layer_norm       layer norm with the residual sum before it
+    linear           activation(x W^T + b) + residual
+    head_stats       head_logprobs with the distribution's entropy and its likeliest tokens
 
 The losses return their gradient with the loss (one pass over the tokens makes both), so a step is
 
@@ -22,6 +26,9 @@ each, as operands of the next products (and gelu' to fp16). In calls of up to 51
 and rows x V x d up to 2^34), the remainders are multiplied too, and gelu' is not rounded: a weight's gradient from few rows
 would else hold little but those roundings. So a row's y, dx and dh differ in their last bits with the number of rows in the
 call: against 64 bits they are off by 2.3e-3 to 2.5e-3 of themselves in the 2-norm above 512, by 1.7e-3 up to there.
+linear and head_stats follow the same rules (linear: up to 512 rows; it keeps the slope in fp16 in any call), and few rows (linear up to
+64, head_stats up to 32) take a kernel that sums in another order. layer_norm rounds its results only. Products are summed in
+fp32 as the tensor cores sum, truncated: a result in fp32 (linear with a residual in fp32) is off by 1e-6 of itself at d = 1536.
 """
 from collections import namedtuple
 
@@ -146,7 +153,8 @@ def head_stats(h, weight, tokens=None, temperatura=1.0, top=0):
       logp        log p[token] (None without tokens), float32, head_logprobs' values
       entropy     - sum p log p, float32
       top_logp, top_tokens   (..., top) the `top` (up to 32) likeliest tokens and their log probabilities, the likeliest first,
-                  equal ones by their number; ranked by scores summed in 64 bits (None without top)
+                  equal ones by their number (None without top). Scores nearer one another than sums in fp32 tell are ranked
+                  by sums in 64 bits
     Differentiable in h and weight through logp and entropy. A negative token leaves its position out (0, tokens -1, no
     gradient, none of the work); a token >= V, and scores whose exponentials have no finite sum, give NaN and tokens -1. d has
     to be a multiple of 8; the backward pass holds what head_logprobs' does."""
