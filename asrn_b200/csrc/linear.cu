@@ -26,7 +26,7 @@ namespace {
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
 constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
 constexpr int64_t kTwiceRows = 512;
-// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 7.0, 65 rows | 11.0; 1536 -> 768 7.9 | 14.5. Where y has more
+// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 6.8, 65 rows | 11.0; 1536 -> 768 8.0 | 14.5. Where y has more
 // values the tiles fill the SMs: 768 -> 8192, 64 rows 13.3 | 11.1; 768 -> 16384, 32 rows 12.2 | 11.4; 768 -> 50304, 16 rows 17,
 // 32 rows 33 | 21.
 constexpr int64_t kFewRows = 64, kFewValues = (int64_t)1 << 20;
@@ -200,7 +200,7 @@ struct Fused {
 // A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
 // memory, and four lanes read 64 neighbouring bytes. A block's warps take every eighth 32 of K; the blocks of a cluster share K
 // where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's. Graph replays at 768 ->
-// 1536: 1, 8, 16, 32, 64 rows 3.5, 3.6, 4.5, 5.7, 7.0 us, launch and one round trip to memory (2.4 MB take 0.4).
+// 1536: 1, 8, 16, 32, 64 rows 3.2, 3.5, 4.4, 5.4, 6.8 us, launch and one round trip to memory (2.4 MB take 0.4).
 constexpr int kFewWarps = 8;
 ASRN_DEV float2 residual_of(const Rest& p, int64_t at) {
   if (p.res_type == kF32) return __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.res) + at));
@@ -225,7 +225,7 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
   wait_previous();
   let_next();
   // Up to 8 rows a thread writes two values at most: their bias and residual are on their way while the products run. (1536 -> 768:
-  // 3.4 us with, 3.7 without; with more rows the registers that hold them cost more, 64 rows 9.1 and 7.7.)
+  // 8 rows 3.8 us with, 4.1 without, before the launches overlapped; with more rows the registers cost more, 64 rows 9.4 and 8.1.)
   const int mine = threadIdx.x * split + rank;
   float2 early = make_float2(0.f, 0.f), shift = early;
   if (NT == 1 && mine / 8 < rows && o0 + mine % 8 * 2 < n) {
