@@ -936,7 +936,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   const RowArgs f{N, (int)V, d, top, parts, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
                   reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own,
                   reinterpret_cast<float*>(kept(sv.head.lse2)), reinterpret_cast<float*>(kept(sv.head.rest)),
-                  reinterpret_cast<float*>(kept(sv.ent)), logp, entropy, top_logp, top_tokens};
+                  reinterpret_cast<float*>(kept(sv.ent)), tokens ? logp : nullptr, entropy, top_logp, top_tokens};
   const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps * std::max(4, d / 48);
   auto rows = span == 1       ? V <= 512 ? (few ? k_stats_rows<16, 8, true> : k_stats_rows<16, 2, true>)
                                          : (few ? k_stats_rows<64, 8, true> : k_stats_rows<64, 2, true>)

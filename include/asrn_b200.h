@@ -326,7 +326,7 @@ int asrn_linear_backward(int64_t N, int32_t d, int32_t n, const void* dy, int32_
 
 /* asrn_head_stats_forward: asrn_head_forward's logp with entropy (N) = - sum p log p, p = softmax(h W^T / tau), and the `top`
  * (0 to 32, at most V) likeliest tokens, top_tokens (N, top) int64 with their log probabilities top_logp (N, top), by
- * their scores summed in 64 bits, equal ones by their numbers. tokens may be NULL: every position counts, and logp is not
+ * their scores (those nearer one another than sums in fp32 tell by sums in 64 bits), equal ones by their numbers. tokens may be NULL: every position counts, and logp is not
  * written. A negative token leaves its position out: 0 everywhere and tokens -1; a token >= V, and scores without a finite log of
  * their sum of exponentials, give NaN and tokens -1. `saved` may be NULL without tokens, where no backward pass follows.
  * asrn_head_stats_backward: from g = dL/dlogp and g_entropy = dL/dentropy (N), either may be NULL. */
