@@ -638,78 +638,86 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   float size = likeliest < f.V ? magnitude(h, f.W, vecs, likeliest) : 0.f, off = 0.f;
   float slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
   auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack + off); };
+  // Those that stand within `width` of their neighbours, down to that far below the last one that counts, by sums in 64 bits; others
+  // keep their places among them.
+  double score;
+  auto settle = [&](float width) {
+    const float then = __shfl_down_sync(0xffffffffu, best.score, 1);
+    const float least = low() - width;
+    unsigned near = __ballot_sync(0xffffffffu, lane < 31 && then >= least && best.score - then <= width);
+    score = best.score;
+    if (!near) return;
+    near |= near << 1;
+    Best<double> exact;
+    unsigned rest = near;
+    for (int q = 0; q < 32; ++q) {
+      if (!(near >> q & 1u)) {
+        const float sc = __shfl_sync(0xffffffffu, best.score, q);
+        exact.put((double)sc, __shfl_sync(0xffffffffu, best.token, q));
+        continue;
+      }
+      if (!(rest >> q & 1u)) continue;
+      int t[4];                                  // the next four of them
+      bool on[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        on[j] = rest != 0;
+        t[j] = __shfl_sync(0xffffffffu, best.token, on[j] ? __ffs(rest) - 1 : q);
+        rest &= rest - 1;
+      }
+      double sums[4];
+      dots(h, f.W, vecs, t, sums);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (on[j]) exact.put(sums[j], t[j]);
+    }
+    best.token = exact.token;
+    score = exact.score;
+  };
   {
-    const float lowest = low() - slack, then = __shfl_down_sync(0xffffffffu, best.score, 1);
+    const float lowest = low() - slack;
     const bool open = size == 0.f || (lane < top && best.token >= f.V) || (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
                       (after >= 0 && above(pair.x) >= lowest) || best.lost >= lowest - slack;
     if (!__any_sync(0xffffffffu, open)) {
-      // Those that stand too near their neighbours: by sums in 64 bits. Others keep their places among them.
-      const unsigned before = __ballot_sync(0xffffffffu, lane < min(top, 31) && best.score - then <= 2 * slack);
-      double score = best.score;
-      if (before) {
-        Best<double> exact;
-        unsigned near = before | before << 1, rest = near;
-        for (int q = 0; q < 32; ++q) {
-          if (!(near >> q & 1u)) {
-            const float sc = __shfl_sync(0xffffffffu, best.score, q);
-            exact.put((double)sc, __shfl_sync(0xffffffffu, best.token, q));
-            continue;
-          }
-          if (!(rest >> q & 1u)) continue;
-          int t[4];                              // the next four of them
-          bool on[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            on[j] = rest != 0;
-            t[j] = __shfl_sync(0xffffffffu, best.token, on[j] ? __ffs(rest) - 1 : q);
-            rest &= rest - 1;
-          }
-          double sums[4];
-          dots(h, f.W, vecs, t, sums);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (on[j]) exact.put(sums[j], t[j]);
-        }
-        best.token = exact.token;
-        score = exact.score;
-      }
+      settle(2 * slack);
       write((float)(score * f.inv_tau - base), best.token);
       return;
     }
   }
 
-  // Else the scores again, sixteen at a time.
-  best = Best<float>{};
-  const int count = have + (y >= 0);
-  for (int q = 0; q < count; q += 16) {
-    int rows[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int at = min(q + (lane >> 2) + 8 * j, count - 1), t = __shfl_sync(0xffffffffu, column, max(min(at, have - 1), 0));
-      rows[j] = at < have ? t : y;
-    }
-    const Pair about = q ? dots16<U, false>(h, f.W, vecs, rows[0], rows[1], nullptr)
-                         : dots16<U, true>(h, f.W, vecs, rows[0], rows[1], &size);
-    for (int j = 0; j < 16 && q + j < count; ++j) {
-      const int t = __shfl_sync(0xffffffffu, j < 8 ? rows[0] : rows[1], j % 8 * 4);
-      best.put(about.of(j), t);
-    }
-  }
-  // What a sum here is off by at most: two chains. The magnitudes: of the first eight, or should those be rows of zeros of eight from
-  // all over the vocabulary.
+  // Else all that may count, by the products' sums or by sums here (two chains, off by less). Where the likeliest one's magnitudes are 0,
+  // those of the others, and should they be rows of zeros those of eight from all over the vocabulary.
   if (size == 0.f) {
-    const int sample = (int)((int64_t)(lane >> 2) * f.V / 8);
-    dots16<U, true>(h, f.W, vecs, sample, sample, &size);
+    const int some = __shfl_sync(0xffffffffu, column, min(lane >> 2, max(have - 1, 0)));
+    if (have) dots16<U, true>(h, f.W, vecs, some, some, &size);
+    if (size == 0.f) {
+      const int sample = (int)((int64_t)(lane >> 2) * f.V / 8);
+      dots16<U, true>(h, f.W, vecs, sample, sample, &size);
+    }
+    slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
   }
-  off = (float)(f.d / 32 + 4) * 0x1p-22f * size;
-  slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
+  off = slack;
+  float bar = low();                             // no more than the last score that counts
+  bar -= fabsf(bar) * 0x1p-15f;
+  unsigned hidden = __ballot_sync(0xffffffffu, lane < have && held.y > -3e38f && above(held.y) >= bar);
+  // Of two that the notes cannot tell apart the noted column may be either's: left to `expand`.
+  const unsigned either = hidden & __ballot_sync(0xffffffffu, held.y >= held.x - fabsf(held.x) * 0x1p-15f);
+  if (either) {
+    best = Best<float>{};
+    for (int q = 0; q < have; ++q) {
+      const float v = __shfl_sync(0xffffffffu, held.x, q);
+      const int t = __shfl_sync(0xffffffffu, column, q);
+      if (!(either >> q & 1u)) best.put(v, t);
+    }
+    if (y >= 0) best.put(own, y);
+  }
   // The columns of a group that may count, but for one and the target's.
   auto expand = [&](int g, int except, auto&& take) {
     const int begin = g * f.span, end = min(f.V, begin + f.span);
     for (int c = begin; c < end; c += 16) {
       const int ra = c + (lane >> 2), rb = ra + 8;
       const Pair about = dots16<U, false>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1), nullptr);
-      const float least = low() - 2 * off;
+      const float least = fmaxf(low(), bar) - 2 * off;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int own = j ? rb : ra;
@@ -723,12 +731,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     }
   };
   auto about_put = [&](float about, int token) { best.put(about, token); };
-  const float lowest = low();
-  unsigned hidden = __ballot_sync(0xffffffffu, lane < have && held.y > -3e38f && above(held.y) >= lowest);
   for (; hidden; hidden &= hidden - 1) {
-    const int q = __ffs(hidden) - 1;
-    if (above(__shfl_sync(0xffffffffu, held.y, q)) >= low())
-      expand(__shfl_sync(0xffffffffu, held_group, q), __shfl_sync(0xffffffffu, column, q), about_put);
+    const int q = __ffs(hidden) - 1, g = __shfl_sync(0xffffffffu, held_group, q), c = __shfl_sync(0xffffffffu, column, q);
+    if (either >> q & 1u)
+      expand(g, -1, about_put);
+    else if (above(__shfl_sync(0xffffffffu, held.y, q)) >= low())
+      expand(g, c, about_put);
   }
   if (after >= 0 && above(pair.x) >= low()) {
     Groups<0, Notes<Whole>> rest(notes, f.groups, order_of(pair.x), after);
@@ -740,31 +748,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   }
 
   // Scores that stand as near one another as the sums may be off: by sums in 64 bits.
-  const float least = low() - 2 * off, then = __shfl_down_sync(0xffffffffu, best.score, 1);
-  const bool near = lane < top && lane < 31 && best.score - then <= 2 * off;
-  double score = best.score;
-  if (__any_sync(0xffffffffu, near) || best.lost >= least) {
+  const float least = low() - 2 * off;
+  if (best.lost < least) {                       // the few that were kept hold all that may count
+    settle(2 * off);
+  } else {
     double s[4];
     Best<double> exact;
-    if (best.lost < least) {                     // the few that were kept hold all that may count
-      for (int q = 0; q < 32; q += 4) {
-        int t[4];
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float sc = __shfl_sync(0xffffffffu, best.score, q + j);
-          const int tk = __shfl_sync(0xffffffffu, best.token, q + j);
-          t[j] = sc >= least && tk < f.V ? tk : -1;
-          any |= t[j] >= 0;
-        }
-        if (!any) break;                         // in order: none after these
-        const int rows[4] = {max(t[0], 0), max(t[1], 0), max(t[2], 0), max(t[3], 0)};
-        dots(h, f.W, vecs, rows, s);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (t[j] >= 0) exact.put(s[j], t[j]);
-      }
-    } else if (size == 0.f && !__any_sync(0xffffffffu, [&] {
+    if (size == 0.f && !__any_sync(0xffffffffu, [&] {
                  uint32_t any = 0;
                  for (int c = lane; c < vecs; c += 32) {
                    const uint4 a = __ldg(h + c);

@@ -208,6 +208,24 @@ def test_rankings_of_many_rows(cuda, N, V, d):
         check(h, w, targets(N, V, 65, 11) if given else None, top=top, grads=False)
 
 
+@pytest.mark.parametrize('N', [5, 900])
+def test_many_near_the_last_one_that_counts(cuda, N):
+    """Tokens of one group and of others whose scores differ by less than fp32 sums tell, more of them than are asked for: which of
+    them come first is a matter of the sums in 64 bits."""
+    V, d = 5003, 256
+    w = rand((V, d), 67, 0.05)
+    base = rand((d,), 68)
+    for i in range(12):                                  # six in one group of 32, six in groups of their own
+        w[320 + 3 * i if i < 6 else 400 * (i - 4)] = base
+    rows = torch.tensor([320 + 3 * i if i < 6 else 400 * (i - 4) for i in range(12)], device='cuda')
+    w[rows, 7] = (torch.randn(12, generator=torch.Generator().manual_seed(69)) * 2.0 ** -10).bfloat16().cuda()
+    h = base.repeat(N, 1) * rand((N, 1), 70).abs().clamp(min=0.1)
+    h[:, 7] = 2.0 ** -5 * torch.where(torch.arange(N, device='cuda') % 2 == 0, 1.0, -1.0).bfloat16()
+    for top in (2, 5, 9, 14):
+        check(h, w, None, top=top, grads=False)
+        check(h, w, targets(N, V, 71, 4), top=top, grads=False)
+
+
 def test_weights_of_zeros(cuda):
     """All tokens are as likely: the first ones, whatever the hidden state."""
     import asrn_b200 as asrn
