@@ -49,18 +49,20 @@ constexpr int kPart = 64;
 __host__ ASRN_DEV int parts_of(int64_t V) { return (int)((V + gemm::kBN - 1) / gemm::kBN) * (gemm::kBN / kPart); }
 
 // Columns of a group: of a group that holds two of the likeliest tokens all have to be looked at, so 32 as long as a row's groups
-// stay few enough for a warp to hold in registers. Where a row would have four such pairs or more, groups of 1: all scores are kept
-// (10816 x 1265 x 608: 20 tokens 296 us so, 402 by groups of 32; 8 tokens 183 and 158).
-int span_of(int64_t V, int top) { return V <= 2048 && 8 * top * top >= V ? 1 : V <= 32768 ? 32 : 64; }
-int64_t notes_of(int64_t V, int top) { return (V + span_of(V, top) - 1) / span_of(V, top); }
+// stay few enough for a warp to hold in registers. Where looking at them (top^2 / V groups, 32 scores of d products) costs more than
+// reading a score of each column, groups of 1: all scores are kept.
+// All scores | groups of 32, us: 10816 x 1265 x 608, 8 tokens 122 | 104, 12 tokens 142 | 157, 32 tokens 283 | 722;
+// 4096 x 2000 x 256, 20 tokens 95 | 73, 32 tokens 151 | 181; 8192 x 256 x 64, 3 tokens 28 | 29, 8 tokens 37 | 47.
+int span_of(int64_t V, int d, int top) { return V <= 2048 && V * V <= 24 * top * top * (int64_t)d ? 1 : V <= 32768 ? 32 : 64; }
+int64_t notes_of(int64_t V, int d, int top) { return (V + span_of(V, d, top) - 1) / span_of(V, d, top); }
 // Bytes of a row's notes: two numbers a group, or one a column (whole chunks of 32).
-int64_t note_bytes(int64_t V, int top) { return span_of(V, top) == 1 ? (V + 31) / 32 * 128 : notes_of(V, top) * 8; }
+int64_t note_bytes(int64_t V, int d, int top) { return span_of(V, d, top) == 1 ? (V + 31) / 32 * 128 : notes_of(V, d, top) * 8; }
 
 struct StatsWs {
   size_t counts, top, part, notes, total;
 };
 
-StatsWs stats_ws(int64_t N, int64_t V, int top) {
+StatsWs stats_ws(int64_t N, int64_t V, int d, int top) {
   StatsWs w{};
   const size_t P = (size_t)pad256(N), parts = (size_t)parts_of(V);
   size_t o = 0;
@@ -68,7 +70,7 @@ StatsWs stats_ws(int64_t N, int64_t V, int top) {
   w.counts = take((size_t)((N + kCountRows - 1) / kCountRows) * 4);
   w.top = take(P * 4);
   w.part = take(parts * P * 16);
-  w.notes = take(top ? (size_t)note_bytes(V, top) * P : 0);
+  w.notes = take(top ? (size_t)note_bytes(V, d, top) * P : 0);
   w.total = o;
   return w;
 }
@@ -540,9 +542,9 @@ struct RowArgs {
   int64_t* top_tokens;
 };
 
-// U: steps of K whose loads are under way together: 8 where a slow row's latency is what counts (50304 x 768, 8 tokens: 2048 rows 54 us
-// against 105 with 2, 4096 78 against 108, 8192 125 against 150), 2 where rows are many and short, so that more share an SM
-// (5003 x 200, 8192 rows: 59 with 8, 50 with 2; 2048 rows 22 and 30).
+// U: steps of K whose loads are under way together: 8 where a slow row's latency is what counts, 2 where rows are many and short, so that
+// more share an SM (8 tokens, us, 8 | 2, before rows kept the products' sums: 50304 x 768, 2048 rows 54 | 105, 4096 78 | 108,
+// 8192 125 | 150; 5003 x 200, 2048 rows 22 | 30, 8192 59 | 50). Now 49 us at 2048 x 50304 x 768, 22 at 2048 x 5003 x 200.
 template <int Each, int U, bool Whole>
 __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7) k_stats_rows(const RowArgs f) {
   const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
@@ -742,8 +744,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     Groups<0, Notes<Whole>> rest(notes, f.groups, order_of(pair.x), after);
     for (; after >= 0 && above(pair.x) >= low(); after = rest.next(pair)) {
       const int c = column_of(after, pair);
-      best.put(dots16<U, false>(h, f.W, vecs, c, c, nullptr).of(0), c);
-      if (pair.y > -3e38f && above(pair.y) >= low()) expand(after, c, about_put);
+      const bool unsure = pair.y > -3e38f && pair.y >= pair.x - fabsf(pair.x) * 0x1p-15f;
+      if (!unsure) best.put(pair.x, c);
+      if (unsure || (pair.y > -3e38f && above(pair.y) >= low())) expand(after, unsure ? -1 : c, about_put);
     }
   }
 
@@ -771,14 +774,22 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
         exact.put(s[0], token);
       };
       if (y >= 0) exact_put(0.f, y);
-      for (int g = 0; g < f.groups; ++g) {
-        const float v = notes.largest(g);
-        if (!(v > -3e38f && above(v) >= low())) continue;
-        // nothing of it comes before the last one that counts so far, not as its equal either
-        const double last = __shfl_sync(0xffffffffu, exact.score, top - 1);
-        const int number = __shfl_sync(0xffffffffu, exact.token, top - 1);
-        if ((double)above(v) < last || ((double)above(v) == last && number < g * f.span)) continue;
-        expand(g, -1, exact_put);
+      for (int g0 = 0; g0 < f.groups; g0 += 32) {
+        const float largest = notes.largest(min(g0 + lane, f.groups - 1)), lowest = low();   // a shuffle: not behind a condition
+        unsigned set = __ballot_sync(0xffffffffu, g0 + lane < f.groups && largest > -3e38f && above(largest) >= lowest);
+        for (; set; set &= set - 1) {
+          const int g = g0 + __ffs(set) - 1;
+          const float most = above(__shfl_sync(0xffffffffu, largest, g - g0));
+          // nothing of it comes before the last one that counts so far, not as its equal either
+          const double last = __shfl_sync(0xffffffffu, exact.score, top - 1);
+          const int number = __shfl_sync(0xffffffffu, exact.token, top - 1);
+          if ((double)most < last || ((double)most == last && number < g * f.span)) continue;
+          if constexpr (Whole) {
+            if (g != y) exact_put(0.f, g);
+          } else {
+            expand(g, -1, exact_put);
+          }
+        }
       }
     }
     best.token = exact.token;
@@ -879,7 +890,7 @@ size_t asrn_head_stats_saved_bytes(int64_t N, int32_t d) {
 
 size_t asrn_head_stats_workspace_bytes(int64_t N, int64_t V, int32_t d, int32_t top, int32_t backward) {
   if (asrn::check_head(N, V, d)) return 0;
-  return backward ? asrn::head_backward_ws(N, V, d).total : asrn::stats_ws(N, V, top).total;
+  return backward ? asrn::head_backward_ws(N, V, d).total : asrn::stats_ws(N, V, d, top).total;
 }
 
 int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, const void* weight, const int64_t* tokens,
@@ -896,7 +907,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
       (uintptr_t)weight % 16)
     return ASRN_ERR_ARG;
   const StatsSaved sv = stats_saved(N, d);
-  const StatsWs ws = stats_ws(N, V, top);
+  const StatsWs ws = stats_ws(N, V, d, top);
   if (!saved && tokens) return ASRN_ERR_WORKSPACE;
   if ((saved && (saved_bytes < sv.total || (uintptr_t)saved % 256)) || !workspace || workspace_bytes < ws.total ||
       (uintptr_t)workspace % 256)
@@ -917,7 +928,7 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   float* own = reinterpret_cast<float*>(W + ws.top);
   float4* part = reinterpret_cast<float4*>(W + ws.part);
   float2* notes = reinterpret_cast<float2*>(W + ws.notes);
-  const int span = span_of(V, top), groups = (int)notes_of(V, top);
+  const int span = span_of(V, d, top), groups = (int)notes_of(V, d, top);
   if (top)
     st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
   else
