@@ -7,9 +7,10 @@
 // rounding to bf16 takes (a in bf16 would move act'(a) by as much as that), and the backward pass has nothing left to compute. dA is rounded once, as
 // operand of both products; up to kTwiceRows rows they take what the rounding took, too.
 //
-//   k_linear_few   up to kFewRows rows: memory bound (the weight is read once, 2 operations a byte and row), so the rows of W are
-//                  spread over all SMs, sixteen a block, K over its warps; mma.sync, whose 16 x 8 tiles fit such rows
-//   k_gemm<Fused>  more rows: tcgen05 products, the rest in the epilogue
+//   k_linear_few   few results: too few tiles of 128 x 256 for the SMs, and with few rows memory bound (the weight is read once,
+//                  2 operations a byte and row), so the rows of W are spread over all SMs, sixteen a block with up to 64 rows of
+//                  x, K over its warps; mma.sync, whose 16 x 8 tiles fit such rows
+//   k_gemm<Fused>  more: tcgen05 products, the rest in the epilogue
 //   k_linear_slope backward: dA in bf16 and its columns' sums by 64 rows; memory bound: 32768 x 1536 from bf16 dY 47 us (302 MB,
 //                  6.3 TB/s), 32768 x 768 from fp32 dY without a slope 24.5
 //   k_gemm x 2     dX, dW (dW in shares of the rows where its tiles are few)
@@ -26,10 +27,11 @@ namespace {
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
 constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
 constexpr int64_t kTwiceRows = 512;
-// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 6.8, 65 rows | 11.0; 1536 -> 768 8.0 | 14.5. Where y has more
-// values the tiles fill the SMs: 768 -> 8192, 64 rows 13.3 | 11.1; 768 -> 16384, 32 rows 12.2 | 11.4; 768 -> 50304, 16 rows 17,
-// 32 rows 33 | 21.
-constexpr int64_t kFewRows = 64, kFewValues = (int64_t)1 << 20;
+// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 6.8 | 11.0, 128 rows 8.6 | 11.4, 384 rows 16 | 12; 1536 -> 768,
+// 128 rows 9.6 | 15.3; 128 -> 128, 2048 rows 6.1 | 7.3, 4096 rows 9.1 | 7.4; 4096 -> 512, 128 rows 15 | 30, 768 rows 29 | 29. A row's
+// values are few blocks' then; where y is wide and rows are few the weight's bytes count: 768 -> 50304, 8 rows 17 | 21, 32 rows
+// 33 | 21; 768 -> 8192, 32 rows 7.1 | 11, 64 rows 13 | 11.
+bool few_rows(int64_t N, int64_t n) { return N * n <= 1 << 18 || (N <= 16 && N * n <= 1 << 20); }
 
 ASRN_DEV uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -196,7 +198,7 @@ struct Fused {
   ASRN_DEV void finish() {}
 };
 
-// 16 columns of y for up to 8 NT rows of x: A = 16 rows of W, B = the rows of x. The order of K inside a tile is free as long as
+// 16 columns of y for 8 NT rows of x: A = 16 rows of W, B = the rows of x. The order of K inside a tile is free as long as
 // A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
 // memory, and four lanes read 64 neighbouring bytes. A block's warps take every eighth 32 of K; the blocks of a cluster share K
 // where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's. Graph replays at 768 ->
@@ -211,17 +213,19 @@ ASRN_DEV float2 residual_of(const Rest& p, int64_t at) {
 ASRN_DEV float2 bias_of(const Rest& p, int c) {
   return p.bias ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.bias + c)) : make_float2(0.f, 0.f);
 }
-template <int NT>
+// Many: more rows than 8 NT, by chunks (blockIdx.y). 64 rows x 1536 -> 768: 8.3 us without, 8.8 with.
+template <int NT, bool Many>
 __global__ void __launch_bounds__(kFewWarps * 32)
-k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
+k_linear_few(int all, int n, int d, int split, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
              const Rest p, void* __restrict__ y, __half* __restrict__ slope) {
   constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
   __shared__ float sh[kFewWarps][8 * NT][17];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int first = Many ? blockIdx.y * 8 * NT : 0, rows = Many ? min(all - first, 8 * NT) : all;
   const int rank = split > 1 ? (int)gemm::cluster_rank() : 0, o0 = blockIdx.x / split * 16, step = split * kFewWarps * 32;
   const bool on[2] = {o0 + g < n, o0 + g + 8 < n};
   const __nv_bfloat16* wp = w + (int64_t)(o0 + g) * d + 8 * t;
-  const __nv_bfloat16* xp = x + (int64_t)g * d + 8 * t;
+  const __nv_bfloat16* xp = x + (int64_t)(first + g) * d + 8 * t;
   wait_previous();
   let_next();
   // Up to 8 rows a thread writes two values at most: their bias and residual are on their way while the products run. (1536 -> 768:
@@ -229,7 +233,7 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
   const int mine = threadIdx.x * split + rank;
   float2 early = make_float2(0.f, 0.f), shift = early;
   if (NT == 1 && mine / 8 < rows && o0 + mine % 8 * 2 < n) {
-    early = residual_of(p, (int64_t)(mine / 8) * n + o0 + mine % 8 * 2);
+    early = residual_of(p, (int64_t)(first + mine / 8) * n + o0 + mine % 8 * 2);
     shift = bias_of(p, o0 + mine % 8 * 2);
   }
   float acc[NT][4] = {};
@@ -294,7 +298,7 @@ k_linear_few(int rows, int n, int d, int split, const __nv_bfloat16* __restrict_
         v[1] += sh[k][r][c + 1];
       }
     }
-    const int64_t at = (int64_t)r * n + o0 + c;
+    const int64_t at = (int64_t)(first + r) * n + o0 + c;
     if (NT > 1) shift = bias_of(p, o0 + c);
     v[0] += shift.x;
     v[1] += shift.y;
@@ -415,13 +419,13 @@ int check_linear(int64_t N, int32_t d, int32_t n) {
 
 int launched() { return cudaGetLastError() == cudaSuccess ? ASRN_OK : ASRN_ERR_CUDA; }
 
-template <int NT>
+template <int NT, bool Many = false>
 int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, void* y, void* slope, cudaStream_t s) {
-  const int blocks = (n + 15) / 16;
+  const int blocks = (n + 15) / 16, chunks = (int)((N + 8 * NT - 1) / (8 * NT));
   int split = 1;                                         // blocks of a cluster: until the SMs are full or K is
-  while (split < 8 && blocks * split < gemm::sm_count() && d > split * kFewWarps * 32) split *= 2;
+  while (split < 8 && blocks * chunks * split < gemm::sm_count() && d > split * kFewWarps * 32) split *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(blocks * split));
+  cfg.gridDim = dim3((unsigned)(blocks * split), (unsigned)chunks);
   cfg.blockDim = dim3(kFewWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -432,7 +436,7 @@ int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, vo
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k_linear_few<NT>, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
+  return cudaLaunchKernelEx(&cfg, k_linear_few<NT, Many>, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
                             reinterpret_cast<const __nv_bfloat16*>(w), p, y, reinterpret_cast<__half*>(slope)) == cudaSuccess
              ? ASRN_OK
              : ASRN_ERR_CUDA;
@@ -455,11 +459,12 @@ int asrn_linear_forward(int64_t N, int32_t d, int32_t n, const void* x, const vo
     return ASRN_ERR_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Rest p{reinterpret_cast<const __nv_bfloat16*>(bias), residual, act, residual ? res_type : kNone, act && slope};
-  if (N <= kFewRows && N * n <= kFewValues)
+  if (few_rows(N, n))
     return N <= 8    ? few<1>(N, d, n, x, weight, p, y, slope, s)
            : N <= 16 ? few<2>(N, d, n, x, weight, p, y, slope, s)
            : N <= 32 ? few<4>(N, d, n, x, weight, p, y, slope, s)
-                     : few<8>(N, d, n, x, weight, p, y, slope, s);
+           : N <= 64 ? few<8>(N, d, n, x, weight, p, y, slope, s)
+                     : few<8, true>(N, d, n, x, weight, p, y, slope, s);
   gemm::Shape a{};
   a.M = (int)N; a.N = n; a.K = d; a.group = 16; a.status = status;
   return gemm::launch<false, false, Fused>(x, d, weight, d, a, p, s, {y, N, n, n, p.res_type == kF32},

@@ -332,6 +332,41 @@ def test_linear_infinities_and_nan(cuda, N, act):
     assert torch.equal(asrn.linear(x, w, None, act)[3], good[3])
 
 
+@pytest.mark.parametrize('N,d,n', [(4096, 72, 64), (4100, 72, 64), (1025, 40, 256), (200, 1000, 1312), (5000, 264, 56), (16, 64, 65536),
+                                   (17, 64, 15424), (96, 2056, 136), (320, 136, 816), (321, 136, 824)])
+@pytest.mark.parametrize('act', ['silu', None])
+def test_linear_sizes_on_both_sides_of_the_rule(cuda, N, d, n, act):
+    check_linear(rand((N, d), 130), rand((n, d), 131, d ** -0.5), rand((n,), 132, 0.3), act, rand((N, n), 133), grads=n < 5000)
+
+
+@pytest.mark.parametrize('N,n', [(900, 328), (270, 1000)])
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('res', [None, F32, BF16])
+@pytest.mark.parametrize('bias', [True, False])
+def test_linear_kinds_of_larger_products(cuda, N, n, act, res, bias):
+    check_linear(rand((N, 136), 134), rand((n, 136), 135, 0.2), rand((n,), 136) if bias else None, act,
+                 None if res is None else rand((N, n), 137, dtype=res))
+
+
+@pytest.mark.parametrize('act', ACTS)
+def test_larger_products_over_the_range_and_with_infinities(cuda, act):
+    test_linear_activations_over_their_range(cuda, act, 4200)
+    test_linear_infinities_and_nan(cuda, 3700, act)
+
+
+@pytest.mark.parametrize('N,n', [(130, 96), (5000, 96)])
+def test_linear_rows_do_not_meet(cuda, N, n):
+    """A row's result is its own: other rows changed, and rows behind the last one of the memory, change nothing."""
+    import asrn_b200 as asrn
+    x, w, r = rand((N + 70, 200), 138), rand((n, 200), 139, 0.1), rand((N + 70, n), 140, dtype=F32)
+    x[N:], r[N:] = float('nan'), float('nan')
+    y = asrn.linear(x[:N], w, None, 'gelu', r[:N])
+    assert y.isfinite().all()
+    x[1::2], r[1::2] = float('nan'), float('nan')
+    z = asrn.linear(x[:N], w, None, 'gelu', r[:N])
+    assert torch.equal(z[::2], y[::2]) and z[1::2].isnan().all()
+
+
 def test_linear_views_streams_and_empty(cuda):
     import asrn_b200 as asrn
     big = rand((300, 400), 41)
