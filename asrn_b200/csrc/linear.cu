@@ -213,19 +213,23 @@ ASRN_DEV float2 residual_of(const Rest& p, int64_t at) {
 ASRN_DEV float2 bias_of(const Rest& p, int c) {
   return p.bias ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.bias + c)) : make_float2(0.f, 0.f);
 }
-// Many: more rows than 8 NT, by chunks (blockIdx.y). 64 rows x 1536 -> 768: 8.3 us without, 8.8 with.
-template <int NT, bool Many>
-__global__ void __launch_bounds__(kFewWarps * 32)
+// U: steps of K whose loads are under way together, no more than a warp has. Many: more rows than 8 NT, by chunks (blockIdx.y).
+template <int NT, int U, bool Many>
+__global__ void __launch_bounds__(kFewWarps * 32, 2)
 k_linear_few(int all, int n, int d, int split, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
              const Rest p, void* __restrict__ y, __half* __restrict__ slope) {
-  constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
   __shared__ float sh[kFewWarps][8 * NT][17];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int first = Many ? blockIdx.y * 8 * NT : 0, rows = Many ? min(all - first, 8 * NT) : all;
   const int rank = split > 1 ? (int)gemm::cluster_rank() : 0, o0 = blockIdx.x / split * 16, step = split * kFewWarps * 32;
-  const bool on[2] = {o0 + g < n, o0 + g + 8 < n};
-  const __nv_bfloat16* wp = w + (int64_t)(o0 + g) * d + 8 * t;
-  const __nv_bfloat16* xp = x + (int64_t)(first + g) * d + 8 * t;
+  // Rows past the last are the last one's again (their sums go nowhere), and what is past K is read from its end, and then zero: loads
+  // without a condition are all under way at once.
+  const __nv_bfloat16 *wp = w + (int64_t)o0 * d + 8 * t, *xp = x + (int64_t)first * d + 8 * t;
+  int wr[2], xr[NT];                                     // to the rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i) wr[i] = min(g + i * 8, n - 1 - o0) * d;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) xr[i] = min(g + i * 8, rows - 1) * d;
   wait_previous();
   let_next();
   // Up to 8 rows a thread writes two values at most: their bias and residual are on their way while the products run. (1536 -> 768:
@@ -237,30 +241,30 @@ k_linear_few(int all, int n, int d, int split, const __nv_bfloat16* __restrict__
     shift = bias_of(p, o0 + mine % 8 * 2);
   }
   float acc[NT][4] = {};
-  for (int k0 = (rank * kFewWarps + wid) * 32; k0 < d; k0 += kU * step) {
-    uint4 a[kU][2], b[kU][NT];
+  for (int k0 = (rank * kFewWarps + wid) * 32; k0 < d; k0 += U * step) {
+    uint4 a[U][2], b[U][NT];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int k = k0 + u * step;
-      const bool in = k + 8 * t < d;
+    for (int u = 0; u < U; ++u) {
+      const int k = min(k0 + u * step, d - 8 - 8 * t);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        a[u][i] = make_uint4(0, 0, 0, 0);
-        if (in && on[i]) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (int64_t)i * 8 * d + k));
-      }
+      for (int i = 0; i < 2; ++i) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (wr[i] + k)));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        b[u][i] = make_uint4(0, 0, 0, 0);
-        if (in && i * 8 + g < rows) b[u][i] = __ldg(reinterpret_cast<const uint4*>(xp + (int64_t)i * 8 * d + k));
-      }
+      for (int i = 0; i < NT; ++i) b[u][i] = __ldg(reinterpret_cast<const uint4*>(xp + (xr[i] + k)));
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u * step >= d) break;                     // the same for the whole warp
+      if (k0 + u * step + 8 * t >= d) {
+        a[u][0] = a[u][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) b[u][i] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         mma16x8(acc[i], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][i].x, b[u][i].y);
         mma16x8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
       }
+    }
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -436,7 +440,11 @@ int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, vo
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k_linear_few<NT, Many>, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
+  const int steps = (d + split * kFewWarps * 32 - 1) / (split * kFewWarps * 32);
+  auto kernel = steps == 1             ? k_linear_few<NT, 1, Many>
+                : steps == 2 || NT > 2 ? k_linear_few<NT, 2, Many>
+                                       : k_linear_few<NT, (NT > 2 ? 2 : 4), Many>;
+  return cudaLaunchKernelEx(&cfg, kernel, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
                             reinterpret_cast<const __nv_bfloat16*>(w), p, y, reinterpret_cast<__half*>(slope)) == cudaSuccess
              ? ASRN_OK
              : ASRN_ERR_CUDA;
