@@ -27,11 +27,11 @@ namespace {
 constexpr int kF32 = 0, kBf16 = 1, kNone = 2;            // types of the C interface
 constexpr int kGelu = 1, kSilu = 2, kRelu = 3;
 constexpr int64_t kTwiceRows = 512;
-// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 6.8 | 11.0, 128 rows 8.6 | 11.4, 384 rows 16 | 12; 1536 -> 768,
-// 128 rows 9.6 | 15.3; 128 -> 128, 2048 rows 6.1 | 7.3, 4096 rows 9.1 | 7.4; 4096 -> 512, 128 rows 15 | 30, 768 rows 29 | 29. A row's
-// values are few blocks' then; where y is wide and rows are few the weight's bytes count: 768 -> 50304, 8 rows 17 | 21, 32 rows
-// 33 | 21; 768 -> 8192, 32 rows 7.1 | 11, 64 rows 13 | 11.
-bool few_rows(int64_t N, int64_t n) { return N * n <= 1 << 18 || (N <= 16 && N * n <= 1 << 20); }
+// Graph replays, us, few | by 128 x 256 tiles: 768 -> 1536, 64 rows 6.8 | 11.0, 213 rows 10.2 | 11.5, 341 rows 11.9 | 11.5;
+// 1536 -> 768, 256 rows 9.4 | 15.1, 682 rows 17 | 15; 128 -> 128, 2048 rows 4.2 | 7.3, 8192 rows 14 | 7.5; 4096 -> 512, 384 rows
+// 17 | 29, 1024 rows 32 | 29; 768 -> 8192, 32 rows 7.3 | 11, 64 rows 12 | 11. Up to 16 rows the weight's bytes count, which it loads
+// faster: 768 -> 50304, 8 rows 15 | 22, 16 rows 21 | 23, 24 rows 33 | 23.
+bool few_rows(int64_t N, int64_t n) { return N * n <= 3 << 17 || (N <= 16 && N * n <= 1 << 20); }
 
 ASRN_DEV uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -202,7 +202,7 @@ struct Fused {
 // A and B agree, so a lane takes 8 neighbouring values (16 bytes) of each operand's row for two multiplications: no shared
 // memory, and four lanes read 64 neighbouring bytes. A block's warps take every eighth 32 of K; the blocks of a cluster share K
 // where the columns alone leave SMs idle; the sums meet in shared memory, the blocks' through the cluster's. Graph replays at 768 ->
-// 1536: 1, 8, 16, 32, 64 rows 3.2, 3.5, 4.4, 5.4, 6.8 us, launch and one round trip to memory (2.4 MB take 0.4).
+// 1536: 1, 8, 16, 32, 64 rows 3.3, 3.4, 3.9, 4.9, 6.8 us, launch and one round trip to memory (2.4 MB take 0.4).
 constexpr int kFewWarps = 8;
 ASRN_DEV float2 residual_of(const Rest& p, int64_t at) {
   if (p.res_type == kF32) return __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.res) + at));
@@ -245,6 +245,7 @@ k_linear_few(int all, int n, int d, int split, const __nv_bfloat16* __restrict__
     uint4 a[U][2], b[U][NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (k0 + u * step >= d) break;                     // the same for the whole warp
       const int k = min(k0 + u * step, d - 8 - 8 * t);
 #pragma unroll
       for (int i = 0; i < 2; ++i) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (wr[i] + k)));
@@ -441,9 +442,11 @@ int few(int64_t N, int d, int n, const void* x, const void* w, const Rest& p, vo
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
   const int steps = (d + split * kFewWarps * 32 - 1) / (split * kFewWarps * 32);
-  auto kernel = steps == 1             ? k_linear_few<NT, 1, Many>
-                : steps == 2 || NT > 2 ? k_linear_few<NT, 2, Many>
-                                       : k_linear_few<NT, (NT > 2 ? 2 : 4), Many>;
+  // Blocks enough to keep the memory busy: more of them on an SM (8 rows x 768 -> 50304: 15 us, with four steps under way 21).
+  const bool many = blocks > 4 * gemm::sm_count();
+  auto kernel = steps == 1                     ? k_linear_few<NT, 1, Many>
+                : steps == 2 || NT > 2 || many ? k_linear_few<NT, 2, Many>
+                                               : k_linear_few<NT, (NT > 2 ? 2 : 4), Many>;
   return cudaLaunchKernelEx(&cfg, kernel, (int)N, n, d, split, reinterpret_cast<const __nv_bfloat16*>(x),
                             reinterpret_cast<const __nv_bfloat16*>(w), p, y, reinterpret_cast<__half*>(slope)) == cudaSuccess
              ? ASRN_OK

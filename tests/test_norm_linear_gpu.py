@@ -333,13 +333,15 @@ def test_linear_infinities_and_nan(cuda, N, act):
 
 
 @pytest.mark.parametrize('N,d,n', [(4096, 72, 64), (4100, 72, 64), (1025, 40, 256), (200, 1000, 1312), (5000, 264, 56), (16, 64, 65536),
-                                   (17, 64, 15424), (96, 2056, 136), (320, 136, 816), (321, 136, 824)])
+                                   (17, 64, 15424), (96, 2056, 136), (320, 136, 816), (321, 136, 824),
+                                   (6144, 72, 64), (6145, 72, 64), (48, 264, 8192), (49, 264, 8192), (16, 72, 50304), (17, 72, 50304),
+                                   (1200, 264, 328), (3000, 1000, 136), (700, 1544, 600)])
 @pytest.mark.parametrize('act', ['silu', None])
 def test_linear_sizes_on_both_sides_of_the_rule(cuda, N, d, n, act):
     check_linear(rand((N, d), 130), rand((n, d), 131, d ** -0.5), rand((n,), 132, 0.3), act, rand((N, n), 133), grads=n < 5000)
 
 
-@pytest.mark.parametrize('N,n', [(900, 328), (270, 1000)])
+@pytest.mark.parametrize('N,n', [(900, 328), (270, 1000), (1300, 328), (400, 1000)])
 @pytest.mark.parametrize('act', ACTS)
 @pytest.mark.parametrize('res', [None, F32, BF16])
 @pytest.mark.parametrize('bias', [True, False])
@@ -352,6 +354,8 @@ def test_linear_kinds_of_larger_products(cuda, N, n, act, res, bias):
 def test_larger_products_over_the_range_and_with_infinities(cuda, act):
     test_linear_activations_over_their_range(cuda, act, 4200)
     test_linear_infinities_and_nan(cuda, 3700, act)
+    test_linear_activations_over_their_range(cuda, act, 6200)
+    test_linear_infinities_and_nan(cuda, 5600, act)
 
 
 @pytest.mark.parametrize('N,n', [(130, 96), (5000, 96)])
