@@ -197,8 +197,8 @@ template <bool Top> struct Scan {
 // registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a lane takes 8
 // neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do. Then a warp per row
 // of h over the 128 scores. 8 x 50304 x 768: 11 to 12 us, 6.4 TB/s and more (part of the 77 MB may be left in L2).
-// The whole call as a graph replay, so | by tiles, us: 50304 x 768, 1 row 17 | 22, 8 rows 19 | 23, 20 rows 26 | 24;
-// 16384 x 768, 8 rows 10 | 12, 16 rows 17 | 13; 5003 x 200, 32 rows 7.8 | 8.9, 64 rows 11.4 | 9.3.
+// The whole call as a graph replay, so | by tiles, us: 50304 x 768, 1 row 16 | 22, 8 rows 17 | 23, 20 rows 26 | 24;
+// 16384 x 768, 8 rows 10 | 12, 16 rows 17 | 13; 5003 x 200, 32 rows 7.3 | 8.9, 64 rows 11.4 | 9.3.
 bool few_rows(int64_t N, int64_t V) { return N <= 8 || (N <= 32 && N * V < (1 << 18)); }
 template <int NT, bool Top>
 __global__ void __launch_bounds__(256)
@@ -208,37 +208,43 @@ k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv
   __shared__ __align__(16) float sh[8 * NT][132];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int v0 = blockIdx.x * 128 + wid * 16;
-  const bool on[2] = {v0 + g < V, v0 + g + 8 < V};
-  const __nv_bfloat16* wp = w + (int64_t)(v0 + g) * d + 8 * t;
-  const __nv_bfloat16* hp = h + (int64_t)g * d + 8 * t;
   wait_previous();
   let_next();
   const int rows = count ? *count : N;
+  if (rows <= 0) return;
+  // Rows past the last are the last one's again (their scores go nowhere), and what is past K is read from its end, and then zero: loads
+  // without a condition are all under way at once.
+  const __nv_bfloat16 *wp[2], *hp[NT];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) wp[i] = w + (int64_t)min(v0 + g + i * 8, V - 1) * d + 8 * t;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) hp[i] = h + (int64_t)min(g + i * 8, rows - 1) * d + 8 * t;
   float acc[NT][4] = {};
   for (int k0 = 0; k0 < d; k0 += kU * 32) {
     uint4 a[kU][2], b[kU][NT];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int k = k0 + u * 32;
-      const bool in = k + 8 * t < d;
+      if (k0 + u * 32 >= d) break;                       // the same for the whole warp
+      const int k = min(k0 + u * 32, d - 8 - 8 * t);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        a[u][i] = make_uint4(0, 0, 0, 0);
-        if (in && on[i]) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp + (int64_t)i * 8 * d + k));
-      }
+      for (int i = 0; i < 2; ++i) a[u][i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + k));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        b[u][i] = make_uint4(0, 0, 0, 0);
-        if (in && i * 8 + g < rows) b[u][i] = __ldg(reinterpret_cast<const uint4*>(hp + (int64_t)i * 8 * d + k));
-      }
+      for (int i = 0; i < NT; ++i) b[u][i] = __ldg(reinterpret_cast<const uint4*>(hp[i] + k));
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < kU; ++u) {
+      if (k0 + u * 32 >= d) break;
+      if (k0 + u * 32 + 8 * t >= d) {
+        a[u][0] = a[u][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) b[u][i] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         mma16x8(acc[i], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][i].x, b[u][i].y);
         mma16x8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
       }
+    }
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i)
