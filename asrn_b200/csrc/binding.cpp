@@ -682,7 +682,8 @@ struct Linear : torch::autograd::Function<Linear> {
     }
     variable_list out{dx, dw, db, Tensor(), Tensor()};
     once("linear", out, grads);
-    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2 + biased)) out[3] = grads[0];       // the residual's gradient is the result's
+    // The residual's gradient is the result's.
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2 + biased)) out[3] = grads[0];
     return out;
   }
 };

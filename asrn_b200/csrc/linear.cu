@@ -4,8 +4,8 @@
 // x, W, b bf16; r bf16 or fp32, y of r's type (bf16 without); act: none, gelu (erf), silu, relu.
 //
 // act'(a) is kept rather than a: it lies in [-0.13, 1.13], where fp16 is off by 2^-11 of it at the most, an eighth of what dA's
-// rounding to bf16 takes (a in bf16 would move act'(a) by as much as that), and the backward pass has nothing left to compute. dA is rounded once, as
-// operand of both products; up to kTwiceRows rows they take what the rounding took, too.
+// rounding to bf16 takes (a in bf16 would move act'(a) by as much as that), and the backward pass has nothing left to compute.
+// dA is rounded once, as operand of both products; up to kTwiceRows rows they take what the rounding took, too.
 //
 //   k_linear_few   few results: too few tiles of 128 x 256 for the SMs, and with few rows memory bound (the weight is read once,
 //                  2 operations a byte and row), so the rows of W are spread over all SMs, sixteen a block with up to 64 rows of

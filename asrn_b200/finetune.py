@@ -26,9 +26,10 @@ each, as operands of the next products (and gelu' to fp16). In calls of up to 51
 and rows x V x d up to 2^34), the remainders are multiplied too, and gelu' is not rounded: a weight's gradient from few rows
 would else hold little but those roundings. So a row's y, dx and dh differ in their last bits with the number of rows in the
 call: against 64 bits they are off by 2.3e-3 to 2.5e-3 of themselves in the 2-norm above 512, by 1.7e-3 up to there.
-linear and head_stats follow the same rules (linear: up to 512 rows; it keeps the slope in fp16 in any call), and small calls (linear up
-to 3 2^17 results, 2^20 of up to 16 rows, head_stats up to 8 rows, 32 of small vocabularies) take a kernel that sums in another order. layer_norm rounds its results only. Products are summed in
-fp32 as the tensor cores sum, truncated: a result in fp32 (linear with a residual in fp32) is off by 1e-6 of itself at d = 1536.
+linear and head_stats follow the same rules (linear: up to 512 rows; it keeps the slope in fp16 in any call), and small
+calls (linear up to 3 2^17 results, 2^20 of up to 16 rows, head_stats up to 8 rows, 32 of small vocabularies) take a kernel
+that sums in another order. layer_norm rounds its results only. Products are summed in fp32 as the tensor cores sum,
+truncated: a result in fp32 (linear with a residual in fp32) is off by 1e-6 of itself at d = 1536.
 """
 from collections import namedtuple
 
@@ -138,7 +139,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual in one product: x (..., d), weight (n, d), bias (n) bfloat16 (or float32
     under bf16 autocast), activation None, 'gelu' (erf), 'silu' or 'relu', residual (..., n) float32 or bfloat16 -> (..., n)
     of the residual's type, bfloat16 without one. d and n have to be multiples of 8. For the backward pass it keeps x and
-    the activation's slope in fp16. Small calls (up to 3 2^17 results, 2^20 of up to 16 rows) take a kernel that spreads the weight over the whole GPU."""
+    the activation's slope in fp16. Small calls (up to 3 2^17 results, 2^20 of up to 16 rows) take a kernel that spreads
+    the weight over the whole GPU."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"linear: activation is None, 'gelu', 'silu' or 'relu'; got {activation!r}")
     return _lib.finetune().linear(x, weight, bias, _ACTIVATIONS[activation], residual)

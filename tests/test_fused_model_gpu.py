@@ -193,6 +193,30 @@ def test_stats_of_the_logits(cuda, fundido):
         assert m.stats(x, y).logp.shape == y.shape
 
 
+def test_stats_of_a_padded_batch(cuda):
+    """What stands behind a sequence's end changes nothing before it, in either direction, and gets nothing itself."""
+    f, x = make(cuda, fundido=True)
+    f.eval()
+    y = torch.nn.functional.pad(x[:, 1:], (0, 1), value=-1)
+    end = torch.tensor([70, 41, 1], device=cuda)
+    y = torch.where(torch.arange(70, device=cuda) < end[:, None], y, -1)
+    keep = f.estado
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        with torch.no_grad():
+            h = keep(x).detach()
+        junk = torch.where((torch.arange(70, device=cuda) < end[:, None])[..., None], h, torch.full_like(h, float('nan')))
+        got = []
+        for state in (h, junk):
+            state = state.clone().requires_grad_()
+            f.estado = lambda x, state=state: state
+            r = f.stats(x, y, top=3)
+            w, = (p for n, p in f.named_parameters() if n == 'emb.weight' or n == 'head.weight')
+            got.append((*(t.detach() for t in r), *torch.autograd.grad(r.logp.sum() + r.entropy.sum(), (state, w))))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    off = y < 0
+    assert (got[0][0][off] == 0).all() and (got[0][3][off] == -1).all() and (got[0][4][off] == 0).all()
+
+
 def test_a_policy_step_with_an_entropy_term(cuda):
     """norms, products, head statistics and policy loss in one step, against the same loss by torch's operations on the logits."""
     import asrn_b200 as asrn

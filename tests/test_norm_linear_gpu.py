@@ -371,6 +371,32 @@ def test_linear_rows_do_not_meet(cuda, N, n):
     assert torch.equal(z[::2], y[::2]) and z[1::2].isnan().all()
 
 
+@pytest.mark.parametrize('N', [30, 900])
+@pytest.mark.parametrize('res', [F32, BF16])
+def test_linear_one_gradient_at_a_time_and_broadcast_inputs(cuda, N, res):
+    import asrn_b200 as asrn
+    t = dict(x=rand((N, 72), 141), w=rand((520, 72), 142, 0.2), b=rand((520,), 143), r=rand((N, 520), 144, dtype=res))
+    dy = rand((N, 520), 145, dtype=res)
+    call = lambda q: asrn.linear(q['x'], q['w'], q['b'], 'gelu', q['r'])  # noqa: E731
+    every = {k: v.clone().requires_grad_() for k, v in t.items()}
+    want = dict(zip(every, torch.autograd.grad(call(every), tuple(every.values()), dy)))
+    assert torch.equal(want['r'], dy)
+    for need in t:
+        one = {k: v.clone().requires_grad_(k == need) for k, v in t.items()}
+        got, = torch.autograd.grad(call(one), (one[need],), dy)
+        assert torch.equal(got, want[need]), need
+    # inputs that are a row given to every row: their gradients are the rows' sums
+    row, rrow = t['x'][:1].clone().requires_grad_(), t['r'][:1].clone().requires_grad_()
+    q = dict(every, x=row.expand(N, 72), r=rrow.expand(N, 520))
+    got = torch.autograd.grad(call(q), (row, rrow), dy)
+    full = dict(every, x=t['x'][:1].repeat(N, 1).requires_grad_(), r=t['r'][:1].repeat(N, 1).requires_grad_())
+    dx, dr = torch.autograd.grad(call(full), (full['x'], full['r']), dy)
+    assert torch.equal(got[0], dx.sum(0, keepdim=True)) and torch.equal(got[1], dr.sum(0, keepdim=True))
+    # a scalar's backward pass: a gradient without strides of its own
+    dx, = torch.autograd.grad(call(every).sum(), (every['x'],))
+    assert torch.equal(dx, torch.autograd.grad(call(every), (every['x'],), torch.ones_like(dy))[0])
+
+
 def test_linear_views_streams_and_empty(cuda):
     import asrn_b200 as asrn
     big = rand((300, 400), 41)
