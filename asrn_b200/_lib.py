@@ -162,6 +162,7 @@ _SIGS = {
     'asrn_sampler_fill': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P, _P, _P, _P]),
     'asrn_sample_argmax': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, _P, _P, _P, _P, _P]),
     'asrn_test_force_cuda_core': (ctypes.c_int, [ctypes.c_int]),
+    'asrn_test_norm_reads': (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, _P, _P]),
     'asrn_test_bounded_wait': (ctypes.c_int, [ctypes.c_uint64, _P, _P, _P]),
 }
 

@@ -211,6 +211,15 @@ ASRN_DEV Raw<8> load_to(const void* p, int64_t at, int64_t total, int t) {
   r.b = make_uint4(w[4], w[5], w[6], w[7]);
   return r;
 }
+// Where the vectors of a row that starts anywhere stand: from `at` on, vector 0 to `last`, its first value the shift-th of vector 0.
+// inside: all of them end within the tensor (a row of few values may be followed by others that do not reach a vector's end).
+struct RowAt {
+  int shift, last;
+  int64_t at;
+  bool inside;
+  __host__ ASRN_DEV RowAt(int64_t row, int64_t rows, int d)
+      : shift((int)(row * d & 7)), last((d + shift - 1) / 8), at(row * d - shift), inside(at + 8 * (int64_t)(last + 1) <= rows * d) {}
+};
 // Those of a vector's values that are the row's: j from `low` on, below `high`.
 struct Span {
   int low, high;
@@ -253,11 +262,11 @@ __global__ void __launch_bounds__(threads_of(T), stay_shifted(C, T)) k_norm_shif
   for (int64_t first = (int64_t)blockIdx.x * kRows; first < f.rows; first += (int64_t)gridDim.x * kRows, turn ^= 1) {
     const int64_t row = min(first + sub, f.rows - 1);
     const bool on = first + sub < f.rows;                // else the last row goes along, for its warp's other half
-    const int shift = (int)(row * f.d & 7);
-    const int64_t at = row * f.d - shift;
-    const int last = (f.d + shift - 1) / 8;              // of the row's vectors
+    const RowAt own(row, f.rows, f.d);
+    const int shift = own.shift, last = own.last;
+    const int64_t at = own.at;
     Raw<8> rx[C], rr[C];
-    if (row + 1 < f.rows) {                              // without a condition of each: all under way at once
+    if (own.inside) {                                    // without a condition of each: all under way at once
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const int64_t to = at + 8 * min(tid + i * T, last);
@@ -452,15 +461,17 @@ __global__ void __launch_bounds__(T, T == 256 ? 2 : 1) k_norm_back_shifted(const
   let_next();
   w.fill(f.w, f.wt, f.d);
   __syncthreads();
-  const int tid = threadIdx.x, shift = (int)((int64_t)blockIdx.x * f.d & 7), last = (f.d + shift - 1) / 8;
+  const RowAt first(blockIdx.x, f.rows, f.d);
+  const int tid = threadIdx.x, shift = first.shift, last = first.last;
   const int64_t total = f.rows * f.d;
   float dw[C * 8] = {}, db[C * 8] = {};
   const float inv = 1.f / (float)f.d;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < f.rows; row += gridDim.x, turn ^= 1) {
-    const int64_t at = row * f.d - shift;
+    const RowAt own(row, f.rows, f.d);
+    const int64_t at = own.at;
     Raw<8> rs[C], ry[C], rd[C];
-    if (row + 1 < f.rows) {
+    if (own.inside) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const int64_t to = at + 8 * min(tid + i * T, last);
@@ -862,6 +873,15 @@ bool placed(const void* p, int t) { return (uintptr_t)p % (t == kBf16 ? 2 : 4) =
 }  // namespace asrn
 
 extern "C" {
+
+int asrn_test_norm_reads(int64_t rows, int32_t d, int64_t row, int64_t* from, int64_t* to) {
+  if (!from || !to || d < 1 || row < 0 || row >= rows) return ASRN_ERR_ARG;
+  const asrn::RowAt own(row, rows, d);
+  const int64_t total = rows * d, end = own.at + 8 * (int64_t)(own.last + 1);
+  *from = own.at;
+  *to = own.inside ? end : std::min(end, total);         // load_to reads no value past the end
+  return ASRN_OK;
+}
 
 int asrn_layer_norm(int64_t rows, int32_t d, const void* x, int32_t x_type, const void* residual, int32_t res_type,
                     const void* weight, const void* bias, int32_t w_type, float eps, void* sum, void* y, int32_t y_type,

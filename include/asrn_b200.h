@@ -548,7 +548,10 @@ int asrn_argmax_rows(int64_t rows, int64_t V, const void* x, int32_t dtype, int6
  * asrn_test_bounded_wait: one kernel holding TMEM waits, with the limit limit_ns, on an mbarrier that nothing arrives
  * on, through the same bounded wait every tcgen05 kernel uses; the wait gives up, records ASRN_ERR_TIMEOUT in *status
  * (device int, ASRN_OK before) and the kernel frees its TMEM and returns; *result (device int) = 1 if the wait had
- * completed, 0 if it gave up. */
+ * completed, 0 if it gave up.
+ * asrn_test_norm_reads (host): *from and *to = the range of elements that asrn_layer_norm reads for `row` of a width that
+ * is no multiple of 8. */
+int asrn_test_norm_reads(int64_t rows, int32_t d, int64_t row, int64_t* from, int64_t* to);
 int asrn_test_force_cuda_core(int on);
 int asrn_test_bounded_wait(uint64_t limit_ns, int* status, int* result, void* stream);
 
