@@ -254,7 +254,8 @@ class ModeloASRN(nn.Module):
         h = self.estado(x)
         if self._cabeza_ok(h):
             return head_stats(h, self.head.weight, objetivos, temperatura, top)
-        lp = torch.log_softmax(self.head(h).float() / temperatura, -1)
+        z = self.head(h).float()
+        lp = torch.log_softmax(z / temperatura, -1)
         entropy = -(lp.exp() * lp.clamp(min=-1e4)).sum(-1)       # 0 for p = 0
         logp = top_logp = top_tokens = None
         out = entropy.isnan()
@@ -266,11 +267,11 @@ class ModeloASRN(nn.Module):
             logp = torch.where(on, torch.where(out, math.nan, logp), zero)
         if top:
             with torch.no_grad():
-                top_logp, top_tokens = lp.sort(dim=-1, descending=True, stable=True)
+                top_tokens = z.sort(dim=-1, descending=True, stable=True).indices[..., :top]   # lp rounds neighbours to one value
                 bad = out.unsqueeze(-1)
-                top_logp = torch.where(bad, math.nan, top_logp[..., :top])
+                top_logp = torch.where(bad, math.nan, lp.gather(-1, top_tokens))
                 top_logp = torch.where(on.unsqueeze(-1), top_logp, torch.zeros_like(top_logp))
-                top_tokens = torch.where(on.unsqueeze(-1) & ~bad, top_tokens[..., :top], -1)
+                top_tokens = torch.where(on.unsqueeze(-1) & ~bad, top_tokens, -1)
         return HeadStats(logp, torch.where(on, torch.where(out, math.nan, entropy), zero), top_logp, top_tokens)
 
     def estado(self, x):
