@@ -254,6 +254,8 @@ class ModeloASRN(nn.Module):
         h = self.estado(x)
         if self._cabeza_ok(h):
             return head_stats(h, self.head.weight, objetivos, temperatura, top)
+        if objetivos is not None:
+            h = torch.where(objetivos.unsqueeze(-1) >= 0, h, 0.0)       # what a position left out holds reaches nothing
         z = self.head(h).float()
         lp = torch.log_softmax(z / temperatura, -1)
         entropy = -(lp.exp() * lp.clamp(min=-1e4)).sum(-1)       # 0 for p = 0

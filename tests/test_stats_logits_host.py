@@ -37,3 +37,20 @@ def test_equal_scores_come_in_the_order_of_their_numbers():
     w[25:] = w[:25]
     r = model(h, w).stats(torch.zeros(1, 2, dtype=torch.int64), top=8)
     assert (r.top_tokens[..., 1::2] == r.top_tokens[..., ::2] + 25).all()
+
+
+def test_positions_left_out_reach_no_gradient():
+    """A state that is not finite, at a position without a target."""
+    h, w, y = rand(2, 3, 16, seed=5), rand(40, 16, seed=6), torch.arange(6).view(2, 3)
+    y[0, 1] = -1
+    grads = []
+    for bad in (0.0, float('nan'), float('inf')):
+        t = h.clone()
+        t[0, 1, 3] = bad
+        t.requires_grad_()
+        m = model(t, w)
+        r = m.stats(torch.zeros(2, 3, dtype=torch.int64), y, temperatura=0.7, top=2)
+        assert r.logp[0, 1] == 0 and r.entropy[0, 1] == 0 and (r.top_tokens[0, 1] == -1).all() and (r.top_logp[0, 1] == 0).all()
+        grads.append(torch.autograd.grad((r.logp.sum() + r.entropy.square().sum()), (t, m.head.weight)))
+    for dh, dw in grads[1:]:
+        assert torch.equal(dh, grads[0][0]) and torch.equal(dw, grads[0][1]) and (dh[0, 1] == 0).all()
