@@ -139,10 +139,12 @@ void to_bf16(const char* what, std::initializer_list<Tensor*> ts) {
 }
 
 // The backward passes here are no differentiable functions themselves. Where one is recorded (create_graph), what it makes
-// depends on the node's inputs and on `more` through a node that raises: a second derivative is refused, not left out.
+// depends on the node's inputs and on `more` through a node that raises: a second derivative is refused, not left out. Gradients
+// of outputs that have none are undefined in `more`.
 std::shared_ptr<torch::autograd::Node> refusal(const char* what, const variable_list& more) {
   torch::autograd::edge_list edges = torch::autograd::get_current_node()->next_edges();
-  for (const Tensor& t : more) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  for (const Tensor& t : more)
+    if (t.defined()) edges.push_back(torch::autograd::impl::gradient_edge(t));
   return std::make_shared<torch::autograd::Error>(text("asrn_b200.", what, ": the second derivative is not implemented"),
                                                   std::move(edges));
 }
