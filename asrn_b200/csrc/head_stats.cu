@@ -9,12 +9,12 @@
 //                  group of 32 or 64 columns the largest score, and the second largest with the largest one's column in its low
 //                  6 bits (small vocabularies: all scores)
 //   k_stats_few    the same for few rows
+//   k_stats_sizes  the largest |w|^2 of W's rows, beside or behind the scan (k_stats_few's blocks find it themselves)
 //   k_stats_rows   a warp per row: its sums joined, logp, H; then the groups with the largest scores, which in most rows are the
 //                  likeliest tokens'. Where a second score of a group may count, scores are formed again from h and W by sums
 //                  in fp32, and where these or the products' leave the order open by sums in 64 bits. So the order of the tokens
-//                  is that of their exact scores, equal ones by their numbers. (What a sum in fp32 may be off by is taken from
-//                  sum |h w| of the likeliest token, times two; a token with more than that and large parts that cancel would
-//                  be ranked by its fp32 sum.)
+//                  is that of their exact scores, equal ones by their numbers. What a sum in fp32 may be off by is taken from
+//                  |h| |w| >= sum |h w|, with the largest |w| of the vocabulary
 //   k_gemm<Slope>  backward: the scores again, dS in bf16; then the two products
 #include <algorithm>
 #include "head.cuh"
@@ -58,8 +58,12 @@ int64_t notes_of(int64_t V, int d, int top) { return (V + span_of(V, d, top) - 1
 // Bytes of a row's notes: two numbers a group, or one a column (whole chunks of 32).
 int64_t note_bytes(int64_t V, int d, int top) { return span_of(V, d, top) == 1 ? (V + 31) / 32 * 128 : notes_of(V, d, top) * 8; }
 
+// Numbers that say how large W's rows are, one of each block of k_stats_few or of k_stats_sizes (no more than stay on the SMs at once).
+constexpr int kSizeWarps = 8, kSizeRows = 4;             // k_stats_sizes: a block's warps, a warp's rows at a time
+int size_blocks(int64_t V) { return (int)std::min<int64_t>(3 * gemm::sm_count(), (V + kSizeWarps * kSizeRows - 1) / (kSizeWarps * kSizeRows)); }
+
 struct StatsWs {
-  size_t counts, top, part, notes, total;
+  size_t counts, top, part, notes, sizes, total;
 };
 
 StatsWs stats_ws(int64_t N, int64_t V, int d, int top) {
@@ -71,6 +75,7 @@ StatsWs stats_ws(int64_t N, int64_t V, int d, int top) {
   w.top = take(P * 4);
   w.part = take(parts * P * 16);
   w.notes = take(top ? (size_t)note_bytes(V, d, top) * P : 0);
+  w.sizes = take(top ? (size_t)std::max(size_blocks(V), parts_of(V) / 2) * 4 : 0);
   w.total = o;
   return w;
 }
@@ -98,6 +103,7 @@ template <bool Top> struct Scan {
     float4* part;                          // m, S, T log2(e): [rows][parts]
     float2* notes;                         // of each group: [rows][groups]; span 1: the scores, floats [rows][whole chunks]
     int span, groups;
+    float* sizes;                          // k_stats_few: the largest |w|^2 of each block's columns
   };
   const Params& p;
   int row, V, y, at, parts;
@@ -193,19 +199,111 @@ template <bool Top> struct Scan {
   }
 };
 
+// Squares of sums |w|^2 whose terms leave fp32's range: below, twice this stands for them.
+constexpr float kSmallSquare = 0x1p-100f;
+ASRN_DEV bool plain_square(float q) { return q >= kSmallSquare && q < INFINITY; }
+// The squares of eight values added up in bf16, by twos (a quarter of fp32's instructions: 8 x 50304 x 768 12.5 us, with mma.sync of the
+// rows by themselves 13.7, with fp32 16.6): half a step is 2^-8, so 16 of them are off by up to 2^-4 of the sum, a norm by 2^-5.
+using Two = __nv_bfloat162;
+ASRN_DEV Two no_squares() { return __floats2bfloat162_rn(0.f, 0.f); }
+ASRN_DEV void add_squares(Two& q, const uint4& a) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Two v = *reinterpret_cast<const Two*>(&x[i]);
+    q = __hfma2(v, v, q);
+  }
+}
+ASRN_DEV float sum_of(const Two& q) { return __low2float(q) + __high2float(q); }
+
+// A row's |w|^2 but for that, for the whole warp: 0 for a row of zeros, and for one with an infinity or a NaN, whose scores are not
+// finite whatever the sums round; infinity where it is out of range.
+ASRN_DEV float row_square(const uint4* row, int vecs) {
+  float q = 0.f;
+  uint32_t any = 0;
+  bool bad = false;
+#pragma unroll 4
+  for (int c = threadIdx.x & 31; c < vecs; c += 32) {
+    const uint4 a = __ldg(row + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+    Two sum = no_squares();
+    add_squares(sum, a);
+    q += sum_of(sum);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      any |= x[k] & 0x7fff7fffu;
+      bad |= (x[k] & 0x7f80u) == 0x7f80u || (x[k] >> 16 & 0x7f80u) == 0x7f80u;
+    }
+  }
+  q = warp_sum(q);
+  if (plain_square(q)) return q;
+  if (__any_sync(0xffffffffu, bad) || !__any_sync(0xffffffffu, any != 0)) return 0.f;
+  return fmaxf(q, 2.f * kSmallSquare);
+}
+
+// The largest |w|^2 of each block's rows of W. Launched behind k_gemm<Scan>, whose blocks let it start once all that was before them is
+// complete: it needs nothing of the scan's, and runs beside it on SMs that the scan leaves idle, else behind it. Then it waits for the
+// scan, so that the kernel behind waits for both. Bound by memory, once over W: 50304 x 768 16.5 us (77 MB, 4.7 TB/s), 9 from L2 behind
+// a scan of few rows; a block for each SM 33 and 22.
+__global__ void __launch_bounds__(kSizeWarps * 32, 3)
+k_stats_sizes(int64_t V, int vecs, const uint4* __restrict__ W, float* __restrict__ sizes) {
+  constexpr int kU = 3;                                  // loads of a row under way together
+  __shared__ float most[kSizeWarps];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  let_next();
+  float best = 0.f;
+  for (int64_t v0 = ((int64_t)blockIdx.x * kSizeWarps + wid) * kSizeRows; v0 < V; v0 += (int64_t)gridDim.x * kSizeWarps * kSizeRows) {
+    const uint4* row[kSizeRows];
+    float sum[kSizeRows] = {};
+#pragma unroll
+    for (int i = 0; i < kSizeRows; ++i) row[i] = W + (v0 + i < V ? v0 + i : V - 1) * vecs;   // past the last one: that one again
+    for (int c = lane; c - lane < vecs; c += 32 * kU) {
+      uint4 a[kU][kSizeRows];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int i = 0; i < kSizeRows; ++i) a[u][i] = __ldg(row[i] + min(c + 32 * u, vecs - 1));
+#pragma unroll
+      for (int i = 0; i < kSizeRows; ++i) {
+        Two q = no_squares();
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (c + 32 * u < vecs) add_squares(q, a[u][i]);
+        sum[i] += sum_of(q);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSizeRows; ++i) {
+      float q = warp_sum(sum[i]);
+      if (!plain_square(q)) q = row_square(row[i], vecs);
+      best = fmaxf(best, q);
+    }
+  }
+  if (lane == 0) most[wid] = best;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 1; k < kSizeWarps; ++k) best = fmaxf(best, most[k]);
+    sizes[blockIdx.x] = best;
+  }
+  wait_previous();
+}
+
 // The same for few rows, bound by the weight's bytes: block = 128 columns, a warp 16 of them and all of K; mma.sync from
 // registers (A = 16 rows of W, B = the rows of h; the order of K inside a tile is free as long as both agree, so a lane takes 8
 // neighbouring values of each), whose loads keep the memory busier than two rounds of 128 x 256 tiles do. Then a warp per row
-// of h over the 128 scores. 8 x 50304 x 768: 11 to 12 us, 6.4 TB/s and more (part of the 77 MB may be left in L2).
-// The whole call as a graph replay, so | by tiles, us: 50304 x 768, 1 row 16 | 22, 8 rows 17 | 23, 20 rows 26 | 24;
-// 16384 x 768, 8 rows 10 | 12, 16 rows 17 | 13; 5003 x 200, 32 rows 7.3 | 8.9, 64 rows 11.4 | 9.3.
-bool few_rows(int64_t N, int64_t V) { return N <= 8 || (N <= 32 && N * V < (1 << 18)); }
+// of h over the 128 scores. 8 x 50304 x 768: 12.5 us with 77 MB partly from L2, 6.2 TB/s (11.8 without the squares of W's rows).
+// The whole call as a graph replay, so | by tiles, us, 5 tokens: 50304 x 768, 1 row 19 | 36, 8 rows 24 | 39, 16 rows 33 | 41, 20 rows 42 | 40;
+// 16384 x 768, 8 rows 16 | 23, 16 rows 20 | 25, 32 rows 24 | 25; 5003 x 200, 32 rows 17 | 18; without tokens: 50304 x 768, 8 rows
+// 13 | 21, 16 rows 20 | 21, 20 rows 27 | 21; 16384 x 768, 16 rows 10 | 12, 32 rows 12 | 11.
+bool few_rows(int64_t N, int64_t V) { return N <= 16 || (N <= 32 && N * V < (1 << 18)); }
 template <int NT, bool Top>
 __global__ void __launch_bounds__(256)
 k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w,
             const int* __restrict__ count, const typename Scan<Top>::Params p) {
   constexpr int kU = NT <= 2 ? 4 : 2;                    // steps of K whose loads are under way together
   __shared__ __align__(16) float sh[8 * NT][132];
+  __shared__ float sizes[8];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int v0 = blockIdx.x * 128 + wid * 16;
   wait_previous();
@@ -220,6 +318,7 @@ k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv
 #pragma unroll
   for (int i = 0; i < NT; ++i) hp[i] = h + (int64_t)min(g + i * 8, rows - 1) * d + 8 * t;
   float acc[NT][4] = {};
+  float squares[2] = {};                                 // of W's two rows
   for (int k0 = 0; k0 < d; k0 += kU * 32) {
     uint4 a[kU][2], b[kU][NT];
 #pragma unroll
@@ -245,12 +344,46 @@ k_stats_few(int N, int V, int d, const __nv_bfloat16* __restrict__ h, const __nv
         mma16x8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
       }
     }
+    if (Top) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Two q = no_squares();
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (k0 + u * 32 < d) add_squares(q, a[u][i]);
+        squares[i] += sum_of(q);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sh[i * 8 + 2 * t + (j & 1)][wid * 16 + g + (j >> 1) * 8] = acc[i][j];
+  if (Top) {
+    float q = 0.f;
+    bool plain = true;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                        // four lanes hold a row's
+      float one = squares[i];
+      one += __shfl_xor_sync(0xffffffffu, one, 1);
+      one += __shfl_xor_sync(0xffffffffu, one, 2);
+      plain &= plain_square(one);
+      q = fmaxf(q, one);
+    }
+    q = warp_max(q);
+    if (!__all_sync(0xffffffffu, plain)) {
+      q = 0.f;
+      for (int i = 0; i < 16; ++i) q = fmaxf(q, row_square(reinterpret_cast<const uint4*>(w) + (int64_t)min(v0 + i, V - 1) * (d / 8), d / 8));
+    }
+    if (lane == 0) sizes[wid] = q;
+  }
   __syncthreads();
+  if (Top && threadIdx.x == 0) {
+    float q = sizes[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) q = fmaxf(q, sizes[k]);
+    p.sizes[blockIdx.x] = q;
+  }
   const int parts = parts_of(V);
   for (int r = wid; r < rows && r < 8 * NT; r += 8) {
     const int y = p.tok ? p.tok[r] : kNoTarget, c0 = blockIdx.x * 128 + lane * 4;
@@ -379,14 +512,13 @@ template <int Each, class Notes> struct Groups {
       best = max(best, key[j]);
     }
   }
-  ASRN_DEV int next(float2& pair) {              // the next group, -1: none left
+  ASRN_DEV int next() {                          // the next group, -1: none left
     const int lane = threadIdx.x & 31;
     const uint32_t most = __reduce_max_sync(0xffffffffu, best & ~127u);
     if (most == 0) return -1;
     const int j = Each - 1 - (int)(best & 127u);
     const int mine = (best & ~127u) == most ? lane + 32 * j : 0x7fffffff;
     const int g = (int)__reduce_min_sync(0xffffffffu, (unsigned)mine);
-    pair = notes(g);
     if (mine == g) {
       best = 0;
 #pragma unroll
@@ -420,13 +552,12 @@ template <class Notes> struct Groups<0, Notes> {
       }
     }
   }
-  ASRN_DEV int next(float2& pair) {
+  ASRN_DEV int next() {
     const uint32_t most = __reduce_max_sync(0xffffffffu, key);
     if (most == 0) return -1;
     const int g = (int)__reduce_min_sync(0xffffffffu, key == most ? (unsigned)group : 0x7fffffffu);
     last = most;
     last_group = g;
-    pair = notes(g);
     if (group == g && key == most) find();
     __syncwarp();
     return g;
@@ -457,22 +588,8 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int (&token)[
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = warp_sum_d(acc[j]);
 }
-// sum |h w| of one row of W.
-ASRN_DEV float magnitude(const uint4* h, const uint4* W, int vecs, int token) {
-  float s = 0.f;
-#pragma unroll 4
-  for (int c = threadIdx.x & 31; c < vecs; c += 32) {
-    const uint4 a = __ldg(h + c), b = __ldg(W + (int64_t)token * vecs + c);
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      s += fabsf(__uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16)) +
-           fabsf(__uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u));
-  }
-  return warp_sum(s);
-}
 // The same for sixteen rows of W by mma.sync, in two chains of fp32 sums: lane 4 j gets the rows j (first) and j + 8 (second)
-// that its lanes 4 j to 4 j + 3 name. Loads as in k_stats_few. size: the largest sum |h w| of the first eight.
+// that its lanes 4 j to 4 j + 3 name. Loads as in k_stats_few.
 struct Pair {
   float a, b;
   ASRN_DEV float of(int j) const {               // row j's, for the whole warp
@@ -480,11 +597,10 @@ struct Pair {
     return j < 8 ? x : y;
   }
 };
-template <int U, bool Size>
-ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int row_b, float* size) {
+template <int U> ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int row_b) {
   const int lane = threadIdx.x & 31, t = lane & 3;
   const uint4 *wa = W + (int64_t)row_a * vecs, *wb = W + (int64_t)row_b * vecs;
-  float acc[2][4] = {}, mag[4] = {};
+  float acc[2][4] = {};
   for (int k = t; k - t < vecs; k += 4 * U) {
     uint4 a[U], b[U], x[U];
 #pragma unroll
@@ -499,14 +615,8 @@ ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int ro
     for (int u = 0; u < U; ++u) {
       mma16x8(acc[u & 1], a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
       mma16x8(acc[u & 1], a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
-      if (Size) {
-        constexpr uint32_t m = 0x7fff7fffu;
-        mma16x8(mag, a[u].x & m, 0, a[u].y & m, 0, x[u].x & m, x[u].y & m);
-        mma16x8(mag, a[u].z & m, 0, a[u].w & m, 0, x[u].z & m, x[u].w & m);
-      }
     }
   }
-  if (Size) *size = warp_max(mag[0]);
   return Pair{acc[0][0] + acc[1][0], acc[0][2] + acc[1][2]};
 }
 
@@ -535,14 +645,18 @@ template <class T> struct Best {
 };
 
 constexpr int kRowWarps = 4;
+// What a product's sum loses by a step, of the magnitudes: a step adds 16 products to the sum so far, each of which loses up to 2^-25 of
+// the largest of them, their sum up to 2^-23: 2.6 2^-22 (one large value and small ones lose 2.05 2^-22 by tcgen05, 1.05 by mma.sync).
+// With what both norms are off by (2^-4) 2.8; the rest is room.
+constexpr float kOff = 3 * 0x1p-22f;
 struct RowArgs {
   int64_t N;
-  int V, d, top, parts, span, groups;
+  int V, d, top, parts, span, groups, sizes_n;
   float k, inv_tau;
   const uint4 *hc, *W;
   const int *pos, *tok;                          // null: every position is a row, without a target
   const float4* part;
-  const float *notes, *own;
+  const float *notes, *own, *sizes;
   float *lse2, *kept_logp, *kept_ent;            // by rows, for the backward pass; or null
   float *logp, *entropy, *top_logp;              // by positions; logp may be null
   int64_t* top_tokens;
@@ -550,9 +664,9 @@ struct RowArgs {
 
 // U: steps of K whose loads are under way together: 8 where a slow row's latency is what counts, 2 where rows are many and short, so that
 // more share an SM (8 tokens, us, 8 | 2, before rows kept the products' sums: 50304 x 768, 2048 rows 54 | 105, 4096 78 | 108,
-// 8192 125 | 150; 5003 x 200, 2048 rows 22 | 30, 8192 59 | 50). Now 49 us at 2048 x 50304 x 768, 22 at 2048 x 5003 x 200.
+// 8192 125 | 150; 5003 x 200, 2048 rows 22 | 30, 8192 59 | 50). Now 45 us at 2048 x 50304 x 768, 22 at 2048 x 5003 x 200.
 template <int Each, int U, bool Whole>
-__global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7) k_stats_rows(const RowArgs f) {
+__global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 6) k_stats_rows(const RowArgs f) {
   const int lane = threadIdx.x & 31, top = f.top, vecs = f.d / 8;
   const int64_t i = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   wait_previous();
@@ -561,6 +675,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   const int r = f.pos ? f.pos[i] : (int)i, y = r < 0 ? -1 : f.tok ? f.tok[r] : kNoTarget;
   float lp = 0.f, H = 0.f, l2 = 0.f, own = 0.f;
   double base = 0.0;
+  // How large the row and W's are, of which more below. Where latency counts: loads that are under way while the sums are joined.
+  constexpr int kEarly = U > 2 ? 16 : 1, kOwn = U > 2 ? 4 : 1;
+  const uint4* h = f.hc + (int64_t)(r < 0 ? 0 : r) * vecs;
+  float early[kEarly];
+  uint4 row[kOwn];
+  if (U > 2 && top && r >= 0) {
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) early[j] = __ldg(f.sizes + min(lane + 32 * j, f.sizes_n - 1));
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) row[j] = __ldg(h + min(lane + 32 * j, vecs - 1));
+  }
   if (r >= 0) {                                  // the row's sums: by lanes, then the lanes'
     own = y >= 0 ? f.own[r] : 0.f;
     const float4* part = f.part + (int64_t)r * f.parts;
@@ -615,36 +740,55 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     write(r < 0 ? 0.f : NAN, -1);
     return;
   }
-  const uint4* h = f.hc + (int64_t)r * vecs;
+  // What a sum of the products may be off by, for any token: kOff a step of |h| |w|, which is no less than sum |h w|.
+  float own_square = 0.f, square = 0.f;
+  if (U > 2) {
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) square = fmaxf(square, early[j]);
+    Two q = no_squares();
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (lane + 32 * j < vecs) add_squares(q, row[j]);
+    own_square = sum_of(q);
+  }
+#pragma unroll 8
+  for (int g = lane + (U > 2 ? 32 * kEarly : 0); g < f.sizes_n; g += 32) square = fmaxf(square, __ldg(f.sizes + g));
+  if (U > 2) own_square = warp_sum(own_square);
+  if (U == 2 || vecs > 32 * kOwn || !plain_square(own_square)) own_square = row_square(h, vecs);
+  square = warp_max(square);
+  const float slack = square == 0.f ? 0.f : (float)(f.d / 16 + 2) * kOff * sqrtf(own_square) * sqrtf(square);
+  if (own_square == 0.f) {                       // a row of zeros: all scores are 0
+    write((float)-base, lane);
+    return;
+  }
   const Notes<Whole> notes{f.notes + (int64_t)r * (Whole ? (f.V + 31) / 32 * 32 : 2 * f.groups)};
   auto column_of = [&](int g, float2 note) { return Whole ? g : g * f.span + (int)(__float_as_uint(note.y) & 63u); };
 
-  // The first `top` groups by lane, and the one after them.
+  // The first groups by lane, `top` and some more, so that the one after them hardly ever counts (where each costs reading the notes
+  // again, without these); and the one after them.
+  const int limit = Each ? min(32, top + 4) : top;
   float2 pair = make_float2(kNothing, kNothing), held = pair;
   int held_group = 0, have = 0, after = -1;
   {
     Groups<Each, Notes<Whole>> groups(notes, f.groups);
     while (true) {
-      after = groups.next(pair);
-      if (after < 0 || have == top) break;
-      if (lane == have) {
-        held = pair;
-        held_group = after;
-      }
+      after = groups.next();
+      if (after < 0 || have == limit) break;
+      if (lane == have) held_group = after;
       ++have;
     }
+    if (lane < have) held = notes(held_group);
+    if (after >= 0) pair = notes(after);
   }
   const int column = column_of(held_group, held);
 
   // Their largest, and the target: in most rows these are the answer, as the products summed them. For the row's scores may be off by
-  // `slack` (sums of 16 products, truncated; with twice the magnitudes of the likeliest one), notes by their low bits more.
+  // `slack`, notes by their low bits more.
   Best<float> best;
   for (int q = 0; q < have; ++q) best.put(__shfl_sync(0xffffffffu, held.x, q), __shfl_sync(0xffffffffu, column, q));
   if (y >= 0) best.put(own, y);
   auto low = [&]() { return __shfl_sync(0xffffffffu, best.score, top - 1); };
-  const int likeliest = __shfl_sync(0xffffffffu, best.token, 0);
-  float size = likeliest < f.V ? magnitude(h, f.W, vecs, likeliest) : 0.f, off = 0.f;
-  float slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
+  float off = 0.f;
   auto above = [&](float v) { return v + (fabsf(v) * 0x1p-15f + slack + off); };
   // Those that stand within `width` of their neighbours, down to that far below the last one that counts, by sums in 64 bits; others
   // keep their places among them.
@@ -652,39 +796,40 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   auto settle = [&](float width) {
     const float then = __shfl_down_sync(0xffffffffu, best.score, 1);
     const float least = low() - width;
-    unsigned near = __ballot_sync(0xffffffffu, lane < 31 && then >= least && best.score - then <= width);
+    unsigned near = __ballot_sync(0xffffffffu, lane < 31 && then > -INFINITY && then >= least && best.score - then <= width);
     score = best.score;
     if (!near) return;
     near |= near << 1;
-    Best<double> exact;
-    unsigned rest = near;
-    for (int q = 0; q < 32; ++q) {
-      if (!(near >> q & 1u)) {
-        const float sc = __shfl_sync(0xffffffffu, best.score, q);
-        exact.put((double)sc, __shfl_sync(0xffffffffu, best.token, q));
-        continue;
-      }
-      if (!(rest >> q & 1u)) continue;
-      int t[4];                                  // the next four of them
-      bool on[4];
+    const int n = 32 - __clz(near);              // those behind keep their places
+    while (near) {                               // four at a time
+      int t[4], from[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        on[j] = rest != 0;
-        t[j] = __shfl_sync(0xffffffffu, best.token, on[j] ? __ffs(rest) - 1 : q);
-        rest &= rest - 1;
+        from[j] = near ? __ffs(near) - 1 : from[max(j - 1, 0)];
+        t[j] = __shfl_sync(0xffffffffu, best.token, from[j]);
+        near &= near - 1;
       }
       double sums[4];
       dots(h, f.W, vecs, t, sums);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (on[j]) exact.put(sums[j], t[j]);
+        if (lane == from[j]) score = sums[j];
     }
-    best.token = exact.token;
-    score = exact.score;
+    // Each lane's place among the n, and whose place is its number. As whole numbers that order as the scores do: without branches.
+    const long long bits = __double_as_longlong(score + 0.0), key = bits ^ (bits >> 63 & 0x7fffffffffffffffll);
+    int place = lane < n ? 0 : lane, whose = lane;
+    for (int q = 0; q < n; ++q) {
+      const long long other = __shfl_sync(0xffffffffu, key, q);
+      const int t = __shfl_sync(0xffffffffu, best.token, q);
+      place += (lane < n) & ((other > key) | ((other == key) & (t < best.token)));
+    }
+    for (int q = 0; q < n; ++q) whose = __shfl_sync(0xffffffffu, place, q) == lane ? q : whose;
+    best.token = __shfl_sync(0xffffffffu, best.token, whose);
+    score = __shfl_sync(0xffffffffu, score, whose);
   };
   {
     const float lowest = low() - slack;
-    const bool open = size == 0.f || (lane < top && best.token >= f.V) || (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
+    const bool open = (lane < top && best.token >= f.V) || (lane < have && held.y > -3e38f && above(held.y) >= lowest) ||
                       (after >= 0 && above(pair.x) >= lowest) || best.lost >= lowest - slack;
     if (!__any_sync(0xffffffffu, open)) {
       settle(2 * slack);
@@ -693,17 +838,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     }
   }
 
-  // Else all that may count, by the products' sums or by sums here (two chains, off by less). Where the likeliest one's magnitudes are 0,
-  // those of the others, and should they be rows of zeros those of eight from all over the vocabulary.
-  if (size == 0.f) {
-    const int some = __shfl_sync(0xffffffffu, column, min(lane >> 2, max(have - 1, 0)));
-    if (have) dots16<U, true>(h, f.W, vecs, some, some, &size);
-    if (size == 0.f) {
-      const int sample = (int)((int64_t)(lane >> 2) * f.V / 8);
-      dots16<U, true>(h, f.W, vecs, sample, sample, &size);
-    }
-    slack = (float)(f.d / 16 + 2) * 0x1p-22f * size;
-  }
+  // Else all that may count, by the products' sums or by sums here (two chains, off by less).
   off = slack;
   float bar = low();                             // no more than the last score that counts
   bar -= fabsf(bar) * 0x1p-15f;
@@ -724,7 +859,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
     const int begin = g * f.span, end = min(f.V, begin + f.span);
     for (int c = begin; c < end; c += 16) {
       const int ra = c + (lane >> 2), rb = ra + 8;
-      const Pair about = dots16<U, false>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1), nullptr);
+      const Pair about = dots16<U>(h, f.W, vecs, min(ra, end - 1), min(rb, end - 1));
       const float least = fmaxf(low(), bar) - 2 * off;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -748,7 +883,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   }
   if (after >= 0 && above(pair.x) >= low()) {
     Groups<0, Notes<Whole>> rest(notes, f.groups, order_of(pair.x), after);
-    for (; after >= 0 && above(pair.x) >= low(); after = rest.next(pair)) {
+    for (; after >= 0; after = rest.next()) {
+      pair = notes(after);
+      if (above(pair.x) < low()) break;
       const int c = column_of(after, pair);
       const bool unsure = pair.y > -3e38f && pair.y >= pair.x - fabsf(pair.x) * 0x1p-15f;
       if (!unsure) best.put(pair.x, c);
@@ -761,40 +898,29 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 7)
   if (best.lost < least) {                       // the few that were kept hold all that may count
     settle(2 * off);
   } else {
-    double s[4];
+    // Many that are equal or all but that: all of them.
     Best<double> exact;
-    if (size == 0.f && !__any_sync(0xffffffffu, [&] {
-                 uint32_t any = 0;
-                 for (int c = lane; c < vecs; c += 32) {
-                   const uint4 a = __ldg(h + c);
-                   any |= (a.x | a.y | a.z | a.w) & 0x7fff7fffu;
-                 }
-                 return any;
-               }())) {                           // a row of zeros: all scores are 0
-      exact.score = 0.0;
-      exact.token = lane;
-    } else {                                     // many that are equal or all but that: all of them
-      auto exact_put = [&](float, int token) {
-        const int t[4] = {token, token, token, token};
-        dots(h, f.W, vecs, t, s);
-        exact.put(s[0], token);
-      };
-      if (y >= 0) exact_put(0.f, y);
-      for (int g0 = 0; g0 < f.groups; g0 += 32) {
-        const float largest = notes.largest(min(g0 + lane, f.groups - 1)), lowest = low();   // a shuffle: not behind a condition
-        unsigned set = __ballot_sync(0xffffffffu, g0 + lane < f.groups && largest > -3e38f && above(largest) >= lowest);
-        for (; set; set &= set - 1) {
-          const int g = g0 + __ffs(set) - 1;
-          const float most = above(__shfl_sync(0xffffffffu, largest, g - g0));
-          // nothing of it comes before the last one that counts so far, not as its equal either
-          const double last = __shfl_sync(0xffffffffu, exact.score, top - 1);
-          const int number = __shfl_sync(0xffffffffu, exact.token, top - 1);
-          if ((double)most < last || ((double)most == last && number < g * f.span)) continue;
-          if constexpr (Whole) {
-            if (g != y) exact_put(0.f, g);
-          } else {
-            expand(g, -1, exact_put);
-          }
+    auto exact_put = [&](float, int token) {
+      const int t[4] = {token, token, token, token};
+      double s[4];
+      dots(h, f.W, vecs, t, s);
+      exact.put(s[0], token);
+    };
+    if (y >= 0) exact_put(0.f, y);
+    for (int g0 = 0; g0 < f.groups; g0 += 32) {
+      const float largest = notes.largest(min(g0 + lane, f.groups - 1)), lowest = low();   // a shuffle: not behind a condition
+      unsigned set = __ballot_sync(0xffffffffu, g0 + lane < f.groups && largest > -3e38f && above(largest) >= lowest);
+      for (; set; set &= set - 1) {
+        const int g = g0 + __ffs(set) - 1;
+        const float most = above(__shfl_sync(0xffffffffu, largest, g - g0));
+        // nothing of it comes before the last one that counts so far, not as its equal either
+        const double last = __shfl_sync(0xffffffffu, exact.score, top - 1);
+        const int number = __shfl_sync(0xffffffffu, exact.token, top - 1);
+        if ((double)most < last || ((double)most == last && number < g * f.span)) continue;
+        if constexpr (Whole) {
+          if (g != y) exact_put(0.f, g);
+        } else {
+          expand(g, -1, exact_put);
         }
       }
     }
@@ -934,14 +1060,19 @@ int asrn_head_stats_forward(int64_t N, int64_t V, int32_t d, const void* h, cons
   float* own = reinterpret_cast<float*>(W + ws.top);
   float4* part = reinterpret_cast<float4*>(W + ws.part);
   float2* notes = reinterpret_cast<float2*>(W + ws.notes);
+  float* sizes = reinterpret_cast<float*>(W + ws.sizes);
   const int span = span_of(V, d, top), groups = (int)notes_of(V, d, top);
   if (top)
-    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
+    st = scan<true>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups, sizes}, s);
   else
-    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups}, s);
+    st = scan<false>(N, V, d, hc, weight, sh, {tok, k, own, part, notes, span, groups, nullptr}, s);
   if (st) return st;
-  const RowArgs f{N, (int)V, d, top, parts, span, groups, k, inv_tau, reinterpret_cast<const uint4*>(hc),
-                  reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own,
+  const bool own_sizes = few_rows(N, V);
+  if (top && !own_sizes &&
+      (st = launch_next(k_stats_sizes, size_blocks(V), kSizeWarps * 32, 0, s, V, d / 8, reinterpret_cast<const uint4*>(weight), sizes)))
+    return st;
+  const RowArgs f{N, (int)V, d, top, parts, span, groups, own_sizes ? parts / 2 : size_blocks(V), k, inv_tau, reinterpret_cast<const uint4*>(hc),
+                  reinterpret_cast<const uint4*>(weight), pos, tok, part, reinterpret_cast<const float*>(notes), own, sizes,
                   reinterpret_cast<float*>(kept(sv.head.lse2)), reinterpret_cast<float*>(kept(sv.head.rest)),
                   reinterpret_cast<float*>(kept(sv.ent)), tokens ? logp : nullptr, entropy, top_logp, top_tokens};
   const bool few = N <= (int64_t)gemm::sm_count() * kRowWarps * std::max(4, d / 48);

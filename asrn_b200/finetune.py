@@ -27,7 +27,7 @@ and rows x V x d up to 2^34), the remainders are multiplied too, and gelu' is no
 would else hold little but those roundings. So a row's y, dx and dh differ in their last bits with the number of rows in the
 call: against 64 bits they are off by 2.3e-3 to 2.5e-3 of themselves in the 2-norm above 512, by 1.7e-3 up to there.
 linear and head_stats follow the same rules (linear: up to 512 rows; it keeps the slope in fp16 in any call), and small
-calls (linear up to 3 2^17 results, 2^20 of up to 16 rows, head_stats up to 8 rows, 32 of small vocabularies) take a kernel
+calls (linear up to 3 2^17 results, 2^20 of up to 16 rows, head_stats up to 16 rows, 32 of small vocabularies) take a kernel
 that sums in another order. layer_norm rounds its results only. Products are summed in fp32 as the tensor cores sum,
 truncated: a result in fp32 (linear with a residual in fp32) is off by 1e-6 of itself at d = 1536.
 """
