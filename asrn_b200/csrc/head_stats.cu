@@ -898,13 +898,21 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 6)
   if (best.lost < least) {                       // the few that were kept hold all that may count
     settle(2 * off);
   } else {
-    // Many that are equal or all but that: all of them.
+    // Many that are equal or all but that: all of them, four at a time.
+    int t[4] = {}, waiting = 0;
     Best<double> exact;
-    auto exact_put = [&](float, int token) {
-      const int t[4] = {token, token, token, token};
+    auto settle_waiting = [&]() {
       double s[4];
       dots(h, f.W, vecs, t, s);
-      exact.put(s[0], token);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < waiting) exact.put(s[j], t[j]);
+      waiting = 0;
+    };
+    auto exact_put = [&](float, int token) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = j == waiting ? token : t[j];
+      if (++waiting == 4) settle_waiting();
     };
     if (y >= 0) exact_put(0.f, y);
     for (int g0 = 0; g0 < f.groups; g0 += 32) {
@@ -924,6 +932,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, U > 2 ? 2 : Each > 32 ? 4 : 6)
         }
       }
     }
+    if (waiting) settle_waiting();
     best.token = exact.token;
     score = exact.score;
   }
