@@ -325,13 +325,14 @@ k_linear_few(int all, int n, int d, int split, const __nv_bfloat16* __restrict__
   if (split > 1) gemm::cluster_sync();                   // no block ends while another reads its sums
 }
 
-// dA = dY slope in bf16 (da null: not wanted; slope null: 1), its remainder `below` rows further on unless that is 0 (then rows
-// from `rows` to `below` are zeros in both), and its columns' sums over 64 rows. Block = 64 rows x 256 columns, a lane 8 columns,
+// dA = dY slope in bf16 (da null: not wanted; slope null: 1; relu: what it left out takes no part, whatever dY holds there), its
+// remainder `below` rows further on unless that is 0 (then rows from `rows` to `below` are zeros in both; an infinity leaves no
+// remainder), and its columns' sums over 64 rows. Block = 64 rows x 256 columns, a lane 8 columns,
 // a warp every eighth row.
 constexpr int kSlopeRows = 64;
 template <bool F32>
 __global__ void __launch_bounds__(256)
-k_linear_slope(int64_t rows, int n, int below, const void* __restrict__ dy, const __half* __restrict__ slope,
+k_linear_slope(int64_t rows, int n, int below, bool relu, const void* __restrict__ dy, const __half* __restrict__ slope,
                __nv_bfloat16* __restrict__ da, float* __restrict__ sums) {
   __shared__ float sh[8][256];
   const int wide = (n + 255) / 256, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -367,8 +368,8 @@ k_linear_slope(int64_t rows, int n, int below, const void* __restrict__ dy, cons
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&z[j]));
-          v[2 * j] *= x.x;
-          v[2 * j + 1] *= x.y;
+          v[2 * j] = !relu ? v[2 * j] * x.x : x.x == 0.f ? 0.f : v[2 * j];
+          v[2 * j + 1] = !relu ? v[2 * j + 1] * x.y : x.y == 0.f ? 0.f : v[2 * j + 1];
         }
       }
 #pragma unroll
@@ -377,7 +378,10 @@ k_linear_slope(int64_t rows, int n, int below, const void* __restrict__ dy, cons
         *reinterpret_cast<uint4*>(da + r * n + c) = gemm::pack8(v);
         if (below) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] -= round_bf16(v[j]);
+          for (int j = 0; j < 8; ++j) {
+            const float r = round_bf16(v[j]);
+            v[j] = fabsf(r) < INFINITY ? v[j] - r : 0.f;
+          }
           *reinterpret_cast<uint4*>(da + (r + below) * n + c) = gemm::pack8(v);
         }
       }
@@ -515,9 +519,9 @@ int asrn_linear_backward(int64_t N, int32_t d, int32_t n, const void* dy, int32_
     __nv_bfloat16* to = own || !(dx || dw) ? nullptr : made;
     const __half* f = act ? reinterpret_cast<const __half*>(slope) : nullptr;
     if (y_type == kF32)
-      k_linear_slope<true><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, dy, f, to, db ? sums : nullptr);
+      k_linear_slope<true><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, act == kRelu, dy, f, to, db ? sums : nullptr);
     else
-      k_linear_slope<false><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, dy, f, to, db ? sums : nullptr);
+      k_linear_slope<false><<<(unsigned)blocks, 256, 0, s>>>(N, n, ws.below, act == kRelu, dy, f, to, db ? sums : nullptr);
     if ((st = launched())) return st;
   }
   const void* da = own ? dy : made;
