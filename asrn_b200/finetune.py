@@ -40,8 +40,8 @@ from . import _lib
 
 def status(device=None, reset=False):
     """0, or the error that these kernels recorded on the device (ASRN_ERR_TIMEOUT: a bounded wait gave up, and the
-    results since then are void). Synchronises. While an error stands head_logprobs, mlp8 and their backward passes raise
-    RuntimeError as soon as the host sees it; reset=True clears it and allows new calls."""
+    results since then are void). Synchronises. While an error stands head_logprobs, head_stats, linear, mlp8 and their backward
+    passes raise RuntimeError as soon as the host sees it; reset=True clears it and allows new calls."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.type != 'cuda':
         raise ValueError(f'status: {dev} is not a CUDA device')
@@ -159,6 +159,7 @@ def head_stats(h, weight, tokens=None, temperatura=1.0, top=0):
                   by sums in 64 bits
     Differentiable in h and weight through logp and entropy. A negative token leaves its position out (0, tokens -1, no
     gradient, none of the work); a token >= V, and scores whose exponentials have no finite sum, give NaN and tokens -1. d has
-    to be a multiple of 8; the call takes V / 4 bytes of workspace a position (with top up to V / 2 more), the backward pass
-    holds what head_logprobs' does."""
+    to be a multiple of 8. The call takes V / 4 bytes of workspace a position; with top as much again (V / 8 above 32768 tokens), or
+    4 V in vocabularies of up to 2048 tokens where top^2 is more than V^2 / (24 d). The backward pass holds what head_logprobs'
+    does."""
     return HeadStats(*_lib.finetune().head_stats(h, weight, tokens, temperatura, top))
