@@ -6,7 +6,8 @@ blocks that keep their activations in 8 bits (checkpoint='8bits').
 
 The prompts are random; a chosen answer repeats its prompt, a rejected one is random. In the second part answers are
 drawn from the model itself and rewarded for each token that the prompt holds; with --entropy the answers' entropy is
-rewarded, too (model.stats). --fused trains with layer_norm and linear in the local blocks (fundido=True).
+rewarded, too (model.stats). --fused trains with layer_norm and linear in the local blocks (fundido=True), whose activations are
+kept as they are then.
 """
 import argparse
 import os
@@ -93,7 +94,7 @@ def main(argv=None):
     a.add_argument('--entropy', type=float, default=0.0)
     a.add_argument('--fused', action='store_true')
     a = a.parse_args(argv)
-    model = asrn.create_model(V=a.V, d=a.d, n_capas=a.layers, semilla=0, checkpoint='8bits',
+    model = asrn.create_model(V=a.V, d=a.d, n_capas=a.layers, semilla=0, checkpoint=False if a.fused else '8bits',
                               fundido=a.fused).cuda().train()
     optimiser = torch.optim.Adam(model.parameters(), lr=1e-3)
     x, targets = pairs(a.pairs, a.length, a.V, seed=0)
