@@ -224,7 +224,7 @@ ASRN_DEV float row_square(const uint4* row, int vecs) {
   bool bad = false;
 #pragma unroll 4
   for (int c = threadIdx.x & 31; c < vecs; c += 32) {
-    const uint4 a = __ldg(row + c);
+    const uint4 a = __ldcg(row + c);                     // from L2, as k_stats_sizes reads
     const uint32_t x[4] = {a.x, a.y, a.z, a.w};
     Two sum = no_squares();
     add_squares(sum, a);
@@ -242,8 +242,8 @@ ASRN_DEV float row_square(const uint4* row, int vecs) {
 }
 
 // The largest |w|^2 of each block's rows of W. Launched behind k_gemm<Scan>, whose blocks let it start once all that was before them is
-// complete: it needs nothing of the scan's, and runs beside it on SMs that the scan leaves idle, else behind it. Then it waits for the
-// scan, so that the kernel behind waits for both. Bound by memory, once over W: 50304 x 768 16.5 us (77 MB, 4.7 TB/s), 9 from L2 behind
+// complete: it needs nothing of the scan's, and runs beside it on SMs that the scan leaves idle, else behind it. (Loads past L1, which
+// no wait of its own has made sure of.) Then it waits for the scan, so that the kernel behind waits for both. Bound by memory, once over W: 50304 x 768 16.5 us (77 MB, 4.7 TB/s), 9 from L2 behind
 // a scan of few rows; a block for each SM 33 and 22.
 __global__ void __launch_bounds__(kSizeWarps * 32, 3)
 k_stats_sizes(int64_t V, int vecs, const uint4* __restrict__ W, float* __restrict__ sizes) {
@@ -262,7 +262,7 @@ k_stats_sizes(int64_t V, int vecs, const uint4* __restrict__ W, float* __restric
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int i = 0; i < kSizeRows; ++i) a[u][i] = __ldg(row[i] + min(c + 32 * u, vecs - 1));
+        for (int i = 0; i < kSizeRows; ++i) a[u][i] = __ldcg(row[i] + min(c + 32 * u, vecs - 1));
 #pragma unroll
       for (int i = 0; i < kSizeRows; ++i) {
         Two q = no_squares();
@@ -592,10 +592,6 @@ ASRN_DEV void dots(const uint4* h, const uint4* W, int vecs, const int (&token)[
 // that its lanes 4 j to 4 j + 3 name. Loads as in k_stats_few.
 struct Pair {
   float a, b;
-  ASRN_DEV float of(int j) const {               // row j's, for the whole warp
-    const float x = __shfl_sync(0xffffffffu, a, j % 8 * 4), y = __shfl_sync(0xffffffffu, b, j % 8 * 4);
-    return j < 8 ? x : y;
-  }
 };
 template <int U> ASRN_DEV Pair dots16(const uint4* h, const uint4* W, int vecs, int row_a, int row_b) {
   const int lane = threadIdx.x & 31, t = lane & 3;
