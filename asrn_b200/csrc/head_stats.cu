@@ -243,8 +243,8 @@ ASRN_DEV float row_square(const uint4* row, int vecs) {
 
 // The largest |w|^2 of each block's rows of W. Launched behind k_gemm<Scan>, whose blocks let it start once all that was before them is
 // complete: it needs nothing of the scan's, and runs beside it on SMs that the scan leaves idle, else behind it. (Loads past L1, which
-// no wait of its own has made sure of.) Then it waits for the scan, so that the kernel behind waits for both. Bound by memory, once over W: 50304 x 768 16.5 us (77 MB, 4.7 TB/s), 9 from L2 behind
-// a scan of few rows; a block for each SM 33 and 22.
+// no wait of its own has made sure of.) Then it waits for the scan, so that the kernel behind waits for both. Bound by memory, once
+// over W: 50304 x 768 16.5 us (77 MB, 4.7 TB/s), 9 from L2 behind a scan of few rows; a block for each SM 33 and 22.
 __global__ void __launch_bounds__(kSizeWarps * 32, 3)
 k_stats_sizes(int64_t V, int vecs, const uint4* __restrict__ W, float* __restrict__ sizes) {
   constexpr int kU = 3;                                  // loads of a row under way together
